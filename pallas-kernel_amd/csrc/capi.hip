@@ -292,6 +292,8 @@ void ktimer_mark(int which, bool stop, hipStream_t st) {
     g_kt_n[which] = n + 1;
 }
 
+int set_error(int code, const char* msg) { return code ? fail(code, "%s", msg) : ok(); }
+
 }  // namespace tops
 
 extern "C" {

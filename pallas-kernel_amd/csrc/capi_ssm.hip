@@ -1,0 +1,280 @@
+// extern "C" entry points declared in include/tops_gla_ssm.h: argument validation and dispatch.
+// No entry point allocates, synchronizes, or launches anything for invalid arguments.
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <initializer_list>
+
+#include "ssm.hpp"
+
+namespace {
+
+constexpr int64_t kMax = 2147483647;
+
+int fail(int code, const char* fmt, ...) {
+  char msg[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return tops::set_error(code, msg);
+}
+
+int done(hipError_t e, const char* what) {
+  if (e == hipSuccess) return tops::set_error(TOPS_GLA_OK, "");
+  return fail(TOPS_GLA_EHIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+bool dtype_ok(int64_t d) { return d == TOPS_GLA_F32 || d == TOPS_GLA_BF16; }
+
+bool any_null(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (p == nullptr) return true;
+  return false;
+}
+
+// Whether every pointer is a multiple of `bytes` and every stride a multiple of `n`.
+bool aligned(std::initializer_list<const void*> ps, std::initializer_list<int64_t> strides,
+             int64_t bytes, int64_t n) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % bytes) return false;
+  for (int64_t s : strides)
+    if (s % n) return false;
+  return true;
+}
+
+int scan_sizes(int64_t D, int64_t N, int64_t G, int64_t dtype) {
+  if (!dtype_ok(dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (D < 1 || D > (1 << 20)) return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)",
+                                          (long long)D);
+  if (N < 1 || N > 64)
+    return fail(TOPS_GLA_EUNSUPPORTED, "state size N must be in [1, 64] (N=%lld)", (long long)N);
+  if (G < 1 || D % G) return fail(TOPS_GLA_EINVAL, "G must divide D (D=%lld, G=%lld)",
+                                  (long long)D, (long long)G);
+  return TOPS_GLA_OK;
+}
+
+int64_t tiles_of(int64_t D, int64_t N, int64_t G) {
+  const int64_t ct = tops::scan_tile_channels((int)N);
+  return (D / G + ct - 1) / ct;
+}
+
+int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (int rc = scan_sizes(a->D, a->N, a->G, a->dtype)) return rc;
+  if (a->batch < 0 || a->T < 0 || a->nseq < 0)
+    return fail(TOPS_GLA_EINVAL, "bad batch, T or nseq");
+  if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMax)
+    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
+  if (a->piece < 16 || a->piece % 16 || a->piece > kMax)
+    return fail(TOPS_GLA_EINVAL, "piece must be a positive multiple of 16 (piece=%lld)",
+                (long long)a->piece);
+  *p = tops::ScanParams{};
+  p->a = *a;
+  p->tokens = a->batch * a->T;
+  if (a->segs) {
+    if (a->batch != 1) return fail(TOPS_GLA_EINVAL, "packed sequences require batch == 1");
+    if (a->nsegs < a->nseq || a->nsegs > kMax)
+      return fail(TOPS_GLA_EINVAL, "bad nsegs (%lld for %lld sequences)", (long long)a->nsegs,
+                  (long long)a->nseq);
+    p->npieces = a->nsegs;
+    p->multi = a->piece_h != nullptr;
+  } else {
+    if (a->nseq != a->batch) return fail(TOPS_GLA_EINVAL, "nseq must be the batch");
+    const int64_t n = std::max<int64_t>(1, (a->T + a->piece - 1) / a->piece);
+    if (n * a->batch > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "too many pieces");
+    p->pieces = (int)n;
+    p->npieces = n * a->batch;
+    p->multi = n > 1;
+    if (p->multi && a->piece_h == nullptr)
+      return fail(TOPS_GLA_EINVAL, "piece_h and piece_dt are required for several pieces");
+  }
+  if (p->multi && a->piece_dt == nullptr)
+    return fail(TOPS_GLA_EINVAL, "piece_dt is required with piece_h");
+  p->tiles_g = (int)tiles_of(a->D, a->N, a->G);
+  if (p->tiles_g * a->G * std::max<int64_t>(p->npieces, 1) > kMax)
+    return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  p->ntiles = p->tiles_g * (int)a->G;
+  if (any_null({a->A})) return fail(TOPS_GLA_EINVAL, "A must not be NULL");
+  if (p->tokens > 0 && any_null({a->u, a->delta, a->B, a->C}))
+    return fail(TOPS_GLA_EINVAL, "u, delta, B and C must not be NULL");
+  const int64_t es = a->dtype == TOPS_GLA_BF16 ? 2 : 4;
+  const int64_t ept = 64 / tops::scan_state_pad((int)a->N);   // channels of a thread: 4, 2 or 1
+  p->vec = (a->D / a->G) % ept == 0 &&
+           aligned({a->u, a->delta, a->z}, {a->u_sb, a->u_st, a->delta_sb, a->delta_st}, es * ept,
+                   ept) &&
+           (a->z == nullptr || aligned({}, {a->z_sb, a->z_st}, 1, ept));
+  if (!backward) {
+    if (p->tokens > 0 && a->y == nullptr) return fail(TOPS_GLA_EINVAL, "y must not be NULL");
+    p->vec = p->vec && aligned({a->y}, {}, es * ept, 1);
+    return TOPS_GLA_OK;
+  }
+  if (p->tokens > 0 && any_null({a->dy, a->du, a->ddelta, a->dB, a->dC, a->chunk_h}))
+    return fail(TOPS_GLA_EINVAL, "dy, du, ddelta, dB, dC and chunk_h must not be NULL");
+  if (p->tokens > 0 && (a->z == nullptr) != (a->dz == nullptr))
+    return fail(TOPS_GLA_EINVAL, "dz must be given exactly when z is");
+  if (a->dA == nullptr) return fail(TOPS_GLA_EINVAL, "dA must not be NULL");
+  p->vec = p->vec && aligned({a->dy, a->du, a->ddelta, a->dz}, {a->dy_sb, a->dy_st}, es * ept, ept);
+  const int64_t need =
+      tops_gla_selective_scan_bwd_ws_bytes(p->tokens, p->npieces, a->D, a->N, a->G);
+  if (need > 0 && (a->ws == nullptr || a->ws_bytes < need))
+    return fail(TOPS_GLA_EINVAL, "ws must hold %lld bytes", (long long)need);
+  const int64_t np = tops::scan_state_pad((int)a->N);
+  p->part_bc = (float*)a->ws;
+  p->part_a = p->part_bc + p->tiles_g * p->tokens * a->G * 2 * np;
+  p->part_d = p->part_a + p->npieces * a->D * np;
+  return TOPS_GLA_OK;
+}
+
+int slots_ok(int64_t batch, int64_t slots, const void* idx) {
+  if (batch < 0 || slots < 0) return fail(TOPS_GLA_EINVAL, "bad batch or slots");
+  if (idx == nullptr && batch > slots)
+    return fail(TOPS_GLA_EINVAL, "the states hold %lld rows, the batch %lld", (long long)slots,
+                (long long)batch);
+  return TOPS_GLA_OK;
+}
+
+int conv_check(const tops_gla_conv_args* a) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (!dtype_ok(a->dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (a->D < 1 || a->D > (1 << 20))
+    return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)", (long long)a->D);
+  if (a->W < 1 || a->W > 8)
+    return fail(TOPS_GLA_EUNSUPPORTED, "kernel width W in 1..8 (W=%lld)", (long long)a->W);
+  if (a->batch < 0 || a->T < 0 || a->nseq < 0)
+    return fail(TOPS_GLA_EINVAL, "bad batch, T or nseq");
+  if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMax)
+    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
+  if (a->cu == nullptr ? a->nseq != a->batch : a->batch != 1)
+    return fail(TOPS_GLA_EINVAL, "packed sequences require batch == 1, others nseq == batch");
+  const int64_t slabs = (a->D + 63) / 64;
+  if (slabs * (a->batch * a->T / 32 + 2) > kMax || slabs * (2 * a->nseq + 2) > kMax)
+    return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->w == nullptr) return fail(TOPS_GLA_EINVAL, "w must not be NULL");
+  if (a->batch * a->T > 0 && a->x == nullptr) return fail(TOPS_GLA_EINVAL, "x must not be NULL");
+  return TOPS_GLA_OK;
+}
+
+int qk_check(const tops_gla_qk_args* a) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (!dtype_ok(a->dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (a->D < 1 || a->D > 512)
+    return fail(TOPS_GLA_EUNSUPPORTED, "head size D must be in [1, 512] (D=%lld)", (long long)a->D);
+  if (a->R < 0 || a->R > a->D || a->R % 2)
+    return fail(TOPS_GLA_EINVAL, "rotated columns R must be even and at most D (R=%lld)",
+                (long long)a->R);
+  if (a->R > 0 && a->inv_freq == nullptr)
+    return fail(TOPS_GLA_EINVAL, "inv_freq must not be NULL");
+  if (a->batch < 0 || a->T < 0 || a->Hq < 0 || a->Hk < 0 || a->Hq > 65536 || a->Hk > 65536)
+    return fail(TOPS_GLA_EINVAL, "bad batch, T, Hq or Hk");
+  if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMax)
+    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
+  return TOPS_GLA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t D, int64_t N, int64_t G) {
+  if (tokens <= 0 || D < 1 || N < 1 || N > 64 || G < 1) return 64;
+  // two blocks a CU; shorter pieces than 64 tokens cost more in their states than they give
+  const int64_t len = (tokens * tiles_of(D, N, G) * G + 511) / 512;
+  return std::min<int64_t>(std::max<int64_t>(64, (len + 15) / 16 * 16), 1 << 30);
+}
+
+int64_t tops_gla_selective_scan_bwd_ws_bytes(int64_t tokens, int64_t nsegs, int64_t D, int64_t N,
+                                             int64_t G) {
+  if (tokens < 0 || nsegs < 0 || D < 1 || N < 1 || N > 64 || G < 1 || D % G) return 0;
+  const int64_t np = tops::scan_state_pad((int)N);
+  return 4 * (tiles_of(D, N, G) * tokens * G * 2 * np + nsegs * D * (np + 2));
+}
+
+int tops_gla_selective_scan_fwd(const tops_gla_scan_args* a, void* stream) {
+  tops::ScanParams p;
+  if (int rc = scan_setup(a, false, &p)) return rc;
+  return done(tops::run_selective_scan(p, false, (hipStream_t)stream), "selective_scan_fwd");
+}
+
+int tops_gla_selective_scan_bwd(const tops_gla_scan_args* a, void* stream) {
+  tops::ScanParams p;
+  if (int rc = scan_setup(a, true, &p)) return rc;
+  return done(tops::run_selective_scan(p, true, (hipStream_t)stream), "selective_scan_bwd");
+}
+
+int tops_gla_selective_scan_step(const tops_gla_scan_step_args* a, void* stream) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (int rc = scan_sizes(a->D, a->N, a->G, a->dtype)) return rc;
+  if (int rc = slots_ok(a->batch, a->slots, a->slots_idx)) return rc;
+  if (a->batch * ((a->D + 15) / 16) > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->batch > 0 && any_null({a->u, a->delta, a->B, a->C, a->A, a->y}))
+    return fail(TOPS_GLA_EINVAL, "u, delta, A, B, C and y must not be NULL");
+  if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
+    return fail(TOPS_GLA_EINVAL, "state must not be NULL");
+  return done(tops::run_scan_step(*a, (hipStream_t)stream), "selective_scan_step");
+}
+
+int64_t tops_gla_causal_conv_bwd_ws_bytes(int64_t tokens, int64_t D, int64_t W) {
+  if (tokens <= 0 || D < 1 || W < 1 || W > 8) return 0;
+  return tops::causal_conv_part_rows((long)tokens) * (W + 1) * D * 4;
+}
+
+int tops_gla_causal_conv_fwd(const tops_gla_conv_args* a, void* stream) {
+  if (int rc = conv_check(a)) return rc;
+  if (a->batch * a->T > 0 && a->y == nullptr) return fail(TOPS_GLA_EINVAL, "y must not be NULL");
+  return done(tops::run_causal_conv_fwd(*a, (hipStream_t)stream), "causal_conv_fwd");
+}
+
+int tops_gla_causal_conv_bwd(const tops_gla_conv_args* a, void* stream) {
+  if (int rc = conv_check(a)) return rc;
+  if (a->batch * a->T > 0 && any_null({a->dy, a->dx}))
+    return fail(TOPS_GLA_EINVAL, "dy and dx must not be NULL");
+  const int64_t need = tops_gla_causal_conv_bwd_ws_bytes(a->batch * a->T, a->D, a->W);
+  if (a->dw && need > 0 && (a->ws == nullptr || a->ws_bytes < need))
+    return fail(TOPS_GLA_EINVAL, "dw needs ws of %lld bytes", (long long)need);
+  return done(tops::run_causal_conv_bwd(*a, (hipStream_t)stream), "causal_conv_bwd");
+}
+
+int tops_gla_causal_conv_step(const tops_gla_conv_step_args* a, void* stream) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (!dtype_ok(a->dtype) || !dtype_ok(a->w_dtype))
+    return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (a->D < 1 || a->D > (1 << 20))
+    return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)", (long long)a->D);
+  if (a->W < 1 || a->W > 8)
+    return fail(TOPS_GLA_EUNSUPPORTED, "kernel width W in 1..8 (W=%lld)", (long long)a->W);
+  if (int rc = slots_ok(a->batch, a->slots, a->slots_idx)) return rc;
+  if (a->batch * ((a->D + 255) / 256) > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->batch > 0 && any_null({a->x, a->w, a->y}))
+    return fail(TOPS_GLA_EINVAL, "x, w and y must not be NULL");
+  if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
+    return fail(TOPS_GLA_EINVAL, "state must not be NULL");
+  return done(tops::run_conv_step(*a, (hipStream_t)stream), "causal_conv_step");
+}
+
+int64_t tops_gla_qk_norm_rope_ws_bytes(int64_t tokens, int64_t D) {
+  if (tokens <= 0 || D < 1 || D > 512) return 0;
+  return tops::qk_norm_rope_part_rows((long)tokens) * 2 * D * 4;
+}
+
+int tops_gla_qk_norm_rope_fwd(const tops_gla_qk_args* a, void* stream) {
+  if (int rc = qk_check(a)) return rc;
+  const int64_t tokens = a->batch * a->T;
+  if (tokens > 0 && ((a->Hq > 0 && any_null({a->q, a->qo})) || (a->Hk > 0 && any_null({a->k, a->ko}))))
+    return fail(TOPS_GLA_EINVAL, "q, k and their outputs must not be NULL");
+  return done(tops::run_qk_norm_rope(*a, false, (hipStream_t)stream), "qk_norm_rope_fwd");
+}
+
+int tops_gla_qk_norm_rope_bwd(const tops_gla_qk_args* a, void* stream) {
+  if (int rc = qk_check(a)) return rc;
+  const int64_t tokens = a->batch * a->T;
+  if (tokens > 0 && ((a->Hq > 0 && any_null({a->q, a->dqo, a->dq})) ||
+                     (a->Hk > 0 && any_null({a->k, a->dko, a->dk}))))
+    return fail(TOPS_GLA_EINVAL, "q, k and their gradients must not be NULL");
+  const int64_t need = tops_gla_qk_norm_rope_ws_bytes(tokens, a->D);
+  if ((a->dqw || a->dkw) && need > 0 && (a->ws == nullptr || a->ws_bytes < need))
+    return fail(TOPS_GLA_EINVAL, "dqw and dkw need ws of %lld bytes", (long long)need);
+  return done(tops::run_qk_norm_rope(*a, true, (hipStream_t)stream), "qk_norm_rope_bwd");
+}
+
+}  // extern "C"

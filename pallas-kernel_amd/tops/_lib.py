@@ -81,10 +81,32 @@ _LAYER_SIGS = {
     "tops_gla_low_rank_gate": [_P, _P, _P, _P, _I64, _I64, _I, _F, _I, _F, _P],
 }
 
+# the selective state space entry points (include/tops_gla_ssm.h): one struct of 8-byte fields,
+# passed as its bytes, and the stream
+_S = ctypes.c_char_p
+_SSM_SIGS = {
+    "tops_gla_selective_scan_fwd": [_S, _P],
+    "tops_gla_selective_scan_bwd": [_S, _P],
+    "tops_gla_selective_scan_bwd_ws_bytes": [_I64] * 5,
+    "tops_gla_selective_scan_piece": [_I64] * 4,
+    "tops_gla_selective_scan_step": [_S, _P],
+    "tops_gla_causal_conv_fwd": [_S, _P],
+    "tops_gla_causal_conv_bwd": [_S, _P],
+    "tops_gla_causal_conv_bwd_ws_bytes": [_I64] * 3,
+    "tops_gla_causal_conv_step": [_S, _P],
+    "tops_gla_qk_norm_rope_fwd": [_S, _P],
+    "tops_gla_qk_norm_rope_bwd": [_S, _P],
+    "tops_gla_qk_norm_rope_ws_bytes": [_I64] * 2,
+}
+
 # entry points that do not return a status code
 _RESTYPE = {"tops_gla_chunk_ws_bytes": ctypes.c_int64, "tops_gla_kernel_ms": ctypes.c_float,
             "tops_gla_rmsnorm_ws_bytes": ctypes.c_int64,
-            "tops_gla_short_conv_ws_bytes": ctypes.c_int64}
+            "tops_gla_short_conv_ws_bytes": ctypes.c_int64,
+            "tops_gla_selective_scan_bwd_ws_bytes": ctypes.c_int64,
+            "tops_gla_selective_scan_piece": ctypes.c_int64,
+            "tops_gla_causal_conv_bwd_ws_bytes": ctypes.c_int64,
+            "tops_gla_qk_norm_rope_ws_bytes": ctypes.c_int64}
 
 EXPORTED = ["tops_gla_last_error", "tops_gla_version"] + list(_SIGS)
 
@@ -122,7 +144,7 @@ def load():
             lib.tops_gla_last_error.argtypes = []
             lib.tops_gla_version.restype = ctypes.c_char_p
             lib.tops_gla_version.argtypes = []
-            for name, args in (*_SIGS.items(), *_LAYER_SIGS.items()):
+            for name, args in (*_SIGS.items(), *_LAYER_SIGS.items(), *_SSM_SIGS.items()):
                 fn = getattr(lib, name)
                 fn.argtypes = args
                 fn.restype = _RESTYPE.get(name, ctypes.c_int)

@@ -1,0 +1,127 @@
+"""Per-head RMS norms of queries and keys and their position rotation, one pass over both, on the
+``tops_gla_qk_norm_rope_*`` kernels."""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ... import _lib
+from ..._lib import call, check_device, dtype_code, require, stream_of
+from ..ssm._common import address, differentiable, f32, io_dtype, rows, strides
+
+_ARGS = struct.Struct("=8q 6q 8q 2q d 2q 6q 4q 2q")
+
+
+def rotary_inv_freq(rotary_dim, theta=10000.0, device=None):
+    """The usual frequencies ``theta^(-2 i / rotary_dim)``, float64 ``[rotary_dim / 2]``."""
+    require(rotary_dim >= 0 and rotary_dim % 2 == 0, "rotary_dim must be even")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    return float(theta) ** (-i / max(1, rotary_dim))
+
+
+def _pack(x, out, interleaved, eps, bwd=None):
+    q, k, qw, kw, freq, pos = x
+    B, T, Hq, D = q.shape
+    return _ARGS.pack(
+        address(q), address(k), address(qw), address(kw), address(freq), address(pos),
+        address(out[0]), address(out[1]), B, T, Hq, k.shape[2], D,
+        0 if freq is None else 2 * freq.shape[0], *strides(q, 0, 1, 2), *strides(k, 0, 1, 2),
+        0 if pos is None or pos.dim() == 1 else pos.stride(0),
+        int(pos is not None and pos.dtype == torch.int64), int(interleaved), dtype_code(q.dtype),
+        float(eps), *(bwd or [0] * 14))
+
+
+def _forward(q, k, qw, kw, freq, pos, eps, interleaved):
+    dev = check_device(q, k, qw, kw, freq, pos)
+    dt = io_dtype(q, k)
+    x = (rows(q, dt), rows(k, dt), f32(qw), f32(kw), freq, pos)
+    qo = torch.empty(q.shape, dtype=dt, device=dev)
+    ko = torch.empty(k.shape, dtype=dt, device=dev)
+    call("tops_gla_qk_norm_rope_fwd", _pack(x, (qo, ko), interleaved, eps), stream_of(dev))
+    return qo.to(q.dtype), ko.to(k.dtype), x
+
+
+class _QkNormRopeFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, freq, pos, eps, interleaved):
+        ctx.set_materialize_grads(False)
+        qo, ko, x = _forward(q, k, qw, kw, freq, pos, eps, interleaved)
+        ctx.save_for_backward(*x)
+        ctx.meta = eps, interleaved
+        ctx.like = [None if t is None else t.dtype for t in (q, k, qw, kw)]
+        return qo, ko
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dqo, dko):
+        x = ctx.saved_tensors
+        q, k, qw, kw = x[:4]
+        eps, interleaved = ctx.meta
+        dev, dt = q.device, q.dtype
+        D = q.shape[-1]
+        g = [torch.zeros(t.shape, dtype=dt, device=dev) if d is None else rows(d, dt)
+             for t, d in ((q, dqo), (k, dko))]
+        dq, dk = (torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k))
+        need = ctx.needs_input_grad
+        dqw = torch.empty(D, dtype=torch.float32, device=dev) if need[2] else None
+        dkw = torch.empty(D, dtype=torch.float32, device=dev) if need[3] else None
+        nws, ws = 0, None
+        if need[2] or need[3]:
+            nws = int(_lib.load().tops_gla_qk_norm_rope_ws_bytes(q.shape[0] * q.shape[1], D))
+            ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+        bwd = [address(g[0]), address(g[1]), *strides(g[0], 0, 1, 2), *strides(g[1], 0, 1, 2),
+               *(address(t) for t in (dq, dk, dqw, dkw, ws)), nws]
+        call("tops_gla_qk_norm_rope_bwd", _pack(x, (None, None), interleaved, eps, bwd),
+             stream_of(dev))
+        return (*(t if t is None or not n else t.to(like)
+                  for t, n, like in zip((dq, dk, dqw, dkw), need, ctx.like)),
+                None, None, None, None)
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, inv_freq=None, positions=None, *, eps=1e-6,
+                 interleaved=False):
+    """RMS norm of every head of q and k, then the rotation by the token's position::
+
+        n = x * rsqrt(mean(x^2) + eps) * weight        (over the head's D columns)
+        n[i], n[j] <- n[i] cos a - n[j] sin a, n[j] cos a + n[i] sin a,   a = position inv_freq[p]
+
+    for the pairs p of the first ``2 len(inv_freq)`` columns: (p, p + len(inv_freq)), or
+    (2 p, 2 p + 1) with ``interleaved``. The other columns are normed only. Computed in float32
+    and rounded once; the angles are formed in 64 bits, which far positions need.
+
+    Args:
+        q, k: ``[B, T, Hq, D]`` and ``[B, T, Hk, D]``, D <= 512; views of a fused projection
+            are read in place (any strides with the last dimension contiguous).
+        q_weight, k_weight: ``[D]`` or None.
+        inv_freq: float64 ``[R / 2]``, R <= D (``rotary_inv_freq``), or None for no rotation.
+        positions: int32 or int64 ``[B, T]`` or ``[T]``; None: 0 .. T - 1 in every row.
+
+    Differentiable in q, k and the weights. Returns ``(q', k')`` in the inputs' types, contiguous.
+    """
+    require(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2]
+            and q.shape[3] == k.shape[3] and 1 <= q.shape[3] <= 512,
+            f"q and k must be [B, T, heads, D] with one D <= 512, got {tuple(q.shape)} and "
+            f"{tuple(k.shape)}")
+    B, T, _, D = q.shape
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        require(w is None or tuple(w.shape) == (D,), f"{name} must be {(D,)}")
+    if inv_freq is not None:
+        require(inv_freq.dim() == 1 and 2 * inv_freq.shape[0] <= D
+                and inv_freq.dtype == torch.float64,
+                f"inv_freq must be float64 [R / 2] with R <= {D}, got {inv_freq.dtype} "
+                f"{tuple(inv_freq.shape)}")
+        inv_freq = inv_freq.contiguous()
+    if positions is not None:
+        require(positions.dtype in (torch.int32, torch.int64)
+                and tuple(positions.shape) in ((B, T), (T,)),
+                f"positions must be int32 or int64 {(B, T)} or {(T,)}, got {positions.dtype} "
+                f"{tuple(positions.shape)}")
+        if positions.shape[-1] > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+    args = (q, k, q_weight, k_weight)
+    if differentiable(*args):
+        return _QkNormRopeFunction.apply(*args, inv_freq, positions, float(eps), bool(interleaved))
+    return _forward(*args, inv_freq, positions, float(eps), bool(interleaved))[:2]

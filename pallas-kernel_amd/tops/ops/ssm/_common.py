@@ -1,0 +1,74 @@
+"""Host helpers of the selective state space operators."""
+
+from __future__ import annotations
+
+import torch
+
+from ..._lib import require, to_list
+
+_IO = (torch.float32, torch.bfloat16)
+
+
+def io_dtype(*tensors):
+    """The type the kernel computes such tensors in: bfloat16 where all are, else float32."""
+    return (torch.bfloat16 if all(t is None or t.dtype == torch.bfloat16 for t in tensors)
+            else torch.float32)
+
+
+def rows(t, dt):
+    """t in type dt with its last dimension contiguous (a view where it already is)."""
+    if t is None:
+        return None
+    if t.dtype != dt:
+        t = t.to(dt)
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def f32(t):
+    """A small parameter or a state as the kernels read it: float32, contiguous."""
+    return None if t is None else t.to(torch.float32).contiguous()
+
+
+def differentiable(*tensors):
+    """Whether a call has to go through autograd (forward-mode differentiation included, which
+    the functions then refuse)."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def refuse_grad(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} updates its state in place and has no gradient: call it under "
+                           "torch.no_grad()")
+
+
+def offsets(cu_seqlens, B, T):
+    """Packed sequences' token offsets as a list (empty sequences allowed), or None."""
+    if cu_seqlens is None:
+        return None
+    cu = to_list(cu_seqlens)
+    require(B == 1, f"cu_seqlens requires B == 1, got B={B}")
+    require(len(cu) >= 2 and cu[0] == 0 and cu[-1] == T
+            and all(b >= a for a, b in zip(cu, cu[1:])),
+            f"cu_seqlens must go from 0 to T={T} without decreasing: {cu}")
+    return cu
+
+
+def slot_args(idx, batch, device_of):
+    """(address, whether int64) of the state slots of a batch."""
+    if idx is None:
+        return 0, 0
+    require(idx.dtype in (torch.int32, torch.int64) and tuple(idx.shape) == (batch,),
+            f"state_indices must be int32 or int64 of shape {(batch,)}, got {idx.dtype} "
+            f"{tuple(idx.shape)}")
+    require(batch <= 1 or idx.stride(0) == 1, "state_indices must be contiguous")
+    return idx.data_ptr(), int(idx.dtype == torch.int64)
+
+
+def address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def strides(t, *dims):
+    return [0] * len(dims) if t is None else [t.stride(d) for d in dims]

@@ -1,0 +1,255 @@
+"""Selective state space scan on the ``tops_gla_selective_scan_*`` kernels."""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ... import _lib
+from ..._lib import call, check_device, dtype_code, require, stream_of
+from ._common import (address, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
+                      slot_args, strides)
+
+_ARGS = struct.Struct("=52q")
+_STEP = struct.Struct("=27q")
+_CHUNK = 16   # tokens between the states kept for the backward
+
+
+class _Pieces:
+    """How the sequences of a call are cut into pieces that run in parallel."""
+
+    _cache: dict = {}
+
+    def __init__(self, B, T, D, N, G, cu, device):
+        lib = _lib.load()
+        self.piece = int(lib.tops_gla_selective_scan_piece(B * T, D, N, G))
+        self.table = None
+        if cu is None:
+            per = max(1, -(-T // self.piece))
+            self.nseq, self.nsegs = B, B * per
+            self.chunks, self.multi = B * -(-T // _CHUNK), per > 1
+            return
+        self.nseq = len(cu) - 1
+        key = (tuple(cu), self.piece, str(device))
+        hit = _Pieces._cache.get(key)
+        if hit is None:
+            segs, c0, multi = [], 0, False
+            for s, (a, b) in enumerate(zip(cu, cu[1:])):
+                n = max(1, -(-(b - a) // self.piece))
+                multi |= n > 1
+                for i in range(n):
+                    t0 = a + i * self.piece
+                    segs += [s, t0, min(b, t0 + self.piece), i, n, c0 + i * self.piece // _CHUNK,
+                             0, 0]
+                c0 += -(-(b - a) // _CHUNK)
+            hit = (torch.tensor(segs, dtype=torch.int32, device=device), len(segs) // 8, c0, multi)
+            if len(_Pieces._cache) > 64:
+                _Pieces._cache.clear()
+            _Pieces._cache[key] = hit
+        self.table, self.nsegs, self.chunks, self.multi = hit
+
+
+def _pad(N):
+    return 16 if N <= 16 else 32 if N <= 32 else 64
+
+
+def _groups(t, N):
+    """B or C as [B, T, G, N]."""
+    return t if t.dim() == 4 else t.unsqueeze(2)
+
+
+def _pack(x, y, ht, chunk_h, ws, pc, shape, softplus, dt, bwd=None):
+    Bt, T, D, N, G = shape
+    u, delta, A, B, C, Dskip, z, bias, h0 = x
+    if bwd is None:
+        bwd = [0] * 15
+    ph, pd = ws
+    return _ARGS.pack(
+        address(u), address(delta), address(z), address(B), address(C), address(A),
+        address(Dskip), address(bias), address(h0), address(y), address(ht), address(chunk_h),
+        address(ph), address(pd), address(pc.table),
+        pc.nsegs, pc.nseq, pc.piece, Bt, T, D, N, G,
+        *strides(u, 0, 1), *strides(delta, 0, 1), *strides(z, 0, 1), *strides(B, 0, 1, 2),
+        *strides(C, 0, 1, 2), int(softplus), dtype_code(dt), *bwd)
+
+
+def _piece_states(pc, D, N, dev):
+    """Workspaces of the pieces' own contributions, where a sequence has several pieces."""
+    if not pc.multi:
+        return None, None
+    return (torch.empty(pc.nsegs, D, _pad(N), dtype=torch.float32, device=dev),
+            torch.empty(pc.nsegs, D, dtype=torch.float32, device=dev))
+
+
+def _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu, keep):
+    """(y, ht, what the kernel read, chunk states, pieces)."""
+    dev = check_device(u, delta, A, B, C, D, z, bias, h0)
+    dt = io_dtype(u, delta, B, C, z)
+    Bt, T, Dn = u.shape
+    N = A.shape[1]
+    x = (rows(u, dt), rows(delta, dt), f32(A), rows(_groups(B, N), dt), rows(_groups(C, N), dt),
+         f32(D), rows(z, dt), f32(bias), f32(h0))
+    G = x[3].shape[2]
+    pc = _Pieces(Bt, T, Dn, N, G, cu, dev)
+    y = torch.empty(Bt, T, Dn, dtype=dt, device=dev)
+    ht = torch.empty(pc.nseq, Dn, N, dtype=torch.float32, device=dev) if want_ht else None
+    chunk_h = (torch.empty(pc.chunks, Dn, _pad(N), dtype=torch.float32, device=dev)
+               if keep else None)
+    ws = _piece_states(pc, Dn, N, dev)
+    call("tops_gla_selective_scan_fwd",
+         _pack(x, y, ht, chunk_h, ws, pc, (Bt, T, Dn, N, G), softplus, dt), stream_of(dev))
+    return y.to(u.dtype), ht, x, chunk_h, pc
+
+
+class _SelectiveScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu):
+        ctx.set_materialize_grads(False)
+        y, ht, x, chunk_h, pc = _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu,
+                                         True)
+        ctx.save_for_backward(*x[:8], chunk_h)
+        ctx.like = [None if t is None else (t.dtype, t.shape)
+                    for t in (u, delta, A, B, C, D, z, bias, h0)]
+        ctx.softplus, ctx.pc = softplus, pc
+        return y, ht
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dht):
+        *x, chunk_h = ctx.saved_tensors
+        u, delta, A, B, C, D, z, bias = x
+        pc, dev, dt = ctx.pc, u.device, u.dtype
+        Bt, T, Dn = u.shape
+        N, G = A.shape[1], B.shape[2]
+        dy = torch.zeros(Bt, T, Dn, dtype=dt, device=dev) if dy is None else rows(dy, dt)
+        dht = f32(dht)
+
+        def new(*shape, dtype=torch.float32):
+            return torch.empty(*shape, dtype=dtype, device=dev)
+
+        du, ddelta = new(Bt, T, Dn, dtype=dt), new(Bt, T, Dn, dtype=dt)
+        dz = None if z is None else new(Bt, T, Dn, dtype=dt)
+        dB, dC = new(Bt, T, G, N, dtype=dt), new(Bt, T, G, N, dtype=dt)
+        dA = new(Dn, N)
+        dD = None if D is None else new(Dn)
+        dbias = None if bias is None else new(Dn)
+        dh0 = None if ctx.like[8] is None else new(pc.nseq, Dn, N)
+        nws = int(_lib.load().tops_gla_selective_scan_bwd_ws_bytes(Bt * T, pc.nsegs, Dn, N, G))
+        ws = new(nws, dtype=torch.uint8)
+        bwd = [address(dy), *strides(dy, 0, 1), *(address(t) for t in (
+            dht, du, ddelta, dz, dB, dC, dA, dD, dbias, dh0, ws)), nws]
+        call("tops_gla_selective_scan_bwd",
+             _pack((*x, None), None, None, chunk_h, _piece_states(pc, Dn, N, dev), pc,
+                   (Bt, T, Dn, N, G), ctx.softplus, dt, bwd), stream_of(dev))
+        grads = (du, ddelta, dA, dB, dC, dD, dz, dbias, dh0)
+        return (*(None if g is None or not need else g.reshape(like[1]).to(like[0])
+                  for g, like, need in zip(grads, ctx.like, ctx.needs_input_grad)),
+                None, None, None)
+
+
+def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False,
+                   initial_state=None, output_final_state=False, cu_seqlens=None):
+    """Selective state space scan, differentiable in every tensor.
+
+    Per channel d with its states n (``delta'`` = ``delta + delta_bias``, its softplus with
+    ``delta_softplus``)::
+
+        h_t[n] = exp(delta'_t A[d, n]) h_{t-1}[n] + delta'_t u_t B_t[n]
+        y_t    = (sum_n C_t[n] h_t[n] + D[d] u_t) * silu(z_t)
+
+    Args:
+        u, delta, z: ``[B, T, D]`` (z optional: the output gate).
+        A: ``[D, N]``, N <= 64.  B, C: ``[B, T, N]``, or ``[B, T, G, N]`` for G groups of D / G
+            consecutive channels each.  D, delta_bias: ``[D]`` or None.
+        initial_state: ``[sequences, D, N]`` or None (zeros).
+        cu_seqlens: offsets of sequences packed into one row (B == 1), from 0 to T, known on the
+            host; empty sequences keep their state.
+
+    Inputs may be views with any strides whose last dimension is contiguous (others are copied).
+    bfloat16 tensors are read and written as they are, other types in float32; states, sums and
+    the gradients of A, D, delta_bias and the state are float32 inside.
+
+    Returns ``(y, final_state)``: y ``[B, T, D]`` in u's type, final_state ``[sequences, D, N]``
+    float32 with ``output_final_state``, else None.
+    """
+    require(u.dim() == 3, f"u must be [B, T, D], got {tuple(u.shape)}")
+    Bt, T, Dn = u.shape
+    require(A.dim() == 2 and A.shape[0] == Dn and 1 <= A.shape[1] <= 64,
+            f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
+    N = A.shape[1]
+    for name, t in (("delta", delta), ("z", z)):
+        require(t is None or tuple(t.shape) == (Bt, T, Dn),
+                f"{name} must be {(Bt, T, Dn)}" if t is not None else "")
+    for name, t in (("B", B), ("C", C)):
+        require(t.dim() in (3, 4) and tuple(t.shape[:2]) == (Bt, T) and t.shape[-1] == N
+                and (t.dim() == 3 or (t.shape[2] > 0 and Dn % t.shape[2] == 0)),
+                f"{name} must be [{Bt}, {T}, {N}] or [{Bt}, {T}, G, {N}] with G dividing {Dn}, "
+                f"got {tuple(t.shape)}")
+    require(B.shape == C.shape, "B and C must have the same shape")
+    require(Dn > 0, "D must be positive")
+    for name, t in (("D", D), ("delta_bias", delta_bias)):
+        require(t is None or tuple(t.shape) == (Dn,),
+                f"{name} must be {(Dn,)}" if t is not None else "")
+    cu = offsets(cu_seqlens, Bt, T)
+    S = Bt if cu is None else len(cu) - 1
+    require(initial_state is None or tuple(initial_state.shape) == (S, Dn, N),
+            f"initial_state must be {(S, Dn, N)}")
+    args = (u, delta, A, B, C, D, z, delta_bias, initial_state)
+    if differentiable(*args):
+        return _SelectiveScanFunction.apply(*args, bool(delta_softplus), bool(output_final_state),
+                                            cu)
+    return _forward(*args, bool(delta_softplus), bool(output_final_state), cu, False)[:2]
+
+
+def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None,
+                        delta_softplus=False, state_indices=None):
+    """One token of ``selective_scan`` for each row of a serving batch; ``state`` is updated in
+    place.
+
+    Args:
+        state: float32 ``[slots, D, N]``, each slot contiguous.
+        u, delta, z: ``[B, D]``.  A, D, delta_bias: as for ``selective_scan``.
+        B, C: ``[B, N]`` or ``[B, G, N]``.
+        state_indices: int32 or int64 ``[B]`` on the device, the slot of each row (None: row b
+            uses slot b). A row whose slot is negative or not below ``slots`` is left out: no
+            state changes for it and its y is 0. No slot may be given to two rows.
+
+    Returns y ``[B, D]`` in u's type.
+    """
+    refuse_grad("selective_scan_step", state, u, delta, A, B, C, D, z, delta_bias)
+    require(u.dim() == 2 and A.dim() == 2, "u must be [B, D], A [D, N]")
+    Bt, Dn = u.shape
+    N = A.shape[1]
+    require(A.shape[0] == Dn and 1 <= N <= 64 and Dn > 0,
+            f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
+    require(delta.shape == u.shape and (z is None or z.shape == u.shape),
+            f"delta and z must be {(Bt, Dn)}")
+    G = B.shape[1] if B.dim() == 3 else 1
+    require(B.shape == C.shape and B.dim() in (2, 3) and B.shape[0] == Bt and B.shape[-1] == N
+            and G > 0 and Dn % G == 0,
+            f"B and C must be [{Bt}, {N}] or [{Bt}, G, {N}] with G dividing {Dn}, got "
+            f"{tuple(B.shape)} and {tuple(C.shape)}")
+    require((D is None or tuple(D.shape) == (Dn,))
+            and (delta_bias is None or tuple(delta_bias.shape) == (Dn,)),
+            f"D and delta_bias must be {(Dn,)}")
+    require(state.dim() == 3 and tuple(state.shape[1:]) == (Dn, N)
+            and state.dtype == torch.float32
+            and (state.stride(2) == 1 or N == 1) and (state.stride(1) == N or Dn == 1),
+            f"state must be float32 [slots, {Dn}, {N}] with contiguous slots")
+    require(state_indices is not None or state.shape[0] >= Bt,
+            f"state holds {state.shape[0]} slots, the batch {Bt}")
+    idx, idx64 = slot_args(state_indices, Bt, u)
+    dev = check_device(state, u, delta, A, B, C, D, z, delta_bias, state_indices)
+    dt = io_dtype(u, delta, B, C, z)
+    uu, dd, bb, cc, zz = (rows(t, dt) for t in (u, delta, B, C, z))
+    aa, sk, bias = f32(A), f32(D), f32(delta_bias)
+    y = torch.empty(Bt, Dn, dtype=dt, device=dev)
+    call("tops_gla_selective_scan_step", _STEP.pack(
+        state.data_ptr(), uu.data_ptr(), dd.data_ptr(), address(zz), bb.data_ptr(), cc.data_ptr(),
+        aa.data_ptr(), address(sk), address(bias), y.data_ptr(), idx, idx64, state.shape[0], Bt,
+        Dn, N, G, state.stride(0), uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0),
+        bb.stride(0), bb.stride(1) if G > 1 else 0, cc.stride(0), cc.stride(1) if G > 1 else 0,
+        int(bool(delta_softplus)), dtype_code(dt)), stream_of(dev))
+    return y if dt == u.dtype else y.to(u.dtype)
