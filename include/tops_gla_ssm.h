@@ -28,12 +28,14 @@ extern "C" {
  *   y_t    = (sum_n C_t[g,n] h_t[n] + Dskip[d] u_t) (* z_t sigmoid(z_t) with z)
  * A sequence is cut into pieces of at most `piece` tokens (a multiple of 16) that run in
  * parallel: piece_h [pieces][D][NP] and piece_dt [pieces][D] hold their own contributions
- * (NP = N rounded up to 16, 32 or 64), not needed when no sequence has two pieces. Fixed length:
+ * (NP = N rounded up to 8, 16, 32 or 64), not needed when no sequence has two pieces. Fixed length:
  * ceil(T / piece) pieces a sequence (at least one). Packed: `segs` holds, for each of `nsegs`
  * pieces in order, {sequence, first token, end token, its index in the sequence, pieces of the
- * sequence, index of its first 16-token chunk, 0, 0}; a sequence of no tokens has one piece.
- * `chunk_h` [chunks][D][NP]: the states entering every 16-token chunk, kept for the backward
- * (NULL: not kept). 1 <= N <= 64.
+ * sequence, index of its first chunk, 0, 0}; a sequence of no tokens has one piece.
+ * `chunk_h` [chunks][D][NP]: the states entering every chunk of
+ * tops_gla_selective_scan_chunk(N) tokens of a sequence, kept for the backward (NULL: not kept).
+ * `bc` [B * T * G + 1][2][NP]: B and C as the kernels read them, written by the forward.
+ * 1 <= N <= 64.
  */
 typedef struct tops_gla_scan_args {
   const void *u, *delta, *z;      /* [B, T, D], z NULL: no gate */
@@ -45,6 +47,7 @@ typedef struct tops_gla_scan_args {
   float *ht;                      /* [sequences, D, N] or NULL */
   float *chunk_h;
   float *piece_h, *piece_dt;
+  float *bc;
   const int32_t *segs;
   int64_t nsegs, nseq, piece;
   int64_t batch, T, D, N, G;
@@ -65,12 +68,15 @@ typedef struct tops_gla_scan_args {
 } tops_gla_scan_args;
 
 int tops_gla_selective_scan_fwd(const tops_gla_scan_args *a, void *stream);
-/* The gradients; chunk_h as the forward left it, piece_h / piece_dt as workspaces. */
+/* The gradients; chunk_h and bc as the forward left them (B and C are not read), piece_h and
+ * piece_dt as workspaces. */
 int tops_gla_selective_scan_bwd(const tops_gla_scan_args *a, void *stream);
 /* Bytes of `ws`, and the tokens of a piece that fill the device for such a call. */
 int64_t tops_gla_selective_scan_bwd_ws_bytes(int64_t tokens, int64_t nsegs, int64_t D, int64_t N,
                                              int64_t G);
 int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t D, int64_t N, int64_t G);
+/* Tokens between the states that the forward keeps (0 for an N that is refused). */
+int64_t tops_gla_selective_scan_chunk(int64_t N);
 
 /*
  * One token of the scan for each row b, its state at state[slot_b] ([slots, D, N], in place):

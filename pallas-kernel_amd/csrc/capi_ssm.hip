@@ -33,16 +33,6 @@ bool any_null(std::initializer_list<const void*> ps) {
   return false;
 }
 
-// Whether every pointer is a multiple of `bytes` and every stride a multiple of `n`.
-bool aligned(std::initializer_list<const void*> ps, std::initializer_list<int64_t> strides,
-             int64_t bytes, int64_t n) {
-  for (const void* p : ps)
-    if ((uintptr_t)p % bytes) return false;
-  for (int64_t s : strides)
-    if (s % n) return false;
-  return true;
-}
-
 int scan_sizes(int64_t D, int64_t N, int64_t G, int64_t dtype) {
   if (!dtype_ok(dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
   if (D < 1 || D > (1 << 20)) return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)",
@@ -54,8 +44,10 @@ int scan_sizes(int64_t D, int64_t N, int64_t G, int64_t dtype) {
   return TOPS_GLA_OK;
 }
 
-int64_t tiles_of(int64_t D, int64_t N, int64_t G) {
-  const int64_t ct = tops::scan_tile_channels((int)N);
+// Channel tiles of a group in the forward's waves and the backward's blocks.
+int64_t tiles_of(int64_t D, int64_t G) { return (D / G + 63) / 64; }
+int64_t bwd_tiles_of(int64_t D, int64_t N, int64_t G) {
+  const int64_t ct = tops::scan_bwd_channels((int)N);
   return (D / G + ct - 1) / ct;
 }
 
@@ -91,22 +83,18 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
   }
   if (p->multi && a->piece_dt == nullptr)
     return fail(TOPS_GLA_EINVAL, "piece_dt is required with piece_h");
-  p->tiles_g = (int)tiles_of(a->D, a->N, a->G);
-  if (p->tiles_g * a->G * std::max<int64_t>(p->npieces, 1) > kMax)
+  const int64_t np = tops::scan_state_pad((int)a->N);
+  p->tiles_g = (int)tiles_of(a->D, a->G);
+  if ((p->tiles_g * a->G + a->D * np / 1024 + 1) * std::max<int64_t>(p->npieces, 1) > kMax)
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   p->ntiles = p->tiles_g * (int)a->G;
+  p->btiles = (int)(bwd_tiles_of(a->D, a->N, a->G) * a->G);
   if (any_null({a->A})) return fail(TOPS_GLA_EINVAL, "A must not be NULL");
-  if (p->tokens > 0 && any_null({a->u, a->delta, a->B, a->C}))
+  if (p->tokens > 0 && (any_null({a->u, a->delta}) || (!backward && any_null({a->B, a->C}))))
     return fail(TOPS_GLA_EINVAL, "u, delta, B and C must not be NULL");
-  const int64_t es = a->dtype == TOPS_GLA_BF16 ? 2 : 4;
-  const int64_t ept = 64 / tops::scan_state_pad((int)a->N);   // channels of a thread: 4, 2 or 1
-  p->vec = (a->D / a->G) % ept == 0 &&
-           aligned({a->u, a->delta, a->z}, {a->u_sb, a->u_st, a->delta_sb, a->delta_st}, es * ept,
-                   ept) &&
-           (a->z == nullptr || aligned({}, {a->z_sb, a->z_st}, 1, ept));
   if (!backward) {
     if (p->tokens > 0 && a->y == nullptr) return fail(TOPS_GLA_EINVAL, "y must not be NULL");
-    p->vec = p->vec && aligned({a->y}, {}, es * ept, 1);
+    if (p->tokens > 0 && a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
     return TOPS_GLA_OK;
   }
   if (p->tokens > 0 && any_null({a->dy, a->du, a->ddelta, a->dB, a->dC, a->chunk_h}))
@@ -114,14 +102,13 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
   if (p->tokens > 0 && (a->z == nullptr) != (a->dz == nullptr))
     return fail(TOPS_GLA_EINVAL, "dz must be given exactly when z is");
   if (a->dA == nullptr) return fail(TOPS_GLA_EINVAL, "dA must not be NULL");
-  p->vec = p->vec && aligned({a->dy, a->du, a->ddelta, a->dz}, {a->dy_sb, a->dy_st}, es * ept, ept);
   const int64_t need =
       tops_gla_selective_scan_bwd_ws_bytes(p->tokens, p->npieces, a->D, a->N, a->G);
   if (need > 0 && (a->ws == nullptr || a->ws_bytes < need))
     return fail(TOPS_GLA_EINVAL, "ws must hold %lld bytes", (long long)need);
-  const int64_t np = tops::scan_state_pad((int)a->N);
+  if (p->tokens > 0 && a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
   p->part_bc = (float*)a->ws;
-  p->part_a = p->part_bc + p->tiles_g * p->tokens * a->G * 2 * np;
+  p->part_a = p->part_bc + p->btiles * p->tokens * 2 * np;
   p->part_d = p->part_a + p->npieces * a->D * np;
   return TOPS_GLA_OK;
 }
@@ -178,16 +165,20 @@ extern "C" {
 
 int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t D, int64_t N, int64_t G) {
   if (tokens <= 0 || D < 1 || N < 1 || N > 64 || G < 1) return 64;
-  // two blocks a CU; shorter pieces than 64 tokens cost more in their states than they give
-  const int64_t len = (tokens * tiles_of(D, N, G) * G + 511) / 512;
-  return std::min<int64_t>(std::max<int64_t>(64, (len + 15) / 16 * 16), 1 << 30);
+  // four waves a SIMD, and at most 512 pieces for the fold to walk
+  const int64_t len = std::max((tokens * tiles_of(D, G) * G + 4095) / 4096, (tokens + 511) / 512);
+  return std::min<int64_t>(std::max<int64_t>(16, (len + 15) / 16 * 16), 1 << 30);
+}
+
+int64_t tops_gla_selective_scan_chunk(int64_t N) {
+  return N < 1 || N > 64 ? 0 : tops::scan_chunk();
 }
 
 int64_t tops_gla_selective_scan_bwd_ws_bytes(int64_t tokens, int64_t nsegs, int64_t D, int64_t N,
                                              int64_t G) {
   if (tokens < 0 || nsegs < 0 || D < 1 || N < 1 || N > 64 || G < 1 || D % G) return 0;
   const int64_t np = tops::scan_state_pad((int)N);
-  return 4 * (tiles_of(D, N, G) * tokens * G * 2 * np + nsegs * D * (np + 2));
+  return 4 * (bwd_tiles_of(D, N, G) * tokens * G * 2 * np + nsegs * D * (np + 2));
 }
 
 int tops_gla_selective_scan_fwd(const tops_gla_scan_args* a, void* stream) {

@@ -17,15 +17,16 @@ int set_error(int code, const char* msg);
 
 struct ScanParams {
   tops_gla_scan_args a;
-  int ntiles, tiles_g;   // channel tiles in all and of a group
+  int ntiles, tiles_g;   // channel tiles of 64 in all and of a group
+  int btiles;            // channel tiles of the backward's blocks
   int pieces;            // pieces of a sequence (fixed length)
   int multi;             // some sequence has more than one piece
-  int vec;               // rows allow wide loads and stores
   long npieces, tokens;
   float *part_bc, *part_a, *part_d;   // the backward's shares
 };
-int scan_state_pad(int N);       // N rounded up to 16, 32 or 64
-int scan_tile_channels(int N);   // channels of a block
+int scan_state_pad(int N);       // N rounded up to 8, 16, 32 or 64
+int scan_bwd_channels(int N);    // channels of a block of the backward
+int scan_chunk();                // tokens between the states kept for the backward
 hipError_t run_selective_scan(const ScanParams& p, bool backward, hipStream_t st);
 
 hipError_t run_scan_step(const tops_gla_scan_step_args& a, hipStream_t st);
@@ -56,41 +57,6 @@ __device__ __forceinline__ float swap16_add(float a, float b) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false,
                                                   false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// v summed over the CPW lanes of consecutive channels (lane bits below log2 CPW): v[0..3] go to
-// out[n0 .. n0 + 3], v[4..7] to out[np + n0 ..].
-template <int CPW>
-__device__ __forceinline__ void sum_channels(float (&v)[8], int lane, float* out, int n0, int np) {
-  if constexpr (CPW == 16) {
-    const bool b3 = lane & 8, b2 = lane & 4;
-    float r[4], s[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {   // lanes with bit 3 set take dC, the others dB
-      const float x = v[i] + dpp<0x128>(v[i]), y = v[4 + i] + dpp<0x128>(v[4 + i]);
-      r[i] = b3 ? y : x;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {   // bit 2: the upper two states (half rows mirrored)
-      const float x = r[i] + dpp<0x141>(r[i]), y = r[2 + i] + dpp<0x141>(r[2 + i]);
-      s[i] = b2 ? y : x;
-      s[i] += dpp<0xb1>(s[i]);      // quad_perm [1, 0, 3, 2]
-      s[i] += dpp<0x4e>(s[i]);      // quad_perm [2, 3, 0, 1]
-    }
-    if ((lane & 3) == 0)
-      *reinterpret_cast<float2*>(out + (b3 ? np : 0) + n0 + (b2 ? 2 : 0)) = make_float2(s[0], s[1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (CPW >= 8) v[i] += dpp<0x141>(v[i]);
-      v[i] += dpp<0xb1>(v[i]);
-      v[i] += dpp<0x4e>(v[i]);
-    }
-    if ((lane & (CPW - 1)) == 0) {
-      *reinterpret_cast<float4*>(out + n0) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(out + np + n0) = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  }
 }
 
 // 1 / (1 + e^-x), with the hardware exponential and reciprocal (1 ulp each); 0 and 1 at the ends.

@@ -1,13 +1,15 @@
 // Selective state space scan, forward and backward (include/tops_gla_ssm.h has the formulas).
 //
-// A wave owns 64 / LQ channels: a lane holds four consecutive states n of one channel, the LQ
-// lanes of a channel are 64 / LQ apart. A block of 8 waves walks a piece of one sequence in
-// tiles of 16 tokens: its threads load the tile's rows as contiguous runs of channels, form
-// delta' and delta' u once for each (token, channel), and leave them in LDS for the waves.
+// A lane owns one channel and keeps its states in registers, so that the sum over the states is
+// a chain of FMAs in the lane, and a wave's 64 channels are one run of each token's row. B_t and
+// C_t are the same for all of a wave's channels: a first launch writes them as float32 rows
+// (`bc`), which the scan then reads through the scalar cache, into scalar registers that the FMAs
+// take directly. Neither a shuffle nor LDS is left in the forward's loop; it is bound by the
+// vector units: an exponential (two issue slots), two products and two FMAs a state and token.
 //
 // Pieces: h_t = a_t h_{t-1} + b_t is linear, so a sequence is cut into pieces that run in
-// parallel: a first launch finds each piece's state from zero (L) and its summed delta' (S), and
-// a piece of the second launch folds those of the pieces before it, h <- exp(A S_j) h + L_j.
+// parallel. A first pass finds each piece's state from zero (L) and its summed delta' (S), a
+// small one folds them in order, h <- exp(A S_j) h + L_j, and leaves every piece's entry state.
 #include "common.hpp"
 #include "ssm.hpp"
 
@@ -15,20 +17,13 @@ namespace tops {
 
 namespace {
 
-constexpr int SS_NT = 512;   // threads of a block
-constexpr int SS_K = 16;     // tokens of a tile, and of a chunk of the backward
+constexpr int SS_K = 8;      // tokens of a tile, and between the states kept for the backward
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int LQ>
-struct Lay {
-  static constexpr int CPW = 64 / LQ;            // channels of a wave
-  static constexpr int CT = 8 * CPW;             // channels of a block
-  static constexpr int NP = 4 * LQ;              // padded state size
-  static constexpr int EPT = SS_K * CT / SS_NT;  // channels of a thread in a tile's row
-  static constexpr int YP = CT + 16;             // row pitch of the tiles in lane order
-  static constexpr int BPT = LQ / 4;             // elements of B and C a thread stages
-};
+// Wave-uniform data that no kernel of the launch writes: read by scalar loads.
+typedef const float __attribute__((address_space(4))) cfloat;
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 struct Piece {
   int seq, t0, t1, idx, np, c0;
@@ -39,7 +34,8 @@ __device__ __forceinline__ Piece piece_of(const ScanParams& p, int i) {
   Piece r;
   if (p.a.segs) {
     const int* s = p.a.segs + 8L * i;
-    r.seq = s[0], r.t0 = s[1], r.t1 = s[2], r.idx = s[3], r.np = s[4], r.c0 = s[5];
+    r.seq = uni(s[0]), r.t0 = uni(s[1]), r.t1 = uni(s[2]), r.idx = uni(s[3]), r.np = uni(s[4]);
+    r.c0 = uni(s[5]);
     r.b = 0;
   } else {
     const int T = (int)p.a.T, len = (int)p.a.piece;
@@ -54,451 +50,503 @@ __device__ __forceinline__ Piece piece_of(const ScanParams& p, int i) {
   return r;
 }
 
-// N consecutive elements from `nv` valid ones (the others read as zero); `vec`: whole, aligned.
-template <typename T, int N>
-__device__ __forceinline__ void load_run(const T* p, int nv, bool vec, float (&x)[N]) {
-  if (vec && nv >= N) {
-    if constexpr (sizeof(T) == 2 && N == 4) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
-      return;
-    } else if constexpr (sizeof(T) == 2 && N == 2) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-      x[0] = bf16_lo(w), x[1] = bf16_hi(w);
-      return;
-    } else if constexpr (sizeof(T) == 4 && N == 4) {
-      const float4 w = *reinterpret_cast<const float4*>(p);
-      x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-      return;
-    } else if constexpr (sizeof(T) == 4 && N == 2) {
-      const float2 w = *reinterpret_cast<const float2*>(p);
-      x[0] = w.x, x[1] = w.y;
-      return;
-    }
+// A channel tile of 64: its group, first channel, and the lane's channel (the first one where the
+// lane has none).
+struct Tile {
+  int grp, d0, nch;
+  __device__ __forceinline__ Tile(const ScanParams& p, int tile) {
+    const int DG = (int)(p.a.D / p.a.G);
+    grp = tile / p.tiles_g;
+    const int cb = (tile - grp * p.tiles_g) * 64;
+    d0 = grp * DG + cb;
+    nch = min(64, DG - cb);
   }
-#pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = e < nv ? to_f32(p[e]) : 0.f;
-}
+};
 
-template <typename T, int N>
-__device__ __forceinline__ void store_n(T* p, int nv, bool vec, const float (&x)[N]) {
-  if constexpr (N > 1) {
-    if (vec && nv >= N) {
-      store_run<T, N>(p, x);
-      return;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (e < nv) p[e] = from_f32<T>(x[e]);
+// A log2(e). -inf (a state that is forgotten at once) stays finite: a token past the end has
+// delta' = 0, and 0 times it has to be 0.
+__device__ __forceinline__ float scaled_a(float a) {
+  a *= kLog2e;
+  return a < -3.4028235e38f ? -3.4028235e38f : a;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Sum of the LQ lanes of each channel for four tokens' values; the lanes of row r = lane / 16
-// end with token {0, 2, 1, 3}[r].
-template <int LQ>
-__device__ __forceinline__ float sum_states(float v0, float v1, float v2, float v3) {
-  float v[4] = {v0, v1, v2, v3};
+// Keeps the compiler from moving LDS reads up, into registers that others need.
+__device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
+
+// N consecutive floats at a 16-byte boundary (N a multiple of 4).
+template <int N>
+__device__ __forceinline__ void load4(const float* p, float (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (LQ >= 8) v[i] += dpp<0x128>(v[i]);    // row_ror:8
-    if constexpr (LQ >= 16) v[i] += dpp<0x124>(v[i]);   // row_ror:4
+  for (int i = 0; i < N; i += 4) {
+    const float4 w = *reinterpret_cast<const float4*>(p + i);
+    x[i] = w.x, x[i + 1] = w.y, x[i + 2] = w.z, x[i + 3] = w.w;
   }
-  const float a = swap32_add(v[0], v[1]), b = swap32_add(v[2], v[3]);
-  return swap16_add(a, b);
+}
+template <int N>
+__device__ __forceinline__ void store4(float* p, const float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+
+// The lane's element of N rows from `t` on, the last one of the piece again past its end (t < t1).
+template <typename T, int N>
+__device__ __forceinline__ void load_rows(const T* p, long st, int t, int t1, uint32_t lo,
+                                          T (&x)[N]) {
+  p += t * st;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = p[lo];
+    p += t + i + 1 < t1 ? st : 0;
+  }
+}
+
+// A row of bc once the states x are there: the scalar loads of all tokens would otherwise be
+// moved to the tile's start, where there are not enough scalar registers for them.
+template <int N>
+__device__ __forceinline__ cfloat* row_after(const float* p, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile(""
+                 : "+s"(p), "+v"(x[i]), "+v"(x[i + 1]), "+v"(x[i + 2]), "+v"(x[i + 3]),
+                   "+v"(x[i + 4]), "+v"(x[i + 5]), "+v"(x[i + 6]), "+v"(x[i + 7]));
+  return (cfloat*)(uintptr_t)p;
+}
+
+// B and C as float32 rows [token][group][2][NP], zeros past N and in one more row, which stands
+// for the tokens past a piece's end.
+template <typename T>
+__global__ __launch_bounds__(256) void scan_bc_kernel(ScanParams p, int NP) {
+  const long rows = p.tokens * p.a.G, total = (rows + 1) * 2 * NP;
+  const int N = (int)p.a.N, G = (int)p.a.G;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
+    const int n = (int)(i % NP), w = (int)(i / NP % 2);
+    const long r = i / (2 * NP), tok = r / G, g = r - tok * G;
+    if (r == rows) {
+      p.a.bc[i] = 0.f;
+      continue;
+    }
+    const long b = tok / p.a.T, t = tok - b * p.a.T;
+    const T* s = w ? (const T*)p.a.C + b * p.a.C_sb + t * p.a.C_st + g * p.a.C_sg
+                   : (const T*)p.a.B + b * p.a.B_sb + t * p.a.B_st + g * p.a.B_sg;
+    p.a.bc[i] = n < N ? to_f32(s[n]) : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------------------
-// Forward: MODE 0 a piece's own state and summed delta', 1 the outputs; MODE 2 the reverse of 0
-// for the backward: the carry that a piece hands to the one before it, from a zero carry.
+// A wave walks a piece for 64 channels. MODE 0: a piece's own state and summed delta'. MODE 1:
+// the outputs. MODE 2: the reverse of 0 for the backward, the carry that a piece hands to the one
+// before it, from a zero carry.
 // ---------------------------------------------------------------------------
-template <typename T, int LQ, int MODE>
-__global__ __launch_bounds__(SS_NT) void scan_kernel(ScanParams p) {
-  using L = Lay<LQ>;
-  __shared__ float2 sDD[SS_K][L::CT];
-  __shared__ float sB[SS_K][L::NP];
-  __shared__ float sC[MODE == 1 ? SS_K : 1][L::NP];
-  __shared__ float sY[MODE == 1 ? SS_K : 1][L::YP];
+template <typename T, int NP, int MODE>
+__global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_kernel(ScanParams p) {
   const tops_gla_scan_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tile = blockIdx.x % p.ntiles, pi = blockIdx.x / p.ntiles;
+  const int lane = threadIdx.x & 63;
+  const long item = blockIdx.x * 4L + uni(threadIdx.x >> 6);
+  if (item >= p.npieces * p.ntiles) return;
+  const int pi = uni((int)(item / p.ntiles));
+  const Tile tl(p, uni((int)(item - (long)pi * p.ntiles)));
   const Piece pc = piece_of(p, pi);
   if (MODE == 0 && pc.idx == pc.np - 1) return;   // nobody folds it
   if (MODE == 2 && pc.idx == 0) return;
   const int D = (int)a.D, N = (int)a.N;
-  const int DG = D / (int)a.G, grp = tile / p.tiles_g;
-  const int cb = (tile % p.tiles_g) * L::CT;      // first channel of the block in its group
-  const int d0 = grp * DG + cb, nch = min(L::CT, DG - cb);
+  const bool live = lane < tl.nch;
+  const uint32_t lo = live ? lane : 0;
+  const long dl = tl.d0 + lo;
 
-  // the lane's states
-  const int ch = wave * L::CPW + (lane & (L::CPW - 1)), n0 = 4 * (lane / L::CPW);
-  const bool live = ch < nch;
-  const long dl = d0 + (live ? ch : 0);
-  float A[4], h[4] = {};
+  float A[NP], h[NP];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A[i] = live && n0 + i < N ? a.A[dl * N + n0 + i] * kLog2e : 0.f;
-  float dsum = 0.f;
+  for (int n = 0; n < NP; ++n) {
+    A[n] = n < N ? scaled_a(a.A[dl * N + n]) : 0.f;
+    h[n] = 0.f;
+  }
   if (MODE == 1) {
-    if (a.h0 && live)
+    if (p.multi) {
+      load4<NP>(a.piece_h + ((long)pi * D + dl) * NP, h);
+    } else if (a.h0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n0 + i < N) h[i] = a.h0[((long)pc.seq * D + dl) * N + n0 + i];
-    for (int j = pi - pc.idx; j < pi; ++j) {
-      const float4 l = *reinterpret_cast<const float4*>(a.piece_h + ((long)j * D + dl) * L::NP + n0);
-      const float s = a.piece_dt[(long)j * D + dl];
-      const float lv[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)   // a zero state stays zero under a decay that overflows
-        h[i] = h[i] == 0.f ? lv[i] : fmaf(exp2_hw(A[i] * s), h[i], lv[i]);
+      for (int n = 0; n < NP; ++n)
+        if (n < N) h[n] = a.h0[((long)pc.seq * D + dl) * N + n];
     }
   }
+  const float bias = a.delta_bias ? a.delta_bias[dl] : 0.f;
+  const float skip = MODE == 1 && a.Dskip ? a.Dskip[dl] : 0.f;
+  const bool has_z = MODE != 0 && a.z != nullptr, softplus = a.softplus;
+  float dsum = 0.f;
 
-  // the thread's part of a tile
-  const int tt = tid / (L::CT / L::EPT), tc = (tid % (L::CT / L::EPT)) * L::EPT;
-  const int nv = min(L::EPT, nch - tc);
-  float bias[L::EPT], dskip[L::EPT];
-#pragma unroll
-  for (int e = 0; e < L::EPT; ++e) {
-    bias[e] = a.delta_bias && e < nv ? a.delta_bias[d0 + tc + e] : 0.f;
-    dskip[e] = MODE == 1 && a.Dskip && e < nv ? a.Dskip[d0 + tc + e] : 0.f;
-  }
-  const T* gu = (const T*)(MODE == 2 ? a.dy : a.u) +
-                pc.b * (MODE == 2 ? a.dy_sb : a.u_sb) + d0 + tc;
+  // rows of the tensors: uniform addresses, a lane's offset of 32 bits
+  const T* gu = MODE == 2 ? (const T*)a.dy + pc.b * a.dy_sb + tl.d0
+                          : (const T*)a.u + pc.b * a.u_sb + tl.d0;
   const long u_st = MODE == 2 ? a.dy_st : a.u_st;
-  const T* gd = (const T*)a.delta + pc.b * a.delta_sb + d0 + tc;
-  const T* gz = (const T*)a.z + (a.z ? pc.b * a.z_sb + d0 + tc : 0);
-  const T* gB = MODE == 2 ? (const T*)a.C + pc.b * a.C_sb + (long)grp * a.C_sg
-                          : (const T*)a.B + pc.b * a.B_sb + (long)grp * a.B_sg;
-  const long B_st = MODE == 2 ? a.C_st : a.B_st;
-  const T* gC = (const T*)a.C + pc.b * a.C_sb + (long)grp * a.C_sg;
-  const bool has_z = a.z != nullptr && MODE != 0;
+  const T* gd = (const T*)a.delta + pc.b * a.delta_sb + tl.d0;
+  const T* gz = has_z ? (const T*)a.z + pc.b * a.z_sb + tl.d0 : nullptr;
+  const long bc_st = a.G * 2 * NP;
+  const float* bc = a.bc + (pc.b * a.T * a.G + tl.grp) * 2 * NP + (MODE == 2 ? NP : 0);
+  const float* bc_end = a.bc + p.tokens * bc_st;
 
-  float ru[L::EPT], rd[L::EPT], rz[L::EPT], rb[L::BPT];
-  constexpr int BN = SS_K * L::NP;   // elements of B of a tile
+  T ru[SS_K], rd[SS_K], rz[SS_K];
   auto load = [&](int t0) {
-    const int t = t0 + tt;
-    const int v = t < pc.t1 ? nv : 0;
-    load_run<T, L::EPT>(gu + (v > 0 ? t * u_st : 0), v, p.vec, ru);
-    load_run<T, L::EPT>(gd + (v > 0 ? t * a.delta_st : 0), v, p.vec, rd);
-    if (has_z) load_run<T, L::EPT>(gz + (v > 0 ? t * a.z_st : 0), v, p.vec, rz);
-#pragma unroll
-    for (int j = 0; j < L::BPT; ++j) {
-      const int i = tid + SS_NT * j;   // B, then C: 2 BN = BPT * SS_NT elements in all
-      const int r = i % BN, bt = t0 + r / L::NP, n = r % L::NP;
-      const bool ok = bt < pc.t1 && n < N && (i < BN || MODE == 1);
-      const T* g = i < BN ? gB + (ok ? bt * B_st : 0) : gC + (ok ? bt * a.C_st : 0);
-      rb[j] = ok ? to_f32(g[n]) : 0.f;
-    }
+    load_rows<T, SS_K>(gu, u_st, t0, pc.t1, lo, ru);
+    load_rows<T, SS_K>(gd, a.delta_st, t0, pc.t1, lo, rd);
+    if (has_z) load_rows<T, SS_K>(gz, a.z_st, t0, pc.t1, lo, rz);
   };
   const int nt = (pc.t1 - pc.t0 + SS_K - 1) / SS_K;
   const int first = MODE == 2 ? nt - 1 : 0, step = MODE == 2 ? -1 : 1;
   if (nt > 0) load(pc.t0 + first * SS_K);
+#pragma unroll 1
   for (int it = 0; it < nt; ++it) {
     const int k = first + it * step, t0 = pc.t0 + k * SS_K;
-    const bool valid = t0 + tt < pc.t1;
-    float ku[L::EPT], kz[L::EPT];
-    float2 dd[L::EPT];
+    float d[SS_K], u[SS_K], z[SS_K], y[SS_K];
 #pragma unroll
-    for (int e = 0; e < L::EPT; ++e) {
-      float d = rd[e] + bias[e], sg;
-      if (a.softplus) softplus_sigmoid(d, d, sg);
-      if (!valid || e >= nv) d = 0.f;   // a token past the end leaves the state as it is
-      float x = d * ru[e];
-      if (MODE == 2) x = has_z ? ru[e] * rz[e] * sigmoid(rz[e]) : ru[e];
-      dd[e] = make_float2(d, x);
-      ku[e] = ru[e];
-      kz[e] = rz[e];
+    for (int i = 0; i < SS_K; ++i) {
+      d[i] = to_f32(rd[i]) + bias;
+      u[i] = to_f32(ru[i]);
+      z[i] = has_z ? to_f32(rz[i]) : 0.f;
     }
+    if (softplus)
 #pragma unroll
-    for (int e = 0; e < L::EPT; ++e) sDD[tt][tc + e] = dd[e];
+      for (int i = 0; i < SS_K; ++i) {
+        float sg;
+        softplus_sigmoid(d[i], d[i], sg);
+      }
+    if (MODE == 2 && has_z)
 #pragma unroll
-    for (int j = 0; j < L::BPT; ++j) {
-      const int i = tid + SS_NT * j, r = i % BN;
-      if (i < BN)
-        sB[r / L::NP][r % L::NP] = rb[j];
-      else if (MODE == 1)
-        sC[r / L::NP][r % L::NP] = rb[j];
-    }
-    __syncthreads();
-    if (it + 1 < nt) load(pc.t0 + (k + step) * SS_K);
+      for (int i = 0; i < SS_K; ++i) u[i] *= z[i] * sigmoid(z[i]);
+#pragma unroll
+    for (int i = 0; i < SS_K; ++i)   // a token past the end leaves the state as it is
+      if (t0 + i >= pc.t1) d[i] = u[i] = 0.f;
+    if (it + 1 < nt) load(t0 + step * SS_K);
     if (MODE == 1 && a.chunk_h && live)
-      *reinterpret_cast<float4*>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * L::NP + n0) =
-          make_float4(h[0], h[1], h[2], h[3]);
+      store4<NP>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * NP, h);
+    const float* rp = bc + t0 * bc_st;
+    if (MODE == 2) rp = t0 + SS_K - 1 < pc.t1 ? rp + (SS_K - 1) * bc_st : bc_end;
 #pragma unroll
-    for (int q = 0; q < SS_K; q += 4) {
-      float yv[4];
+    for (int j = 0; j < SS_K; ++j) {
+      const int i = MODE == 2 ? SS_K - 1 - j : j;
+      cfloat* row = row_after(rp, h);
+      if (MODE == 2)
+        rp = t0 + i - 1 < pc.t1 ? bc + (t0 + i - 1) * bc_st : bc_end;
+      else
+        rp = t0 + i + 1 < pc.t1 ? rp + bc_st : bc_end;
+      const float x = MODE == 2 ? u[i] : d[i] * u[i];
+      float acc[2] = {0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int t = MODE == 2 ? SS_K - 1 - (q + s) : q + s;
-        const float2 d = sDD[t][ch];
-        const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][n0]);
-        const float bv[4] = {b4.x, b4.y, b4.z, b4.w};
-        float cv[4] = {};
-        if (MODE == 1) {
-          const float4 c4 = *reinterpret_cast<const float4*>(&sC[t][n0]);
-          cv[0] = c4.x, cv[1] = c4.y, cv[2] = c4.z, cv[3] = c4.w;
+      for (int n = 0; n < NP; ++n) {
+        const float ex = exp2_hw(A[n] * d[i]);
+        if (MODE == 2) {
+          h[n] = ex * fmaf(x, row[n], h[n]);
+        } else {
+          h[n] = fmaf(ex, h[n], x * row[n]);
+          if (MODE == 1) acc[n & 1] = fmaf(h[n], row[NP + n], acc[n & 1]);
         }
-        float y = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float ex = exp2_hw(A[i] * d.x);
-          if (MODE == 2) {
-            h[i] = ex * fmaf(bv[i], d.y, h[i]);
-          } else {
-            h[i] = fmaf(ex, h[i], d.y * bv[i]);
-            if (MODE == 1) y = i == 0 ? cv[0] * h[0] : fmaf(cv[i], h[i], y);
-          }
-        }
-        yv[s] = y;
-        if (MODE != 1) dsum += d.x;
       }
-      if (MODE == 1) {
-        const float y = sum_states<LQ>(yv[0], yv[1], yv[2], yv[3]);
-        const int row = lane >> 4, tm = ((row & 1) << 1) | (row >> 1);
-        if ((lane & 15) < L::CPW) sY[q + tm][wave * L::CPW + (lane & (L::CPW - 1))] = y;
-      }
+      y[i] = acc[0] + acc[1];
+      if (MODE == 1) asm volatile("" : "+v"(y[i]));   // before the next token's rows, like h
+      if (MODE != 1) dsum += d[i];
     }
-    __syncthreads();
-    if (MODE == 1 && valid && nv > 0) {
-      float o[L::EPT];
+    if (MODE == 1) {
+      T* gy = (T*)a.y + (pc.b * a.T + t0) * D + tl.d0;
 #pragma unroll
-      for (int e = 0; e < L::EPT; ++e) {
-        o[e] = fmaf(dskip[e], ku[e], sY[tt][tc + e]);
-        if (has_z) o[e] *= kz[e] * sigmoid(kz[e]);
-      }
-      T* gy = (T*)a.y + (pc.b * a.T + t0 + tt) * D + d0 + tc;
-      store_n<T, L::EPT>(gy, nv, p.vec, o);
+      for (int i = 0; i < SS_K; ++i) y[i] = fmaf(skip, u[i], y[i]);
+      if (has_z)
+#pragma unroll
+        for (int i = 0; i < SS_K; ++i) y[i] *= z[i] * sigmoid(z[i]);
+      if (live)
+#pragma unroll
+        for (int i = 0; i < SS_K; ++i)
+          if (t0 + i < pc.t1) (gy + (long)i * D)[lo] = from_f32<T>(y[i]);
     }
   }
   if (!live) return;
   if (MODE == 1) {
     if (a.ht && pc.idx == pc.np - 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n0 + i < N) a.ht[((long)pc.seq * D + dl) * N + n0 + i] = h[i];
+      for (int n = 0; n < NP; ++n)
+        if (n < N) a.ht[((long)pc.seq * D + dl) * N + n] = h[n];
   } else {
-    *reinterpret_cast<float4*>(a.piece_h + ((long)pi * D + dl) * L::NP + n0) =
-        make_float4(h[0], h[1], h[2], h[3]);
-    if (n0 == 0) a.piece_dt[(long)pi * D + dl] = dsum;
+    store4<NP>(a.piece_h + ((long)pi * D + dl) * NP, h);
+    a.piece_dt[(long)pi * D + dl] = dsum;
+  }
+}
+
+// The pieces' entry states in the place of their own ones, a thread for four states of a channel
+// of a sequence: h <- exp(A S_j) h + L_j from h0 on, or backward from dht on with REV.
+template <int NP, bool REV>
+__global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
+  const tops_gla_scan_args& a = p.a;
+  const int pi = blockIdx.x / nb;
+  const Piece pc = piece_of(p, pi);
+  if (pc.idx != 0) return;
+  const int q = (blockIdx.x - pi * nb) * 256 + threadIdx.x;
+  const int D = (int)a.D, N = (int)a.N, d = q / (NP / 4), n0 = q % (NP / 4) * 4;
+  if (d >= D) return;
+  const float* init = REV ? a.dht : a.h0;
+  float A[4], h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = n0 + i < N;
+    A[i] = in ? scaled_a(a.A[(long)d * N + n0 + i]) : 0.f;
+    h[i] = in && init ? init[((long)pc.seq * D + d) * N + n0 + i] : 0.f;
+  }
+  constexpr int U = 8;
+  const long hs = (REV ? -1L : 1L) * D * NP, ss = (REV ? -1L : 1L) * D;
+  const long j0 = pi + (REV ? pc.np - 1 : 0);
+  float* H = a.piece_h + (j0 * D + d) * NP + n0;
+  const float* S = a.piece_dt + j0 * D + d;
+  for (int j = 0; j < pc.np; j += U) {
+    float4 l[U];
+    float s[U];
+    const int m = min(U, pc.np - 1 - j);   // the last piece's own state is not there
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = max(0, min(i, m - 1));
+      l[i] = *reinterpret_cast<const float4*>(H + c * hs);
+      s[i] = S[c * ss];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (j + i < pc.np) {
+        *reinterpret_cast<float4*>(H + i * hs) = make_float4(h[0], h[1], h[2], h[3]);
+        const float lv[4] = {l[i].x, l[i].y, l[i].z, l[i].w};
+        if (i < m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)   // a zero state stays zero under a decay that overflows
+            h[e] = h[e] == 0.f ? lv[e] : fmaf(exp2_hw(A[e] * s[i]), h[e], lv[e]);
+      }
+    }
+    H += U * hs;
+    S += U * ss;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Backward, over a piece's chunks of 16 tokens from the last one on. With g_t the gradient of
-// h_t, g_t = C_t dy_t + a_{t+1} g_{t+1}:
+// Backward, over a piece's tiles of 8 tokens from the last one on. With g_t the gradient of h_t,
+// g_t = C_t dy_t + a_{t+1} g_{t+1}:
 //   dC_t = sum_d dy_t h_t          dB_t = sum_d g_t delta' u        du = delta' sum_n g B + D dy
 //   ddelta' = u sum_n g B + sum_n g a h_{t-1} A                     dA = sum_t g a h_{t-1} delta'
-// A chunk's states run forward again from the one that the forward kept, with a_t and h_t of its
-// 16 tokens in registers (recovering h_{t-1} from h_t would divide by a_t).
+// A tile's states run forward again from the one that the forward kept, with a_t and h_t of its
+// tokens in registers (recovering h_{t-1} from h_t would divide by a_t).
+//
+// A lane holds 8 states of a channel, the NW = NP / 8 waves of a channel group a part of the
+// states each. They share what is formed once for a (token, channel) through LDS: each wave
+// stages 8 / NW of the tile's tokens and, once the waves' sums over n are there, finishes them.
 // ---------------------------------------------------------------------------
-template <typename T, int LQ>
-__global__ __launch_bounds__(SS_NT, 2) void scan_bwd_kernel(ScanParams p) {
-  using L = Lay<LQ>;
-  __shared__ float2 sDD[SS_K][L::CT];
-  __shared__ float sDy[SS_K][L::CT];
-  __shared__ float sB[SS_K][L::NP], sC[SS_K][L::NP];
-  __shared__ float sS[3][SS_K][L::YP];            // sum_n g B, sum_n g a h A log2(e), sum_n C h
-  __shared__ float sBC[8][SS_K][2 * L::NP];       // a wave's dB and dC
-  const tops_gla_scan_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tile = blockIdx.x % p.ntiles, pi = blockIdx.x / p.ntiles;
-  const Piece pc = piece_of(p, pi);
-  const int D = (int)a.D, N = (int)a.N;
-  const int DG = D / (int)a.G, grp = tile / p.tiles_g;
-  const int cb = (tile % p.tiles_g) * L::CT;
-  const int d0 = grp * DG + cb, nch = min(L::CT, DG - cb);
-  const int ch = wave * L::CPW + (lane & (L::CPW - 1)), n0 = 4 * (lane / L::CPW);
-  const bool live = ch < nch;
-  const long dl = d0 + (live ? ch : 0);
-  float A[4], carry[4] = {}, dA[4] = {};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) A[i] = live && n0 + i < N ? a.A[dl * N + n0 + i] * kLog2e : 0.f;
-  if (a.dht && live)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n0 + i < N) carry[i] = a.dht[((long)pc.seq * D + dl) * N + n0 + i];
-  for (int j = pi - pc.idx + pc.np - 1; j > pi; --j) {
-    const float4 l = *reinterpret_cast<const float4*>(a.piece_h + ((long)j * D + dl) * L::NP + n0);
-    const float s = a.piece_dt[(long)j * D + dl];
-    const float lv[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      carry[i] = carry[i] == 0.f ? lv[i] : fmaf(exp2_hw(A[i] * s), carry[i], lv[i]);
-  }
+template <int NP>
+struct Bwd {
+  static constexpr int NW = NP / 8;                // waves of a channel group
+  static constexpr int WAVES = NP == 64 ? 8 : 4;   // of a block
+  static constexpr int GPB = WAVES / NW;           // channel groups (of 64) of a block
+  static constexpr int CT = 64 * GPB;
+  static constexpr int TPW = SS_K / NW;            // tokens that a wave stages
+};
 
-  const int tt = tid / (L::CT / L::EPT), tc = (tid % (L::CT / L::EPT)) * L::EPT;
-  const int nv = min(L::EPT, nch - tc);
-  float bias[L::EPT], dskip[L::EPT], accD[L::EPT] = {}, accB[L::EPT] = {};
+// Level of a transposing sum over the lanes of a row of 16: lanes of the banks that `odd` names
+// get b's sum with lane `ctrl`, the others a's. (A DPP or swap operand may be read two wait states
+// after it was written; the compiler does not see these writes and reads.)
+#define TOPS_PAIR4(ctrl, odd, a0, b0, a1, b1, a2, b2, a3, b3)                                   \
+  asm("s_nop 1\n\t"                                                                             \
+      "v_add_f32_dpp %0, %0, %0 " ctrl " row_mask:0xf bank_mask:0xf\n\t"                        \
+      "v_add_f32_dpp %1, %1, %1 " ctrl " row_mask:0xf bank_mask:0xf\n\t"                        \
+      "v_add_f32_dpp %2, %2, %2 " ctrl " row_mask:0xf bank_mask:0xf\n\t"                        \
+      "v_add_f32_dpp %3, %3, %3 " ctrl " row_mask:0xf bank_mask:0xf\n\t"                        \
+      "v_add_f32_dpp %0, %4, %4 " ctrl " row_mask:0xf bank_mask:" odd "\n\t"                    \
+      "v_add_f32_dpp %1, %5, %5 " ctrl " row_mask:0xf bank_mask:" odd "\n\t"                    \
+      "v_add_f32_dpp %2, %6, %6 " ctrl " row_mask:0xf bank_mask:" odd "\n\t"                    \
+      "v_add_f32_dpp %3, %7, %7 " ctrl " row_mask:0xf bank_mask:" odd "\n\ts_nop 1"              \
+      : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3)                                                  \
+      : "v"(b0), "v"(b1), "v"(b2), "v"(b3))
+
+// x[0..7] and y[0..7] summed over the 64 lanes: lane l ends with element 4 l[2] + 2 l[4] + l[5]
+// of x, of y where bit 3 is set (l[i]: bit i of l).
+__device__ __forceinline__ float sum_channels(float (&x)[8], float (&y)[8]) {
+  TOPS_PAIR4("row_ror:8", "0xc", x[0], y[0], x[1], y[1], x[2], y[2], x[3], y[3]);
+  TOPS_PAIR4("row_ror:8", "0xc", x[4], y[4], x[5], y[5], x[6], y[6], x[7], y[7]);
+  TOPS_PAIR4("row_half_mirror", "0xa", x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]);
+  float s = swap32_add(swap16_add(x[0], x[2]), swap16_add(x[1], x[3]));
+  s += dpp<0xb1>(s);      // quad_perm [1, 0, 3, 2]
+  return s + dpp<0x4e>(s);   // quad_perm [2, 3, 0, 1]
+}
+
+template <typename T, int NP>
+__global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanParams p) {
+  using L = Bwd<NP>;
+  __shared__ float sD[SS_K][L::CT], sU[SS_K][L::CT], sG[SS_K][L::CT];   // delta', u, dy silu(z)
+  __shared__ float sS[L::NW][3][SS_K][L::CT];   // sum_n g B, sum_n g a h A log2(e), sum_n C h
+  __shared__ float sBC[L::GPB][SS_K][2 * NP];   // a channel group's dB and dC
+  const tops_gla_scan_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int part = wave % L::NW, cg = wave / L::NW;
+  const int tile = blockIdx.x % p.btiles, pi = blockIdx.x / p.btiles;
+  const Piece pc = piece_of(p, pi);
+  const int D = (int)a.D, N = (int)a.N, DG = D / (int)a.G;
+  const int btiles_g = p.btiles / (int)a.G, grp = tile / btiles_g;
+  const int cb = (tile - grp * btiles_g) * L::CT + 64 * cg;   // first channel in its group
+  const int d0 = grp * DG + min(cb, DG - 1);
+  const bool live = cb + lane < DG;
+  const uint32_t lo = live ? lane : 0;
+  const long dl = d0 + lo;
+  const int n0 = 8 * part, col = 64 * cg + lane;
+  float A[8], carry[8], dA[8];
 #pragma unroll
-  for (int e = 0; e < L::EPT; ++e) {
-    bias[e] = a.delta_bias && e < nv ? a.delta_bias[d0 + tc + e] : 0.f;
-    dskip[e] = a.Dskip && e < nv ? a.Dskip[d0 + tc + e] : 0.f;
+  for (int n = 0; n < 8; ++n) {
+    A[n] = live && n0 + n < N ? scaled_a(a.A[dl * N + n0 + n]) : 0.f;
+    carry[n] = dA[n] = 0.f;
   }
-  const T* gu = (const T*)a.u + pc.b * a.u_sb + d0 + tc;
-  const T* gd = (const T*)a.delta + pc.b * a.delta_sb + d0 + tc;
-  const T* gz = (const T*)a.z + (a.z ? pc.b * a.z_sb + d0 + tc : 0);
-  const T* gy = (const T*)a.dy + pc.b * a.dy_sb + d0 + tc;
-  const T* gB = (const T*)a.B + pc.b * a.B_sb + (long)grp * a.B_sg;
-  const T* gC = (const T*)a.C + pc.b * a.C_sb + (long)grp * a.C_sg;
-  const bool has_z = a.z != nullptr;
-  float ru[L::EPT], rd[L::EPT], rz[L::EPT], ry[L::EPT], rb[L::BPT];
-  float4 rh;
-  constexpr int BN = SS_K * L::NP;
-  auto load = [&](int k) {
-    const int t0 = pc.t0 + k * SS_K, t = t0 + tt;
-    const int v = t < pc.t1 ? nv : 0;
-    load_run<T, L::EPT>(gu + (v > 0 ? t * a.u_st : 0), v, p.vec, ru);
-    load_run<T, L::EPT>(gd + (v > 0 ? t * a.delta_st : 0), v, p.vec, rd);
-    if (has_z) load_run<T, L::EPT>(gz + (v > 0 ? t * a.z_st : 0), v, p.vec, rz);
-    load_run<T, L::EPT>(gy + (v > 0 ? t * a.dy_st : 0), v, p.vec, ry);
+  if (live) {
+    if (p.multi) {
+      load4<8>(a.piece_h + ((long)pi * D + dl) * NP + n0, carry);
+    } else if (a.dht) {
 #pragma unroll
-    for (int j = 0; j < L::BPT; ++j) {
-      const int i = tid + SS_NT * j;
-      const int r = i % BN, bt = t0 + r / L::NP, n = r % L::NP;
-      const bool ok = bt < pc.t1 && n < N;
-      const T* g = i < BN ? gB + (ok ? bt * a.B_st : 0) : gC + (ok ? bt * a.C_st : 0);
-      rb[j] = ok ? to_f32(g[n]) : 0.f;
+      for (int n = 0; n < 8; ++n)
+        if (n0 + n < N) carry[n] = a.dht[((long)pc.seq * D + dl) * N + n0 + n];
     }
-    rh = *reinterpret_cast<const float4*>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * L::NP + n0);
+  }
+  const float bias = a.delta_bias ? a.delta_bias[dl] : 0.f;
+  const float skip = a.Dskip ? a.Dskip[dl] : 0.f;
+  const bool has_z = a.z != nullptr, softplus = a.softplus;
+  float accD = 0.f, accB = 0.f;
+
+  const T* gu = (const T*)a.u + pc.b * a.u_sb + d0;
+  const T* gd = (const T*)a.delta + pc.b * a.delta_sb + d0;
+  const T* gz = has_z ? (const T*)a.z + pc.b * a.z_sb + d0 : nullptr;
+  const T* gy = (const T*)a.dy + pc.b * a.dy_sb + d0;
+  const float* bc = a.bc + (pc.b * a.T * a.G + grp) * 2 * NP + n0;
+  const long bc_st = a.G * 2 * NP;
+  const float* bc_end = a.bc + p.tokens * bc_st;
+  T ru[L::TPW], rd[L::TPW], rz[L::TPW], ry[L::TPW];
+  float rh[8];
+  auto load = [&](int k) {
+    const int t0 = min(pc.t0 + k * SS_K + part * L::TPW, pc.t1 - 1);
+    load_rows<T, L::TPW>(gu, a.u_st, t0, pc.t1, lo, ru);
+    load_rows<T, L::TPW>(gd, a.delta_st, t0, pc.t1, lo, rd);
+    load_rows<T, L::TPW>(gy, a.dy_st, t0, pc.t1, lo, ry);
+    if (has_z) load_rows<T, L::TPW>(gz, a.z_st, t0, pc.t1, lo, rz);
+    load4<8>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * NP + n0, rh);
   };
   const int nt = (pc.t1 - pc.t0 + SS_K - 1) / SS_K;
   if (nt > 0) load(nt - 1);
+#pragma unroll 1
   for (int k = nt - 1; k >= 0; --k) {
-    const int t0 = pc.t0 + k * SS_K;
-    const bool valid = t0 + tt < pc.t1;
-    float kd[L::EPT], ks[L::EPT], ku[L::EPT], kz[L::EPT], ky[L::EPT];
+    const int t0 = pc.t0 + k * SS_K, ts = part * L::TPW;
+    float ks[L::TPW], kz[L::TPW], ky[L::TPW];
 #pragma unroll
-    for (int e = 0; e < L::EPT; ++e) {
-      float d = rd[e] + bias[e], sg = 1.f;
-      if (a.softplus) softplus_sigmoid(d, d, sg);
-      if (!valid || e >= nv) d = 0.f;
-      kd[e] = d;
-      ks[e] = sg;
-      ku[e] = ru[e];
-      kz[e] = has_z ? rz[e] : 0.f;
-      ky[e] = ry[e];
-      sDD[tt][tc + e] = make_float2(d, d * ru[e]);
-      sDy[tt][tc + e] = has_z ? ry[e] * rz[e] * sigmoid(rz[e]) : ry[e];
+    for (int i = 0; i < L::TPW; ++i) {
+      const bool in = live && t0 + ts + i < pc.t1;
+      float d = to_f32(rd[i]) + bias, sg = 1.f;
+      if (softplus) softplus_sigmoid(d, d, sg);
+      ks[i] = sg;
+      ky[i] = to_f32(ry[i]);
+      kz[i] = has_z ? to_f32(rz[i]) : 0.f;
+      const float g = has_z ? ky[i] * kz[i] * sigmoid(kz[i]) : ky[i];
+      sD[ts + i][col] = in ? d : 0.f;
+      sU[ts + i][col] = in ? to_f32(ru[i]) : 0.f;
+      sG[ts + i][col] = in ? g : 0.f;
     }
+    float av[SS_K][8], hv[SS_K][8], hin[8];
 #pragma unroll
-    for (int j = 0; j < L::BPT; ++j) {
-      const int i = tid + SS_NT * j, r = i % BN;
-      (i < BN ? sB : sC)[r / L::NP][r % L::NP] = rb[j];
-    }
-    const float hin[4] = {live ? rh.x : 0.f, live ? rh.y : 0.f, live ? rh.z : 0.f,
-                          live ? rh.w : 0.f};
+    for (int n = 0; n < 8; ++n) hin[n] = live ? rh[n] : 0.f;
     __syncthreads();
     if (k > 0) load(k - 1);
 
-    float av[SS_K][4], hv[SS_K][4];
+    const float* rp = bc + t0 * bc_st;
 #pragma unroll
     for (int t = 0; t < SS_K; ++t) {
-      const float2 d = sDD[t][ch];
-      const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][n0]);
-      const float bv[4] = {b4.x, b4.y, b4.z, b4.w};
+      cfloat* row = row_after(rp, t ? hv[t - 1] : hin);
+      if (t < SS_K - 1) rp = t0 + t + 1 < pc.t1 ? rp + bc_st : bc_end;
+      const float d = sD[t][col], x = d * sU[t][col];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        av[t][i] = exp2_hw(A[i] * d.x);
-        hv[t][i] = fmaf(av[t][i], t ? hv[t - 1][i] : hin[i], d.y * bv[i]);
+      for (int n = 0; n < 8; ++n) {
+        av[t][n] = exp2_hw(A[n] * d);
+        hv[t][n] = fmaf(av[t][n], t ? hv[t - 1][n] : hin[n], x * row[n]);
       }
     }
+    fence();
 #pragma unroll
-    for (int q = SS_K - 4; q >= 0; q -= 4) {
-      float s1[4], s2[4], s3[4];
+    for (int t = SS_K - 1; t >= 0; --t) {
+      cfloat* row = row_after(rp, carry);
+      rp = t0 + t - 1 < pc.t1 ? bc + (t0 + t - 1) * bc_st : bc_end;
+      const float d = sD[t][col], x = d * sU[t][col], dy = sG[t][col];
+      float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-      for (int s = 3; s >= 0; --s) {
-        const int t = q + s;
-        const float2 d = sDD[t][ch];
-        const float dy = sDy[t][ch];
-        const float4 b4 = *reinterpret_cast<const float4*>(&sB[t][n0]);
-        const float4 c4 = *reinterpret_cast<const float4*>(&sC[t][n0]);
-        const float bv[4] = {b4.x, b4.y, b4.z, b4.w}, cv[4] = {c4.x, c4.y, c4.z, c4.w};
-        float v[8];
-        s1[s] = s2[s] = s3[s] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float g = fmaf(cv[i], dy, carry[i]);
-          const float hp = t ? hv[t - 1][i] : hin[i];
-          v[i] = g * d.y;
-          v[4 + i] = dy * hv[t][i];
-          s1[s] = fmaf(g, bv[i], s1[s]);
-          carry[i] = av[t][i] * g;
-          const float gp = carry[i] * hp;
-          s2[s] = fmaf(gp, A[i], s2[s]);
-          s3[s] = fmaf(cv[i], hv[t][i], s3[s]);
-          dA[i] = fmaf(gp, d.x, dA[i]);
-        }
-        sum_channels<L::CPW>(v, lane, &sBC[wave][t][0], n0, L::NP);
+      for (int n = 0; n < 8; ++n) {
+        const float g = fmaf(dy, row[NP + n], carry[n]);
+        const float hp = t ? hv[t - 1][n] : hin[n];
+        vb[n] = g * x;
+        vc[n] = dy * hv[t][n];
+        s1 = fmaf(g, row[n], s1);
+        carry[n] = av[t][n] * g;
+        const float gp = carry[n] * hp;
+        s2 = fmaf(gp, A[n], s2);
+        s3 = fmaf(hv[t][n], row[NP + n], s3);
+        dA[n] = fmaf(gp, d, dA[n]);
       }
-      const int row = lane >> 4, tm = ((row & 1) << 1) | (row >> 1);
-      const float r1 = sum_states<LQ>(s1[0], s1[1], s1[2], s1[3]);
-      const float r2 = sum_states<LQ>(s2[0], s2[1], s2[2], s2[3]);
-      const float r3 = has_z ? sum_states<LQ>(s3[0], s3[1], s3[2], s3[3]) : 0.f;
-      if ((lane & 15) < L::CPW) {
-        const int c = wave * L::CPW + (lane & (L::CPW - 1));
-        sS[0][q + tm][c] = r1;
-        sS[1][q + tm][c] = r2;
-        sS[2][q + tm][c] = r3;
-      }
+      sS[part][0][t][col] = s1;
+      sS[part][1][t][col] = s2;
+      sS[part][2][t][col] = s3;
+      const float r = sum_channels(vb, vc);
+      if ((lane & 3) == 0)
+        sBC[cg][t][(lane & 8 ? NP : 0) + n0 + (lane & 4) + ((lane >> 3) & 2) + (lane >> 5)] = r;
+      fence();
     }
     __syncthreads();
-    if (valid && nv > 0) {
-      float odu[L::EPT], odd[L::EPT], odz[L::EPT];
 #pragma unroll
-      for (int e = 0; e < L::EPT; ++e) {
-        const float s1 = sS[0][tt][tc + e], s2 = sS[1][tt][tc + e];
-        float dy = ky[e];
-        if (has_z) {
-          const float sz = sigmoid(kz[e]);
-          dy = ky[e] * kz[e] * sz;
-          odz[e] = ky[e] * fmaf(dskip[e], ku[e], sS[2][tt][tc + e]) *
-                   (sz * fmaf(kz[e], 1.f - sz, 1.f));
-        }
-        odu[e] = fmaf(s1, kd[e], dskip[e] * dy);
-        odd[e] = fmaf(s1, ku[e], s2 * kLn2) * ks[e];
-        accD[e] = fmaf(dy, ku[e], accD[e]);
-        accB[e] += odd[e];
+    for (int i = 0; i < L::TPW; ++i) {
+      const int t = ts + i;
+      float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+      for (int w = 0; w < L::NW; ++w) {
+        s1 += sS[w][0][t][col];
+        s2 += sS[w][1][t][col];
+        s3 += sS[w][2][t][col];
       }
-      const long o = (pc.b * a.T + t0 + tt) * D + d0 + tc;
-      store_n<T, L::EPT>((T*)a.du + o, nv, p.vec, odu);
-      store_n<T, L::EPT>((T*)a.ddelta + o, nv, p.vec, odd);
-      if (has_z) store_n<T, L::EPT>((T*)a.dz + o, nv, p.vec, odz);
+      const float d = sD[t][col], u = sU[t][col], dy = sG[t][col];
+      const float du = fmaf(s1, d, skip * dy), dd = fmaf(s1, u, s2 * kLn2) * ks[i];
+      const float sz = sigmoid(kz[i]);
+      const float dz = ky[i] * fmaf(skip, u, s3) * (sz * fmaf(kz[i], 1.f - sz, 1.f));
+      if (live && t0 + t < pc.t1) {
+        accD = fmaf(dy, u, accD);
+        accB += dd;
+        const long o = (pc.b * a.T + t0 + t) * D + d0;
+        ((T*)a.du + o)[lo] = from_f32<T>(du);
+        ((T*)a.ddelta + o)[lo] = from_f32<T>(dd);
+        if (has_z) ((T*)a.dz + o)[lo] = from_f32<T>(dz);
+      }
     }
     // the block's share of dB and dC: [tile of the group][token][group][2][NP]
-    for (int i = tid; i < SS_K * 2 * L::NP; i += SS_NT) {
-      const int t = i / (2 * L::NP), c = i % (2 * L::NP);
+    for (int i = tid; i < SS_K * 2 * NP; i += 64 * L::WAVES) {
+      const int t = i / (2 * NP), c = i % (2 * NP);
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += sBC[w][t][c];
+      for (int w = 0; w < L::GPB; ++w) s += sBC[w][t][c];
       if (t0 + t < pc.t1)
-        p.part_bc[(((long)(tile % p.tiles_g) * p.tokens + pc.b * a.T + t0 + t) * a.G + grp) *
-                      (2 * L::NP) + c] = s;
+        p.part_bc[(((long)(tile - grp * btiles_g) * p.tokens + pc.b * a.T + t0 + t) * a.G + grp) *
+                      (2 * NP) + c] = s;
     }
-    // no wave writes sS or sBC again before the next barrier
+    // sD, sU and sG are written next by the wave that read them here; sS and sBC after a barrier
   }
   if (live) {
     if (pc.idx == 0 && a.dh0)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n0 + i < N) a.dh0[((long)pc.seq * D + dl) * N + n0 + i] = carry[i];
-    *reinterpret_cast<float4*>(p.part_a + ((long)pi * D + dl) * L::NP + n0) =
-        make_float4(dA[0], dA[1], dA[2], dA[3]);
+      for (int n = 0; n < 8; ++n)
+        if (n0 + n < N) a.dh0[((long)pc.seq * D + dl) * N + n0 + n] = carry[n];
+    store4<8>(p.part_a + ((long)pi * D + dl) * NP + n0, dA);
   }
-  // dD and the bias: sum over the block's 16 token rows
+  // dD and the bias: sum over the waves of a channel group
   __syncthreads();
-  float* s0 = &sS[0][0][0];
+  sS[part][0][0][col] = accD;
+  sS[part][1][0][col] = accB;
+  __syncthreads();
+  if (part == 0 && live) {
+    float sd = 0.f, sb = 0.f;
 #pragma unroll
-  for (int e = 0; e < L::EPT; ++e) {
-    s0[tt * L::CT + tc + e] = accD[e];
-    s0[(SS_K + tt) * L::CT + tc + e] = accB[e];
-  }
-  __syncthreads();
-  for (int i = tid; i < 2 * L::CT; i += SS_NT) {
-    const int w = i / L::CT, c = i % L::CT;
-    float s = 0.f;
-    for (int t = 0; t < SS_K; ++t) s += s0[(w * SS_K + t) * L::CT + c];
-    if (c < nch) p.part_d[((long)pi * 2 + w) * D + d0 + c] = s;
+    for (int w = 0; w < L::NW; ++w) {
+      sd += sS[w][0][0][col];
+      sb += sS[w][1][0][col];
+    }
+    p.part_d[(long)pi * 2 * D + dl] = sd;
+    p.part_d[((long)pi * 2 + 1) * D + dl] = sb;
   }
 }
 
@@ -506,10 +554,10 @@ __global__ __launch_bounds__(SS_NT, 2) void scan_bwd_kernel(ScanParams p) {
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bwd_bc_kernel(ScanParams p, int NP) {
   const long total = p.tokens * p.a.G * 2 * NP;
-  const int N = (int)p.a.N;
+  const int N = (int)p.a.N, tiles = p.btiles / (int)p.a.G;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     float s = 0.f;
-    for (int t = 0; t < p.tiles_g; ++t) s += p.part_bc[t * total + i];
+    for (int t = 0; t < tiles; ++t) s += p.part_bc[t * total + i];
     const int c = (int)(i % (2 * NP)), n = c % NP;
     if (n < N) ((T*)(c < NP ? p.a.dB : p.a.dC))[(i / (2 * NP)) * N + n] = from_f32<T>(s);
   }
@@ -534,53 +582,79 @@ __global__ __launch_bounds__(256) void scan_bwd_a_kernel(ScanParams p, int NP) {
   }
 }
 
-template <typename T, int LQ>
-hipError_t scan_fwd(const ScanParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.npieces * p.ntiles));
-  if (p.multi) {
-    hipLaunchKernelGGL((scan_kernel<T, LQ, 0>), grid, dim3(SS_NT), 0, st, p);
-    if (hipError_t e = hipGetLastError()) return e;
-  }
-  hipLaunchKernelGGL((scan_kernel<T, LQ, 1>), grid, dim3(SS_NT), 0, st, p);
+unsigned grid_of(long threads) {
+  return (unsigned)std::min<long>((threads + 255) / 256, 1L << 20);
+}
+
+template <int NP, bool REV>
+hipError_t scan_fold(const ScanParams& p, hipStream_t st) {
+  const int nb = (int)((p.a.D * (NP / 4) + 255) / 256);
+  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.npieces)), dim3(256), 0,
+                     st, p, nb);
   return hipGetLastError();
 }
 
-template <typename T, int LQ>
-hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.npieces * p.ntiles));
-  if (p.multi) {
-    hipLaunchKernelGGL((scan_kernel<T, LQ, 2>), grid, dim3(SS_NT), 0, st, p);
+template <typename T, int NP>
+hipError_t scan_fwd(const ScanParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.npieces * p.ntiles + 3) / 4));
+  const long nbc = (p.tokens * p.a.G + 1) * 2 * NP;
+  if (p.tokens > 0) {
+    hipLaunchKernelGGL((scan_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
     if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (p.multi) {
+    hipLaunchKernelGGL((scan_kernel<T, NP, 0>), grid, dim3(256), 0, st, p);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = scan_fold<NP, false>(p, st)) return e;
+  }
+  hipLaunchKernelGGL((scan_kernel<T, NP, 1>), grid, dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+template <typename T, int NP>
+hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
+  if (p.multi) {
+    const dim3 grid((unsigned)((p.npieces * p.ntiles + 3) / 4));
+    hipLaunchKernelGGL((scan_kernel<T, NP, 2>), grid, dim3(256), 0, st, p);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = scan_fold<NP, true>(p, st)) return e;
   }
   if (p.npieces > 0) {
-    hipLaunchKernelGGL((scan_bwd_kernel<T, LQ>), grid, dim3(SS_NT), 0, st, p);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, NP>), dim3((unsigned)(p.npieces * p.btiles)),
+                       dim3(64 * Bwd<NP>::WAVES), 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  constexpr int NP = Lay<LQ>::NP;
   const long nbc = p.tokens * p.a.G * 2 * NP, na = p.a.D * (NP + 2);
   if (nbc > 0) {
-    hipLaunchKernelGGL((scan_bwd_bc_kernel<T>), dim3((unsigned)std::min<long>((nbc + 255) / 256, 1L << 20)),
-                       dim3(256), 0, st, p, NP);
+    hipLaunchKernelGGL((scan_bwd_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  hipLaunchKernelGGL(scan_bwd_a_kernel, dim3((unsigned)std::min<long>((na + 255) / 256, 1L << 20)),
-                     dim3(256), 0, st, p, NP);
+  hipLaunchKernelGGL(scan_bwd_a_kernel, dim3(grid_of(na)), dim3(256), 0, st, p, NP);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t scan_any(const ScanParams& p, bool backward, hipStream_t st) {
   switch (scan_state_pad((int)p.a.N)) {
-    case 16: return backward ? scan_bwd<T, 4>(p, st) : scan_fwd<T, 4>(p, st);
-    case 32: return backward ? scan_bwd<T, 8>(p, st) : scan_fwd<T, 8>(p, st);
-    default: return backward ? scan_bwd<T, 16>(p, st) : scan_fwd<T, 16>(p, st);
+    case 8: return backward ? scan_bwd<T, 8>(p, st) : scan_fwd<T, 8>(p, st);
+    case 16: return backward ? scan_bwd<T, 16>(p, st) : scan_fwd<T, 16>(p, st);
+    case 32: return backward ? scan_bwd<T, 32>(p, st) : scan_fwd<T, 32>(p, st);
+    default: return backward ? scan_bwd<T, 64>(p, st) : scan_fwd<T, 64>(p, st);
   }
 }
 
 }  // namespace
 
-int scan_state_pad(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
-int scan_tile_channels(int N) { return 2048 / scan_state_pad(N); }
+int scan_state_pad(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+int scan_chunk() { return SS_K; }
+int scan_bwd_channels(int N) {
+  switch (scan_state_pad(N)) {
+    case 8: return Bwd<8>::CT;
+    case 16: return Bwd<16>::CT;
+    case 32: return Bwd<32>::CT;
+    default: return Bwd<64>::CT;
+  }
+}
 
 hipError_t run_selective_scan(const ScanParams& p, bool backward, hipStream_t st) {
   if (p.a.D == 0 || (p.npieces == 0 && !backward)) return hipSuccess;

@@ -89,6 +89,7 @@ _SSM_SIGS = {
     "tops_gla_selective_scan_bwd": [_S, _P],
     "tops_gla_selective_scan_bwd_ws_bytes": [_I64] * 5,
     "tops_gla_selective_scan_piece": [_I64] * 4,
+    "tops_gla_selective_scan_chunk": [_I64],
     "tops_gla_selective_scan_step": [_S, _P],
     "tops_gla_causal_conv_fwd": [_S, _P],
     "tops_gla_causal_conv_bwd": [_S, _P],
@@ -105,6 +106,7 @@ _RESTYPE = {"tops_gla_chunk_ws_bytes": ctypes.c_int64, "tops_gla_kernel_ms": cty
             "tops_gla_short_conv_ws_bytes": ctypes.c_int64,
             "tops_gla_selective_scan_bwd_ws_bytes": ctypes.c_int64,
             "tops_gla_selective_scan_piece": ctypes.c_int64,
+            "tops_gla_selective_scan_chunk": ctypes.c_int64,
             "tops_gla_causal_conv_bwd_ws_bytes": ctypes.c_int64,
             "tops_gla_qk_norm_rope_ws_bytes": ctypes.c_int64}
 

@@ -55,6 +55,33 @@ def offsets(cu_seqlens, B, T):
     return cu
 
 
+_tables: dict = {}
+_held: list = []
+
+
+def device_table(key, make, device):
+    """``make()`` -> (int32 values, anything else) with the values as a device tensor, kept by its
+    key, device and stream: one stream writes, reads and frees a table, in this order. A table
+    that a graph captures is kept for good, as the graph's replays read it."""
+    key = (key, str(device), torch.cuda.current_stream(device).cuda_stream)
+    capturing = torch.cuda.is_current_stream_capturing()
+    hit = _tables.get(key)
+    if hit is None and capturing:
+        # a capture runs on its own stream, and cannot upload a table of its own
+        hit = next((v for k, v in _tables.items() if k[:2] == key[:2]), None)
+        if hit is None:
+            raise RuntimeError("packed sequences in a graph capture: run the call once with the "
+                               "same cu_seqlens before the capture")
+    if hit is None:
+        values, rest = make()
+        if len(_tables) > 64:
+            _tables.clear()
+        hit = _tables[key] = (torch.tensor(values, dtype=torch.int32, device=device), rest)
+    if capturing and not any(h is hit for h in _held):
+        _held.append(hit)
+    return hit
+
+
 def slot_args(idx, batch, device_of):
     """(address, whether int64) of the state slots of a batch."""
     if idx is None:

@@ -10,26 +10,15 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
+from ._common import (address, device_table, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
                       slot_args, strides)
 
 _ARGS = struct.Struct("=26q")
 _STEP = struct.Struct("=16q")
 
-_cu_cache: dict = {}
-
-
 def _cu_tensor(cu, device):
-    """The offsets as a device int32 array (cached by their values)."""
-    if cu is None:
-        return None
-    key = (tuple(cu), str(device))
-    hit = _cu_cache.get(key)
-    if hit is None:
-        if len(_cu_cache) > 64:
-            _cu_cache.clear()
-        hit = _cu_cache[key] = torch.tensor(cu, dtype=torch.int32, device=device)
-    return hit
+    """The offsets as a device int32 array."""
+    return None if cu is None else device_table(tuple(cu), lambda: (cu, None), device)[0]
 
 
 def _silu(activation):

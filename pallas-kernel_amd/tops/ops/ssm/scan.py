@@ -9,50 +9,46 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
+from ._common import (address, device_table, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
                       slot_args, strides)
 
-_ARGS = struct.Struct("=52q")
+_ARGS = struct.Struct("=53q")
 _STEP = struct.Struct("=27q")
-_CHUNK = 16   # tokens between the states kept for the backward
 
 
 class _Pieces:
     """How the sequences of a call are cut into pieces that run in parallel."""
 
-    _cache: dict = {}
-
     def __init__(self, B, T, D, N, G, cu, device):
         lib = _lib.load()
+        chunk = int(lib.tops_gla_selective_scan_chunk(N))
         self.piece = int(lib.tops_gla_selective_scan_piece(B * T, D, N, G))
         self.table = None
         if cu is None:
             per = max(1, -(-T // self.piece))
             self.nseq, self.nsegs = B, B * per
-            self.chunks, self.multi = B * -(-T // _CHUNK), per > 1
+            self.chunks, self.multi = B * -(-T // chunk), per > 1
             return
         self.nseq = len(cu) - 1
-        key = (tuple(cu), self.piece, str(device))
-        hit = _Pieces._cache.get(key)
-        if hit is None:
+
+        def make():
             segs, c0, multi = [], 0, False
             for s, (a, b) in enumerate(zip(cu, cu[1:])):
                 n = max(1, -(-(b - a) // self.piece))
                 multi |= n > 1
                 for i in range(n):
                     t0 = a + i * self.piece
-                    segs += [s, t0, min(b, t0 + self.piece), i, n, c0 + i * self.piece // _CHUNK,
+                    segs += [s, t0, min(b, t0 + self.piece), i, n, c0 + i * self.piece // chunk,
                              0, 0]
-                c0 += -(-(b - a) // _CHUNK)
-            hit = (torch.tensor(segs, dtype=torch.int32, device=device), len(segs) // 8, c0, multi)
-            if len(_Pieces._cache) > 64:
-                _Pieces._cache.clear()
-            _Pieces._cache[key] = hit
-        self.table, self.nsegs, self.chunks, self.multi = hit
+                c0 += -(-(b - a) // chunk)
+            return segs, (len(segs) // 8, c0, multi)
+
+        self.table, (self.nsegs, self.chunks, self.multi) = device_table(
+            (tuple(cu), self.piece, chunk), make, device)
 
 
 def _pad(N):
-    return 16 if N <= 16 else 32 if N <= 32 else 64
+    return 8 if N <= 8 else 16 if N <= 16 else 32 if N <= 32 else 64
 
 
 def _groups(t, N):
@@ -60,7 +56,7 @@ def _groups(t, N):
     return t if t.dim() == 4 else t.unsqueeze(2)
 
 
-def _pack(x, y, ht, chunk_h, ws, pc, shape, softplus, dt, bwd=None):
+def _pack(x, y, ht, chunk_h, ws, bc, pc, shape, softplus, dt, bwd=None):
     Bt, T, D, N, G = shape
     u, delta, A, B, C, Dskip, z, bias, h0 = x
     if bwd is None:
@@ -69,7 +65,7 @@ def _pack(x, y, ht, chunk_h, ws, pc, shape, softplus, dt, bwd=None):
     return _ARGS.pack(
         address(u), address(delta), address(z), address(B), address(C), address(A),
         address(Dskip), address(bias), address(h0), address(y), address(ht), address(chunk_h),
-        address(ph), address(pd), address(pc.table),
+        address(ph), address(pd), address(bc), address(pc.table),
         pc.nsegs, pc.nseq, pc.piece, Bt, T, D, N, G,
         *strides(u, 0, 1), *strides(delta, 0, 1), *strides(z, 0, 1), *strides(B, 0, 1, 2),
         *strides(C, 0, 1, 2), int(softplus), dtype_code(dt), *bwd)
@@ -98,18 +94,20 @@ def _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu, keep):
     chunk_h = (torch.empty(pc.chunks, Dn, _pad(N), dtype=torch.float32, device=dev)
                if keep else None)
     ws = _piece_states(pc, Dn, N, dev)
+    bc = torch.empty(Bt * T * G + 1, 2, _pad(N), dtype=torch.float32, device=dev)
     call("tops_gla_selective_scan_fwd",
-         _pack(x, y, ht, chunk_h, ws, pc, (Bt, T, Dn, N, G), softplus, dt), stream_of(dev))
-    return y.to(u.dtype), ht, x, chunk_h, pc
+         _pack(x, y, ht, chunk_h, ws, bc, pc, (Bt, T, Dn, N, G), softplus, dt), stream_of(dev))
+    return y.to(u.dtype), ht, x, chunk_h, bc, pc
 
 
 class _SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu):
         ctx.set_materialize_grads(False)
-        y, ht, x, chunk_h, pc = _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu,
-                                         True)
-        ctx.save_for_backward(*x[:8], chunk_h)
+        y, ht, x, chunk_h, bc, pc = _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht,
+                                             cu, True)
+        ctx.save_for_backward(*x[:3], *x[5:8], chunk_h, bc)
+        ctx.G = x[3].shape[2]
         ctx.like = [None if t is None else (t.dtype, t.shape)
                     for t in (u, delta, A, B, C, D, z, bias, h0)]
         ctx.softplus, ctx.pc = softplus, pc
@@ -118,11 +116,11 @@ class _SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dht):
-        *x, chunk_h = ctx.saved_tensors
-        u, delta, A, B, C, D, z, bias = x
+        u, delta, A, D, z, bias, chunk_h, bc = ctx.saved_tensors
+        x = u, delta, A, None, None, D, z, bias, None
         pc, dev, dt = ctx.pc, u.device, u.dtype
         Bt, T, Dn = u.shape
-        N, G = A.shape[1], B.shape[2]
+        N, G = A.shape[1], ctx.G
         dy = torch.zeros(Bt, T, Dn, dtype=dt, device=dev) if dy is None else rows(dy, dt)
         dht = f32(dht)
 
@@ -141,7 +139,7 @@ class _SelectiveScanFunction(torch.autograd.Function):
         bwd = [address(dy), *strides(dy, 0, 1), *(address(t) for t in (
             dht, du, ddelta, dz, dB, dC, dA, dD, dbias, dh0, ws)), nws]
         call("tops_gla_selective_scan_bwd",
-             _pack((*x, None), None, None, chunk_h, _piece_states(pc, Dn, N, dev), pc,
+             _pack(x, None, None, chunk_h, _piece_states(pc, Dn, N, dev), bc, pc,
                    (Bt, T, Dn, N, G), ctx.softplus, dt, bwd), stream_of(dev))
         grads = (du, ddelta, dA, dB, dC, dD, dz, dbias, dh0)
         return (*(None if g is None or not need else g.reshape(like[1]).to(like[0])
