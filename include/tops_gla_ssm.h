@@ -27,14 +27,16 @@ extern "C" {
  *   h_t[n] = exp(delta'_t A[d,n]) h_{t-1}[n] + delta'_t u_t B_t[g,n]
  *   y_t    = (sum_n C_t[g,n] h_t[n] + Dskip[d] u_t) (* z_t sigmoid(z_t) with z)
  * A sequence is cut into pieces of at most `piece` tokens (a multiple of 16) that run in
- * parallel: piece_h [pieces][D][NP] and piece_dt [pieces][D] hold their own contributions
- * (NP = N rounded up to 8, 16, 32 or 64), not needed when no sequence has two pieces. Fixed length:
- * ceil(T / piece) pieces a sequence (at least one). Packed: `segs` holds, for each of `nsegs`
- * pieces in order, {sequence, first token, end token, its index in the sequence, pieces of the
- * sequence, index of its first chunk, 0, 0}; a sequence of no tokens has one piece.
- * `chunk_h` [chunks][D][NP]: the states entering every chunk of
+ * parallel: piece_h [pieces][NP][D] and piece_dt [pieces][D] hold their own contributions
+ * (NP = N rounded up to 8, 16, 32 or 64), not needed when no sequence has two pieces. Fixed
+ * length: ceil(T / piece) pieces a sequence (at least one). Packed: `segs` holds, for each of
+ * `nsegs` pieces in order, {sequence, first token, end token, its index in the sequence, pieces
+ * of the sequence, index of its first chunk, f, 0}; f of row s is the first piece of sequence s.
+ * A sequence of no tokens has one piece.
+ * `chunk_h` [chunks][NP][D]: the states entering every chunk of
  * tops_gla_selective_scan_chunk(N) tokens of a sequence, kept for the backward (NULL: not kept).
- * `bc` [B * T * G + 1][2][NP]: B and C as the kernels read them, written by the forward.
+ * `bc`: B, C and A as the kernels read them, (B * T * G + 1) * 2 * NP + NP * D floats, written by
+ * the forward.
  * 1 <= N <= 64.
  */
 typedef struct tops_gla_scan_args {

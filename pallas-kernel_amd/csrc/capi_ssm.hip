@@ -85,16 +85,18 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
     return fail(TOPS_GLA_EINVAL, "piece_dt is required with piece_h");
   const int64_t np = tops::scan_state_pad((int)a->N);
   p->tiles_g = (int)tiles_of(a->D, a->G);
-  if ((p->tiles_g * a->G + a->D * np / 1024 + 1) * std::max<int64_t>(p->npieces, 1) > kMax)
+  if (p->tiles_g * a->G * std::max<int64_t>(p->npieces, 1) > kMax ||
+      (a->D * np / 64 + 1) * a->nseq > kMax)
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   p->ntiles = p->tiles_g * (int)a->G;
+  p->at = a->bc + (p->tokens * a->G + 1) * 2 * np;
   p->btiles = (int)(bwd_tiles_of(a->D, a->N, a->G) * a->G);
   if (any_null({a->A})) return fail(TOPS_GLA_EINVAL, "A must not be NULL");
   if (p->tokens > 0 && (any_null({a->u, a->delta}) || (!backward && any_null({a->B, a->C}))))
     return fail(TOPS_GLA_EINVAL, "u, delta, B and C must not be NULL");
   if (!backward) {
     if (p->tokens > 0 && a->y == nullptr) return fail(TOPS_GLA_EINVAL, "y must not be NULL");
-    if (p->tokens > 0 && a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
+    if (a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
     return TOPS_GLA_OK;
   }
   if (p->tokens > 0 && any_null({a->dy, a->du, a->ddelta, a->dB, a->dC, a->chunk_h}))
@@ -106,7 +108,7 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
       tops_gla_selective_scan_bwd_ws_bytes(p->tokens, p->npieces, a->D, a->N, a->G);
   if (need > 0 && (a->ws == nullptr || a->ws_bytes < need))
     return fail(TOPS_GLA_EINVAL, "ws must hold %lld bytes", (long long)need);
-  if (p->tokens > 0 && a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
+  if (a->bc == nullptr) return fail(TOPS_GLA_EINVAL, "bc must not be NULL");
   p->part_bc = (float*)a->ws;
   p->part_a = p->part_bc + p->btiles * p->tokens * 2 * np;
   p->part_d = p->part_a + p->npieces * a->D * np;

@@ -22,6 +22,7 @@ struct ScanParams {
   int pieces;            // pieces of a sequence (fixed length)
   int multi;             // some sequence has more than one piece
   long npieces, tokens;
+  const float* at;       // A log2(e), [NP][D], behind the rows of bc
   float *part_bc, *part_a, *part_d;   // the backward's shares
 };
 int scan_state_pad(int N);       // N rounded up to 8, 16, 32 or 64

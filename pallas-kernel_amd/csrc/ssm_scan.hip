@@ -75,20 +75,16 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // Keeps the compiler from moving LDS reads up, into registers that others need.
 __device__ __forceinline__ void fence() { asm volatile("" ::: "memory"); }
 
-// N consecutive floats at a 16-byte boundary (N a multiple of 4).
+// The N states of a lane's channel, in rows of D channels.
 template <int N>
-__device__ __forceinline__ void load4(const float* p, float (&x)[N]) {
+__device__ __forceinline__ void load_states(const float* p, int D, uint32_t lo, float (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const float4 w = *reinterpret_cast<const float4*>(p + i);
-    x[i] = w.x, x[i + 1] = w.y, x[i + 2] = w.z, x[i + 3] = w.w;
-  }
+  for (int i = 0; i < N; ++i, p += D) x[i] = p[lo];
 }
 template <int N>
-__device__ __forceinline__ void store4(float* p, const float (&x)[N]) {
+__device__ __forceinline__ void store_states(float* p, int D, uint32_t lo, const float (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 4)
-    *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  for (int i = 0; i < N; ++i, p += D) p[lo] = x[i];
 }
 
 // The lane's element of N rows from `t` on, the last one of the piece again past its end (t < t1).
@@ -115,17 +111,23 @@ __device__ __forceinline__ cfloat* row_after(const float* p, float (&x)[N]) {
   return (cfloat*)(uintptr_t)p;
 }
 
+__device__ __forceinline__ void load_row(cfloat* p, float (&x)[8]) {
+#pragma unroll
+  for (int n = 0; n < 8; ++n) x[n] = p[n];
+}
+
 // B and C as float32 rows [token][group][2][NP], zeros past N and in one more row, which stands
-// for the tokens past a piece's end.
+// for the tokens past a piece's end; then A log2(e) as rows of D channels [NP][D].
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(ScanParams p, int NP) {
-  const long rows = p.tokens * p.a.G, total = (rows + 1) * 2 * NP;
+  const long rows = p.tokens * p.a.G, nbc = (rows + 1) * 2 * NP, total = nbc + p.a.D * NP;
   const int N = (int)p.a.N, G = (int)p.a.G;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     const int n = (int)(i % NP), w = (int)(i / NP % 2);
     const long r = i / (2 * NP), tok = r / G, g = r - tok * G;
-    if (r == rows) {
-      p.a.bc[i] = 0.f;
+    if (r >= rows) {
+      const long j = i - nbc, m = j >= 0 ? j / p.a.D : N;
+      p.a.bc[i] = m < N ? scaled_a(p.a.A[(j - m * p.a.D) * N + m]) : 0.f;
       continue;
     }
     const long b = tok / p.a.T, t = tok - b * p.a.T;
@@ -158,13 +160,11 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
 
   float A[NP], h[NP];
 #pragma unroll
-  for (int n = 0; n < NP; ++n) {
-    A[n] = n < N ? scaled_a(a.A[dl * N + n]) : 0.f;
-    h[n] = 0.f;
-  }
+  for (int n = 0; n < NP; ++n) h[n] = 0.f;
+  load_states<NP>(p.at + tl.d0, D, lo, A);
   if (MODE == 1) {
     if (p.multi) {
-      load4<NP>(a.piece_h + ((long)pi * D + dl) * NP, h);
+      load_states<NP>(a.piece_h + (long)pi * NP * D + tl.d0, D, lo, h);
     } else if (a.h0) {
 #pragma unroll
       for (int n = 0; n < NP; ++n)
@@ -219,12 +219,14 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
       if (t0 + i >= pc.t1) d[i] = u[i] = 0.f;
     if (it + 1 < nt) load(t0 + step * SS_K);
     if (MODE == 1 && a.chunk_h && live)
-      store4<NP>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * NP, h);
+      store_states<NP>(a.chunk_h + (long)(pc.c0 + k) * NP * D + tl.d0, D, lo, h);
     const float* rp = bc + t0 * bc_st;
+    float ahead[2] = {0.f, 0.f};
     if (MODE == 2) rp = t0 + SS_K - 1 < pc.t1 ? rp + (SS_K - 1) * bc_st : bc_end;
 #pragma unroll
     for (int j = 0; j < SS_K; ++j) {
       const int i = MODE == 2 ? SS_K - 1 - j : j;
+      asm volatile("" : : "s"(ahead[0]), "s"(ahead[1]));
       cfloat* row = row_after(rp, h);
       if (MODE == 2)
         rp = t0 + i - 1 < pc.t1 ? bc + (t0 + i - 1) * bc_st : bc_end;
@@ -240,6 +242,13 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
         } else {
           h[n] = fmaf(ex, h[n], x * row[n]);
           if (MODE == 1) acc[n & 1] = fmaf(h[n], row[NP + n], acc[n & 1]);
+        }
+        if (n == 0 && j + 1 < SS_K) {
+          // this token's rows are there: fetch the next one's into the scalar cache
+          const float* np = rp;
+          asm volatile("" : "+s"(np), "+v"(h[0]));
+          ahead[0] = *(cfloat*)(uintptr_t)np;
+          if (MODE == 1) ahead[1] = *(cfloat*)(uintptr_t)(np + NP);
         }
       }
       y[i] = acc[0] + acc[1];
@@ -266,59 +275,68 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
       for (int n = 0; n < NP; ++n)
         if (n < N) a.ht[((long)pc.seq * D + dl) * N + n] = h[n];
   } else {
-    store4<NP>(a.piece_h + ((long)pi * D + dl) * NP, h);
+    store_states<NP>(a.piece_h + (long)pi * NP * D + tl.d0, D, lo, h);
     a.piece_dt[(long)pi * D + dl] = dsum;
   }
 }
 
-// The pieces' entry states in the place of their own ones, a thread for four states of a channel
-// of a sequence: h <- exp(A S_j) h + L_j from h0 on, or backward from dht on with REV.
+// The pieces' entry states in the place of their own ones: h <- exp(A S_j) h + L_j over a
+// sequence's pieces from h0 on, or backward from dht on with REV. A thread folds a run of the
+// pieces for a state of a channel, 4 threads share a sequence's runs: each finds its run's own L
+// and S, then its entry from those of the runs before, then its pieces' entries.
+constexpr int FOLD_R = 4, FOLD_U = 8;
 template <int NP, bool REV>
 __global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
+  __shared__ float sL[FOLD_R][64], sS[FOLD_R][64];
   const tops_gla_scan_args& a = p.a;
-  const int pi = blockIdx.x / nb;
-  const Piece pc = piece_of(p, pi);
-  if (pc.idx != 0) return;
-  const int q = (blockIdx.x - pi * nb) * 256 + threadIdx.x;
-  const int D = (int)a.D, N = (int)a.N, d = q / (NP / 4), n0 = q % (NP / 4) * 4;
-  if (d >= D) return;
+  const int seq = blockIdx.x / nb;
+  const long pi = a.segs ? a.segs[8L * seq + 6] : (long)seq * p.pieces;
+  const int np = piece_of(p, (int)pi).np, m = (np + FOLD_R - 1) / FOLD_R;
+  const int run = threadIdx.x / 64, c = threadIdx.x % 64;
+  const int D = (int)a.D, N = (int)a.N;
+  const long q = (long)(blockIdx.x - seq * nb) * 64 + c, nd = (long)D * NP;
+  const bool live = q < nd;
+  const int n = live ? (int)(q / D) : 0, d = live ? (int)(q - (long)n * D) : 0;
+  const int j0 = min(np, run * m), j1 = min(np, j0 + m);
   const float* init = REV ? a.dht : a.h0;
-  float A[4], h[4];
+  const float A = p.at[(long)n * D + d];
+  const long first = pi + (REV ? np - 1 : 0);
+  const long hs = (REV ? -1L : 1L) * nd, ss = (REV ? -1L : 1L) * D;
+  float* H = a.piece_h + first * nd + (long)n * D + d;
+  const float* S = a.piece_dt + first * D + d;
+  float h = 0.f, s = 0.f;
+  // h through the pieces j .. end - 1, each piece's entry state written with `put`; the last piece
+  // has no own state
+  auto walk = [&](int j, int end, bool put) {
+    for (; j < end; j += FOLD_U) {
+      float l[FOLD_U], dt[FOLD_U];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = n0 + i < N;
-    A[i] = in ? scaled_a(a.A[(long)d * N + n0 + i]) : 0.f;
-    h[i] = in && init ? init[((long)pc.seq * D + d) * N + n0 + i] : 0.f;
-  }
-  constexpr int U = 8;
-  const long hs = (REV ? -1L : 1L) * D * NP, ss = (REV ? -1L : 1L) * D;
-  const long j0 = pi + (REV ? pc.np - 1 : 0);
-  float* H = a.piece_h + (j0 * D + d) * NP + n0;
-  const float* S = a.piece_dt + j0 * D + d;
-  for (int j = 0; j < pc.np; j += U) {
-    float4 l[U];
-    float s[U];
-    const int m = min(U, pc.np - 1 - j);   // the last piece's own state is not there
+      for (int i = 0; i < FOLD_U; ++i) {
+        const int at = max(0, min(j + i, np - 2));
+        l[i] = H[at * hs];
+        dt[i] = S[at * ss];
+      }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = max(0, min(i, m - 1));
-      l[i] = *reinterpret_cast<const float4*>(H + c * hs);
-      s[i] = S[c * ss];
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (j + i < pc.np) {
-        *reinterpret_cast<float4*>(H + i * hs) = make_float4(h[0], h[1], h[2], h[3]);
-        const float lv[4] = {l[i].x, l[i].y, l[i].z, l[i].w};
-        if (i < m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)   // a zero state stays zero under a decay that overflows
-            h[e] = h[e] == 0.f ? lv[e] : fmaf(exp2_hw(A[e] * s[i]), h[e], lv[e]);
+      for (int i = 0; i < FOLD_U; ++i) {
+        if (j + i >= end) break;
+        if (put) H[(j + i) * hs] = h;
+        if (j + i < np - 1) {   // a zero state stays zero under a decay that overflows
+          h = h == 0.f ? l[i] : fmaf(exp2_hw(A * dt[i]), h, l[i]);
+          s += dt[i];
+        }
       }
     }
-    H += U * hs;
-    S += U * ss;
+  };
+  if (run < FOLD_R - 1) walk(j0, j1, false);
+  sL[run][c] = h;
+  sS[run][c] = s;
+  __syncthreads();
+  h = n < N && init ? init[((long)seq * D + d) * N + n] : 0.f;
+  for (int r = 0; r < run; ++r) {
+    const float l = sL[r][c];
+    h = h == 0.f ? l : fmaf(exp2_hw(A * sS[r][c]), h, l);
   }
+  if (live) walk(j0, j1, true);
 }
 
 // ---------------------------------------------------------------------------
@@ -390,13 +408,11 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
   const int n0 = 8 * part, col = 64 * cg + lane;
   float A[8], carry[8], dA[8];
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    A[n] = live && n0 + n < N ? scaled_a(a.A[dl * N + n0 + n]) : 0.f;
-    carry[n] = dA[n] = 0.f;
-  }
+  for (int n = 0; n < 8; ++n) carry[n] = dA[n] = 0.f;
+  load_states<8>(p.at + (long)n0 * D + d0, D, lo, A);
   if (live) {
     if (p.multi) {
-      load4<8>(a.piece_h + ((long)pi * D + dl) * NP + n0, carry);
+      load_states<8>(a.piece_h + ((long)pi * NP + n0) * D + d0, D, lo, carry);
     } else if (a.dht) {
 #pragma unroll
       for (int n = 0; n < 8; ++n)
@@ -423,7 +439,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
     load_rows<T, L::TPW>(gd, a.delta_st, t0, pc.t1, lo, rd);
     load_rows<T, L::TPW>(gy, a.dy_st, t0, pc.t1, lo, ry);
     if (has_z) load_rows<T, L::TPW>(gz, a.z_st, t0, pc.t1, lo, rz);
-    load4<8>(a.chunk_h + ((long)(pc.c0 + k) * D + dl) * NP + n0, rh);
+    load_states<8>(a.chunk_h + ((long)(pc.c0 + k) * NP + n0) * D + d0, D, lo, rh);
   };
   const int nt = (pc.t1 - pc.t0 + SS_K - 1) / SS_K;
   if (nt > 0) load(nt - 1);
@@ -447,39 +463,57 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
     float av[SS_K][8], hv[SS_K][8], hin[8];
 #pragma unroll
     for (int n = 0; n < 8; ++n) hin[n] = live ? rh[n] : 0.f;
+    const float* rp = bc + t0 * bc_st;
+    float nb[8], nc[8];
+    load_row(row_after(rp, hin), nb);
     __syncthreads();
     if (k > 0) load(k - 1);
 
-    const float* rp = bc + t0 * bc_st;
 #pragma unroll
     for (int t = 0; t < SS_K; ++t) {
-      cfloat* row = row_after(rp, t ? hv[t - 1] : hin);
-      if (t < SS_K - 1) rp = t0 + t + 1 < pc.t1 ? rp + bc_st : bc_end;
+      float rb[8];   // this token's B; the next one's is on its way while this one is computed
+#pragma unroll
+      for (int n = 0; n < 8; ++n) rb[n] = nb[n];
+      if (t < SS_K - 1) {
+        rp = t0 + t + 1 < pc.t1 ? rp + bc_st : bc_end;
+        load_row(row_after(rp, t ? hv[t - 1] : hin), nb);
+      } else {
+        cfloat* row = row_after(rp, hv[t - 1]);
+        load_row(row, nb);
+        load_row(row + NP, nc);
+      }
       const float d = sD[t][col], x = d * sU[t][col];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         av[t][n] = exp2_hw(A[n] * d);
-        hv[t][n] = fmaf(av[t][n], t ? hv[t - 1][n] : hin[n], x * row[n]);
+        hv[t][n] = fmaf(av[t][n], t ? hv[t - 1][n] : hin[n], x * rb[n]);
       }
     }
     fence();
 #pragma unroll
     for (int t = SS_K - 1; t >= 0; --t) {
-      cfloat* row = row_after(rp, carry);
-      rp = t0 + t - 1 < pc.t1 ? bc + (t0 + t - 1) * bc_st : bc_end;
+      float rb[8], rc[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) rb[n] = nb[n], rc[n] = nc[n];
+      if (t > 0) {
+        rp = t0 + t - 1 < pc.t1 ? bc + (t0 + t - 1) * bc_st : bc_end;
+        cfloat* row = row_after(rp, carry);
+        load_row(row, nb);
+        load_row(row + NP, nc);
+      }
       const float d = sD[t][col], x = d * sU[t][col], dy = sG[t][col];
       float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const float g = fmaf(dy, row[NP + n], carry[n]);
+        const float g = fmaf(dy, rc[n], carry[n]);
         const float hp = t ? hv[t - 1][n] : hin[n];
         vb[n] = g * x;
         vc[n] = dy * hv[t][n];
-        s1 = fmaf(g, row[n], s1);
+        s1 = fmaf(g, rb[n], s1);
         carry[n] = av[t][n] * g;
         const float gp = carry[n] * hp;
         s2 = fmaf(gp, A[n], s2);
-        s3 = fmaf(hv[t][n], row[NP + n], s3);
+        s3 = fmaf(hv[t][n], rc[n], s3);
         dA[n] = fmaf(gp, d, dA[n]);
       }
       sS[part][0][t][col] = s1;
@@ -531,7 +565,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
 #pragma unroll
       for (int n = 0; n < 8; ++n)
         if (n0 + n < N) a.dh0[((long)pc.seq * D + dl) * N + n0 + n] = carry[n];
-    store4<8>(p.part_a + ((long)pi * D + dl) * NP + n0, dA);
+    store_states<8>(p.part_a + ((long)pi * NP + n0) * D + d0, D, lo, dA);
   }
   // dD and the bias: sum over the waves of a channel group
   __syncthreads();
@@ -557,28 +591,39 @@ __global__ __launch_bounds__(256) void scan_bwd_bc_kernel(ScanParams p, int NP) 
   const int N = (int)p.a.N, tiles = p.btiles / (int)p.a.G;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     float s = 0.f;
+#pragma unroll 8
     for (int t = 0; t < tiles; ++t) s += p.part_bc[t * total + i];
     const int c = (int)(i % (2 * NP)), n = c % NP;
     if (n < N) ((T*)(c < NP ? p.a.dB : p.a.dC))[(i / (2 * NP)) * N + n] = from_f32<T>(s);
   }
 }
 
-// dA, dD, dbias from the pieces' shares.
+// dA, dD, dbias from the pieces' shares, 8 threads a column.
 __global__ __launch_bounds__(256) void scan_bwd_a_kernel(ScanParams p, int NP) {
-  const long D = p.a.D, na = D * NP, total = na + 2 * D;
-  const int N = (int)p.a.N;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
-    float s = 0.f;
-    if (i < na) {
-      for (long j = 0; j < p.npieces; ++j) s += p.part_a[j * na + i];
-      const long d = i / NP, n = i % NP;
-      if (n < N) p.a.dA[d * N + n] = s;
-    } else {
-      const long r = i - na;
-      for (long j = 0; j < p.npieces; ++j) s += p.part_d[j * 2 * D + r];
-      float* out = r < D ? p.a.dD : p.a.dbias;
-      if (out) out[r % D] = s;
-    }
+  __shared__ float red[8][32];
+  const long D = p.a.D, na = D * NP;
+  const int N = (int)p.a.N, row = threadIdx.x / 32, c = threadIdx.x % 32;
+  const long i = blockIdx.x * 32L + c;
+  const bool isa = i < na, in = i < na + 2 * D;
+  const float* src = isa ? p.part_a + i : p.part_d + (i - na);
+  const long st = isa ? na : 2 * D;
+  float s = 0.f;
+  if (in)
+#pragma unroll 8
+    for (long j = row; j < p.npieces; j += 8) s += src[j * st];
+  red[row][c] = s;
+  __syncthreads();
+  if (row || !in) return;
+  s = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s += red[r][c];
+  if (isa) {
+    const long n = i / D, d = i - n * D;
+    if (n < N) p.a.dA[d * N + n] = s;
+  } else {
+    const long r = i - na;
+    float* out = r < D ? p.a.dD : p.a.dbias;
+    if (out) out[r % D] = s;
   }
 }
 
@@ -588,8 +633,8 @@ unsigned grid_of(long threads) {
 
 template <int NP, bool REV>
 hipError_t scan_fold(const ScanParams& p, hipStream_t st) {
-  const int nb = (int)((p.a.D * (NP / 4) + 255) / 256);
-  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.npieces)), dim3(256), 0,
+  const int nb = (int)((p.a.D * NP + 63) / 64);
+  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.a.nseq)), dim3(256), 0,
                      st, p, nb);
   return hipGetLastError();
 }
@@ -597,11 +642,9 @@ hipError_t scan_fold(const ScanParams& p, hipStream_t st) {
 template <typename T, int NP>
 hipError_t scan_fwd(const ScanParams& p, hipStream_t st) {
   const dim3 grid((unsigned)((p.npieces * p.ntiles + 3) / 4));
-  const long nbc = (p.tokens * p.a.G + 1) * 2 * NP;
-  if (p.tokens > 0) {
-    hipLaunchKernelGGL((scan_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
-    if (hipError_t e = hipGetLastError()) return e;
-  }
+  const long nbc = (p.tokens * p.a.G + 1) * 2 * NP + p.a.D * NP;
+  hipLaunchKernelGGL((scan_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
+  if (hipError_t e = hipGetLastError()) return e;
   if (p.multi) {
     hipLaunchKernelGGL((scan_kernel<T, NP, 0>), grid, dim3(256), 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
@@ -629,7 +672,7 @@ hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
     hipLaunchKernelGGL((scan_bwd_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  hipLaunchKernelGGL(scan_bwd_a_kernel, dim3(grid_of(na)), dim3(256), 0, st, p, NP);
+  hipLaunchKernelGGL(scan_bwd_a_kernel, dim3((unsigned)((na + 31) / 32)), dim3(256), 0, st, p, NP);
   return hipGetLastError();
 }
 

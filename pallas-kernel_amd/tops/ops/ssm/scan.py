@@ -32,15 +32,18 @@ class _Pieces:
         self.nseq = len(cu) - 1
 
         def make():
-            segs, c0, multi = [], 0, False
+            segs, first, c0, multi = [], [], 0, False
             for s, (a, b) in enumerate(zip(cu, cu[1:])):
                 n = max(1, -(-(b - a) // self.piece))
                 multi |= n > 1
+                first.append(len(segs) // 8)
                 for i in range(n):
                     t0 = a + i * self.piece
                     segs += [s, t0, min(b, t0 + self.piece), i, n, c0 + i * self.piece // chunk,
                              0, 0]
                 c0 += -(-(b - a) // chunk)
+            for s, i in enumerate(first):
+                segs[8 * s + 6] = i
             return segs, (len(segs) // 8, c0, multi)
 
         self.table, (self.nsegs, self.chunks, self.multi) = device_table(
@@ -75,7 +78,7 @@ def _piece_states(pc, D, N, dev):
     """Workspaces of the pieces' own contributions, where a sequence has several pieces."""
     if not pc.multi:
         return None, None
-    return (torch.empty(pc.nsegs, D, _pad(N), dtype=torch.float32, device=dev),
+    return (torch.empty(pc.nsegs, _pad(N), D, dtype=torch.float32, device=dev),
             torch.empty(pc.nsegs, D, dtype=torch.float32, device=dev))
 
 
@@ -91,10 +94,10 @@ def _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu, keep):
     pc = _Pieces(Bt, T, Dn, N, G, cu, dev)
     y = torch.empty(Bt, T, Dn, dtype=dt, device=dev)
     ht = torch.empty(pc.nseq, Dn, N, dtype=torch.float32, device=dev) if want_ht else None
-    chunk_h = (torch.empty(pc.chunks, Dn, _pad(N), dtype=torch.float32, device=dev)
+    chunk_h = (torch.empty(pc.chunks, _pad(N), Dn, dtype=torch.float32, device=dev)
                if keep else None)
     ws = _piece_states(pc, Dn, N, dev)
-    bc = torch.empty(Bt * T * G + 1, 2, _pad(N), dtype=torch.float32, device=dev)
+    bc = torch.empty(((Bt * T * G + 1) * 2 + Dn) * _pad(N), dtype=torch.float32, device=dev)
     call("tops_gla_selective_scan_fwd",
          _pack(x, y, ht, chunk_h, ws, bc, pc, (Bt, T, Dn, N, G), softplus, dt), stream_of(dev))
     return y.to(u.dtype), ht, x, chunk_h, bc, pc
