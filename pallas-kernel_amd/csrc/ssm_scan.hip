@@ -111,9 +111,27 @@ __device__ __forceinline__ cfloat* row_after(const float* p, float (&x)[N]) {
   return (cfloat*)(uintptr_t)p;
 }
 
-__device__ __forceinline__ void load_row(cfloat* p, float (&x)[8]) {
+// Has x computed here: the compiler would put sums off and keep their terms in registers.
+__device__ __forceinline__ void pin(float (&x)[8]) {
+  asm volatile(""
+               : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]),
+                 "+v"(x[6]), "+v"(x[7]));
+}
+
+// Waits here for a scalar row.
+template <int N>
+__device__ __forceinline__ void arrived(float (&x)[N]) {
 #pragma unroll
-  for (int n = 0; n < 8; ++n) x[n] = p[n];
+  for (int i = 0; i < N; i += 8)
+    asm volatile(""
+                 : "+s"(x[i]), "+s"(x[i + 1]), "+s"(x[i + 2]), "+s"(x[i + 3]), "+s"(x[i + 4]),
+                   "+s"(x[i + 5]), "+s"(x[i + 6]), "+s"(x[i + 7]));
+}
+
+template <int N>
+__device__ __forceinline__ void load_row(cfloat* p, float (&x)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = p[n];
 }
 
 // B and C as float32 rows [token][group][2][NP], zeros past N and in one more row, which stands
@@ -158,6 +176,7 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
   const uint32_t lo = live ? lane : 0;
   const long dl = tl.d0 + lo;
 
+  constexpr int GN = NP < 16 ? NP : 16;   // states whose rows are in scalar registers at a time
   float A[NP], h[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) h[n] = 0.f;
@@ -220,39 +239,45 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
     if (it + 1 < nt) load(t0 + step * SS_K);
     if (MODE == 1 && a.chunk_h && live)
       store_states<NP>(a.chunk_h + (long)(pc.c0 + k) * NP * D + tl.d0, D, lo, h);
-    const float* rp = bc + t0 * bc_st;
+    const float* q = bc + (t0 + (MODE == 2 ? SS_K - 1 : 0)) * bc_st;
     float ahead[2] = {0.f, 0.f};
-    if (MODE == 2) rp = t0 + SS_K - 1 < pc.t1 ? rp + (SS_K - 1) * bc_st : bc_end;
 #pragma unroll
     for (int j = 0; j < SS_K; ++j) {
       const int i = MODE == 2 ? SS_K - 1 - j : j;
-      asm volatile("" : : "s"(ahead[0]), "s"(ahead[1]));
-      cfloat* row = row_after(rp, h);
-      if (MODE == 2)
-        rp = t0 + i - 1 < pc.t1 ? bc + (t0 + i - 1) * bc_st : bc_end;
-      else
-        rp = t0 + i + 1 < pc.t1 ? rp + bc_st : bc_end;
       const float x = MODE == 2 ? u[i] : d[i] * u[i];
       float acc[2] = {0.f, 0.f};
+      const float* at = t0 + i < pc.t1 ? q : bc_end;
+      q += MODE == 2 ? -bc_st : bc_st;
 #pragma unroll
-      for (int n = 0; n < NP; ++n) {
-        const float ex = exp2_hw(A[n] * d[i]);
-        if (MODE == 2) {
-          h[n] = ex * fmaf(x, row[n], h[n]);
-        } else {
-          h[n] = fmaf(ex, h[n], x * row[n]);
-          if (MODE == 1) acc[n & 1] = fmaf(h[n], row[NP + n], acc[n & 1]);
+      for (int g = 0; g < NP; g += GN) {
+        float(&hg)[GN] = *reinterpret_cast<float(*)[GN]>(&h[g]);
+        float rb[GN], rc[GN];
+        asm volatile("" : : "s"(ahead[0]), "s"(ahead[1]));
+        cfloat* row = row_after(at, hg);
+        load_row(row + g, rb);
+        if (MODE == 1) load_row(row + NP + g, rc);
+        arrived(rb);
+        if (MODE == 1) arrived(rc);
+        const bool more = g + GN < NP;
+        if (more || j + 1 < SS_K) {   // the next rows into the scalar cache
+          cfloat* np = more ? row + g + GN
+                            : (cfloat*)(uintptr_t)(t0 + i + (MODE == 2 ? -1 : 1) < pc.t1 ? q : bc_end);
+          ahead[0] = np[0];
+          if (MODE == 1) ahead[1] = np[NP];
         }
-        if (n == 0 && j + 1 < SS_K) {
-          // this token's rows are there: fetch the next one's into the scalar cache
-          const float* np = rp;
-          asm volatile("" : "+s"(np), "+v"(h[0]));
-          ahead[0] = *(cfloat*)(uintptr_t)np;
-          if (MODE == 1) ahead[1] = *(cfloat*)(uintptr_t)(np + NP);
+#pragma unroll
+        for (int n = 0; n < GN; ++n) {
+          const float ex = exp2_hw(A[g + n] * d[i]);
+          if (MODE == 2) {
+            hg[n] = ex * fmaf(x, rb[n], hg[n]);
+          } else {
+            hg[n] = fmaf(ex, hg[n], x * rb[n]);
+            if (MODE == 1) acc[n & 1] = fmaf(hg[n], rc[n], acc[n & 1]);
+          }
         }
+        if (MODE == 1) asm volatile("" : "+v"(acc[0]), "+v"(acc[1]));   // like h: now
       }
       y[i] = acc[0] + acc[1];
-      if (MODE == 1) asm volatile("" : "+v"(y[i]));   // before the next token's rows, like h
       if (MODE != 1) dsum += d[i];
     }
     if (MODE == 1) {
@@ -463,45 +488,58 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
     float av[SS_K][8], hv[SS_K][8], hin[8];
 #pragma unroll
     for (int n = 0; n < 8; ++n) hin[n] = live ? rh[n] : 0.f;
-    const float* rp = bc + t0 * bc_st;
+    // The rows of a token are fetched while the one before it is computed: B and C into scalar
+    // registers, delta', u and dy from LDS. One counter stands for both kinds of loads, and the
+    // scalar ones come in any order: a wait has to be for all of them, before the next are sent.
+    const float* q = bc + t0 * bc_st;
     float nb[8], nc[8];
-    load_row(row_after(rp, hin), nb);
+    load_row(row_after(q, hin), nb);
     __syncthreads();
     if (k > 0) load(k - 1);
-
+    float nd = sD[0][col], nu = sU[0][col], ng;
 #pragma unroll
     for (int t = 0; t < SS_K; ++t) {
-      float rb[8];   // this token's B; the next one's is on its way while this one is computed
+      float rb[8];
+      arrived(nb);
+      asm volatile("" : "+v"(nd), "+v"(nu));
 #pragma unroll
       for (int n = 0; n < 8; ++n) rb[n] = nb[n];
+      const float d = nd, x = d * nu;
+      if (t < SS_K - 1) q += bc_st;
+      cfloat* row = row_after(t0 + min(t + 1, SS_K - 1) < pc.t1 ? q : bc_end,
+                              t ? hv[t - 1] : hin);
+      load_row(row, nb);
       if (t < SS_K - 1) {
-        rp = t0 + t + 1 < pc.t1 ? rp + bc_st : bc_end;
-        load_row(row_after(rp, t ? hv[t - 1] : hin), nb);
+        nd = sD[t + 1][col];
+        nu = sU[t + 1][col];
       } else {
-        cfloat* row = row_after(rp, hv[t - 1]);
-        load_row(row, nb);
         load_row(row + NP, nc);
+        ng = sG[t][col];
       }
-      const float d = sD[t][col], x = d * sU[t][col];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         av[t][n] = exp2_hw(A[n] * d);
         hv[t][n] = fmaf(av[t][n], t ? hv[t - 1][n] : hin[n], x * rb[n]);
       }
     }
-    fence();
 #pragma unroll
     for (int t = SS_K - 1; t >= 0; --t) {
       float rb[8], rc[8];
+      arrived(nb);
+      arrived(nc);
+      asm volatile("" : "+v"(nd), "+v"(nu), "+v"(ng));
 #pragma unroll
       for (int n = 0; n < 8; ++n) rb[n] = nb[n], rc[n] = nc[n];
+      const float d = nd, x = d * nu, dy = ng;
       if (t > 0) {
-        rp = t0 + t - 1 < pc.t1 ? bc + (t0 + t - 1) * bc_st : bc_end;
-        cfloat* row = row_after(rp, carry);
+        q -= bc_st;
+        cfloat* row = row_after(t0 + t - 1 < pc.t1 ? q : bc_end, t < SS_K - 1 ? carry : hv[t]);
         load_row(row, nb);
         load_row(row + NP, nc);
+        nd = sD[t - 1][col];
+        nu = sU[t - 1][col];
+        ng = sG[t - 1][col];
       }
-      const float d = sD[t][col], x = d * sU[t][col], dy = sG[t][col];
       float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -516,6 +554,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
         s3 = fmaf(hv[t][n], rc[n], s3);
         dA[n] = fmaf(gp, d, dA[n]);
       }
+      pin(dA);
       sS[part][0][t][col] = s1;
       sS[part][1][t][col] = s2;
       sS[part][2][t][col] = s3;
@@ -525,6 +564,8 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
       fence();
     }
     __syncthreads();
+    const long o = (pc.b * a.T + t0 + ts) * D + d0;
+    T *odu = (T*)a.du + o, *odd = (T*)a.ddelta + o, *odz = (T*)a.dz + o;
 #pragma unroll
     for (int i = 0; i < L::TPW; ++i) {
       const int t = ts + i;
@@ -542,11 +583,13 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
       if (live && t0 + t < pc.t1) {
         accD = fmaf(dy, u, accD);
         accB += dd;
-        const long o = (pc.b * a.T + t0 + t) * D + d0;
-        ((T*)a.du + o)[lo] = from_f32<T>(du);
-        ((T*)a.ddelta + o)[lo] = from_f32<T>(dd);
-        if (has_z) ((T*)a.dz + o)[lo] = from_f32<T>(dz);
+        odu[lo] = from_f32<T>(du);
+        odd[lo] = from_f32<T>(dd);
+        if (has_z) odz[lo] = from_f32<T>(dz);
       }
+      odu += D;
+      odd += D;
+      odz += D;
     }
     // the block's share of dB and dC: [tile of the group][token][group][2][NP]
     for (int i = tid; i < SS_K * 2 * NP; i += 64 * L::WAVES) {
