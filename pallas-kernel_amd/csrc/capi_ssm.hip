@@ -86,7 +86,7 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
   const int64_t np = tops::scan_state_pad((int)a->N);
   p->tiles_g = (int)tiles_of(a->D, a->G);
   if (p->tiles_g * a->G * std::max<int64_t>(p->npieces, 1) > kMax ||
-      (a->D * np / 64 + 1) * a->nseq > kMax)
+      (a->D + 63) / 64 * np * a->nseq > kMax)
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   p->ntiles = p->tiles_g * (int)a->G;
   p->at = a->bc + (p->tokens * a->G + 1) * 2 * np;
@@ -167,8 +167,8 @@ extern "C" {
 
 int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t D, int64_t N, int64_t G) {
   if (tokens <= 0 || D < 1 || N < 1 || N > 64 || G < 1) return 64;
-  // four waves a SIMD, and at most 512 pieces for the fold to walk
-  const int64_t len = std::max((tokens * tiles_of(D, G) * G + 4095) / 4096, (tokens + 511) / 512);
+  // eight waves a SIMD, which take turns, and at most 512 pieces for the fold to walk
+  const int64_t len = std::max((tokens * tiles_of(D, G) * G + 8191) / 8192, (tokens + 511) / 512);
   return std::min<int64_t>(std::max<int64_t>(16, (len + 15) / 16 * 16), 1 << 30);
 }
 

@@ -136,19 +136,21 @@ __device__ __forceinline__ void load_row(cfloat* p, float (&x)[N]) {
 
 // B and C as float32 rows [token][group][2][NP], zeros past N and in one more row, which stands
 // for the tokens past a piece's end; then A log2(e) as rows of D channels [NP][D].
-template <typename T>
-__global__ __launch_bounds__(256) void scan_bc_kernel(ScanParams p, int NP) {
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void scan_bc_kernel(ScanParams p) {
   const long rows = p.tokens * p.a.G, nbc = (rows + 1) * 2 * NP, total = nbc + p.a.D * NP;
   const int N = (int)p.a.N, G = (int)p.a.G;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     const int n = (int)(i % NP), w = (int)(i / NP % 2);
-    const long r = i / (2 * NP), tok = r / G, g = r - tok * G;
+    const long r = i / (2 * NP);
+    const int tok = G == 1 ? (int)r : (int)(r / G);   // B T < 2^31
+    const long g = r - (long)tok * G;
     if (r >= rows) {
-      const long j = i - nbc, m = j >= 0 ? j / p.a.D : N;
-      p.a.bc[i] = m < N ? scaled_a(p.a.A[(j - m * p.a.D) * N + m]) : 0.f;
+      const int j = (int)(i - nbc), m = j >= 0 ? j / (int)p.a.D : N;   // D NP <= 2^26
+      p.a.bc[i] = m < N ? scaled_a(p.a.A[(j - m * (int)p.a.D) * (long)N + m]) : 0.f;
       continue;
     }
-    const long b = tok / p.a.T, t = tok - b * p.a.T;
+    const long b = p.a.batch == 1 ? 0 : tok / (int)p.a.T, t = tok - b * p.a.T;
     const T* s = w ? (const T*)p.a.C + b * p.a.C_sb + t * p.a.C_st + g * p.a.C_sg
                    : (const T*)p.a.B + b * p.a.B_sb + t * p.a.B_st + g * p.a.B_sg;
     p.a.bc[i] = n < N ? to_f32(s[n]) : 0.f;
@@ -308,20 +310,21 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
 // The pieces' entry states in the place of their own ones: h <- exp(A S_j) h + L_j over a
 // sequence's pieces from h0 on, or backward from dht on with REV. A thread folds a run of the
 // pieces for a state of a channel, 4 threads share a sequence's runs: each finds its run's own L
-// and S, then its entry from those of the runs before, then its pieces' entries.
-constexpr int FOLD_R = 4, FOLD_U = 8;
+// and S, then its entry from those of the runs before, then its pieces' entries. Runs of up to 16
+// pieces are read once.
+constexpr int FOLD_R = 4, FOLD_U = 16, FOLD_NT = 64 * FOLD_R;
 template <int NP, bool REV>
-__global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
+__global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p, int nb) {
   __shared__ float sL[FOLD_R][64], sS[FOLD_R][64];
   const tops_gla_scan_args& a = p.a;
-  const int seq = blockIdx.x / nb;
+  const int seq = uni(blockIdx.x / nb);
   const long pi = a.segs ? a.segs[8L * seq + 6] : (long)seq * p.pieces;
-  const int np = piece_of(p, (int)pi).np, m = (np + FOLD_R - 1) / FOLD_R;
-  const int run = threadIdx.x / 64, c = threadIdx.x % 64;
+  const int np = uni(piece_of(p, (int)pi).np), m = (np + FOLD_R - 1) / FOLD_R;
+  const int run = uni(threadIdx.x / 64), c = threadIdx.x % 64;
   const int D = (int)a.D, N = (int)a.N;
-  const long q = (long)(blockIdx.x - seq * nb) * 64 + c, nd = (long)D * NP;
-  const bool live = q < nd;
-  const int n = live ? (int)(q / D) : 0, d = live ? (int)(q - (long)n * D) : 0;
+  const int n = uni((blockIdx.x - seq * nb) % NP), d = (blockIdx.x - seq * nb) / NP * 64 + c;
+  const long nd = (long)D * NP;
+  if (d >= D) return;   // the same lanes of every wave: their columns of sL and sS are not used
   const int j0 = min(np, run * m), j1 = min(np, j0 + m);
   const float* init = REV ? a.dht : a.h0;
   const float A = p.at[(long)n * D + d];
@@ -330,17 +333,18 @@ __global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
   float* H = a.piece_h + first * nd + (long)n * D + d;
   const float* S = a.piece_dt + first * D + d;
   float h = 0.f, s = 0.f;
+  float l[FOLD_U], dt[FOLD_U];
   // h through the pieces j .. end - 1, each piece's entry state written with `put`; the last piece
   // has no own state
   auto walk = [&](int j, int end, bool put) {
     for (; j < end; j += FOLD_U) {
-      float l[FOLD_U], dt[FOLD_U];
+      if (!put || m > FOLD_U)
 #pragma unroll
-      for (int i = 0; i < FOLD_U; ++i) {
-        const int at = max(0, min(j + i, np - 2));
-        l[i] = H[at * hs];
-        dt[i] = S[at * ss];
-      }
+        for (int i = 0; i < FOLD_U; ++i) {
+          if (j + i >= min(end, np - 1)) break;
+          l[i] = H[(j + i) * hs];
+          dt[i] = S[(j + i) * ss];
+        }
 #pragma unroll
       for (int i = 0; i < FOLD_U; ++i) {
         if (j + i >= end) break;
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
       }
     }
   };
-  if (run < FOLD_R - 1) walk(j0, j1, false);
+  walk(j0, j1, false);
   sL[run][c] = h;
   sS[run][c] = s;
   __syncthreads();
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(256) void scan_fold_kernel(ScanParams p, int nb) {
     const float l = sL[r][c];
     h = h == 0.f ? l : fmaf(exp2_hw(A * sS[r][c]), h, l);
   }
-  if (live) walk(j0, j1, true);
+  walk(j0, j1, true);
 }
 
 // ---------------------------------------------------------------------------
@@ -628,8 +632,8 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
 }
 
 // dB, dC from the blocks' shares: one thread per (token, group, array, n).
-template <typename T>
-__global__ __launch_bounds__(256) void scan_bwd_bc_kernel(ScanParams p, int NP) {
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void scan_bwd_bc_kernel(ScanParams p) {
   const long total = p.tokens * p.a.G * 2 * NP;
   const int N = (int)p.a.N, tiles = p.btiles / (int)p.a.G;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
@@ -661,7 +665,8 @@ __global__ __launch_bounds__(256) void scan_bwd_a_kernel(ScanParams p, int NP) {
 #pragma unroll
   for (int r = 0; r < 8; ++r) s += red[r][c];
   if (isa) {
-    const long n = i / D, d = i - n * D;
+    const int n = (int)i / (int)D;   // D NP <= 2^26
+    const long d = i - n * D;
     if (n < N) p.a.dA[d * N + n] = s;
   } else {
     const long r = i - na;
@@ -676,9 +681,9 @@ unsigned grid_of(long threads) {
 
 template <int NP, bool REV>
 hipError_t scan_fold(const ScanParams& p, hipStream_t st) {
-  const int nb = (int)((p.a.D * NP + 63) / 64);
-  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.a.nseq)), dim3(256), 0,
-                     st, p, nb);
+  const int nb = (int)((p.a.D + 63) / 64) * NP;
+  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.a.nseq)),
+                     dim3(FOLD_NT), 0, st, p, nb);
   return hipGetLastError();
 }
 
@@ -686,7 +691,7 @@ template <typename T, int NP>
 hipError_t scan_fwd(const ScanParams& p, hipStream_t st) {
   const dim3 grid((unsigned)((p.npieces * p.ntiles + 3) / 4));
   const long nbc = (p.tokens * p.a.G + 1) * 2 * NP + p.a.D * NP;
-  hipLaunchKernelGGL((scan_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
+  hipLaunchKernelGGL((scan_bc_kernel<T, NP>), dim3(grid_of(nbc)), dim3(256), 0, st, p);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.multi) {
     hipLaunchKernelGGL((scan_kernel<T, NP, 0>), grid, dim3(256), 0, st, p);
@@ -712,7 +717,7 @@ hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
   }
   const long nbc = p.tokens * p.a.G * 2 * NP, na = p.a.D * (NP + 2);
   if (nbc > 0) {
-    hipLaunchKernelGGL((scan_bwd_bc_kernel<T>), dim3(grid_of(nbc)), dim3(256), 0, st, p, NP);
+    hipLaunchKernelGGL((scan_bwd_bc_kernel<T, NP>), dim3(grid_of(nbc)), dim3(256), 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
   }
   hipLaunchKernelGGL(scan_bwd_a_kernel, dim3((unsigned)((na + 31) / 32)), dim3(256), 0, st, p, NP);
