@@ -41,7 +41,7 @@ def _forward(q, k, qw, kw, freq, pos, eps, interleaved):
     qo = torch.empty(q.shape, dtype=dt, device=dev)
     ko = torch.empty(k.shape, dtype=dt, device=dev)
     call("tops_gla_qk_norm_rope_fwd", _pack(x, (qo, ko), interleaved, eps), stream_of(dev))
-    return qo.to(q.dtype), ko.to(k.dtype), x
+    return qo if dt is q.dtype else qo.to(q.dtype), ko if dt is k.dtype else ko.to(k.dtype), x
 
 
 class _QkNormRopeFunction(torch.autograd.Function):

@@ -11,22 +11,25 @@ _IO = (torch.float32, torch.bfloat16)
 
 def io_dtype(*tensors):
     """The type the kernel computes such tensors in: bfloat16 where all are, else float32."""
-    return (torch.bfloat16 if all(t is None or t.dtype == torch.bfloat16 for t in tensors)
-            else torch.float32)
+    for t in tensors:
+        if t is not None and t.dtype is not torch.bfloat16:
+            return torch.float32
+    return torch.bfloat16
 
 
 def rows(t, dt):
     """t in type dt with its last dimension contiguous (a view where it already is)."""
-    if t is None:
-        return None
-    if t.dtype != dt:
-        t = t.to(dt)
+    if t is None or (t.dtype is dt and t.stride(-1) == 1):
+        return t
+    t = t.to(dt)
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def f32(t):
     """A small parameter or a state as the kernels read it: float32, contiguous."""
-    return None if t is None else t.to(torch.float32).contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def differentiable(*tensors):
@@ -34,11 +37,15 @@ def differentiable(*tensors):
     the functions then refuse)."""
     if torch.autograd.forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def refuse_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and differentiable(*tensors):
         raise RuntimeError(f"{name} updates its state in place and has no gradient: call it under "
                            "torch.no_grad()")
 
@@ -93,9 +100,25 @@ def slot_args(idx, batch, device_of):
     return idx.data_ptr(), int(idx.dtype == torch.int64)
 
 
+def gradients(grads, like, need):
+    """The gradients in the types and shapes of their inputs, None where none is wanted."""
+    out = []
+    for g, want, n in zip(grads, like, need):
+        if g is None or not n:
+            out.append(None)
+            continue
+        if g.shape != want[1]:
+            g = g.reshape(want[1])
+        out.append(g if g.dtype is want[0] else g.to(want[0]))
+    return out
+
+
 def address(t):
     return 0 if t is None else t.data_ptr()
 
 
 def strides(t, *dims):
-    return [0] * len(dims) if t is None else [t.stride(d) for d in dims]
+    if t is None:
+        return (0,) * len(dims)
+    s = t.stride()
+    return [s[d] for d in dims]

@@ -10,7 +10,7 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, device_table, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
+from ._common import (address, device_table, differentiable, f32, gradients, io_dtype, offsets, refuse_grad, rows,
                       slot_args, strides)
 
 _ARGS = struct.Struct("=26q")
@@ -28,7 +28,9 @@ def _silu(activation):
 
 
 def _contiguous(t, dt):
-    return None if t is None else t.to(dt).contiguous()
+    if t is None or (t.dtype is dt and t.is_contiguous()):
+        return t
+    return t.to(dt).contiguous()
 
 
 def _pack(x, y, fin, cu_t, nseq, silu, bwd=None):
@@ -50,7 +52,9 @@ def _forward(x, weight, bias, init, silu, want, cu):
     y = torch.empty(B, T, D, dtype=dt, device=dev)
     fin = torch.empty(nseq, W, D, dtype=dt, device=dev) if want else None
     call("tops_gla_causal_conv_fwd", _pack(a, y, fin, cu_t, nseq, silu), stream_of(dev))
-    return y.to(x.dtype), None if fin is None else fin.to(x.dtype), a, cu_t
+    if dt is not x.dtype:
+        y, fin = y.to(x.dtype), None if fin is None else fin.to(x.dtype)
+    return y, fin, a, cu_t
 
 
 class _CausalConvFunction(torch.autograd.Function):
@@ -84,10 +88,8 @@ class _CausalConvFunction(torch.autograd.Function):
         bwd = [*(address(t) for t in (dy, dfin, dx, dinit, dw, db, ws)), nws, *strides(dy, 0, 1)]
         call("tops_gla_causal_conv_bwd", _pack((x, w, b, init), None, None, cu_t, ctx.nseq,
                                                ctx.silu, bwd), stream_of(dev))
-        return (*(None if g is None or like is None or not need
-                  else g.reshape(like[1]).to(like[0])
-                  for g, like, need in zip((dx, dw, db, dinit), ctx.like, ctx.needs_input_grad)),
-                None, None, None)
+        return (*gradients((dx, dw, None if ctx.like[2] is None else db, dinit), ctx.like,
+                           ctx.needs_input_grad), None, None, None)
 
 
 def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None,

@@ -9,7 +9,7 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, device_table, differentiable, f32, io_dtype, offsets, refuse_grad, rows,
+from ._common import (address, device_table, differentiable, f32, gradients, io_dtype, offsets, refuse_grad, rows,
                       slot_args, strides)
 
 _ARGS = struct.Struct("=53q")
@@ -64,22 +64,25 @@ def _pack(x, y, ht, chunk_h, ws, bc, pc, shape, softplus, dt, bwd=None):
     u, delta, A, B, C, Dskip, z, bias, h0 = x
     if bwd is None:
         bwd = [0] * 15
-    ph, pd = ws
+    ph = pd = 0
+    if ws is not None:
+        ph = ws.data_ptr()
+        pd = ph + 4 * pc.nsegs * _pad(N) * D
     return _ARGS.pack(
         address(u), address(delta), address(z), address(B), address(C), address(A),
         address(Dskip), address(bias), address(h0), address(y), address(ht), address(chunk_h),
-        address(ph), address(pd), address(bc), address(pc.table),
+        ph, pd, address(bc), address(pc.table),
         pc.nsegs, pc.nseq, pc.piece, Bt, T, D, N, G,
         *strides(u, 0, 1), *strides(delta, 0, 1), *strides(z, 0, 1), *strides(B, 0, 1, 2),
         *strides(C, 0, 1, 2), int(softplus), dtype_code(dt), *bwd)
 
 
 def _piece_states(pc, D, N, dev):
-    """Workspaces of the pieces' own contributions, where a sequence has several pieces."""
+    """Workspace of the pieces' own contributions, [pieces][NP + 1][D] in two parts, where a
+    sequence has several pieces."""
     if not pc.multi:
-        return None, None
-    return (torch.empty(pc.nsegs, _pad(N), D, dtype=torch.float32, device=dev),
-            torch.empty(pc.nsegs, D, dtype=torch.float32, device=dev))
+        return None
+    return torch.empty(pc.nsegs * (_pad(N) + 1) * D, dtype=torch.float32, device=dev)
 
 
 def _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu, keep):
@@ -100,7 +103,7 @@ def _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht, cu, keep):
     bc = torch.empty(((Bt * T * G + 1) * 2 + Dn) * _pad(N), dtype=torch.float32, device=dev)
     call("tops_gla_selective_scan_fwd",
          _pack(x, y, ht, chunk_h, ws, bc, pc, (Bt, T, Dn, N, G), softplus, dt), stream_of(dev))
-    return y.to(u.dtype), ht, x, chunk_h, bc, pc
+    return y if dt is u.dtype else y.to(u.dtype), ht, x, chunk_h, bc, pc
 
 
 class _SelectiveScanFunction(torch.autograd.Function):
@@ -138,16 +141,14 @@ class _SelectiveScanFunction(torch.autograd.Function):
         dbias = None if bias is None else new(Dn)
         dh0 = None if ctx.like[8] is None else new(pc.nseq, Dn, N)
         nws = int(_lib.load().tops_gla_selective_scan_bwd_ws_bytes(Bt * T, pc.nsegs, Dn, N, G))
-        ws = new(nws, dtype=torch.uint8)
+        ws, ps = new(nws, dtype=torch.uint8), _piece_states(pc, Dn, N, dev)
         bwd = [address(dy), *strides(dy, 0, 1), *(address(t) for t in (
             dht, du, ddelta, dz, dB, dC, dA, dD, dbias, dh0, ws)), nws]
         call("tops_gla_selective_scan_bwd",
-             _pack(x, None, None, chunk_h, _piece_states(pc, Dn, N, dev), bc, pc,
+             _pack(x, None, None, chunk_h, ps, bc, pc,
                    (Bt, T, Dn, N, G), ctx.softplus, dt, bwd), stream_of(dev))
         grads = (du, ddelta, dA, dB, dC, dD, dz, dbias, dh0)
-        return (*(None if g is None or not need else g.reshape(like[1]).to(like[0])
-                  for g, like, need in zip(grads, ctx.like, ctx.needs_input_grad)),
-                None, None, None)
+        return (*gradients(grads, ctx.like, ctx.needs_input_grad), None, None, None)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False,
