@@ -13,7 +13,7 @@ namespace tops {
 namespace {
 
 constexpr int QK_NT = 256;
-constexpr int QK_TB = 4;   // tokens whose angles a block forms at a time
+constexpr int QK_MAXTB = 16;   // most tokens whose angles a block forms at a time
 
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x) {
@@ -276,29 +276,365 @@ __global__ __launch_bounds__(QK_NT) void qk_bwd_kernel(tops_gla_qk_args a, long 
     }
 }
 
-// The weights' gradients from the blocks' rows, a wave a column.
-__global__ __launch_bounds__(QK_NT) void qk_dw_kernel(const float* part, int rows, int D,
-                                                      float* dqw, float* dkw) {
-  const int i = blockIdx.x * (QK_NT / 64) + threadIdx.x / 64, lane = threadIdx.x & 63;
-  if (i >= 2 * D) return;
+// The weights' gradients from the blocks' rows, 64 threads a column.
+constexpr int QD_C = 16, QD_R = 64;
+__global__ __launch_bounds__(QD_C * QD_R) void qk_dw_kernel(const float* part, int rows, int D,
+                                                            float* dqw, float* dkw) {
+  __shared__ float red[QD_R][QD_C + 1];
+  const int c = threadIdx.x % QD_C, r0 = threadIdx.x / QD_C, i = blockIdx.x * QD_C + c;
   float s = 0.f;
-  for (int r = lane; r < rows; r += 64) s += part[(long)r * 2 * D + i];
-  s = row_sum<64>(s);
+  if (i < 2 * D)
+#pragma unroll 8
+    for (int r = r0; r < rows; r += QD_R) s += part[(long)r * 2 * D + i];
+  red[r0][c] = s;
+  __syncthreads();
+  for (int n = QD_R / 2; n > 0; n /= 2) {
+    if (r0 < n) red[r0][c] += red[r0 + n][c];
+    __syncthreads();
+  }
   float* out = i < D ? dqw : dkw;
-  if (lane == 0 && out) out[i % D] = s;
+  if (r0 == 0 && i < 2 * D && out) out[i % D] = red[0][c];
+}
+
+// ---------------------------------------------------------------------------
+// Rows that one wave's lanes hold whole in pieces of VEC > 1 elements (every aligned head of up to
+// 256 or 512 columns): the partner of a rotated piece comes from its lane, and the rows of the
+// next batch are on their way while one is computed.
+// ---------------------------------------------------------------------------
+constexpr int QK_U = 4;    // rows of a thread in a batch of the forward
+constexpr int QK_UB = 2;   // of the backward
+
+template <typename T, int VEC>
+struct Piece {
+  static constexpr int W = VEC * sizeof(T) / 4;
+  uint32_t w[W];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void piece_load(Piece<T, VEC>& r, const T* p) {
+  if constexpr (Piece<T, VEC>::W == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = x.x, r.w[1] = x.y, r.w[2] = x.z, r.w[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = x.x, r.w[1] = x.y;
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void piece_values(const Piece<T, VEC>& r, float (&x)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < Piece<T, VEC>::W; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      x[2 * i] = bf16_lo(r.w[i]);
+      x[2 * i + 1] = bf16_hi(r.w[i]);
+    } else {
+      x[i] = __uint_as_float(r.w[i]);
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void piece_of_lane(Piece<T, VEC>& r, int lane4) {
+#pragma unroll
+  for (int i = 0; i < Piece<T, VEC>::W; ++i)
+    r.w[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(lane4, (int)r.w[i]);
+}
+
+// Element offsets of the block's tokens in q and k (and in their gradients).
+__device__ __forceinline__ void token_offsets(const tops_gla_qk_args& a, long tau0, int nt,
+                                              bool backward, long (*off)[4]) {
+  const int k = threadIdx.x;
+  if (k >= nt) return;
+  const long tau = tau0 + k, b = tau / a.T, t = tau - b * a.T;
+  off[k][0] = b * a.q_sb + t * a.q_st;
+  off[k][1] = b * a.k_sb + t * a.k_st;
+  if (backward) {
+    off[k][2] = b * a.dq_sb + t * a.dq_st;
+    off[k][3] = b * a.dk_sb + t * a.dk_st;
+  }
+}
+
+// A lane's place in a row: its piece, the piece's partner, and what a rotation does with it.
+template <int VEC, int LPR, bool INTER>
+struct Lane {
+  int c, f, lane4;
+  bool in, rot, hi;
+  __device__ __forceinline__ Lane(int D, int R) {
+    const int lane = threadIdx.x % LPR, R2 = R / 2;
+    c = lane * VEC;
+    in = c < D;
+    rot = c < R;
+    hi = !INTER && rot && c >= R2;
+    f = !rot ? 0 : INTER ? c / 2 : hi ? c - R2 : c;
+    const int m = INTER || !rot ? 0 : hi ? -(R2 / VEC) : R2 / VEC;
+    lane4 = 4 * ((threadIdx.x & 63) + m);
+  }
+  // column of the partner's piece
+  __device__ __forceinline__ int pc(int R) const {
+    return INTER || !rot ? c : hi ? c - R / 2 : c + R / 2;
+  }
+};
+
+// x turned by the angles of cs (sign -1: back), xp being its partner piece.
+template <int VEC, int LPR, bool INTER>
+__device__ __forceinline__ void turn_piece(float (&x)[VEC], const float (&xp)[VEC],
+                                           const float2* cs, const Lane<VEC, LPR, INTER>& l, int R,
+                                           float sign) {
+  turn<VEC, INTER>(x, xp, cs, l.rot, l.hi, l.c, R, sign);
+}
+
+// `magic[p]` = ceil(2^32 / heads of part p): row / heads = mulhi(row, magic) for row < 2^16.
+template <typename T, int VEC, int LPR, bool INTER>
+__global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, int tb,
+                                                            uint32_t magic_q, uint32_t magic_k) {
+  extern __shared__ float2 cs[];
+  __shared__ long off[QK_MAXTB][4];
+  constexpr int RPB = QK_NT / LPR;
+  constexpr bool PAIR = !INTER;
+  const int row0 = threadIdx.x / LPR;
+  const int D = (int)a.D, R = (int)a.R, R2 = R / 2;
+  const long tokens = a.batch * a.T, tau0 = (long)blockIdx.x * tb;
+  const int nt = (int)min((long)tb, tokens - tau0);
+  const Lane<VEC, LPR, INTER> l(D, R);
+  const int cl = l.in ? l.c : 0;
+  token_offsets(a, tau0, nt, false, off);
+  __syncthreads();
+  const int rq = nt * (int)a.Hq, rk = nt * (int)a.Hk;   // rows of the two parts, and batches
+  const int nbq = (rq + RPB * QK_U - 1) / (RPB * QK_U), nb = nbq + (rk + RPB * QK_U - 1) / (RPB * QK_U);
+  Piece<T, VEC> nx[QK_U];
+  auto load = [&](int i) {
+    const bool part = i >= nbq;
+    const int H = (int)(part ? a.Hk : a.Hq), rows = part ? rk : rq;
+    const uint32_t magic = part ? magic_k : magic_q;
+    const T* src = (const T*)(part ? a.k : a.q);
+    const long sh = part ? a.k_sh : a.q_sh;
+    const int r0 = (i - (part ? nbq : 0)) * RPB * QK_U + row0;
+#pragma unroll
+    for (int u = 0; u < QK_U; ++u) {
+      const int r = min(r0 + u * RPB, rows - 1);
+      const int tk = H == 1 ? r : (int)__umulhi((uint32_t)r, magic);
+      piece_load<T, VEC>(nx[u], src + off[tk][part] + (r - tk * H) * sh + cl);
+    }
+  };
+  if (nb > 0) load(0);
+  angles(a, tau0, nt, cs);
+  __syncthreads();
+  const float inv_d = 1.f / (float)D, eps = (float)a.eps;
+  float wv[VEC], wp[VEC];
+#pragma unroll 1
+  for (int i = 0; i < nb; ++i) {
+    const bool part = i >= nbq;
+    if (i == 0 || i == nbq) {
+      const float* w = part ? a.kw : a.qw;
+      const int pc = l.in ? l.pc(R) : 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        wv[e] = w ? w[cl + e] : 1.f;
+        wp[e] = w ? w[pc + e] : 1.f;
+      }
+    }
+    Piece<T, VEC> x[QK_U];
+#pragma unroll
+    for (int u = 0; u < QK_U; ++u) x[u] = nx[u];
+    if (i + 1 < nb) load(i + 1);
+    const int H = (int)(part ? a.Hk : a.Hq), rows = part ? rk : rq;
+    const uint32_t magic = part ? magic_k : magic_q;
+    T* dst = (T*)(part ? a.ko : a.qo) + tau0 * H * D;
+    const int r0 = (i - (part ? nbq : 0)) * RPB * QK_U + row0;
+#pragma unroll
+    for (int u = 0; u < QK_U; ++u) {
+      const int r = r0 + u * RPB;
+      float v[VEC], p[VEC], ss = 0.f;
+      piece_values<T, VEC>(x[u], v);
+      if (PAIR) {
+        piece_of_lane<T, VEC>(x[u], l.lane4);
+        piece_values<T, VEC>(x[u], p);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (!l.in) v[e] = 0.f;
+        ss = fmaf(v[e], v[e], ss);
+      }
+      const float rstd = rsqrtf(fmaf(row_sum<LPR>(ss), inv_d, eps));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[e] *= rstd * wv[e];
+        if (PAIR) p[e] *= rstd * wp[e];
+      }
+      if (r < rows && l.in) {
+        const int tk = H == 1 ? r : (int)__umulhi((uint32_t)r, magic);
+        turn_piece<VEC, LPR, INTER>(v, p, cs + tk * R2 + l.f, l, R, 1.f);
+        store_run<T, VEC>(dst + (long)r * D + l.c, v);
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int LPR, bool INTER>
+__global__ __launch_bounds__(QK_NT) void qk_bwd_rows_kernel(tops_gla_qk_args a, long ngroups,
+                                                            int tb, uint32_t magic_q,
+                                                            uint32_t magic_k, float* part_w) {
+  extern __shared__ float2 cs[];
+  __shared__ float red[QK_NT * VEC];
+  __shared__ long off[QK_MAXTB][4];
+  constexpr int RPB = QK_NT / LPR;
+  constexpr bool PAIR = !INTER;
+  const int row0 = threadIdx.x / LPR;
+  const int D = (int)a.D, R = (int)a.R, R2 = R / 2;
+  const long tokens = a.batch * a.T;
+  const Lane<VEC, LPR, INTER> l(D, R);
+  const int cl = l.in ? l.c : 0;
+  const float inv_d = 1.f / (float)D, eps = (float)a.eps;
+  float dw[2][VEC] = {};
+  for (long g = blockIdx.x; g < ngroups; g += gridDim.x) {
+    const long tau0 = g * tb;
+    const int nt = (int)min((long)tb, tokens - tau0);
+    const int rq = nt * (int)a.Hq, rk = nt * (int)a.Hk;
+    const int nbq = (rq + RPB * QK_UB - 1) / (RPB * QK_UB),
+              nb = nbq + (rk + RPB * QK_UB - 1) / (RPB * QK_UB);
+    __syncthreads();
+    token_offsets(a, tau0, nt, true, off);
+    __syncthreads();
+    Piece<T, VEC> nx[QK_UB], ng[QK_UB];
+    auto load = [&](int i) {
+      const bool part = i >= nbq;
+      const int H = (int)(part ? a.Hk : a.Hq), rows = part ? rk : rq;
+      const uint32_t magic = part ? magic_k : magic_q;
+      const T* src = (const T*)(part ? a.k : a.q);
+      const T* gsrc = (const T*)(part ? a.dko : a.dqo);
+      const long sh = part ? a.k_sh : a.q_sh, gh = part ? a.dk_sh : a.dq_sh;
+      const int r0 = (i - (part ? nbq : 0)) * RPB * QK_UB + row0;
+#pragma unroll
+      for (int u = 0; u < QK_UB; ++u) {
+        const int r = min(r0 + u * RPB, rows - 1);
+        const int tk = H == 1 ? r : (int)__umulhi((uint32_t)r, magic), hd = r - tk * H;
+        piece_load<T, VEC>(nx[u], src + off[tk][part] + hd * sh + cl);
+        piece_load<T, VEC>(ng[u], gsrc + off[tk][2 + part] + hd * gh + cl);
+      }
+    };
+    if (nb > 0) load(0);
+    angles(a, tau0, nt, cs);
+    __syncthreads();
+    float wv[VEC];
+#pragma unroll 1
+    for (int i = 0; i < nb; ++i) {
+      const bool part = i >= nbq;
+      if (i == 0 || i == nbq) {
+        const float* w = part ? a.kw : a.qw;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) wv[e] = w ? w[cl + e] : 1.f;
+      }
+      Piece<T, VEC> x[QK_UB], gy[QK_UB];
+#pragma unroll
+      for (int u = 0; u < QK_UB; ++u) x[u] = nx[u], gy[u] = ng[u];
+      if (i + 1 < nb) load(i + 1);
+      const int H = (int)(part ? a.Hk : a.Hq), rows = part ? rk : rq;
+      const uint32_t magic = part ? magic_k : magic_q;
+      T* dst = (T*)(part ? a.dk : a.dq) + tau0 * H * D;
+      const int r0 = (i - (part ? nbq : 0)) * RPB * QK_UB + row0;
+#pragma unroll
+      for (int u = 0; u < QK_UB; ++u) {
+        const int r = r0 + u * RPB;
+        const bool on = r < rows && l.in;
+        const int tk = H == 1 ? min(r, nt - 1)
+                              : (int)__umulhi((uint32_t)min(r, rows - 1), magic);
+        float v[VEC], d[VEC], p[VEC], ss = 0.f, em = 0.f;
+        piece_values<T, VEC>(x[u], v);
+        piece_values<T, VEC>(gy[u], d);
+        if (PAIR) {
+          piece_of_lane<T, VEC>(gy[u], l.lane4);
+          piece_values<T, VEC>(gy[u], p);
+        }
+        turn_piece<VEC, LPR, INTER>(d, p, cs + tk * R2 + l.f, l, R, -1.f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (!on) v[e] = d[e] = 0.f;
+          ss = fmaf(v[e], v[e], ss);
+          em = fmaf(d[e] * wv[e], v[e], em);
+        }
+        const float rstd = rsqrtf(fmaf(row_sum<LPR>(ss), inv_d, eps));
+        const float mean = row_sum<LPR>(em) * rstd * inv_d;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float m = v[e] * rstd, t = on ? d[e] * m : 0.f;
+          if (part)
+            dw[1][e] += t;
+          else
+            dw[0][e] += t;
+          v[e] = rstd * (d[e] * wv[e] - m * mean);
+        }
+        if (on) store_run<T, VEC>(dst + (long)r * D + l.c, v);
+      }
+    }
+  }
+  if (!part_w) return;   // uniform: no weight gradients wanted
+  float* out = part_w + (long)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) red[threadIdx.x * VEC + e] = dw[part][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += QK_NT) {
+      float s = 0.f;
+      for (int q = 0; q < RPB; ++q) s += red[q * LPR * VEC + i];
+      out[(long)part * D + i] = s;
+    }
+  }
 }
 
 constexpr long kQkBlocks = 1024;   // of the backward: rows of partial weight gradients
 
-// Tokens of a block: four where there are enough to fill the device.
-int tokens_per_block(long tokens) { return tokens >= 4096 ? QK_TB : 1; }
+// Tokens of a block at a time, as long as the blocks fill the device: a block whose threads have
+// several batches of rows pays less for its start (64 heads of 128 columns, 32768 tokens: 161 us
+// forward with 64 rows a batch and part in all, 115 with 256; backward 174 and 164 with 128).
+int tokens_per_block(long tokens, long heads, bool backward) {
+  int tb = 1;
+  while (tb < QK_MAXTB && tb * heads < (backward ? 256 : 512) && tokens >= 2048L * tb) tb *= 2;
+  return tb;
+}
+uint32_t magic_of(long heads) { return heads < 2 ? 0 : (uint32_t)(((1ULL << 32) + heads - 1) / heads); }
+
+template <typename T, int VEC, int LPR>
+hipError_t qk_rows_launch(const tops_gla_qk_args& a, bool backward, int tb, long groups, size_t lds,
+                          hipStream_t st) {
+  const uint32_t mq = magic_of(a.Hq), mk = magic_of(a.Hk);
+  const dim3 nt(QK_NT);
+  if (!backward) {
+    const dim3 grid((unsigned)groups);
+    if (a.interleaved)
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, true>), grid, nt, lds, st, a, tb, mq, mk);
+    else
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, false>), grid, nt, lds, st, a, tb, mq, mk);
+    return hipGetLastError();
+  }
+  const long blocks = std::min(groups, kQkBlocks);
+  float* part = a.dqw || a.dkw ? (float*)a.ws : nullptr;
+  if (blocks > 0) {
+    const dim3 grid((unsigned)blocks);
+    if (a.interleaved)
+      hipLaunchKernelGGL((qk_bwd_rows_kernel<T, VEC, LPR, true>), grid, nt, lds, st, a, groups, tb,
+                         mq, mk, part);
+    else
+      hipLaunchKernelGGL((qk_bwd_rows_kernel<T, VEC, LPR, false>), grid, nt, lds, st, a, groups, tb,
+                         mq, mk, part);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (!a.dqw && !a.dkw) return hipSuccess;
+  hipLaunchKernelGGL(qk_dw_kernel, dim3((unsigned)((2 * a.D + QD_C - 1) / QD_C)),
+                     dim3(QD_C * QD_R), 0, st, part, (int)blocks, (int)a.D, a.dqw, a.dkw);
+  return hipGetLastError();
+}
 
 template <typename T, int VEC, int LPR, int NI>
 hipError_t qk_launch(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
   const long tokens = a.batch * a.T;
-  const int tb = tokens_per_block(tokens);
+  const int tb = tokens_per_block(tokens, a.Hq + a.Hk, backward);
   const long groups = (tokens + tb - 1) / tb;
   const size_t lds = (size_t)tb * (a.R / 2) * sizeof(float2);
+  if constexpr (VEC > 1 && NI == 1) {
+    // a row's index times the magic number is exact below 2^16 rows
+    if (tb * std::max(a.Hq, a.Hk) < 65536) return qk_rows_launch<T, VEC, LPR>(a, backward, tb, groups, lds, st);
+  }
   if (!backward) {
     if (a.interleaved)
       hipLaunchKernelGGL((qk_fwd_kernel<T, VEC, LPR, NI, true>), dim3((unsigned)groups), dim3(QK_NT),
@@ -320,8 +656,8 @@ hipError_t qk_launch(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
     if (hipError_t e = hipGetLastError()) return e;
   }
   if (part || a.dqw || a.dkw) {
-    hipLaunchKernelGGL(qk_dw_kernel, dim3((unsigned)((2 * a.D + 3) / 4)), dim3(QK_NT), 0, st, part,
-                       (int)blocks, (int)a.D, a.dqw, a.dkw);
+    hipLaunchKernelGGL(qk_dw_kernel, dim3((unsigned)((2 * a.D + QD_C - 1) / QD_C)),
+                       dim3(QD_C * QD_R), 0, st, part, (int)blocks, (int)a.D, a.dqw, a.dkw);
     return hipGetLastError();
   }
   return hipSuccess;
@@ -357,10 +693,7 @@ hipError_t qk_rows(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
 
 }  // namespace
 
-long qk_norm_rope_part_rows(long tokens) {
-  const int tb = tokens_per_block(tokens);
-  return std::min((tokens + tb - 1) / tb, kQkBlocks);
-}
+long qk_norm_rope_part_rows(long tokens) { return std::min(tokens, kQkBlocks); }
 
 hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
   if (a.batch * a.T == 0 && !backward) return hipSuccess;
