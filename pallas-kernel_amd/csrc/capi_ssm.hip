@@ -209,7 +209,7 @@ int tops_gla_selective_scan_step(const tops_gla_scan_step_args* a, void* stream)
 
 int64_t tops_gla_causal_conv_bwd_ws_bytes(int64_t tokens, int64_t D, int64_t W) {
   if (tokens <= 0 || D < 1 || W < 1 || W > 8) return 0;
-  return tops::causal_conv_part_rows((long)tokens) * (W + 1) * D * 4;
+  return tops::causal_conv_part_rows((long)tokens, (long)D) * (W + 1) * D * 4;
 }
 
 int tops_gla_causal_conv_fwd(const tops_gla_conv_args* a, void* stream) {

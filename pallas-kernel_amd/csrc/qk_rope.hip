@@ -58,10 +58,10 @@ __device__ __forceinline__ void angles(const tops_gla_qk_args& a, long tau0, int
   const int R2 = (int)a.R / 2;
   for (int i = threadIdx.x; i < nt * R2; i += QK_NT) {
     const int k = i / R2, f = i - k * R2;
-    const long tau = tau0 + k, b = tau / a.T, t = tau - b * a.T;
+    const uint32_t tau = (uint32_t)(tau0 + k), b = tau / (uint32_t)a.T, t = tau - b * (uint32_t)a.T;
     long pos = t;
     if (a.positions) {
-      const long at = b * a.pos_sb + t;
+      const long at = (long)b * a.pos_sb + t;
       pos = a.pos64 ? (long)((const int64_t*)a.positions)[at]
                     : (long)((const int32_t*)a.positions)[at];
     }
@@ -344,7 +344,8 @@ __device__ __forceinline__ void token_offsets(const tops_gla_qk_args& a, long ta
                                               bool backward, long (*off)[4]) {
   const int k = threadIdx.x;
   if (k >= nt) return;
-  const long tau = tau0 + k, b = tau / a.T, t = tau - b * a.T;
+  const uint32_t tau = (uint32_t)(tau0 + k), bb = tau / (uint32_t)a.T;   // B T < 2^31
+  const long b = bb, t = tau - bb * (uint32_t)a.T;
   off[k][0] = b * a.q_sb + t * a.q_st;
   off[k][1] = b * a.k_sb + t * a.k_st;
   if (backward) {

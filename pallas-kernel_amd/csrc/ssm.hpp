@@ -35,7 +35,7 @@ hipError_t run_conv_step(const tops_gla_conv_step_args& a, hipStream_t st);
 
 hipError_t run_causal_conv_fwd(const tops_gla_conv_args& a, hipStream_t st);
 hipError_t run_causal_conv_bwd(const tops_gla_conv_args& a, hipStream_t st);
-long causal_conv_part_rows(long tokens);   // rows of (W + 1) D partial weight gradients
+long causal_conv_part_rows(long tokens, long D);   // rows of (W + 1) D partial weight gradients
 
 hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_t st);
 long qk_norm_rope_part_rows(long tokens);  // rows of 2 D partial weight gradients

@@ -1,7 +1,7 @@
 // Causal depthwise convolution of width W <= 8 with the window carried in and out, forward and
 // backward (include/tops_gla_ssm.h).
 //
-// Bound by memory. A thread walks a run of tokens for VEC channels (16 bytes a row) with the
+// Bound by memory. A thread walks a run of tokens for VEC channels (8 bytes a row) with the
 // last W rows in registers, so that a row is loaded once by it, beside W - 1 rows at the run's
 // ends; a block's threads lie along the channels. Packed sequences share one row of tokens: a
 // run that holds a boundary is walked sequence by sequence.
@@ -331,34 +331,40 @@ __global__ __launch_bounds__(CV_NT) void conv_dinit_kernel(tops_gla_conv_args a,
   }
 }
 
-// The summed rows [D][W], [D] to the two outputs.
+// The summed rows [D][W], [D] to the two outputs, 8 threads a column.
 __global__ __launch_bounds__(256) void conv_dw_kernel(const float* __restrict__ part, int rows,
                                                       long m, long dw_n, float* dw, float* db) {
-  const long i = blockIdx.x * 256L + threadIdx.x;
-  if (i >= m) return;
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-  int r = 0;
-  for (; r + 3 < rows; r += 4) {
-    s0 += part[r * m + i];
-    s1 += part[(r + 1) * m + i];
-    s2 += part[(r + 2) * m + i];
-    s3 += part[(r + 3) * m + i];
-  }
-  for (; r < rows; ++r) s0 += part[r * m + i];
-  const float s = (s0 + s1) + (s2 + s3);
+  __shared__ float red[8][32];
+  const int c = threadIdx.x % 32, row = threadIdx.x / 32;
+  const long i = blockIdx.x * 32L + c;
+  float s = 0.f;
+  if (i < m)
+#pragma unroll 8
+    for (int r = row; r < rows; r += 8) s += part[r * m + i];
+  red[row][c] = s;
+  __syncthreads();
+  if (row || i >= m) return;
+  s = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s += red[r][c];
   if (i < dw_n)
     dw[i] = s;
   else if (db)
     db[i - dw_n] = s;
 }
 
-// Tokens of a run: long ones re-read fewer rows at their ends, as long as the runs fill the card.
-int run_of(long tokens) { return tokens >= 16384 ? 64 : tokens >= 2048 ? 16 : 8; }
+// Tokens of a run: long ones re-read fewer rows at their ends, as long as the blocks (of 4 runs
+// and 256 channels) fill the card.
+int run_of(long tokens, long D) {
+  int run = 128;
+  while (run > 8 && (D + 255) / 256 * (tokens / (4 * run)) < 1024) run /= 2;
+  return run;
+}
 
 template <typename T, int VEC, int W>
 hipError_t conv_launch(const tops_gla_conv_args& a, bool backward, hipStream_t st) {
   const long tokens = a.batch * a.T;
-  const int run = run_of(tokens);
+  const int run = run_of(tokens, a.D);
   const long tiles = (tokens + 4L * run - 1) / (4L * run);
   const unsigned gx = (unsigned)((a.D + CV_CX * VEC - 1) / (CV_CX * VEC));
   if (!backward) {
@@ -375,7 +381,7 @@ hipError_t conv_launch(const tops_gla_conv_args& a, bool backward, hipStream_t s
   }
   if (a.dw) {
     const long m = (W + 1) * a.D;
-    hipLaunchKernelGGL(conv_dw_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st,
+    hipLaunchKernelGGL(conv_dw_kernel, dim3((unsigned)((m + 31) / 32)), dim3(256), 0, st,
                        (const float*)a.ws, (int)tiles, m, W * a.D, a.dw, a.dbias);
     if (hipError_t e = hipGetLastError()) return e;
   }
@@ -401,8 +407,10 @@ bool rows_aligned(const tops_gla_conv_args& a, bool backward, int n) {
 
 template <typename T, int W>
 hipError_t conv_width(const tops_gla_conv_args& a, bool backward, hipStream_t st) {
-  // wide windows take half the channels: the backward holds 4 W + 2 rows of them in registers
-  constexpr int FULL = 16 / (int)sizeof(T), VEC = W <= 4 ? FULL : FULL / 2;
+  // 8 bytes of a row a thread: the backward holds 4 W + 2 rows in registers (with 16 bytes 256 of
+  // them, one wave a SIMD: 249 us against 178 for 32768 tokens of 4096 channels, bf16), and the
+  // forward of few tokens has more waves (8192 tokens, 2048 channels: 27 and 20 us)
+  constexpr int VEC = 8 / (int)sizeof(T);
   if (rows_aligned(a, backward, VEC)) return conv_launch<T, VEC, W>(a, backward, st);
   return conv_launch<T, 1, W>(a, backward, st);
 }
@@ -428,8 +436,8 @@ hipError_t conv_run(const tops_gla_conv_args& a, bool backward, hipStream_t st) 
 
 }  // namespace
 
-long causal_conv_part_rows(long tokens) {
-  const long per = 4L * run_of(tokens);
+long causal_conv_part_rows(long tokens, long D) {
+  const long per = 4L * run_of(tokens, D);
   return (tokens + per - 1) / per;
 }
 
