@@ -301,8 +301,7 @@ __global__ __launch_bounds__(QD_C * QD_R) void qk_dw_kernel(const float* part, i
 // 256 or 512 columns): the partner of a rotated piece comes from its lane, and the rows of the
 // next batch are on their way while one is computed.
 // ---------------------------------------------------------------------------
-constexpr int QK_U = 4;    // rows of a thread in a batch of the forward
-constexpr int QK_UB = 2;   // of the backward
+constexpr int QK_UB = 2;   // rows of a thread in a batch of the backward
 
 template <typename T, int VEC>
 struct Piece {
@@ -384,7 +383,7 @@ __device__ __forceinline__ void turn_piece(float (&x)[VEC], const float (&xp)[VE
 }
 
 // `magic[p]` = ceil(2^32 / heads of part p): row / heads = mulhi(row, magic) for row < 2^16.
-template <typename T, int VEC, int LPR, bool INTER>
+template <typename T, int VEC, int LPR, bool INTER, int QK_U>
 __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, int tb,
                                                             uint32_t magic_q, uint32_t magic_k) {
   extern __shared__ float2 cs[];
@@ -416,23 +415,25 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
       piece_load<T, VEC>(nx[u], src + off[tk][part] + (r - tk * H) * sh + cl);
     }
   };
+  float wv[VEC], wp[VEC];
+  auto weights = [&](int part) {
+    const float* w = part ? a.kw : a.qw;
+    const int pc = l.in ? l.pc(R) : 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      wv[e] = w ? w[cl + e] : 1.f;
+      wp[e] = w ? w[pc + e] : 1.f;
+    }
+  };
   if (nb > 0) load(0);
+  weights(nbq == 0);
   angles(a, tau0, nt, cs);
   __syncthreads();
   const float inv_d = 1.f / (float)D, eps = (float)a.eps;
-  float wv[VEC], wp[VEC];
 #pragma unroll 1
   for (int i = 0; i < nb; ++i) {
     const bool part = i >= nbq;
-    if (i == 0 || i == nbq) {
-      const float* w = part ? a.kw : a.qw;
-      const int pc = l.in ? l.pc(R) : 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        wv[e] = w ? w[cl + e] : 1.f;
-        wp[e] = w ? w[pc + e] : 1.f;
-      }
-    }
+    if (i == nbq && i > 0) weights(1);
     Piece<T, VEC> x[QK_U];
 #pragma unroll
     for (int u = 0; u < QK_U; ++u) x[u] = nx[u];
@@ -602,10 +603,16 @@ hipError_t qk_rows_launch(const tops_gla_qk_args& a, bool backward, int tb, long
   const dim3 nt(QK_NT);
   if (!backward) {
     const dim3 grid((unsigned)groups);
-    if (a.interleaved)
-      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, true>), grid, nt, lds, st, a, tb, mq, mk);
+    // four rows of a thread in a batch, one where a block has no more of them
+    const bool few = tb * std::max(a.Hq, a.Hk) <= 2 * (QK_NT / LPR);
+    if (a.interleaved && few)
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, true, 1>), grid, nt, lds, st, a, tb, mq, mk);
+    else if (a.interleaved)
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, true, 4>), grid, nt, lds, st, a, tb, mq, mk);
+    else if (few)
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, false, 1>), grid, nt, lds, st, a, tb, mq, mk);
     else
-      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, false>), grid, nt, lds, st, a, tb, mq, mk);
+      hipLaunchKernelGGL((qk_fwd_rows_kernel<T, VEC, LPR, false, 4>), grid, nt, lds, st, a, tb, mq, mk);
     return hipGetLastError();
   }
   const long blocks = std::min(groups, kQkBlocks);

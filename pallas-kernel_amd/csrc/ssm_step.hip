@@ -24,26 +24,68 @@ __device__ __forceinline__ float sum_adjacent(float x) {
   return x;
 }
 
+// Four elements at an address that is a multiple of theirs.
+__device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {
+  const float4 w = *reinterpret_cast<const float4*>(p);
+  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+}
+__device__ __forceinline__ void load_four(const bf16* p, float (&x)[4]) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
+}
+
 constexpr int ST_NT = 256;
 
 // LPR lanes hold a channel's states, four each: a wave reads and writes whole runs of the state.
-// A block takes `rows` rows of the batch, whose A it reads once.
-template <typename T, int LPR>
-__global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_args a, int rows,
-                                                          int cb, int vec) {
+// A block takes up to U rows of the batch, whose A it reads once and whose loads are all sent
+// before the first row is computed.
+template <typename T, int LPR, int U>
+__global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_args a, int cb,
+                                                          int vec, int vecbc) {
   const int q = threadIdx.x % LPR, n0 = 4 * q;
   const int d = blockIdx.x % cb * (ST_NT / LPR) + threadIdx.x / LPR;
-  const int b0 = blockIdx.x / cb * rows;
+  const int b0 = blockIdx.x / cb * U;
   const int D = (int)a.D, N = (int)a.N;
   const bool live = d < D;
   const int dd = live ? d : 0;
-  const int grp = dd / (D / (int)a.G);
+  const int grp = a.G == 1 ? 0 : dd / (D / (int)a.G);
   const int nn = live ? min(4, N - n0) : 0;   // valid states of the lane
-  const bool v4 = vec && nn == 4;
-  float A[4] = {};
+  const bool v4 = vec && nn == 4, v4bc = vecbc && nn == 4;
+  const int rows = min(U, (int)a.batch - b0);
+  float h[U][4], u[U], dt[U], z[U], B[U][4], C[U][4];
+  float* s[U];
+  bool there[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int b = b0 + min(k, rows - 1);
+    const long slot = slot_of(a.slots_idx, a.idx64, b);
+    there[k] = k < rows && slot >= 0 && slot < a.slots;
+    s[k] = a.state + (there[k] ? slot : 0) * a.state_ss + (long)dd * N + n0;
+    u[k] = to_f32(((const T*)a.u)[b * a.u_sb + dd]);
+    dt[k] = to_f32(((const T*)a.delta)[b * a.delta_sb + dd]);
+    z[k] = a.z ? to_f32(((const T*)a.z)[b * a.z_sb + dd]) : 0.f;
+    const T* Bp = (const T*)a.B + b * a.B_sb + grp * a.B_sg + n0;
+    const T* Cp = (const T*)a.C + b * a.C_sb + grp * a.C_sg + n0;
+    if (v4bc) {
+      load_four(Bp, B[k]);
+      load_four(Cp, C[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        B[k][i] = i < nn ? to_f32(Bp[i]) : 0.f;
+        C[k][i] = i < nn ? to_f32(Cp[i]) : 0.f;
+      }
+    }
+    if (a.slots > 0 && v4) {   // slot 0 in the place of one that is not there
+      load_four((const float*)s[k], h[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[k][i] = a.slots > 0 && i < nn ? s[k][i] : 0.f;
+    }
+  }
+  float A[4];
   if (v4) {
-    const float4 w = *reinterpret_cast<const float4*>(a.A + (long)dd * N + n0);
-    A[0] = w.x, A[1] = w.y, A[2] = w.z, A[3] = w.w;
+    load_four(a.A + (long)dd * N + n0, A);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) A[i] = i < nn ? a.A[(long)dd * N + n0 + i] : 0.f;
@@ -52,127 +94,141 @@ __global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_arg
   for (int i = 0; i < 4; ++i) A[i] *= 1.4426950408889634f;
   const float bias = a.delta_bias ? a.delta_bias[dd] : 0.f;
   const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
-  const int b1 = min((int)a.batch, b0 + rows);
-  for (int b = b0; b < b1; ++b) {
-    const long slot = slot_of(a.slots_idx, a.idx64, b);
-    const bool there = slot >= 0 && slot < a.slots;
-    float y = 0.f, h[4] = {};
-    float* s = a.state + (there ? slot : 0) * a.state_ss + (long)dd * N + n0;
-    if (there) {
-      if (v4) {
-        const float4 w = *reinterpret_cast<const float4*>(s);
-        h[0] = w.x, h[1] = w.y, h[2] = w.z, h[3] = w.w;
-      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = i < nn ? s[i] : 0.f;
-      }
-    }
-    const float u = to_f32(((const T*)a.u)[b * a.u_sb + dd]);
-    float dt = to_f32(((const T*)a.delta)[b * a.delta_sb + dd]) + bias, sg;
-    const float z = a.z ? to_f32(((const T*)a.z)[b * a.z_sb + dd]) : 0.f;
-    const T* Bp = (const T*)a.B + b * a.B_sb + grp * a.B_sg + n0;
-    const T* Cp = (const T*)a.C + b * a.C_sb + grp * a.C_sg + n0;
-    float Bv[4], Cv[4];
+  for (int k = 0; k < U; ++k) {
+    float t = dt[k] + bias, sg, y = 0.f;
+    if (a.softplus) softplus_sigmoid(t, t, sg);
+    const float du = t * u[k];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      Bv[i] = i < nn ? to_f32(Bp[i]) : 0.f;
-      Cv[i] = i < nn ? to_f32(Cp[i]) : 0.f;
+      h[k][i] = fmaf(__builtin_amdgcn_exp2f(A[i] * t), h[k][i], du * B[k][i]);
+      y = fmaf(C[k][i], h[k][i], y);
     }
-    if (a.softplus) softplus_sigmoid(dt, dt, sg);
-    const float du = dt * u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = fmaf(__builtin_amdgcn_exp2f(A[i] * dt), h[i], du * Bv[i]);
-      y = fmaf(Cv[i], h[i], y);
-    }
-    if (there) {
+    if (there[k]) {
       if (v4) {
-        *reinterpret_cast<float4*>(s) = make_float4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<float4*>(s[k]) = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < nn) s[i] = h[i];
+          if (i < nn) s[k][i] = h[k][i];
       }
     }
     y = sum_adjacent<LPR>(nn > 0 ? y : 0.f);
-    if (q == 0 && live) {
-      y = fmaf(skip, u, y);
-      if (a.z) y *= z * sigmoid(z);
-      ((T*)a.y)[(long)b * D + d] = from_f32<T>(there ? y : 0.f);
+    if (q == 0 && live && k < rows) {
+      y = fmaf(skip, u[k], y);
+      if (a.z) y *= z[k] * sigmoid(z[k]);
+      ((T*)a.y)[(long)(b0 + k) * D + d] = from_f32<T>(there[k] ? y : 0.f);
     }
   }
+}
+
+template <typename T, int LPR>
+hipError_t scan_step_lanes(const tops_gla_scan_step_args& a, int vec, int vecbc, hipStream_t st) {
+  const int cb = (int)((a.D + ST_NT / LPR - 1) / (ST_NT / LPR));
+  // four rows a block as long as the blocks fill the device
+  if (cb * ((a.batch + 3) / 4) >= 1024)
+    hipLaunchKernelGGL((scan_step_kernel<T, LPR, 4>), dim3((unsigned)(cb * ((a.batch + 3) / 4))),
+                       dim3(ST_NT), 0, st, a, cb, vec, vecbc);
+  else
+    hipLaunchKernelGGL((scan_step_kernel<T, LPR, 1>), dim3((unsigned)(cb * a.batch)), dim3(ST_NT), 0,
+                       st, a, cb, vec, vecbc);
+  return hipGetLastError();
 }
 
 template <typename T>
 hipError_t scan_step(const tops_gla_scan_step_args& a, hipStream_t st) {
-  const int N = (int)a.N;
+  const int N = (int)a.N, es = (int)sizeof(T);
   const int vec = N % 4 == 0 && a.state_ss % 4 == 0 && ((uintptr_t)a.state & 15) == 0 &&
                   ((uintptr_t)a.A & 15) == 0;
-  const int lpr = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
-  const int cb = (int)((a.D + ST_NT / lpr - 1) / (ST_NT / lpr));
-  // rows of a block: A is read once for all of them, as long as the blocks fill the device
-  int rows = 1;
-  while (rows < 8 && (long)cb * ((a.batch + 2 * rows - 1) / (2 * rows)) >= 2048) rows *= 2;
-  const dim3 grid((unsigned)(cb * ((a.batch + rows - 1) / rows)));
-  switch (lpr) {
-    case 1: hipLaunchKernelGGL((scan_step_kernel<T, 1>), grid, dim3(ST_NT), 0, st, a, rows, cb, vec); break;
-    case 2: hipLaunchKernelGGL((scan_step_kernel<T, 2>), grid, dim3(ST_NT), 0, st, a, rows, cb, vec); break;
-    case 4: hipLaunchKernelGGL((scan_step_kernel<T, 4>), grid, dim3(ST_NT), 0, st, a, rows, cb, vec); break;
-    case 8: hipLaunchKernelGGL((scan_step_kernel<T, 8>), grid, dim3(ST_NT), 0, st, a, rows, cb, vec); break;
-    default: hipLaunchKernelGGL((scan_step_kernel<T, 16>), grid, dim3(ST_NT), 0, st, a, rows, cb, vec);
-  }
-  return hipGetLastError();
+  const int vecbc = a.B_sb % 4 == 0 && a.C_sb % 4 == 0 && a.B_sg % 4 == 0 && a.C_sg % 4 == 0 &&
+                    ((uintptr_t)a.B & (4 * es - 1)) == 0 && ((uintptr_t)a.C & (4 * es - 1)) == 0;
+  if (N <= 4) return scan_step_lanes<T, 1>(a, vec, vecbc, st);
+  if (N <= 8) return scan_step_lanes<T, 2>(a, vec, vecbc, st);
+  if (N <= 16) return scan_step_lanes<T, 4>(a, vec, vecbc, st);
+  if (N <= 32) return scan_step_lanes<T, 8>(a, vec, vecbc, st);
+  return scan_step_lanes<T, 16>(a, vec, vecbc, st);
 }
 
 // One thread per (row, VEC channels): the window moves up a row in place.
-template <typename T, typename TW, int VEC>
+template <typename T, typename TW, int VEC, int W>
 __global__ __launch_bounds__(ST_NT) void conv_step_kernel(tops_gla_conv_step_args a, int cb) {
-  const int D = (int)a.D, W = (int)a.W;
+  const int D = (int)a.D;
   const int c = (blockIdx.x % cb * ST_NT + threadIdx.x) * VEC, b = blockIdx.x / cb;
   if (c >= D) return;
-  const long slot = slot_of(a.slots_idx, a.idx64, b);
-  const bool there = slot >= 0 && slot < a.slots;
-  float y[VEC] = {};
-  if (there) {
-    T* s = (T*)a.state + slot * a.state_ss + c;
-    const TW* w = (const TW*)a.w + (long)c * W;
+  struct alignas(VEC * sizeof(T)) Raw { T v[VEC]; };
+  const Raw x = *reinterpret_cast<const Raw*>((const T*)a.x + b * a.x_sb + c);
+  float w[VEC * W], y[VEC] = {};
+  const TW* wp = (const TW*)a.w + (long)c * W;
+  if constexpr (VEC == 4) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) y[e] = a.bias ? to_f32(((const TW*)a.bias)[c + e]) : 0.f;
-    struct alignas(VEC * sizeof(T)) Raw { T v[VEC]; };
-    Raw r[8];
-    const Raw x = *reinterpret_cast<const Raw*>((const T*)a.x + b * a.x_sb + c);
+    for (int j = 0; j < W; ++j) {
+      float four[4];
+      load_four(wp + 4 * j, four);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)   // the row that moves to j
-      if (j < W) r[j] = j == W - 1 ? x : *reinterpret_cast<const Raw*>(s + (long)(j + 1) * D);
+      for (int e = 0; e < 4; ++e) w[4 * j + e] = four[e];
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < W) {
-        *reinterpret_cast<Raw*>(s + (long)j * D) = r[j];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) y[e] = fmaf(to_f32(w[e * W + j]), to_f32(r[j].v[e]), y[e]);
-      }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (a.silu) y[e] *= sigmoid(y[e]);
+    for (int j = 0; j < VEC * W; ++j) w[j] = to_f32(wp[j]);
   }
+  if (a.bias)
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) ((T*)a.y)[(long)b * D + c + e] = from_f32<T>(y[e]);
+    for (int e = 0; e < VEC; ++e) y[e] = to_f32(((const TW*)a.bias)[c + e]);
+  const long slot = slot_of(a.slots_idx, a.idx64, b);
+  if (slot >= 0 && slot < a.slots) {
+    T* s = (T*)a.state + slot * a.state_ss + c;
+    Raw r[W];   // the rows that move to 0 .. W - 1
+#pragma unroll
+    for (int j = 0; j + 1 < W; ++j) r[j] = *reinterpret_cast<const Raw*>(s + (long)(j + 1) * D);
+    r[W - 1] = x;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      *reinterpret_cast<Raw*>(s + (long)j * D) = r[j];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = fmaf(w[e * W + j], to_f32(r[j].v[e]), y[e]);
+    }
+    if (a.silu)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] *= sigmoid(y[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = 0.f;
+  }
+  Raw o;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(y[e]);
+  *reinterpret_cast<Raw*>((T*)a.y + (long)b * D + c) = o;
 }
 
-template <typename T, typename TW>
-hipError_t conv_step(const tops_gla_conv_step_args& a, hipStream_t st) {
+template <typename T, typename TW, int W>
+hipError_t conv_step_width(const tops_gla_conv_step_args& a, hipStream_t st) {
   // four channels a thread where the rows allow it (a step has few threads to begin with)
+  const auto at = [](const void* p, size_t by) { return ((uintptr_t)p & (by - 1)) == 0; };
   const bool vec = a.D % 4 == 0 && a.x_sb % 4 == 0 && a.state_ss % 4 == 0 &&
-                   ((uintptr_t)a.x & (4 * sizeof(T) - 1)) == 0 &&
-                   ((uintptr_t)a.state & (4 * sizeof(T) - 1)) == 0;
+                   at(a.x, 4 * sizeof(T)) && at(a.state, 4 * sizeof(T)) && at(a.y, 4 * sizeof(T)) &&
+                   at(a.w, 4 * sizeof(TW));
   const long per = vec ? 4 : 1;
   const int cb = (int)((a.D + ST_NT * per - 1) / (ST_NT * per));
   const dim3 grid((unsigned)(cb * a.batch));
   if (vec)
-    hipLaunchKernelGGL((conv_step_kernel<T, TW, 4>), grid, dim3(ST_NT), 0, st, a, cb);
+    hipLaunchKernelGGL((conv_step_kernel<T, TW, 4, W>), grid, dim3(ST_NT), 0, st, a, cb);
   else
-    hipLaunchKernelGGL((conv_step_kernel<T, TW, 1>), grid, dim3(ST_NT), 0, st, a, cb);
+    hipLaunchKernelGGL((conv_step_kernel<T, TW, 1, W>), grid, dim3(ST_NT), 0, st, a, cb);
   return hipGetLastError();
+}
+
+template <typename T, typename TW>
+hipError_t conv_step(const tops_gla_conv_step_args& a, hipStream_t st) {
+  switch (a.W) {
+    case 1: return conv_step_width<T, TW, 1>(a, st);
+    case 2: return conv_step_width<T, TW, 2>(a, st);
+    case 3: return conv_step_width<T, TW, 3>(a, st);
+    case 4: return conv_step_width<T, TW, 4>(a, st);
+    case 5: return conv_step_width<T, TW, 5>(a, st);
+    case 6: return conv_step_width<T, TW, 6>(a, st);
+    case 7: return conv_step_width<T, TW, 7>(a, st);
+    default: return conv_step_width<T, TW, 8>(a, st);
+  }
 }
 
 }  // namespace
