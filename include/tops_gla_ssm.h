@@ -107,15 +107,15 @@ int tops_gla_selective_scan_step(const tops_gla_scan_step_args *a, void *stream)
  */
 typedef struct tops_gla_conv_args {
   const void *x;                  /* [B, T, D] */
-  const float *w, *bias;          /* [D, W], [D] or NULL */
+  const void *w, *bias;           /* [D, W], [D] or NULL, of type w_dtype */
   const void *init;               /* [sequences, W, D] or NULL */
   void *y, *final_state;          /* final_state NULL: not wanted */
   const int32_t *cu;
-  int64_t nseq, batch, T, D, W, x_sb, x_st, silu, dtype;
+  int64_t nseq, batch, T, D, W, x_sb, x_st, silu, dtype, w_dtype;
   /* backward only */
   const void *dy, *dfinal;        /* dfinal [sequences, W, D] or NULL */
   void *dx, *dinit;               /* dinit [sequences, W, D] or NULL */
-  float *dw, *dbias;              /* [D, W], [D]; both or neither */
+  void *dw, *dbias;               /* [D, W], [D] of type w_dtype; dbias only with dw */
   void *ws;                       /* with dw: tops_gla_causal_conv_bwd_ws_bytes */
   int64_t ws_bytes, dy_sb, dy_st;
 } tops_gla_conv_args;

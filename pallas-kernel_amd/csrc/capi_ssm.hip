@@ -125,7 +125,7 @@ int slots_ok(int64_t batch, int64_t slots, const void* idx) {
 
 int conv_check(const tops_gla_conv_args* a) {
   if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
-  if (!dtype_ok(a->dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (!dtype_ok(a->dtype) || !dtype_ok(a->w_dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
   if (a->D < 1 || a->D > (1 << 20))
     return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)", (long long)a->D);
   if (a->W < 1 || a->W > 8)

@@ -40,6 +40,16 @@ long causal_conv_part_rows(long tokens, long D);   // rows of (W + 1) D partial 
 hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_t st);
 long qk_norm_rope_part_rows(long tokens);  // rows of 2 D partial weight gradients
 
+// Four elements at an address that is a multiple of theirs.
+__device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {
+  const float4 w = *reinterpret_cast<const float4*>(p);
+  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+}
+__device__ __forceinline__ void load_four(const bf16* p, float (&x)[4]) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
+}
+
 // Value of a lane of the same row of 16 (CTRL: 0x120 + r rotates right by r).
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {

@@ -79,15 +79,32 @@ __device__ __forceinline__ void head(const tops_gla_conv_args& a, int s, long bo
   }
 }
 
+template <typename TW, int VEC, int W>
+__device__ __forceinline__ void weights_of(const TW* w0, const TW* b0, int c, float (&w)[W][VEC],
+                                           float (&b)[VEC]) {
+  float x[VEC * W];
+  const TW* p = w0 + (long)c * W;
+  if (VEC == 4 && (uintptr_t)w0 % (4 * sizeof(TW)) == 0) {
+#pragma unroll
+    for (int j = 0; j + 3 < VEC * W; j += 4) load_four(p + j, reinterpret_cast<float(&)[4]>(x[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC * W; ++j) x[j] = to_f32(p[j]);
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    b[e] = b0 ? to_f32(b0[c + e]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][e] = x[e * W + j];
+  }
+}
 template <int VEC, int W>
 __device__ __forceinline__ void weights(const tops_gla_conv_args& a, int c, float (&w)[W][VEC],
                                         float (&b)[VEC]) {
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    b[e] = a.bias ? a.bias[c + e] : 0.f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j][e] = a.w[(long)(c + e) * W + j];
-  }
+  if (a.w_dtype == DT_BF16)
+    weights_of<bf16, VEC, W>((const bf16*)a.w, (const bf16*)a.bias, c, w, b);
+  else
+    weights_of<float, VEC, W>((const float*)a.w, (const float*)a.bias, c, w, b);
 }
 
 template <int VEC, int W>
@@ -333,7 +350,8 @@ __global__ __launch_bounds__(CV_NT) void conv_dinit_kernel(tops_gla_conv_args a,
 
 // The summed rows [D][W], [D] to the two outputs, 8 threads a column.
 __global__ __launch_bounds__(256) void conv_dw_kernel(const float* __restrict__ part, int rows,
-                                                      long m, long dw_n, float* dw, float* db) {
+                                                      long m, long dw_n, void* dw, void* db,
+                                                      int bf) {
   __shared__ float red[8][32];
   const int c = threadIdx.x % 32, row = threadIdx.x / 32;
   const long i = blockIdx.x * 32L + c;
@@ -347,10 +365,12 @@ __global__ __launch_bounds__(256) void conv_dw_kernel(const float* __restrict__ 
   s = 0.f;
 #pragma unroll
   for (int r = 0; r < 8; ++r) s += red[r][c];
-  if (i < dw_n)
-    dw[i] = s;
-  else if (db)
-    db[i - dw_n] = s;
+  void* out = i < dw_n ? dw : db;
+  const long at = i < dw_n ? i : i - dw_n;
+  if (out && bf)
+    ((bf16*)out)[at] = from_f32<bf16>(s);
+  else if (out)
+    ((float*)out)[at] = s;
 }
 
 // Tokens of a run: long ones re-read fewer rows at their ends, as long as the blocks (of 4 runs
@@ -382,7 +402,8 @@ hipError_t conv_launch(const tops_gla_conv_args& a, bool backward, hipStream_t s
   if (a.dw) {
     const long m = (W + 1) * a.D;
     hipLaunchKernelGGL(conv_dw_kernel, dim3((unsigned)((m + 31) / 32)), dim3(256), 0, st,
-                       (const float*)a.ws, (int)tiles, m, W * a.D, a.dw, a.dbias);
+                       (const float*)a.ws, (int)tiles, m, W * a.D, a.dw, a.dbias,
+                       (int)(a.w_dtype == DT_BF16));
     if (hipError_t e = hipGetLastError()) return e;
   }
   if (a.dinit && a.nseq > 0) {

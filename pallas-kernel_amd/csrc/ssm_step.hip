@@ -24,16 +24,6 @@ __device__ __forceinline__ float sum_adjacent(float x) {
   return x;
 }
 
-// Four elements at an address that is a multiple of theirs.
-__device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {
-  const float4 w = *reinterpret_cast<const float4*>(p);
-  x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-}
-__device__ __forceinline__ void load_four(const bf16* p, float (&x)[4]) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
-}
-
 constexpr int ST_NT = 256;
 
 // LPR lanes hold a channel's states, four each: a wave reads and writes whole runs of the state.

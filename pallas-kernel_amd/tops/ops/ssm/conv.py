@@ -10,10 +10,10 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, device_table, differentiable, f32, gradients, io_dtype, offsets, refuse_grad, rows,
-                      slot_args, strides)
+from ._common import (address, device_table, differentiable, gradients, io_dtype, offsets,
+                      refuse_grad, rows, slot_args, strides)
 
-_ARGS = struct.Struct("=26q")
+_ARGS = struct.Struct("=27q")
 _STEP = struct.Struct("=16q")
 
 def _cu_tensor(cu, device):
@@ -38,7 +38,7 @@ def _pack(x, y, fin, cu_t, nseq, silu, bwd=None):
     B, T, D = xx.shape
     return _ARGS.pack(address(xx), address(w), address(b), address(init), address(y),
                       address(fin), address(cu_t), nseq, B, T, D, w.shape[1], *strides(xx, 0, 1),
-                      int(silu), dtype_code(xx.dtype), *(bwd or [0] * 10))
+                      int(silu), dtype_code(xx.dtype), dtype_code(w.dtype), *(bwd or [0] * 10))
 
 
 def _forward(x, weight, bias, init, silu, want, cu):
@@ -46,7 +46,9 @@ def _forward(x, weight, bias, init, silu, want, cu):
     dt = io_dtype(x)
     B, T, D = x.shape
     W = weight.shape[-1]
-    a = (rows(x, dt), f32(weight.reshape(D, W)), f32(bias), _contiguous(init, dt))
+    wt = io_dtype(weight, bias)
+    a = (rows(x, dt), _contiguous(weight if weight.dim() == 2 else weight.reshape(D, W), wt),
+         _contiguous(bias, wt), _contiguous(init, dt))
     nseq = B if cu is None else len(cu) - 1
     cu_t = _cu_tensor(cu, dev)
     y = torch.empty(B, T, D, dtype=dt, device=dev)
@@ -81,15 +83,15 @@ class _CausalConvFunction(torch.autograd.Function):
         dw = db = ws = None
         nws = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw = torch.empty(D, W, dtype=torch.float32, device=dev)
-            db = torch.empty(D, dtype=torch.float32, device=dev)
+            dw = torch.empty(D, W, dtype=w.dtype, device=dev)
+            db = None if b is None else torch.empty(D, dtype=w.dtype, device=dev)
             nws = int(_lib.load().tops_gla_causal_conv_bwd_ws_bytes(B * T, D, W))
             ws = torch.empty(nws, dtype=torch.uint8, device=dev)
         bwd = [*(address(t) for t in (dy, dfin, dx, dinit, dw, db, ws)), nws, *strides(dy, 0, 1)]
         call("tops_gla_causal_conv_bwd", _pack((x, w, b, init), None, None, cu_t, ctx.nseq,
                                                ctx.silu, bwd), stream_of(dev))
-        return (*gradients((dx, dw, None if ctx.like[2] is None else db, dinit), ctx.like,
-                           ctx.needs_input_grad), None, None, None)
+        return (*gradients((dx, dw, db, dinit), ctx.like, ctx.needs_input_grad), None, None,
+                None)
 
 
 def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None,
