@@ -10,6 +10,8 @@
 // Pieces: h_t = a_t h_{t-1} + b_t is linear, so a sequence is cut into pieces that run in
 // parallel. A first pass finds each piece's state from zero (L) and its summed delta' (S), a
 // small one folds them in order, h <- exp(A S_j) h + L_j, and leaves every piece's entry state.
+#include <type_traits>
+
 #include "common.hpp"
 #include "ssm.hpp"
 
@@ -380,6 +382,24 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p, int nb
 // states each. They share what is formed once for a (token, channel) through LDS: each wave
 // stages 8 / NW of the tile's tokens and, once the waves' sums over n are there, finishes them.
 // ---------------------------------------------------------------------------
+constexpr int HK = SS_K / 2;
+// Steps 0 .. 5 HK - 1 of a tile: forward to its middle; the second half forward, and back; the
+// first half forward, and back. The token of a step, and whether it goes back.
+constexpr bool is_back(int e) { return e / HK == 2 || e / HK == 4; }
+constexpr int token_of(int e) {
+  return e < 2 * HK   ? e
+         : e < 3 * HK ? 4 * HK - 1 - e
+         : e < 4 * HK ? e - 3 * HK
+                      : 5 * HK - 1 - e;
+}
+template <int I, int N, typename F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<I + 1, N>(f);
+  }
+}
+
 template <int NP>
 struct Bwd {
   static constexpr int NW = NP / 8;                // waves of a channel group
@@ -417,9 +437,10 @@ __device__ __forceinline__ float sum_channels(float (&x)[8], float (&y)[8]) {
 }
 
 template <typename T, int NP>
-__global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanParams p) {
+__global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd_kernel(ScanParams p) {
   using L = Bwd<NP>;
   __shared__ float sD[SS_K][L::CT], sU[SS_K][L::CT], sG[SS_K][L::CT];   // delta', u, dy silu(z)
+  __shared__ float sK[2][SS_K][L::CT];          // softplus', dy silu'(z): for the wave that staged them
   __shared__ float sS[L::NW][3][SS_K][L::CT];   // sum_n g B, sum_n g a h A log2(e), sum_n C h
   __shared__ float sBC[L::GPB][SS_K][2 * NP];   // a channel group's dB and dC
   const tops_gla_scan_args& a = p.a;
@@ -475,98 +496,102 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
 #pragma unroll 1
   for (int k = nt - 1; k >= 0; --k) {
     const int t0 = pc.t0 + k * SS_K, ts = part * L::TPW;
-    float ks[L::TPW], kz[L::TPW], ky[L::TPW];
 #pragma unroll
     for (int i = 0; i < L::TPW; ++i) {
       const bool in = live && t0 + ts + i < pc.t1;
       float d = to_f32(rd[i]) + bias, sg = 1.f;
       if (softplus) softplus_sigmoid(d, d, sg);
-      ks[i] = sg;
-      ky[i] = to_f32(ry[i]);
-      kz[i] = has_z ? to_f32(rz[i]) : 0.f;
-      const float g = has_z ? ky[i] * kz[i] * sigmoid(kz[i]) : ky[i];
+      const float dy = to_f32(ry[i]), z = has_z ? to_f32(rz[i]) : 0.f;
+      const float sz = sigmoid(z), g = has_z ? dy * z * sz : dy;
+      sK[0][ts + i][col] = sg;
+      sK[1][ts + i][col] = dy * (sz * fmaf(z, 1.f - sz, 1.f));   // dy silu'(z)
       sD[ts + i][col] = in ? d : 0.f;
       sU[ts + i][col] = in ? to_f32(ru[i]) : 0.f;
       sG[ts + i][col] = in ? g : 0.f;
     }
-    float av[SS_K][8], hv[SS_K][8], hin[8];
+    float hin[8], hm[8];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) hin[n] = live ? rh[n] : 0.f;
+    for (int n = 0; n < 8; ++n) hin[n] = hm[n] = live ? rh[n] : 0.f;
+    // Three sweeps over four tokens at a time: the first half's states forward without keeping
+    // them, then each half, the second one first, forward with a_t and h_t in registers and back.
     // The rows of a token are fetched while the one before it is computed: B and C into scalar
     // registers, delta', u and dy from LDS. One counter stands for both kinds of loads, and the
     // scalar ones come in any order: a wait has to be for all of them, before the next are sent.
-    const float* q = bc + t0 * bc_st;
-    float nb[8], nc[8];
-    load_row(row_after(q, hin), nb);
+    const float* rows = bc + t0 * bc_st;
+    float nb[8], nc[8], nd, nu, ng, av[HK][8], hv[HK][8];
+    load_row(row_after(rows, hin), nb);
     __syncthreads();
-    if (k > 0) load(k - 1);
-    float nd = sD[0][col], nu = sU[0][col], ng;
-#pragma unroll
-    for (int t = 0; t < SS_K; ++t) {
-      float rb[8];
-      arrived(nb);
-      asm volatile("" : "+v"(nd), "+v"(nu));
-#pragma unroll
-      for (int n = 0; n < 8; ++n) rb[n] = nb[n];
-      const float d = nd, x = d * nu;
-      if (t < SS_K - 1) q += bc_st;
-      cfloat* row = row_after(t0 + min(t + 1, SS_K - 1) < pc.t1 ? q : bc_end,
-                              t ? hv[t - 1] : hin);
-      load_row(row, nb);
-      if (t < SS_K - 1) {
-        nd = sD[t + 1][col];
-        nu = sU[t + 1][col];
-      } else {
-        load_row(row + NP, nc);
-        ng = sG[t][col];
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        av[t][n] = exp2_hw(A[n] * d);
-        hv[t][n] = fmaf(av[t][n], t ? hv[t - 1][n] : hin[n], x * rb[n]);
-      }
-    }
-#pragma unroll
-    for (int t = SS_K - 1; t >= 0; --t) {
+    nd = sD[0][col];
+    nu = sU[0][col];
+    static_for<0, 5 * HK>([&](auto step) {
+      constexpr int e = decltype(step)::value, sweep = e / HK;
+      constexpr bool back = is_back(e), nback = is_back(e + 1);
+      constexpr int t = token_of(e), tn = token_of(e + 1), s = t % HK;
+      float(&h0)[8] = sweep < 3 ? hm : hin;
       float rb[8], rc[8];
       arrived(nb);
-      arrived(nc);
-      asm volatile("" : "+v"(nd), "+v"(nu), "+v"(ng));
+      asm volatile("" : "+v"(nd), "+v"(nu));
+      if constexpr (back) {
+        arrived(nc);
+        asm volatile("" : "+v"(ng));
+      }
 #pragma unroll
-      for (int n = 0; n < 8; ++n) rb[n] = nb[n], rc[n] = nc[n];
+      for (int n = 0; n < 8; ++n) rb[n] = nb[n], rc[n] = back ? nc[n] : 0.f;
       const float d = nd, x = d * nu, dy = ng;
-      if (t > 0) {
-        q -= bc_st;
-        cfloat* row = row_after(t0 + t - 1 < pc.t1 ? q : bc_end, t < SS_K - 1 ? carry : hv[t]);
+      if constexpr (e + 1 < 5 * HK) {
+        const float* at = t0 + tn < pc.t1 ? rows + tn * bc_st : bc_end;
+        cfloat* row;
+        if constexpr (back)
+          row = row_after(at, carry);
+        else if constexpr (sweep == 0 || s == 0)
+          row = row_after(at, h0);
+        else
+          row = row_after(at, hv[s - 1]);
         load_row(row, nb);
-        load_row(row + NP, nc);
-        nd = sD[t - 1][col];
-        nu = sU[t - 1][col];
-        ng = sG[t - 1][col];
+        if (nback) load_row(row + NP, nc);
+        nd = sD[tn][col];
+        nu = sU[tn][col];
+        if (nback) ng = sG[tn][col];
       }
-      float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      if (e == 3 * HK && k > 0) load(k - 1);
+      if constexpr (sweep == 0) {
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float g = fmaf(dy, rc[n], carry[n]);
-        const float hp = t ? hv[t - 1][n] : hin[n];
-        vb[n] = g * x;
-        vc[n] = dy * hv[t][n];
-        s1 = fmaf(g, rb[n], s1);
-        carry[n] = av[t][n] * g;
-        const float gp = carry[n] * hp;
-        s2 = fmaf(gp, A[n], s2);
-        s3 = fmaf(hv[t][n], rc[n], s3);
-        dA[n] = fmaf(gp, d, dA[n]);
+        for (int n = 0; n < 8; ++n) hm[n] = fmaf(exp2_hw(A[n] * d), hm[n], x * rb[n]);
+      } else if constexpr (!back) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          av[s][n] = exp2_hw(A[n] * d);
+          if constexpr (s > 0)
+            hv[s][n] = fmaf(av[s][n], hv[s - 1][n], x * rb[n]);
+          else
+            hv[s][n] = fmaf(av[s][n], h0[n], x * rb[n]);
+        }
+      } else {
+        float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const float g = fmaf(dy, rc[n], carry[n]);
+          float hp = h0[n];
+          if constexpr (s > 0) hp = hv[s - 1][n];
+          vb[n] = g * x;
+          vc[n] = dy * hv[s][n];
+          s1 = fmaf(g, rb[n], s1);
+          carry[n] = av[s][n] * g;
+          const float gp = carry[n] * hp;
+          s2 = fmaf(gp, A[n], s2);
+          s3 = fmaf(hv[s][n], rc[n], s3);
+          dA[n] = fmaf(gp, d, dA[n]);
+        }
+        pin(dA);
+        sS[part][0][t][col] = s1;
+        sS[part][1][t][col] = s2;
+        sS[part][2][t][col] = s3;
+        const float r = sum_channels(vb, vc);
+        if ((lane & 3) == 0)
+          sBC[cg][t][(lane & 8 ? NP : 0) + n0 + (lane & 4) + ((lane >> 3) & 2) + (lane >> 5)] = r;
+        fence();
       }
-      pin(dA);
-      sS[part][0][t][col] = s1;
-      sS[part][1][t][col] = s2;
-      sS[part][2][t][col] = s3;
-      const float r = sum_channels(vb, vc);
-      if ((lane & 3) == 0)
-        sBC[cg][t][(lane & 8 ? NP : 0) + n0 + (lane & 4) + ((lane >> 3) & 2) + (lane >> 5)] = r;
-      fence();
-    }
+    });
     __syncthreads();
     const long o = (pc.b * a.T + t0 + ts) * D + d0;
     T *odu = (T*)a.du + o, *odd = (T*)a.ddelta + o, *odz = (T*)a.dz + o;
@@ -581,9 +606,8 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, 2) void scan_bwd_kernel(ScanPa
         s3 += sS[w][2][t][col];
       }
       const float d = sD[t][col], u = sU[t][col], dy = sG[t][col];
-      const float du = fmaf(s1, d, skip * dy), dd = fmaf(s1, u, s2 * kLn2) * ks[i];
-      const float sz = sigmoid(kz[i]);
-      const float dz = ky[i] * fmaf(skip, u, s3) * (sz * fmaf(kz[i], 1.f - sz, 1.f));
+      const float du = fmaf(s1, d, skip * dy), dd = fmaf(s1, u, s2 * kLn2) * sK[0][t][col];
+      const float dz = sK[1][t][col] * fmaf(skip, u, s3);
       if (live && t0 + t < pc.t1) {
         accD = fmaf(dy, u, accD);
         accB += dd;
