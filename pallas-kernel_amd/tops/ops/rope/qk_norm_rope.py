@@ -101,24 +101,24 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, inv_freq=None, positions=No
 
     Differentiable in q, k and the weights. Returns ``(q', k')`` in the inputs' types, contiguous.
     """
-    require(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2]
-            and q.shape[3] == k.shape[3] and 1 <= q.shape[3] <= 512,
-            f"q and k must be [B, T, heads, D] with one D <= 512, got {tuple(q.shape)} and "
-            f"{tuple(k.shape)}")
+    if (q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]
+            or not 1 <= q.shape[3] <= 512):
+        require(False, f"q and k must be [B, T, heads, D] with one D <= 512, got "
+                       f"{tuple(q.shape)} and {tuple(k.shape)}")
     B, T, _, D = q.shape
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        require(w is None or tuple(w.shape) == (D,), f"{name} must be {(D,)}")
+        if w is not None and w.shape != (D,):
+            require(False, f"{name} must be {(D,)}, got {tuple(w.shape)}")
     if inv_freq is not None:
-        require(inv_freq.dim() == 1 and 2 * inv_freq.shape[0] <= D
-                and inv_freq.dtype == torch.float64,
-                f"inv_freq must be float64 [R / 2] with R <= {D}, got {inv_freq.dtype} "
-                f"{tuple(inv_freq.shape)}")
+        if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > D or inv_freq.dtype is not torch.float64:
+            require(False, f"inv_freq must be float64 [R / 2] with R <= {D}, got "
+                           f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
         inv_freq = inv_freq.contiguous()
     if positions is not None:
-        require(positions.dtype in (torch.int32, torch.int64)
-                and tuple(positions.shape) in ((B, T), (T,)),
-                f"positions must be int32 or int64 {(B, T)} or {(T,)}, got {positions.dtype} "
-                f"{tuple(positions.shape)}")
+        if (positions.dtype not in (torch.int32, torch.int64)
+                or positions.shape not in ((B, T), (T,))):
+            require(False, f"positions must be int32 or int64 {(B, T)} or {(T,)}, got "
+                           f"{positions.dtype} {tuple(positions.shape)}")
         if positions.shape[-1] > 1 and positions.stride(-1) != 1:
             positions = positions.contiguous()
     args = (q, k, q_weight, k_weight)

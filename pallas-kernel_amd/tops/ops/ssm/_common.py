@@ -55,10 +55,11 @@ def offsets(cu_seqlens, B, T):
     if cu_seqlens is None:
         return None
     cu = to_list(cu_seqlens)
-    require(B == 1, f"cu_seqlens requires B == 1, got B={B}")
-    require(len(cu) >= 2 and cu[0] == 0 and cu[-1] == T
-            and all(b >= a for a, b in zip(cu, cu[1:])),
-            f"cu_seqlens must go from 0 to T={T} without decreasing: {cu}")
+    if B != 1:
+        require(False, f"cu_seqlens requires B == 1, got B={B}")
+    if (len(cu) < 2 or cu[0] != 0 or cu[-1] != T
+            or any(b < a for a, b in zip(cu, cu[1:]))):
+        require(False, f"cu_seqlens must go from 0 to T={T} without decreasing: {cu}")
     return cu
 
 
@@ -93,9 +94,9 @@ def slot_args(idx, batch, device_of):
     """(address, whether int64) of the state slots of a batch."""
     if idx is None:
         return 0, 0
-    require(idx.dtype in (torch.int32, torch.int64) and tuple(idx.shape) == (batch,),
-            f"state_indices must be int32 or int64 of shape {(batch,)}, got {idx.dtype} "
-            f"{tuple(idx.shape)}")
+    if idx.dtype not in (torch.int32, torch.int64) or idx.shape != (batch,):
+        require(False, f"state_indices must be int32 or int64 of shape {(batch,)}, got "
+                       f"{idx.dtype} {tuple(idx.shape)}")
     require(batch <= 1 or idx.stride(0) == 1, "state_indices must be contiguous")
     return idx.data_ptr(), int(idx.dtype == torch.int64)
 

@@ -22,8 +22,8 @@ def _cu_tensor(cu, device):
 
 
 def _silu(activation):
-    require(activation in (None, "silu", "swish"),
-            f"activation must be None, 'silu' or 'swish', got {activation!r}")
+    if activation not in (None, "silu", "swish"):
+        require(False, f"activation must be None, 'silu' or 'swish', got {activation!r}")
     return activation is not None
 
 
@@ -31,6 +31,14 @@ def _contiguous(t, dt):
     if t is None or (t.dtype is dt and t.is_contiguous()):
         return t
     return t.to(dt).contiguous()
+
+
+def _check_weight(weight, bias, D, W):
+    if weight.shape not in ((D, W), (D, 1, W)) or not 1 <= W <= 8 or D < 1:
+        require(False, f"weight must be [{D}, W] or [{D}, 1, W] with W <= 8, got "
+                       f"{tuple(weight.shape)}")
+    if bias is not None and bias.shape != (D,):
+        require(False, f"bias must be {(D,)}, got {tuple(bias.shape)}")
 
 
 def _pack(x, y, fin, cu_t, nseq, silu, bwd=None):
@@ -117,17 +125,16 @@ def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None,
     Returns ``(y, final_state)`` in x's type; final_state ``[sequences, W, D]`` with
     ``output_final_state``, else None.
     """
-    require(x.dim() == 3, f"x must be [B, T, D], got {tuple(x.shape)}")
+    if x.dim() != 3:
+        require(False, f"x must be [B, T, D], got {tuple(x.shape)}")
     B, T, D = x.shape
     W = weight.shape[-1]
-    require(tuple(weight.shape) in ((D, W), (D, 1, W)) and 1 <= W <= 8 and D > 0,
-            f"weight must be [{D}, W] or [{D}, 1, W] with W <= 8, got {tuple(weight.shape)}")
-    require(bias is None or tuple(bias.shape) == (D,), f"bias must be {(D,)}")
+    _check_weight(weight, bias, D, W)
     silu = _silu(activation)
     cu = offsets(cu_seqlens, B, T)
     S = B if cu is None else len(cu) - 1
-    require(initial_state is None or tuple(initial_state.shape) == (S, W, D),
-            f"initial_state must be {(S, W, D)}")
+    if initial_state is not None and initial_state.shape != (S, W, D):
+        require(False, f"initial_state must be {(S, W, D)}, got {tuple(initial_state.shape)}")
     args = (x, weight, bias, initial_state)
     if differentiable(*args):
         return _CausalConvFunction.apply(*args, silu, bool(output_final_state), cu)
@@ -146,18 +153,18 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     Returns y ``[B, D]`` in x's type.
     """
     refuse_grad("causal_conv1d_step", x, state, weight, bias)
-    require(x.dim() == 2, f"x must be [B, D], got {tuple(x.shape)}")
+    if x.dim() != 2:
+        require(False, f"x must be [B, D], got {tuple(x.shape)}")
     B, D = x.shape
     W = weight.shape[-1]
-    require(tuple(weight.shape) in ((D, W), (D, 1, W)) and 1 <= W <= 8 and D > 0,
-            f"weight must be [{D}, W] or [{D}, 1, W] with W <= 8, got {tuple(weight.shape)}")
-    require(bias is None or tuple(bias.shape) == (D,), f"bias must be {(D,)}")
+    _check_weight(weight, bias, D, W)
     silu = _silu(activation)
-    require(state.dim() == 3 and tuple(state.shape[1:]) == (W, D) and state.dtype == x.dtype
-            and (state.stride(2) == 1 or D == 1) and (state.stride(1) == D or W == 1),
-            f"state must be {x.dtype} [slots, {W}, {D}] with contiguous slots")
-    require(state_indices is not None or state.shape[0] >= B,
-            f"state holds {state.shape[0]} slots, the batch {B}")
+    ss = state.stride()
+    if (state.dim() != 3 or state.shape[1:] != (W, D) or state.dtype is not x.dtype
+            or (ss[2] != 1 and D > 1) or (ss[1] != D and W > 1)):
+        require(False, f"state must be {x.dtype} [slots, {W}, {D}] with contiguous slots")
+    if state_indices is None and state.shape[0] < B:
+        require(False, f"state holds {state.shape[0]} slots, the batch {B}")
     idx, idx64 = slot_args(state_indices, B, x)
     dev = check_device(x, state, weight, bias, state_indices)
     dt = dtype_code(x.dtype)
@@ -167,6 +174,6 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     y = torch.empty(B, D, dtype=x.dtype, device=dev)
     call("tops_gla_causal_conv_step", _STEP.pack(
         xx.data_ptr(), state.data_ptr(), ww.data_ptr(), address(bb), y.data_ptr(), idx, idx64,
-        state.shape[0], B, D, W, state.stride(0), xx.stride(0), int(silu), dt, dtype_code(wt)),
+        state.shape[0], B, D, W, ss[0], xx.stride(0), int(silu), dt, dtype_code(wt)),
         stream_of(dev))
     return y

@@ -176,28 +176,29 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     Returns ``(y, final_state)``: y ``[B, T, D]`` in u's type, final_state ``[sequences, D, N]``
     float32 with ``output_final_state``, else None.
     """
-    require(u.dim() == 3, f"u must be [B, T, D], got {tuple(u.shape)}")
+    if u.dim() != 3:
+        require(False, f"u must be [B, T, D], got {tuple(u.shape)}")
     Bt, T, Dn = u.shape
-    require(A.dim() == 2 and A.shape[0] == Dn and 1 <= A.shape[1] <= 64,
-            f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
+    if A.dim() != 2 or A.shape[0] != Dn or not 1 <= A.shape[1] <= 64:
+        require(False, f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
     N = A.shape[1]
     for name, t in (("delta", delta), ("z", z)):
-        require(t is None or tuple(t.shape) == (Bt, T, Dn),
-                f"{name} must be {(Bt, T, Dn)}" if t is not None else "")
+        if t is not None and t.shape != u.shape:
+            require(False, f"{name} must be {(Bt, T, Dn)}, got {tuple(t.shape)}")
     for name, t in (("B", B), ("C", C)):
-        require(t.dim() in (3, 4) and tuple(t.shape[:2]) == (Bt, T) and t.shape[-1] == N
-                and (t.dim() == 3 or (t.shape[2] > 0 and Dn % t.shape[2] == 0)),
-                f"{name} must be [{Bt}, {T}, {N}] or [{Bt}, {T}, G, {N}] with G dividing {Dn}, "
-                f"got {tuple(t.shape)}")
+        if (t.dim() not in (3, 4) or t.shape[:2] != u.shape[:2] or t.shape[-1] != N
+                or (t.dim() == 4 and (t.shape[2] < 1 or Dn % t.shape[2]))):
+            require(False, f"{name} must be [{Bt}, {T}, {N}] or [{Bt}, {T}, G, {N}] with G "
+                           f"dividing {Dn}, got {tuple(t.shape)}")
     require(B.shape == C.shape, "B and C must have the same shape")
     require(Dn > 0, "D must be positive")
     for name, t in (("D", D), ("delta_bias", delta_bias)):
-        require(t is None or tuple(t.shape) == (Dn,),
-                f"{name} must be {(Dn,)}" if t is not None else "")
+        if t is not None and t.shape != (Dn,):
+            require(False, f"{name} must be {(Dn,)}, got {tuple(t.shape)}")
     cu = offsets(cu_seqlens, Bt, T)
     S = Bt if cu is None else len(cu) - 1
-    require(initial_state is None or tuple(initial_state.shape) == (S, Dn, N),
-            f"initial_state must be {(S, Dn, N)}")
+    if initial_state is not None and initial_state.shape != (S, Dn, N):
+        require(False, f"initial_state must be {(S, Dn, N)}, got {tuple(initial_state.shape)}")
     args = (u, delta, A, B, C, D, z, delta_bias, initial_state)
     if differentiable(*args):
         return _SelectiveScanFunction.apply(*args, bool(delta_softplus), bool(output_final_state),
@@ -224,24 +225,24 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     require(u.dim() == 2 and A.dim() == 2, "u must be [B, D], A [D, N]")
     Bt, Dn = u.shape
     N = A.shape[1]
-    require(A.shape[0] == Dn and 1 <= N <= 64 and Dn > 0,
-            f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
-    require(delta.shape == u.shape and (z is None or z.shape == u.shape),
-            f"delta and z must be {(Bt, Dn)}")
+    if A.shape[0] != Dn or not 1 <= N <= 64 or Dn < 1:
+        require(False, f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
+    if delta.shape != u.shape or (z is not None and z.shape != u.shape):
+        require(False, f"delta and z must be {(Bt, Dn)}")
     G = B.shape[1] if B.dim() == 3 else 1
-    require(B.shape == C.shape and B.dim() in (2, 3) and B.shape[0] == Bt and B.shape[-1] == N
-            and G > 0 and Dn % G == 0,
-            f"B and C must be [{Bt}, {N}] or [{Bt}, G, {N}] with G dividing {Dn}, got "
-            f"{tuple(B.shape)} and {tuple(C.shape)}")
-    require((D is None or tuple(D.shape) == (Dn,))
-            and (delta_bias is None or tuple(delta_bias.shape) == (Dn,)),
-            f"D and delta_bias must be {(Dn,)}")
-    require(state.dim() == 3 and tuple(state.shape[1:]) == (Dn, N)
-            and state.dtype == torch.float32
-            and (state.stride(2) == 1 or N == 1) and (state.stride(1) == N or Dn == 1),
-            f"state must be float32 [slots, {Dn}, {N}] with contiguous slots")
-    require(state_indices is not None or state.shape[0] >= Bt,
-            f"state holds {state.shape[0]} slots, the batch {Bt}")
+    if (B.shape != C.shape or B.dim() not in (2, 3) or B.shape[0] != Bt or B.shape[-1] != N
+            or G < 1 or Dn % G):
+        require(False, f"B and C must be [{Bt}, {N}] or [{Bt}, G, {N}] with G dividing {Dn}, got "
+                       f"{tuple(B.shape)} and {tuple(C.shape)}")
+    if ((D is not None and D.shape != (Dn,))
+            or (delta_bias is not None and delta_bias.shape != (Dn,))):
+        require(False, f"D and delta_bias must be {(Dn,)}")
+    ss = state.stride()
+    if (state.dim() != 3 or state.shape[1:] != A.shape or state.dtype is not torch.float32
+            or (ss[2] != 1 and N > 1) or (ss[1] != N and Dn > 1)):
+        require(False, f"state must be float32 [slots, {Dn}, {N}] with contiguous slots")
+    if state_indices is None and state.shape[0] < Bt:
+        require(False, f"state holds {state.shape[0]} slots, the batch {Bt}")
     idx, idx64 = slot_args(state_indices, Bt, u)
     dev = check_device(state, u, delta, A, B, C, D, z, delta_bias, state_indices)
     dt = io_dtype(u, delta, B, C, z)
@@ -251,7 +252,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     call("tops_gla_selective_scan_step", _STEP.pack(
         state.data_ptr(), uu.data_ptr(), dd.data_ptr(), address(zz), bb.data_ptr(), cc.data_ptr(),
         aa.data_ptr(), address(sk), address(bias), y.data_ptr(), idx, idx64, state.shape[0], Bt,
-        Dn, N, G, state.stride(0), uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0),
+        Dn, N, G, ss[0], uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0),
         bb.stride(0), bb.stride(1) if G > 1 else 0, cc.stride(0), cc.stride(1) if G > 1 else 0,
         int(bool(delta_softplus)), dtype_code(dt)), stream_of(dev))
     return y if dt == u.dtype else y.to(u.dtype)
