@@ -19,7 +19,8 @@ namespace tops {
 
 namespace {
 
-constexpr int SS_K = 8;      // tokens of a tile, and between the states kept for the backward
+constexpr int SS_K = 8;      // tokens of a tile of the backward, and between the states kept for it
+constexpr int FT = 4;        // tokens of a tile of the forward
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -209,45 +210,45 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
   const float* bc = a.bc + (pc.b * a.T * a.G + tl.grp) * 2 * NP + (MODE == 2 ? NP : 0);
   const float* bc_end = a.bc + p.tokens * bc_st;
 
-  T ru[SS_K], rd[SS_K], rz[SS_K];
+  T ru[FT], rd[FT], rz[FT];
   auto load = [&](int t0) {
-    load_rows<T, SS_K>(gu, u_st, t0, pc.t1, lo, ru);
-    load_rows<T, SS_K>(gd, a.delta_st, t0, pc.t1, lo, rd);
-    if (has_z) load_rows<T, SS_K>(gz, a.z_st, t0, pc.t1, lo, rz);
+    load_rows<T, FT>(gu, u_st, t0, pc.t1, lo, ru);
+    load_rows<T, FT>(gd, a.delta_st, t0, pc.t1, lo, rd);
+    if (has_z) load_rows<T, FT>(gz, a.z_st, t0, pc.t1, lo, rz);
   };
-  const int nt = (pc.t1 - pc.t0 + SS_K - 1) / SS_K;
+  const int nt = (pc.t1 - pc.t0 + FT - 1) / FT;
   const int first = MODE == 2 ? nt - 1 : 0, step = MODE == 2 ? -1 : 1;
-  if (nt > 0) load(pc.t0 + first * SS_K);
+  if (nt > 0) load(pc.t0 + first * FT);
 #pragma unroll 1
   for (int it = 0; it < nt; ++it) {
-    const int k = first + it * step, t0 = pc.t0 + k * SS_K;
-    float d[SS_K], u[SS_K], z[SS_K], y[SS_K];
+    const int k = first + it * step, t0 = pc.t0 + k * FT;
+    float d[FT], u[FT], z[FT], y[FT];
 #pragma unroll
-    for (int i = 0; i < SS_K; ++i) {
+    for (int i = 0; i < FT; ++i) {
       d[i] = to_f32(rd[i]) + bias;
       u[i] = to_f32(ru[i]);
       z[i] = has_z ? to_f32(rz[i]) : 0.f;
     }
     if (softplus)
 #pragma unroll
-      for (int i = 0; i < SS_K; ++i) {
+      for (int i = 0; i < FT; ++i) {
         float sg;
         softplus_sigmoid(d[i], d[i], sg);
       }
     if (MODE == 2 && has_z)
 #pragma unroll
-      for (int i = 0; i < SS_K; ++i) u[i] *= z[i] * sigmoid(z[i]);
+      for (int i = 0; i < FT; ++i) u[i] *= z[i] * sigmoid(z[i]);
 #pragma unroll
-    for (int i = 0; i < SS_K; ++i)   // a token past the end leaves the state as it is
+    for (int i = 0; i < FT; ++i)   // a token past the end leaves the state as it is
       if (t0 + i >= pc.t1) d[i] = u[i] = 0.f;
-    if (it + 1 < nt) load(t0 + step * SS_K);
-    if (MODE == 1 && a.chunk_h && live)
-      store_states<NP>(a.chunk_h + (long)(pc.c0 + k) * NP * D + tl.d0, D, lo, h);
-    const float* q = bc + (t0 + (MODE == 2 ? SS_K - 1 : 0)) * bc_st;
+    if (it + 1 < nt) load(t0 + step * FT);
+    if (MODE == 1 && k % (SS_K / FT) == 0 && a.chunk_h && live)
+      store_states<NP>(a.chunk_h + (long)(pc.c0 + k / (SS_K / FT)) * NP * D + tl.d0, D, lo, h);
+    const float* q = bc + (t0 + (MODE == 2 ? FT - 1 : 0)) * bc_st;
     float ahead[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < SS_K; ++j) {
-      const int i = MODE == 2 ? SS_K - 1 - j : j;
+    for (int j = 0; j < FT; ++j) {
+      const int i = MODE == 2 ? FT - 1 - j : j;
       const float x = MODE == 2 ? u[i] : d[i] * u[i];
       float acc[2] = {0.f, 0.f};
       const float* at = t0 + i < pc.t1 ? q : bc_end;
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
         arrived(rb);
         if (MODE == 1) arrived(rc);
         const bool more = g + GN < NP;
-        if (more || j + 1 < SS_K) {   // the next rows into the scalar cache
+        if (more || j + 1 < FT) {   // the next rows into the scalar cache
           cfloat* np = more ? row + g + GN
                             : (cfloat*)(uintptr_t)(t0 + i + (MODE == 2 ? -1 : 1) < pc.t1 ? q : bc_end);
           ahead[0] = np[0];
@@ -287,13 +288,13 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
     if (MODE == 1) {
       T* gy = (T*)a.y + (pc.b * a.T + t0) * D + tl.d0;
 #pragma unroll
-      for (int i = 0; i < SS_K; ++i) y[i] = fmaf(skip, u[i], y[i]);
+      for (int i = 0; i < FT; ++i) y[i] = fmaf(skip, u[i], y[i]);
       if (has_z)
 #pragma unroll
-        for (int i = 0; i < SS_K; ++i) y[i] *= z[i] * sigmoid(z[i]);
+        for (int i = 0; i < FT; ++i) y[i] *= z[i] * sigmoid(z[i]);
       if (live)
 #pragma unroll
-        for (int i = 0; i < SS_K; ++i)
+        for (int i = 0; i < FT; ++i)
           if (t0 + i < pc.t1) (gy + (long)i * D)[lo] = from_f32<T>(y[i]);
     }
   }
