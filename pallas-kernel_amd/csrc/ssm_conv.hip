@@ -15,8 +15,10 @@ constexpr int CV_NT = 256;
 constexpr int CV_CX = 64;    // threads along the channels
 constexpr int CV_U = 8;      // rows in flight
 
+// VEC consecutive elements of a row, at any address of theirs: the wide loads and stores need no
+// alignment beyond the element's.
 template <typename T, int VEC>
-struct alignas(VEC * sizeof(T)) Row {
+struct Row {
   T v[VEC];
 };
 template <typename T, int VEC>
@@ -34,6 +36,14 @@ __device__ __forceinline__ void put(T* p, const float (&x)[VEC]) {
 template <typename T, int VEC>
 __device__ __forceinline__ Row<T, VEC> get(const T* p) {
   return *reinterpret_cast<const Row<T, VEC>*>(p);
+}
+
+// First channel of the i-th thread along them, -1 past the last. Where D is no multiple of VEC the
+// last thread takes the last VEC channels: some of them twice, to the same values.
+template <int VEC>
+__device__ __forceinline__ int channel_of(const tops_gla_conv_args& a, int i) {
+  const int c = i * VEC, D = (int)a.D;
+  return c >= D ? -1 : min(c, D - VEC);
 }
 
 // First and end token of sequence s, in the flattened tokens.
@@ -84,12 +94,12 @@ __device__ __forceinline__ void weights_of(const TW* w0, const TW* b0, int c, fl
                                            float (&b)[VEC]) {
   float x[VEC * W];
   const TW* p = w0 + (long)c * W;
-  if (VEC == 4 && (uintptr_t)w0 % (4 * sizeof(TW)) == 0) {
 #pragma unroll
-    for (int j = 0; j + 3 < VEC * W; j += 4) load_four(p + j, reinterpret_cast<float(&)[4]>(x[j]));
-  } else {
+  for (int j = 0; j < W; ++j) {
+    float v[VEC];
+    unpack<TW, VEC>(get<TW, VEC>(p + VEC * j), v);
 #pragma unroll
-    for (int j = 0; j < VEC * W; ++j) x[j] = to_f32(p[j]);
+    for (int e = 0; e < VEC; ++e) x[VEC * j + e] = v[e];
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
@@ -153,8 +163,8 @@ __global__ __launch_bounds__(CV_NT) void conv_fwd_kernel(tops_gla_conv_args a, i
                                                          int slabs) {
   const int slab = blockIdx.x % slabs;
   const long group = blockIdx.x / slabs;
-  const int c = (slab * CV_CX + threadIdx.x % CV_CX) * VEC;
-  if (c >= a.D) return;
+  const int c = channel_of<VEC>(a, slab * CV_CX + threadIdx.x % CV_CX);
+  if (c < 0) return;
   const int ry = __builtin_amdgcn_readfirstlane(threadIdx.x / CV_CX);
   if (group >= tiles) {
     const long i = (group - tiles) * 4 + ry;
@@ -205,8 +215,8 @@ __global__ __launch_bounds__(CV_NT) void conv_bwd_kernel(tops_gla_conv_args a, i
   const int ry = __builtin_amdgcn_readfirstlane(threadIdx.x / CV_CX);
   const int slab = blockIdx.x % slabs;
   const long group = blockIdx.x / slabs;
-  const int c = (slab * CV_CX + cx) * VEC;
-  const bool live = c < a.D;
+  const int c = channel_of<VEC>(a, slab * CV_CX + cx);
+  const bool live = c >= 0;
   const long tokens = a.batch * a.T;
   long tau = (group * 4 + ry) * run;
   const long end = min(tokens, tau + run);
@@ -415,24 +425,13 @@ hipError_t conv_launch(const tops_gla_conv_args& a, bool backward, hipStream_t s
   return hipSuccess;
 }
 
-// Whole, aligned runs of n elements in every row that a thread reads or writes.
-bool rows_aligned(const tops_gla_conv_args& a, bool backward, int n) {
-  const long es = a.dtype == DT_BF16 ? 2 : 4, by = n * es;
-  if (a.D % n || a.x_sb % n || a.x_st % n) return false;
-  if (backward && (a.dy_sb % n || a.dy_st % n)) return false;
-  for (const void* q : {a.x, a.init, (const void*)a.y, (const void*)a.final_state, a.dy, a.dfinal,
-                        (const void*)a.dx})
-    if ((uintptr_t)q % by) return false;
-  return true;
-}
-
 template <typename T, int W>
 hipError_t conv_width(const tops_gla_conv_args& a, bool backward, hipStream_t st) {
   // 8 bytes of a row a thread: the backward holds 4 W + 2 rows in registers (with 16 bytes 256 of
   // them, one wave a SIMD: 249 us against 178 for 32768 tokens of 4096 channels, bf16), and the
   // forward of few tokens has more waves (8192 tokens, 2048 channels: 27 and 20 us)
   constexpr int VEC = 8 / (int)sizeof(T);
-  if (rows_aligned(a, backward, VEC)) return conv_launch<T, VEC, W>(a, backward, st);
+  if (a.D >= VEC) return conv_launch<T, VEC, W>(a, backward, st);
   return conv_launch<T, 1, W>(a, backward, st);
 }
 
