@@ -314,6 +314,8 @@ __device__ __forceinline__ void piece_load(Piece<T, VEC>& r, const T* p) {
   if constexpr (Piece<T, VEC>::W == 4) {
     const uint4 x = *reinterpret_cast<const uint4*>(p);
     r.w[0] = x.x, r.w[1] = x.y, r.w[2] = x.z, r.w[3] = x.w;
+  } else if constexpr (Piece<T, VEC>::W == 1) {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else {
     const uint2 x = *reinterpret_cast<const uint2*>(p);
     r.w[0] = x.x, r.w[1] = x.y;
@@ -356,8 +358,11 @@ __device__ __forceinline__ void token_offsets(const tops_gla_qk_args& a, long ta
 // A lane's place in a row: its piece, the piece's partner, and what a rotation does with it.
 template <int VEC, int LPR, bool INTER>
 struct Lane {
+  static constexpr bool EACH = VEC == 2 && !INTER;   // partners by the element, not the piece
   int c, f, lane4;
   bool in, rot, hi;
+  int fe[2], pe[2], lane4e[2], odd;   // EACH: an element's frequency, partner's column and lane
+  bool hie[2];
   __device__ __forceinline__ Lane(int D, int R) {
     const int lane = threadIdx.x % LPR, R2 = R / 2;
     c = lane * VEC;
@@ -367,6 +372,18 @@ struct Lane {
     f = !rot ? 0 : INTER ? c / 2 : hi ? c - R2 : c;
     const int m = INTER || !rot ? 0 : hi ? -(R2 / VEC) : R2 / VEC;
     lane4 = 4 * ((threadIdx.x & 63) + m);
+    if (EACH) {
+      // half the rotated columns may be odd in number: the elements of a piece then have their
+      // partners in two pieces, and one piece lies on both sides of the middle
+      odd = R2 & 1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        hie[e] = rot && c + e >= R2;
+        fe[e] = !rot ? 0 : hie[e] ? c + e - R2 : c + e;
+        pe[e] = !rot ? c + e : hie[e] ? c + e - R2 : c + e + R2;
+        lane4e[e] = 4 * ((threadIdx.x & 63) + pe[e] / 2 - c / 2);
+      }
+    }
   }
   // column of the partner's piece
   __device__ __forceinline__ int pc(int R) const {
@@ -374,12 +391,44 @@ struct Lane {
   }
 };
 
-// x turned by the angles of cs (sign -1: back), xp being its partner piece.
+// The values of a piece's partners.
+template <typename T, int VEC, int LPR, bool INTER>
+__device__ __forceinline__ void partners(const Piece<T, VEC>& x, const Lane<VEC, LPR, INTER>& l,
+                                         float (&p)[VEC]) {
+  if constexpr (Lane<VEC, LPR, INTER>::EACH) {
+    constexpr int W = Piece<T, VEC>::W;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      Piece<T, VEC> r;
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        r.w[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(l.lane4e[e], (int)x.w[i]);
+      piece_values<T, VEC>(r, v);
+      p[e] = l.odd ? v[1 - e] : v[e];
+    }
+  } else if constexpr (!INTER) {
+    Piece<T, VEC> r = x;
+    piece_of_lane<T, VEC>(r, l.lane4);
+    piece_values<T, VEC>(r, p);
+  }
+}
+
+// x turned by a token's angles cs (sign -1: back), xp being its partners.
 template <int VEC, int LPR, bool INTER>
 __device__ __forceinline__ void turn_piece(float (&x)[VEC], const float (&xp)[VEC],
                                            const float2* cs, const Lane<VEC, LPR, INTER>& l, int R,
                                            float sign) {
-  turn<VEC, INTER>(x, xp, cs, l.rot, l.hi, l.c, R, sign);
+  if constexpr (Lane<VEC, LPR, INTER>::EACH) {
+    if (l.rot)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 k = cs[l.fe[e]];
+        x[e] = fmaf(xp[e], l.hie[e] ? sign * k.y : -sign * k.y, x[e] * k.x);
+      }
+  } else {
+    turn<VEC, INTER>(x, xp, cs + l.f, l.rot, l.hi, l.c, R, sign);
+  }
 }
 
 // `magic[p]` = ceil(2^32 / heads of part p): row / heads = mulhi(row, magic) for row < 2^16.
@@ -422,7 +471,7 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       wv[e] = w ? w[cl + e] : 1.f;
-      wp[e] = w ? w[pc + e] : 1.f;
+      wp[e] = !w ? 1.f : Lane<VEC, LPR, INTER>::EACH ? w[l.in ? l.pe[e] : 0] : w[pc + e];
     }
   };
   if (nb > 0) load(0);
@@ -447,10 +496,7 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
       const int r = r0 + u * RPB;
       float v[VEC], p[VEC], ss = 0.f;
       piece_values<T, VEC>(x[u], v);
-      if (PAIR) {
-        piece_of_lane<T, VEC>(x[u], l.lane4);
-        piece_values<T, VEC>(x[u], p);
-      }
+      if (PAIR) partners(x[u], l, p);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         if (!l.in) v[e] = 0.f;
@@ -464,7 +510,7 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
       }
       if (r < rows && l.in) {
         const int tk = H == 1 ? r : (int)__umulhi((uint32_t)r, magic);
-        turn_piece<VEC, LPR, INTER>(v, p, cs + tk * R2 + l.f, l, R, 1.f);
+        turn_piece<VEC, LPR, INTER>(v, p, cs + tk * R2, l, R, 1.f);
         store_run<T, VEC>(dst + (long)r * D + l.c, v);
       }
     }
@@ -542,11 +588,8 @@ __global__ __launch_bounds__(QK_NT) void qk_bwd_rows_kernel(tops_gla_qk_args a, 
         float v[VEC], d[VEC], p[VEC], ss = 0.f, em = 0.f;
         piece_values<T, VEC>(x[u], v);
         piece_values<T, VEC>(gy[u], d);
-        if (PAIR) {
-          piece_of_lane<T, VEC>(gy[u], l.lane4);
-          piece_values<T, VEC>(gy[u], p);
-        }
-        turn_piece<VEC, LPR, INTER>(d, p, cs + tk * R2 + l.f, l, R, -1.f);
+        if (PAIR) partners(gy[u], l, p);
+        turn_piece<VEC, LPR, INTER>(d, p, cs + tk * R2, l, R, -1.f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           if (!on) v[e] = d[e] = 0.f;
@@ -596,9 +639,14 @@ int tokens_per_block(long tokens, long heads, bool backward) {
 }
 uint32_t magic_of(long heads) { return heads < 2 ? 0 : (uint32_t)(((1ULL << 32) + heads - 1) / heads); }
 
+// A block's rows are at most 2^16 (heads are, and more tokens than one only for fewer than 512 of
+// them), as a row's index times the magic number has to be exact.
 template <typename T, int VEC, int LPR>
-hipError_t qk_rows_launch(const tops_gla_qk_args& a, bool backward, int tb, long groups, size_t lds,
-                          hipStream_t st) {
+hipError_t qk_rows_launch(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
+  const long tokens = a.batch * a.T;
+  const int tb = tokens_per_block(tokens, a.Hq + a.Hk, backward);
+  const long groups = (tokens + tb - 1) / tb;
+  const size_t lds = (size_t)tb * (a.R / 2) * sizeof(float2);
   const uint32_t mq = magic_of(a.Hq), mk = magic_of(a.Hk);
   const dim3 nt(QK_NT);
   if (!backward) {
@@ -639,10 +687,6 @@ hipError_t qk_launch(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
   const int tb = tokens_per_block(tokens, a.Hq + a.Hk, backward);
   const long groups = (tokens + tb - 1) / tb;
   const size_t lds = (size_t)tb * (a.R / 2) * sizeof(float2);
-  if constexpr (VEC > 1 && NI == 1) {
-    // a row's index times the magic number is exact below 2^16 rows
-    if (tb * std::max(a.Hq, a.Hk) < 65536) return qk_rows_launch<T, VEC, LPR>(a, backward, tb, groups, lds, st);
-  }
   if (!backward) {
     if (a.interleaved)
       hipLaunchKernelGGL((qk_fwd_kernel<T, VEC, LPR, NI, true>), dim3((unsigned)groups), dim3(QK_NT),
@@ -674,7 +718,7 @@ hipError_t qk_launch(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
 // Whole, aligned pieces of n elements in every row, and partners on such pieces.
 bool pieces_of(const tops_gla_qk_args& a, bool backward, int n) {
   const long by = n * (a.dtype == DT_BF16 ? 2 : 4);
-  if (a.D % n || (!a.interleaved && (a.R / 2) % n)) return false;
+  if (a.D % n || (!a.interleaved && n > 2 && (a.R / 2) % n)) return false;
   for (int64_t s : {a.q_sb, a.q_st, a.q_sh, a.k_sb, a.k_st, a.k_sh})
     if (s % n) return false;
   for (const void* p : {a.q, a.k, (const void*)a.qo, (const void*)a.ko})
@@ -687,16 +731,35 @@ bool pieces_of(const tops_gla_qk_args& a, bool backward, int n) {
   return true;
 }
 
+// Pieces of two elements, for heads of up to 128 columns: 4 or 8 bytes a lane.
+template <typename T>
+hipError_t qk_pairs(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
+  if (a.D <= 32) return qk_rows_launch<T, 2, 16>(a, backward, st);
+  if (a.D <= 64) return qk_rows_launch<T, 2, 32>(a, backward, st);
+  return qk_rows_launch<T, 2, 64>(a, backward, st);
+}
+
+// Heads of an odd size, or rows that are not aligned: an element a lane.
+template <typename T>
+hipError_t qk_elements(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
+  if (a.D <= 8) return qk_launch<T, 1, 8, 1>(a, backward, st);
+  if (a.D <= 16) return qk_launch<T, 1, 16, 1>(a, backward, st);
+  if (a.D <= 32) return qk_launch<T, 1, 32, 1>(a, backward, st);
+  if (a.D <= 64) return qk_launch<T, 1, 64, 1>(a, backward, st);
+  if (a.D <= 128) return qk_launch<T, 1, 64, 2>(a, backward, st);
+  return qk_launch<T, 1, 64, 8>(a, backward, st);
+}
+
 template <typename T, int VEC>
 hipError_t qk_rows(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
-  const long pieces = (a.D + VEC - 1) / VEC;
-  if (pieces <= 8) return qk_launch<T, VEC, 8, 1>(a, backward, st);
-  if (pieces <= 16) return qk_launch<T, VEC, 16, 1>(a, backward, st);
-  if (pieces <= 32) return qk_launch<T, VEC, 32, 1>(a, backward, st);
+  const long pieces = a.D / VEC;
+  if (pieces <= 8) return qk_rows_launch<T, VEC, 8>(a, backward, st);
+  if (pieces <= 16) return qk_rows_launch<T, VEC, 16>(a, backward, st);
+  if (pieces <= 32) return qk_rows_launch<T, VEC, 32>(a, backward, st);
   constexpr int NI = 512 / VEC / 64;   // rows of up to 512 elements
   if constexpr (NI > 1)
-    if (pieces <= 64) return qk_launch<T, VEC, 64, 1>(a, backward, st);
-  return qk_launch<T, VEC, 64, NI>(a, backward, st);
+    if (pieces > 64) return qk_launch<T, VEC, 64, NI>(a, backward, st);
+  return qk_rows_launch<T, VEC, 64>(a, backward, st);
 }
 
 }  // namespace
@@ -708,10 +771,12 @@ hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_
   if (a.dtype == DT_BF16) {
     if (pieces_of(a, backward, 8)) return qk_rows<bf16, 8>(a, backward, st);
     if (pieces_of(a, backward, 4)) return qk_rows<bf16, 4>(a, backward, st);
-    return qk_rows<bf16, 1>(a, backward, st);
+    if (a.D <= 128 && pieces_of(a, backward, 2)) return qk_pairs<bf16>(a, backward, st);
+    return qk_elements<bf16>(a, backward, st);
   }
   if (pieces_of(a, backward, 4)) return qk_rows<float, 4>(a, backward, st);
-  return qk_rows<float, 1>(a, backward, st);
+  if (a.D <= 128 && pieces_of(a, backward, 2)) return qk_pairs<float>(a, backward, st);
+  return qk_elements<float>(a, backward, st);
 }
 
 }  // namespace tops
