@@ -231,16 +231,14 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
     }
     if (softplus)
 #pragma unroll
-      for (int i = 0; i < FT; ++i) {
-        float sg;
-        softplus_sigmoid(d[i], d[i], sg);
-      }
+      for (int i = 0; i < FT; ++i) d[i] = tops::softplus(d[i]);
     if (MODE == 2 && has_z)
 #pragma unroll
       for (int i = 0; i < FT; ++i) u[i] *= z[i] * sigmoid(z[i]);
+    if (t0 + FT > pc.t1)
 #pragma unroll
-    for (int i = 0; i < FT; ++i)   // a token past the end leaves the state as it is
-      if (t0 + i >= pc.t1) d[i] = u[i] = 0.f;
+      for (int i = 0; i < FT; ++i)   // a token past the end leaves the state as it is
+        if (t0 + i >= pc.t1) d[i] = u[i] = 0.f;
     if (it + 1 < nt) load(t0 + step * FT);
     if (MODE == 1 && k % (SS_K / FT) == 0 && a.chunk_h && live)
       store_states<NP>(a.chunk_h + (long)(pc.c0 + k / (SS_K / FT)) * NP * D + tl.d0, D, lo, h);

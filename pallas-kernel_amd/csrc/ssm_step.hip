@@ -86,8 +86,8 @@ __global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_arg
   const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    float t = dt[k] + bias, sg, y = 0.f;
-    if (a.softplus) softplus_sigmoid(t, t, sg);
+    float t = dt[k] + bias, y = 0.f;
+    if (a.softplus) t = softplus(t);
     const float du = t * u[k];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
