@@ -15,6 +15,9 @@ from ..ssm._common import address, differentiable, f32, io_dtype, rows, strides
 _ARGS = struct.Struct("=8q 6q 8q 2q d 2q 6q 4q 2q")
 
 
+_NO_BWD = (0,) * 14
+
+
 def rotary_inv_freq(rotary_dim, theta=10000.0, device=None):
     """The usual frequencies ``theta^(-2 i / rotary_dim)``, float64 ``[rotary_dim / 2]``."""
     require(rotary_dim >= 0 and rotary_dim % 2 == 0, "rotary_dim must be even")
@@ -25,13 +28,16 @@ def rotary_inv_freq(rotary_dim, theta=10000.0, device=None):
 def _pack(x, out, interleaved, eps, bwd=None):
     q, k, qw, kw, freq, pos = x
     B, T, Hq, D = q.shape
+    pos_sb = pos64 = 0
+    if pos is not None:
+        pos64 = 1 if pos.dtype is torch.int64 else 0
+        if pos.dim() == 2:
+            pos_sb = pos.stride(0)
     return _ARGS.pack(
-        address(q), address(k), address(qw), address(kw), address(freq), address(pos),
+        q.data_ptr(), k.data_ptr(), address(qw), address(kw), address(freq), address(pos),
         address(out[0]), address(out[1]), B, T, Hq, k.shape[2], D,
-        0 if freq is None else 2 * freq.shape[0], *strides(q, 0, 1, 2), *strides(k, 0, 1, 2),
-        0 if pos is None or pos.dim() == 1 else pos.stride(0),
-        int(pos is not None and pos.dtype == torch.int64), int(interleaved), dtype_code(q.dtype),
-        float(eps), *(bwd or [0] * 14))
+        0 if freq is None else 2 * freq.shape[0], *q.stride()[:3], *k.stride()[:3], pos_sb, pos64,
+        1 if interleaved else 0, dtype_code(q.dtype), eps, *(bwd or _NO_BWD))
 
 
 def _forward(q, k, qw, kw, freq, pos, eps, interleaved):
@@ -101,11 +107,12 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, inv_freq=None, positions=No
 
     Differentiable in q, k and the weights. Returns ``(q', k')`` in the inputs' types, contiguous.
     """
-    if (q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]
-            or not 1 <= q.shape[3] <= 512):
+    qs, ks = q.shape, k.shape
+    if (len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[1] != ks[1] or qs[3] != ks[3]
+            or not 1 <= qs[3] <= 512):
         require(False, f"q and k must be [B, T, heads, D] with one D <= 512, got "
-                       f"{tuple(q.shape)} and {tuple(k.shape)}")
-    B, T, _, D = q.shape
+                       f"{tuple(qs)} and {tuple(ks)}")
+    B, T, _, D = qs
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and w.shape != (D,):
             require(False, f"{name} must be {(D,)}, got {tuple(w.shape)}")
@@ -113,7 +120,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, inv_freq=None, positions=No
         if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > D or inv_freq.dtype is not torch.float64:
             require(False, f"inv_freq must be float64 [R / 2] with R <= {D}, got "
                            f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
-        inv_freq = inv_freq.contiguous()
+        if not inv_freq.is_contiguous():
+            inv_freq = inv_freq.contiguous()
     if positions is not None:
         if (positions.dtype not in (torch.int32, torch.int64)
                 or positions.shape not in ((B, T), (T,))):

@@ -153,27 +153,27 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     Returns y ``[B, D]`` in x's type.
     """
     refuse_grad("causal_conv1d_step", x, state, weight, bias)
-    if x.dim() != 2:
-        require(False, f"x must be [B, D], got {tuple(x.shape)}")
-    B, D = x.shape
+    shape, ss, dtype = x.shape, state.shape, x.dtype
+    if len(shape) != 2:
+        require(False, f"x must be [B, D], got {tuple(shape)}")
+    B, D = shape
     W = weight.shape[-1]
     _check_weight(weight, bias, D, W)
     silu = _silu(activation)
-    ss = state.stride()
-    if (state.dim() != 3 or state.shape[1:] != (W, D) or state.dtype is not x.dtype
-            or (ss[2] != 1 and D > 1) or (ss[1] != D and W > 1)):
-        require(False, f"state must be {x.dtype} [slots, {W}, {D}] with contiguous slots")
-    if state_indices is None and state.shape[0] < B:
-        require(False, f"state holds {state.shape[0]} slots, the batch {B}")
+    st = state.stride()
+    if (len(ss) != 3 or ss[1] != W or ss[2] != D or state.dtype is not dtype
+            or (st[2] != 1 and D > 1) or (st[1] != D and W > 1)):
+        require(False, f"state must be {dtype} [slots, {W}, {D}] with contiguous slots")
+    if state_indices is None and ss[0] < B:
+        require(False, f"state holds {ss[0]} slots, the batch {B}")
     idx, idx64 = slot_args(state_indices, B, x)
     dev = check_device(x, state, weight, bias, state_indices)
-    dt = dtype_code(x.dtype)
+    dt = dtype_code(dtype)
     wt = io_dtype(weight, bias)
-    xx = rows(x, x.dtype)
+    xx = rows(x, dtype)
     ww, bb = _contiguous(weight, wt), _contiguous(bias, wt)
-    y = torch.empty(B, D, dtype=x.dtype, device=dev)
+    y = torch.empty(shape, dtype=dtype, device=dev)
     call("tops_gla_causal_conv_step", _STEP.pack(
         xx.data_ptr(), state.data_ptr(), ww.data_ptr(), address(bb), y.data_ptr(), idx, idx64,
-        state.shape[0], B, D, W, ss[0], xx.stride(0), int(silu), dt, dtype_code(wt)),
-        stream_of(dev))
+        ss[0], B, D, W, st[0], xx.stride(0), int(silu), dt, dtype_code(wt)), stream_of(dev))
     return y

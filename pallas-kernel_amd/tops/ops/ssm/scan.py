@@ -222,37 +222,40 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     Returns y ``[B, D]`` in u's type.
     """
     refuse_grad("selective_scan_step", state, u, delta, A, B, C, D, z, delta_bias)
-    require(u.dim() == 2 and A.dim() == 2, "u must be [B, D], A [D, N]")
-    Bt, Dn = u.shape
-    N = A.shape[1]
-    if A.shape[0] != Dn or not 1 <= N <= 64 or Dn < 1:
-        require(False, f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(A.shape)}")
-    if delta.shape != u.shape or (z is not None and z.shape != u.shape):
+    ushape, ashape, bshape, ss = u.shape, A.shape, B.shape, state.shape
+    if len(ushape) != 2 or len(ashape) != 2:
+        require(False, f"u must be [B, D], A [D, N], got {tuple(ushape)} and {tuple(ashape)}")
+    Bt, Dn = ushape
+    N = ashape[1]
+    if ashape[0] != Dn or not 1 <= N <= 64 or Dn < 1:
+        require(False, f"A must be [{Dn}, N] with 1 <= N <= 64, got {tuple(ashape)}")
+    if delta.shape != ushape or (z is not None and z.shape != ushape):
         require(False, f"delta and z must be {(Bt, Dn)}")
-    G = B.shape[1] if B.dim() == 3 else 1
-    if (B.shape != C.shape or B.dim() not in (2, 3) or B.shape[0] != Bt or B.shape[-1] != N
+    G = bshape[1] if len(bshape) == 3 else 1
+    if (bshape != C.shape or len(bshape) not in (2, 3) or bshape[0] != Bt or bshape[-1] != N
             or G < 1 or Dn % G):
         require(False, f"B and C must be [{Bt}, {N}] or [{Bt}, G, {N}] with G dividing {Dn}, got "
-                       f"{tuple(B.shape)} and {tuple(C.shape)}")
+                       f"{tuple(bshape)} and {tuple(C.shape)}")
     if ((D is not None and D.shape != (Dn,))
             or (delta_bias is not None and delta_bias.shape != (Dn,))):
         require(False, f"D and delta_bias must be {(Dn,)}")
-    ss = state.stride()
-    if (state.dim() != 3 or state.shape[1:] != A.shape or state.dtype is not torch.float32
-            or (ss[2] != 1 and N > 1) or (ss[1] != N and Dn > 1)):
+    st = state.stride()
+    if (len(ss) != 3 or ss[1] != Dn or ss[2] != N or state.dtype is not torch.float32
+            or (st[2] != 1 and N > 1) or (st[1] != N and Dn > 1)):
         require(False, f"state must be float32 [slots, {Dn}, {N}] with contiguous slots")
-    if state_indices is None and state.shape[0] < Bt:
-        require(False, f"state holds {state.shape[0]} slots, the batch {Bt}")
+    if state_indices is None and ss[0] < Bt:
+        require(False, f"state holds {ss[0]} slots, the batch {Bt}")
     idx, idx64 = slot_args(state_indices, Bt, u)
     dev = check_device(state, u, delta, A, B, C, D, z, delta_bias, state_indices)
     dt = io_dtype(u, delta, B, C, z)
-    uu, dd, bb, cc, zz = (rows(t, dt) for t in (u, delta, B, C, z))
+    uu, dd, bb, cc, zz = rows(u, dt), rows(delta, dt), rows(B, dt), rows(C, dt), rows(z, dt)
     aa, sk, bias = f32(A), f32(D), f32(delta_bias)
-    y = torch.empty(Bt, Dn, dtype=dt, device=dev)
+    y = torch.empty(ushape, dtype=dt, device=dev)
+    bs, cs = bb.stride(), cc.stride()
     call("tops_gla_selective_scan_step", _STEP.pack(
         state.data_ptr(), uu.data_ptr(), dd.data_ptr(), address(zz), bb.data_ptr(), cc.data_ptr(),
-        aa.data_ptr(), address(sk), address(bias), y.data_ptr(), idx, idx64, state.shape[0], Bt,
-        Dn, N, G, ss[0], uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0),
-        bb.stride(0), bb.stride(1) if G > 1 else 0, cc.stride(0), cc.stride(1) if G > 1 else 0,
-        int(bool(delta_softplus)), dtype_code(dt)), stream_of(dev))
-    return y if dt == u.dtype else y.to(u.dtype)
+        aa.data_ptr(), address(sk), address(bias), y.data_ptr(), idx, idx64, ss[0], Bt, Dn, N, G,
+        st[0], uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0), bs[0],
+        bs[1] if G > 1 else 0, cs[0], cs[1] if G > 1 else 0, 1 if delta_softplus else 0,
+        dtype_code(dt)), stream_of(dev))
+    return y if dt is u.dtype else y.to(u.dtype)
