@@ -75,35 +75,31 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
 
-// log(1 + e^x) and its derivative. With w = e^-|x| and u = 1 + w rounded, log(1 + w) = log(u) +
+// log(1 + e^x), and its derivative. With w = e^-|x| and u = 1 + w rounded, log(1 + w) = log(u) +
 // (w - (u - 1)) / u to second order, which keeps the relative accuracy of a small result; the
-// exponent's rounding is put back to first order, as it grows with |x|.
-// log(1 + e^x) alone, in fewer steps: e^-|x| is cut at |x| = 104, where float32 has nothing left
-// of it, so that infinities need no case of their own (the minimum passes a NaN on), and the
-// second-order term's 1 / u is 1 - w / 2, as that term is at most half a step of u.
-__device__ __forceinline__ float softplus(float x) {
-  const float L2E = 1.4426950408889634f, L2E_LO = 1.9259629911266175e-8f, LN2 = 0.6931471805599453f;
+// exponent's rounding is put back to first order, as it grows with |x|. w is cut at |x| = 104,
+// where float32 has nothing left of it, so that infinities need no case of their own (the minimum
+// passes a NaN on).
+__device__ __forceinline__ float exp_minus_abs(float x) {
+  const float L2E = 1.4426950408889634f, L2E_LO = 1.9259629911266175e-8f;
   const float ax = __builtin_elementwise_minimum(fabsf(x), 104.f);
   const float e = -ax * L2E;
   const float r = fmaf(-ax, L2E_LO, fmaf(-ax, L2E, -e));   // what the product lost
-  const float w0 = __builtin_amdgcn_exp2f(e), w = fmaf(w0 * r, LN2, w0);
-  const float u = 1.f + w;
-  const float l = fmaf(w - (u - 1.f), fmaf(-0.5f, w, 1.f), __builtin_amdgcn_logf(u) * LN2);
-  return fmaxf(x, 0.f) + l;
+  const float w = __builtin_amdgcn_exp2f(e);
+  return fmaf(w * r, 0.6931471805599453f, w);
 }
-
 __device__ __forceinline__ void softplus_sigmoid(float x, float& sp, float& sg) {
-  const float L2E = 1.4426950408889634f, L2E_LO = 1.9259629911266175e-8f;
-  const float ax = fabsf(x);
-  const float e = -ax * L2E;
-  float r = -fmaf(ax, L2E, e);            // what the product lost
-  r = fmaf(-ax, L2E_LO, r);
-  float w = __builtin_amdgcn_exp2f(e);
-  w = w > 0.f ? fmaf(w, r * 0.6931471805599453f, w) : 0.f;   // |x| = inf: r is NaN, w is 0
-  const float u = 1.f + w, iu = __builtin_amdgcn_rcpf(u);
-  const float l = fmaf(w - (u - 1.f), iu, __builtin_amdgcn_logf(u) * 0.6931471805599453f);
-  sp = x != x ? x : fmaxf(x, 0.f) + l;
-  sg = x != x ? x : x >= 0.f ? iu : w * iu;
+  const float w = exp_minus_abs(x), u = 1.f + w, iu = __builtin_amdgcn_rcpf(u);
+  sp = fmaxf(x, 0.f) +
+       fmaf(w - (u - 1.f), iu, __builtin_amdgcn_logf(u) * 0.6931471805599453f);
+  sg = x >= 0.f ? iu : w * iu;
+}
+// log(1 + e^x) alone: the second-order term is at most half a step of u, so that 1 - w / 2 does
+// for its 1 / u.
+__device__ __forceinline__ float softplus(float x) {
+  const float w = exp_minus_abs(x), u = 1.f + w;
+  return fmaxf(x, 0.f) + fmaf(w - (u - 1.f), fmaf(-0.5f, w, 1.f),
+                              __builtin_amdgcn_logf(u) * 0.6931471805599453f);
 }
 
 }  // namespace tops

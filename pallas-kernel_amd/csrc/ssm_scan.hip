@@ -121,21 +121,13 @@ __device__ __forceinline__ void pin(float (&x)[8]) {
                  "+v"(x[6]), "+v"(x[7]));
 }
 
-// Waits here for a scalar row.
-template <int N>
-__device__ __forceinline__ void arrived(float (&x)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 8)
-    asm volatile(""
-                 : "+s"(x[i]), "+s"(x[i + 1]), "+s"(x[i + 2]), "+s"(x[i + 3]), "+s"(x[i + 4]),
-                   "+s"(x[i + 5]), "+s"(x[i + 6]), "+s"(x[i + 7]));
+// Eight floats of a row, in eight scalar registers in a row as a scalar load leaves them.
+typedef float row8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ row8 load_row(cfloat* p) {
+  return *(const row8 __attribute__((address_space(4)))*)p;
 }
-
-template <int N>
-__device__ __forceinline__ void load_row(cfloat* p, float (&x)[N]) {
-#pragma unroll
-  for (int n = 0; n < N; ++n) x[n] = p[n];
-}
+// Waits here for them.
+__device__ __forceinline__ void arrived(row8& x) { asm volatile("" : "+s"(x)); }
 
 // B and C as float32 rows [token][group][2][NP], zeros past N and in one more row, which stands
 // for the tokens past a piece's end; then A log2(e) as rows of D channels [NP][D].
@@ -254,13 +246,19 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
 #pragma unroll
       for (int g = 0; g < NP; g += GN) {
         float(&hg)[GN] = *reinterpret_cast<float(*)[GN]>(&h[g]);
-        float rb[GN], rc[GN];
+        row8 rb[GN / 8], rc[GN / 8];
         asm volatile("" : : "s"(ahead[0]), "s"(ahead[1]));
         cfloat* row = row_after(at, hg);
-        load_row(row + g, rb);
-        if (MODE == 1) load_row(row + NP + g, rc);
-        arrived(rb);
-        if (MODE == 1) arrived(rc);
+#pragma unroll
+        for (int i8 = 0; i8 < GN / 8; ++i8) {
+          rb[i8] = load_row(row + g + 8 * i8);
+          if (MODE == 1) rc[i8] = load_row(row + NP + g + 8 * i8);
+        }
+#pragma unroll
+        for (int i8 = 0; i8 < GN / 8; ++i8) {
+          arrived(rb[i8]);
+          if (MODE == 1) arrived(rc[i8]);
+        }
         const bool more = g + GN < NP;
         if (more || j + 1 < FT) {   // the next rows into the scalar cache
           cfloat* np = more ? row + g + GN
@@ -272,10 +270,10 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
         for (int n = 0; n < GN; ++n) {
           const float ex = exp2_hw(A[g + n] * d[i]);
           if (MODE == 2) {
-            hg[n] = ex * fmaf(x, rb[n], hg[n]);
+            hg[n] = ex * fmaf(x, rb[n / 8][n % 8], hg[n]);
           } else {
-            hg[n] = fmaf(ex, hg[n], x * rb[n]);
-            if (MODE == 1) acc[n & 1] = fmaf(hg[n], rc[n], acc[n & 1]);
+            hg[n] = fmaf(ex, hg[n], x * rb[n / 8][n % 8]);
+            if (MODE == 1) acc[n & 1] = fmaf(hg[n], rc[n / 8][n % 8], acc[n & 1]);
           }
         }
         if (MODE == 1) asm volatile("" : "+v"(acc[0]), "+v"(acc[1]));   // like h: now
@@ -495,14 +493,19 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd
 #pragma unroll 1
   for (int k = nt - 1; k >= 0; --k) {
     const int t0 = pc.t0 + k * SS_K, ts = part * L::TPW;
+    float sd[L::TPW], sg[L::TPW];
+#pragma unroll
+    for (int i = 0; i < L::TPW; ++i) sd[i] = to_f32(rd[i]) + bias, sg[i] = 1.f;
+    if (softplus)
+#pragma unroll
+      for (int i = 0; i < L::TPW; ++i) softplus_sigmoid(sd[i], sd[i], sg[i]);
 #pragma unroll
     for (int i = 0; i < L::TPW; ++i) {
       const bool in = live && t0 + ts + i < pc.t1;
-      float d = to_f32(rd[i]) + bias, sg = 1.f;
-      if (softplus) softplus_sigmoid(d, d, sg);
+      const float d = sd[i];
       const float dy = to_f32(ry[i]), z = has_z ? to_f32(rz[i]) : 0.f;
       const float sz = sigmoid(z), g = has_z ? dy * z * sz : dy;
-      sK[0][ts + i][col] = sg;
+      sK[0][ts + i][col] = sg[i];
       sK[1][ts + i][col] = dy * (sz * fmaf(z, 1.f - sz, 1.f));   // dy silu'(z)
       sD[ts + i][col] = in ? d : 0.f;
       sU[ts + i][col] = in ? to_f32(ru[i]) : 0.f;
@@ -517,8 +520,8 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd
     // registers, delta', u and dy from LDS. One counter stands for both kinds of loads, and the
     // scalar ones come in any order: a wait has to be for all of them, before the next are sent.
     const float* rows = bc + t0 * bc_st;
-    float nb[8], nc[8], nd, nu, ng, av[HK][8], hv[HK][8];
-    load_row(row_after(rows, hin), nb);
+    float nd, nu, ng, av[HK][8], hv[HK][8];
+    row8 nb = load_row(row_after(rows, hin)), nc;
     __syncthreads();
     nd = sD[0][col];
     nu = sU[0][col];
@@ -527,15 +530,13 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd
       constexpr bool back = is_back(e), nback = is_back(e + 1);
       constexpr int t = token_of(e), tn = token_of(e + 1), s = t % HK;
       float(&h0)[8] = sweep < 3 ? hm : hin;
-      float rb[8], rc[8];
       arrived(nb);
       asm volatile("" : "+v"(nd), "+v"(nu));
       if constexpr (back) {
         arrived(nc);
         asm volatile("" : "+v"(ng));
       }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) rb[n] = nb[n], rc[n] = back ? nc[n] : 0.f;
+      const row8 rb = nb, rc = nc;
       const float d = nd, x = d * nu, dy = ng;
       if constexpr (e + 1 < 5 * HK) {
         const float* at = t0 + tn < pc.t1 ? rows + tn * bc_st : bc_end;
@@ -546,8 +547,8 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd
           row = row_after(at, h0);
         else
           row = row_after(at, hv[s - 1]);
-        load_row(row, nb);
-        if (nback) load_row(row + NP, nc);
+        nb = load_row(row);
+        if (nback) nc = load_row(row + NP);
         nd = sD[tn][col];
         nu = sU[tn][col];
         if (nback) ng = sG[tn][col];
