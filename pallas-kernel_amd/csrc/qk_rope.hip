@@ -1,11 +1,14 @@
 // Norms of queries and keys for each head with the position rotation in the same pass, forward
 // and backward (include/tops_gla_ssm.h).
 //
-// Bound by memory: a head's row is read and written once. LPR lanes hold a row, VEC elements
-// each, so that its mean square is a sum over LPR lanes; the partner of a rotated element is
-// read again (it is in the cache) instead of moved between lanes. cos and sin of a token's angles
-// are formed once for all its heads, in LDS: the angle is taken in turns in 64 bits, where a far
-// position times a frequency keeps its fraction, and only the fraction is rounded to 32.
+// Bound by memory: a head's row is read and written once. LPR lanes hold a row, VEC elements each,
+// so that its mean square is a sum over LPR lanes; a rotated element's partner comes from its lane.
+// cos and sin of a token's angles are formed once for all its heads, in LDS: the angle is taken in
+// turns in 64 bits, where a far position times a frequency keeps its fraction, and only the fraction
+// is rounded to 32. MI355X, B4 T8192 H16+16 D128 bf16: forward 112 us (4.7 TB/s), backward 164 (4.9).
+//
+// Heads of an odd size and rows at odd addresses take the first two kernels, an element (or, above
+// 256 columns, four) a lane and the partner read again.
 #include "ssm.hpp"
 
 namespace tops {
@@ -630,8 +633,8 @@ __global__ __launch_bounds__(QK_NT) void qk_bwd_rows_kernel(tops_gla_qk_args a, 
 constexpr long kQkBlocks = 1024;   // of the backward: rows of partial weight gradients
 
 // Tokens of a block at a time, as long as the blocks fill the device: a block whose threads have
-// several batches of rows pays less for its start (64 heads of 128 columns, 32768 tokens: 161 us
-// forward with 64 rows a batch and part in all, 115 with 256; backward 174 and 164 with 128).
+// several batches of rows pays less for its start (16 + 16 heads of 128 columns, 32768 tokens: 161 us
+// forward with 4 tokens a block, 115 with 16; backward 174 with 4, 164 with 8).
 int tokens_per_block(long tokens, long heads, bool backward) {
   int tb = 1;
   while (tb < QK_MAXTB && tb * heads < (backward ? 256 : 512) && tokens >= 2048L * tb) tb *= 2;

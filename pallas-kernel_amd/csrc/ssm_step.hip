@@ -2,7 +2,8 @@
 // a serving batch, the states updated in place (include/tops_gla_ssm.h).
 //
 // Both are bound by the states' traffic (a row's state is read and written once), and for a few
-// rows by the launch.
+// rows by the launch. MI355X: scan, 128 rows of 4096 channels, N 16: 15.8 us (4.5 TB/s), one row of
+// 2048 channels 3.2; convolution, W 4: 4.1 and 2.4.
 #include "ssm.hpp"
 
 namespace tops {
