@@ -76,7 +76,8 @@ int tops_gla_selective_scan_bwd(const tops_gla_scan_args *a, void *stream);
 /* Bytes of `ws`, and the tokens of a piece that fill the device for such a call. */
 int64_t tops_gla_selective_scan_bwd_ws_bytes(int64_t tokens, int64_t nsegs, int64_t D, int64_t N,
                                              int64_t G);
-int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t D, int64_t N, int64_t G);
+int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t nseq, int64_t D, int64_t N,
+                                      int64_t G);
 /* Tokens between the states that the forward keeps (0 for an N that is refused). */
 int64_t tops_gla_selective_scan_chunk(int64_t N);
 

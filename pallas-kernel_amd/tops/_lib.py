@@ -88,7 +88,7 @@ _SSM_SIGS = {
     "tops_gla_selective_scan_fwd": [_S, _P],
     "tops_gla_selective_scan_bwd": [_S, _P],
     "tops_gla_selective_scan_bwd_ws_bytes": [_I64] * 5,
-    "tops_gla_selective_scan_piece": [_I64] * 4,
+    "tops_gla_selective_scan_piece": [_I64] * 5,
     "tops_gla_selective_scan_chunk": [_I64],
     "tops_gla_selective_scan_step": [_S, _P],
     "tops_gla_causal_conv_fwd": [_S, _P],

@@ -22,7 +22,8 @@ class _Pieces:
     def __init__(self, B, T, D, N, G, cu, device):
         lib = _lib.load()
         chunk = int(lib.tops_gla_selective_scan_chunk(N))
-        self.piece = int(lib.tops_gla_selective_scan_piece(B * T, D, N, G))
+        # packed sequences differ in length: the longest ones are cut however many there are
+        self.piece = int(lib.tops_gla_selective_scan_piece(B * T, B if cu is None else 1, D, N, G))
         self.table = None
         if cu is None:
             per = max(1, -(-T // self.piece))

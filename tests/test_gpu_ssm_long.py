@@ -160,3 +160,24 @@ def test_packed_sequences_in_a_graph():
         with pytest.raises(RuntimeError, match="capture"):
             with torch.cuda.graph(other):
                 step([0, 7, 300])
+
+
+def test_scan_of_uncut_sequences():
+    """A batch that fills the device is not cut into pieces: the same values as a few of its rows,
+    which are cut, to float32 roundings (an output's sum has the state of up to 200 tokens before
+    it, each good to 4 roundings of the largest magnitude)."""
+    B, T, D, N = 256, 200, 512, 16
+    x, r = scan_tests.make(B, T, D, N, torch.float32)
+    d = {n: t.to(DEV).requires_grad_() for n, t in x.items()}
+    y, ht = selective_scan(**d, delta_softplus=True, output_final_state=True)
+    dy = r(B, T, D).to(DEV)
+    names = ["u", "delta", "z", "B", "C", "initial_state"]
+    got = torch.autograd.grad(y, [d[n] for n in names], dy)
+    rows = [0, 101, 255]
+    ref, mag = scan_tests.reference({n: t[rows] if t.shape[0] == B else t for n, t in x.items()},
+                                    True, None, dy[rows].cpu(), torch.zeros(3, D, N))
+    terms = 4 * T + 64
+    close("y", y[rows], ref["y"], mag["y"], terms)
+    close("ht", ht[rows], ref["ht"], mag["ht"], terms)
+    for n, g in zip(names, got):
+        close("d" + n, g[rows], ref["d" + n], mag["d" + n], terms + T + D)
