@@ -172,8 +172,11 @@ int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t nseq, int64_t D, i
   // costs more than the third to eighth wave give (D4096 N16 bf16, forward, whole and cut: 2048
   // waves of 256 tokens 200 and 293 us, 4096 of 128 157 and 315; but 1024 of 512 321 and 273)
   if (nseq * tiles_of(D, G) * G >= 2048) return 1 << 30;
-  // eight waves a SIMD, which take turns, and at most 512 pieces for the fold to walk
-  const int64_t len = std::max((tokens * tiles_of(D, G) * G + 8191) / 8192, (tokens + 511) / 512);
+  // as many waves a SIMD as their states in registers allow, eight with 16 of them, and at most 512
+  // pieces for the fold to walk
+  const int64_t np = tops::scan_state_pad((int)N), waves = np <= 16 ? 8192 : 131072 / np;
+  const int64_t len =
+      std::max((tokens * tiles_of(D, G) * G + waves - 1) / waves, (tokens + 511) / 512);
   return std::min<int64_t>(std::max<int64_t>(16, (len + 15) / 16 * 16), 1 << 30);
 }
 

@@ -388,14 +388,16 @@ struct Lane {
       }
     }
   }
+  // whether an element is the second one of its pair, which the first is added to when it turns
+  __device__ __forceinline__ bool second(int e) const { return EACH ? hie[e] : hi; }
   // column of the partner's piece
   __device__ __forceinline__ int pc(int R) const {
     return INTER || !rot ? c : hi ? c - R / 2 : c + R / 2;
   }
 };
 
-// The values of a piece's partners.
-template <typename T, int VEC, int LPR, bool INTER>
+// The values of a piece's partners; BACK: those of second elements negated, as a turn back has them.
+template <bool BACK, typename T, int VEC, int LPR, bool INTER>
 __device__ __forceinline__ void partners(const Piece<T, VEC>& x, const Lane<VEC, LPR, INTER>& l,
                                          float (&p)[VEC]) {
   if constexpr (Lane<VEC, LPR, INTER>::EACH) {
@@ -409,15 +411,22 @@ __device__ __forceinline__ void partners(const Piece<T, VEC>& x, const Lane<VEC,
         r.w[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(l.lane4e[e], (int)x.w[i]);
       piece_values<T, VEC>(r, v);
       p[e] = l.odd ? v[1 - e] : v[e];
+      if (BACK && l.hie[e]) p[e] = -p[e];
     }
   } else if constexpr (!INTER) {
     Piece<T, VEC> r = x;
     piece_of_lane<T, VEC>(r, l.lane4);
+    if (BACK) {
+      const uint32_t flip = l.hi ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+      for (int i = 0; i < Piece<T, VEC>::W; ++i) r.w[i] ^= flip;
+    }
     piece_values<T, VEC>(r, p);
   }
 }
 
-// x turned by a token's angles cs (sign -1: back), xp being its partners.
+// x turned by a token's angles cs, xp being its partners with their signs; whole pairs (INTER) turn
+// by sign times the angles.
 template <int VEC, int LPR, bool INTER>
 __device__ __forceinline__ void turn_piece(float (&x)[VEC], const float (&xp)[VEC],
                                            const float2* cs, const Lane<VEC, LPR, INTER>& l, int R,
@@ -427,10 +436,16 @@ __device__ __forceinline__ void turn_piece(float (&x)[VEC], const float (&xp)[VE
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float2 k = cs[l.fe[e]];
-        x[e] = fmaf(xp[e], l.hie[e] ? sign * k.y : -sign * k.y, x[e] * k.x);
+        x[e] = fmaf(xp[e], k.y, x[e] * k.x);
       }
-  } else {
+  } else if constexpr (INTER) {
     turn<VEC, INTER>(x, xp, cs + l.f, l.rot, l.hi, l.c, R, sign);
+  } else if (l.rot) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float2 k = cs[l.f + e];
+      x[e] = fmaf(xp[e], k.y, x[e] * k.x);
+    }
   }
 }
 
@@ -475,6 +490,7 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
     for (int e = 0; e < VEC; ++e) {
       wv[e] = w ? w[cl + e] : 1.f;
       wp[e] = !w ? 1.f : Lane<VEC, LPR, INTER>::EACH ? w[l.in ? l.pe[e] : 0] : w[pc + e];
+      if (PAIR && !l.second(e)) wp[e] = -wp[e];   // the sign of a pair's first half
     }
   };
   if (nb > 0) load(0);
@@ -499,21 +515,20 @@ __global__ __launch_bounds__(QK_NT) void qk_fwd_rows_kernel(tops_gla_qk_args a, 
       const int r = r0 + u * RPB;
       float v[VEC], p[VEC], ss = 0.f;
       piece_values<T, VEC>(x[u], v);
-      if (PAIR) partners(x[u], l, p);
+      if (PAIR) partners<false>(x[u], l, p);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) ss = fmaf(v[e], v[e], ss);
+      const float rstd = rsqrtf(fmaf(row_sum<LPR>(l.in ? ss : 0.f), inv_d, eps));
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (!l.in) v[e] = 0.f;
-        ss = fmaf(v[e], v[e], ss);
-      }
-      const float rstd = rsqrtf(fmaf(row_sum<LPR>(ss), inv_d, eps));
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        v[e] *= rstd * wv[e];
-        if (PAIR) p[e] *= rstd * wp[e];
+        v[e] *= wv[e];
+        if (PAIR) p[e] *= wp[e];
       }
       if (r < rows && l.in) {
         const int tk = H == 1 ? r : (int)__umulhi((uint32_t)r, magic);
         turn_piece<VEC, LPR, INTER>(v, p, cs + tk * R2, l, R, 1.f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] *= rstd;
         store_run<T, VEC>(dst + (long)r * D + l.c, v);
       }
     }
@@ -591,16 +606,15 @@ __global__ __launch_bounds__(QK_NT) void qk_bwd_rows_kernel(tops_gla_qk_args a, 
         float v[VEC], d[VEC], p[VEC], ss = 0.f, em = 0.f;
         piece_values<T, VEC>(x[u], v);
         piece_values<T, VEC>(gy[u], d);
-        if (PAIR) partners(gy[u], l, p);
+        if (PAIR) partners<true>(gy[u], l, p);
         turn_piece<VEC, LPR, INTER>(d, p, cs + tk * R2, l, R, -1.f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          if (!on) v[e] = d[e] = 0.f;
           ss = fmaf(v[e], v[e], ss);
           em = fmaf(d[e] * wv[e], v[e], em);
         }
-        const float rstd = rsqrtf(fmaf(row_sum<LPR>(ss), inv_d, eps));
-        const float mean = row_sum<LPR>(em) * rstd * inv_d;
+        const float rstd = rsqrtf(fmaf(row_sum<LPR>(l.in ? ss : 0.f), inv_d, eps));
+        const float mean = row_sum<LPR>(l.in ? em : 0.f) * rstd * inv_d;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float m = v[e] * rstd, t = on ? d[e] * m : 0.f;

@@ -442,7 +442,7 @@ __device__ __forceinline__ float sum_channels(float (&x)[8], float (&y)[8]) {
 }
 
 template <typename T, int NP>
-__global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 8 ? 2 : 3) void scan_bwd_kernel(ScanParams p) {
+__global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) void scan_bwd_kernel(ScanParams p) {
   using L = Bwd<NP>;
   __shared__ float sD[SS_K][L::CT], sU[SS_K][L::CT], sG[SS_K][L::CT];   // delta', u, dy silu(z)
   __shared__ float sK[2][SS_K][L::CT];          // softplus', dy silu'(z): for the wave that staged them
