@@ -181,3 +181,58 @@ def test_scan_of_uncut_sequences():
     close("ht", ht[rows], ref["ht"], mag["ht"], terms)
     for n, g in zip(names, got):
         close("d" + n, g[rows], ref["d" + n], mag["d" + n], terms + T + D)
+
+
+def far(t, buf, at):
+    """t's rows 2^26 elements apart in `buf`, from column `at` on: the last ones past 2^31."""
+    v = buf[at:].as_strided(t.shape, (0, (1 << 26) + 8, *t.stride()[2:]))
+    v.copy_(t)
+    return v
+
+
+def test_offsets_past_32_bits():
+    T, D, N = 40, 136, 16
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    buf = torch.empty(T * ((1 << 26) + 8) + 4096, dtype=torch.bfloat16, device=DEV)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).bfloat16()   # noqa: E731
+    near = {n: r(1, T, D) for n in ("u", "delta", "z", "dy")} | {n: r(1, T, N) for n in ("B", "C")}
+    A, w = -torch.rand(D, N, generator=gen, device=DEV), r(D, 4)
+    freq = rotary_inv_freq(8, device=DEV)
+    x = {n: far(t, buf, 256 * i) for i, (n, t) in enumerate(near.items())}
+    got, want = [], []
+    for out, v in ((want, near), (got, x)):
+        v = {n: t.detach().requires_grad_(n != "dy") for n, t in v.items()}
+        y, _ = selective_scan(v["u"], v["delta"], A, v["B"], v["C"], z=v["z"], delta_softplus=True)
+        out += [y, *torch.autograd.grad(y, [v[n] for n in ("u", "delta", "z", "B", "C")], v["dy"])]
+        y, _ = causal_conv1d(v["u"], w, None, "silu")
+        out += [y, *torch.autograd.grad(y, [v["u"]], v["dy"])]
+        q, k, dq = (v[n].unflatten(2, (17, 8)) for n in ("u", "delta", "dy"))
+        o = qk_norm_rope(q, k, None, None, freq)
+        out += [*o, *torch.autograd.grad(o, [q, k], [dq, dq])]
+    assert x["C"].data_ptr() + 2 * x["C"].stride(1) * (T - 1) - buf.data_ptr() > 1 << 32
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_slots_past_32_bits():
+    from tops.ops.ssm import causal_conv1d_step, selective_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)   # noqa: E731
+    D, N, W = 2048, 16, 4
+    slots = torch.tensor([70000, 3, 65536], dtype=torch.int64, device=DEV)   # times 2^15 floats
+    few = torch.arange(3, device=DEV)
+    small, pool = r(3, D, N), torch.empty(70001, D, N, device=DEV)
+    pool[slots] = small
+    a = [r(3, D), r(3, D), -torch.rand(D, N, generator=gen, device=DEV), r(3, N), r(3, N)]
+    assert torch.equal(selective_scan_step(pool, *a, delta_softplus=True, state_indices=slots),
+                       selective_scan_step(small, *a, delta_softplus=True, state_indices=few))
+    assert torch.equal(pool[slots], small)
+    del pool
+    slots = slots * 8   # times 2^13 elements
+    small, pool = r(3, W, D).bfloat16(), torch.empty(560001, W, D, dtype=torch.bfloat16, device=DEV)
+    pool[slots] = small
+    x, w = r(3, D).bfloat16(), r(D, W)
+    assert torch.equal(causal_conv1d_step(x, pool, w, state_indices=slots),
+                       causal_conv1d_step(x, small, w, state_indices=few))
+    assert torch.equal(pool[slots], small)
