@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from ..._lib import require, to_list
+from ..._lib import require, stream_of, to_list
 
 _IO = (torch.float32, torch.bfloat16)
 
@@ -71,7 +71,7 @@ def device_table(key, make, device):
     """``make()`` -> (int32 values, anything else) with the values as a device tensor, kept by its
     key, device and stream: one stream writes, reads and frees a table, in this order. A table
     that a graph captures is kept for good, as the graph's replays read it."""
-    key = (key, str(device), torch.cuda.current_stream(device).cuda_stream)
+    key = (key, device.index, stream_of(device).value)
     capturing = torch.cuda.is_current_stream_capturing()
     hit = _tables.get(key)
     if hit is None and capturing:
@@ -84,7 +84,9 @@ def device_table(key, make, device):
         values, rest = make()
         if len(_tables) > 64:
             _tables.clear()
-        hit = _tables[key] = (torch.tensor(values, dtype=torch.int32, device=device), rest)
+        # pinned, so that the copy is one of the stream's own and nothing waits for it
+        table = torch.tensor(values, dtype=torch.int32, pin_memory=True)
+        hit = _tables[key] = (table.to(device, non_blocking=True), rest)
     if capturing and not any(h is hit for h in _held):
         _held.append(hit)
     return hit

@@ -21,9 +21,9 @@ class _Pieces:
 
     def __init__(self, B, T, D, N, G, cu, device):
         lib = _lib.load()
-        chunk = int(lib.tops_gla_selective_scan_chunk(N))
+        chunk = lib.tops_gla_selective_scan_chunk(N)
         # packed sequences differ in length: the longest ones are cut however many there are
-        self.piece = int(lib.tops_gla_selective_scan_piece(B * T, B if cu is None else 1, D, N, G))
+        self.piece = lib.tops_gla_selective_scan_piece(B * T, B if cu is None else 1, D, N, G)
         self.table = None
         if cu is None:
             per = max(1, -(-T // self.piece))
