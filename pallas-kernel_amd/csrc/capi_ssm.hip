@@ -33,6 +33,9 @@ bool any_null(std::initializer_list<const void*> ps) {
   return false;
 }
 
+// Whether a launch has fewer than 2^32 threads, as it must.
+bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (1LL << 32) / threads; }
+
 int scan_sizes(int64_t D, int64_t N, int64_t G, int64_t dtype) {
   if (!dtype_ok(dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
   if (D < 1 || D > (1 << 20)) return fail(TOPS_GLA_EINVAL, "D must be in [1, 2^20] (D=%lld)",
@@ -85,12 +88,12 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
     return fail(TOPS_GLA_EINVAL, "piece_dt is required with piece_h");
   const int64_t np = tops::scan_state_pad((int)a->N);
   p->tiles_g = (int)tiles_of(a->D, a->G);
-  if (p->tiles_g * a->G * std::max<int64_t>(p->npieces, 1) > kMax ||
-      (a->D + 63) / 64 * np * a->nseq > kMax)
+  p->btiles = (int)(bwd_tiles_of(a->D, a->N, a->G) * a->G);
+  if (!grid_fits((p->tiles_g * a->G * p->npieces + 3) / 4, 256) ||
+      (backward && !grid_fits(p->btiles * p->npieces, tops::scan_bwd_threads((int)a->N))))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   p->ntiles = p->tiles_g * (int)a->G;
   p->at = a->bc + (p->tokens * a->G + 1) * 2 * np;
-  p->btiles = (int)(bwd_tiles_of(a->D, a->N, a->G) * a->G);
   if (any_null({a->A})) return fail(TOPS_GLA_EINVAL, "A must not be NULL");
   if (p->tokens > 0 && (any_null({a->u, a->delta}) || (!backward && any_null({a->B, a->C}))))
     return fail(TOPS_GLA_EINVAL, "u, delta, B and C must not be NULL");
@@ -136,8 +139,10 @@ int conv_check(const tops_gla_conv_args* a) {
     return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
   if (a->cu == nullptr ? a->nseq != a->batch : a->batch != 1)
     return fail(TOPS_GLA_EINVAL, "packed sequences require batch == 1, others nseq == batch");
-  const int64_t slabs = (a->D + 63) / 64;
-  if (slabs * (a->batch * a->T / 32 + 2) > kMax || slabs * (2 * a->nseq + 2) > kMax)
+  const int64_t vec = 8 / (a->dtype == TOPS_GLA_BF16 ? 2 : 4), per = 64 * (a->D < vec ? 1 : vec);
+  const int64_t tiles = tops::causal_conv_part_rows(a->batch * a->T, a->D);
+  if (a->nseq > kMax || !grid_fits((a->D + per - 1) / per * (tiles + (a->nseq * a->W + 3) / 4), 256) ||
+      !grid_fits((a->D + 255) / 256 * a->nseq, 256))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   if (a->w == nullptr) return fail(TOPS_GLA_EINVAL, "w must not be NULL");
   if (a->batch * a->T > 0 && a->x == nullptr) return fail(TOPS_GLA_EINVAL, "x must not be NULL");
@@ -158,6 +163,8 @@ int qk_check(const tops_gla_qk_args* a) {
     return fail(TOPS_GLA_EINVAL, "bad batch, T, Hq or Hk");
   if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMax)
     return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
+  if (!grid_fits(tops::qk_norm_rope_blocks(a->batch * a->T, a->Hq + a->Hk), 256))
+    return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   return TOPS_GLA_OK;
 }
 
@@ -207,7 +214,9 @@ int tops_gla_selective_scan_step(const tops_gla_scan_step_args* a, void* stream)
   if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
   if (int rc = scan_sizes(a->D, a->N, a->G, a->dtype)) return rc;
   if (int rc = slots_ok(a->batch, a->slots, a->slots_idx)) return rc;
-  if (a->batch * ((a->D + 15) / 16) > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  // 4 of a row's states a lane; many rows go in pairs
+  const int64_t cpb = 256 / (a->N <= 4 ? 1 : tops::scan_state_pad((int)a->N) / 4);
+  if (a->batch > kMax || !grid_fits((a->D + cpb - 1) / cpb * ((a->batch + 1) / 2), 256)) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   if (a->batch > 0 && any_null({a->u, a->delta, a->B, a->C, a->A, a->y}))
     return fail(TOPS_GLA_EINVAL, "u, delta, A, B, C and y must not be NULL");
   if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
@@ -245,7 +254,7 @@ int tops_gla_causal_conv_step(const tops_gla_conv_step_args* a, void* stream) {
   if (a->W < 1 || a->W > 8)
     return fail(TOPS_GLA_EUNSUPPORTED, "kernel width W in 1..8 (W=%lld)", (long long)a->W);
   if (int rc = slots_ok(a->batch, a->slots, a->slots_idx)) return rc;
-  if (a->batch * ((a->D + 255) / 256) > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->batch > kMax || !grid_fits(a->batch * ((a->D + 255) / 256), 256)) return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   if (a->batch > 0 && any_null({a->x, a->w, a->y}))
     return fail(TOPS_GLA_EINVAL, "x, w and y must not be NULL");
   if (a->batch > 0 && a->slots > 0 && a->state == nullptr)

@@ -781,6 +781,10 @@ hipError_t qk_rows(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
 
 }  // namespace
 
+long qk_norm_rope_blocks(long tokens, long heads) {
+  const long tb = tokens_per_block(tokens, heads, false);
+  return (tokens + tb - 1) / tb;
+}
 long qk_norm_rope_part_rows(long tokens) { return std::min(tokens, kQkBlocks); }
 
 hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_t st) {

@@ -27,6 +27,7 @@ struct ScanParams {
 };
 int scan_state_pad(int N);       // N rounded up to 8, 16, 32 or 64
 int scan_bwd_channels(int N);    // channels of a block of the backward
+int scan_bwd_threads(int N);     // and threads
 int scan_chunk();                // tokens between the states kept for the backward
 hipError_t run_selective_scan(const ScanParams& p, bool backward, hipStream_t st);
 
@@ -39,6 +40,7 @@ long causal_conv_part_rows(long tokens, long D);   // rows of (W + 1) D partial 
 
 hipError_t run_qk_norm_rope(const tops_gla_qk_args& a, bool backward, hipStream_t st);
 long qk_norm_rope_part_rows(long tokens);  // rows of 2 D partial weight gradients
+long qk_norm_rope_blocks(long tokens, long heads);   // of the forward, 256 threads each
 
 // Four elements at an address that is a multiple of theirs.
 __device__ __forceinline__ void load_four(const float* p, float (&x)[4]) {

@@ -317,15 +317,16 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
 // pieces are read once.
 constexpr int FOLD_R = 4, FOLD_U = 16, FOLD_NT = 64 * FOLD_R;
 template <int NP, bool REV>
-__global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p, int nb) {
+__global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p) {
   __shared__ float sL[FOLD_R][64], sS[FOLD_R][64];
   const tops_gla_scan_args& a = p.a;
-  const int seq = uni(blockIdx.x / nb);
-  const long pi = a.segs ? a.segs[8L * seq + 6] : (long)seq * p.pieces;
+  const long seq = blockIdx.y + (long)blockIdx.z * gridDim.y;
+  if (seq >= a.nseq) return;
+  const long pi = a.segs ? a.segs[8 * seq + 6] : seq * p.pieces;
   const int np = uni(piece_of(p, (int)pi).np), m = (np + FOLD_R - 1) / FOLD_R;
   const int run = uni(threadIdx.x / 64), c = threadIdx.x % 64;
   const int D = (int)a.D, N = (int)a.N;
-  const int n = uni((blockIdx.x - seq * nb) % NP), d = (blockIdx.x - seq * nb) / NP * 64 + c;
+  const int n = blockIdx.x % NP, d = blockIdx.x / NP * 64 + c;
   const long nd = (long)D * NP;
   if (d >= D) return;   // the same lanes of every wave: their columns of sL and sS are not used
   const int j0 = min(np, run * m), j1 = min(np, j0 + m);
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p, int nb
   sL[run][c] = h;
   sS[run][c] = s;
   __syncthreads();
-  h = n < N && init ? init[((long)seq * D + d) * N + n] : 0.f;
+  h = n < N && init ? init[(seq * D + d) * N + n] : 0.f;
   for (int r = 0; r < run; ++r) {
     const float l = sL[r][c];
     h = h == 0.f ? l : fmaf(exp2_hw(A * sS[r][c]), h, l);
@@ -427,7 +428,7 @@ struct Bwd {
       "v_add_f32_dpp %1, %5, %5 " ctrl " row_mask:0xf bank_mask:" odd "\n\t"                    \
       "v_add_f32_dpp %2, %6, %6 " ctrl " row_mask:0xf bank_mask:" odd "\n\t"                    \
       "v_add_f32_dpp %3, %7, %7 " ctrl " row_mask:0xf bank_mask:" odd "\n\ts_nop 1"              \
-      : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3)                                                  \
+      : "+&v"(a0), "+&v"(a1), "+&v"(a2), "+&v"(a3)                                              \
       : "v"(b0), "v"(b1), "v"(b2), "v"(b3))
 
 // x[0..7] and y[0..7] summed over the 64 lanes: lane l ends with element 4 l[2] + 2 l[4] + l[5]
@@ -713,9 +714,10 @@ unsigned grid_of(long threads) {
 
 template <int NP, bool REV>
 hipError_t scan_fold(const ScanParams& p, hipStream_t st) {
-  const int nb = (int)((p.a.D + 63) / 64) * NP;
-  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), dim3((unsigned)(nb * p.a.nseq)),
-                     dim3(FOLD_NT), 0, st, p, nb);
+  // a sequence in y and z: all in x, many packed sequences would be 2^32 threads and more
+  const unsigned y = (unsigned)std::clamp<long>(p.a.nseq, 1, 65535);
+  const dim3 grid((unsigned)((p.a.D + 63) / 64 * NP), y, (unsigned)((p.a.nseq + y - 1) / y));
+  hipLaunchKernelGGL((scan_fold_kernel<NP, REV>), grid, dim3(FOLD_NT), 0, st, p);
   return hipGetLastError();
 }
 
@@ -770,6 +772,7 @@ hipError_t scan_any(const ScanParams& p, bool backward, hipStream_t st) {
 
 int scan_state_pad(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int scan_chunk() { return SS_K; }
+int scan_bwd_threads(int N) { return scan_state_pad(N) == 64 ? 64 * Bwd<64>::WAVES : 64 * Bwd<32>::WAVES; }
 int scan_bwd_channels(int N) {
   switch (scan_state_pad(N)) {
     case 8: return Bwd<8>::CT;

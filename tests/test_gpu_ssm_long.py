@@ -183,6 +183,29 @@ def test_scan_of_uncut_sequences():
         close("d" + n, g[rows], ref["d" + n], mag["d" + n], terms + T + D)
 
 
+def test_scan_of_many_packed_sequences():
+    """More sequences than one dimension of the fold's grid could hold with 64 states of 1024
+    channels, one of them cut into pieces: the short ones have their own values, bit by bit."""
+    S, D, N, first = 16400, 1024, 64, 600
+    T = first + S
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)   # noqa: E731
+    x = dict(u=r(1, T, D), delta=r(1, T, D), B=r(1, T, N), C=r(1, T, N))
+    A, dy = -torch.rand(D, N, generator=gen, device=DEV), r(1, T, D)
+    cu = [0, *range(first, T + 1)]
+
+    def run(x, dy, cu):
+        x = {n: t.detach().requires_grad_() for n, t in x.items()}
+        y, _ = selective_scan(x["u"], x["delta"], A, x["B"], x["C"], delta_softplus=True,
+                              cu_seqlens=cu)
+        return [y.detach(), *torch.autograd.grad(y, list(x.values()), dy)]
+
+    alone = {n: t[0, first:].unsqueeze(1) for n, t in x.items()}
+    want = run(alone, dy[0, first:].unsqueeze(1), None)
+    for a, b in zip(run(x, dy, cu), want):
+        assert torch.equal(a[0, first:], b.squeeze(1))
+
+
 def far(t, buf, at):
     """t's rows 2^26 elements apart in `buf`, from column `at` on: the last ones past 2^31."""
     v = buf[at:].as_strided(t.shape, (0, (1 << 26) + 8, *t.stride()[2:]))
