@@ -104,16 +104,9 @@ def slot_args(idx, batch, device_of):
 
 
 def gradients(grads, like, need):
-    """The gradients in the types and shapes of their inputs, None where none is wanted."""
-    out = []
-    for g, want, n in zip(grads, like, need):
-        if g is None or not n:
-            out.append(None)
-            continue
-        if g.shape != want[1]:
-            g = g.reshape(want[1])
-        out.append(g if g.dtype is want[0] else g.to(want[0]))
-    return out
+    """The gradients in the types of their inputs, None where none is wanted."""
+    return [None if g is None or not n else g if g.dtype is dt else g.to(dt)
+            for g, dt, n in zip(grads, like, need)]
 
 
 def address(t):

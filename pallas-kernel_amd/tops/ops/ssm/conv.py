@@ -73,7 +73,8 @@ class _CausalConvFunction(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         y, fin, a, cu_t = _forward(x, weight, bias, init, silu, want, cu)
         ctx.save_for_backward(*a, cu_t)
-        ctx.like = [None if t is None else (t.dtype, t.shape) for t in (x, weight, bias, init)]
+        ctx.like = [None if t is None else t.dtype for t in (x, weight, bias, init)]
+        ctx.wshape = weight.shape
         ctx.silu, ctx.nseq = silu, x.shape[0] if cu is None else len(cu) - 1
         return y, fin
 
@@ -91,7 +92,7 @@ class _CausalConvFunction(torch.autograd.Function):
         dw = db = ws = None
         nws = 0
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw = torch.empty(D, W, dtype=w.dtype, device=dev)
+            dw = torch.empty(ctx.wshape, dtype=w.dtype, device=dev)
             db = None if b is None else torch.empty(D, dtype=w.dtype, device=dev)
             nws = int(_lib.load().tops_gla_causal_conv_bwd_ws_bytes(B * T, D, W))
             ws = torch.empty(nws, dtype=torch.uint8, device=dev)

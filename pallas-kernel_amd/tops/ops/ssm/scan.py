@@ -9,11 +9,13 @@ from torch.autograd.function import once_differentiable
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
-from ._common import (address, device_table, differentiable, f32, gradients, io_dtype, offsets, refuse_grad, rows,
-                      slot_args, strides)
+from ._common import (address, device_table, differentiable, f32, gradients, io_dtype, offsets,
+                      refuse_grad, rows, slot_args, strides)
 
 _ARGS = struct.Struct("=53q")
 _STEP = struct.Struct("=27q")
+_NO_BWD = (0,) * 15
+_NONE = (0,) * 4   # the strides of a tensor that is not there
 
 
 class _Pieces:
@@ -60,11 +62,10 @@ def _groups(t, N):
     return t if t.dim() == 4 else t.unsqueeze(2)
 
 
-def _pack(x, y, ht, chunk_h, ws, bc, pc, shape, softplus, dt, bwd=None):
+def _pack(x, y, ht, chunk_h, ws, bc, pc, shape, softplus, dt, bwd=_NO_BWD):
     Bt, T, D, N, G = shape
     u, delta, A, B, C, Dskip, z, bias, h0 = x
-    if bwd is None:
-        bwd = [0] * 15
+    us, ds, zs, bs, cs = (_NONE if t is None else t.stride() for t in (u, delta, z, B, C))
     ph = pd = 0
     if ws is not None:
         ph = ws.data_ptr()
@@ -74,8 +75,8 @@ def _pack(x, y, ht, chunk_h, ws, bc, pc, shape, softplus, dt, bwd=None):
         address(Dskip), address(bias), address(h0), address(y), address(ht), address(chunk_h),
         ph, pd, address(bc), address(pc.table),
         pc.nsegs, pc.nseq, pc.piece, Bt, T, D, N, G,
-        *strides(u, 0, 1), *strides(delta, 0, 1), *strides(z, 0, 1), *strides(B, 0, 1, 2),
-        *strides(C, 0, 1, 2), int(softplus), dtype_code(dt), *bwd)
+        us[0], us[1], ds[0], ds[1], zs[0], zs[1], *bs[:3], *cs[:3], int(softplus), dtype_code(dt),
+        *bwd)
 
 
 def _piece_states(pc, D, N, dev):
@@ -114,9 +115,8 @@ class _SelectiveScanFunction(torch.autograd.Function):
         y, ht, x, chunk_h, bc, pc = _forward(u, delta, A, B, C, D, z, bias, h0, softplus, want_ht,
                                              cu, True)
         ctx.save_for_backward(*x[:3], *x[5:8], chunk_h, bc)
-        ctx.G = x[3].shape[2]
-        ctx.like = [None if t is None else (t.dtype, t.shape)
-                    for t in (u, delta, A, B, C, D, z, bias, h0)]
+        ctx.G, ctx.bshape = x[3].shape[2], B.shape
+        ctx.like = [None if t is None else t.dtype for t in (u, delta, A, B, C, D, z, bias, h0)]
         ctx.softplus, ctx.pc = softplus, pc
         return y, ht
 
@@ -131,18 +131,17 @@ class _SelectiveScanFunction(torch.autograd.Function):
         dy = torch.zeros(Bt, T, Dn, dtype=dt, device=dev) if dy is None else rows(dy, dt)
         dht = f32(dht)
 
-        def new(*shape, dtype=torch.float32):
-            return torch.empty(*shape, dtype=dtype, device=dev)
-
-        du, ddelta = new(Bt, T, Dn, dtype=dt), new(Bt, T, Dn, dtype=dt)
-        dz = None if z is None else new(Bt, T, Dn, dtype=dt)
-        dB, dC = new(Bt, T, G, N, dtype=dt), new(Bt, T, G, N, dtype=dt)
-        dA = new(Dn, N)
-        dD = None if D is None else new(Dn)
-        dbias = None if bias is None else new(Dn)
-        dh0 = None if ctx.like[8] is None else new(pc.nseq, Dn, N)
+        new, f = torch.empty, torch.float32
+        du = new(Bt, T, Dn, dtype=dt, device=dev)
+        ddelta = new(Bt, T, Dn, dtype=dt, device=dev)
+        dz = None if z is None else new(Bt, T, Dn, dtype=dt, device=dev)
+        dB, dC = new(ctx.bshape, dtype=dt, device=dev), new(ctx.bshape, dtype=dt, device=dev)
+        dA = new(Dn, N, dtype=f, device=dev)
+        dD = None if D is None else new(Dn, dtype=f, device=dev)
+        dbias = None if bias is None else new(Dn, dtype=f, device=dev)
+        dh0 = None if ctx.like[8] is None else new(pc.nseq, Dn, N, dtype=f, device=dev)
         nws = int(_lib.load().tops_gla_selective_scan_bwd_ws_bytes(Bt * T, pc.nsegs, Dn, N, G))
-        ws, ps = new(nws, dtype=torch.uint8), _piece_states(pc, Dn, N, dev)
+        ws, ps = new(nws, dtype=torch.uint8, device=dev), _piece_states(pc, Dn, N, dev)
         bwd = [address(dy), *strides(dy, 0, 1), *(address(t) for t in (
             dht, du, ddelta, dz, dB, dC, dA, dD, dbias, dh0, ws)), nws]
         call("tops_gla_selective_scan_bwd",
