@@ -37,7 +37,7 @@ extern "C" {
  * tops_gla_selective_scan_chunk(N) tokens of a sequence, kept for the backward (NULL: not kept).
  * `bc`: B, C and A as the kernels read them, (B * T * G + 1) * 2 * NP + NP * D floats, written by
  * the forward.
- * 1 <= N <= 64.
+ * 1 <= N <= 64, B * T <= 2^31 - 64.
  */
 typedef struct tops_gla_scan_args {
   const void *u, *delta, *z;      /* [B, T, D], z NULL: no gate */

@@ -10,6 +10,8 @@
 namespace {
 
 constexpr int64_t kMax = 2147483647;
+// Tokens of a scan: its kernels form token indices of 32 bits up to a tile past a piece's end.
+constexpr int64_t kMaxScanTokens = (1LL << 31) - 64;
 
 int fail(int code, const char* fmt, ...) {
   char msg[400];
@@ -59,8 +61,8 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
   if (int rc = scan_sizes(a->D, a->N, a->G, a->dtype)) return rc;
   if (a->batch < 0 || a->T < 0 || a->nseq < 0)
     return fail(TOPS_GLA_EINVAL, "bad batch, T or nseq");
-  if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMax)
-    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 tokens");
+  if (a->T > kMax || a->batch > kMax || a->batch * a->T > kMaxScanTokens)
+    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 - 64 tokens");
   if (a->piece < 16 || a->piece % 16 || a->piece > kMax)
     return fail(TOPS_GLA_EINVAL, "piece must be a positive multiple of 16 (piece=%lld)",
                 (long long)a->piece);

@@ -50,7 +50,7 @@ __device__ __forceinline__ Piece piece_of(const ScanParams& p, int i) {
     r.seq = i / r.np;
     r.idx = i - r.seq * r.np;
     r.t0 = r.idx * len;
-    r.t1 = min(T, r.t0 + len);
+    r.t1 = r.t0 + min(T - r.t0, len);   // t0 + len may pass 32 bits
     r.c0 = r.seq * ((T + SS_K - 1) / SS_K) + r.t0 / SS_K;
     r.b = r.seq;
   }

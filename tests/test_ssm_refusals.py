@@ -256,3 +256,13 @@ def test_null_arguments():
         if sig[0] is ctypes.c_char_p:
             assert getattr(lib, name)(None, None) == 1
             assert b"NULL" in lib.tops_gla_last_error()
+
+
+@pytest.mark.parametrize("T,fits", [((1 << 31) - 64, True), ((1 << 31) - 63, False),
+                                    ((1 << 31) - 1, False)])
+def test_scan_entry_tokens(T, fits):
+    """The kernels' token indices go up to a tile past the last token, in 32 bits."""
+    rc, msg = entry("tops_gla_selective_scan_fwd", "tops_gla_scan_args",
+                    **{**SCAN, "T": T, "D": 1, "N": 1, "piece": 1 << 22, "piece_h": 64,
+                       "piece_dt": 64})
+    assert (rc, ("A must" if fits else "2^31") in msg) == (1 if fits else 2, True), msg
