@@ -84,7 +84,8 @@ int64_t tops_gla_selective_scan_chunk(int64_t N);
 /*
  * One token of the scan for each row b, its state at state[slot_b] ([slots, D, N], in place):
  * slot_b = slots_idx[b] (int32 or int64, idx64) or b. A slot outside [0, slots) leaves every
- * state as it is and gives y = 0; no slot may be given twice.
+ * state as it is and gives y = 0; no slot may be given twice, and slots are at least their size
+ * apart (state_ss).
  */
 typedef struct tops_gla_scan_step_args {
   float *state;

@@ -128,6 +128,14 @@ int slots_ok(int64_t batch, int64_t slots, const void* idx) {
   return TOPS_GLA_OK;
 }
 
+// Slots of `size` elements, `ss` apart: rows that share one would read and write it at once.
+int slots_apart(int64_t slots, int64_t ss, int64_t size) {
+  if (slots > 1 && ss < size)
+    return fail(TOPS_GLA_EINVAL, "the slots overlap (%lld elements, a stride of %lld)",
+                (long long)size, (long long)ss);
+  return TOPS_GLA_OK;
+}
+
 int conv_check(const tops_gla_conv_args* a) {
   if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
   if (!dtype_ok(a->dtype) || !dtype_ok(a->w_dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
@@ -223,6 +231,7 @@ int tops_gla_selective_scan_step(const tops_gla_scan_step_args* a, void* stream)
     return fail(TOPS_GLA_EINVAL, "u, delta, A, B, C and y must not be NULL");
   if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
     return fail(TOPS_GLA_EINVAL, "state must not be NULL");
+  if (int rc = slots_apart(a->slots, a->state_ss, a->D * a->N)) return rc;
   return done(tops::run_scan_step(*a, (hipStream_t)stream), "selective_scan_step");
 }
 
@@ -261,6 +270,7 @@ int tops_gla_causal_conv_step(const tops_gla_conv_step_args* a, void* stream) {
     return fail(TOPS_GLA_EINVAL, "x, w and y must not be NULL");
   if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
     return fail(TOPS_GLA_EINVAL, "state must not be NULL");
+  if (int rc = slots_apart(a->slots, a->state_ss, a->W * a->D)) return rc;
   return done(tops::run_conv_step(*a, (hipStream_t)stream), "causal_conv_step");
 }
 

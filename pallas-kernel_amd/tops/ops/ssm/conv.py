@@ -147,7 +147,8 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     and takes x, in place.
 
     Args:
-        x: ``[B, D]``.  state: ``[slots, W, D]`` of x's type, each slot contiguous.
+        x: ``[B, D]``.
+        state: ``[slots, W, D]`` of x's type, each slot contiguous and none on another.
         weight, bias, activation: as for ``causal_conv1d``.
         state_indices: as for ``selective_scan_step``.
 
@@ -163,8 +164,10 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     silu = _silu(activation)
     st = state.stride()
     if (len(ss) != 3 or ss[1] != W or ss[2] != D or state.dtype is not dtype
-            or (st[2] != 1 and D > 1) or (st[1] != D and W > 1)):
-        require(False, f"state must be {dtype} [slots, {W}, {D}] with contiguous slots")
+            or (st[2] != 1 and D > 1) or (st[1] != D and W > 1)
+            or (st[0] < W * D and ss[0] > 1)):
+        require(False, f"state must be {dtype} [slots, {W}, {D}] with contiguous slots that do "
+                       "not overlap")
     if state_indices is None and ss[0] < B:
         require(False, f"state holds {ss[0]} slots, the batch {B}")
     idx, idx64 = slot_args(state_indices, B, x)

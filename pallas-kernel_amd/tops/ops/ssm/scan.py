@@ -212,7 +212,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     place.
 
     Args:
-        state: float32 ``[slots, D, N]``, each slot contiguous.
+        state: float32 ``[slots, D, N]``, each slot contiguous and none on another.
         u, delta, z: ``[B, D]``.  A, D, delta_bias: as for ``selective_scan``.
         B, C: ``[B, N]`` or ``[B, G, N]``.
         state_indices: int32 or int64 ``[B]`` on the device, the slot of each row (None: row b
@@ -241,8 +241,10 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
         require(False, f"D and delta_bias must be {(Dn,)}")
     st = state.stride()
     if (len(ss) != 3 or ss[1] != Dn or ss[2] != N or state.dtype is not torch.float32
-            or (st[2] != 1 and N > 1) or (st[1] != N and Dn > 1)):
-        require(False, f"state must be float32 [slots, {Dn}, {N}] with contiguous slots")
+            or (st[2] != 1 and N > 1) or (st[1] != N and Dn > 1)
+            or (st[0] < Dn * N and ss[0] > 1)):
+        require(False, f"state must be float32 [slots, {Dn}, {N}] with contiguous slots that do "
+                       "not overlap")
     if state_indices is None and ss[0] < Bt:
         require(False, f"state holds {ss[0]} slots, the batch {Bt}")
     idx, idx64 = slot_args(state_indices, Bt, u)

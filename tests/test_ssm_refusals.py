@@ -266,3 +266,39 @@ def test_scan_entry_tokens(T, fits):
                     **{**SCAN, "T": T, "D": 1, "N": 1, "piece": 1 << 22, "piece_h": 64,
                        "piece_dt": 64})
     assert (rc, ("A must" if fits else "2^31") in msg) == (1 if fits else 2, True), msg
+
+
+@pytest.mark.parametrize("state", [
+    z(1, 6, 3).expand(2, 6, 3), z(100).as_strided((2, 6, 3), (17, 3, 1)),
+    z(100).as_strided((3, 6, 3), (9, 3, 1))])
+def test_scan_step_slots_that_overlap(state):
+    with pytest.raises(ValueError, match="slots"):
+        selective_scan_step(**step_args(state=state))
+
+
+@pytest.mark.parametrize("state", [
+    z(1, 4, 6).expand(2, 4, 6), z(100).as_strided((2, 4, 6), (23, 6, 1))])
+def test_conv_step_slots_that_overlap(state):
+    with pytest.raises(ValueError, match="slots"):
+        causal_conv1d_step(z(2, 6), state, z(6, 4))
+
+
+@pytest.mark.parametrize("state", [z(100).as_strided((1, 6, 3), (0, 3, 1)),
+                                   z(100).as_strided((2, 6, 3), (18, 3, 1)),
+                                   z(100).as_strided((2, 6, 3), (20, 3, 1))])
+def test_scan_step_slots_that_do_not(state):
+    a = step_args(state=state)
+    n = state.shape[0]
+    a.update({k: a[k][:n] for k in ("u", "delta", "B", "C")})
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        selective_scan_step(**a)
+
+
+def test_step_entries_with_slots_that_overlap():
+    ptrs = dict.fromkeys(("state", "u", "delta", "B", "C", "A", "y", "x", "w"), 64)
+    scan = dict(batch=2, slots=2, D=8, N=4, G=1, dtype=1, state_ss=31)
+    conv = dict(batch=2, slots=2, D=8, W=4, dtype=1, state_ss=31)
+    for name, s, a in (("tops_gla_selective_scan_step", "tops_gla_scan_step_args", scan),
+                       ("tops_gla_causal_conv_step", "tops_gla_conv_step_args", conv)):
+        rc, msg = entry(name, s, **{**a, **{k: v for k, v in ptrs.items() if k in STRUCTS[s]}})
+        assert rc == 1 and "overlap" in msg, msg
