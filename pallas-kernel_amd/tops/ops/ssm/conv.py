@@ -7,6 +7,7 @@ import struct
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
@@ -180,4 +181,5 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, state_indic
     call("tops_gla_causal_conv_step", _STEP.pack(
         xx.data_ptr(), state.data_ptr(), ww.data_ptr(), address(bb), y.data_ptr(), idx, idx64,
         ss[0], B, D, W, st[0], xx.stride(0), int(silu), dt, dtype_code(wt)), stream_of(dev))
+    increment_version(state)   # as torch's own in-place operations do
     return y

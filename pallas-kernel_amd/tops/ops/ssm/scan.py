@@ -6,6 +6,7 @@ import struct
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from ... import _lib
 from ..._lib import call, check_device, dtype_code, require, stream_of
@@ -260,4 +261,5 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
         st[0], uu.stride(0), dd.stride(0), 0 if zz is None else zz.stride(0), bs[0],
         bs[1] if G > 1 else 0, cs[0], cs[1] if G > 1 else 0, 1 if delta_softplus else 0,
         dtype_code(dt)), stream_of(dev))
+    increment_version(state)   # as torch's own in-place operations do
     return y if dt is u.dtype else y.to(u.dtype)

@@ -261,3 +261,25 @@ def test_steps_equal_the_convolution():
     state = d["initial_state"].clone()
     ys = [causal_conv1d_step(d["x"][:, t], state, d["weight"], d["bias"], "silu") for t in range(30)]
     assert torch.equal(torch.stack(ys, 1), y) and torch.equal(state, ht)
+
+
+def test_step_of_a_state_that_a_backward_needs():
+    """The step counts as an in-place operation on its state: a convolution that kept it for its
+    backward says so instead of using the new values. States without a counter work as before."""
+    x, r = make(2, 9, 24, 4, torch.float32)
+    d = {n: t.to(DEV) for n, t in x.items()}
+    pool = d["initial_state"]
+    w = d["weight"].requires_grad_()
+    y, _ = causal_conv1d(d["x"], w, d["bias"], "silu", initial_state=pool)
+    version = pool._version
+    with torch.no_grad():
+        causal_conv1d_step(d["x"][:, 0], pool, w, d["bias"], "silu")
+    assert pool._version > version
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        state = pool.clone()
+        assert state.is_inference()
+        want = causal_conv1d_step(d["x"][:, 1], pool, w, d["bias"], "silu")
+        assert torch.equal(causal_conv1d_step(d["x"][:, 1], state, w, d["bias"], "silu"), want)
+        assert torch.equal(state, pool)

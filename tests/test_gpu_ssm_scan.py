@@ -355,3 +355,24 @@ def test_empty_step():
     args = {n: t[:0, 0].to(DEV) if n in ("u", "delta", "z", "B", "C") else t.to(DEV)
             for n, t in x.items() if n != "initial_state"}
     assert selective_scan_step(torch.zeros(0, 8, 4, device=DEV), **args).shape == (0, 8)
+
+
+def test_step_of_a_state_that_a_backward_needs():
+    """The step counts as an in-place operation on its state: an expression that kept it for its
+    backward says so instead of using the new values. States without a counter work as before."""
+    x, _ = make(2, 1, 24, 16, torch.float32)
+    d = {n: t[:, 0].to(DEV) if n in ("u", "delta", "z", "B", "C") else t.to(DEV)
+         for n, t in x.items()}
+    pool = d.pop("initial_state")
+    w = torch.ones_like(pool).requires_grad_()
+    loss, version = (w * pool).sum(), pool._version
+    selective_scan_step(pool, **d, delta_softplus=True)
+    assert pool._version > version
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        state = pool.clone()
+        assert state.is_inference()
+        want = selective_scan_step(pool, **d, delta_softplus=True)
+        assert torch.equal(selective_scan_step(state, **d, delta_softplus=True), want)
+        assert torch.equal(state, pool)
