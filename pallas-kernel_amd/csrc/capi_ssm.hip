@@ -75,14 +75,14 @@ int scan_setup(const tops_gla_scan_args* a, bool backward, tops::ScanParams* p) 
       return fail(TOPS_GLA_EINVAL, "bad nsegs (%lld for %lld sequences)", (long long)a->nsegs,
                   (long long)a->nseq);
     p->npieces = a->nsegs;
-    p->multi = a->piece_h != nullptr;
+    p->multi = a->piece_h != nullptr && a->nsegs > 0;
   } else {
     if (a->nseq != a->batch) return fail(TOPS_GLA_EINVAL, "nseq must be the batch");
     const int64_t n = std::max<int64_t>(1, (a->T + a->piece - 1) / a->piece);
     if (n * a->batch > kMax) return fail(TOPS_GLA_EUNSUPPORTED, "too many pieces");
     p->pieces = (int)n;
     p->npieces = n * a->batch;
-    p->multi = n > 1;
+    p->multi = p->npieces > a->batch;   // not without a batch: there is nothing to launch for
     if (p->multi && a->piece_h == nullptr)
       return fail(TOPS_GLA_EINVAL, "piece_h and piece_dt are required for several pieces");
   }

@@ -31,7 +31,7 @@ class _Pieces:
         if cu is None:
             per = max(1, -(-T // self.piece))
             self.nseq, self.nsegs = B, B * per
-            self.chunks, self.multi = B * -(-T // chunk), per > 1
+            self.chunks, self.multi = B * -(-T // chunk), self.nsegs > B
             return
         self.nseq = len(cu) - 1
 

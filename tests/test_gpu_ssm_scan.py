@@ -376,3 +376,12 @@ def test_step_of_a_state_that_a_backward_needs():
         want = selective_scan_step(pool, **d, delta_softplus=True)
         assert torch.equal(selective_scan_step(state, **d, delta_softplus=True), want)
         assert torch.equal(state, pool)
+
+
+def test_empty_batch_of_long_sequences():
+    x, _ = make(0, 100, 24, 16, torch.bfloat16)
+    d = {n: t.to(DEV).requires_grad_() for n, t in x.items()}
+    y, ht = selective_scan(**d, delta_softplus=True, output_final_state=True)
+    assert y.shape == (0, 100, 24) and ht.shape == (0, 24, 16)
+    g = torch.autograd.grad([y, ht], list(d.values()), [y.detach(), ht.detach()])
+    assert all(t.shape == d[n].shape and (t == 0).all() for n, t in zip(d, g))

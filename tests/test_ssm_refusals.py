@@ -302,3 +302,16 @@ def test_step_entries_with_slots_that_overlap():
                        ("tops_gla_causal_conv_step", "tops_gla_conv_step_args", conv)):
         rc, msg = entry(name, s, **{**a, **{k: v for k, v in ptrs.items() if k in STRUCTS[s]}})
         assert rc == 1 and "overlap" in msg, msg
+
+
+@pytest.mark.parametrize("T", [64, 65, 1 << 20])
+def test_scan_entry_of_an_empty_batch(T):
+    """No sequences: one piece each, whatever their length, and nothing to launch for them."""
+    lib = _lib.load()
+    piece = lib.tops_gla_selective_scan_piece(0, 0, 8, 4, 1)
+    rc, msg = entry("tops_gla_selective_scan_fwd", "tops_gla_scan_args",
+                    **{**SCAN, "batch": 0, "nseq": 0, "T": T, "piece": piece})
+    assert rc == 1 and "A must" in msg, msg   # the check after those of the pieces
+    rc, msg = entry("tops_gla_selective_scan_fwd", "tops_gla_scan_args",
+                    **{**SCAN, "batch": 0, "nseq": 0, "T": T, "piece": piece, "A": 64})
+    assert rc == 1 and "bc must" in msg, msg
