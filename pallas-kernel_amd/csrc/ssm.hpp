@@ -72,6 +72,13 @@ __device__ __forceinline__ float swap16_add(float a, float b) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A log2(e). -inf (a state that is forgotten at once) stays finite: where delta' is 0 the state is
+// kept, as for every other A, and a token past a sequence's end has a delta' of 0.
+__device__ __forceinline__ float scaled_a(float a) {
+  a *= 1.4426950408889634f;
+  return a < -3.4028235e38f ? -3.4028235e38f : a;
+}
+
 // 1 / (1 + e^-x), with the hardware exponential and reciprocal (1 ulp each); 0 and 1 at the ends.
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));

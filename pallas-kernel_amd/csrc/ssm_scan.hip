@@ -25,7 +25,6 @@ namespace {
 
 constexpr int SS_K = 8;      // tokens of a tile of the backward, and between the states kept for it
 constexpr int FT = 4;        // tokens of a tile of the forward
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Wave-uniform data that no kernel of the launch writes: read by scalar loads.
@@ -69,13 +68,6 @@ struct Tile {
     nch = min(64, DG - cb);
   }
 };
-
-// A log2(e). -inf (a state that is forgotten at once) stays finite: a token past the end has
-// delta' = 0, and 0 times it has to be 0.
-__device__ __forceinline__ float scaled_a(float a) {
-  a *= kLog2e;
-  return a < -3.4028235e38f ? -3.4028235e38f : a;
-}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_arg
     for (int i = 0; i < 4; ++i) A[i] = i < nn ? a.A[(long)dd * N + n0 + i] : 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A[i] *= 1.4426950408889634f;
+  for (int i = 0; i < 4; ++i) A[i] = scaled_a(A[i]);
   const float bias = a.delta_bias ? a.delta_bias[dd] : 0.f;
   const float skip = a.Dskip ? a.Dskip[dd] : 0.f;
 #pragma unroll

@@ -164,8 +164,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
 
     Args:
         u, delta, z: ``[B, T, D]`` (z optional: the output gate).
-        A: ``[D, N]``, N <= 64.  B, C: ``[B, T, N]``, or ``[B, T, G, N]`` for G groups of D / G
-            consecutive channels each.  D, delta_bias: ``[D]`` or None.
+        A: ``[D, N]``, N <= 64 (-inf: a state that any ``delta' > 0`` forgets, and that
+            ``delta' = 0`` keeps).  B, C: ``[B, T, N]``, or ``[B, T, G, N]`` for G groups of
+            D / G consecutive channels each.  D, delta_bias: ``[D]`` or None.
         initial_state: ``[sequences, D, N]`` or None (zeros).
         cu_seqlens: offsets of sequences packed into one row (B == 1), from 0 to T, known on the
             host; empty sequences keep their state.

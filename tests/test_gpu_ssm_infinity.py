@@ -1,0 +1,57 @@
+"""Infinities in the selective state space operators, against the recurrence in 64 bits: where that
+is finite the result has the bound of the finite tests, where it is an infinity it is the same
+infinity, and a NaN only where the formula has one (inf - inf, 0 * inf).
+
+The other values are positive (A negative), so that an infinity's effects all have one sign and the
+recurrence keeps it an infinity almost everywhere."""
+
+import pytest
+import torch
+
+import test_gpu_ssm_scan as scan_tests
+from ssm_ref import close
+from tops.ops.ssm import selective_scan, selective_scan_step
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF = float("inf")
+
+
+def make(B, T, D, N, z=True, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: 0.5 + torch.rand(*s, generator=gen)   # noqa: E731
+    x = dict(u=r(B, T, D), delta=0.2 * r(B, T, D), A=-0.2 * r(D, N), B=r(B, T, N), C=r(B, T, N),
+             D=r(D), z=r(B, T, D) if z else None, delta_bias=0.1 * r(D),
+             initial_state=r(B, D, N))
+    return x, r
+
+
+def same(name, got, ref, mag, terms):
+    got = got.detach().cpu()
+    ok = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), f"{name}: NaN in other places"
+    odd = ~ok & ~torch.isnan(ref)
+    assert torch.equal(got[odd].double(), ref[odd]), f"{name}: other infinities"
+    close(name, got[ok], ref[ok], mag[ok], terms)
+
+
+@pytest.mark.parametrize("N", [12, 16])
+@pytest.mark.parametrize("softplus", [True, False])
+def test_infinite_decay_of_no_step(N, softplus):
+    """A of -inf: a token with delta' = 0 leaves the state as it is, any other forgets it, the same
+    in the scan and in its single-token form."""
+    x, _ = make(3, 1, 20, N)
+    x["A"][:, 0] = -INF
+    x["delta"][:] = -INF if softplus else 0.0
+    x["delta_bias"] = torch.zeros(20)
+    x["delta"][2] = 0.25
+    ref, mag = scan_tests.reference(dict(x, A=x["A"].double().clamp(min=-1e300)), softplus, None)
+    d = {n: t.to(DEV) for n, t in x.items()}
+    y, ht = selective_scan(**d, delta_softplus=softplus, output_final_state=True)
+    same("y", y, ref["y"], mag["y"], 68)
+    same("ht", ht, ref["ht"], mag["ht"], 68)
+    state = d.pop("initial_state")
+    y = selective_scan_step(state, **{n: t[:, 0] if n in ("u", "delta", "z", "B", "C") else t
+                                      for n, t in d.items()}, delta_softplus=softplus)
+    same("y", y, ref["y"][:, 0], mag["y"][:, 0], 68)
+    same("state", state, ref["ht"], mag["ht"], 68)
