@@ -93,7 +93,7 @@ __global__ __launch_bounds__(ST_NT) void scan_step_kernel(tops_gla_scan_step_arg
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[k][i] = fmaf(__builtin_amdgcn_exp2f(A[i] * t), h[k][i], du * B[k][i]);
-      y = fmaf(C[k][i], h[k][i], y);
+      if (i < nn) y = fmaf(C[k][i], h[k][i], y);   // an infinite u makes a NaN of a lane's rest
     }
     if (there[k]) {
       if (v4) {

@@ -55,3 +55,16 @@ def test_infinite_decay_of_no_step(N, softplus):
                                       for n, t in d.items()}, delta_softplus=softplus)
     same("y", y, ref["y"][:, 0], mag["y"][:, 0], 68)
     same("state", state, ref["ht"], mag["ht"], 68)
+
+
+@pytest.mark.parametrize("N", [1, 2, 5, 12, 13, 16, 33])
+def test_infinite_inputs_of_a_step(N):
+    x, r = make(6, 1, 40, N)
+    x["u"][1, 0, 3], x["u"][2, 0, 39], x["u"][5, 0, 0] = INF, -INF, INF
+    x["delta"][3, 0, 7] = INF
+    ref, mag = scan_tests.reference(x, False, None)
+    state = x.pop("initial_state").to(DEV)
+    y = selective_scan_step(state, **{n: t[:, 0].to(DEV) if n in ("u", "delta", "z", "B", "C")
+                                      else t.to(DEV) for n, t in x.items()})
+    same("y", y, ref["y"][:, 0], mag["y"][:, 0], 68)
+    same("state", state, ref["ht"], mag["ht"], 68)
