@@ -568,7 +568,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
             hv[s][n] = fmaf(av[s][n], h0[n], x * rb[n]);
         }
       } else {
-        float vb[8], vc[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        float vb[8], vc[8], gd[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
           const float g = fmaf(dy, rc[n], carry[n]);
@@ -581,8 +581,11 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
           const float gp = carry[n] * hp;
           s2 = fmaf(gp, A[n], s2);
           s3 = fmaf(hv[s][n], rc[n], s3);
-          dA[n] = fmaf(gp, d, dA[n]);
+          gd[n] = gp;
         }
+        if (t0 + t < pc.t1)   // past the end 0 times a state, which an infinity makes NaN
+#pragma unroll
+          for (int n = 0; n < 8; ++n) dA[n] = fmaf(gd[n], d, dA[n]);
         pin(dA);
         sS[part][0][t][col] = s1;
         sS[part][1][t][col] = s2;

@@ -68,3 +68,51 @@ def test_infinite_inputs_of_a_step(N):
                                       else t.to(DEV) for n, t in x.items()})
     same("y", y, ref["y"][:, 0], mag["y"][:, 0], 68)
     same("state", state, ref["ht"], mag["ht"], 68)
+
+
+def check(x, r, dy=None, dht=None):
+    d = {n: None if t is None else t.to(DEV).requires_grad_() for n, t in x.items()}
+    y, ht = selective_scan(**d, output_final_state=True)
+    dy = r(*y.shape) if dy is None else dy
+    dht = r(*ht.shape) if dht is None else dht
+    names = [n for n, t in d.items() if t is not None]
+    got = torch.autograd.grad([y, ht], [d[n] for n in names], [dy.to(DEV), dht.to(DEV)])
+    ref, mag = scan_tests.reference(x, False, None, dy, dht)
+    B, T, D = x["u"].shape
+    terms = 4 * T + 64
+    same("y", y, ref["y"], mag["y"], terms)
+    same("ht", ht, ref["ht"], mag["ht"], terms)
+    for n, t in zip(names, got):
+        same("d" + n, t, ref["d" + n], mag["d" + n], terms + B * T + D)
+
+
+def infinite_inputs(N, T, z):
+    """An infinity in the first, a middle and the last token of a sequence."""
+    x, r = make(3, T, 70, N, z)
+    for b, (t, v) in enumerate(((0, INF), (T // 2, -INF), (T - 1, INF))):
+        x["u"][b, t, 3 * b] = x["u"][b, t, 69 - b] = v
+    return x, r
+
+
+# a last tile that is full and one that is not; one piece and several
+@pytest.mark.parametrize("N", [8, 16, 32])
+@pytest.mark.parametrize("T", [13, 37, 40, 150])
+@pytest.mark.parametrize("z", [True, False])
+def test_infinite_inputs(N, T, z):
+    check(*infinite_inputs(N, T, z))
+
+
+def infinite_inputs(N, T, z):
+    """An infinity in the first, a middle and the last token of a sequence."""
+    x, r = make(3, T, 70, N, z)
+    for b, (t, v) in enumerate(((0, INF), (T // 2, -INF), (T - 1, INF))):
+        x["u"][b, t, 3 * b] = x["u"][b, t, 69 - b] = v
+    return x, r
+
+
+# a last tile that is full and one that is not; one piece and several
+@pytest.mark.parametrize("N", [8, 16, 32])
+@pytest.mark.parametrize("T", [13, 37, 40, 150])
+@pytest.mark.parametrize("z", [True, False])
+def test_infinite_inputs(N, T, z):
+    check(*infinite_inputs(N, T, z))
