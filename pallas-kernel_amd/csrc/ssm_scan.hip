@@ -302,6 +302,16 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
   }
 }
 
+// The state after a piece of summed delta' s and own state l, entered with h. A zero state stays
+// zero under a decay that overflows. An infinite one stays infinite under a decay that is too small
+// for a float as the product of its tokens' (2^-126 in its place: nothing to a finite state), but
+// not under one that forgets at once (A of -inf).
+__device__ __forceinline__ float folded(float h, float A, float s, float l) {
+  const float e = A * s, f = exp2_hw(e);
+  const float g = e > -1e30f ? fmaxf(f, 1.17549435e-38f) : f;
+  return h == 0.f ? l : fmaf(g, h, l);
+}
+
 // The pieces' entry states in the place of their own ones: h <- exp(A S_j) h + L_j over a
 // sequence's pieces from h0 on, or backward from dht on with REV. A thread folds a run of the
 // pieces for a state of a channel, 4 threads share a sequence's runs: each finds its run's own L
@@ -345,8 +355,8 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p) {
       for (int i = 0; i < FOLD_U; ++i) {
         if (j + i >= end) break;
         if (put) H[(j + i) * hs] = h;
-        if (j + i < np - 1) {   // a zero state stays zero under a decay that overflows
-          h = h == 0.f ? l[i] : fmaf(exp2_hw(A * dt[i]), h, l[i]);
+        if (j + i < np - 1) {
+          h = folded(h, A, dt[i], l[i]);
           s += dt[i];
         }
       }
@@ -357,10 +367,7 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p) {
   sS[run][c] = s;
   __syncthreads();
   h = n < N && init ? init[(seq * D + d) * N + n] : 0.f;
-  for (int r = 0; r < run; ++r) {
-    const float l = sL[r][c];
-    h = h == 0.f ? l : fmaf(exp2_hw(A * sS[r][c]), h, l);
-  }
+  for (int r = 0; r < run; ++r) h = folded(h, A, sS[r][c], sL[r][c]);
   walk(j0, j1, true);
 }
 

@@ -116,3 +116,43 @@ def infinite_inputs(N, T, z):
 @pytest.mark.parametrize("z", [True, False])
 def test_infinite_inputs(N, T, z):
     check(*infinite_inputs(N, T, z))
+
+
+def infinite_gradients(N, T):
+    """An infinite gradient of the first, a middle and the last token's output."""
+    x, r = make(3, T, 70, N)
+    dy = r(3, T, 70)
+    for b, t in enumerate((0, T // 2, T - 1)):
+        dy[b, t, 3 * b] = INF
+    return x, r, dy
+
+
+@pytest.mark.parametrize("N", [8, 16])
+@pytest.mark.parametrize("T", [13, 150])
+def test_infinite_gradients(N, T):
+    check(*infinite_gradients(N, T))
+
+
+@pytest.mark.parametrize("N", [1, 12, 13, 16])
+@pytest.mark.parametrize("T", [13, 150])
+def test_infinite_gradient_of_the_final_state(N, T):
+    x, r = make(2, T, 70, N)
+    dht = r(2, 70, N)
+    dht[1, 7, 0] = INF
+    check(x, r, None, dht)
+
+
+@pytest.mark.parametrize("T", [60, 700])
+def test_infinite_states_under_strong_decay(T):
+    """Each token's decay is far above the smallest number, a piece's product of them is below it:
+    an infinite state stays infinite, as it does in the recurrence."""
+    x, r = make(2, T, 8, 16, z=False)
+    x["A"], x["delta_bias"] = torch.full((8, 16), -20.0), None
+    x["delta"] = torch.ones(2, T, 8)
+    x["u"][0, 3, 2] = INF
+    x["initial_state"][1, 5, 7] = INF
+    check(x, r)
+    dht = r(2, 8, 16)
+    dht[0, 1, 4] = INF
+    check(make(2, T, 8, 16, z=False)[0] | {n: x[n] for n in ("A", "delta", "delta_bias")}, r, None,
+          dht)
