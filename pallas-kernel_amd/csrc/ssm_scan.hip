@@ -110,6 +110,17 @@ __device__ __forceinline__ cfloat* row_after(const float* p, float (&x)[N]) {
   return (cfloat*)(uintptr_t)p;
 }
 
+// The states that fill N up to 8, 16, 32 or 64 are zero: their B and C are, and A as well. But an
+// infinite input times their B is a NaN, which would reach the sums: they are set to zero again
+// wherever the lanes' x are not all finite, in kernels of their own (PAD).
+__device__ __forceinline__ bool any_odd(float x) { return __any(!(fabsf(x) <= 3.4028235e38f)); }
+template <int N>
+__device__ __forceinline__ void clear_pads(float (&h)[N], int real) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (n >= real) h[n] = 0.f;
+}
+
 // Has x computed here: the compiler would put sums off and keep their terms in registers.
 __device__ __forceinline__ void pin(float (&x)[8]) {
   asm volatile(""
@@ -151,9 +162,9 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(ScanParams p) {
 // ---------------------------------------------------------------------------
 // A wave walks a piece for 64 channels. MODE 0: a piece's own state and summed delta'. MODE 1:
 // the outputs. MODE 2: the reverse of 0 for the backward, the carry that a piece hands to the one
-// before it, from a zero carry.
+// before it, from a zero carry. PAD: N < NP (MODE 1).
 // ---------------------------------------------------------------------------
-template <typename T, int NP, int MODE>
+template <typename T, int NP, int MODE, bool PAD>
 __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_kernel(ScanParams p) {
   const tops_gla_scan_args& a = p.a;
   const int lane = threadIdx.x & 63;
@@ -269,8 +280,13 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
             hg[n] = ex * fmaf(x, rb[n / 8][n % 8], hg[n]);
           } else {
             hg[n] = fmaf(ex, hg[n], x * rb[n / 8][n % 8]);
-            if (MODE == 1) acc[n & 1] = fmaf(hg[n], rc[n / 8][n % 8], acc[n & 1]);
+            if (MODE == 1 && !PAD) acc[n & 1] = fmaf(hg[n], rc[n / 8][n % 8], acc[n & 1]);
           }
+        }
+        if (PAD) {
+          if (any_odd(x)) clear_pads<GN>(hg, N - g);
+#pragma unroll
+          for (int n = 0; n < GN; ++n) acc[n & 1] = fmaf(hg[n], rc[n / 8][n % 8], acc[n & 1]);
         }
         if (MODE == 1) asm volatile("" : "+v"(acc[0]), "+v"(acc[1]));   // like h: now
       }
@@ -297,6 +313,7 @@ __global__ __launch_bounds__(256, NP <= 16 ? 4 : NP <= 32 ? 3 : 2) void scan_ker
       for (int n = 0; n < NP; ++n)
         if (n < N) a.ht[((long)pc.seq * D + dl) * N + n] = h[n];
   } else {
+    if (N < NP) clear_pads<NP>(h, N);
     store_states<NP>(a.piece_h + (long)pi * NP * D + tl.d0, D, lo, h);
     a.piece_dt[(long)pi * D + dl] = dsum;
   }
@@ -441,7 +458,7 @@ __device__ __forceinline__ float sum_channels(float (&x)[8], float (&y)[8]) {
   return s + dpp<0x4e>(s);   // quad_perm [2, 3, 0, 1]
 }
 
-template <typename T, int NP>
+template <typename T, int NP, bool PAD>
 __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) void scan_bwd_kernel(ScanParams p) {
   using L = Bwd<NP>;
   __shared__ float sD[SS_K][L::CT], sU[SS_K][L::CT], sG[SS_K][L::CT];   // delta', u, dy silu(z)
@@ -565,6 +582,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
       if constexpr (sweep == 0) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) hm[n] = fmaf(exp2_hw(A[n] * d), hm[n], x * rb[n]);
+        if (PAD && any_odd(x)) clear_pads<8>(hm, N - n0);
       } else if constexpr (!back) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -574,11 +592,18 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
           else
             hv[s][n] = fmaf(av[s][n], h0[n], x * rb[n]);
         }
+        if (PAD && any_odd(x)) {
+          clear_pads<8>(av[s], N - n0);   // 0 times an infinite delta'
+          clear_pads<8>(hv[s], N - n0);
+        }
       } else {
         float vb[8], vc[8], gd[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
+        for (int n = 0; n < 8; ++n) carry[n] = fmaf(dy, rc[n], carry[n]);
+        if (PAD && any_odd(dy)) clear_pads<8>(carry, N - n0);
+#pragma unroll
         for (int n = 0; n < 8; ++n) {
-          const float g = fmaf(dy, rc[n], carry[n]);
+          const float g = carry[n];
           float hp = h0[n];
           if constexpr (s > 0) hp = hv[s - 1][n];
           vb[n] = g * x;
@@ -730,11 +755,14 @@ hipError_t scan_fwd(const ScanParams& p, hipStream_t st) {
   hipLaunchKernelGGL((scan_bc_kernel<T, NP>), dim3(grid_of(nbc)), dim3(256), 0, st, p);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.multi) {
-    hipLaunchKernelGGL((scan_kernel<T, NP, 0>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((scan_kernel<T, NP, 0, false>), grid, dim3(256), 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
     if (hipError_t e = scan_fold<NP, false>(p, st)) return e;
   }
-  hipLaunchKernelGGL((scan_kernel<T, NP, 1>), grid, dim3(256), 0, st, p);
+  if (p.a.N < NP)
+    hipLaunchKernelGGL((scan_kernel<T, NP, 1, true>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((scan_kernel<T, NP, 1, false>), grid, dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
@@ -742,13 +770,16 @@ template <typename T, int NP>
 hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
   if (p.multi) {
     const dim3 grid((unsigned)((p.npieces * p.ntiles + 3) / 4));
-    hipLaunchKernelGGL((scan_kernel<T, NP, 2>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((scan_kernel<T, NP, 2, false>), grid, dim3(256), 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
     if (hipError_t e = scan_fold<NP, true>(p, st)) return e;
   }
   if (p.npieces > 0) {
-    hipLaunchKernelGGL((scan_bwd_kernel<T, NP>), dim3((unsigned)(p.npieces * p.btiles)),
-                       dim3(64 * Bwd<NP>::WAVES), 0, st, p);
+    const dim3 bgrid((unsigned)(p.npieces * p.btiles)), nt(64 * Bwd<NP>::WAVES);
+    if (p.a.N < NP)
+      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, true>), bgrid, nt, 0, st, p);
+    else
+      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, false>), bgrid, nt, 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
   }
   const long nbc = p.tokens * p.a.G * 2 * NP, na = p.a.D * (NP + 2);

@@ -156,3 +156,28 @@ def test_infinite_states_under_strong_decay(T):
     dht[0, 1, 4] = INF
     check(make(2, T, 8, 16, z=False)[0] | {n: x[n] for n in ("A", "delta", "delta_bias")}, r, None,
           dht)
+
+
+@pytest.mark.parametrize("N", [1, 5, 12, 13, 33])
+@pytest.mark.parametrize("T", [13, 37, 40, 150])
+@pytest.mark.parametrize("z", [True, False])
+def test_infinite_inputs_beside_padded_states(N, T, z):
+    check(*infinite_inputs(N, T, z))
+
+
+@pytest.mark.parametrize("N", [1, 12, 13])
+@pytest.mark.parametrize("T", [13, 150])
+def test_infinite_gradients_beside_padded_states(N, T):
+    check(*infinite_gradients(N, T))
+
+
+@pytest.mark.parametrize("N", [12, 16])
+def test_infinite_steps(N):
+    """An infinite delta forgets the state and adds an infinity to it."""
+    x, _ = make(2, 45, 70, N)
+    x["delta"][0, 20, 3] = x["delta"][1, 44, 69] = INF
+    d = {n: t.to(DEV) for n, t in x.items()}
+    y, ht = selective_scan(**d, output_final_state=True)
+    ref, mag = scan_tests.reference(x, False, None)
+    same("y", y, ref["y"], mag["y"], 4 * 45 + 64)
+    same("ht", ht, ref["ht"], mag["ht"], 4 * 45 + 64)
