@@ -403,6 +403,10 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p) {
 // them all). Bound by vector issue, 85 % busy: 24 instructions a state and token, 18 of them the
 // formulas'; MI355X, B2 T4096 D4096 N16 bf16: 476 us (a token more in registers costs the third
 // wave of a SIMD: all 8 at two waves 574; four lanes a channel and LDS rows of B and C 1145).
+//
+// EDGE: 1 with padded states, 2 where some lanes have no channel (padded states or not). Infinite
+// values must not meet their zeros; the checks cost 1.5 and 3 % of the training pass (B2 T4096, N 12,
+// D 4096 and 4000).
 // ---------------------------------------------------------------------------
 constexpr int HK = SS_K / 2;
 // Steps 0 .. 5 HK - 1 of a tile: forward to its middle; the second half forward, and back; the
@@ -458,7 +462,7 @@ __device__ __forceinline__ float sum_channels(float (&x)[8], float (&y)[8]) {
   return s + dpp<0x4e>(s);   // quad_perm [2, 3, 0, 1]
 }
 
-template <typename T, int NP, bool PAD>
+template <typename T, int NP, int EDGE>
 __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) void scan_bwd_kernel(ScanParams p) {
   using L = Bwd<NP>;
   __shared__ float sD[SS_K][L::CT], sU[SS_K][L::CT], sG[SS_K][L::CT];   // delta', u, dy silu(z)
@@ -478,6 +482,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
   const uint32_t lo = live ? lane : 0;
   const long dl = d0 + lo;
   const int n0 = 8 * part, col = 64 * cg + lane;
+  const bool pads = EDGE == 1 || (EDGE == 2 && N < NP);
   float A[8], carry[8], dA[8];
 #pragma unroll
   for (int n = 0; n < 8; ++n) carry[n] = dA[n] = 0.f;
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
       if constexpr (sweep == 0) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) hm[n] = fmaf(exp2_hw(A[n] * d), hm[n], x * rb[n]);
-        if (PAD && any_odd(x)) clear_pads<8>(hm, N - n0);
+        if (pads && any_odd(x)) clear_pads<8>(hm, N - n0);
       } else if constexpr (!back) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
           else
             hv[s][n] = fmaf(av[s][n], h0[n], x * rb[n]);
         }
-        if (PAD && any_odd(x)) {
+        if (pads && any_odd(x)) {
           clear_pads<8>(av[s], N - n0);   // 0 times an infinite delta'
           clear_pads<8>(hv[s], N - n0);
         }
@@ -600,7 +605,7 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
         float vb[8], vc[8], gd[8], s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int n = 0; n < 8; ++n) carry[n] = fmaf(dy, rc[n], carry[n]);
-        if (PAD && any_odd(dy)) clear_pads<8>(carry, N - n0);
+        if (pads && any_odd(dy)) clear_pads<8>(carry, N - n0);
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
           const float g = carry[n];
@@ -622,6 +627,9 @@ __global__ __launch_bounds__(64 * Bwd<NP>::WAVES, NP == 16 || NP == 32 ? 3 : 2) 
         sS[part][0][t][col] = s1;
         sS[part][1][t][col] = s2;
         sS[part][2][t][col] = s3;
+        if (EDGE == 2 && cb + 64 > DG)   // lanes without a channel: zeros, but not times an infinite B or C
+#pragma unroll
+          for (int n = 0; n < 8; ++n) vb[n] = live ? vb[n] : 0.f, vc[n] = live ? vc[n] : 0.f;
         const float r = sum_channels(vb, vc);
         if ((lane & 3) == 0)
           sBC[cg][t][(lane & 8 ? NP : 0) + n0 + (lane & 4) + ((lane >> 3) & 2) + (lane >> 5)] = r;
@@ -776,10 +784,12 @@ hipError_t scan_bwd(const ScanParams& p, hipStream_t st) {
   }
   if (p.npieces > 0) {
     const dim3 bgrid((unsigned)(p.npieces * p.btiles)), nt(64 * Bwd<NP>::WAVES);
-    if (p.a.N < NP)
-      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, true>), bgrid, nt, 0, st, p);
+    if (p.a.D / p.a.G % Bwd<NP>::CT)
+      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, 2>), bgrid, nt, 0, st, p);
+    else if (p.a.N < NP)
+      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, 1>), bgrid, nt, 0, st, p);
     else
-      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, false>), bgrid, nt, 0, st, p);
+      hipLaunchKernelGGL((scan_bwd_kernel<T, NP, 0>), bgrid, nt, 0, st, p);
     if (hipError_t e = hipGetLastError()) return e;
   }
   const long nbc = p.tokens * p.a.G * 2 * NP, na = p.a.D * (NP + 2);

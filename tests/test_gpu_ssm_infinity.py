@@ -181,3 +181,12 @@ def test_infinite_steps(N):
     ref, mag = scan_tests.reference(x, False, None)
     same("y", y, ref["y"], mag["y"], 4 * 45 + 64)
     same("ht", ht, ref["ht"], mag["ht"], 4 * 45 + 64)
+
+
+@pytest.mark.parametrize("n", ["B", "C"])
+@pytest.mark.parametrize("D,N", [(1, 16), (70, 12), (130, 16), (64, 16), (9, 5), (20, 40)])
+def test_infinite_rows(n, D, N):
+    """A row that all channels read: the lanes without a channel add nothing to its gradient."""
+    x, r = make(2, 37, D, N)
+    x[n][0, 20, N - 1] = INF
+    check(x, r)
