@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from ..._lib import require, stream_of, to_list
@@ -65,6 +67,7 @@ def offsets(cu_seqlens, B, T):
 
 _tables: dict = {}
 _held: list = []
+_tables_lock = threading.Lock()
 
 
 def device_table(key, make, device):
@@ -73,22 +76,23 @@ def device_table(key, make, device):
     that a graph captures is kept for good, as the graph's replays read it."""
     key = (key, device.index, stream_of(device).value)
     capturing = torch.cuda.is_current_stream_capturing()
-    hit = _tables.get(key)
-    if hit is None and capturing:
-        # a capture runs on its own stream, and cannot upload a table of its own
-        hit = next((v for k, v in _tables.items() if k[:2] == key[:2]), None)
+    with _tables_lock:
+        hit = _tables.get(key)
+        if hit is None and capturing:
+            # a capture runs on its own stream, and cannot upload a table of its own
+            hit = next((v for k, v in _tables.items() if k[:2] == key[:2]), None)
+            if hit is None:
+                raise RuntimeError("packed sequences in a graph capture: run the call once with "
+                                   "the same cu_seqlens before the capture")
         if hit is None:
-            raise RuntimeError("packed sequences in a graph capture: run the call once with the "
-                               "same cu_seqlens before the capture")
-    if hit is None:
-        values, rest = make()
-        if len(_tables) > 64:
-            _tables.clear()
-        # pinned, so that the copy is one of the stream's own and nothing waits for it
-        table = torch.tensor(values, dtype=torch.int32, pin_memory=True)
-        hit = _tables[key] = (table.to(device, non_blocking=True), rest)
-    if capturing and not any(h is hit for h in _held):
-        _held.append(hit)
+            values, rest = make()
+            if len(_tables) > 64:
+                _tables.clear()
+            # pinned, so that the copy is one of the stream's own and nothing waits for it
+            table = torch.tensor(values, dtype=torch.int32, pin_memory=True)
+            hit = _tables[key] = (table.to(device, non_blocking=True), rest)
+        if capturing and not any(h is hit for h in _held):
+            _held.append(hit)
     return hit
 
 

@@ -315,3 +315,39 @@ def test_scan_entry_of_an_empty_batch(T):
     rc, msg = entry("tops_gla_selective_scan_fwd", "tops_gla_scan_args",
                     **{**SCAN, "batch": 0, "nseq": 0, "T": T, "piece": piece, "A": 64})
     assert rc == 1 and "bc must" in msg, msg
+
+
+def test_tables_of_two_threads(monkeypatch):
+    """A table made by one thread while another looks one up in a capture."""
+    import importlib
+    import threading
+
+    common = importlib.import_module("tops.ops.ssm._common")
+    second, tensor = [], torch.tensor
+
+    class Tables(dict):
+        def items(self):
+            it = iter(super().items())
+            yield next(it)
+            second.append(threading.Thread(target=make, args=("b",)))
+            second[0].start()
+            second[0].join(0.2)
+            yield from it
+
+    def make(key):
+        return common.device_table(key, lambda: ([1], key), torch.device("cpu"))
+
+    monkeypatch.setattr(common, "_tables", Tables())
+    monkeypatch.setattr(common, "_held", [])
+    monkeypatch.setattr(common, "stream_of", lambda d: ctypes.c_void_p(streams.pop(0)))
+    monkeypatch.setattr(torch, "tensor", lambda v, dtype, pin_memory: tensor(v, dtype=dtype))
+    capturing = threading.local()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing",
+                        lambda: getattr(capturing, "now", False))
+    streams = [1, 1, 2, 1]
+    make("x")
+    want = make("a")
+    capturing.now = True   # stream 2, whose own table it cannot make
+    assert make("a") is want
+    second[0].join()
+    assert len(common._tables) == 3
