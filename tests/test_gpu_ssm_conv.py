@@ -283,3 +283,49 @@ def test_step_of_a_state_that_a_backward_needs():
         want = causal_conv1d_step(d["x"][:, 1], pool, w, d["bias"], "silu")
         assert torch.equal(causal_conv1d_step(d["x"][:, 1], state, w, d["bias"], "silu"), want)
         assert torch.equal(state, pool)
+
+
+@pytest.mark.parametrize("D", [4096, 4099])
+def test_packed_sequences_in_long_runs(D):
+    """Runs of 128 tokens with the boundaries of sequences inside them, at their first and last
+    token and in the rows that a run reads past its end; the weights' and the bias's gradients to
+    float32 roundings, for a part of the channels."""
+    T, W = 40000, 4
+    cu = [0, 1, 128, 130, 131, 131, 253, 256, 257, 511, 515, 20000, 20479, 20480, 20607, 32768, T]
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)   # noqa: E731
+    x, dy = r(1, T, D).bfloat16(), r(1, T, D).bfloat16()
+    w, b, init = 0.5 * r(D, W), 0.3 * r(D), r(len(cu) - 1, W, D).bfloat16()
+    leaves = [t.requires_grad_() for t in (x, w, b, init)]
+    y, ht = causal_conv1d(x, w, b, "silu", init, True, cu)
+    dx, dw, db, di = torch.autograd.grad(y, leaves, dy)
+    cols = torch.cat([torch.arange(6), torch.arange(D // 2, D // 2 + 6), torch.arange(D - 9, D)])
+    cols = cols.to(DEV)
+    cut = lambda t, dim: t.detach().index_select(dim, cols).double()   # noqa: E731
+    X, G, K, S = cut(x, 2)[0], cut(dy, 2)[0], cut(w, 0), cut(init, 2)
+    rows = torch.cat([torch.cat([S[s], X[a:e]]) for s, (a, e) in enumerate(zip(cu, cu[1:]))])
+    first = torch.repeat_interleave(torch.arange(1, len(cu), device=DEV) * W,
+                                    torch.tensor(cu, device=DEV).diff())
+    at = first + torch.arange(T, device=DEV)   # a token's row in `rows`, W more a sequence
+    p = torch.stack([rows[at - W + 1 + j] for j in range(W)], -1)   # [T, cols, W]
+    z = (p * K).sum(-1) + cut(b, 0)
+    zm = (p.abs() * K.abs()).sum(-1) + cut(b, 0).abs()
+    sg = torch.sigmoid(z)
+    close("y", cut(y, 2)[0].to(y.dtype), (z * sg).cpu(), (1.1 * zm).cpu(), W + 9)
+    dz, dzm = G * sg * (1 + z * (1 - sg)), G.abs() * (1.1 + 0.5 * zm)
+    # sums of 128 tokens in a row, of four runs, then of a column's T / 512 partial sums by eight
+    # threads, and the roundings of a term
+    many = 128 + 4 + T // 512 // 8 + 1 + 8 + 2 * (W + 9)
+    close("dweight", dw.index_select(0, cols), (dz[..., None] * p).sum(0).cpu(),
+          (dzm[..., None] * p.abs()).sum(0).cpu(), many)
+    close("dbias", db.index_select(0, cols), dz.sum(0).cpu(), dzm.sum(0).cpu(), many)
+    back, mag = torch.zeros_like(rows), torch.zeros_like(rows)
+    for j in range(W):
+        back.index_add_(0, at - W + 1 + j, dz * K[:, j])
+        mag.index_add_(0, at - W + 1 + j, dzm * K[:, j].abs())
+    close("dx", dx.index_select(2, cols)[0], back[at].cpu(), mag[at].cpu(), 2 * (W + 9) + W)
+    first = torch.tensor([c + W * s for s, c in enumerate(cu[:-1])], device=DEV)
+    at = first[:, None] + torch.arange(W, device=DEV)
+    close("dinit", di.index_select(2, cols), back[at].cpu(), mag[at].cpu(), 2 * (W + 9) + W)
+    end = torch.tensor([c + W * s for s, c in enumerate(cu[1:])], device=DEV)
+    assert torch.equal(cut(ht, 2), rows[end[:, None] + torch.arange(W, device=DEV)])
