@@ -7,8 +7,9 @@
 // turns in 64 bits, where a far position times a frequency keeps its fraction, and only the fraction
 // is rounded to 32. MI355X, B4 T8192 H16+16 D128 bf16: forward 112 us (4.7 TB/s), backward 164 (4.9).
 //
-// Heads of an odd size and rows at odd addresses take the first two kernels, an element (or, above
-// 256 columns, four) a lane and the partner read again.
+// The first two kernels, an element (or, for rows of more than 64 pieces, a piece of four) a lane and
+// the partner read again, take what is left: heads of an odd size, rows at odd addresses, and above
+// 128 columns those whose size or, in the half layout, rotated half is no multiple of four.
 #include "ssm.hpp"
 
 namespace tops {
@@ -300,8 +301,8 @@ __global__ __launch_bounds__(QD_C * QD_R) void qk_dw_kernel(const float* part, i
 }
 
 // ---------------------------------------------------------------------------
-// Rows that one wave's lanes hold whole in pieces of VEC > 1 elements (every aligned head of up to
-// 256 or 512 columns): the partner of a rotated piece comes from its lane, and the rows of the
+// Rows that one wave's lanes hold whole in pieces of VEC > 1 elements (aligned heads of up to 64
+// pieces: 512 columns in pieces of eight, 256 of four, 128 of two): the partner of a rotated piece comes from its lane, and the rows of the
 // next batch are on their way while one is computed.
 // ---------------------------------------------------------------------------
 constexpr int QK_UB = 2;   // rows of a thread in a batch of the backward
@@ -756,7 +757,8 @@ hipError_t qk_pairs(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
   return qk_rows_launch<T, 2, 64>(a, backward, st);
 }
 
-// Heads of an odd size, or rows that are not aligned: an element a lane.
+// Heads of an odd size, rows that are not aligned, and wide heads that are no whole pieces of four:
+// an element a lane.
 template <typename T>
 hipError_t qk_elements(const tops_gla_qk_args& a, bool backward, hipStream_t st) {
   if (a.D <= 8) return qk_launch<T, 1, 8, 1>(a, backward, st);

@@ -204,3 +204,14 @@ def test_empty_calls():
     assert q.shape == (2, 0, 4, 64)
     g, = torch.autograd.grad(q, d["q_weight"], q.detach())
     assert (g == 0).all()
+
+
+@pytest.mark.parametrize("D,R", [(130, 130), (256, 100), (200, 4), (258, 2), (512, 500), (384, 0),
+                                 (257, 256), (512, 512)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_wide_heads(D, R, inter, dt):
+    """More than 128 columns on aligned rows, with a rotated half that is no whole number of the
+    lanes' pieces, and with one that is."""
+    x, r = make(2, 5, 3, 2, D, dt)
+    check(x, rotary_inv_freq(R), None, inter, r)
