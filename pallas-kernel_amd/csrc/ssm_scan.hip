@@ -5,15 +5,17 @@
 // C_t are the same for all of a wave's channels: a first launch writes them as float32 rows
 // (`bc`), which the scan then reads through the scalar cache, into scalar registers that the FMAs
 // take directly. Neither a shuffle nor LDS is left in the forward's loop; it is bound by the
-// vector units: an exponential (two issue slots), two products and two FMAs a state and token.
-// MI355X, B2 T4096 D4096 N16 bf16: 160 us the outputs with the states kept for the backward, 84 %
-// vector issue (3.4 T state steps a second); four lanes a channel with B, C and delta' in LDS
-// took 204.
+// vector units: an exponential, two products and two FMAs a state and token. Measured costs of a
+// wave's operation in cycles of its SIMD: exponential 8, one with a scalar operand 4, any other 2.
+// MI355X, B2 T4096 D4096 N16 bf16: 161 us the outputs with the states kept for the backward (3.3 T
+// state steps a second; vector units active 82 % of the time as the counter has it, four cycles for
+// any operation but the exponential; 58 % at the costs above); four lanes a channel with B, C
+// and delta' in LDS took 204.
 //
 // Pieces: h_t = a_t h_{t-1} + b_t is linear, so a sequence is cut into pieces that run in
 // parallel. A first pass finds each piece's state from zero (L) and its summed delta' (S), a
 // small one folds them in order, h <- exp(A S_j) h + L_j, and leaves every piece's entry state
-// (at the sizes above 115 us and 17 us: the price of 8192 waves instead of 128).
+// (at the sizes above 114 us and 18 us: the price of 8192 waves instead of 128).
 #include <type_traits>
 
 #include "common.hpp"
@@ -400,8 +402,9 @@ __global__ __launch_bounds__(FOLD_NT) void scan_fold_kernel(ScanParams p) {
 // states each. They share what is formed once for a (token, channel) through LDS: each wave
 // stages 8 / NW of the tile's tokens and, once the waves' sums over n are there, finishes them. The
 // sums over the channels, of 16 values a token, transpose on their way down (32 operations for
-// them all). Bound by vector issue, 85 % busy: 24 instructions a state and token, 18 of them the
-// formulas'; MI355X, B2 T4096 D4096 N16 bf16: 476 us (a token more in registers costs the third
+// them all). Bound by vector issue (active 87 % of the time as counted, 53 % at the costs above): 25
+// instructions a state and token, 18 of them the formulas'; the compiler moves 60 to 105 scalars to
+// lanes of vector registers (82 with 16 states). MI355X, B2 T4096 D4096 N16 bf16: 481 us (a token more in registers costs the third
 // wave of a SIMD: all 8 at two waves 574; four lanes a channel and LDS rows of B and C 1145).
 //
 // EDGE: 1 with padded states, 2 where some lanes have no channel (padded states or not). Infinite
