@@ -191,7 +191,7 @@ int64_t tops_gla_selective_scan_piece(int64_t tokens, int64_t nseq, int64_t D, i
   if (nseq * tiles_of(D, G) * G >= 2048) return 1 << 30;
   // as many waves a SIMD as the states in registers allow in the pieces' own passes, eight with 16
   // of them (62 and 64 registers), and at most 512 pieces for the fold to walk. The outputs' pass
-  // holds five (82), its second round of them is not full: still the best of those measured (4096,
+  // holds five (82), and its last waves leave SIMDs idle: still the best of those measured (4096,
   // 5461, 6144, 8192, 10923, 16384 waves in all, N 16: 8192 packed tokens of 2048 channels 179, 179,
   // 167, 162, 162, 171 us; training B2 T4096 D4096 912, 931, 927, 870, 899, 918)
   const int64_t np = tops::scan_state_pad((int)N), waves = np <= 16 ? 8192 : 131072 / np;
