@@ -1,0 +1,198 @@
+// extern "C" entry points declared in include/tops_gla_delta.h: argument validation and dispatch.
+// No entry point allocates, synchronizes, or launches anything for invalid arguments.
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <initializer_list>
+
+#include "delta.hpp"
+
+namespace {
+
+constexpr int64_t kMax = 2147483647;
+// Tokens of a call: the kernels form token indices of 32 bits up to a chunk past a sequence's end.
+constexpr int64_t kMaxTokens = (1LL << 31) - 64;
+
+int fail(int code, const char* fmt, ...) {
+  char msg[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return tops::set_error(code, msg);
+}
+
+int done(hipError_t e, const char* what) {
+  if (e == hipSuccess) return tops::set_error(TOPS_GLA_OK, "");
+  return fail(TOPS_GLA_EHIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+bool dtype_ok(int64_t d) { return d == TOPS_GLA_F32 || d == TOPS_GLA_BF16; }
+
+bool any_null(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (p == nullptr) return true;
+  return false;
+}
+
+// Whether a launch has fewer than 2^32 threads and 2^31 blocks, as it must.
+bool grid_fits(int64_t blocks, int64_t threads) {
+  return blocks < (1LL << 32) / threads && blocks <= kMax;
+}
+
+int head_sizes(int64_t H, int64_t HV, int64_t K, int64_t V) {
+  if (K < 1 || K > 256)
+    return fail(TOPS_GLA_EUNSUPPORTED, "key size K must be in [1, 256] (K=%lld)", (long long)K);
+  if (V < 1 || V > 65536)
+    return fail(TOPS_GLA_EUNSUPPORTED, "value size V must be in [1, 65536] (V=%lld)", (long long)V);
+  if (H < 1 || HV < 1 || HV > 65536 || HV % H)
+    return fail(TOPS_GLA_EINVAL, "H must divide HV (H=%lld, HV=%lld)", (long long)H, (long long)HV);
+  return TOPS_GLA_OK;
+}
+
+int types(int64_t dtype, int64_t g_dtype, int64_t beta_dtype) {
+  if (!dtype_ok(dtype) || !dtype_ok(g_dtype) || !dtype_ok(beta_dtype))
+    return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  return TOPS_GLA_OK;
+}
+
+bool aligned(const void* p) { return ((uintptr_t)p & 255) == 0; }
+
+int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* p) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (int rc = types(a->dtype, a->g_dtype, a->beta_dtype)) return rc;
+  if (int rc = head_sizes(a->H, a->HV, a->K, a->V)) return rc;
+  if (a->batch < 0 || a->T < 0 || a->nseq < 0 || a->chunks < 0)
+    return fail(TOPS_GLA_EINVAL, "bad batch, T, nseq or chunks");
+  if (a->T > kMax || a->batch > kMax || a->batch * a->T >= kMaxTokens)
+    return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 - 64 tokens");
+  const int64_t C = tops::delta_chunk_of((int)a->dtype), per = (a->T + C - 1) / C;
+  if (a->seqs == nullptr) {
+    if (a->nseq != a->batch || a->chunks != a->batch * per)
+      return fail(TOPS_GLA_EINVAL, "nseq must be the batch, chunks its chunks");
+  } else {
+    if (a->batch != 1) return fail(TOPS_GLA_EINVAL, "packed sequences require batch == 1");
+    if (a->nseq > kMax / 2 || a->chunks < per || a->chunks > per + a->nseq)
+      return fail(TOPS_GLA_EINVAL, "bad nseq or chunks");
+  }
+  // the blocks of the largest launches, of 256 threads or fewer
+  if (!grid_fits(a->chunks, 1) || !grid_fits(a->chunks * a->HV, 256) ||
+      !grid_fits((a->V + 31) / 32 * a->HV, 256) ||
+      !grid_fits((a->V + 31) / 32 * a->HV * a->nseq, 256))
+    return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->chunks > 0 && any_null({a->q, a->k, a->v, a->g, a->beta}))
+    return fail(TOPS_GLA_EINVAL, "q, k, v, g and beta must not be NULL");
+  if (!backward && a->chunks > 0 && a->o == nullptr)
+    return fail(TOPS_GLA_EINVAL, "o must not be NULL");
+  *p = tops::delta_layout(a->chunks, a->HV, a->K, a->V, (int)a->dtype, a->train || backward,
+                          a->keep, a->ws);
+  if (p->keep_bytes > 0 &&
+      (a->keep == nullptr || a->keep_bytes < p->keep_bytes || !aligned(a->keep)))
+    return fail(TOPS_GLA_EINVAL, "keep must hold %lld bytes, 256-byte aligned",
+                (long long)p->keep_bytes);
+  p->a = *a;
+  if (!backward) return TOPS_GLA_OK;
+  if (a->chunks > 0 && any_null({a->dout, a->dq, a->dk, a->dv, a->dg, a->dbeta}))
+    return fail(TOPS_GLA_EINVAL, "dout, dq, dk, dv, dg and dbeta must not be NULL");
+  if (p->ws_bytes > 0 && (a->ws == nullptr || a->ws_bytes < p->ws_bytes || !aligned(a->ws)))
+    return fail(TOPS_GLA_EINVAL, "ws must hold %lld bytes, 256-byte aligned",
+                (long long)p->ws_bytes);
+  return TOPS_GLA_OK;
+}
+
+int norm_check(const tops_gla_layer_norm_args* a) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (!dtype_ok(a->dtype)) return fail(TOPS_GLA_EINVAL, "dtype must be F32 (0) or BF16 (1)");
+  if (a->rows < 0 || a->rows > (1LL << 40)) return fail(TOPS_GLA_EINVAL, "bad rows");
+  if (a->D < 1 || a->D > 16384)
+    return fail(TOPS_GLA_EUNSUPPORTED, "D must be in [1, 16384] (D=%lld)", (long long)a->D);
+  if (a->rows > 0 && a->x == nullptr) return fail(TOPS_GLA_EINVAL, "x must not be NULL");
+  return TOPS_GLA_OK;
+}
+
+bool sizes_ok(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype) {
+  return chunks >= 0 && chunks <= kMax && HV >= 1 && HV <= 65536 && K >= 1 && K <= 256 && V >= 1 &&
+         V <= 65536 && dtype_ok(dtype) && chunks * HV <= kMax;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t tops_gla_delta_chunk(int64_t dtype) {
+  return dtype_ok(dtype) ? tops::delta_chunk_of((int)dtype) : 0;
+}
+
+int64_t tops_gla_delta_keep_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype,
+                                  int64_t train) {
+  if (!sizes_ok(chunks, HV, K, V, dtype)) return 0;
+  return tops::delta_layout(chunks, HV, K, V, (int)dtype, train != 0, nullptr, nullptr).keep_bytes;
+}
+
+int64_t tops_gla_delta_ws_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype) {
+  if (!sizes_ok(chunks, HV, K, V, dtype)) return 0;
+  return tops::delta_layout(chunks, HV, K, V, (int)dtype, true, nullptr, nullptr).ws_bytes;
+}
+
+int tops_gla_delta_fwd(const tops_gla_delta_args* a, void* stream) {
+  tops::DeltaParams p;
+  if (int rc = delta_setup(a, false, &p)) return rc;
+  return done(tops::run_delta_fwd(p, (hipStream_t)stream), "delta_fwd");
+}
+
+int tops_gla_delta_bwd(const tops_gla_delta_args* a, void* stream) {
+  tops::DeltaParams p;
+  if (int rc = delta_setup(a, true, &p)) return rc;
+  return done(tops::run_delta_bwd(p, (hipStream_t)stream), "delta_bwd");
+}
+
+int tops_gla_delta_step(const tops_gla_delta_step_args* a, void* stream) {
+  if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
+  if (int rc = types(a->dtype, a->g_dtype, a->beta_dtype)) return rc;
+  if (int rc = head_sizes(a->H, a->HV, a->K, a->V)) return rc;
+  if (a->batch < 0 || a->T < 0 || a->slots < 0)
+    return fail(TOPS_GLA_EINVAL, "bad batch, T or slots");
+  if (a->slots_idx == nullptr && a->batch > a->slots)
+    return fail(TOPS_GLA_EINVAL, "the states hold %lld rows, the batch %lld", (long long)a->slots,
+                (long long)a->batch);
+  if (a->batch > kMax || a->T > kMax || !grid_fits((a->V + 63) / 64 * a->HV, 256) ||
+      !grid_fits((a->V + 63) / 64 * a->HV * a->batch, 256))
+    return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  if (a->batch > 0 && a->T > 0 && any_null({a->q, a->k, a->v, a->g, a->beta, a->o}))
+    return fail(TOPS_GLA_EINVAL, "q, k, v, g, beta and o must not be NULL");
+  if (a->batch > 0 && a->slots > 0 && a->state == nullptr)
+    return fail(TOPS_GLA_EINVAL, "state must not be NULL");
+  if (a->slots > 1 && a->state_ss < a->HV * a->K * a->V)
+    return fail(TOPS_GLA_EINVAL, "the slots overlap (%lld elements, a stride of %lld)",
+                (long long)(a->HV * a->K * a->V), (long long)a->state_ss);
+  return done(tops::run_delta_step(*a, (hipStream_t)stream), "delta_step");
+}
+
+int64_t tops_gla_layer_norm_ws_bytes(int64_t rows, int64_t D, int64_t dtype) {
+  if (rows < 0 || D < 1 || D > 16384 || !dtype_ok(dtype)) return 0;
+  // one row at least: the sums of no rows are written too
+  return std::max<int64_t>(1, tops::layer_norm_part_rows((long)rows, (long)D, (int)dtype)) * 8 * D;
+}
+
+int tops_gla_layer_norm_fwd(const tops_gla_layer_norm_args* a, void* stream) {
+  if (int rc = norm_check(a)) return rc;
+  if (a->rows > 0 && a->y == nullptr) return fail(TOPS_GLA_EINVAL, "y must not be NULL");
+  return done(tops::run_layer_norm_fwd(*a, (hipStream_t)stream), "layer_norm_fwd");
+}
+
+int tops_gla_layer_norm_bwd(const tops_gla_layer_norm_args* a, void* stream) {
+  if (int rc = norm_check(a)) return rc;
+  if (a->rows > 0 && any_null({a->stats, a->dy, a->dx}))
+    return fail(TOPS_GLA_EINVAL, "stats, dy and dx must not be NULL");
+  tops_gla_layer_norm_args c = *a;
+  if (a->dw || a->db) {
+    const int64_t need = tops_gla_layer_norm_ws_bytes(a->rows, a->D, a->dtype);
+    if (a->ws == nullptr || a->ws_bytes < need)
+      return fail(TOPS_GLA_EINVAL, "dw and db need ws of %lld bytes", (long long)need);
+  } else {
+    c.ws = nullptr;
+  }
+  return done(tops::run_layer_norm_bwd(c, (hipStream_t)stream), "layer_norm_bwd");
+}
+
+}  // extern "C"

@@ -1,0 +1,283 @@
+// Launch interface and device helpers of the gated delta rule and of the layer norm.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/tops_gla.h"
+#include "../../include/tops_gla_delta.h"
+#include "common.hpp"
+#include "kernels.hpp"
+#include "ssm.hpp"
+
+namespace tops {
+
+hipError_t run_layer_norm_fwd(const tops_gla_layer_norm_args& a, hipStream_t st);
+hipError_t run_layer_norm_bwd(const tops_gla_layer_norm_args& a, hipStream_t st);
+long layer_norm_part_rows(long rows, long D, int dtype);   // rows of 2 D partial sums
+
+hipError_t run_delta_step(const tops_gla_delta_step_args& a, hipStream_t st);
+
+// N consecutive elements at any address of theirs: the wide loads and stores need no alignment
+// beyond the element's.
+template <typename T, int N>
+struct Run {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Run<T, N> get_run(const T* p) {
+  return *reinterpret_cast<const Run<T, N>*>(p);
+}
+// The first n of them, zeros behind.
+template <typename T, int N>
+__device__ __forceinline__ Run<T, N> get_run(const T* p, int n) {
+  if (n >= N) return get_run<T, N>(p);
+  Run<T, N> r;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r.v[e] = e < n ? p[e] : zero_elem<T>();
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void put_run(T* p, const float (&x)[N], int n = N) {
+  if (n >= N) {
+    Run<T, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = from_f32<T>(x[e]);
+    *reinterpret_cast<Run<T, N>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < n) p[e] = from_f32<T>(x[e]);
+  }
+}
+
+// Element i of a tensor of either type.
+__device__ __forceinline__ float get_any(const void* p, int dtype, long i) {
+  return dtype == DT_BF16 ? to_f32(((const bf16*)p)[i]) : ((const float*)p)[i];
+}
+__device__ __forceinline__ void put_any(void* p, int dtype, long i, float x) {
+  if (dtype == DT_BF16)
+    ((bf16*)p)[i] = from_f32<bf16>(x);
+  else
+    ((float*)p)[i] = x;
+}
+
+constexpr float DELTA_L2_EPS = 1e-6f;
+
+// e^g as the log decay that the kernels work with: -inf (a state that is forgotten) stays finite,
+// so that differences of its sums do; e^-10000 is 0 all the same.
+__device__ __forceinline__ float log_decay(float g) { return g < -1e4f ? -1e4f : g; }
+
+// ---------------------------------------------------------------------------
+// The chunked form
+// ---------------------------------------------------------------------------
+
+// Tokens of a chunk: 64 in bfloat16, and 32 in float32, whose tiles take twice the LDS.
+template <typename T>
+constexpr int delta_c() {
+  return sizeof(T) == 2 ? 64 : 32;
+}
+inline int delta_chunk_of(int dtype) { return dtype == DT_BF16 ? 64 : 32; }
+inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
+
+// Per chunk and value head ("unit"): vectors over the chunk's tokens, [5][C] float and [C] double:
+//   e^{G_i}, e^{G_C - G_i}, beta, 1 / |k| (1 without l2norm), scale / |q|, and G, the sum of the
+//   log decays up to a token (in 64 bits: differences of it go into exponentials);
+// then, as tiles in the operands' type (two of them, high and low part, where it is bfloat16)
+//   Tm [C][C] the inverse of 1 + tril(beta k k^T decay), P [C][C] the masked scores,
+// and  N [V][C] the written values,  S [V][KP] the state before the chunk.
+struct DeltaParams {
+  tops_gla_delta_args a;
+  int C, KP, parts;   // tokens of a chunk, padded keys, parts of a split tile (2 or 1)
+  char *vec, *Tm, *P, *N, *S;   // in keep
+  char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
+                                // right side
+  long vec_bytes, keep_bytes, ws_bytes;
+};
+// The layout for given sizes; pointers from base addresses that may be NULL.
+DeltaParams delta_layout(int64_t chunks, int64_t HV, int64_t K, int64_t V, int dtype, bool train,
+                         void* keep, void* ws);
+hipError_t run_delta_fwd(const DeltaParams& p, hipStream_t st);
+hipError_t run_delta_bwd(const DeltaParams& p, hipStream_t st);
+
+struct ChunkAt {
+  int b, t, len;   // batch row, first token in it, tokens
+};
+__device__ __forceinline__ ChunkAt delta_chunk_at(const tops_gla_delta_args& a, int C, int c) {
+  ChunkAt x;
+  if (a.seqs) {
+    const int* cc = a.seqs + a.nseq + 1;
+    int lo = 0, hi = (int)a.nseq - 1;   // the last sequence whose first chunk is not behind c
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (cc[m] <= c) lo = m; else hi = m - 1;
+    }
+    x.b = 0;
+    x.t = a.seqs[lo] + (c - cc[lo]) * C;
+    x.len = min(C, a.seqs[lo + 1] - x.t);
+  } else {
+    const int nt = (int)((a.T + C - 1) / C);
+    x.b = c / nt;
+    x.t = (c - x.b * nt) * C;
+    x.len = min(C, (int)a.T - x.t);
+  }
+  return x;
+}
+
+__device__ __forceinline__ float* delta_vec(const DeltaParams& p, long unit) {
+  return (float*)(p.vec + unit * p.vec_bytes);
+}
+__device__ __forceinline__ double* delta_gsum(const DeltaParams& p, long unit) {
+  return (double*)(p.vec + unit * p.vec_bytes + 20 * p.C);
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_of(const Run<T, 8>& r) {
+  return __builtin_bit_cast(Frag<T>, r);
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_of(const float (&x)[8]);
+template <>
+__device__ __forceinline__ Frag<float> frag_of<float>(const float (&x)[8]) {
+  Frag<float> f;
+  f.a = make_float4(x[0], x[1], x[2], x[3]);
+  f.b = make_float4(x[4], x[5], x[6], x[7]);
+  return f;
+}
+template <>
+__device__ __forceinline__ Frag<bf16> frag_of<bf16>(const float (&x)[8]) {
+  Frag<bf16> f;
+  f.d = make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]),
+                   pack2_bf16(x[6], x[7]));
+  return f;
+}
+__device__ __forceinline__ void values_of(const Frag<float>& f, float (&x)[8]) {
+  x[0] = f.a.x, x[1] = f.a.y, x[2] = f.a.z, x[3] = f.a.w;
+  x[4] = f.b.x, x[5] = f.b.y, x[6] = f.b.z, x[7] = f.b.w;
+}
+__device__ __forceinline__ void values_of(const Frag<bf16>& f, float (&x)[8]) {
+  const uint32_t w[4] = {f.d.x, f.d.y, f.d.z, f.d.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
+}
+template <typename T>
+__device__ __forceinline__ void st_frag(T* p, const Frag<T>& f) {   // 16-byte aligned
+  __builtin_memcpy(__builtin_assume_aligned(p, 16), &f, sizeof(f));
+}
+
+// A float operand with the accuracy of its accumulator: in bfloat16 a high and a low part, whose
+// sum is 2^-18 of the value off at most. States and what they are made of go through products of
+// such operands, so that a state is as exact in bfloat16 calls as float32 allows.
+template <typename T>
+struct Split;
+template <>
+struct Split<float> {
+  Frag<float> f;
+};
+template <>
+struct Split<bf16> {
+  Frag<bf16> hi, lo;
+};
+template <typename T>
+__device__ __forceinline__ Split<T> split_of(const float (&x)[8]);
+template <>
+__device__ __forceinline__ Split<float> split_of<float>(const float (&x)[8]) {
+  return {frag_of<float>(x)};
+}
+template <>
+__device__ __forceinline__ Split<bf16> split_of<bf16>(const float (&x)[8]) {
+  Split<bf16> s;
+  s.hi = frag_of<bf16>(x);
+  float h[8];
+  values_of(s.hi, h);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = x[e] - h[e];
+  s.lo = frag_of<bf16>(h);
+  return s;
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Frag<float>& a, const Split<float>& b) {
+  mma(acc, a, b.f);
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Frag<bf16>& a, const Split<bf16>& b) {
+  mma(acc, a, b.lo);
+  mma(acc, a, b.hi);
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Split<float>& a, const Frag<float>& b) {
+  mma(acc, a.f, b);
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Split<bf16>& a, const Frag<bf16>& b) {
+  mma(acc, a.lo, b);
+  mma(acc, a.hi, b);
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Split<float>& a, const Split<float>& b) {
+  mma(acc, a.f, b.f);
+}
+__device__ __forceinline__ void mma(f32x4& acc, const Split<bf16>& a, const Split<bf16>& b) {
+  mma(acc, a.hi, b.lo);   // the product of the low parts is below what the sum keeps
+  mma(acc, a.lo, b.hi);
+  mma(acc, a.hi, b.hi);
+}
+
+// Output tiles come in pairs (h = 0, 1) of 32 rows: row 4 g + r of tile h stands for row
+// 8 g + 4 h + r, so that a lane's accumulators of both tiles are 8 consecutive rows of its column,
+// which is what an operand fragment over those rows holds: a result becomes the next product's
+// operand without leaving its lane. The row that lane i supplies to tile h as the first operand:
+__device__ __forceinline__ int pair_row(int lane, int h) {
+  return 8 * ((lane & 15) >> 2) + 4 * h + (lane & 3);
+}
+// The same rows read from a row-major [k][row] tile in LDS (M at element [k0][row0]).
+__device__ __forceinline__ Frag<bf16> ld_pair_t(const bf16* M, int P, int lane, int h) {
+  const int g = lane >> 4, j = lane & 15;
+  const bf16* p1 = M + (8 * g + (j >> 2)) * P + 8 * (j & 3) + 4 * h;
+  const s4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s4_t*)(p1));
+  const s4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s4_t*)(p1 + 4 * P));
+  const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+  Frag<bf16> f;
+  f.d = make_uint4(ua.x, ua.y, ub.x, ub.y);
+  return f;
+}
+__device__ __forceinline__ Frag<float> ld_pair_t(const float* M, int P, int lane, int h) {
+  const float* p = M + (8 * (lane >> 4)) * P + pair_row(lane, h);
+  Frag<float> f;
+  f.a = make_float4(p[0], p[P], p[2 * P], p[3 * P]);
+  f.b = make_float4(p[4 * P], p[5 * P], p[6 * P], p[7 * P]);
+  return f;
+}
+// The 8 values of a lane in a pair of accumulators.
+__device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, float (&x)[8]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = a[r], x[4 + r] = b[r];
+}
+
+// A [C][w] tile on its way to LDS, w a multiple of 8: pieces of 8 elements, zeros past `len` rows
+// and `cols` columns.
+template <typename T, int C, int W, int NT>
+struct TileFetch {
+  static constexpr int PER = C * W / 8, N = (PER + NT - 1) / NT;
+  Run<T, 8> r[N];
+  __device__ __forceinline__ void get(const T* src, long st, int len, int cols, int tid) {
+    const bool whole = cols % 8 == 0;   // the same for all: pieces end where the columns do
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * NT + tid, row = p / (W / 8), col = p % (W / 8) * 8;
+      r[i] = Run<T, 8>{};
+      if ((PER % NT == 0 || p < PER) && row < len && col < cols) {
+        if (whole)
+          r[i] = get_run<T, 8>(src + row * st + col);
+        else
+          r[i] = get_run<T, 8>(src + row * st + col, cols - col);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(T* dst, int pitch, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * NT + tid;
+      if (PER % NT == 0 || p < PER)
+        st_frag(dst + p / (W / 8) * pitch + p % (W / 8) * 8, frag_of<T>(r[i]));
+    }
+  }
+};
+
+}  // namespace tops

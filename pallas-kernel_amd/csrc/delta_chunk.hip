@@ -1,0 +1,535 @@
+// The gated delta rule over chunks of C tokens, forward (include/tops_gla_delta.h).
+//
+// Within a chunk with the state S before it, G_i the sum of the log decays up to token i and
+// D_ij = e^{G_i - G_j} for j <= i, the written values solve a unit triangular system:
+//   (1 + A) N = beta (V - e^G (K S)),  A_ij = beta_i (k_i . k_j) D_ij below the diagonal.
+// With Tm = (1 + A)^-1, which needs no state:
+//   N = Tm (beta (V - e^G (K S))),   S <- e^{G_C} S + K^T (e^{G_C - G} N),
+//   o = scale (e^G (Q S) + ((Q K^T) D) N).
+// Three launches: Tm of every chunk at once; the states, which go from chunk to chunk; the outputs
+// of every chunk at once. The columns of S and N are independent of one another, so that a wave of
+// the second launch owns 16 of them over all chunks of a sequence and head, with the state in its
+// accumulators: K S, Tm R and K^T N hand their results on as operands without leaving a lane.
+#include "delta.hpp"
+
+namespace tops {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Tm and the vectors of a chunk
+// ---------------------------------------------------------------------------
+
+// X . Y over 16 with float operands: X row-major in LDS, Y in accumulator layout.
+__device__ __forceinline__ void mma16(f32x4& acc, const float* X, int px, const f32x4& y,
+                                      int lane) {
+  const float4 x = *reinterpret_cast<const float4*>(X + (lane & 15) * px + 4 * (lane >> 4));
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y[2], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y[3], acc, 0, 0, 0);
+}
+
+// A block has a chunk and a key head, and goes through its value heads. K K^T on the matrix units;
+// the inverse in float32: the 16 x 16 diagonal blocks by substitution, a lane a column, then the
+// blocks below them, one diagonal after another: T_ij = -T_ii sum_k A_ik T_kj.
+template <typename T, int KP>
+__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
+  constexpr int C = delta_c<T>(), NB = C / 16, PK = pitch_of<T>(KP), PA = C + 4;
+  __shared__ __attribute__((aligned(16))) T sK[C * PK];
+  __shared__ __attribute__((aligned(16))) float sA[C * PA], sT[C * PA];
+  __shared__ double sG[C];
+  __shared__ float sBeta[C], sRk[C];
+  const tops_gla_delta_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int H = (int)a.H, HV = (int)a.HV, K = (int)a.K;
+  const int chunk = (int)(blockIdx.x / H), h = (int)(blockIdx.x % H);
+  const ChunkAt at = delta_chunk_at(a, C, chunk);
+  {
+    TileFetch<T, C, KP, 256> f;
+    f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
+    f.put(sK, PK, tid);
+  }
+  __syncthreads();
+  {   // 1 / |k|: 256 / C threads a row
+    constexpr int TR = 256 / C;
+    const int row = tid / TR;
+    float s = 0.f;
+    if (a.l2norm) {
+      for (int c = tid % TR; c < K; c += TR) {
+        const float x = to_f32(sK[row * PK + c]);
+        s = fmaf(x, x, s);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < TR; o <<= 1) s += __shfl_xor(s, o);
+    if (tid % TR == 0) sRk[row] = a.l2norm ? rsqrtf(s + DELTA_L2_EPS) : 1.f;
+  }
+  f32x4 kk[NB];
+  if (wave < NB) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      kk[j] = zero4();
+      if (j <= wave) mma_tile<T>(kk[j], sK + wave * 16 * PK, PK, sK + j * 16 * PK, PK, KP, lane);
+    }
+  }
+  const int group = HV / H;
+  for (int gi = 0; gi < group; ++gi) {
+    const int hv = h * group + gi;
+    const long unit = (long)chunk * HV + hv;
+    if (wave == 0) {
+      float g = 0.f, beta = 0.f;
+      if (lane < at.len) {
+        g = log_decay(get_any(a.g, (int)a.g_dtype, at.b * a.g_sb + (at.t + lane) * a.g_st + hv));
+        beta = get_any(a.beta, (int)a.beta_dtype,
+                       at.b * a.beta_sb + (at.t + lane) * a.beta_st + hv);
+      }
+      double s = g;
+#pragma unroll
+      for (int o = 1; o < C; o <<= 1) {
+        const double x = __shfl_up(s, o);
+        if (lane >= o) s += x;
+      }
+      if (lane < C) {
+        sG[lane] = s;
+        sBeta[lane] = beta;
+      }
+    }
+    for (int i = tid; i < C * C; i += 256) sT[i / C * PA + i % C] = 0.f;
+    __syncthreads();
+    if (tid < C) {
+      float* vec = delta_vec(p, unit);
+      const double G = sG[tid];
+      vec[tid] = expf((float)G);
+      vec[C + tid] = expf((float)(sG[C - 1] - G));
+      vec[2 * C + tid] = sBeta[tid];
+      vec[3 * C + tid] = sRk[tid];
+      vec[4 * C + tid] = 0.f;   // the outputs' launch writes it for the tokens there are
+      delta_gsum(p, unit)[tid] = G;
+    }
+    if (wave < NB) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        if (j > wave) continue;
+        const int col = 16 * j + (lane & 15);
+        const double gj = sG[col];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * wave + 4 * (lane >> 4) + r;
+          // a product only where it counts: what is masked may be anything
+          sA[row * PA + col] =
+              row > col ? sBeta[row] * sRk[row] * sRk[col] * kk[j][r] * expf((float)(sG[row] - gj))
+                        : 0.f;
+        }
+      }
+    }
+    __syncthreads();
+    if (wave < NB && lane < 16) {
+      float x[16];
+      const float* A = sA + 16 * wave * PA + 16 * wave;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float s = i == lane ? 1.f : 0.f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) s = fmaf(-A[i * PA + j], x[j], s);
+        x[i] = s;
+        sT[(16 * wave + i) * PA + 16 * wave + lane] = s;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < NB; ++d) {
+      __syncthreads();
+      if (wave < NB - d) {   // block (wave + d, wave)
+        const int bi = wave + d, bj = wave;
+        f32x4 m = zero4(), t = zero4();
+#pragma unroll
+        for (int k = 0; k < d; ++k) {   // A_ik T_kj, k from bj on
+          const float* y = sT + (16 * (bj + k) + 4 * (lane >> 4)) * PA + 16 * bj + (lane & 15);
+          const f32x4 yv = {y[0], y[PA], y[2 * PA], y[3 * PA]};
+          mma16(m, sA + 16 * bi * PA + 16 * (bj + k), PA, yv, lane);
+        }
+        mma16(t, sT + 16 * bi * PA + 16 * bi, PA, m, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          sT[(16 * bi + 4 * (lane >> 4) + r) * PA + 16 * bj + (lane & 15)] = -t[r];
+      }
+    }
+    __syncthreads();
+    T* out = (T*)(p.Tm + unit * (C * C * 4));
+    for (int i = tid; i < C * C / 8; i += 256) {
+      const int row = i / (C / 8), col = i % (C / 8) * 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = sT[row * PA + col + e];
+      const Split<T> s = split_of<T>(x);
+      if constexpr (sizeof(T) == 2) {
+        st_frag(out + row * C + col, s.hi);
+        st_frag(out + C * C + row * C + col, s.lo);
+      } else {
+        st_frag(out + row * C + col, s.f);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The states
+// ---------------------------------------------------------------------------
+
+template <typename T, int KP, int NW>
+struct ScanLds {
+  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(16 * NW);
+  static constexpr int K0 = 0, T0 = C * PK, V0 = T0 + PARTS * C * PT, END = V0 + C * PV;
+  static constexpr int F0 = END * (int)sizeof(T);                // three vectors of floats, e^{G_C}
+  static constexpr int BYTES = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // of one of two buffers
+};
+
+template <typename T>
+__device__ __forceinline__ Split<T> ld_split(const T* tile, int lo, int off);
+template <>
+__device__ __forceinline__ Split<float> ld_split<float>(const float* tile, int, int off) {
+  return {ld_frag(tile + off)};
+}
+template <>
+__device__ __forceinline__ Split<bf16> ld_split<bf16>(const bf16* tile, int lo, int off) {
+  return {ld_frag(tile + off), ld_frag(tile + lo + off)};
+}
+
+template <typename T, int KP, int NW>
+__global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
+  using L = ScanLds<T, KP, NW>;
+  constexpr int C = L::C, NT = 64 * NW, NS = KP / 32, NU = C / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const tops_gla_delta_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = lane >> 4, ci = lane & 15;
+  const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
+  const int vt = (V + 16 * NW - 1) / (16 * NW);
+  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);   // a head's columns on one XCD
+  const int vb = blk % vt;
+  blk /= vt;
+  const int hv = blk % HV, seq = blk / HV, h = hv / (HV / (int)a.H);
+  int b = 0, t0 = 0, T_ = (int)a.T, c0 = 0;
+  if (a.seqs) {
+    t0 = a.seqs[seq];
+    T_ = a.seqs[seq + 1] - t0;
+    c0 = a.seqs[a.nseq + 1 + seq];
+  } else {
+    b = seq;
+    c0 = seq * ((T_ + C - 1) / C);
+  }
+  const int nc = (T_ + C - 1) / C;
+  const T* kp = (const T*)a.k + b * a.k_sb + t0 * a.k_st + h * a.k_sh;
+  const T* vp = (const T*)a.v + b * a.v_sb + t0 * a.v_st + hv * a.v_sh + vb * 16 * NW;
+  const int v = vb * 16 * NW + 16 * wave + ci;
+  const bool vin = v < V;
+
+  // K row 32 s + 8 g + 4 h + r of the state in S[2 s + h][r]
+  f32x4 S[2 * NS];
+  const long st0 = ((long)seq * HV + hv) * K * V + v;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
+      S[i][r] = a.h0 && vin && k < K ? a.h0[st0 + (long)k * V] : 0.f;
+    }
+
+  TileFetch<T, C, KP, NT> fk;
+  TileFetch<T, L::PARTS * C, C, NT> ft;
+  TileFetch<T, C, 16 * NW, NT> fv;
+  constexpr int NF = (3 * C + NT) / NT;
+  float ff[NF];
+  auto fetch = [&](int n) {
+    const int len = min(C, T_ - n * C);
+    const long unit = (long)(c0 + n) * HV + hv;
+    fk.get(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
+    ft.get((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
+    fv.get(vp + (long)n * C * a.v_st, a.v_st, len, V - vb * 16 * NW, tid);
+    const float* vec = delta_vec(p, unit);
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta
+      const int x = i * NT + tid;
+      if (x < 2 * C)
+        ff[i] = vec[x] * vec[3 * C + x % C];
+      else if (x <= 3 * C)
+        ff[i] = vec[x < 3 * C ? x : C - 1];
+    }
+  };
+  auto put = [&](int n) {
+    T* sm = (T*)(smem + (n & 1) * L::BYTES);
+    fk.put(sm + L::K0, L::PK, tid);
+    ft.put(sm + L::T0, L::PT, tid);
+    fv.put(sm + L::V0, L::PV, tid);
+    float* sf = (float*)(smem + (n & 1) * L::BYTES + L::F0);
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i];
+  };
+  if (nc > 0) {
+    fetch(0);
+    put(0);
+  }
+  for (int n = 0; n < nc; ++n) {
+    __syncthreads();
+    if (n + 1 < nc) fetch(n + 1);
+    const T* sm = (const T*)(smem + (n & 1) * L::BYTES);
+    const T *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + 16 * wave;
+    const float* sf = (const float*)(smem + (n & 1) * L::BYTES + L::F0);
+    const long unit = (long)(c0 + n) * HV + hv;
+    const float last = sf[3 * C];
+
+    f32x4 acc[2 * NU];
+#pragma unroll
+    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
+    T* So = (T*)p.S + (unit * V + v) * KP + 8 * g;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      float x[8];
+      pair_values(S[2 * s], S[2 * s + 1], x);
+      const Split<T> f = split_of<T>(x);
+      if constexpr (sizeof(T) == 2) {
+        if (vin) st_frag(So + 32 * s, f.hi);
+      } else {
+        if (vin) st_frag(So + 32 * s, f.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NU; ++i)
+        mma(acc[i], ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g),
+            f);
+    }
+    Split<T> R[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      float x[8], y[8];
+      values_of(ld_frag_t(sV + 32 * u * L::PV, L::PV, lane), y);
+      pair_values(acc[2 * u], acc[2 * u + 1], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int t = 32 * u + 8 * g + e;
+        x[e] = sf[2 * C + t] * (y[e] - sf[t] * x[e]);
+      }
+      R[u] = split_of<T>(x);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
+#pragma unroll
+    for (int w = 0; w < NU; ++w)
+#pragma unroll
+      for (int i = 0; i < 2 * NU; ++i)
+        if (w <= (i >> 1))
+          mma(acc[i], ld_split<T>(sT, C * L::PT, (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PT +
+                                                     32 * w + 8 * g), R[w]);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
+    T* No = (T*)p.N + (unit * V + v) * C + 8 * g;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      float x[8];
+      pair_values(acc[2 * u], acc[2 * u + 1], x);
+      if (vin) st_frag(No + 32 * u, frag_of<T>(x));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
+      const Split<T> f = split_of<T>(x);
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i)
+        mma(S[i], ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1), f);
+    }
+    if (n + 1 < nc) put(n + 1);
+  }
+  if (a.ht && vin) {
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
+        if (k < K) a.ht[st0 + (long)k * V] = S[i][r];
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The outputs
+// ---------------------------------------------------------------------------
+
+// 8 elements of row `r` of q or k from column c on, zeros past K.
+template <typename T>
+__device__ __forceinline__ Frag<T> ld_row(const T* base, long st, int r, int c, int K) {
+  if (c >= K) return frag_of<T>(Run<T, 8>{});
+  if (K % 8 == 0) return frag_of<T>(get_run<T, 8>(base + r * st + c));
+  return frag_of<T>(get_run<T, 8>(base + r * st + c, K - c));
+}
+
+// A wave has 16 tokens of a chunk as columns: scores (rows: the tokens before them), then outputs
+// (rows: the values), whose lanes hold 8 consecutive values of their token.
+template <typename T, int KP>
+__global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams p) {
+  constexpr int C = delta_c<T>(), NU = C / 32, NS = KP / 32;
+  __shared__ double sG[C];
+  __shared__ float sRk[C];
+  const tops_gla_delta_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = lane >> 4, ci = lane & 15;
+  const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
+  const int chunk = (int)(blockIdx.x / HV), hv = (int)(blockIdx.x % HV);
+  const int h = hv / (HV / (int)a.H);
+  const long unit = blockIdx.x;
+  const ChunkAt at = delta_chunk_at(a, C, chunk);
+  float* vec = delta_vec(p, unit);
+  if (tid < C) {
+    sG[tid] = delta_gsum(p, unit)[tid];
+    sRk[tid] = vec[3 * C + tid];
+  }
+  __syncthreads();
+  if (16 * wave >= at.len) return;
+  const int i = 16 * wave + ci, row = min(i, at.len - 1);   // the last token again past the end
+  const T* q = (const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh;
+  const T* k = (const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh;
+  Frag<T> qf[NS];
+  float qq = 0.f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = ld_row(q, a.q_st, row, 32 * s + 8 * g, K);
+    float x[8];
+    values_of(qf[s], x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qq = fmaf(x[e], x[e], qq);
+  }
+  qq = swap32_add(qq, qq);
+  qq = swap16_add(qq, qq);
+  const float fq = (float)a.scale * (a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f);
+  if (a.train && lane < 16) vec[4 * C + i] = fq;
+  const float fo = fq * vec[i];
+  const double gi = sG[i];
+  Frag<T> pf[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    if (32 * u > 16 * wave + 15) continue;
+    f32x4 acc[2] = {zero4(), zero4()};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+        mma(acc[hh], ld_row(k, a.k_st, min(32 * u + pair_row(lane, hh), at.len - 1),
+                            32 * s + 8 * g, K), qf[s]);
+    float x[8];
+    pair_values(acc[0], acc[1], x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = 32 * u + 8 * g + e;
+      x[e] = j <= i ? fq * sRk[j] * x[e] * gexp<T>((float)(gi - sG[j])) : 0.f;
+    }
+    const Split<T> sp = split_of<T>(x);
+    T* out = (T*)(p.P + unit * (C * C * 4)) + i * C + 32 * u + 8 * g;
+    if constexpr (sizeof(T) == 2) {
+      pf[u] = sp.hi;
+      if (a.train) {
+        st_frag(out, sp.hi);
+        st_frag(out + C * C, sp.lo);
+      }
+    } else {
+      pf[u] = sp.f;
+      if (a.train) st_frag(out, sp.f);
+    }
+  }
+  T* o = (T*)a.o + (((long)at.b * a.T + at.t + i) * HV + hv) * V;
+  const T* S = (const T*)p.S + unit * V * KP + 8 * g;
+  const T* N = (const T*)p.N + unit * V * C + 8 * g;
+  for (int v0 = 0; v0 < V; v0 += 32) {
+    const int va = min(v0 + pair_row(lane, 0), V - 1), vb = min(v0 + pair_row(lane, 1), V - 1);
+    f32x4 acc[2] = {zero4(), zero4()};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      mma(acc[0], ld_frag(S + (long)va * KP + 32 * s), qf[s]);
+      mma(acc[1], ld_frag(S + (long)vb * KP + 32 * s), qf[s]);
+    }
+    acc[0] *= fo;
+    acc[1] *= fo;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if (32 * u > 16 * wave + 15) continue;
+      mma(acc[0], ld_frag(N + (long)va * C + 32 * u), pf[u]);
+      mma(acc[1], ld_frag(N + (long)vb * C + 32 * u), pf[u]);
+    }
+    float x[8];
+    pair_values(acc[0], acc[1], x);
+    const int c = v0 + 8 * g;
+    if (i < at.len && c < V) put_run<T, 8>(o + c, x, V - c);
+  }
+}
+
+// Waves of a block of the states' launch, 16 columns each: they share the chunk's tiles in LDS.
+int scan_waves(const DeltaParams& p) {
+  const long w = (p.a.V + 15) / 16 * p.a.HV * p.a.nseq;
+  return p.a.V <= 32 || w <= 512 ? 2 : 4;
+}
+
+template <typename T, int KP, int NW>
+hipError_t launch_scan(const DeltaParams& p, hipStream_t st) {
+  constexpr int lds = 2 * ScanLds<T, KP, NW>::BYTES;
+  const hipError_t e = hipFuncSetAttribute((const void*)delta_scan_kernel<T, KP, NW>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return e;
+  const long grid = (p.a.V + 16 * NW - 1) / (16 * NW) * p.a.HV * p.a.nseq;
+  delta_scan_kernel<T, KP, NW><<<(unsigned)grid, 64 * NW, lds, st>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T, int KP>
+hipError_t run(const DeltaParams& p, hipStream_t st) {
+  const tops_gla_delta_args& a = p.a;
+  if (a.chunks > 0) {
+    delta_prep_kernel<T, KP><<<(unsigned)(a.chunks * a.H), 256, 0, st>>>(p);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  if (a.nseq > 0) {
+    const hipError_t e = scan_waves(p) == 2 ? launch_scan<T, KP, 2>(p, st)
+                                            : launch_scan<T, KP, 4>(p, st);
+    if (e != hipSuccess) return e;
+  }
+  if (a.chunks > 0)
+    delta_out_kernel<T, KP><<<(unsigned)(a.chunks * a.HV), 4 * delta_c<T>(), 0, st>>>(p);
+  return hipGetLastError();
+}
+
+long up(long n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+DeltaParams delta_layout(int64_t chunks, int64_t HV, int64_t K, int64_t V, int dtype, bool train,
+                         void* keep, void* ws) {
+  DeltaParams p{};
+  const long es = dtype == DT_BF16 ? 2 : 4, units = chunks * HV;
+  p.C = delta_chunk_of(dtype);
+  p.KP = delta_key_pad(K);
+  p.vec_bytes = 28 * p.C;
+  long at = 0;
+  auto take = [&](void* base, long bytes) {
+    char* x = (char*)base + at;
+    at += up(bytes);
+    return x;
+  };
+  p.vec = take(keep, units * p.vec_bytes);
+  p.Tm = take(keep, units * p.C * p.C * 4);
+  p.N = take(keep, units * V * p.C * es);
+  p.S = take(keep, units * V * p.KP * es);
+  p.P = take(keep, train ? units * p.C * p.C * 4 : 0);
+  p.keep_bytes = at;
+  at = 0;
+  p.dS = take(ws, units * V * p.KP * es);
+  p.Y = take(ws, units * V * p.C * es);
+  p.ws_bytes = at;
+  return p;
+}
+
+hipError_t run_delta_fwd(const DeltaParams& p, hipStream_t st) {
+  if (p.a.dtype == DT_BF16)
+    return p.KP == 64 ? run<bf16, 64>(p, st) : p.KP == 128 ? run<bf16, 128>(p, st)
+                                                           : run<bf16, 256>(p, st);
+  return p.KP == 64 ? run<float, 64>(p, st) : p.KP == 128 ? run<float, 128>(p, st)
+                                                          : run<float, 256>(p, st);
+}
+
+}  // namespace tops

@@ -1,0 +1,143 @@
+// The gated delta rule for the next tokens of a serving batch, states updated in place
+// (include/tops_gla_delta.h).
+//
+// Bound by memory: the state of a row and head is read and written once, however many tokens come.
+// A wave holds all K rows of 16 columns of the state: a lane four columns of K / 16 consecutive
+// rows, so that the sums over the keys are sums of a lane and of the 16 lanes with its columns
+// (two rotations in a row of lanes, two swaps of rows), without LDS. One round of them serves a
+// token: with S' = e^g S, o = scale S_t^T q = scale (S'^T q + (q k) n), so S'^T k, S'^T q, q k and
+// the norms are summed together, before n is known.
+#include "delta.hpp"
+
+namespace tops {
+
+namespace {
+
+__device__ __forceinline__ float key_sum(float x) {
+  x += dpp<0x124>(x);
+  x += dpp<0x128>(x);
+  x = swap16_add(x, x);
+  return swap32_add(x, x);
+}
+
+// KR: rows of the state a lane.
+template <typename T, int KR>
+__global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_args a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int K = (int)a.K, V = (int)a.V, T_ = (int)a.T;
+  const int vt = (V + 63) / 64;
+  long blk = blockIdx.x;
+  const int vb = (int)(blk % vt);
+  blk /= vt;
+  const int hv = (int)(blk % a.HV);
+  const long b = blk / a.HV;
+  const int h = hv / (int)(a.HV / a.H);
+  const int c0 = vb * 64 + wave * 16 + (lane & 3) * 4;
+  const int r0 = (lane >> 2) * KR;
+  if (vb * 64 + wave * 16 >= V) return;
+  const int nc = V - c0, nr = K - r0;
+  T* o = (T*)a.o + ((b * T_) * a.HV + hv) * V + c0;
+  const long o_st = a.HV * V;
+
+  long slot = b;
+  if (a.slots_idx)
+    slot = a.idx64 ? ((const int64_t*)a.slots_idx)[b] : (long)((const int32_t*)a.slots_idx)[b];
+  if (slot < 0 || slot >= a.slots) {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    if (lane < 4 && nc > 0)
+      for (int t = 0; t < T_; ++t) put_run<T, 4>(o + t * o_st, zero, nc);
+    return;
+  }
+  float* S = a.state + slot * a.state_ss + (long)hv * K * V + (long)r0 * V + c0;
+  float s[KR][4];
+#pragma unroll
+  for (int r = 0; r < KR; ++r) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
+    if (r < nr && nc > 0) {
+      const auto x = get_run<float, 4>(S + (long)r * V, nc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[r][e] = x.v[e];
+    }
+  }
+  const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh + r0;
+  const T* k = (const T*)a.k + b * a.k_sb + h * a.k_sh + r0;
+  const T* v = (const T*)a.v + b * a.v_sb + hv * a.v_sh + c0;
+  const long g0 = b * a.g_sb + hv, b0 = b * a.beta_sb + hv;
+  for (int t = 0; t < T_; ++t) {
+    Run<T, KR> qr = {}, kr = {};
+    if (nr > 0) {
+      qr = get_run<T, KR>(q + t * a.q_st, nr);
+      kr = get_run<T, KR>(k + t * a.k_st, nr);
+    }
+    Run<T, 4> vr = {};
+    if (nc > 0) vr = get_run<T, 4>(v + t * a.v_st, nc);
+    const float ge = expf(get_any(a.g, (int)a.g_dtype, g0 + t * a.g_st));
+    const float beta = get_any(a.beta, (int)a.beta_dtype, b0 + t * a.beta_st);
+    float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f}, qk = 0.f, qq = 0.f, kk = 0.f;
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      const float x = to_f32(qr.v[r]), y = to_f32(kr.v[r]);
+      qk = fmaf(x, y, qk);
+      qq = fmaf(x, x, qq);
+      kk = fmaf(y, y, kk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sk[e] = fmaf(s[r][e], y, sk[e]);
+        sq[e] = fmaf(s[r][e], x, sq[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sk[e] = key_sum(sk[e]);
+      sq[e] = key_sum(sq[e]);
+    }
+    qk = key_sum(qk);
+    float rq = 1.f, rk = 1.f;
+    if (a.l2norm) {
+      rq = rsqrtf(key_sum(qq) + DELTA_L2_EPS);
+      rk = rsqrtf(key_sum(kk) + DELTA_L2_EPS);
+    }
+    float n[4], y[4];
+    const float fq = (float)a.scale * rq;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      n[e] = rk * beta * (to_f32(vr.v[e]) - ge * rk * sk[e]);   // what the raw key writes
+      y[e] = fq * fmaf(qk, n[e], ge * sq[e]);
+    }
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      const float x = to_f32(kr.v[r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[r][e] = fmaf(x, n[e], ge * s[r][e]);
+    }
+    if (lane < 4 && nc > 0) put_run<T, 4>(o + t * o_st, y, nc);
+  }
+#pragma unroll
+  for (int r = 0; r < KR; ++r)
+    if (r < nr && nc > 0) put_run<float, 4>(S + (long)r * V, s[r], nc);
+}
+
+template <typename T>
+void launch(const tops_gla_delta_step_args& a, unsigned grid, hipStream_t st) {
+  if (a.K <= 64)
+    delta_step_kernel<T, 4><<<grid, 256, 0, st>>>(a);
+  else if (a.K <= 128)
+    delta_step_kernel<T, 8><<<grid, 256, 0, st>>>(a);
+  else
+    delta_step_kernel<T, 16><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
+hipError_t run_delta_step(const tops_gla_delta_step_args& a, hipStream_t st) {
+  if (a.batch == 0 || a.T == 0) return hipSuccess;
+  const unsigned grid = (unsigned)((a.V + 63) / 64 * a.HV * a.batch);
+  if (a.dtype == DT_BF16)
+    launch<bf16>(a, grid, st);
+  else
+    launch<float>(a, grid, st);
+  return hipGetLastError();
+}
+
+}  // namespace tops

@@ -1,0 +1,305 @@
+// Layer norm and its gradients (include/tops_gla_delta.h).
+//
+//   y  = (x - mean) rstd w + b
+//   dx = rstd (u - mean(u) - n mean(u n)),  u = dy w,  n = (x - mean) rstd,
+//   dw = sum over rows of dy n,  db = sum over rows of dy
+//
+// Bound by memory: x (and dy) are read once into registers, the mean comes before the squares of
+// the differences (a variance from sum and sum of squares loses what a large mean covers), and the
+// next row's loads are on their way while a row is worked on. A row belongs to one wave up to 2048
+// features, to a block of 4 or 8 waves above; a thread holds at most 32 features, whose share of
+// w, b, dw and db stays in its registers over all its rows. The weights' sums go through one
+// partial row a block in a workspace and a second kernel, in fixed order.
+#include "delta.hpp"
+
+namespace tops {
+
+namespace {
+
+// Threads of a row by its features: 32 a thread at most.
+int row_threads(long D) { return D <= 2048 ? 64 : D <= 8192 ? 256 : 512; }
+int block_threads(long D) { return D <= 8192 ? 256 : 512; }
+long norm_blocks(long rows, long D, bool backward) {
+  const long per = block_threads(D) / row_threads(D);
+  // two waves a SIMD in the backward, four in the forward; fewer where the rows do not go round
+  const long most = (backward ? 512 : 1024) * 256 / block_threads(D);
+  return std::min((rows + per - 1) / per, most);
+}
+
+template <int NT>
+__device__ __forceinline__ float row_sum(float x, float* sm, int tid) {
+  x += dpp<0x121>(x);
+  x += dpp<0x122>(x);
+  x += dpp<0x124>(x);
+  x += dpp<0x128>(x);
+  x = swap16_add(x, x);
+  x = swap32_add(x, x);
+  if constexpr (NT > 64) {
+    __syncthreads();   // the values of the sum before have been read
+    if ((tid & 63) == 0) sm[tid >> 6] = x;
+    __syncthreads();
+    x = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) x += sm[i];
+  }
+  return x;
+}
+
+// Features c .. c + VEC - 1 of run i of a thread: runs of a row's threads lie side by side.
+template <int NT, int VEC>
+__device__ __forceinline__ int run_col(int tid, int i) {
+  return (i * NT + tid) * VEC;
+}
+
+template <int NT, int R, int VEC>
+__device__ __forceinline__ void load_weights(const float* w, int D, int tid, float none,
+                                             float (&x)[R][VEC]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int c = run_col<NT, VEC>(tid, i);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[i][e] = none;
+    if (w && c < D) {
+      const auto r = get_run<float, VEC>(w + c, D - c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[i][e] = r.v[e];
+    }
+  }
+}
+
+template <typename T, int NT, int R>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_fwd_kernel(
+    tops_gla_layer_norm_args a) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int PER = (NT > 256 ? NT : 256) / NT;
+  __shared__ float sm[8];
+  const int D = (int)a.D, tid = threadIdx.x % NT;
+  const T* x = (const T*)a.x;
+  T* y = (T*)a.y;
+  float w[R][VEC], b[R][VEC];
+  load_weights<NT, R, VEC>(a.w, D, tid, 1.f, w);
+  load_weights<NT, R, VEC>(a.b, D, tid, 0.f, b);
+  const long step = (long)gridDim.x * PER;
+  long row = (long)blockIdx.x * PER + threadIdx.x / NT;
+  Run<T, VEC> nx[R];
+  auto load = [&](long r) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+      if (c < D) nx[i] = get_run<T, VEC>(x + r * a.x_st + c, D - c);
+    }
+  };
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step) {
+    float v[R][VEC], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool in = run_col<NT, VEC>(tid, i) < D;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[i][e] = in ? to_f32(nx[i].v[e]) : 0.f;
+        s += v[i][e];
+      }
+    }
+    if (row + step < a.rows) load(row + step);
+    const float mean = row_sum<NT>(s, sm, tid) / (float)D;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[i][e] = c + e < D ? v[i][e] - mean : 0.f;
+        s = fmaf(v[i][e], v[i][e], s);
+      }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<NT>(s, sm, tid) / (float)D + (float)a.eps);
+    if (a.stats && tid == 0) {
+      a.stats[2 * row] = mean;
+      a.stats[2 * row + 1] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+      float r[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r[e] = fmaf(v[i][e] * rstd, w[i][e], b[i][e]);
+      if (c < D) put_run<T, VEC>(y + row * D + c, r, D - c);
+    }
+  }
+}
+
+template <typename T, int NT, int R>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
+    tops_gla_layer_norm_args a) {
+  constexpr int VEC = 16 / (int)sizeof(T), BT = NT > 256 ? NT : 256;
+  constexpr int PER = BT / NT;
+  __shared__ float sm[8];
+  __shared__ float part[PER > 1 ? 2 * R * VEC * NT : 1];
+  const int D = (int)a.D, tid = threadIdx.x % NT;
+  const T *x = (const T*)a.x, *dy = (const T*)a.dy;
+  T* dx = (T*)a.dx;
+  float w[R][VEC], dw[R][VEC], db[R][VEC];
+  load_weights<NT, R, VEC>(a.w, D, tid, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
+  const long step = (long)gridDim.x * PER;
+  long row = (long)blockIdx.x * PER + threadIdx.x / NT;
+  Run<T, VEC> nx[R], nd[R];
+  float mean = 0.f, rstd = 0.f;
+  auto load = [&](long r) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+      if (c < D) {
+        nx[i] = get_run<T, VEC>(x + r * a.x_st + c, D - c);
+        nd[i] = get_run<T, VEC>(dy + r * a.dy_st + c, D - c);
+      }
+    }
+    mean = a.stats[2 * r];
+    rstd = a.stats[2 * r + 1];
+  };
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step) {
+    float n[R][VEC], u[R][VEC], s = 0.f, sn = 0.f;
+    const float m = mean, rs = rstd;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const bool in = c + e < D;
+        n[i][e] = in ? (to_f32(nx[i].v[e]) - m) * rs : 0.f;
+        const float d = in ? to_f32(nd[i].v[e]) : 0.f;
+        db[i][e] += d;
+        dw[i][e] = fmaf(d, n[i][e], dw[i][e]);
+        u[i][e] = d * w[i][e];
+        s += u[i][e];
+        sn = fmaf(u[i][e], n[i][e], sn);
+      }
+    }
+    if (row + step < a.rows) load(row + step);
+    s = row_sum<NT>(s, sm, tid) / (float)D;
+    sn = row_sum<NT>(sn, sm, tid) / (float)D;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+      float r[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r[e] = rs * (u[i][e] - s - n[i][e] * sn);
+      if (c < D) put_run<T, VEC>(dx + row * D + c, r, D - c);
+    }
+  }
+  if (!a.ws) return;
+  float* out = (float*)a.ws + (long)blockIdx.x * 2 * D;
+  if constexpr (PER > 1) {   // the block's waves one after another, in their order
+    for (int p = 0; p < PER; ++p) {
+      if ((int)threadIdx.x / NT == p) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float* q = part + (i * VEC + e) * NT + tid;
+            q[0] = p ? q[0] + dw[i][e] : dw[i][e];
+            q[R * VEC * NT] = p ? q[R * VEC * NT] + db[i][e] : db[i][e];
+          }
+      }
+      __syncthreads();
+    }
+    if ((int)threadIdx.x < NT) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          dw[i][e] = part[(i * VEC + e) * NT + tid];
+          db[i][e] = part[(R * VEC + i * VEC + e) * NT + tid];
+        }
+    }
+  }
+  if ((int)threadIdx.x < NT) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = run_col<NT, VEC>(tid, i);
+      if (c < D) {
+        put_run<float, VEC>(out + c, dw[i], D - c);
+        put_run<float, VEC>(out + D + c, db[i], D - c);
+      }
+    }
+  }
+}
+
+// Sums `parts` rows of 2 D partial sums: 64 columns a block, its 16 waves a sixteenth of the rows
+// each.
+__global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* ws, int parts, int D,
+                                                              float* dw, float* db) {
+  __shared__ float sm[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < 2 * D)
+    for (int r = wave; r < parts; r += 16) s += ws[(long)r * 2 * D + c];
+  sm[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < 2 * D) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += sm[i][lane];
+    if (c < D) {
+      if (dw) dw[c] = s;
+    } else if (db) {
+      db[c - D] = s;
+    }
+  }
+}
+
+template <typename T, int NT, int R>
+void launch(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
+  const int nb = (int)norm_blocks(a.rows, a.D, backward), bt = NT > 256 ? NT : 256;
+  if (backward)
+    layer_norm_bwd_kernel<T, NT, R><<<nb, bt, 0, st>>>(a);
+  else
+    layer_norm_fwd_kernel<T, NT, R><<<nb, bt, 0, st>>>(a);
+}
+
+template <typename T>
+hipError_t run(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int nt = row_threads(a.D);
+  const long r = (a.D + (long)nt * VEC - 1) / ((long)nt * VEC);   // runs a thread
+  if (a.rows > 0) {
+    if (nt == 64) {
+      if (r <= 1) launch<T, 64, 1>(a, backward, st);
+      else if (r <= 2) launch<T, 64, 2>(a, backward, st);
+      else if (r <= 4) launch<T, 64, 4>(a, backward, st);
+      else if constexpr (VEC == 4) launch<T, 64, 8>(a, backward, st);
+    } else if (nt == 256) {
+      if (r <= 2) launch<T, 256, 2>(a, backward, st);
+      else if (r <= 4) launch<T, 256, 4>(a, backward, st);
+      else if constexpr (VEC == 4) launch<T, 256, 8>(a, backward, st);
+    } else {
+      if (r <= 4) launch<T, 512, 4>(a, backward, st);
+      else if constexpr (VEC == 4) launch<T, 512, 8>(a, backward, st);
+    }
+  }
+  if (backward && a.ws) {
+    const int parts = (int)norm_blocks(a.rows, a.D, true);
+    layer_norm_sum_kernel<<<(unsigned)((2 * a.D + 63) / 64), 1024, 0, st>>>(
+        (const float*)a.ws, parts, (int)a.D, a.dw, a.db);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+long layer_norm_part_rows(long rows, long D, int) { return norm_blocks(rows, D, true); }
+
+hipError_t run_layer_norm_fwd(const tops_gla_layer_norm_args& a, hipStream_t st) {
+  return a.dtype == DT_BF16 ? run<bf16>(a, false, st) : run<float>(a, false, st);
+}
+hipError_t run_layer_norm_bwd(const tops_gla_layer_norm_args& a, hipStream_t st) {
+  return a.dtype == DT_BF16 ? run<bf16>(a, true, st) : run<float>(a, true, st);
+}
+
+}  // namespace tops

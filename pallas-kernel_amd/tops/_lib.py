@@ -100,6 +100,19 @@ _SSM_SIGS = {
     "tops_gla_qk_norm_rope_ws_bytes": [_I64] * 2,
 }
 
+# the gated delta rule and the layer norm (include/tops_gla_delta.h), in the same form
+_DELTA_SIGS = {
+    "tops_gla_delta_fwd": [_S, _P],
+    "tops_gla_delta_bwd": [_S, _P],
+    "tops_gla_delta_chunk": [_I64],
+    "tops_gla_delta_keep_bytes": [_I64] * 6,
+    "tops_gla_delta_ws_bytes": [_I64] * 5,
+    "tops_gla_delta_step": [_S, _P],
+    "tops_gla_layer_norm_fwd": [_S, _P],
+    "tops_gla_layer_norm_bwd": [_S, _P],
+    "tops_gla_layer_norm_ws_bytes": [_I64] * 3,
+}
+
 # entry points that do not return a status code
 _RESTYPE = {"tops_gla_chunk_ws_bytes": ctypes.c_int64, "tops_gla_kernel_ms": ctypes.c_float,
             "tops_gla_rmsnorm_ws_bytes": ctypes.c_int64,
@@ -108,7 +121,11 @@ _RESTYPE = {"tops_gla_chunk_ws_bytes": ctypes.c_int64, "tops_gla_kernel_ms": cty
             "tops_gla_selective_scan_piece": ctypes.c_int64,
             "tops_gla_selective_scan_chunk": ctypes.c_int64,
             "tops_gla_causal_conv_bwd_ws_bytes": ctypes.c_int64,
-            "tops_gla_qk_norm_rope_ws_bytes": ctypes.c_int64}
+            "tops_gla_qk_norm_rope_ws_bytes": ctypes.c_int64,
+            "tops_gla_delta_chunk": ctypes.c_int64,
+            "tops_gla_delta_keep_bytes": ctypes.c_int64,
+            "tops_gla_delta_ws_bytes": ctypes.c_int64,
+            "tops_gla_layer_norm_ws_bytes": ctypes.c_int64}
 
 EXPORTED = ["tops_gla_last_error", "tops_gla_version"] + list(_SIGS)
 
@@ -146,7 +163,8 @@ def load():
             lib.tops_gla_last_error.argtypes = []
             lib.tops_gla_version.restype = ctypes.c_char_p
             lib.tops_gla_version.argtypes = []
-            for name, args in (*_SIGS.items(), *_LAYER_SIGS.items(), *_SSM_SIGS.items()):
+            for name, args in (*_SIGS.items(), *_LAYER_SIGS.items(), *_SSM_SIGS.items(),
+                               *_DELTA_SIGS.items()):
                 fn = getattr(lib, name)
                 fn.argtypes = args
                 fn.restype = _RESTYPE.get(name, ctypes.c_int)
@@ -170,6 +188,16 @@ def call(name, *args):
         if rc == 2:
             raise NotImplementedError(f"{name}: {msg}")
         raise RuntimeError(f"{name}: {msg}")
+
+
+def call_on(device, name, packed):
+    """``call`` of an entry point that takes one packed struct, on a device's current stream, which
+    need not be the current device's (the default stream's address is the same for all)."""
+    if torch.cuda.current_device() == device.index:
+        call(name, packed, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, packed, stream_of(device))
 
 
 def full_head(K, V, chunk, dtype, backward):
