@@ -80,8 +80,8 @@ inline int delta_chunk_of(int dtype) { return dtype == DT_BF16 ? 64 : 32; }
 inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 
 // Per chunk and value head ("unit"): vectors over the chunk's tokens, [5][C] float and [C] double:
-//   e^{G_i}, e^{G_C - G_i}, beta, 1 / |k| (1 without l2norm), scale / |q|, and G, the sum of the
-//   log decays up to a token (in 64 bits: differences of it go into exponentials);
+//   e^{G_i}, e^{G_C - G_i}, beta, 1 / |k|, 1 / |q| (1 without l2norm), and G, the sum of the log
+//   decays up to a token (in 64 bits: differences of it go into exponentials);
 // then, as tiles in the operands' type (two of them, high and low part, where it is bfloat16)
 //   Tm [C][C] the inverse of 1 + tril(beta k k^T decay), P [C][C] the masked scores,
 // and  N [V][C] the written values,  S [V][KP] the state before the chunk.
@@ -243,6 +243,30 @@ __device__ __forceinline__ Frag<float> ld_pair_t(const float* M, int P, int lane
   f.a = make_float4(p[0], p[P], p[2 * P], p[3 * P]);
   f.b = make_float4(p[4 * P], p[5 * P], p[6 * P], p[7 * P]);
   return f;
+}
+// Split fragments of a tile in LDS whose low part lies `lo` elements behind its high part.
+template <typename T>
+__device__ __forceinline__ Split<T> ld_split(const T* tile, int lo, int off);
+template <>
+__device__ __forceinline__ Split<float> ld_split<float>(const float* tile, int, int off) {
+  return {ld_frag(tile + off)};
+}
+template <>
+__device__ __forceinline__ Split<bf16> ld_split<bf16>(const bf16* tile, int lo, int off) {
+  return {ld_frag(tile + off), ld_frag(tile + lo + off)};
+}
+
+template <typename T>
+__device__ __forceinline__ Split<T> ld_split_t(const T* tile, int lo, int P, int lane, int h);
+template <>
+__device__ __forceinline__ Split<float> ld_split_t<float>(const float* tile, int, int P, int lane,
+                                                          int h) {
+  return {ld_pair_t(tile, P, lane, h)};
+}
+template <>
+__device__ __forceinline__ Split<bf16> ld_split_t<bf16>(const bf16* tile, int lo, int P, int lane,
+                                                        int h) {
+  return {ld_pair_t(tile, P, lane, h), ld_pair_t(tile + lo, P, lane, h)};
 }
 // The 8 values of a lane in a pair of accumulators.
 __device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, float (&x)[8]) {

@@ -186,17 +186,6 @@ struct ScanLds {
   static constexpr int BYTES = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // of one of two buffers
 };
 
-template <typename T>
-__device__ __forceinline__ Split<T> ld_split(const T* tile, int lo, int off);
-template <>
-__device__ __forceinline__ Split<float> ld_split<float>(const float* tile, int, int off) {
-  return {ld_frag(tile + off)};
-}
-template <>
-__device__ __forceinline__ Split<bf16> ld_split<bf16>(const bf16* tile, int lo, int off) {
-  return {ld_frag(tile + off), ld_frag(tile + lo + off)};
-}
-
 template <typename T, int KP, int NW>
 __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   using L = ScanLds<T, KP, NW>;
@@ -399,8 +388,8 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams
   }
   qq = swap32_add(qq, qq);
   qq = swap16_add(qq, qq);
-  const float fq = (float)a.scale * (a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f);
-  if (a.train && lane < 16) vec[4 * C + i] = fq;
+  const float rq = a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f, fq = (float)a.scale * rq;
+  if (a.train && lane < 16) vec[4 * C + i] = rq;
   const float fo = fq * vec[i];
   const double gi = sG[i];
   Frag<T> pf[NU];
