@@ -30,7 +30,7 @@ extern "C" {
  * chunks of all sequences.
  * `keep` (tops_gla_delta_keep_bytes, 256-byte aligned) is the forward's workspace; with `train` it
  * also holds what the backward reads.
- * 1 <= K <= 256, 1 <= V <= 65536, batch * T < 2^31 - 64.
+ * 8 <= K <= 256, 8 <= V <= 65536, batch * T < 2^31 - 64.
  */
 typedef struct tops_gla_delta_args {
   const void *q, *k;              /* [B, T, H, K] */
@@ -70,7 +70,7 @@ int64_t tops_gla_delta_ws_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V
  * The next T tokens of each row b, its state at state[slot_b] ([slots, HV, K, V], updated in
  * place): slot_b = slots_idx[b] (int32 or int64, idx64) or b. A slot outside [0, slots) leaves
  * every state as it is and gives o = 0; no slot may be given twice, and slots are at least their
- * size apart (state_ss). K <= 256.
+ * size apart (state_ss). 1 <= K <= 256, 1 <= V <= 65536.
  */
 typedef struct tops_gla_delta_step_args {
   float *state;

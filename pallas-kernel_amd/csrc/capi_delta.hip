@@ -62,6 +62,9 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
   if (a == nullptr) return fail(TOPS_GLA_EINVAL, "NULL arguments");
   if (int rc = types(a->dtype, a->g_dtype, a->beta_dtype)) return rc;
   if (int rc = head_sizes(a->H, a->HV, a->K, a->V)) return rc;
+  if (a->K < 8 || a->V < 8)   // rows are read 8 columns at a time
+    return fail(TOPS_GLA_EUNSUPPORTED, "K and V must be at least 8 (K=%lld, V=%lld)",
+                (long long)a->K, (long long)a->V);
   if (a->batch < 0 || a->T < 0 || a->nseq < 0 || a->chunks < 0)
     return fail(TOPS_GLA_EINVAL, "bad batch, T, nseq or chunks");
   if (a->T > kMax || a->batch > kMax || a->batch * a->T >= kMaxTokens)

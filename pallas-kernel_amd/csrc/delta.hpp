@@ -50,6 +50,34 @@ __device__ __forceinline__ void put_run(T* p, const float (&x)[N], int n = N) {
   }
 }
 
+// The 8 elements from column c on, zeros from `cols` on, of the 8 that were loaded from
+// min(c, cols - 8).
+__device__ __forceinline__ Run<bf16, 8> cut_run(const Run<bf16, 8>& r, int c, int cols) {
+  uint4 x = __builtin_bit_cast(uint4, r);
+  if (cols % 8) {   // the same for all lanes
+    const int s = max(0, min(c - (cols - 8), 8));
+    if (s & 4) x = make_uint4(x.z, x.w, 0, 0);
+    if (s & 2) x = make_uint4(x.y, x.z, x.w, 0);
+    if (s & 1)
+      x = make_uint4(x.x >> 16 | x.y << 16, x.y >> 16 | x.z << 16, x.z >> 16 | x.w << 16,
+                     x.w >> 16);
+  }
+  return __builtin_bit_cast(Run<bf16, 8>, mask16(x, c < cols ? ~0u : 0u));
+}
+__device__ __forceinline__ Run<float, 8> cut_run(const Run<float, 8>& r, int c, int cols) {
+  Run<float, 8> x = r;
+  if (cols % 8) {
+    const int s = max(0, min(c - (cols - 8), 8));
+#pragma unroll
+    for (int b = 4; b > 0; b >>= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.v[e] = s & b ? (e + b < 8 ? x.v[e + b] : 0.f) : x.v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x.v[e] = c < cols ? x.v[e] : 0.f;
+  return x;
+}
+
 // Element i of a tensor of either type.
 __device__ __forceinline__ float get_any(const void* p, int dtype, long i) {
   return dtype == DT_BF16 ? to_f32(((const bf16*)p)[i]) : ((const float*)p)[i];
@@ -86,7 +114,7 @@ inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 //   Tm [C][C] the inverse of 1 + tril(beta k k^T decay), P [C][C] the masked scores,
 // and  N [V][C] the written values,  S [V][KP] the state before the chunk.
 struct DeltaParams {
-  tops_gla_delta_args a;
+  tops_gla_delta_args a;   // 8 <= K, 8 <= V
   int C, KP, parts;   // tokens of a chunk, padded keys, parts of a split tile (2 or 1)
   char *vec, *Tm, *P, *N, *S;   // in keep
   char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
@@ -274,27 +302,31 @@ __device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, floa
   for (int r = 0; r < 4; ++r) x[r] = a[r], x[4 + r] = b[r];
 }
 
-// A [C][w] tile on its way to LDS, w a multiple of 8: pieces of 8 elements, zeros past `len` rows
-// and `cols` columns.
+// A [C][W] tile on its way to LDS in pieces of 8 elements. The loads have no conditions, so that
+// they are all on their way at once: a piece past the tile's rows or columns loads one inside.
+// `put` zeroes what is past `len` rows and `cols` columns. Fewer than 8 columns may be left of rows
+// that hold 8 at least: the load then begins before them.
 template <typename T, int C, int W, int NT>
 struct TileFetch {
   static constexpr int PER = C * W / 8, N = (PER + NT - 1) / NT;
   Run<T, 8> r[N];
   __device__ __forceinline__ void get(const T* src, long st, int len, int cols, int tid) {
-    const bool whole = cols % 8 == 0;   // the same for all: pieces end where the columns do
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int p = i * NT + tid, row = p / (W / 8), col = p % (W / 8) * 8;
-      r[i] = Run<T, 8>{};
-      if ((PER % NT == 0 || p < PER) && row < len && col < cols) {
-        if (whole)
-          r[i] = get_run<T, 8>(src + row * st + col);
-        else
-          r[i] = get_run<T, 8>(src + row * st + col, cols - col);
-      }
+      const int p = i * NT + tid;
+      r[i] = get_run<T, 8>(src + min(p / (W / 8), len - 1) * st + min(p % (W / 8) * 8, cols - 8));
     }
   }
-  __device__ __forceinline__ void put(T* dst, int pitch, int tid) const {
+  __device__ __forceinline__ void mask(int len, int cols, int tid) {
+    if (len >= C && cols >= W && PER % NT == 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * NT + tid, row = p / (W / 8);
+      r[i] = row < len ? cut_run(r[i], p % (W / 8) * 8, cols) : Run<T, 8>{};
+    }
+  }
+  __device__ __forceinline__ void put(T* dst, int pitch, int len, int cols, int tid) {
+    mask(len, cols, tid);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int p = i * NT + tid;

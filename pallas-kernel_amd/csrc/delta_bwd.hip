@@ -62,6 +62,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   const int nc = (T_ + C - 1) / C;
   const T* kp = (const T*)a.k + b * a.k_sb + t0 * a.k_st + h * a.k_sh;
   const T* qp = (const T*)a.q + b * a.q_sb + t0 * a.q_st + h * a.q_sh;
+  const int vc = V - vb * 16 * NW;
   const T* dp = (const T*)a.dout + b * a.do_sb + t0 * a.do_st + hv * a.do_sh + vb * 16 * NW;
   const int v = vb * 16 * NW + 16 * wave + ci;
   const bool vin = v < V;
@@ -69,19 +70,29 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   f32x4 S[2 * NS];   // dS, as the forward's states
   const long st0 = ((long)seq * HV + hv) * K * V + v;
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i)
+  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
+  if (a.dht) {
+    const float* s0 = a.dht + st0 - v + min(v, V - 1);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-      S[i][r] = a.dht && vin && k < K ? a.dht[st0 + (long)k * V] : 0.f;
-    }
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
+        S[i][r] = s0[(long)min(k, K - 1) * V];
+      }
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!vin || 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
+  }
 
   TileFetch<T, C, KP, NT> fk, fq;
   TileFetch<T, L::PARTS * C, C, NT> ft;
   TileFetch<T, C, C, NT> fp[L::PARTS];
   TileFetch<T, C, 16 * NW, NT> fd;
   constexpr int NF = (3 * C + NT) / NT;
-  float ff[NF];
+  float ff[NF], fr[NF];
   auto fetch = [&](int n) {
     const int len = min(C, T_ - n * C);
     const long unit = (long)(c0 + n) * HV + hv;
@@ -91,19 +102,14 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < L::PARTS; ++i)   // rows past the end have not been written
       fp[i].get((const T*)(p.P + unit * (C * C * 4)) + i * C * C, C, len, C, tid);
-    fd.get(dp + (long)n * C * a.do_st, a.do_st, len, V - vb * 16 * NW, tid);
+    fd.get(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
     for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|
       const int x = i * NT + tid, t = x % C;
-      if (x < C)
-        ff[i] = vec[C + t] * vec[3 * C + t];
-      else if (x < 2 * C)
-        ff[i] = vec[2 * C + t] * vec[t] * vec[3 * C + t];
-      else if (x < 3 * C)
-        ff[i] = (float)a.scale * vec[t] * vec[4 * C + t];
-      else if (x == 3 * C)
-        ff[i] = vec[C - 1];
+      const float e = vec[t + (x < C ? C : 0)], n = vec[t + (x < 2 * C ? 3 * C : 4 * C)];
+      ff[i] = x < 3 * C ? e * n : vec[C - 1];
+      fr[i] = x < C ? 1.f : x < 2 * C ? vec[2 * C + t] : x < 3 * C ? (float)a.scale : 1.f;
     }
   };
   T* sm = (T*)smem;
@@ -112,15 +118,16 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   if (nc > 0) fetch(nc - 1);
   for (int n = nc - 1; n >= 0; --n) {
     __syncthreads();
-    fk.put(sK, L::PK, tid);
-    fq.put(sQ, L::PK, tid);
-    ft.put(sT, L::PT, tid);
+    const int len = min(C, T_ - n * C);
+    fk.put(sK, L::PK, len, K, tid);
+    fq.put(sQ, L::PK, len, K, tid);
+    ft.put(sT, L::PT, L::PARTS * C, C, tid);
 #pragma unroll
-    for (int i = 0; i < L::PARTS; ++i) fp[i].put(sP + i * LO, L::PT, tid);
-    fd.put(sV, L::PV, tid);
+    for (int i = 0; i < L::PARTS; ++i) fp[i].put(sP + i * LO, L::PT, len, C, tid);
+    fd.put(sV, L::PV, len, vc, tid);
 #pragma unroll
     for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i];
+      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i] * fr[i];
     __syncthreads();
     if (n > 0) fetch(n - 1);
     const long unit = (long)(c0 + n) * HV + hv;
@@ -267,9 +274,9 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   {
     TileFetch<T, C, KP, NT> f;
     f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
-    f.put(sK, L::PK, tid);
+    f.put(sK, L::PK, at.len, K, tid);
     f.get((const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh, a.q_st, at.len, K, tid);
-    f.put(sQ, L::PK, tid);
+    f.put(sQ, L::PK, at.len, K, tid);
   }
   const T *kr = sK + i * L::PK, *qr = sQ + i * L::PK;
   const float scale = (float)a.scale;
@@ -284,18 +291,21 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     const int hv = h * group + gi;
     const long unit = (long)chunk * HV + hv;
     const long tok = (long)at.b * a.T + at.t + i;
-    const T* vp = (const T*)a.v + at.b * a.v_sb + (at.t + (long)i) * a.v_st + hv * a.v_sh;
+    const T* vp = (const T*)a.v + at.b * a.v_sb + (at.t + (long)min(i, at.len - 1)) * a.v_st +
+                  hv * a.v_sh;
     const T* dop = (const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh;
     T* dvp = (T*)a.dv + (tok * HV + hv) * V;
     TileFetch<T, VS, C, NT> fn, fy;
     TileFetch<T, VS, KP, NT> fs, fd;
     TileFetch<T, C, VS, NT> fo;
+    Run<T, 8> fv;
     auto fetch = [&](int v0) {
       fn.get((const T*)p.N + (unit * V + v0) * C, C, V - v0, C, tid);
       fy.get((const T*)p.Y + (unit * V + v0) * C, C, V - v0, C, tid);
       fs.get((const T*)p.S + (unit * V + v0) * KP, KP, V - v0, KP, tid);
       fd.get((const T*)p.dS + (unit * V + v0) * KP, KP, V - v0, KP, tid);
       fo.get(dop + v0, a.do_st, at.len, V - v0, tid);
+      fv = get_run<T, 8>(vp + min(v0 + 8 * g, V - 8));
     };
     fetch(0);
     if (GROUP) __syncthreads();   // the vectors of the head before have been read
@@ -313,32 +323,33 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     float beta = 0.f;
     for (int v0 = 0; v0 < V; v0 += VS) {
       __syncthreads();
-      fn.put(sN, L::PC, tid);
-      fy.put(sY, L::PC, tid);
-      fs.put(sS, L::PK, tid);
-      fd.put(sD, L::PK, tid);
-      fo.put(sO, L::PS, tid);
+      fn.put(sN, L::PC, V - v0, C, tid);
+      fy.put(sY, L::PC, V - v0, C, tid);
+      fs.put(sS, L::PK, V - v0, KP, tid);
+      fd.put(sD, L::PK, V - v0, KP, tid);
+      fo.put(sO, L::PS, at.len, V - v0, tid);
 #pragma unroll
       for (int x = 0; x < decltype(fs)::N; ++x)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sd = fmaf(to_f32(fs.r[x].v[e]), to_f32(fd.r[x].v[e]), sd);
       __syncthreads();
+      const Run<T, 8> vr = fv;
       if (v0 + VS < V) fetch(v0 + VS);
       if (v0 == 0) beta = sf[2 * C + i];
       const Frag<T> of = ld_frag(sO + i * L::PS + 8 * g);
       const Frag<T> yf = ld_frag_t(sY + 16 * wave, L::PC, lane);
       const Frag<T> nf = ld_frag_t(sN + 16 * wave, L::PC, lane);
       const int c = v0 + 8 * g;
-      if (in && c < V) {   // dv, and v . Y
+      {   // dv, and v . Y (Y is 0 past the end)
         float y[8], x[8];
         values_of(yf, y);
-        values_of(frag_of<T>(get_run<T, 8>(vp + c, V - c)), x);
+        values_of(frag_of<T>(cut_run(vr, c, V)), x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          vy = fmaf(x[e], y[e], vy);
+          vy = in ? fmaf(x[e], y[e], vy) : 0.f;
           y[e] *= beta;
         }
-        put_run<T, 8>(dvp + c, y, V - c);
+        if (in && c < V) put_run<T, 8>(dvp + c, y, V - c);
       }
 #pragma unroll
       for (int x = 0; x < 2 * NU; ++x) {

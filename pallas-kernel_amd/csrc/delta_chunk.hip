@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
   {
     TileFetch<T, C, KP, 256> f;
     f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
-    f.put(sK, PK, tid);
+    f.put(sK, PK, at.len, K, tid);
   }
   __syncthreads();
   {   // 1 / |k|: 256 / C threads a row
@@ -211,6 +211,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   }
   const int nc = (T_ + C - 1) / C;
   const T* kp = (const T*)a.k + b * a.k_sb + t0 * a.k_st + h * a.k_sh;
+  // the block's columns; the last block's few may begin before them, where there are fewer than 8
+  const int vc = V - vb * 16 * NW;
   const T* vp = (const T*)a.v + b * a.v_sb + t0 * a.v_st + hv * a.v_sh + vb * 16 * NW;
   const int v = vb * 16 * NW + 16 * wave + ci;
   const bool vin = v < V;
@@ -219,43 +221,52 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   f32x4 S[2 * NS];
   const long st0 = ((long)seq * HV + hv) * K * V + v;
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i)
+  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
+  if (a.h0) {
+    const float* s0 = a.h0 + st0 - v + min(v, V - 1);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-      S[i][r] = a.h0 && vin && k < K ? a.h0[st0 + (long)k * V] : 0.f;
-    }
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
+        S[i][r] = s0[(long)min(k, K - 1) * V];
+      }
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!vin || 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
+  }
 
   TileFetch<T, C, KP, NT> fk;
   TileFetch<T, L::PARTS * C, C, NT> ft;
   TileFetch<T, C, 16 * NW, NT> fv;
   constexpr int NF = (3 * C + NT) / NT;
-  float ff[NF];
+  float ff[NF], fr[NF];
   auto fetch = [&](int n) {
     const int len = min(C, T_ - n * C);
     const long unit = (long)(c0 + n) * HV + hv;
     fk.get(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
     ft.get((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
-    fv.get(vp + (long)n * C * a.v_st, a.v_st, len, V - vb * 16 * NW, tid);
+    fv.get(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta
+    for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta, e^{G_C}
       const int x = i * NT + tid;
-      if (x < 2 * C)
-        ff[i] = vec[x] * vec[3 * C + x % C];
-      else if (x <= 3 * C)
-        ff[i] = vec[x < 3 * C ? x : C - 1];
+      ff[i] = vec[x < 3 * C ? x : C - 1];
+      fr[i] = vec[3 * C + x % C];
     }
   };
   auto put = [&](int n) {
     T* sm = (T*)(smem + (n & 1) * L::BYTES);
-    fk.put(sm + L::K0, L::PK, tid);
-    ft.put(sm + L::T0, L::PT, tid);
-    fv.put(sm + L::V0, L::PV, tid);
+    const int len = min(C, T_ - n * C);
+    fk.put(sm + L::K0, L::PK, len, K, tid);
+    ft.put(sm + L::T0, L::PT, L::PARTS * C, C, tid);
+    fv.put(sm + L::V0, L::PV, len, vc, tid);
     float* sf = (float*)(smem + (n & 1) * L::BYTES + L::F0);
 #pragma unroll
     for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i];
+      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = i * NT + tid < 2 * C ? ff[i] * fr[i] : ff[i];
   };
   if (nc > 0) {
     fetch(0);
@@ -346,9 +357,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 // 8 elements of row `r` of q or k from column c on, zeros past K.
 template <typename T>
 __device__ __forceinline__ Frag<T> ld_row(const T* base, long st, int r, int c, int K) {
-  if (c >= K) return frag_of<T>(Run<T, 8>{});
-  if (K % 8 == 0) return frag_of<T>(get_run<T, 8>(base + r * st + c));
-  return frag_of<T>(get_run<T, 8>(base + r * st + c, K - c));
+  return frag_of<T>(cut_run(get_run<T, 8>(base + r * st + min(c, K - 8)), c, K));
 }
 
 // A wave has 16 tokens of a chunk as columns: scores (rows: the tokens before them), then outputs

@@ -50,28 +50,46 @@ __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_arg
   }
   float* S = a.state + slot * a.state_ss + (long)hv * K * V + (long)r0 * V + c0;
   float s[KR][4];
+  if (V % 4 == 0) {   // loads without conditions, all on their way at once: from inside, past the end
+    const float* S0 = S - r0 * (long)V - c0 + min(c0, V - 4);
 #pragma unroll
-  for (int r = 0; r < KR; ++r) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
-    if (r < nr && nc > 0) {
-      const auto x = get_run<float, 4>(S + (long)r * V, nc);
+    for (int r = 0; r < KR; ++r) {
+      const auto x = get_run<float, 4>(S0 + (long)min(r0 + r, K - 1) * V);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[r][e] = x.v[e];
     }
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+      if (r >= nr || nc <= 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][e] = 0.f;
+  } else {
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[r][e] = r < nr && e < nc ? S[(long)r * V + e] : 0.f;
   }
   const T* q = (const T*)a.q + b * a.q_sb + h * a.q_sh + r0;
   const T* k = (const T*)a.k + b * a.k_sb + h * a.k_sh + r0;
   const T* v = (const T*)a.v + b * a.v_sb + hv * a.v_sh + c0;
   const long g0 = b * a.g_sb + hv, b0 = b * a.beta_sb + hv;
+  const bool whole = K == 16 * KR && V % 16 == 0;   // no lane of a wave is past the end
   for (int t = 0; t < T_; ++t) {
-    Run<T, KR> qr = {}, kr = {};
-    if (nr > 0) {
-      qr = get_run<T, KR>(q + t * a.q_st, nr);
-      kr = get_run<T, KR>(k + t * a.k_st, nr);
+    Run<T, KR> qr, kr;
+    Run<T, 4> vr;
+    if (whole) {
+      qr = get_run<T, KR>(q + t * a.q_st);
+      kr = get_run<T, KR>(k + t * a.k_st);
+      vr = get_run<T, 4>(v + t * a.v_st);
+    } else {
+#pragma unroll
+      for (int r = 0; r < KR; ++r) {
+        qr.v[r] = r < nr ? q[t * a.q_st + r] : zero_elem<T>();
+        kr.v[r] = r < nr ? k[t * a.k_st + r] : zero_elem<T>();
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vr.v[e] = e < nc ? v[t * a.v_st + e] : zero_elem<T>();
     }
-    Run<T, 4> vr = {};
-    if (nc > 0) vr = get_run<T, 4>(v + t * a.v_st, nc);
     const float ge = expf(get_any(a.g, (int)a.g_dtype, g0 + t * a.g_st));
     const float beta = get_any(a.beta, (int)a.beta_dtype, b0 + t * a.beta_st);
     float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f}, qk = 0.f, qq = 0.f, kk = 0.f;

@@ -51,6 +51,18 @@ __device__ __forceinline__ int run_col(int tid, int i) {
   return (i * NT + tid) * VEC;
 }
 
+// The VEC features from c on of a row of D, zeros past its end. Where VEC divides D the load has no
+// condition (a run past the end loads the last one), so that a row's loads are all on their way at
+// once; the caller leaves such a run out.
+template <typename T, int VEC>
+__device__ __forceinline__ Run<T, VEC> load_run(const T* row, int c, int D) {
+  if (D % VEC == 0) return get_run<T, VEC>(row + min(c, D - VEC));
+  Run<T, VEC> r;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) r.v[e] = c + e < D ? row[c + e] : zero_elem<T>();
+  return r;
+}
+
 template <int NT, int R, int VEC>
 __device__ __forceinline__ void load_weights(const float* w, int D, int tid, float none,
                                              float (&x)[R][VEC]) {
@@ -59,10 +71,10 @@ __device__ __forceinline__ void load_weights(const float* w, int D, int tid, flo
     const int c = run_col<NT, VEC>(tid, i);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) x[i][e] = none;
-    if (w && c < D) {
-      const auto r = get_run<float, VEC>(w + c, D - c);
+    if (w) {
+      const auto r = load_run<float, VEC>(w, c, D);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[i][e] = r.v[e];
+      for (int e = 0; e < VEC; ++e) x[i][e] = c + e < D ? r.v[e] : 0.f;
     }
   }
 }
@@ -85,8 +97,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_fwd_kernel(
   auto load = [&](long r) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int c = run_col<NT, VEC>(tid, i);
-      if (c < D) nx[i] = get_run<T, VEC>(x + r * a.x_st + c, D - c);
+      nx[i] = load_run<T, VEC>(x + r * a.x_st, run_col<NT, VEC>(tid, i), D);
     }
   };
   if (row < a.rows) load(row);
@@ -153,10 +164,8 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int c = run_col<NT, VEC>(tid, i);
-      if (c < D) {
-        nx[i] = get_run<T, VEC>(x + r * a.x_st + c, D - c);
-        nd[i] = get_run<T, VEC>(dy + r * a.dy_st + c, D - c);
-      }
+      nx[i] = load_run<T, VEC>(x + r * a.x_st, c, D);
+      nd[i] = load_run<T, VEC>(dy + r * a.dy_st, c, D);
     }
     mean = a.stats[2 * r];
     rstd = a.stats[2 * r + 1];

@@ -5,6 +5,7 @@ from __future__ import annotations
 import struct
 
 import torch
+import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -169,6 +170,13 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
     if initial_state is not None and initial_state.shape != (S, HV, K, V):
         require(False, f"initial_state must be {(S, HV, K, V)}, got {tuple(initial_state.shape)}")
     scale = K ** -0.5 if scale is None else float(scale)
+    if K < 8 or V < 8:   # the kernels read 8 columns at a time: zeros beside them change nothing
+        pk, pv = max(0, 8 - K), max(0, 8 - V)
+        o, ht = gated_delta_rule(
+            F.pad(q, (0, pk)), F.pad(k, (0, pk)), F.pad(v, (0, pv)), g, beta, scale,
+            None if initial_state is None else F.pad(initial_state, (0, pv, 0, pk)),
+            output_final_state, cu, qk_l2norm)
+        return o[..., :V], None if ht is None else ht[..., :K, :V]
     args = (q, k, v, g, beta, initial_state)
     if differentiable(*args):
         return _GatedDeltaRuleFunction.apply(*args, scale, bool(qk_l2norm),
