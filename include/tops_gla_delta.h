@@ -30,7 +30,8 @@ extern "C" {
  * chunks of all sequences.
  * `keep` (tops_gla_delta_keep_bytes, 256-byte aligned) is the forward's workspace; with `train` it
  * also holds what the backward reads.
- * 8 <= K <= 256, 8 <= V <= 65536, batch * T < 2^31 - 64.
+ * 8 <= K <= 256, 8 <= V <= 65536, batch * T < 2^31 - 64, tokens of q, k, v and dout less than 2^24
+ * elements apart.
  */
 typedef struct tops_gla_delta_args {
   const void *q, *k;              /* [B, T, H, K] */

@@ -83,6 +83,11 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
       !grid_fits((a->V + 31) / 32 * a->HV, 256) ||
       !grid_fits((a->V + 31) / 32 * a->HV * a->nseq, 256))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
+  // offsets within a chunk are 32 bits of bytes
+  for (int64_t st : {a->q_st, a->k_st, a->v_st, backward ? a->do_st : 0})
+    if (st >= (1 << 24) || st <= -(1 << 24))
+      return fail(TOPS_GLA_EUNSUPPORTED, "tokens must lie less than 2^24 elements apart (%lld)",
+                  (long long)st);
   if (a->chunks > 0 && any_null({a->q, a->k, a->v, a->g, a->beta}))
     return fail(TOPS_GLA_EINVAL, "q, k, v, g and beta must not be NULL");
   if (!backward && a->chunks > 0 && a->o == nullptr)

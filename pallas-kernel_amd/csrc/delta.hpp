@@ -305,17 +305,20 @@ __device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, floa
 // A [C][W] tile on its way to LDS in pieces of 8 elements. The loads have no conditions, so that
 // they are all on their way at once: a piece past the tile's rows or columns loads one inside.
 // `put` zeroes what is past `len` rows and `cols` columns. Fewer than 8 columns may be left of rows
-// that hold 8 at least: the load then begins before them.
+// that hold 8 at least: the load then begins before them. Offsets are 32 bits of bytes from a base
+// that is the same for all lanes (rows lie less than 2^24 elements apart).
 template <typename T, int C, int W, int NT>
 struct TileFetch {
   static constexpr int PER = C * W / 8, N = (PER + NT - 1) / NT;
   Run<T, 8> r[N];
+  __device__ __forceinline__ static int offset(int i, int st, int len, int cols, int tid) {
+    const int p = i * NT + tid;
+    return (min(p / (W / 8), len - 1) * st + min(p % (W / 8) * 8, cols - 8)) * (int)sizeof(T);
+  }
   __device__ __forceinline__ void get(const T* src, long st, int len, int cols, int tid) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int p = i * NT + tid;
-      r[i] = get_run<T, 8>(src + min(p / (W / 8), len - 1) * st + min(p % (W / 8) * 8, cols - 8));
-    }
+    for (int i = 0; i < N; ++i)
+      r[i] = get_run<T, 8>((const T*)((const char*)src + offset(i, (int)st, len, cols, tid)));
   }
   __device__ __forceinline__ void mask(int len, int cols, int tid) {
     if (len >= C && cols >= W && PER % NT == 0) return;
@@ -335,5 +338,110 @@ struct TileFetch {
     }
   }
 };
+// The same for tile after tile of one source: the offsets of whole tiles stay in registers.
+template <typename T, int C, int W, int NT>
+struct TileStream : TileFetch<T, C, W, NT> {
+  using Base = TileFetch<T, C, W, NT>;
+  int off[Base::N];
+  __device__ __forceinline__ TileStream(long st, int cols, int tid) {
+#pragma unroll
+    for (int i = 0; i < Base::N; ++i) off[i] = Base::offset(i, (int)st, C, cols, tid);
+  }
+  __device__ __forceinline__ void next(const T* src, long st, int len, int cols, int tid) {
+    if (len < C) {   // a sequence's last tile
+      Base::get(src, st, len, cols, tid);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < Base::N; ++i)
+      Base::r[i] = get_run<T, 8>((const T*)((const char*)src + off[i]));
+  }
+};
+
+// acc[i] += A(i) B for N tiles of rows, part after part of a split operand, so that a product does
+// not wait for the one before it.
+template <int N, typename F>
+__device__ __forceinline__ void mma_rows(f32x4* acc, const F& rows, const Split<float>& b) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma(acc[i], rows(i), b.f);
+}
+template <int N, typename F>
+__device__ __forceinline__ void mma_rows(f32x4* acc, const F& rows, const Split<bf16>& b) {
+  Frag<bf16> a[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = rows(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma(acc[i], a[i], b.lo);
+#pragma unroll
+  for (int i = 0; i < N; ++i) mma(acc[i], a[i], b.hi);
+}
+
+__device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }
+__device__ __forceinline__ Frag<bf16> high_of(const Split<bf16>& s) { return s.hi; }
+
+// A wave's rows of a state, from row k on in steps of 32: row k + 32 s + 4 h + r in S[2 s + h][r];
+// `at` is its column in row 0, which is inside also where the lane's own is not.
+template <int NS>
+__device__ __forceinline__ void load_state(f32x4 (&S)[2 * NS], const float* from, long at,
+                                           bool inside, int k, int K, int V) {
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
+  if (!from) return;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      S[i][r] = from[at + (long)min(k + 32 * (i >> 1) + 4 * (i & 1) + r, K - 1) * V];
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (!inside || k + 32 * (i >> 1) + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
+}
+template <int NS>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[2 * NS], float* to, long at,
+                                            bool inside, int k, int K, int V) {
+  if (!to || !inside) return;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = k + 32 * (i >> 1) + 4 * (i & 1) + r;
+      if (row < K) to[at + (long)row * V] = S[i][r];
+    }
+}
+
+// The waves of the launches that go from chunk to chunk: NW lots of 16 columns a block, and KW
+// waves for each, which share the rows of its state (KP / KW each). Those hand one another their
+// shares of the products with the state through LDS and do the triangular system alike.
+// Few columns in all want many waves for each, as one chunk's chain of products is what counts;
+// many want few, as the system is then solved once.
+struct DeltaWaves {
+  int nw, kw;
+};
+inline DeltaWaves delta_waves(const tops_gla_delta_args& a, int KP) {
+  const long lots = (a.V + 15) / 16 * a.HV * a.nseq;
+  if (lots <= 512) return {1, KP == 64 ? 2 : 4};
+  if (lots <= 1024) return {2, 2};
+  return {4, 1};
+}
+
+// Sums tiles over the KW waves of a lot, in the same order for each. `x`: N * 64 quads for each
+// wave of the block.
+template <int N, int KW, int NW>
+__device__ __forceinline__ void share_sum(f32x4 (&acc)[N], f32x4* x, int wave, int lane) {
+  if constexpr (KW > 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[(wave * N + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    const int c = wave % NW;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      acc[i] = x[(c * N + i) * 64 + lane];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) acc[i] += x[((c + k * NW) * N + i) * 64 + lane];
+    }
+  }
+}
 
 }  // namespace tops

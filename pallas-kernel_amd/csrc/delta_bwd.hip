@@ -26,23 +26,25 @@ namespace {
 // The states' gradients
 // ---------------------------------------------------------------------------
 
-template <typename T, int KP, int NW>
+template <typename T, int KP, int NW, int KW>
 struct DscanLds {
   static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1;
   static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(16 * NW);
   static constexpr int K0 = 0, Q0 = C * PK, T0 = 2 * C * PK, P0 = T0 + PARTS * C * PT;
   static constexpr int V0 = P0 + PARTS * C * PT, END = V0 + C * PV;
   static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
-  static constexpr int BYTES = F0 + (3 * C + 1) * 4;
+  static constexpr int X0 = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // shares of the waves
+  static constexpr int BYTES = X0 + (KW > 1 ? NW * KW * (C / 16) * 1024 : 0);
 };
 
-template <typename T, int KP, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
-  using L = DscanLds<T, KP, NW>;
-  constexpr int C = L::C, NT = 64 * NW, NS = KP / 32, NU = C / 32, LO = C * L::PT;
+template <typename T, int KP, int NW, int KW>
+__global__ __launch_bounds__(64 * NW * KW) void delta_dscan_kernel(DeltaParams p) {
+  using L = DscanLds<T, KP, NW, KW>;
+  constexpr int C = L::C, NT = 64 * NW * KW, NS = KP / 32 / KW, NU = C / 32, LO = C * L::PT;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cw = wave % NW, kw = wave / NW, k0 = kw * (KP / KW);
   const int g = lane >> 4, ci = lane & 15;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + 16 * NW - 1) / (16 * NW);
@@ -64,51 +66,35 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   const T* qp = (const T*)a.q + b * a.q_sb + t0 * a.q_st + h * a.q_sh;
   const int vc = V - vb * 16 * NW;
   const T* dp = (const T*)a.dout + b * a.do_sb + t0 * a.do_st + hv * a.do_sh + vb * 16 * NW;
-  const int v = vb * 16 * NW + 16 * wave + ci;
+  const int v = vb * 16 * NW + 16 * cw + ci;
   const bool vin = v < V;
 
   f32x4 S[2 * NS];   // dS, as the forward's states
   const long st0 = ((long)seq * HV + hv) * K * V + v;
-#pragma unroll
-  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
-  if (a.dht) {
-    const float* s0 = a.dht + st0 - v + min(v, V - 1);
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-        S[i][r] = s0[(long)min(k, K - 1) * V];
-      }
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (!vin || 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
-  }
+  load_state<NS>(S, a.dht, st0 - v + min(v, V - 1), vin, k0 + 8 * g, K, V);
 
-  TileFetch<T, C, KP, NT> fk, fq;
-  TileFetch<T, L::PARTS * C, C, NT> ft;
-  TileFetch<T, C, C, NT> fp[L::PARTS];
-  TileFetch<T, C, 16 * NW, NT> fd;
+  TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
+  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
+  TileStream<T, C, C, NT> fp[2] = {{C, C, tid}, {C, C, tid}};
+  TileStream<T, C, 16 * NW, NT> fd(a.do_st, vc, tid);
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
   auto fetch = [&](int n) {
     const int len = min(C, T_ - n * C);
     const long unit = (long)(c0 + n) * HV + hv;
-    fk.get(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    fq.get(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
-    ft.get((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
+    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
+    fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
+    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
 #pragma unroll
     for (int i = 0; i < L::PARTS; ++i)   // rows past the end have not been written
-      fp[i].get((const T*)(p.P + unit * (C * C * 4)) + i * C * C, C, len, C, tid);
-    fd.get(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
+      fp[i].next((const T*)(p.P + unit * (C * C * 4)) + i * C * C, C, len, C, tid);
+    fd.next(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
     for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|
       const int x = i * NT + tid, t = x % C;
-      const float e = vec[t + (x < C ? C : 0)], n = vec[t + (x < 2 * C ? 3 * C : 4 * C)];
-      ff[i] = x < 3 * C ? e * n : vec[C - 1];
+      const float e = vec[t + (x < C ? C : 0)], r = vec[t + (x < 2 * C ? 3 * C : 4 * C)];
+      ff[i] = x < 3 * C ? e * r : vec[C - 1];
       fr[i] = x < C ? 1.f : x < 2 * C ? vec[2 * C + t] : x < 3 * C ? (float)a.scale : 1.f;
     }
   };
@@ -136,25 +122,20 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     f32x4 acc[2 * NU];
 #pragma unroll
     for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-    T* So = (T*)p.dS + (unit * V + v) * KP + 8 * g;
+    T* So = (T*)p.dS + (unit * V + v) * KP + k0 + 8 * g;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Split<T> f = split_of<T>(x);
-      if constexpr (sizeof(T) == 2) {
-        if (vin) st_frag(So + 32 * s, f.hi);
-      } else {
-        if (vin) st_frag(So + 32 * s, f.f);
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        mma(acc[i], ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g),
-            f);
+      if (vin) st_frag(So + 32 * s, high_of(f));
+      mma_rows<2 * NU>(acc, [&](int i) {
+        return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + k0 + 32 * s + 8 * g);
+      }, f);
     }
     Frag<T> df[NU];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) df[u] = ld_frag_t(sV + 16 * wave + 32 * u * L::PV, L::PV, lane);
+    for (int u = 0; u < NU; ++u) df[u] = ld_frag_t(sV + 16 * cw + 32 * u * L::PV, L::PV, lane);
 #pragma unroll
     for (int i = 0; i < 2 * NU; ++i)
 #pragma unroll
@@ -163,9 +144,10 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     for (int w = 0; w < NU; ++w)
 #pragma unroll
       for (int i = 0; i < 2 * NU; ++i)
-        if (w >= (i >> 1))
+        if (w >= (i >> 1) && i % KW == kw)
           mma(acc[i], ld_split_t<T>(sP + 32 * w * L::PT + 32 * (i >> 1), LO, L::PT, lane, i & 1),
               df[w]);
+    share_sum<2 * NU, KW, NW>(acc, (f32x4*)(smem + L::X0), wave, lane);
     Split<T> R[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -191,29 +173,19 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       values_of(df[u], x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= sf[2 * C + 32 * u + 8 * g + e];
-      const Split<T> fo = split_of<T>(x);
+      mma_rows<2 * NS>(S, [&](int i) {
+        return ld_pair_t(sQ + k0 + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
+      }, split_of<T>(x));
       pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (vin) st_frag(Yo + 32 * u, frag_of<T>(x));
+      if (vin && kw == u % KW) st_frag(Yo + 32 * u, frag_of<T>(x));
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
-      const Split<T> fy = split_of<T>(x);
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) {
-        const int off = 32 * u * L::PK + 32 * (i >> 1);
-        mma(S[i], ld_pair_t(sQ + off, L::PK, lane, i & 1), fo);
-        mma(S[i], ld_pair_t(sK + off, L::PK, lane, i & 1), fy);
-      }
+      mma_rows<2 * NS>(S, [&](int i) {
+        return ld_pair_t(sK + k0 + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
+      }, split_of<T>(x));
     }
   }
-  if (a.dh0 && vin) {
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-        if (k < K) a.dh0[st0 + (long)k * V] = S[i][r];
-      }
-  }
+  store_state<NS>(S, a.dh0, st0, vin, k0 + 8 * g, K, V);
 }
 
 // ---------------------------------------------------------------------------
@@ -498,19 +470,14 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   }
 }
 
-int dscan_waves(const DeltaParams& p) {
-  const long w = (p.a.V + 15) / 16 * p.a.HV * p.a.nseq;
-  return p.a.V <= 32 || w <= 512 ? 2 : 4;
-}
-
-template <typename T, int KP, int NW>
+template <typename T, int KP, int NW, int KW>
 hipError_t launch_dscan(const DeltaParams& p, hipStream_t st) {
-  constexpr int lds = DscanLds<T, KP, NW>::BYTES;
-  const hipError_t e = hipFuncSetAttribute((const void*)delta_dscan_kernel<T, KP, NW>,
+  constexpr int lds = DscanLds<T, KP, NW, KW>::BYTES;
+  const hipError_t e = hipFuncSetAttribute((const void*)delta_dscan_kernel<T, KP, NW, KW>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   const long grid = (p.a.V + 16 * NW - 1) / (16 * NW) * p.a.HV * p.a.nseq;
-  delta_dscan_kernel<T, KP, NW><<<(unsigned)grid, 64 * NW, lds, st>>>(p);
+  delta_dscan_kernel<T, KP, NW, KW><<<(unsigned)grid, 64 * NW * KW, lds, st>>>(p);
   return hipGetLastError();
 }
 
@@ -528,8 +495,10 @@ hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
 template <typename T, int KP>
 hipError_t run(const DeltaParams& p, hipStream_t st) {
   if (p.a.nseq > 0) {
-    const hipError_t e = dscan_waves(p) == 2 ? launch_dscan<T, KP, 2>(p, st)
-                                             : launch_dscan<T, KP, 4>(p, st);
+    const DeltaWaves w = delta_waves(p.a, KP);
+    const hipError_t e = w.nw == 1   ? launch_dscan<T, KP, 1, KP == 64 ? 2 : 4>(p, st)
+                         : w.nw == 2 ? launch_dscan<T, KP, 2, 2>(p, st)
+                                     : launch_dscan<T, KP, 4, 1>(p, st);
     if (e != hipSuccess) return e;
   }
   if (p.a.chunks == 0) return hipSuccess;

@@ -162,12 +162,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = sT[row * PA + col + e];
       const Split<T> s = split_of<T>(x);
-      if constexpr (sizeof(T) == 2) {
-        st_frag(out + row * C + col, s.hi);
-        st_frag(out + C * C + row * C + col, s.lo);
-      } else {
-        st_frag(out + row * C + col, s.f);
-      }
+      st_frag(out + row * C + col, high_of(s));
+      if constexpr (sizeof(T) == 2) st_frag(out + C * C + row * C + col, s.lo);
     }
     __syncthreads();
   }
@@ -177,22 +173,25 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
 // The states
 // ---------------------------------------------------------------------------
 
-template <typename T, int KP, int NW>
+template <typename T, int KP, int NW, int KW>
 struct ScanLds {
   static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1;
   static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(16 * NW);
   static constexpr int K0 = 0, T0 = C * PK, V0 = T0 + PARTS * C * PT, END = V0 + C * PV;
-  static constexpr int F0 = END * (int)sizeof(T);                // three vectors of floats, e^{G_C}
-  static constexpr int BYTES = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // of one of two buffers
+  static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
+  static constexpr int ONE = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // one of two buffers
+  static constexpr int X0 = 2 * ONE;                                  // shares of the waves
+  static constexpr int BYTES = X0 + (KW > 1 ? NW * KW * (C / 16) * 1024 : 0);
 };
 
-template <typename T, int KP, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
-  using L = ScanLds<T, KP, NW>;
-  constexpr int C = L::C, NT = 64 * NW, NS = KP / 32, NU = C / 32;
+template <typename T, int KP, int NW, int KW>
+__global__ __launch_bounds__(64 * NW * KW) void delta_scan_kernel(DeltaParams p) {
+  using L = ScanLds<T, KP, NW, KW>;
+  constexpr int C = L::C, NT = 64 * NW * KW, NS = KP / 32 / KW, NU = C / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cw = wave % NW, k0 = wave / NW * (KP / KW);   // its 16 columns, its rows of the state
   const int g = lane >> 4, ci = lane & 15;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + 16 * NW - 1) / (16 * NW);
@@ -214,41 +213,25 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   // the block's columns; the last block's few may begin before them, where there are fewer than 8
   const int vc = V - vb * 16 * NW;
   const T* vp = (const T*)a.v + b * a.v_sb + t0 * a.v_st + hv * a.v_sh + vb * 16 * NW;
-  const int v = vb * 16 * NW + 16 * wave + ci;
+  const int v = vb * 16 * NW + 16 * cw + ci;
   const bool vin = v < V;
 
-  // K row 32 s + 8 g + 4 h + r of the state in S[2 s + h][r]
+  // row k0 + 32 s + 8 g + 4 h + r of the state in S[2 s + h][r]
   f32x4 S[2 * NS];
   const long st0 = ((long)seq * HV + hv) * K * V + v;
-#pragma unroll
-  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
-  if (a.h0) {
-    const float* s0 = a.h0 + st0 - v + min(v, V - 1);
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-        S[i][r] = s0[(long)min(k, K - 1) * V];
-      }
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (!vin || 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
-  }
+  load_state<NS>(S, a.h0, st0 - v + min(v, V - 1), vin, k0 + 8 * g, K, V);
 
-  TileFetch<T, C, KP, NT> fk;
-  TileFetch<T, L::PARTS * C, C, NT> ft;
-  TileFetch<T, C, 16 * NW, NT> fv;
+  TileStream<T, C, KP, NT> fk(a.k_st, K, tid);
+  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
+  TileStream<T, C, 16 * NW, NT> fv(a.v_st, vc, tid);
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
   auto fetch = [&](int n) {
     const int len = min(C, T_ - n * C);
     const long unit = (long)(c0 + n) * HV + hv;
-    fk.get(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    ft.get((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
-    fv.get(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
+    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
+    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
+    fv.next(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
     for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta, e^{G_C}
@@ -258,12 +241,12 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     }
   };
   auto put = [&](int n) {
-    T* sm = (T*)(smem + (n & 1) * L::BYTES);
+    T* sm = (T*)(smem + (n & 1) * L::ONE);
     const int len = min(C, T_ - n * C);
     fk.put(sm + L::K0, L::PK, len, K, tid);
     ft.put(sm + L::T0, L::PT, L::PARTS * C, C, tid);
     fv.put(sm + L::V0, L::PV, len, vc, tid);
-    float* sf = (float*)(smem + (n & 1) * L::BYTES + L::F0);
+    float* sf = (float*)(smem + (n & 1) * L::ONE + L::F0);
 #pragma unroll
     for (int i = 0; i < NF; ++i)
       if (i * NT + tid <= 3 * C) sf[i * NT + tid] = i * NT + tid < 2 * C ? ff[i] * fr[i] : ff[i];
@@ -275,31 +258,27 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   for (int n = 0; n < nc; ++n) {
     __syncthreads();
     if (n + 1 < nc) fetch(n + 1);
-    const T* sm = (const T*)(smem + (n & 1) * L::BYTES);
-    const T *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + 16 * wave;
-    const float* sf = (const float*)(smem + (n & 1) * L::BYTES + L::F0);
+    const T* sm = (const T*)(smem + (n & 1) * L::ONE);
+    const T *sK = sm + L::K0 + k0, *sT = sm + L::T0, *sV = sm + L::V0 + 16 * cw;
+    const float* sf = (const float*)(smem + (n & 1) * L::ONE + L::F0);
     const long unit = (long)(c0 + n) * HV + hv;
     const float last = sf[3 * C];
 
     f32x4 acc[2 * NU];
 #pragma unroll
     for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-    T* So = (T*)p.S + (unit * V + v) * KP + 8 * g;
+    T* So = (T*)p.S + (unit * V + v) * KP + k0 + 8 * g;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Split<T> f = split_of<T>(x);
-      if constexpr (sizeof(T) == 2) {
-        if (vin) st_frag(So + 32 * s, f.hi);
-      } else {
-        if (vin) st_frag(So + 32 * s, f.f);
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        mma(acc[i], ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g),
-            f);
+      if (vin) st_frag(So + 32 * s, high_of(f));
+      mma_rows<2 * NU>(acc, [&](int i) {
+        return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
+      }, f);
     }
+    share_sum<2 * NU, KW, NW>(acc, (f32x4*)(smem + L::X0), wave, lane);
     Split<T> R[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -329,25 +308,16 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     for (int u = 0; u < NU; ++u) {
       float x[8];
       pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (vin) st_frag(No + 32 * u, frag_of<T>(x));
+      if (vin && wave / NW == u % KW) st_frag(No + 32 * u, frag_of<T>(x));
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
-      const Split<T> f = split_of<T>(x);
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i)
-        mma(S[i], ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1), f);
+      mma_rows<2 * NS>(S, [&](int i) {
+        return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
+      }, split_of<T>(x));
     }
     if (n + 1 < nc) put(n + 1);
   }
-  if (a.ht && vin) {
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-        if (k < K) a.ht[st0 + (long)k * V] = S[i][r];
-      }
-  }
+  store_state<NS>(S, a.ht, st0, vin, k0 + 8 * g, K, V);
 }
 
 // ---------------------------------------------------------------------------
@@ -401,7 +371,7 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams
   if (a.train && lane < 16) vec[4 * C + i] = rq;
   const float fo = fq * vec[i];
   const double gi = sG[i];
-  Frag<T> pf[NU];
+  Split<T> pf[NU];   // in two parts: of the three operands of o this one is free to be exact
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
     if (32 * u > 16 * wave + 15) continue;
@@ -419,17 +389,11 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams
       const int j = 32 * u + 8 * g + e;
       x[e] = j <= i ? fq * sRk[j] * x[e] * gexp<T>((float)(gi - sG[j])) : 0.f;
     }
-    const Split<T> sp = split_of<T>(x);
+    pf[u] = split_of<T>(x);
     T* out = (T*)(p.P + unit * (C * C * 4)) + i * C + 32 * u + 8 * g;
-    if constexpr (sizeof(T) == 2) {
-      pf[u] = sp.hi;
-      if (a.train) {
-        st_frag(out, sp.hi);
-        st_frag(out + C * C, sp.lo);
-      }
-    } else {
-      pf[u] = sp.f;
-      if (a.train) st_frag(out, sp.f);
+    if (a.train) {
+      st_frag(out, high_of(pf[u]));
+      if constexpr (sizeof(T) == 2) st_frag(out + C * C, pf[u].lo);
     }
   }
   T* o = (T*)a.o + (((long)at.b * a.T + at.t + i) * HV + hv) * V;
@@ -458,20 +422,14 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams
   }
 }
 
-// Waves of a block of the states' launch, 16 columns each: they share the chunk's tiles in LDS.
-int scan_waves(const DeltaParams& p) {
-  const long w = (p.a.V + 15) / 16 * p.a.HV * p.a.nseq;
-  return p.a.V <= 32 || w <= 512 ? 2 : 4;
-}
-
-template <typename T, int KP, int NW>
+template <typename T, int KP, int NW, int KW>
 hipError_t launch_scan(const DeltaParams& p, hipStream_t st) {
-  constexpr int lds = 2 * ScanLds<T, KP, NW>::BYTES;
-  const hipError_t e = hipFuncSetAttribute((const void*)delta_scan_kernel<T, KP, NW>,
+  constexpr int lds = ScanLds<T, KP, NW, KW>::BYTES;
+  const hipError_t e = hipFuncSetAttribute((const void*)delta_scan_kernel<T, KP, NW, KW>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   const long grid = (p.a.V + 16 * NW - 1) / (16 * NW) * p.a.HV * p.a.nseq;
-  delta_scan_kernel<T, KP, NW><<<(unsigned)grid, 64 * NW, lds, st>>>(p);
+  delta_scan_kernel<T, KP, NW, KW><<<(unsigned)grid, 64 * NW * KW, lds, st>>>(p);
   return hipGetLastError();
 }
 
@@ -483,8 +441,10 @@ hipError_t run(const DeltaParams& p, hipStream_t st) {
     if (const hipError_t e = hipGetLastError()) return e;
   }
   if (a.nseq > 0) {
-    const hipError_t e = scan_waves(p) == 2 ? launch_scan<T, KP, 2>(p, st)
-                                            : launch_scan<T, KP, 4>(p, st);
+    const DeltaWaves w = delta_waves(a, KP);
+    const hipError_t e = w.nw == 1   ? launch_scan<T, KP, 1, KP == 64 ? 2 : 4>(p, st)
+                         : w.nw == 2 ? launch_scan<T, KP, 2, 2>(p, st)
+                                     : launch_scan<T, KP, 4, 1>(p, st);
     if (e != hipSuccess) return e;
   }
   if (a.chunks > 0)

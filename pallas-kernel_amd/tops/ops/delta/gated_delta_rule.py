@@ -26,6 +26,12 @@ def _gate(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _tokens(t, dt):
+    """``rows`` of [B, T, heads, columns]; the kernels step from token to token in 32 bits."""
+    t = rows(t, dt)
+    return t if -(1 << 24) < t.stride(1) < 1 << 24 else t.contiguous()
+
+
 class _Chunks:
     """The chunks that a call's sequences are cut into."""
 
@@ -61,7 +67,7 @@ def _forward(q, k, v, g, beta, h0, scale, norm, want, cu, train):
     dt = io_dtype(q, k, v)
     B, T, H, K = q.shape
     HV, V = v.shape[2:]
-    x = rows(q, dt), rows(k, dt), rows(v, dt), _gate(g), _gate(beta)
+    x = _tokens(q, dt), _tokens(k, dt), _tokens(v, dt), _gate(g), _gate(beta)
     h0 = f32(h0)
     ch = _Chunks(B, T, cu, dt, dev)
     o = torch.empty(B, T, HV, V, dtype=dt, device=dev)
@@ -91,7 +97,7 @@ class _GatedDeltaRuleFunction(torch.autograd.Function):
         dev, dt, ch = q.device, q.dtype, ctx.ch
         B, T, H, K = q.shape
         HV, V = v.shape[2:]
-        do = torch.zeros(B, T, HV, V, dtype=dt, device=dev) if do is None else rows(do, dt)
+        do = torch.zeros(B, T, HV, V, dtype=dt, device=dev) if do is None else _tokens(do, dt)
         dht = f32(dht)
         new = torch.empty
         dq, dk = new(B, T, H, K, dtype=dt, device=dev), new(B, T, H, K, dtype=dt, device=dev)
