@@ -24,12 +24,14 @@ extern "C" {
  *   S' = e^{g_t} S_{t-1},  n_t = beta_t (v_t - S'^T k_t),  S_t = S' + k_t n_t^T,
  *   o_t = scale S_t^T q_t.
  * With `l2norm` q_t and k_t stand for q_t / sqrt(|q_t|^2 + 1e-6) and the same of k_t.
- * Sequences are cut into chunks of tops_gla_delta_chunk(dtype) tokens: fixed length (`seqs` NULL:
- * batch sequences of T tokens) or packed (batch == 1), with `seqs` a device int32 table of nseq + 1
- * token offsets (from 0 to T, not decreasing) and nseq + 1 chunk offsets; `chunks` is the number of
- * chunks of all sequences.
- * `keep` (tops_gla_delta_keep_bytes, 256-byte aligned) is the forward's workspace; with `train` it
- * also holds what the backward reads.
+ * Sequences are cut into chunks of tops_gla_delta_chunk(dtype) tokens, and these into segments of
+ * `seg_chunks` chunks (the last of a sequence may be shorter; a sequence without tokens has one
+ * segment), which run in parallel; tops_gla_delta_segment says how many. `chunks` and `nsegs` are
+ * those of all sequences. Fixed length (`seqs` NULL): batch sequences of T tokens. Packed (batch ==
+ * 1): `seqs` is a device int32 table of nseq + 1 token offsets (from 0 to T, not decreasing), nseq +
+ * 1 chunk offsets, nseq + 1 segment offsets, and the sequence of each segment.
+ * `keep` (tops_gla_delta_bytes, 256-byte aligned) is the forward's workspace; with `train` it also
+ * holds what the backward reads.
  * 8 <= K <= 256, 8 <= V <= 65536, batch * T < 2^31 - 64, tokens of q, k, v and dout less than 2^24
  * elements apart.
  */
@@ -43,7 +45,7 @@ typedef struct tops_gla_delta_args {
   const int32_t *seqs;
   void *keep;
   int64_t keep_bytes;
-  int64_t nseq, chunks, batch, T, H, HV, K, V;
+  int64_t nseq, chunks, nsegs, seg_chunks, batch, T, H, HV, K, V;
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
   int64_t g_sb, g_st, beta_sb, beta_st;
   int64_t l2norm, train, dtype, g_dtype, beta_dtype;
@@ -55,17 +57,21 @@ typedef struct tops_gla_delta_args {
   void *dq, *dk, *dv;
   void *dg, *dbeta;               /* of g's and beta's types */
   float *dh0;                     /* [sequences, HV, K, V] or NULL */
-  void *ws;                       /* tops_gla_delta_ws_bytes, 256-byte aligned */
+  void *ws;                       /* tops_gla_delta_bytes, 256-byte aligned */
   int64_t ws_bytes;
 } tops_gla_delta_args;
 int tops_gla_delta_fwd(const tops_gla_delta_args *a, void *stream);
 /* The gradients; keep as a forward with `train` left it. */
 int tops_gla_delta_bwd(const tops_gla_delta_args *a, void *stream);
-/* Tokens of a chunk (0 for a type that is refused), bytes of `keep` and of `ws`. */
+/* Tokens of a chunk (0 for a type that is refused). */
 int64_t tops_gla_delta_chunk(int64_t dtype);
-int64_t tops_gla_delta_keep_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype,
-                                  int64_t train);
-int64_t tops_gla_delta_ws_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype);
+/* Chunks of a segment that fill the device, for nseq sequences of `chunks` chunks in all. */
+int64_t tops_gla_delta_segment(int64_t nseq, int64_t chunks, int64_t HV, int64_t V);
+/* Bytes of `keep`, or with `backward` of `ws` (0 for sizes that are refused). */
+typedef struct tops_gla_delta_sizes {
+  int64_t nseq, chunks, nsegs, HV, K, V, dtype, train;
+} tops_gla_delta_sizes;
+int64_t tops_gla_delta_bytes(const tops_gla_delta_sizes *z, int64_t backward);
 
 /*
  * The next T tokens of each row b, its state at state[slot_b] ([slots, HV, K, V], updated in

@@ -69,19 +69,24 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
     return fail(TOPS_GLA_EINVAL, "bad batch, T, nseq or chunks");
   if (a->T > kMax || a->batch > kMax || a->batch * a->T >= kMaxTokens)
     return fail(TOPS_GLA_EUNSUPPORTED, "B*T exceeds 2^31 - 64 tokens");
+  if (a->seg_chunks < 1 || a->seg_chunks > kMax / 64)
+    return fail(TOPS_GLA_EINVAL, "bad seg_chunks");
   const int64_t C = tops::delta_chunk_of((int)a->dtype), per = (a->T + C - 1) / C;
   if (a->seqs == nullptr) {
-    if (a->nseq != a->batch || a->chunks != a->batch * per)
-      return fail(TOPS_GLA_EINVAL, "nseq must be the batch, chunks its chunks");
+    const int64_t segs = std::max<int64_t>(1, (per + a->seg_chunks - 1) / a->seg_chunks);
+    if (a->nseq != a->batch || a->chunks != a->batch * per || a->nsegs != a->batch * segs)
+      return fail(TOPS_GLA_EINVAL, "nseq must be the batch, chunks and nsegs its own");
   } else {
     if (a->batch != 1) return fail(TOPS_GLA_EINVAL, "packed sequences require batch == 1");
-    if (a->nseq > kMax / 2 || a->chunks < per || a->chunks > per + a->nseq)
-      return fail(TOPS_GLA_EINVAL, "bad nseq or chunks");
+    if (a->nseq > kMax / 4 || a->chunks < per || a->chunks > per + a->nseq ||
+        a->nsegs < a->nseq || a->nsegs > a->chunks + a->nseq)
+      return fail(TOPS_GLA_EINVAL, "bad nseq, chunks or nsegs");
   }
   // the blocks of the largest launches, of 256 threads or fewer
   if (!grid_fits(a->chunks, 1) || !grid_fits(a->chunks * a->HV, 256) ||
-      !grid_fits((a->V + 31) / 32 * a->HV, 256) ||
-      !grid_fits((a->V + 31) / 32 * a->HV * a->nseq, 256))
+      !grid_fits((a->V / 64 + 5) * a->HV, 256) ||
+      !grid_fits((a->V / 64 + 5) * a->HV * a->nsegs, 256) ||
+      !grid_fits((a->V / 16 + 1) * a->HV * a->nseq, 64))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   // offsets within a chunk are 32 bits of bytes
   for (int64_t st : {a->q_st, a->k_st, a->v_st, backward ? a->do_st : 0})
@@ -92,13 +97,14 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
     return fail(TOPS_GLA_EINVAL, "q, k, v, g and beta must not be NULL");
   if (!backward && a->chunks > 0 && a->o == nullptr)
     return fail(TOPS_GLA_EINVAL, "o must not be NULL");
-  *p = tops::delta_layout(a->chunks, a->HV, a->K, a->V, (int)a->dtype, a->train || backward,
-                          a->keep, a->ws);
+  *p = tops::delta_layout({a->nseq, a->chunks, a->nsegs, a->HV, a->K, a->V, a->dtype,
+                           a->train || backward}, a->keep, a->ws);
   if (p->keep_bytes > 0 &&
       (a->keep == nullptr || a->keep_bytes < p->keep_bytes || !aligned(a->keep)))
     return fail(TOPS_GLA_EINVAL, "keep must hold %lld bytes, 256-byte aligned",
                 (long long)p->keep_bytes);
   p->a = *a;
+  p->a.train = a->train || backward;
   if (!backward) return TOPS_GLA_OK;
   if (a->chunks > 0 && any_null({a->dout, a->dq, a->dk, a->dv, a->dg, a->dbeta}))
     return fail(TOPS_GLA_EINVAL, "dout, dq, dk, dv, dg and dbeta must not be NULL");
@@ -118,9 +124,18 @@ int norm_check(const tops_gla_layer_norm_args* a) {
   return TOPS_GLA_OK;
 }
 
-bool sizes_ok(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype) {
-  return chunks >= 0 && chunks <= kMax && HV >= 1 && HV <= 65536 && K >= 1 && K <= 256 && V >= 1 &&
-         V <= 65536 && dtype_ok(dtype) && chunks * HV <= kMax;
+// The launches of a call, one after another.
+hipError_t run_fwd(const tops::DeltaParams& p, hipStream_t st) {
+  if (p.a.chunks > 0)
+    if (const hipError_t e = tops::run_delta_prep(p, st)) return e;
+  if (p.a.nseq > 0)
+    if (const hipError_t e = tops::run_delta_scan(p, false, st)) return e;
+  return p.a.chunks > 0 ? tops::run_delta_out(p, st) : hipSuccess;
+}
+hipError_t run_bwd(const tops::DeltaParams& p, hipStream_t st) {
+  if (p.a.nseq > 0)
+    if (const hipError_t e = tops::run_delta_scan(p, true, st)) return e;
+  return p.a.chunks > 0 ? tops::run_delta_grad(p, st) : hipSuccess;
 }
 
 }  // namespace
@@ -131,27 +146,38 @@ int64_t tops_gla_delta_chunk(int64_t dtype) {
   return dtype_ok(dtype) ? tops::delta_chunk_of((int)dtype) : 0;
 }
 
-int64_t tops_gla_delta_keep_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype,
-                                  int64_t train) {
-  if (!sizes_ok(chunks, HV, K, V, dtype)) return 0;
-  return tops::delta_layout(chunks, HV, K, V, (int)dtype, train != 0, nullptr, nullptr).keep_bytes;
+int64_t tops_gla_delta_segment(int64_t nseq, int64_t chunks, int64_t HV, int64_t V) {
+  if (nseq < 1 || chunks < 1 || HV < 1 || V < 1) return 1 << 20;
+  // a block for each CU of the second pass; a first pass costs twice that, so that two or three
+  // segments of a sequence gain nothing
+  const int64_t blocks = (V + 127) / 128 * HV * nseq, per = (chunks + nseq - 1) / nseq;
+  const int64_t segs = std::min<int64_t>(256 / std::max<int64_t>(1, blocks), per / 4);
+  return segs < 4 ? 1 << 20 : std::min<int64_t>((per + segs - 1) / segs, 1 << 20);
 }
 
-int64_t tops_gla_delta_ws_bytes(int64_t chunks, int64_t HV, int64_t K, int64_t V, int64_t dtype) {
-  if (!sizes_ok(chunks, HV, K, V, dtype)) return 0;
-  return tops::delta_layout(chunks, HV, K, V, (int)dtype, true, nullptr, nullptr).ws_bytes;
+int64_t tops_gla_delta_bytes(const tops_gla_delta_sizes* z, int64_t backward) {
+  if (z == nullptr) {
+    fail(TOPS_GLA_EINVAL, "NULL arguments");
+    return 0;
+  }
+  if (z->nseq < 0 || z->chunks < 0 || z->chunks > kMax || z->nsegs < z->nseq || z->nsegs > kMax ||
+      z->HV < 1 || z->HV > 65536 || z->K < 1 || z->K > 256 || z->V < 1 || z->V > 65536 ||
+      !dtype_ok(z->dtype) || z->chunks * z->HV > kMax || z->nsegs * z->HV > kMax)
+    return 0;
+  const tops::DeltaParams p = tops::delta_layout(*z, nullptr, nullptr);
+  return backward ? p.ws_bytes : p.keep_bytes;
 }
 
 int tops_gla_delta_fwd(const tops_gla_delta_args* a, void* stream) {
   tops::DeltaParams p;
   if (int rc = delta_setup(a, false, &p)) return rc;
-  return done(tops::run_delta_fwd(p, (hipStream_t)stream), "delta_fwd");
+  return done(run_fwd(p, (hipStream_t)stream), "delta_fwd");
 }
 
 int tops_gla_delta_bwd(const tops_gla_delta_args* a, void* stream) {
   tops::DeltaParams p;
   if (int rc = delta_setup(a, true, &p)) return rc;
-  return done(tops::run_delta_bwd(p, (hipStream_t)stream), "delta_bwd");
+  return done(run_bwd(p, (hipStream_t)stream), "delta_bwd");
 }
 
 int tops_gla_delta_step(const tops_gla_delta_step_args* a, void* stream) {

@@ -119,13 +119,20 @@ struct DeltaParams {
   char *vec, *Tm, *P, *N, *S;   // in keep
   char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
                                 // right side
+  // where a sequence has several segments, for each of all segments and value heads: the state
+  // after it [K][V] (E) or the gradient of the state before it (dE), float32, and what it makes of
+  // a state before it, [KP][KP] in two layouts (M row-major, Mt column-major), tiles as Tm's
+  float *E, *dE;
+  char *M, *Mt;
+  int multi;
   long vec_bytes, keep_bytes, ws_bytes;
 };
 // The layout for given sizes; pointers from base addresses that may be NULL.
-DeltaParams delta_layout(int64_t chunks, int64_t HV, int64_t K, int64_t V, int dtype, bool train,
-                         void* keep, void* ws);
-hipError_t run_delta_fwd(const DeltaParams& p, hipStream_t st);
-hipError_t run_delta_bwd(const DeltaParams& p, hipStream_t st);
+DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws);
+hipError_t run_delta_prep(const DeltaParams& p, hipStream_t st);
+hipError_t run_delta_scan(const DeltaParams& p, bool backward, hipStream_t st);
+hipError_t run_delta_out(const DeltaParams& p, hipStream_t st);
+hipError_t run_delta_grad(const DeltaParams& p, hipStream_t st);
 
 struct ChunkAt {
   int b, t, len;   // batch row, first token in it, tokens
@@ -358,90 +365,93 @@ struct TileStream : TileFetch<T, C, W, NT> {
   }
 };
 
-// acc[i] += A(i) B for N tiles of rows, part after part of a split operand, so that a product does
-// not wait for the one before it.
-template <int N, typename F>
-__device__ __forceinline__ void mma_rows(f32x4* acc, const F& rows, const Split<float>& b) {
+// acc[c][i] += A(i) B[c] for N tiles of rows and CW of columns, part after part of a split operand,
+// so that a product does not wait for the one before it.
+template <int N, int CW, typename F>
+__device__ __forceinline__ void mma_rows(f32x4 (&acc)[CW][N], const F& rows,
+                                         const Split<float> (&b)[CW]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) mma(acc[i], rows(i), b.f);
+  for (int i = 0; i < N; ++i) {
+    const Frag<float> a = rows(i);
+#pragma unroll
+    for (int c = 0; c < CW; ++c) mma(acc[c][i], a, b[c].f);
+  }
 }
-template <int N, typename F>
-__device__ __forceinline__ void mma_rows(f32x4* acc, const F& rows, const Split<bf16>& b) {
-  Frag<bf16> a[N];
+template <int N, int CW, typename F>
+__device__ __forceinline__ void mma_rows(f32x4 (&acc)[CW][N], const F& rows,
+                                         const Split<bf16> (&b)[CW]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) a[i] = rows(i);
+  for (int i = 0; i < N; i += 2) {
+    const Frag<bf16> a[2] = {rows(i), rows(i + 1)};
 #pragma unroll
-  for (int i = 0; i < N; ++i) mma(acc[i], a[i], b.lo);
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-  for (int i = 0; i < N; ++i) mma(acc[i], a[i], b.hi);
+      for (int c = 0; c < CW; ++c) mma(acc[c][i + x], a[x], b[c].lo);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int c = 0; c < CW; ++c) mma(acc[c][i + x], a[x], b[c].hi);
+  }
+}
+// The same with the rows in two parts too; `use(i)` says which tiles have a part in the product.
+template <int N, int CW, typename F, typename U>
+__device__ __forceinline__ void mma_split_rows(f32x4 (&acc)[CW][N], const F& rows, const U& use,
+                                               const Split<float> (&b)[CW]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (use(i)) {
+      const Split<float> a = rows(i);
+#pragma unroll
+      for (int c = 0; c < CW; ++c) mma(acc[c][i], a.f, b[c].f);
+    }
+}
+template <int N, int CW, typename F, typename U>
+__device__ __forceinline__ void mma_split_rows(f32x4 (&acc)[CW][N], const F& rows, const U& use,
+                                               const Split<bf16> (&b)[CW]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+    if (use(i)) {   // the tiles of a pair alike
+      const Split<bf16> a[2] = {rows(i), rows(i + 1)};
+#pragma unroll
+      for (int part = 0; part < 3; ++part)   // the product of the low parts is below the sum's step
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int c = 0; c < CW; ++c)
+            mma(acc[c][i + x], part == 1 ? a[x].lo : a[x].hi, part == 0 ? b[c].lo : b[c].hi);
+    }
 }
 
 __device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }
 __device__ __forceinline__ Frag<bf16> high_of(const Split<bf16>& s) { return s.hi; }
 
-// A wave's rows of a state, from row k on in steps of 32: row k + 32 s + 4 h + r in S[2 s + h][r];
-// `at` is its column in row 0, which is inside also where the lane's own is not.
-template <int NS>
-__device__ __forceinline__ void load_state(f32x4 (&S)[2 * NS], const float* from, long at,
-                                           bool inside, int k, int K, int V) {
+// A wave's 16 columns of a state: row 32 s + 8 g + 4 h + r in S[2 s + h][r] of the lanes of group g.
+// `at`: the lane's column in row 0, or one inside where it has none.
+template <int N>
+__device__ __forceinline__ void load_state(f32x4 (&S)[N], const float* at, bool inside, int g,
+                                           int K, int V) {
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
-  if (!from) return;
-#pragma unroll
-  for (int i = 0; i < 2 * NS; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      S[i][r] = from[at + (long)min(k + 32 * (i >> 1) + 4 * (i & 1) + r, K - 1) * V];
+      S[i][r] = at[(long)min(32 * (i >> 1) + 8 * g + 4 * (i & 1) + r, K - 1) * V];
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (!inside || k + 32 * (i >> 1) + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
+      if (!inside || 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r >= K) S[i][r] = 0.f;
 }
-template <int NS>
-__device__ __forceinline__ void store_state(const f32x4 (&S)[2 * NS], float* to, long at,
-                                            bool inside, int k, int K, int V) {
-  if (!to || !inside) return;
+template <int N>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[N], float* at, bool inside, int g,
+                                            int K, int V) {
+  if (!inside) return;
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = k + 32 * (i >> 1) + 4 * (i & 1) + r;
-      if (row < K) to[at + (long)row * V] = S[i][r];
+      const int row = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
+      if (row < K) at[(long)row * V] = S[i][r];
     }
-}
-
-// The waves of the launches that go from chunk to chunk: NW lots of 16 columns a block, and KW
-// waves for each, which share the rows of its state (KP / KW each). Those hand one another their
-// shares of the products with the state through LDS and do the triangular system alike.
-// Few columns in all want many waves for each, as one chunk's chain of products is what counts;
-// many want few, as the system is then solved once.
-struct DeltaWaves {
-  int nw, kw;
-};
-inline DeltaWaves delta_waves(const tops_gla_delta_args& a, int KP) {
-  const long lots = (a.V + 15) / 16 * a.HV * a.nseq;
-  if (lots <= 512) return {1, KP == 64 ? 2 : 4};
-  if (lots <= 1024) return {2, 2};
-  return {4, 1};
-}
-
-// Sums tiles over the KW waves of a lot, in the same order for each. `x`: N * 64 quads for each
-// wave of the block.
-template <int N, int KW, int NW>
-__device__ __forceinline__ void share_sum(f32x4 (&acc)[N], f32x4* x, int wave, int lane) {
-  if constexpr (KW > 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[(wave * N + i) * 64 + lane] = acc[i];
-    __syncthreads();
-    const int c = wave % NW;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      acc[i] = x[(c * N + i) * 64 + lane];
-#pragma unroll
-      for (int k = 1; k < KW; ++k) acc[i] += x[((c + k * NW) * N + i) * 64 + lane];
-    }
-  }
 }
 
 }  // namespace tops

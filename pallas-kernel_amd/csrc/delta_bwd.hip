@@ -5,8 +5,7 @@
 // normed ones:
 //   dN = P^T dO + e^{G_C - G} (K dS),   Y = Tm^T dN,
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) - K^T (beta e^G Y),
-// which one launch takes from chunk to chunk, columns as the forward's states; then, for every
-// chunk at once, with dP = dO N^T for j <= i and E = Y N^T for j < i:
+// which goes from chunk to chunk (delta_scan.hip); then, here, for every chunk at once, with dP = dO N^T for j <= i and E = Y N^T for j < i:
 //   dq  = scale (e^G (dO S^T) + (dP D) K),
 //   z   = -(e^G (Y S^T) + (E D) K),                    (what k reads with, over beta)
 //   dkw = e^{G_C - G} (N dS^T) + scale (dP D)^T Q - (beta E D)^T K,     (what k writes with)
@@ -21,176 +20,6 @@
 namespace tops {
 
 namespace {
-
-// ---------------------------------------------------------------------------
-// The states' gradients
-// ---------------------------------------------------------------------------
-
-template <typename T, int KP, int NW, int KW>
-struct DscanLds {
-  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1;
-  static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(16 * NW);
-  static constexpr int K0 = 0, Q0 = C * PK, T0 = 2 * C * PK, P0 = T0 + PARTS * C * PT;
-  static constexpr int V0 = P0 + PARTS * C * PT, END = V0 + C * PV;
-  static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
-  static constexpr int X0 = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // shares of the waves
-  static constexpr int BYTES = X0 + (KW > 1 ? NW * KW * (C / 16) * 1024 : 0);
-};
-
-template <typename T, int KP, int NW, int KW>
-__global__ __launch_bounds__(64 * NW * KW) void delta_dscan_kernel(DeltaParams p) {
-  using L = DscanLds<T, KP, NW, KW>;
-  constexpr int C = L::C, NT = 64 * NW * KW, NS = KP / 32 / KW, NU = C / 32, LO = C * L::PT;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const tops_gla_delta_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int cw = wave % NW, kw = wave / NW, k0 = kw * (KP / KW);
-  const int g = lane >> 4, ci = lane & 15;
-  const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
-  const int vt = (V + 16 * NW - 1) / (16 * NW);
-  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);
-  const int vb = blk % vt;
-  blk /= vt;
-  const int hv = blk % HV, seq = blk / HV, h = hv / (HV / (int)a.H);
-  int b = 0, t0 = 0, T_ = (int)a.T, c0 = 0;
-  if (a.seqs) {
-    t0 = a.seqs[seq];
-    T_ = a.seqs[seq + 1] - t0;
-    c0 = a.seqs[a.nseq + 1 + seq];
-  } else {
-    b = seq;
-    c0 = seq * ((T_ + C - 1) / C);
-  }
-  const int nc = (T_ + C - 1) / C;
-  const T* kp = (const T*)a.k + b * a.k_sb + t0 * a.k_st + h * a.k_sh;
-  const T* qp = (const T*)a.q + b * a.q_sb + t0 * a.q_st + h * a.q_sh;
-  const int vc = V - vb * 16 * NW;
-  const T* dp = (const T*)a.dout + b * a.do_sb + t0 * a.do_st + hv * a.do_sh + vb * 16 * NW;
-  const int v = vb * 16 * NW + 16 * cw + ci;
-  const bool vin = v < V;
-
-  f32x4 S[2 * NS];   // dS, as the forward's states
-  const long st0 = ((long)seq * HV + hv) * K * V + v;
-  load_state<NS>(S, a.dht, st0 - v + min(v, V - 1), vin, k0 + 8 * g, K, V);
-
-  TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
-  TileStream<T, C, C, NT> fp[2] = {{C, C, tid}, {C, C, tid}};
-  TileStream<T, C, 16 * NW, NT> fd(a.do_st, vc, tid);
-  constexpr int NF = (3 * C + NT) / NT;
-  float ff[NF], fr[NF];
-  auto fetch = [&](int n) {
-    const int len = min(C, T_ - n * C);
-    const long unit = (long)(c0 + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
-#pragma unroll
-    for (int i = 0; i < L::PARTS; ++i)   // rows past the end have not been written
-      fp[i].next((const T*)(p.P + unit * (C * C * 4)) + i * C * C, C, len, C, tid);
-    fd.next(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
-    const float* vec = delta_vec(p, unit);
-#pragma unroll
-    for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|
-      const int x = i * NT + tid, t = x % C;
-      const float e = vec[t + (x < C ? C : 0)], r = vec[t + (x < 2 * C ? 3 * C : 4 * C)];
-      ff[i] = x < 3 * C ? e * r : vec[C - 1];
-      fr[i] = x < C ? 1.f : x < 2 * C ? vec[2 * C + t] : x < 3 * C ? (float)a.scale : 1.f;
-    }
-  };
-  T* sm = (T*)smem;
-  T *sK = sm + L::K0, *sQ = sm + L::Q0, *sT = sm + L::T0, *sP = sm + L::P0, *sV = sm + L::V0;
-  float* sf = (float*)(smem + L::F0);
-  if (nc > 0) fetch(nc - 1);
-  for (int n = nc - 1; n >= 0; --n) {
-    __syncthreads();
-    const int len = min(C, T_ - n * C);
-    fk.put(sK, L::PK, len, K, tid);
-    fq.put(sQ, L::PK, len, K, tid);
-    ft.put(sT, L::PT, L::PARTS * C, C, tid);
-#pragma unroll
-    for (int i = 0; i < L::PARTS; ++i) fp[i].put(sP + i * LO, L::PT, len, C, tid);
-    fd.put(sV, L::PV, len, vc, tid);
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i] * fr[i];
-    __syncthreads();
-    if (n > 0) fetch(n - 1);
-    const long unit = (long)(c0 + n) * HV + hv;
-    const float last = sf[3 * C];
-
-    f32x4 acc[2 * NU];
-#pragma unroll
-    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-    T* So = (T*)p.dS + (unit * V + v) * KP + k0 + 8 * g;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      float x[8];
-      pair_values(S[2 * s], S[2 * s + 1], x);
-      const Split<T> f = split_of<T>(x);
-      if (vin) st_frag(So + 32 * s, high_of(f));
-      mma_rows<2 * NU>(acc, [&](int i) {
-        return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + k0 + 32 * s + 8 * g);
-      }, f);
-    }
-    Frag<T> df[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) df[u] = ld_frag_t(sV + 16 * cw + 32 * u * L::PV, L::PV, lane);
-#pragma unroll
-    for (int i = 0; i < 2 * NU; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][r] *= sf[32 * (i >> 1) + 8 * g + 4 * (i & 1) + r];
-#pragma unroll
-    for (int w = 0; w < NU; ++w)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        if (w >= (i >> 1) && i % KW == kw)
-          mma(acc[i], ld_split_t<T>(sP + 32 * w * L::PT + 32 * (i >> 1), LO, L::PT, lane, i & 1),
-              df[w]);
-    share_sum<2 * NU, KW, NW>(acc, (f32x4*)(smem + L::X0), wave, lane);
-    Split<T> R[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      float x[8];
-      pair_values(acc[2 * u], acc[2 * u + 1], x);
-      R[u] = split_of<T>(x);
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-#pragma unroll
-    for (int w = 0; w < NU; ++w)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        if (w >= (i >> 1))
-          mma(acc[i], ld_split_t<T>(sT + 32 * w * L::PT + 32 * (i >> 1), LO, L::PT, lane, i & 1),
-              R[w]);
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
-    T* Yo = (T*)p.Y + (unit * V + v) * C + 8 * g;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      float x[8];
-      values_of(df[u], x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= sf[2 * C + 32 * u + 8 * g + e];
-      mma_rows<2 * NS>(S, [&](int i) {
-        return ld_pair_t(sQ + k0 + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, split_of<T>(x));
-      pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (vin && kw == u % KW) st_frag(Yo + 32 * u, frag_of<T>(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
-      mma_rows<2 * NS>(S, [&](int i) {
-        return ld_pair_t(sK + k0 + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, split_of<T>(x));
-    }
-  }
-  store_state<NS>(S, a.dh0, st0, vin, k0 + 8 * g, K, V);
-}
-
-// ---------------------------------------------------------------------------
-// The inputs' gradients
-// ---------------------------------------------------------------------------
 
 template <typename T, int KP>
 struct GradLds {
@@ -470,17 +299,6 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   }
 }
 
-template <typename T, int KP, int NW, int KW>
-hipError_t launch_dscan(const DeltaParams& p, hipStream_t st) {
-  constexpr int lds = DscanLds<T, KP, NW, KW>::BYTES;
-  const hipError_t e = hipFuncSetAttribute((const void*)delta_dscan_kernel<T, KP, NW, KW>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return e;
-  const long grid = (p.a.V + 16 * NW - 1) / (16 * NW) * p.a.HV * p.a.nseq;
-  delta_dscan_kernel<T, KP, NW, KW><<<(unsigned)grid, 64 * NW * KW, lds, st>>>(p);
-  return hipGetLastError();
-}
-
 template <typename T, int KP, bool GROUP>
 hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
   constexpr int lds = GradLds<T, KP>::BYTES;
@@ -494,20 +312,12 @@ hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
 
 template <typename T, int KP>
 hipError_t run(const DeltaParams& p, hipStream_t st) {
-  if (p.a.nseq > 0) {
-    const DeltaWaves w = delta_waves(p.a, KP);
-    const hipError_t e = w.nw == 1   ? launch_dscan<T, KP, 1, KP == 64 ? 2 : 4>(p, st)
-                         : w.nw == 2 ? launch_dscan<T, KP, 2, 2>(p, st)
-                                     : launch_dscan<T, KP, 4, 1>(p, st);
-    if (e != hipSuccess) return e;
-  }
-  if (p.a.chunks == 0) return hipSuccess;
   return p.a.HV > p.a.H ? launch_grad<T, KP, true>(p, st) : launch_grad<T, KP, false>(p, st);
 }
 
 }  // namespace
 
-hipError_t run_delta_bwd(const DeltaParams& p, hipStream_t st) {
+hipError_t run_delta_grad(const DeltaParams& p, hipStream_t st) {
   if (p.a.dtype == DT_BF16)
     return p.KP == 64 ? run<bf16, 64>(p, st) : p.KP == 128 ? run<bf16, 128>(p, st)
                                                            : run<bf16, 256>(p, st);

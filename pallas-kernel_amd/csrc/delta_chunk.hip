@@ -6,10 +6,8 @@
 // With Tm = (1 + A)^-1, which needs no state:
 //   N = Tm (beta (V - e^G (K S))),   S <- e^{G_C} S + K^T (e^{G_C - G} N),
 //   o = scale (e^G (Q S) + ((Q K^T) D) N).
-// Three launches: Tm of every chunk at once; the states, which go from chunk to chunk; the outputs
-// of every chunk at once. The columns of S and N are independent of one another, so that a wave of
-// the second launch owns 16 of them over all chunks of a sequence and head, with the state in its
-// accumulators: K S, Tm R and K^T N hand their results on as operands without leaving a lane.
+// Three launches: Tm of every chunk at once; the states, which go from chunk to chunk
+// (delta_scan.hip); the outputs of every chunk at once.
 #include "delta.hpp"
 
 namespace tops {
@@ -170,157 +168,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// The states
-// ---------------------------------------------------------------------------
-
-template <typename T, int KP, int NW, int KW>
-struct ScanLds {
-  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1;
-  static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(16 * NW);
-  static constexpr int K0 = 0, T0 = C * PK, V0 = T0 + PARTS * C * PT, END = V0 + C * PV;
-  static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
-  static constexpr int ONE = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // one of two buffers
-  static constexpr int X0 = 2 * ONE;                                  // shares of the waves
-  static constexpr int BYTES = X0 + (KW > 1 ? NW * KW * (C / 16) * 1024 : 0);
-};
-
-template <typename T, int KP, int NW, int KW>
-__global__ __launch_bounds__(64 * NW * KW) void delta_scan_kernel(DeltaParams p) {
-  using L = ScanLds<T, KP, NW, KW>;
-  constexpr int C = L::C, NT = 64 * NW * KW, NS = KP / 32 / KW, NU = C / 32;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const tops_gla_delta_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int cw = wave % NW, k0 = wave / NW * (KP / KW);   // its 16 columns, its rows of the state
-  const int g = lane >> 4, ci = lane & 15;
-  const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
-  const int vt = (V + 16 * NW - 1) / (16 * NW);
-  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);   // a head's columns on one XCD
-  const int vb = blk % vt;
-  blk /= vt;
-  const int hv = blk % HV, seq = blk / HV, h = hv / (HV / (int)a.H);
-  int b = 0, t0 = 0, T_ = (int)a.T, c0 = 0;
-  if (a.seqs) {
-    t0 = a.seqs[seq];
-    T_ = a.seqs[seq + 1] - t0;
-    c0 = a.seqs[a.nseq + 1 + seq];
-  } else {
-    b = seq;
-    c0 = seq * ((T_ + C - 1) / C);
-  }
-  const int nc = (T_ + C - 1) / C;
-  const T* kp = (const T*)a.k + b * a.k_sb + t0 * a.k_st + h * a.k_sh;
-  // the block's columns; the last block's few may begin before them, where there are fewer than 8
-  const int vc = V - vb * 16 * NW;
-  const T* vp = (const T*)a.v + b * a.v_sb + t0 * a.v_st + hv * a.v_sh + vb * 16 * NW;
-  const int v = vb * 16 * NW + 16 * cw + ci;
-  const bool vin = v < V;
-
-  // row k0 + 32 s + 8 g + 4 h + r of the state in S[2 s + h][r]
-  f32x4 S[2 * NS];
-  const long st0 = ((long)seq * HV + hv) * K * V + v;
-  load_state<NS>(S, a.h0, st0 - v + min(v, V - 1), vin, k0 + 8 * g, K, V);
-
-  TileStream<T, C, KP, NT> fk(a.k_st, K, tid);
-  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
-  TileStream<T, C, 16 * NW, NT> fv(a.v_st, vc, tid);
-  constexpr int NF = (3 * C + NT) / NT;
-  float ff[NF], fr[NF];
-  auto fetch = [&](int n) {
-    const int len = min(C, T_ - n * C);
-    const long unit = (long)(c0 + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
-    fv.next(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
-    const float* vec = delta_vec(p, unit);
-#pragma unroll
-    for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta, e^{G_C}
-      const int x = i * NT + tid;
-      ff[i] = vec[x < 3 * C ? x : C - 1];
-      fr[i] = vec[3 * C + x % C];
-    }
-  };
-  auto put = [&](int n) {
-    T* sm = (T*)(smem + (n & 1) * L::ONE);
-    const int len = min(C, T_ - n * C);
-    fk.put(sm + L::K0, L::PK, len, K, tid);
-    ft.put(sm + L::T0, L::PT, L::PARTS * C, C, tid);
-    fv.put(sm + L::V0, L::PV, len, vc, tid);
-    float* sf = (float*)(smem + (n & 1) * L::ONE + L::F0);
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = i * NT + tid < 2 * C ? ff[i] * fr[i] : ff[i];
-  };
-  if (nc > 0) {
-    fetch(0);
-    put(0);
-  }
-  for (int n = 0; n < nc; ++n) {
-    __syncthreads();
-    if (n + 1 < nc) fetch(n + 1);
-    const T* sm = (const T*)(smem + (n & 1) * L::ONE);
-    const T *sK = sm + L::K0 + k0, *sT = sm + L::T0, *sV = sm + L::V0 + 16 * cw;
-    const float* sf = (const float*)(smem + (n & 1) * L::ONE + L::F0);
-    const long unit = (long)(c0 + n) * HV + hv;
-    const float last = sf[3 * C];
-
-    f32x4 acc[2 * NU];
-#pragma unroll
-    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-    T* So = (T*)p.S + (unit * V + v) * KP + k0 + 8 * g;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      float x[8];
-      pair_values(S[2 * s], S[2 * s + 1], x);
-      const Split<T> f = split_of<T>(x);
-      if (vin) st_frag(So + 32 * s, high_of(f));
-      mma_rows<2 * NU>(acc, [&](int i) {
-        return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
-      }, f);
-    }
-    share_sum<2 * NU, KW, NW>(acc, (f32x4*)(smem + L::X0), wave, lane);
-    Split<T> R[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      float x[8], y[8];
-      values_of(ld_frag_t(sV + 32 * u * L::PV, L::PV, lane), y);
-      pair_values(acc[2 * u], acc[2 * u + 1], x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int t = 32 * u + 8 * g + e;
-        x[e] = sf[2 * C + t] * (y[e] - sf[t] * x[e]);
-      }
-      R[u] = split_of<T>(x);
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
-#pragma unroll
-    for (int w = 0; w < NU; ++w)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        if (w <= (i >> 1))
-          mma(acc[i], ld_split<T>(sT, C * L::PT, (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PT +
-                                                     32 * w + 8 * g), R[w]);
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
-    T* No = (T*)p.N + (unit * V + v) * C + 8 * g;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      float x[8];
-      pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (vin && wave / NW == u % KW) st_frag(No + 32 * u, frag_of<T>(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
-      mma_rows<2 * NS>(S, [&](int i) {
-        return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, split_of<T>(x));
-    }
-    if (n + 1 < nc) put(n + 1);
-  }
-  store_state<NS>(S, a.ht, st0, vin, k0 + 8 * g, K, V);
-}
-
-// ---------------------------------------------------------------------------
 // The outputs
 // ---------------------------------------------------------------------------
 
@@ -422,72 +269,65 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams
   }
 }
 
-template <typename T, int KP, int NW, int KW>
-hipError_t launch_scan(const DeltaParams& p, hipStream_t st) {
-  constexpr int lds = ScanLds<T, KP, NW, KW>::BYTES;
-  const hipError_t e = hipFuncSetAttribute((const void*)delta_scan_kernel<T, KP, NW, KW>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return e;
-  const long grid = (p.a.V + 16 * NW - 1) / (16 * NW) * p.a.HV * p.a.nseq;
-  delta_scan_kernel<T, KP, NW, KW><<<(unsigned)grid, 64 * NW * KW, lds, st>>>(p);
-  return hipGetLastError();
-}
-
-template <typename T, int KP>
-hipError_t run(const DeltaParams& p, hipStream_t st) {
-  const tops_gla_delta_args& a = p.a;
-  if (a.chunks > 0) {
-    delta_prep_kernel<T, KP><<<(unsigned)(a.chunks * a.H), 256, 0, st>>>(p);
-    if (const hipError_t e = hipGetLastError()) return e;
-  }
-  if (a.nseq > 0) {
-    const DeltaWaves w = delta_waves(a, KP);
-    const hipError_t e = w.nw == 1   ? launch_scan<T, KP, 1, KP == 64 ? 2 : 4>(p, st)
-                         : w.nw == 2 ? launch_scan<T, KP, 2, 2>(p, st)
-                                     : launch_scan<T, KP, 4, 1>(p, st);
-    if (e != hipSuccess) return e;
-  }
-  if (a.chunks > 0)
-    delta_out_kernel<T, KP><<<(unsigned)(a.chunks * a.HV), 4 * delta_c<T>(), 0, st>>>(p);
-  return hipGetLastError();
-}
-
 long up(long n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-DeltaParams delta_layout(int64_t chunks, int64_t HV, int64_t K, int64_t V, int dtype, bool train,
-                         void* keep, void* ws) {
+DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   DeltaParams p{};
-  const long es = dtype == DT_BF16 ? 2 : 4, units = chunks * HV;
-  p.C = delta_chunk_of(dtype);
-  p.KP = delta_key_pad(K);
+  const long es = z.dtype == DT_BF16 ? 2 : 4, units = z.chunks * z.HV, segs = z.nsegs * z.HV;
+  p.C = delta_chunk_of((int)z.dtype);
+  p.KP = delta_key_pad(z.K);
   p.vec_bytes = 28 * p.C;
+  p.multi = z.nsegs > z.nseq;
   long at = 0;
   auto take = [&](void* base, long bytes) {
     char* x = (char*)base + at;
     at += up(bytes);
     return x;
   };
+  const long ends = p.multi ? segs * z.K * z.V * 4 : 0, maps = p.multi ? segs * p.KP * p.KP * 4 : 0;
   p.vec = take(keep, units * p.vec_bytes);
   p.Tm = take(keep, units * p.C * p.C * 4);
-  p.N = take(keep, units * V * p.C * es);
-  p.S = take(keep, units * V * p.KP * es);
-  p.P = take(keep, train ? units * p.C * p.C * 4 : 0);
+  p.N = take(keep, units * z.V * p.C * es);
+  p.S = take(keep, units * z.V * p.KP * es);
+  p.P = take(keep, z.train ? units * p.C * p.C * 4 : 0);
+  p.E = (float*)take(keep, ends);
+  p.M = take(keep, maps);
+  p.Mt = take(keep, z.train ? maps : 0);
   p.keep_bytes = at;
   at = 0;
-  p.dS = take(ws, units * V * p.KP * es);
-  p.Y = take(ws, units * V * p.C * es);
+  p.dS = take(ws, units * z.V * p.KP * es);
+  p.Y = take(ws, units * z.V * p.C * es);
+  p.dE = (float*)take(ws, ends);
   p.ws_bytes = at;
   return p;
 }
 
-hipError_t run_delta_fwd(const DeltaParams& p, hipStream_t st) {
+template <typename T, int KP>
+static hipError_t prep(const DeltaParams& p, hipStream_t st) {
+  delta_prep_kernel<T, KP><<<(unsigned)(p.a.chunks * p.a.H), 256, 0, st>>>(p);
+  return hipGetLastError();
+}
+template <typename T, int KP>
+static hipError_t out(const DeltaParams& p, hipStream_t st) {
+  delta_out_kernel<T, KP><<<(unsigned)(p.a.chunks * p.a.HV), 4 * delta_c<T>(), 0, st>>>(p);
+  return hipGetLastError();
+}
+
+hipError_t run_delta_prep(const DeltaParams& p, hipStream_t st) {
   if (p.a.dtype == DT_BF16)
-    return p.KP == 64 ? run<bf16, 64>(p, st) : p.KP == 128 ? run<bf16, 128>(p, st)
-                                                           : run<bf16, 256>(p, st);
-  return p.KP == 64 ? run<float, 64>(p, st) : p.KP == 128 ? run<float, 128>(p, st)
-                                                          : run<float, 256>(p, st);
+    return p.KP == 64 ? prep<bf16, 64>(p, st) : p.KP == 128 ? prep<bf16, 128>(p, st)
+                                                            : prep<bf16, 256>(p, st);
+  return p.KP == 64 ? prep<float, 64>(p, st) : p.KP == 128 ? prep<float, 128>(p, st)
+                                                           : prep<float, 256>(p, st);
+}
+hipError_t run_delta_out(const DeltaParams& p, hipStream_t st) {
+  if (p.a.dtype == DT_BF16)
+    return p.KP == 64 ? out<bf16, 64>(p, st) : p.KP == 128 ? out<bf16, 128>(p, st)
+                                                           : out<bf16, 256>(p, st);
+  return p.KP == 64 ? out<float, 64>(p, st) : p.KP == 128 ? out<float, 128>(p, st)
+                                                          : out<float, 256>(p, st);
 }
 
 }  // namespace tops

@@ -105,8 +105,8 @@ _DELTA_SIGS = {
     "tops_gla_delta_fwd": [_S, _P],
     "tops_gla_delta_bwd": [_S, _P],
     "tops_gla_delta_chunk": [_I64],
-    "tops_gla_delta_keep_bytes": [_I64] * 6,
-    "tops_gla_delta_ws_bytes": [_I64] * 5,
+    "tops_gla_delta_segment": [_I64] * 4,
+    "tops_gla_delta_bytes": [_S, _I64],
     "tops_gla_delta_step": [_S, _P],
     "tops_gla_layer_norm_fwd": [_S, _P],
     "tops_gla_layer_norm_bwd": [_S, _P],
@@ -123,8 +123,8 @@ _RESTYPE = {"tops_gla_chunk_ws_bytes": ctypes.c_int64, "tops_gla_kernel_ms": cty
             "tops_gla_causal_conv_bwd_ws_bytes": ctypes.c_int64,
             "tops_gla_qk_norm_rope_ws_bytes": ctypes.c_int64,
             "tops_gla_delta_chunk": ctypes.c_int64,
-            "tops_gla_delta_keep_bytes": ctypes.c_int64,
-            "tops_gla_delta_ws_bytes": ctypes.c_int64,
+            "tops_gla_delta_segment": ctypes.c_int64,
+            "tops_gla_delta_bytes": ctypes.c_int64,
             "tops_gla_layer_norm_ws_bytes": ctypes.c_int64}
 
 EXPORTED = ["tops_gla_last_error", "tops_gla_version"] + list(_SIGS)

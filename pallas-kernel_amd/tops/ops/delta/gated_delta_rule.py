@@ -14,7 +14,8 @@ from ..._lib import call_on, check_device, dtype_code, require
 from ..ssm._common import (address, device_table, differentiable, f32, gradients, io_dtype,
                            offsets, refuse_grad, rows, slot_args, strides)
 
-_ARGS = struct.Struct("=37qd13q")
+_ARGS = struct.Struct("=39qd13q")
+_SIZES = struct.Struct("=8q")
 _STEP = struct.Struct("=34qd")
 _NO_BWD = (0,) * 13
 
@@ -33,30 +34,47 @@ def _tokens(t, dt):
 
 
 class _Chunks:
-    """The chunks that a call's sequences are cut into."""
+    """The chunks that a call's sequences are cut into, and the segments that these run in."""
 
-    def __init__(self, B, T, cu, dt, device):
-        C = _lib.load().tops_gla_delta_chunk(dtype_code(dt))
+    def __init__(self, B, T, cu, dt, HV, V, device):
+        lib = _lib.load()
+        C = lib.tops_gla_delta_chunk(dtype_code(dt))
         self.table = None
         if cu is None:
-            self.nseq, self.n = B, B * -(-T // C)
+            per = -(-T // C)
+            self.nseq, self.n = B, B * per
+            self.L = lib.tops_gla_delta_segment(B, self.n, HV, V)
+            self.nsegs = B * max(1, -(-per // self.L))
             return
         self.nseq = len(cu) - 1
+        counts = [-((a - b) // C) for a, b in zip(cu, cu[1:])]
+        self.n = sum(counts)
+        # the longest sequences are cut however many there are
+        self.L = lib.tops_gla_delta_segment(1, self.n, HV, V)
 
         def make():
-            first = [0]
-            for a, b in zip(cu, cu[1:]):
-                first.append(first[-1] - (a - b) // C)
-            return [*cu, *first], first[-1]
+            chunks, segs, seq = [0], [0], []
+            for s, n in enumerate(counts):
+                k = max(1, -(-n // self.L))
+                chunks.append(chunks[-1] + n)
+                segs.append(segs[-1] + k)
+                seq += [s] * k
+            return [*cu, *chunks, *segs, *seq], len(seq)
 
-        self.table, self.n = device_table(("delta", tuple(cu), C), make, device)
+        self.table, self.nsegs = device_table(("delta", tuple(cu), C, self.L), make, device)
+
+    def bytes(self, HV, K, V, dt, train, backward):
+        return _lib.load().tops_gla_delta_bytes(
+            _SIZES.pack(self.nseq, self.n, self.nsegs, HV, K, V, dtype_code(dt), int(train)),
+            int(backward))
 
 
 def _pack(x, h0, o, ht, keep, nkeep, ch, shape, norm, train, scale, bwd=_NO_BWD):
     q, k, v, g, beta = x
     return _ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), address(h0),
-        address(o), address(ht), address(ch.table), address(keep), nkeep, ch.nseq, ch.n, *shape,
+        address(o), address(ht), address(ch.table), address(keep), nkeep, ch.nseq, ch.n, ch.nsegs,
+        ch.L, *shape,
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()[:2], *beta.stride()[:2],
         int(norm), int(train), dtype_code(q.dtype), dtype_code(g.dtype), dtype_code(beta.dtype),
         scale, *bwd)
@@ -69,10 +87,10 @@ def _forward(q, k, v, g, beta, h0, scale, norm, want, cu, train):
     HV, V = v.shape[2:]
     x = _tokens(q, dt), _tokens(k, dt), _tokens(v, dt), _gate(g), _gate(beta)
     h0 = f32(h0)
-    ch = _Chunks(B, T, cu, dt, dev)
+    ch = _Chunks(B, T, cu, dt, HV, V, dev)
     o = torch.empty(B, T, HV, V, dtype=dt, device=dev)
     ht = torch.empty(ch.nseq, HV, K, V, dtype=torch.float32, device=dev) if want else None
-    nkeep = _lib.load().tops_gla_delta_keep_bytes(ch.n, HV, K, V, dtype_code(dt), int(train))
+    nkeep = ch.bytes(HV, K, V, dt, train, False)
     keep = torch.empty(nkeep, dtype=torch.uint8, device=dev)
     call_on(dev, "tops_gla_delta_fwd", _pack(x, h0, o, ht, keep, nkeep, ch,
                                              (B, T, H, HV, K, V), norm, train, scale))
@@ -106,7 +124,7 @@ class _GatedDeltaRuleFunction(torch.autograd.Function):
         dbeta = new(B, T, HV, dtype=beta.dtype, device=dev)
         dh0 = (None if ctx.like[5] is None
                else new(ch.nseq, HV, K, V, dtype=torch.float32, device=dev))
-        nws = _lib.load().tops_gla_delta_ws_bytes(ch.n, HV, K, V, dtype_code(dt))
+        nws = ch.bytes(HV, K, V, dt, True, True)
         ws = new(nws, dtype=torch.uint8, device=dev)
         bwd = [do.data_ptr(), *strides(do, 0, 1, 2), *(address(t) for t in (
             dht, dq, dk, dv, dg, dbeta, dh0, ws)), nws]

@@ -140,7 +140,8 @@ def test_binding_matches_the_header():
     assert set(re.findall(r"\b(?:int|int64_t) (tops_gla_\w+)\(", src)) == set(_lib._DELTA_SIGS)
 
 
-DELTA = dict(batch=1, nseq=1, T=4, H=1, HV=2, K=16, V=16, chunks=1, dtype=1)
+DELTA = dict(batch=1, nseq=1, T=4, H=1, HV=2, K=16, V=16, chunks=1, nsegs=1, seg_chunks=4,
+             dtype=1)
 PTRS = dict.fromkeys(("q", "k", "v", "g", "beta", "o"), 64)
 
 
@@ -149,12 +150,16 @@ PTRS = dict.fromkeys(("q", "k", "v", "g", "beta", "o"), 64)
     (dict(K=0), 2, "K must"), (dict(K=257), 2, "K must"), (dict(K=7), 2, "at least 8"),
     (dict(V=4), 2, "at least 8"), (dict(V=0), 2, "V must"), (dict(V=65537), 2, "V must"),
     (dict(H=0), 1, "divide"), (dict(HV=3, H=2), 1, "divide"), (dict(T=-1), 1, "bad"),
-    (dict(chunks=2), 1, "chunks"), (dict(nseq=2), 1, "nseq"), (dict(T=65), 1, "chunks"),
+    (dict(chunks=2), 1, "chunks"), (dict(nseq=2), 1, "nseq"), (dict(T=65), 1, "chunks"), (dict(nsegs=2), 1, "nsegs"),
+    (dict(seg_chunks=0), 1, "seg_chunks"), (dict(seg_chunks=1 << 26), 1, "seg_chunks"),
+    (dict(T=320, chunks=5), 1, "nsegs"), (dict(seqs=64, nsegs=0), 1, "bad nseq"),
+    (dict(seqs=64, nsegs=3), 1, "bad nseq"),
     (dict(T=65, dtype=0, chunks=2), 1, "chunks"), (dict(seqs=64, batch=2), 1, "batch == 1"),
-    (dict(seqs=64, chunks=3), 1, "bad nseq or chunks"), (dict(seqs=64, chunks=0), 1, "bad nseq"),
+    (dict(seqs=64, chunks=3), 1, "bad nseq, chunks"), (dict(seqs=64, chunks=0), 1, "bad nseq"),
     (dict(batch=1 << 20, nseq=1 << 20, T=1 << 20), 2, "2^31"),
+    (dict(PTRS, q_st=1 << 24), 2, "2^24"), (dict(PTRS, v_st=-(1 << 24)), 2, "2^24"),
     (dict(T=(1 << 31) - 64, chunks=(1 << 25) - 1), 2, "2^31"),
-    (dict(T=1 << 30, chunks=1 << 24, HV=1 << 12), 2, "grid"), (dict(), 1, "NULL"),
+    (dict(T=1 << 30, chunks=1 << 24, nsegs=1 << 22, HV=1 << 12), 2, "grid"), (dict(), 1, "NULL"),
     (dict(PTRS, o=0), 1, "o must"), (PTRS, 1, "keep"), (dict(PTRS, keep=256), 1, "keep"),
     (dict(PTRS, keep=128, keep_bytes=1 << 30), 1, "keep")])
 def test_delta_entry(over, code, what):
@@ -216,13 +221,31 @@ def test_workspace_sizes():
     lib = _lib.load()
     assert lib.tops_gla_delta_chunk(1) == 64 and lib.tops_gla_delta_chunk(0) == 32
     assert lib.tops_gla_delta_chunk(2) == 0
-    small = lib.tops_gla_delta_keep_bytes(3, 2, 100, 72, 1, 0)
+
+    def size(back, nseq=1, chunks=3, nsegs=1, HV=2, K=100, V=72, dtype=1, train=0):
+        return lib.tops_gla_delta_bytes(
+            struct.pack("=8q", nseq, chunks, nsegs, HV, K, V, dtype, train), back)
+
     # the state's 72 x 128 and the values' 72 x 64 elements of a chunk and head among them
-    assert small >= 6 * 2 * (72 * 128 + 72 * 64)
-    assert lib.tops_gla_delta_keep_bytes(3, 2, 100, 72, 1, 1) > small
-    assert lib.tops_gla_delta_ws_bytes(3, 2, 100, 72, 1) >= 6 * 2 * (72 * 128 + 72 * 64)
-    assert lib.tops_gla_delta_keep_bytes(-1, 2, 100, 72, 1, 0) == 0
-    assert lib.tops_gla_delta_ws_bytes(3, 2, 300, 72, 1) == 0
+    assert size(0) >= 6 * 2 * (72 * 128 + 72 * 64) and size(0, train=1) > size(0)
+    assert size(1, train=1) >= 6 * 2 * (72 * 128 + 72 * 64)
+    # and of three segments and two heads a state's 100 x 72 floats and a map's 128 x 128 pairs
+    assert size(0, nsegs=3) - size(0) >= 6 * 4 * (100 * 72 + 128 * 128)
+    assert size(1, nsegs=3) - size(1) >= 6 * 4 * 100 * 72
+    assert not any(size(0, **bad) for bad in (
+        dict(chunks=-1), dict(K=300), dict(V=0), dict(dtype=2), dict(nsegs=0), dict(HV=0)))
+    assert lib.tops_gla_delta_bytes(None, 0) == 0
+
+
+def test_segments():
+    """Few columns in all are cut, many or short sequences are not."""
+    f = _lib.load().tops_gla_delta_segment
+    whole = 1 << 20
+    assert f(1, 256, 16, 128) == 16 and f(2, 128, 16, 128) == 8
+    assert f(1, 3, 1, 64) == whole and f(1, 12, 1, 64) == whole and f(1, 16, 1, 64) == 4
+    assert f(8, 1024, 32, 128) == whole and f(2, 128, 64, 128) == whole
+    assert f(0, 0, 1, 64) == whole and f(1, 0, 1, 64) == whole
+    assert f(1, 1 << 25, 1, 64) == 1 << 17
     assert lib.tops_gla_layer_norm_ws_bytes(0, 8, 0) == 64
     assert lib.tops_gla_layer_norm_ws_bytes(5, 0, 0) == 0
 

@@ -97,6 +97,21 @@ def test_packed(lens, init, dt):
     check(x, r, cu=cu, norm=True)
 
 
+@pytest.mark.parametrize("lens", [[1100], [1500, 20, 700, 0, 300, 64], [1025]])
+@pytest.mark.parametrize("K,V", [(64, 20), (100, 90)])
+@pytest.mark.parametrize("dt", [FL, BF])
+def test_segments(lens, K, V, dt):
+    """Sequences long enough to be cut into segments that run in parallel."""
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    x, r = make(1, cu[-1], 1, 2, K, V, dt, S=len(lens), norm=True)
+    x["g"] *= 0.05   # what is before a segment has to matter at its end
+    check(x, r, cu=cu, norm=True)
+    if len(lens) == 1:
+        check(x, r, norm=True)
+
+
 @pytest.mark.parametrize("B,T", [(0, 5), (2, 0), (0, 0)])
 @pytest.mark.parametrize("dt", [FL, BF])
 def test_no_tokens(B, T, dt):
