@@ -222,6 +222,8 @@ template <>
 __device__ __forceinline__ Split<bf16> split_of<bf16>(const float (&x)[8]) {
   Split<bf16> s;
   s.hi = frag_of<bf16>(x);
+  // hides the packed words, whose halves the compiler would otherwise convert once more
+  asm("" : "+v"(s.hi.d.x), "+v"(s.hi.d.y), "+v"(s.hi.d.z), "+v"(s.hi.d.w));
   float h[8];
   values_of(s.hi, h);
 #pragma unroll
@@ -332,7 +334,7 @@ struct TileFetch {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int p = i * NT + tid, row = p / (W / 8);
-      r[i] = row < len ? cut_run(r[i], p % (W / 8) * 8, cols) : Run<T, 8>{};
+      r[i] = row < min(len, C) ? cut_run(r[i], p % (W / 8) * 8, cols) : Run<T, 8>{};
     }
   }
   __device__ __forceinline__ void put(T* dst, int pitch, int len, int cols, int tid) {
@@ -425,16 +427,32 @@ __device__ __forceinline__ void mma_split_rows(f32x4 (&acc)[CW][N], const F& row
 __device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }
 __device__ __forceinline__ Frag<bf16> high_of(const Split<bf16>& s) { return s.hi; }
 
-// A wave's 16 columns of a state: row 32 s + 8 g + 4 h + r in S[2 s + h][r] of the lanes of group g.
-// `at`: the lane's column in row 0, or one inside where it has none.
+// A lane's rows of its column of a state: row k + 32 s + 4 h + r in S[2 s + h][r], k its first. `at`
+// is the column in row 0. Rows past K are the last one's when they are loaded.
 template <int N>
-__device__ __forceinline__ void load_state(f32x4 (&S)[N], const float* at, bool inside, int g,
-                                           int K, int V) {
+__device__ __forceinline__ void load_rows(f32x4 (&S)[N], const float* at, int k, int K, int V) {
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      S[i][r] = at[(long)min(32 * (i >> 1) + 8 * g + 4 * (i & 1) + r, K - 1) * V];
+      S[i][r] = at[(long)min(k + 32 * (i >> 1) + 4 * (i & 1) + r, K - 1) * V];
+}
+template <int N>
+__device__ __forceinline__ void store_rows(const f32x4 (&S)[N], float* at, int k, int K, int V) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = k + 32 * (i >> 1) + 4 * (i & 1) + r;
+      if (row < K) at[(long)row * V] = S[i][r];
+    }
+}
+// The same of all rows of a state for a wave's 16 columns, zeros where a lane has no column;
+// `at` is then one inside.
+template <int N>
+__device__ __forceinline__ void load_state(f32x4 (&S)[N], const float* at, bool inside, int g,
+                                           int K, int V) {
+  load_rows(S, at, 8 * g, K, V);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -444,14 +462,7 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[N], const float* at, bool 
 template <int N>
 __device__ __forceinline__ void store_state(const f32x4 (&S)[N], float* at, bool inside, int g,
                                             int K, int V) {
-  if (!inside) return;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r;
-      if (row < K) at[(long)row * V] = S[i][r];
-    }
+  if (inside) store_rows(S, at, 8 * g, K, V);
 }
 
 }  // namespace tops

@@ -27,9 +27,11 @@ struct GradLds {
   static constexpr int PK = pitch_of<T>(KP), PC = pitch_of<T>(C), PS = pitch_of<T>(VS);
   static constexpr int K0 = 0, Q0 = C * PK, N0 = 2 * C * PK, Y0 = N0 + VS * PC, S0 = Y0 + VS * PC;
   static constexpr int D0 = S0 + VS * PK, O0 = D0 + VS * PK, END = O0 + C * PS;
-  static constexpr int G0 = (END * (int)sizeof(T) + 15) / 16 * 16;   // G [C] in 64 bits
-  static constexpr int F0 = G0 + 8 * C;                              // [6][C] floats
-  static constexpr int BYTES = F0 + (6 * C + 8) * 4;
+  // beta z on its way to the waves of the keys, where the slabs were
+  static constexpr int PX = KP + 4, X0 = N0 * (int)sizeof(T);
+  static constexpr int G0 = (std::max(END * (int)sizeof(T), X0 + C * PX * 4) + 15) / 16 * 16;
+  static constexpr int F0 = G0 + 8 * C;                // after G [C] in 64 bits: [7][C] floats
+  static constexpr int BYTES = F0 + (7 * C + 8) * 4;
 };
 
 __device__ __forceinline__ float group_sum(float x) {   // over the four lanes of a column
@@ -52,16 +54,20 @@ __device__ __forceinline__ float row_dot(const T* row, const f32x4 (&acc)[2 * NS
   return group_sum(sum);
 }
 
-// A wave has 16 tokens of a chunk as columns of all its products; a block goes through the value
-// heads of its key head (GROUP: more than one), so that their sums need no second launch.
+// Each wave has 16 tokens of a chunk as columns of all its products: half of a block's waves have
+// them as queries (dq, z, dv and their rows of the scores' gradients), half as keys (dkw and their
+// columns of these), so that no wave holds more accumulators than two waves a SIMD leave it. A block
+// goes through the value heads of its key head (GROUP: more than one), so that their sums need no
+// second launch.
 template <typename T, int KP, bool GROUP>
-__global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParams p) {
+__global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParams p) {
   using L = GradLds<T, KP>;
-  constexpr int C = L::C, NT = 4 * C, NS = KP / 32, NU = C / 32, VS = L::VS;
+  constexpr int C = L::C, NT = 8 * C, NS = KP / 32, NU = C / 32, VS = L::VS, NW = C / 16;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int g = lane >> 4, i = 16 * wave + (lane & 15), uw = wave / 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tw = wave % NW;
+  const bool key = wave >= NW;
+  const int g = lane >> 4, i = 16 * tw + (lane & 15), uw = tw / 2;
   const int K = (int)a.K, V = (int)a.V, H = (int)a.H, HV = (int)a.HV;
   const int chunk = (int)(blockIdx.x / H), h = (int)(blockIdx.x % H);
   const ChunkAt at = delta_chunk_at(a, C, chunk);
@@ -69,9 +75,10 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   T* sm = (T*)smem;
   T *sK = sm + L::K0, *sQ = sm + L::Q0, *sN = sm + L::N0, *sY = sm + L::Y0, *sS = sm + L::S0;
   T *sD = sm + L::D0, *sO = sm + L::O0;
+  float* sX = (float*)(smem + L::X0);
   double* sG = (double*)(smem + L::G0);
-  float* sf = (float*)(smem + L::F0);   // e^G, e^{G_C - G}, beta, 1 / |k|, 1 / |q|; dG; <S, dS>
-  float *sdG = sf + 5 * C, *sSum = sf + 6 * C;
+  float* sf = (float*)(smem + L::F0);   // e^G, e^{G_C - G}, beta, 1 / |k|, 1 / |q|; dG; k . beta z
+  float *sdG = sf + 5 * C, *sKz = sf + 6 * C, *sSum = sf + 7 * C;   // then <S, dS>
   {
     TileFetch<T, C, KP, NT> f;
     f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
@@ -81,11 +88,10 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   }
   const T *kr = sK + i * L::PK, *qr = sQ + i * L::PK;
   const float scale = (float)a.scale;
-  constexpr int NG = GROUP ? 2 * NS : 1;
-  f32x4 dqs[NG], dks[NG];
-  float sqs = 0.f, sks = 0.f;
+  f32x4 sum[GROUP ? 2 * NS : 1];   // over the value heads: dq, or dk
+  float dots = 0.f;                // and its product with q, or k
 #pragma unroll
-  for (int x = 0; x < NG; ++x) dqs[x] = dks[x] = zero4();
+  for (int x = 0; x < (GROUP ? 2 * NS : 1); ++x) sum[x] = zero4();
 
   const int group = HV / H;
   for (int gi = 0; gi < group; ++gi) {
@@ -106,7 +112,7 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       fs.get((const T*)p.S + (unit * V + v0) * KP, KP, V - v0, KP, tid);
       fd.get((const T*)p.dS + (unit * V + v0) * KP, KP, V - v0, KP, tid);
       fo.get(dop + v0, a.do_st, at.len, V - v0, tid);
-      fv = get_run<T, 8>(vp + min(v0 + 8 * g, V - 8));
+      if (!key) fv = get_run<T, 8>(vp + min(v0 + 8 * g, V - 8));
     };
     fetch(0);
     if (GROUP) __syncthreads();   // the vectors of the head before have been read
@@ -115,13 +121,14 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       for (int x = tid; x < 5 * C; x += NT) sf[x] = vec[x];
       if (tid < C) sG[tid] = delta_gsum(p, unit)[tid];
     }
-    f32x4 dq[2 * NS], z[2 * NS], dkw[2 * NS], PT[2 * NU], ET[2 * NU], P2[2 * NU], E2[2 * NU];
+    // of a query: dq, z, and its rows of dP and E, transposed; of a key: dkw (and nothing), and its
+    // columns of them
+    f32x4 A[2][2 * NS], B[2][2 * NU];
 #pragma unroll
-    for (int x = 0; x < 2 * NS; ++x) dq[x] = z[x] = dkw[x] = zero4();
+    for (int x = 0; x < 2 * NS; ++x) A[0][x] = A[1][x] = zero4();
 #pragma unroll
-    for (int x = 0; x < 2 * NU; ++x) PT[x] = ET[x] = P2[x] = E2[x] = zero4();
-    float vy = 0.f, sd = 0.f;
-    float beta = 0.f;
+    for (int x = 0; x < 2 * NU; ++x) B[0][x] = B[1][x] = zero4();
+    float vy = 0.f, sd = 0.f, beta = 0.f;
     for (int v0 = 0; v0 < V; v0 += VS) {
       __syncthreads();
       fn.put(sN, L::PC, V - v0, C, tid);
@@ -133,16 +140,15 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       for (int x = 0; x < decltype(fs)::N; ++x)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sd = fmaf(to_f32(fs.r[x].v[e]), to_f32(fd.r[x].v[e]), sd);
-      __syncthreads();
       const Run<T, 8> vr = fv;
+      __syncthreads();
       if (v0 + VS < V) fetch(v0 + VS);
-      if (v0 == 0) beta = sf[2 * C + i];
-      const Frag<T> of = ld_frag(sO + i * L::PS + 8 * g);
-      const Frag<T> yf = ld_frag_t(sY + 16 * wave, L::PC, lane);
-      const Frag<T> nf = ld_frag_t(sN + 16 * wave, L::PC, lane);
-      const int c = v0 + 8 * g;
-      {   // dv, and v . Y (Y is 0 past the end)
-        float y[8], x[8];
+      beta = sf[2 * C + i];
+      if (!key) {
+        const Frag<T> of = ld_frag(sO + i * L::PS + 8 * g);
+        const Frag<T> yf = ld_frag_t(sY + 16 * tw, L::PC, lane);
+        const int c = v0 + 8 * g;
+        float y[8], x[8];   // dv, and v . Y (Y is 0 past the end)
         values_of(yf, y);
         values_of(frag_of<T>(cut_run(vr, c, V)), x);
 #pragma unroll
@@ -151,92 +157,107 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
           y[e] *= beta;
         }
         if (in && c < V) put_run<T, 8>(dvp + c, y, V - c);
-      }
 #pragma unroll
-      for (int x = 0; x < 2 * NU; ++x) {
-        const int u = x >> 1;
-        if (u <= uw) {   // columns: this wave's tokens i, rows: tokens j
-          const Frag<T> f = ld_pair_t(sN + 32 * u, L::PC, lane, x & 1);
-          mma(PT[x], f, of);
-          mma(ET[x], f, yf);
-        }
-        if (u >= uw) {   // columns: this wave's tokens as j, rows: tokens i
-          mma(P2[x], ld_frag(sO + (32 * u + pair_row(lane, x & 1)) * L::PS + 8 * g), nf);
-          mma(E2[x], ld_pair_t(sY + 32 * u, L::PC, lane, x & 1), nf);
-        }
-      }
+        for (int n = 0; n < 2 * NU; ++n)
+          if ((n >> 1) <= uw) {
+            const Frag<T> f = ld_pair_t(sN + 32 * (n >> 1), L::PC, lane, n & 1);
+            mma(B[0][n], f, of);
+            mma(B[1][n], f, yf);
+          }
 #pragma unroll
-      for (int x = 0; x < 2 * NS; ++x) {
-        const Frag<T> f = ld_pair_t(sS + 32 * (x >> 1), L::PK, lane, x & 1);
-        mma(dq[x], f, of);
-        mma(z[x], f, yf);
-        mma(dkw[x], ld_pair_t(sD + 32 * (x >> 1), L::PK, lane, x & 1), nf);
+        for (int n = 0; n < 2 * NS; ++n) {
+          const Frag<T> f = ld_pair_t(sS + 32 * (n >> 1), L::PK, lane, n & 1);
+          mma(A[0][n], f, of);
+          mma(A[1][n], f, yf);
+        }
+      } else {
+        const Frag<T> nf = ld_frag_t(sN + 16 * tw, L::PC, lane);
+#pragma unroll
+        for (int n = 0; n < 2 * NU; ++n)
+          if ((n >> 1) >= uw) {
+            mma(B[0][n], ld_frag(sO + (32 * (n >> 1) + pair_row(lane, n & 1)) * L::PS + 8 * g), nf);
+            mma(B[1][n], ld_pair_t(sY + 32 * (n >> 1), L::PC, lane, n & 1), nf);
+          }
+#pragma unroll
+        for (int n = 0; n < 2 * NS; ++n)
+          mma(A[0][n], ld_pair_t(sD + 32 * (n >> 1), L::PK, lane, n & 1), nf);
       }
     }
-    const float gam = sf[i], gbar = sf[C + i], rk = sf[3 * C + i], rq = sf[4 * C + i];
-    const double Gi = sG[i];
-    // gradients of the raw q and k, but for the norms' own part; z times beta (times 1 where beta
-    // is nothing that can be divided by: its own gradient needs z alone)
-    const float aq = scale * rq, bz = fabsf(beta) < 0x1p-64f ? 1.f : beta, ak = bz * rk;
+    // Gradients of the raw q and k, but for the norms' own part; z times beta (times 1 where beta is
+    // nothing that can be divided by: its own gradient needs z alone).
+    const float rk = sf[3 * C + i], aq = scale * sf[4 * C + i];
+    const float bz = fabsf(beta) < 0x1p-64f ? 1.f : beta, ak = bz * rk;
     const float zb = bz == beta ? 1.f : beta;   // beta z over the accumulated
+    const double Gi = sG[i];
+    float sw = 0.f;
+    if (!key) {
+      const float gam = sf[i];
 #pragma unroll
-    for (int x = 0; x < 2 * NS; ++x) {
-      dq[x] *= gam * aq;
-      z[x] *= gam * ak;
-      dkw[x] *= gbar * rk;
-    }
-    const float left = row_dot<T, NS>(kr, dkw, g);
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      float x[8], y[8];
-      if (u <= uw) {
-        pair_values(PT[2 * u], PT[2 * u + 1], x);
-        pair_values(ET[2 * u], ET[2 * u + 1], y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = 32 * u + 8 * g + e;
-          const float d = j <= i ? gexp<T>((float)(Gi - sG[j])) : 0.f, rj = sf[3 * C + j];
-          x[e] = j <= i ? x[e] * (d * (aq * rj)) : 0.f;
-          y[e] = j < i ? y[e] * (d * (ak * rj)) : 0.f;
-        }
-        const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
-#pragma unroll
-        for (int s = 0; s < 2 * NS; ++s) {
-          const Frag<T> f = ld_pair_t(sK + 32 * u * L::PK + 32 * (s >> 1), L::PK, lane, s & 1);
-          mma(dq[s], f, fx);
-          mma(z[s], f, fyy);
-        }
+      for (int n = 0; n < 2 * NS; ++n) {
+        A[0][n] *= gam * aq;
+        A[1][n] *= gam * ak;
       }
-      if (u >= uw) {
-        pair_values(P2[2 * u], P2[2 * u + 1], x);
-        pair_values(E2[2 * u], E2[2 * u + 1], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = 32 * u + 8 * g + e;
-          const float d = j >= i ? gexp<T>((float)(sG[j] - Gi)) : 0.f;
-          const float aj = scale * sf[4 * C + j], bj = sf[2 * C + j] * sf[3 * C + j];
-          x[e] = j >= i ? x[e] * (d * (aj * rk)) : 0.f;
-          y[e] = j > i ? -(y[e] * (d * (bj * rk))) : 0.f;
-        }
-        const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
+      for (int u = 0; u < NU; ++u)
+        if (u <= uw) {
+          float x[8], y[8];
+          pair_values(B[0][2 * u], B[0][2 * u + 1], x);
+          pair_values(B[1][2 * u], B[1][2 * u + 1], y);
 #pragma unroll
-        for (int s = 0; s < 2 * NS; ++s) {
-          const int off = 32 * u * L::PK + 32 * (s >> 1);
-          mma(dkw[s], ld_pair_t(sQ + off, L::PK, lane, s & 1), fx);
-          mma(dkw[s], ld_pair_t(sK + off, L::PK, lane, s & 1), fyy);
+          for (int e = 0; e < 8; ++e) {
+            const int j = 32 * u + 8 * g + e;
+            const float d = j <= i ? gexp<T>((float)(Gi - sG[j])) : 0.f, rj = sf[3 * C + j];
+            x[e] = j <= i ? x[e] * (d * (aq * rj)) : 0.f;
+            y[e] = j < i ? y[e] * (d * (ak * rj)) : 0.f;
+          }
+          const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
+#pragma unroll
+          for (int n = 0; n < 2 * NS; ++n) {
+            const Frag<T> f = ld_pair_t(sK + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1);
+            mma(A[0][n], f, fx);
+            mma(A[1][n], f, fyy);
+          }
         }
+      const float sq = row_dot<T, NS>(qr, A[0], g), sz = -row_dot<T, NS>(kr, A[1], g);
+      vy = group_sum(vy);
+      if (g == 0) {
+        sdG[i] = sq + zb * sz;
+        sKz[i] = zb * sz;
+        if (in) put_any(a.dbeta, (int)a.beta_dtype, tok * HV + hv, sz / bz + vy);
       }
-    }
-    const float sq = row_dot<T, NS>(qr, dq, g), sw = row_dot<T, NS>(kr, dkw, g);
-    const float sz = -row_dot<T, NS>(kr, z, g);
-    vy = group_sum(vy);
-    if (g == 0) {
-      sdG[i] = sq + zb * sz - sw;
-      if (in) put_any(a.dbeta, (int)a.beta_dtype, tok * HV + hv, sz / bz + vy);
+      dots += sq;
+    } else {
+      const float gbar = sf[C + i];
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n) A[0][n] *= gbar * rk;
+      const float left = row_dot<T, NS>(kr, A[0], g);
+      sd = sd * sf[C - 1] + (g == 0 ? left : 0.f);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        if (u >= uw) {
+          float x[8], y[8];
+          pair_values(B[0][2 * u], B[0][2 * u + 1], x);
+          pair_values(B[1][2 * u], B[1][2 * u + 1], y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = 32 * u + 8 * g + e;
+            const float d = j >= i ? gexp<T>((float)(sG[j] - Gi)) : 0.f;
+            const float aj = scale * sf[4 * C + j], bj = sf[2 * C + j] * sf[3 * C + j];
+            x[e] = j >= i ? x[e] * (d * (aj * rk)) : 0.f;
+            y[e] = j > i ? -(y[e] * (d * (bj * rk))) : 0.f;
+          }
+          const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
+#pragma unroll
+          for (int n = 0; n < 2 * NS; ++n) {
+            const int off = 32 * u * L::PK + 32 * (n >> 1);
+            mma(A[0][n], ld_pair_t(sQ + off, L::PK, lane, n & 1), fx);
+            mma(A[0][n], ld_pair_t(sK + off, L::PK, lane, n & 1), fyy);
+          }
+        }
+      sw = row_dot<T, NS>(kr, A[0], g);
     }
     {   // e^{G_C} <S, dS>, and the part of dG_C that the tokens' decays to it have
-      sd *= sf[C - 1];
-      sd += g == 0 ? left : 0.f;
+      if (!key) sd *= sf[C - 1];
       sd += dpp<0x121>(sd);
       sd += dpp<0x122>(sd);
       sd += dpp<0x124>(sd);
@@ -244,11 +265,32 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       sd = group_sum(sd);
       if (lane == 0) sSum[wave] = sd;
     }
+    __syncthreads();   // nobody reads the slabs any more
+    if (!key) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          f32x4 w = A[1][2 * s + x] * zb;
+          *reinterpret_cast<f32x4*>(sX + i * L::PX + 32 * s + 8 * g + 4 * x) = w;
+        }
+    }
+    __syncthreads();
+    if (key) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          A[0][2 * s + x] -=
+              *reinterpret_cast<const f32x4*>(sX + i * L::PX + 32 * s + 8 * g + 4 * x);
+      dots += sKz[i] + sw;
+      if (g == 0) sdG[i] -= sw;
+    }
     __syncthreads();
     if (wave == 0) {
       float s = lane < C ? sdG[lane] : 0.f;
 #pragma unroll
-      for (int w = 0; w < C / 16; ++w) s += lane == C - 1 ? sSum[w] : 0.f;
+      for (int w = 0; w < 2 * NW; ++w) s += lane == C - 1 ? sSum[w] : 0.f;
 #pragma unroll
       for (int o = 1; o < C; o <<= 1) {
         const float x = __shfl_down(s, o);
@@ -258,42 +300,28 @@ __global__ __launch_bounds__(4 * delta_c<T>()) void delta_grad_kernel(DeltaParam
         put_any(a.dg, (int)a.g_dtype,
                 ((long)at.b * a.T + at.t + lane) * HV + hv, s);
     }
-    const float sk = zb * sz + sw;
     if (GROUP) {
 #pragma unroll
-      for (int x = 0; x < 2 * NS; ++x) {
-        dqs[GROUP ? x : 0] += dq[x];
-        dks[GROUP ? x : 0] += dkw[x] - zb * z[x];
-      }
-      sqs += sq;
-      sks += sk;
+      for (int x = 0; x < 2 * NS; ++x) sum[GROUP ? x : 0] += A[0][x];
       if (gi + 1 < group) continue;
     }
-    const float nq = a.l2norm ? rq * rq * (GROUP ? sqs : sq) : 0.f;
-    const float nk = a.l2norm ? rk * rk * (GROUP ? sks : sk) : 0.f;
     if (in) {
-      T* dqo = (T*)a.dq + (tok * H + h) * K;
-      T* dko = (T*)a.dk + (tok * H + h) * K;
+      const float r = sf[(key ? 3 : 4) * C + i], norm = a.l2norm ? r * r * dots : 0.f;
+      const T* row = key ? kr : qr;
+      T* to = (T*)(key ? a.dk : a.dq) + (tok * H + h) * K;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int c = 32 * s + 8 * g;
         if (c >= K) continue;
         float x[8], y[8];
-        values_of(ld_frag(qr + c), x);
+        values_of(ld_frag(row + c), x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float d = GROUP ? dqs[GROUP ? 2 * s + e / 4 : 0][e % 4] : dq[2 * s + e / 4][e % 4];
-          y[e] = d - nq * x[e];
+          const float d =
+              GROUP ? sum[GROUP ? 2 * s + e / 4 : 0][e % 4] : A[0][2 * s + e / 4][e % 4];
+          y[e] = d - norm * x[e];
         }
-        put_run<T, 8>(dqo + c, y, K - c);
-        values_of(ld_frag(kr + c), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float d = GROUP ? dks[GROUP ? 2 * s + e / 4 : 0][e % 4]
-                                : dkw[2 * s + e / 4][e % 4] - zb * z[2 * s + e / 4][e % 4];
-          y[e] = d - nk * x[e];
-        }
-        put_run<T, 8>(dko + c, y, K - c);
+        put_run<T, 8>(to + c, y, K - c);
       }
     }
   }
@@ -306,7 +334,7 @@ hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   delta_grad_kernel<T, KP, GROUP>
-      <<<(unsigned)(p.a.chunks * p.a.H), 4 * delta_c<T>(), lds, st>>>(p);
+      <<<(unsigned)(p.a.chunks * p.a.H), 8 * delta_c<T>(), lds, st>>>(p);
   return hipGetLastError();
 }
 

@@ -459,12 +459,15 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 }
 
 // E_j <- M_j E_{j-1} + E_j along the segments of a sequence and head, or dE_j <- M_j^T dE_{j+1} +
-// dE_j the other way; a wave has 16 columns.
+// dE_j the other way. A block has 16 columns, each of its waves KP / 4 or KP / 2 of the rows; the
+// states go from wave to wave through LDS as operands, the maps and parts of the next segment are
+// on their way meanwhile.
 template <typename T, int KP, bool BACK>
-__global__ __launch_bounds__(64) void delta_fold_kernel(DeltaParams p) {
-  constexpr int NS = KP / 32, PARTS = sizeof(T) == 2 ? 2 : 1;
+__global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaParams p) {
+  constexpr int NS = KP / 32, NW = KP == 64 ? 2 : 4, NR = NS / NW, PARTS = sizeof(T) == 2 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) Frag<T> sh[2][PARTS][NS][64];
   const tops_gla_delta_args& a = p.a;
-  const int lane = threadIdx.x, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + 15) / 16;
   int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);
@@ -481,29 +484,60 @@ __global__ __launch_bounds__(64) void delta_fold_kernel(DeltaParams p) {
     first = seq * count;
   }
   if (count < 3) return;   // the first segment to run is where it should be
-  float* E = BACK ? p.dE : p.E;
   const long tile = (long)KP * KP;
-  f32x4 S[1][2 * NS];
-  auto state = [&](int j) { return E + ((long)(first + j) * HV + hv) * K * V; };
-  load_state(S[0], state(BACK ? count - 1 : 0) + min(v, V - 1), v < V, g, K, V);
-  for (int n = 1; n + 1 < count; ++n) {
+  const int k0 = wave * NR * 32;   // the wave's rows: k0 + 32 s + 8 g + 4 h + r as ever
+  auto state = [&](int n) {
     const int j = BACK ? count - 1 - n : n;
-    const T* M = (const T*)((BACK ? p.Mt : p.M) + ((long)(first + j) * HV + hv) * tile * 4);
-    f32x4 acc[1][2 * NS];
-    load_state(acc[0], state(j) + min(v, V - 1), v < V, g, K, V);
+    return (BACK ? p.dE : p.E) + ((long)(first + j) * HV + hv) * K * V;
+  };
+  Split<T> M[2 * NR][NS];
+  f32x4 E[2 * NR];
+  auto fetch = [&](int n) {
+    const int j = BACK ? count - 1 - n : n;
+    const T* m = (const T*)((BACK ? p.Mt : p.M) + ((long)(first + j) * HV + hv) * tile * 4);
+#pragma unroll
+    for (int i = 0; i < 2 * NR; ++i)
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        M[i][s] = ld_split<T>(m, (int)tile, (k0 + 32 * (i >> 1) + pair_row(lane, i & 1)) * KP +
+                                                32 * s + 8 * g);
+    load_rows(E, state(n) + min(v, V - 1), k0 + 8 * g, K, V);
+  };
+  auto share = [&](int n) {   // the wave's rows of the state after step n, and to memory
+#pragma unroll
+    for (int s = 0; s < NR; ++s) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = v < V && k0 + 32 * s + 8 * g + e < K ? E[2 * s + e / 4][e % 4] : 0.f;
+      const Split<T> f = split_of<T>(x);
+      sh[n & 1][0][wave * NR + s][lane] = high_of(f);
+      if constexpr (PARTS == 2) sh[n & 1][1][wave * NR + s][lane] = f.lo;
+    }
+    if (n > 0 && v < V) store_rows(E, state(n) + v, k0 + 8 * g, K, V);
+  };
+  load_rows(E, state(0) + min(v, V - 1), k0 + 8 * g, K, V);
+  share(0);
+  fetch(1);
+  for (int n = 1; n + 1 < count; ++n) {
+    __syncthreads();
+    f32x4 acc[2 * NR];
+#pragma unroll
+    for (int i = 0; i < 2 * NR; ++i) acc[i] = E[i];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      float x[8];
-      pair_values(S[0][2 * s], S[0][2 * s + 1], x);
-      const Split<T> f[1] = {split_of<T>(x)};
-      mma_split_rows(acc, [&](int i) {
-        return ld_split<T>(M, PARTS == 2 ? (int)tile : 0,
-                           (32 * (i >> 1) + pair_row(lane, i & 1)) * KP + 32 * s + 8 * g);
-      }, [](int) { return true; }, f);
+      Split<T> f;
+      if constexpr (PARTS == 2)
+        f = {sh[(n - 1) & 1][0][s][lane], sh[(n - 1) & 1][1][s][lane]};
+      else
+        f = {sh[(n - 1) & 1][0][s][lane]};
+#pragma unroll
+      for (int i = 0; i < 2 * NR; ++i) mma(acc[i], M[i][s], f);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) S[0][i] = acc[0][i];
-    store_state(S[0], state(j) + v, v < V, g, K, V);
+    for (int i = 0; i < 2 * NR; ++i) E[i] = acc[i];
+    share(n);
+    if (n + 2 < count) fetch(n + 1);
   }
 }
 
@@ -533,7 +567,7 @@ hipError_t passes(const DeltaParams& p, hipStream_t st) {
   if (p.multi) {
     if (const hipError_t e = launch<T, KP, CW, NW, BACK, true>(p, st)) return e;
     const unsigned grid = (unsigned)((p.a.V + 15) / 16 * p.a.HV * p.a.nseq);
-    delta_fold_kernel<T, KP, BACK><<<grid, 64, 0, st>>>(p);
+    delta_fold_kernel<T, KP, BACK><<<grid, KP == 64 ? 128 : 256, 0, st>>>(p);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   return launch<T, KP, CW, NW, BACK, false>(p, st);
@@ -544,7 +578,7 @@ hipError_t run(const DeltaParams& p, hipStream_t st) {
   // two lots of 16 columns a wave read each of the chunk's tiles once for both; with 256 keys their
   // states do not fit the registers
   if constexpr (KP < 256)
-    if (p.a.V > 64) return passes<T, KP, 2, 4, BACK>(p, st);
+    if (p.a.V > 64) return passes<T, KP, 1, 8, BACK>(p, st);
   return passes<T, KP, 1, 4, BACK>(p, st);
 }
 template <typename T, int KP>

@@ -212,13 +212,15 @@ def test_norm_bwd_entry(over, what):
 def test_null_arguments():
     lib = _lib.load()
     for name, sig in _lib._DELTA_SIGS.items():
-        if sig[0] is ctypes.c_char_p:
+        if sig == [ctypes.c_char_p, ctypes.c_void_p]:
             assert getattr(lib, name)(None, None) == 1
             assert b"NULL" in lib.tops_gla_last_error()
 
 
 def test_workspace_sizes():
     lib = _lib.load()
+    assert lib.tops_gla_layer_norm_ws_bytes(0, 8, 0) == 64
+    assert lib.tops_gla_layer_norm_ws_bytes(5, 0, 0) == 0
     assert lib.tops_gla_delta_chunk(1) == 64 and lib.tops_gla_delta_chunk(0) == 32
     assert lib.tops_gla_delta_chunk(2) == 0
 
@@ -246,8 +248,6 @@ def test_segments():
     assert f(8, 1024, 32, 128) == whole and f(2, 128, 64, 128) == whole
     assert f(0, 0, 1, 64) == whole and f(1, 0, 1, 64) == whole
     assert f(1, 1 << 25, 1, 64) == 1 << 17
-    assert lib.tops_gla_layer_norm_ws_bytes(0, 8, 0) == 64
-    assert lib.tops_gla_layer_norm_ws_bytes(5, 0, 0) == 0
 
 
 # ---------------------------------------------------------------------------
