@@ -128,9 +128,7 @@ int norm_check(const tops_gla_layer_norm_args* a) {
 hipError_t run_fwd(const tops::DeltaParams& p, hipStream_t st) {
   if (p.a.chunks > 0)
     if (const hipError_t e = tops::run_delta_prep(p, st)) return e;
-  if (p.a.nseq > 0)
-    if (const hipError_t e = tops::run_delta_scan(p, false, st)) return e;
-  return p.a.chunks > 0 ? tops::run_delta_out(p, st) : hipSuccess;
+  return p.a.nseq > 0 ? tops::run_delta_scan(p, false, st) : hipSuccess;
 }
 hipError_t run_bwd(const tops::DeltaParams& p, hipStream_t st) {
   if (p.a.nseq > 0)

@@ -105,18 +105,24 @@ constexpr int delta_c() {
   return sizeof(T) == 2 ? 64 : 32;
 }
 inline int delta_chunk_of(int dtype) { return dtype == DT_BF16 ? 64 : 32; }
+template <typename T>
+constexpr int delta_blocks() {   // lower 32 x 32 blocks of a tile of C x C
+  return delta_c<T>() == 64 ? 3 : 1;
+}
+__device__ __forceinline__ constexpr int tri_block(int u, int w) { return u * (u + 1) / 2 + w; }
 inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 
-// Per chunk and value head ("unit"): vectors over the chunk's tokens, [5][C] float and [C] double:
-//   e^{G_i}, e^{G_C - G_i}, beta, 1 / |k|, 1 / |q| (1 without l2norm), and G, the sum of the log
-//   decays up to a token (in 64 bits: differences of it go into exponentials);
-// then, as tiles in the operands' type (two of them, high and low part, where it is bfloat16)
-//   Tm [C][C] the inverse of 1 + tril(beta k k^T decay), P [C][C] the masked scores,
-// and  N [V][C] the written values,  S [V][KP] the state before the chunk.
+// Per chunk and value head ("unit"): vectors over the chunk's tokens, [7][C] float and [C] double,
+//   e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|, e^G, e^{G_C - G}, 1 / |q|
+// (norms 1 without l2norm) and G, the sums of the log decays (in 64 bits: differences of it go into
+// exponentials); then, in the operands' type, two of them (high and low part) where it is bfloat16,
+//   Tm the inverse of 1 + tril(beta k k^T decay), P the masked and scaled scores, both as the lower
+// of their 32 x 32 blocks (0, 0), (1, 0), (1, 1);
+// and, for the backward, N [V][C] the written values, S [V][KP] the state before the chunk.
 struct DeltaParams {
   tops_gla_delta_args a;   // 8 <= K, 8 <= V
   int C, KP, parts;   // tokens of a chunk, padded keys, parts of a split tile (2 or 1)
-  char *vec, *Tm, *P, *N, *S;   // in keep
+  char *vec, *Tm, *P, *N, *S;   // in keep, the last three with `train`
   char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
                                 // right side
   // where a sequence has several segments, for each of all segments and value heads: the state
@@ -125,13 +131,12 @@ struct DeltaParams {
   float *E, *dE;
   char *M, *Mt;
   int multi;
-  long vec_bytes, keep_bytes, ws_bytes;
+  long vec_bytes, tri_bytes, keep_bytes, ws_bytes;
 };
 // The layout for given sizes; pointers from base addresses that may be NULL.
 DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws);
 hipError_t run_delta_prep(const DeltaParams& p, hipStream_t st);
 hipError_t run_delta_scan(const DeltaParams& p, bool backward, hipStream_t st);
-hipError_t run_delta_out(const DeltaParams& p, hipStream_t st);
 hipError_t run_delta_grad(const DeltaParams& p, hipStream_t st);
 
 struct ChunkAt {
@@ -162,7 +167,7 @@ __device__ __forceinline__ float* delta_vec(const DeltaParams& p, long unit) {
   return (float*)(p.vec + unit * p.vec_bytes);
 }
 __device__ __forceinline__ double* delta_gsum(const DeltaParams& p, long unit) {
-  return (double*)(p.vec + unit * p.vec_bytes + 20 * p.C);
+  return (double*)(p.vec + unit * p.vec_bytes + 28 * p.C);
 }
 
 template <typename T>
@@ -367,61 +372,43 @@ struct TileStream : TileFetch<T, C, W, NT> {
   }
 };
 
-// acc[c][i] += A(i) B[c] for N tiles of rows and CW of columns, part after part of a split operand,
-// so that a product does not wait for the one before it.
-template <int N, int CW, typename F>
-__device__ __forceinline__ void mma_rows(f32x4 (&acc)[CW][N], const F& rows,
-                                         const Split<float> (&b)[CW]) {
+// acc[i] += A(i) B for N tiles of rows, part after part of a split operand, so that a product does
+// not wait for the one before it.
+template <int N, typename F>
+__device__ __forceinline__ void mma_rows(f32x4 (&acc)[N], const F& rows, const Split<float>& b) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const Frag<float> a = rows(i);
+  for (int i = 0; i < N; ++i) mma(acc[i], rows(i), b.f);
+}
+template <int N, typename F>
+__device__ __forceinline__ void mma_rows(f32x4 (&acc)[N], const F& rows, const Split<bf16>& b) {
+  constexpr int W = N < 4 ? N : 4;
 #pragma unroll
-    for (int c = 0; c < CW; ++c) mma(acc[c][i], a, b[c].f);
+  for (int i = 0; i < N; i += W) {
+    Frag<bf16> a[W];
+#pragma unroll
+    for (int x = 0; x < W; ++x) a[x] = rows(i + x);
+#pragma unroll
+    for (int x = 0; x < W; ++x) mma(acc[i + x], a[x], b.lo);
+#pragma unroll
+    for (int x = 0; x < W; ++x) mma(acc[i + x], a[x], b.hi);
   }
 }
-template <int N, int CW, typename F>
-__device__ __forceinline__ void mma_rows(f32x4 (&acc)[CW][N], const F& rows,
-                                         const Split<bf16> (&b)[CW]) {
+// The same with the rows in two parts too, for the pair of tiles u.
+template <int N, typename F>
+__device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& rows,
+                                               const Split<float>& b) {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const Frag<bf16> a[2] = {rows(i), rows(i + 1)};
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int c = 0; c < CW; ++c) mma(acc[c][i + x], a[x], b[c].lo);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int c = 0; c < CW; ++c) mma(acc[c][i + x], a[x], b[c].hi);
-  }
+  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], rows(h), b);
 }
-// The same with the rows in two parts too; `use(i)` says which tiles have a part in the product.
-template <int N, int CW, typename F, typename U>
-__device__ __forceinline__ void mma_split_rows(f32x4 (&acc)[CW][N], const F& rows, const U& use,
-                                               const Split<float> (&b)[CW]) {
+template <int N, typename F>
+__device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& rows,
+                                               const Split<bf16>& b) {
+  const Split<bf16> a[2] = {rows(0), rows(1)};
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (use(i)) {
-      const Split<float> a = rows(i);
+  for (int part = 0; part < 3; ++part)   // the product of the low parts is below the sum's step
 #pragma unroll
-      for (int c = 0; c < CW; ++c) mma(acc[c][i], a.f, b[c].f);
-    }
-}
-template <int N, int CW, typename F, typename U>
-__device__ __forceinline__ void mma_split_rows(f32x4 (&acc)[CW][N], const F& rows, const U& use,
-                                               const Split<bf16> (&b)[CW]) {
-#pragma unroll
-  for (int i = 0; i < N; i += 2)
-    if (use(i)) {   // the tiles of a pair alike
-      const Split<bf16> a[2] = {rows(i), rows(i + 1)};
-#pragma unroll
-      for (int part = 0; part < 3; ++part)   // the product of the low parts is below the sum's step
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int c = 0; c < CW; ++c)
-            mma(acc[c][i + x], part == 1 ? a[x].lo : a[x].hi, part == 0 ? b[c].lo : b[c].hi);
-    }
+    for (int h = 0; h < 2; ++h)
+      mma(acc[2 * u + h], part == 1 ? a[h].lo : a[h].hi, part == 0 ? b.lo : b.hi);
 }
 
 __device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }

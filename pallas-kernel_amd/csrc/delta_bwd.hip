@@ -30,8 +30,8 @@ struct GradLds {
   // beta z on its way to the waves of the keys, where the slabs were
   static constexpr int PX = KP + 4, X0 = N0 * (int)sizeof(T);
   static constexpr int G0 = (std::max(END * (int)sizeof(T), X0 + C * PX * 4) + 15) / 16 * 16;
-  static constexpr int F0 = G0 + 8 * C;                // after G [C] in 64 bits: [7][C] floats
-  static constexpr int BYTES = F0 + (7 * C + 8) * 4;
+  static constexpr int F0 = G0 + 8 * C;                // after G [C] in 64 bits: [9][C] floats
+  static constexpr int BYTES = F0 + (9 * C + 8) * 4;
 };
 
 __device__ __forceinline__ float group_sum(float x) {   // over the four lanes of a column
@@ -77,8 +77,8 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   T *sD = sm + L::D0, *sO = sm + L::O0;
   float* sX = (float*)(smem + L::X0);
   double* sG = (double*)(smem + L::G0);
-  float* sf = (float*)(smem + L::F0);   // e^G, e^{G_C - G}, beta, 1 / |k|, 1 / |q|; dG; k . beta z
-  float *sdG = sf + 5 * C, *sKz = sf + 6 * C, *sSum = sf + 7 * C;   // then <S, dS>
+  float* sf = (float*)(smem + L::F0);   // the unit's vectors; dG, k . beta z, <S, dS>
+  float *sdG = sf + 7 * C, *sKz = sf + 8 * C, *sSum = sf + 9 * C;
   {
     TileFetch<T, C, KP, NT> f;
     f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     if (GROUP) __syncthreads();   // the vectors of the head before have been read
     {
       const float* vec = delta_vec(p, unit);
-      for (int x = tid; x < 5 * C; x += NT) sf[x] = vec[x];
+      for (int x = tid; x < 7 * C; x += NT) sf[x] = vec[x];
       if (tid < C) sG[tid] = delta_gsum(p, unit)[tid];
     }
     // of a query: dq, z, and its rows of dP and E, transposed; of a key: dkw (and nothing), and its
@@ -185,13 +185,13 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     }
     // Gradients of the raw q and k, but for the norms' own part; z times beta (times 1 where beta is
     // nothing that can be divided by: its own gradient needs z alone).
-    const float rk = sf[3 * C + i], aq = scale * sf[4 * C + i];
+    const float rk = sf[3 * C + i], aq = scale * sf[6 * C + i];
     const float bz = fabsf(beta) < 0x1p-64f ? 1.f : beta, ak = bz * rk;
     const float zb = bz == beta ? 1.f : beta;   // beta z over the accumulated
     const double Gi = sG[i];
     float sw = 0.f;
     if (!key) {
-      const float gam = sf[i];
+      const float gam = sf[4 * C + i];
 #pragma unroll
       for (int n = 0; n < 2 * NS; ++n) {
         A[0][n] *= gam * aq;
@@ -227,11 +227,11 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       }
       dots += sq;
     } else {
-      const float gbar = sf[C + i];
+      const float gbar = sf[5 * C + i];
 #pragma unroll
       for (int n = 0; n < 2 * NS; ++n) A[0][n] *= gbar * rk;
       const float left = row_dot<T, NS>(kr, A[0], g);
-      sd = sd * sf[C - 1] + (g == 0 ? left : 0.f);
+      sd = sd * sf[5 * C - 1] + (g == 0 ? left : 0.f);
 #pragma unroll
       for (int u = 0; u < NU; ++u)
         if (u >= uw) {
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
           for (int e = 0; e < 8; ++e) {
             const int j = 32 * u + 8 * g + e;
             const float d = j >= i ? gexp<T>((float)(sG[j] - Gi)) : 0.f;
-            const float aj = scale * sf[4 * C + j], bj = sf[2 * C + j] * sf[3 * C + j];
+            const float aj = scale * sf[6 * C + j], bj = sf[2 * C + j] * sf[3 * C + j];
             x[e] = j >= i ? x[e] * (d * (aj * rk)) : 0.f;
             y[e] = j > i ? -(y[e] * (d * (bj * rk))) : 0.f;
           }
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       sw = row_dot<T, NS>(kr, A[0], g);
     }
     {   // e^{G_C} <S, dS>, and the part of dG_C that the tokens' decays to it have
-      if (!key) sd *= sf[C - 1];
+      if (!key) sd *= sf[5 * C - 1];
       sd += dpp<0x121>(sd);
       sd += dpp<0x122>(sd);
       sd += dpp<0x124>(sd);
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       if (gi + 1 < group) continue;
     }
     if (in) {
-      const float r = sf[(key ? 3 : 4) * C + i], norm = a.l2norm ? r * r * dots : 0.f;
+      const float r = sf[(key ? 3 : 6) * C + i], norm = a.l2norm ? r * r * dots : 0.f;
       const T* row = key ? kr : qr;
       T* to = (T*)(key ? a.dk : a.dq) + (tok * H + h) * K;
 #pragma unroll

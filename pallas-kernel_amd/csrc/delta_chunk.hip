@@ -6,8 +6,8 @@
 // With Tm = (1 + A)^-1, which needs no state:
 //   N = Tm (beta (V - e^G (K S))),   S <- e^{G_C} S + K^T (e^{G_C - G} N),
 //   o = scale (e^G (Q S) + ((Q K^T) D) N).
-// Three launches: Tm of every chunk at once; the states, which go from chunk to chunk
-// (delta_scan.hip); the outputs of every chunk at once.
+// Here: Tm of every chunk at once. The states go from chunk to chunk, and the outputs with them
+// (delta_scan.hip).
 #include "delta.hpp"
 
 namespace tops {
@@ -98,11 +98,13 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
     if (tid < C) {
       float* vec = delta_vec(p, unit);
       const double G = sG[tid];
-      vec[tid] = expf((float)G);
-      vec[C + tid] = expf((float)(sG[C - 1] - G));
+      const float rk = sRk[tid], e = expf((float)G), l = expf((float)(sG[C - 1] - G));
+      vec[tid] = e * rk;
+      vec[C + tid] = l * rk;
       vec[2 * C + tid] = sBeta[tid];
-      vec[3 * C + tid] = sRk[tid];
-      vec[4 * C + tid] = 0.f;   // the outputs' launch writes it for the tokens there are
+      vec[3 * C + tid] = rk;
+      vec[4 * C + tid] = e;
+      vec[5 * C + tid] = l;
       delta_gsum(p, unit)[tid] = G;
     }
     if (wave < NB) {
@@ -153,119 +155,19 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
       }
     }
     __syncthreads();
-    T* out = (T*)(p.Tm + unit * (C * C * 4));
-    for (int i = tid; i < C * C / 8; i += 256) {
-      const int row = i / (C / 8), col = i % (C / 8) * 8;
-      float x[8];
+    T* out = (T*)(p.Tm + unit * p.tri_bytes);
+    constexpr int TRI = delta_blocks<T>() * 1024;
+    for (int i = tid; i < TRI / 8; i += 256) {   // 8 elements of block x
+      const int x = i / 128, row = i % 128 / 4, col = i % 4 * 8;
+      const float* t = sT + (32 * (x > 0) + row) * PA + 32 * (x == 2) + col;
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = sT[row * PA + col + e];
-      const Split<T> s = split_of<T>(x);
-      st_frag(out + row * C + col, high_of(s));
-      if constexpr (sizeof(T) == 2) st_frag(out + C * C + row * C + col, s.lo);
+      for (int e = 0; e < 8; ++e) y[e] = t[e];
+      const Split<T> s = split_of<T>(y);
+      st_frag(out + 8 * i, high_of(s));
+      if constexpr (sizeof(T) == 2) st_frag(out + TRI + 8 * i, s.lo);
     }
     __syncthreads();
-  }
-}
-
-// ---------------------------------------------------------------------------
-// The outputs
-// ---------------------------------------------------------------------------
-
-// 8 elements of row `r` of q or k from column c on, zeros past K.
-template <typename T>
-__device__ __forceinline__ Frag<T> ld_row(const T* base, long st, int r, int c, int K) {
-  return frag_of<T>(cut_run(get_run<T, 8>(base + r * st + min(c, K - 8)), c, K));
-}
-
-// A wave has 16 tokens of a chunk as columns: scores (rows: the tokens before them), then outputs
-// (rows: the values), whose lanes hold 8 consecutive values of their token.
-template <typename T, int KP>
-__global__ __launch_bounds__(4 * delta_c<T>()) void delta_out_kernel(DeltaParams p) {
-  constexpr int C = delta_c<T>(), NU = C / 32, NS = KP / 32;
-  __shared__ double sG[C];
-  __shared__ float sRk[C];
-  const tops_gla_delta_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int g = lane >> 4, ci = lane & 15;
-  const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
-  const int chunk = (int)(blockIdx.x / HV), hv = (int)(blockIdx.x % HV);
-  const int h = hv / (HV / (int)a.H);
-  const long unit = blockIdx.x;
-  const ChunkAt at = delta_chunk_at(a, C, chunk);
-  float* vec = delta_vec(p, unit);
-  if (tid < C) {
-    sG[tid] = delta_gsum(p, unit)[tid];
-    sRk[tid] = vec[3 * C + tid];
-  }
-  __syncthreads();
-  if (16 * wave >= at.len) return;
-  const int i = 16 * wave + ci, row = min(i, at.len - 1);   // the last token again past the end
-  const T* q = (const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh;
-  const T* k = (const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh;
-  Frag<T> qf[NS];
-  float qq = 0.f;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    qf[s] = ld_row(q, a.q_st, row, 32 * s + 8 * g, K);
-    float x[8];
-    values_of(qf[s], x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) qq = fmaf(x[e], x[e], qq);
-  }
-  qq = swap32_add(qq, qq);
-  qq = swap16_add(qq, qq);
-  const float rq = a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f, fq = (float)a.scale * rq;
-  if (a.train && lane < 16) vec[4 * C + i] = rq;
-  const float fo = fq * vec[i];
-  const double gi = sG[i];
-  Split<T> pf[NU];   // in two parts: of the three operands of o this one is free to be exact
-#pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    if (32 * u > 16 * wave + 15) continue;
-    f32x4 acc[2] = {zero4(), zero4()};
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
-        mma(acc[hh], ld_row(k, a.k_st, min(32 * u + pair_row(lane, hh), at.len - 1),
-                            32 * s + 8 * g, K), qf[s]);
-    float x[8];
-    pair_values(acc[0], acc[1], x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = 32 * u + 8 * g + e;
-      x[e] = j <= i ? fq * sRk[j] * x[e] * gexp<T>((float)(gi - sG[j])) : 0.f;
-    }
-    pf[u] = split_of<T>(x);
-    T* out = (T*)(p.P + unit * (C * C * 4)) + i * C + 32 * u + 8 * g;
-    if (a.train) {
-      st_frag(out, high_of(pf[u]));
-      if constexpr (sizeof(T) == 2) st_frag(out + C * C, pf[u].lo);
-    }
-  }
-  T* o = (T*)a.o + (((long)at.b * a.T + at.t + i) * HV + hv) * V;
-  const T* S = (const T*)p.S + unit * V * KP + 8 * g;
-  const T* N = (const T*)p.N + unit * V * C + 8 * g;
-  for (int v0 = 0; v0 < V; v0 += 32) {
-    const int va = min(v0 + pair_row(lane, 0), V - 1), vb = min(v0 + pair_row(lane, 1), V - 1);
-    f32x4 acc[2] = {zero4(), zero4()};
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      mma(acc[0], ld_frag(S + (long)va * KP + 32 * s), qf[s]);
-      mma(acc[1], ld_frag(S + (long)vb * KP + 32 * s), qf[s]);
-    }
-    acc[0] *= fo;
-    acc[1] *= fo;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      if (32 * u > 16 * wave + 15) continue;
-      mma(acc[0], ld_frag(N + (long)va * C + 32 * u), pf[u]);
-      mma(acc[1], ld_frag(N + (long)vb * C + 32 * u), pf[u]);
-    }
-    float x[8];
-    pair_values(acc[0], acc[1], x);
-    const int c = v0 + 8 * g;
-    if (i < at.len && c < V) put_run<T, 8>(o + c, x, V - c);
   }
 }
 
@@ -278,7 +180,8 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   const long es = z.dtype == DT_BF16 ? 2 : 4, units = z.chunks * z.HV, segs = z.nsegs * z.HV;
   p.C = delta_chunk_of((int)z.dtype);
   p.KP = delta_key_pad(z.K);
-  p.vec_bytes = 28 * p.C;
+  p.vec_bytes = 36 * p.C;
+  p.tri_bytes = z.dtype == DT_BF16 ? 3 * 1024 * 4 : 1024 * 4;
   p.multi = z.nsegs > z.nseq;
   long at = 0;
   auto take = [&](void* base, long bytes) {
@@ -288,10 +191,10 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   };
   const long ends = p.multi ? segs * z.K * z.V * 4 : 0, maps = p.multi ? segs * p.KP * p.KP * 4 : 0;
   p.vec = take(keep, units * p.vec_bytes);
-  p.Tm = take(keep, units * p.C * p.C * 4);
-  p.N = take(keep, units * z.V * p.C * es);
-  p.S = take(keep, units * z.V * p.KP * es);
-  p.P = take(keep, z.train ? units * p.C * p.C * 4 : 0);
+  p.Tm = take(keep, units * p.tri_bytes);
+  p.P = take(keep, z.train ? units * p.tri_bytes : 0);
+  p.N = take(keep, z.train ? units * z.V * p.C * es : 0);
+  p.S = take(keep, z.train ? units * z.V * p.KP * es : 0);
   p.E = (float*)take(keep, ends);
   p.M = take(keep, maps);
   p.Mt = take(keep, z.train ? maps : 0);
@@ -309,25 +212,12 @@ static hipError_t prep(const DeltaParams& p, hipStream_t st) {
   delta_prep_kernel<T, KP><<<(unsigned)(p.a.chunks * p.a.H), 256, 0, st>>>(p);
   return hipGetLastError();
 }
-template <typename T, int KP>
-static hipError_t out(const DeltaParams& p, hipStream_t st) {
-  delta_out_kernel<T, KP><<<(unsigned)(p.a.chunks * p.a.HV), 4 * delta_c<T>(), 0, st>>>(p);
-  return hipGetLastError();
-}
-
 hipError_t run_delta_prep(const DeltaParams& p, hipStream_t st) {
   if (p.a.dtype == DT_BF16)
     return p.KP == 64 ? prep<bf16, 64>(p, st) : p.KP == 128 ? prep<bf16, 128>(p, st)
                                                             : prep<bf16, 256>(p, st);
   return p.KP == 64 ? prep<float, 64>(p, st) : p.KP == 128 ? prep<float, 128>(p, st)
                                                            : prep<float, 256>(p, st);
-}
-hipError_t run_delta_out(const DeltaParams& p, hipStream_t st) {
-  if (p.a.dtype == DT_BF16)
-    return p.KP == 64 ? out<bf16, 64>(p, st) : p.KP == 128 ? out<bf16, 128>(p, st)
-                                                           : out<bf16, 256>(p, st);
-  return p.KP == 64 ? out<float, 64>(p, st) : p.KP == 128 ? out<float, 128>(p, st)
-                                                          : out<float, 256>(p, st);
 }
 
 }  // namespace tops

@@ -56,29 +56,35 @@ __device__ __forceinline__ SegAt seg_at(const tops_gla_delta_args& a, int C, int
   return x;
 }
 
-// Blocks of a head: NW waves of 16 CW columns each, of V or, in a first pass, then of KP for M.
-template <typename T, int KP, int CW, int NW>
+// A head's columns go to blocks of NW waves of 16, of V or, in a first pass, then of KP for M.
+template <typename T, int KP, int NW>
 struct ScanShape {
-  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1, COLS = 16 * CW * NW;
-  static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(C), PV = pitch_of<T>(COLS);
-  static constexpr int NT = 64 * NW;
+  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1, COLS = 16 * NW;
+  static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(32), PV = pitch_of<T>(COLS);
+  static constexpr int NT = 64 * NW, TRI = PARTS * delta_blocks<T>() * 32;   // rows of Tm or P
+  static constexpr int LO = delta_blocks<T>() * 32 * PT;   // from a high part to its low part
+};
+constexpr int LDS_MOST = 160 * 1024;
+
+// FIRST: the first pass, which has E (and M) and no outputs.
+template <typename T, int KP, int NW, bool FIRST>
+struct ScanLds : ScanShape<T, KP, NW> {
+  using B = ScanShape<T, KP, NW>;
+  static constexpr int C = B::C, ES = (int)sizeof(T);
+  static constexpr int K0 = 0, T0 = C * B::PK, V0 = T0 + B::TRI * B::PT, END = V0 + C * B::PV;
+  static constexpr int F0 = END * ES;   // five vectors of floats
+  static constexpr int ONE = F0 + 5 * C * 4;
+  // the scores' part: q, P, the sums of log decays, 1 / |q|
+  static constexpr int Q0 = 0, P0 = C * B::PK, G0 = (P0 + B::TRI * B::PT) * ES, R0 = G0 + 8 * C;
+  static constexpr int REST = FIRST ? 0 : R0 + 4 * C;
+  static constexpr int BUFS = 2 * ONE + REST <= LDS_MOST ? 2 : 1;   // of the chunk's tiles
+  static constexpr int BYTES = BUFS * ONE + REST;
+  static_assert(BYTES <= LDS_MOST && ONE % 16 == 0 && G0 % 8 == 0, "LDS");
 };
 
-template <typename T, int KP, int CW, int NW>
-struct ScanLds : ScanShape<T, KP, CW, NW> {
-  using B = ScanShape<T, KP, CW, NW>;
-  static constexpr int C = B::C;
-  static constexpr int K0 = 0, T0 = C * B::PK, V0 = T0 + B::PARTS * C * B::PT,
-                       END = V0 + C * B::PV;
-  static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
-  static constexpr int ONE = (F0 + (3 * C + 1) * 4 + 15) / 16 * 16;   // one of two buffers
-  static constexpr int BYTES = 2 * ONE;
-};
-
-// FIRST: the first pass, which has E (and M) and leaves no states of chunks.
-template <typename T, int KP, int CW, int NW, bool FIRST>
+template <typename T, int KP, int NW, bool FIRST>
 __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
-  using L = ScanLds<T, KP, CW, NW>;
+  using L = ScanLds<T, KP, NW, FIRST>;
   constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, COLS = L::COLS;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
@@ -95,14 +101,15 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   if (FIRST && (at.j + 1 >= at.count || (map && at.j == 0))) return;   // nobody asks for these
   const int nc = at.n;
   const T* kp = (const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh;
+  const T* qp = (const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh;
   // the block's columns; the last block's few may begin before them, where there are fewer than 8
   const int vc = map ? COLS : V - vb * COLS;
   const T* vp = (const T*)a.v + at.b * a.v_sb + at.t * a.v_st + hv * a.v_sh + (map ? 0 : vb * COLS);
-  const int w0 = 16 * CW * wave, v0 = (map ? vb - vt : vb) * COLS + w0 + ci;
-  const int width = map ? KP : V;
-  const bool idle = v0 - ci >= width;   // a wave past the columns only helps with the tiles
+  const int w0 = 16 * wave, v = (map ? vb - vt : vb) * COLS + w0 + ci;
+  const bool idle = v - ci >= (map ? KP : V);   // a wave past the columns only helps with the tiles
+  const bool vin = v < V;
 
-  f32x4 S[CW][2 * NS];
+  f32x4 S[2 * NS];
   const float* from = nullptr;
   if (at.j > 0) {
     if (!FIRST) from = p.E + ((long)(at.seg - 1) * HV + hv) * K * V;
@@ -110,45 +117,51 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     from = a.h0 + ((long)at.seq * HV + hv) * K * V;
   }
 #pragma unroll
-  for (int c = 0; c < CW; ++c) {
-    const int v = v0 + 16 * c;
+  for (int i = 0; i < 2 * NS; ++i)
 #pragma unroll
-    for (int i = 0; i < 2 * NS; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S[c][i][r] = map && v == 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r ? 1.f : 0.f;
-    if (from && !map) load_state(S[c], from + min(v, V - 1), v < V, g, K, V);
-  }
+    for (int r = 0; r < 4; ++r)
+      S[i][r] = map && v == 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r ? 1.f : 0.f;
+  if (from && !map) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
-  TileStream<T, C, KP, NT> fk(a.k_st, K, tid);
-  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
+  TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
+  TileStream<T, L::TRI, 32, NT> ft(32, 32, tid);
   TileStream<T, C, COLS, NT> fv(a.v_st, min(vc, V), tid);
-  constexpr int NF = (3 * C + NT) / NT;
-  float ff[NF], fr[NF];
+  constexpr int NF = (5 * C + NT - 1) / NT;
+  float ff[NF];
+  double fg = 0.;
   auto fetch = [&](int n) {
     const int len = min(C, at.T - n * C);
     const long unit = (long)(at.chunk + n) * HV + hv;
     fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
+    ft.next((const T*)(p.Tm + unit * p.tri_bytes), 32, L::TRI, 32, tid);
     if (!map) fv.next(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {   // e^G / |k|, e^{G_C - G} / |k|, beta, e^{G_C}
-      const int x = i * NT + tid;
-      ff[i] = vec[x < 3 * C ? x : C - 1];
-      fr[i] = vec[3 * C + x % C];
+    for (int i = 0; i < NF; ++i) ff[i] = vec[min(i * NT + tid, 5 * C - 1)];
+    if (!FIRST) {
+      fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
+      fg = delta_gsum(p, unit)[min(tid, C - 1)];
     }
   };
+  unsigned char* rest = smem + L::BUFS * L::ONE;
+  T *sQ = (T*)rest + L::Q0, *sP = (T*)rest + L::P0;
+  double* sG = (double*)(rest + L::G0);
+  float* sRq = (float*)(rest + L::R0);
   auto put = [&](int n) {
-    T* sm = (T*)(smem + (n & 1) * L::ONE);
+    unsigned char* buf = smem + n % L::BUFS * L::ONE;
+    T* sm = (T*)buf;
     const int len = min(C, at.T - n * C);
     fk.put(sm + L::K0, L::PK, len, K, tid);
-    ft.put(sm + L::T0, L::PT, L::PARTS * C, C, tid);
+    ft.put(sm + L::T0, L::PT, L::TRI, 32, tid);
     fv.put(sm + L::V0, L::PV, map ? 0 : len, vc, tid);
-    float* sf = (float*)(smem + (n & 1) * L::ONE + L::F0);
+    float* sf = (float*)(buf + L::F0);
 #pragma unroll
     for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = i * NT + tid < 2 * C ? ff[i] * fr[i] : ff[i];
+      if (i * NT + tid < 5 * C) sf[i * NT + tid] = ff[i];
+    if (!FIRST) {
+      fq.put(sQ, L::PK, len, K, tid);
+      if (tid < C) sG[tid] = fg;
+    }
   };
   if (nc > 0) {
     fetch(0);
@@ -157,127 +170,201 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   for (int n = 0; n < nc; ++n) {
     __syncthreads();
     if (n + 1 < nc) fetch(n + 1);
-    const T* sm = (const T*)(smem + (n & 1) * L::ONE);
-    const T *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + w0;
-    const float* sf = (const float*)(smem + (n & 1) * L::ONE + L::F0);
-    const long unit = (long)(at.chunk + n) * HV + hv;
-    const float last = sf[3 * C];
+    const unsigned char* buf = smem + n % L::BUFS * L::ONE;
+    const T *sm = (const T*)buf, *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + w0;
+    const float* sf = (const float*)(buf + L::F0);   // e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|,
+    const long unit = (long)(at.chunk + n) * HV + hv;   // e^G
+    const float last = sf[5 * C - 1];
+    if (!FIRST) {
+      // The scores of 16 tokens (columns) with 32 before or among them (rows), item after item of the
+      // lower ones: a lane has 8 in a row of P.
+      constexpr int ITEMS = NU == 2 ? 6 : 2;
+      for (int it = wave; it < ITEMS; it += NW) {
+        const int u = it == 4 || it == 5, tile = it < 4 ? it : it - 2, i = 16 * tile + ci;
+        f32x4 acc[2] = {zero4(), zero4()};
+        float qq = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const Frag<T> qf = ld_frag(sQ + i * L::PK + 32 * s + 8 * g);
+          float x[8];
+          values_of(qf, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qq = fmaf(x[e], x[e], qq);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            mma(acc[x], ld_frag(sK + (32 * u + pair_row(lane, x)) * L::PK + 32 * s + 8 * g), qf);
+        }
+        qq = swap32_add(qq, qq);
+        qq = swap16_add(qq, qq);
+        const float rq = a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f, fq = (float)a.scale * rq;
+        if (u == 0 && g == 0) {
+          sRq[i] = rq;
+          if (a.train && vb == 0) delta_vec(p, unit)[6 * C + i] = rq;
+        }
+        const double gi = sG[i];
+        float x[8];
+        pair_values(acc[0], acc[1], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = 32 * u + 8 * g + e;
+          x[e] = j <= i ? fq * sf[3 * C + j] * x[e] * gexp<T>((float)(gi - sG[j])) : 0.f;
+        }
+        // in two parts: of the three operands of o this one is the cheapest to have exact
+        const Split<T> f = split_of<T>(x);
+        const int row = 32 * tri_block(tile / 2, u) + i % 32;
+        T* out = (T*)(p.P + unit * p.tri_bytes) + row * 32 + 8 * g;
+        st_frag(sP + row * L::PT + 8 * g, high_of(f));
+        if (a.train && vb == 0) st_frag(out, high_of(f));
+        if constexpr (sizeof(T) == 2) {
+          st_frag(sP + L::LO + row * L::PT + 8 * g, f.lo);
+          if (a.train && vb == 0) st_frag(out + delta_blocks<T>() * 1024, f.lo);
+        }
+      }
+    }
+    f32x4 acc[2 * NU], o[FIRST ? 1 : 2 * NU];
+    Frag<T> nf[NU];
     if (!idle) {
-      f32x4 acc[CW][2 * NU];
 #pragma unroll
-      for (int c = 0; c < CW; ++c)
-#pragma unroll
-        for (int i = 0; i < 2 * NU; ++i) acc[c][i] = zero4();
+      for (int i = 0; i < 2 * NU; ++i) acc[i] = o[FIRST ? 0 : i] = zero4();
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        Split<T> f[CW];
-#pragma unroll
-        for (int c = 0; c < CW; ++c) {
-          float x[8];
-          pair_values(S[c][2 * s], S[c][2 * s + 1], x);
-          f[c] = split_of<T>(x);
-          if (!FIRST && v0 + 16 * c < V)
-            st_frag((T*)p.S + (unit * V + v0 + 16 * c) * KP + 32 * s + 8 * g, high_of(f[c]));
-        }
+        float x[8];
+        pair_values(S[2 * s], S[2 * s + 1], x);
+        const Split<T> f = split_of<T>(x);
         mma_rows(acc, [&](int i) {
           return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
         }, f);
-      }
-      Split<T> R[NU][CW];
+        if constexpr (!FIRST) {
+          if (a.train && vin)
+            st_frag((T*)p.S + (unit * V + v) * KP + 32 * s + 8 * g, high_of(f));
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int c = 0; c < CW; ++c) {
-          float x[8], y[8];
-          values_of(ld_frag_t(sV + 16 * c + 32 * u * L::PV, L::PV, lane), y);
-          pair_values(acc[c][2 * u], acc[c][2 * u + 1], x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int t = 32 * u + 8 * g + e;
-            x[e] = sf[2 * C + t] * (y[e] - sf[t] * x[e]);
-          }
-          R[u][c] = split_of<T>(x);
+          for (int i = 0; i < 2 * NU; ++i)
+            mma(o[i],
+                ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g),
+                high_of(f));
         }
-#pragma unroll
-      for (int c = 0; c < CW; ++c)
-#pragma unroll
-        for (int i = 0; i < 2 * NU; ++i) acc[c][i] = zero4();
-#pragma unroll
-      for (int w = 0; w < NU; ++w)
-        mma_split_rows(acc, [&](int i) {
-          return ld_split<T>(sT, C * L::PT, (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PT +
-                                                32 * w + 8 * g);
-        }, [&](int i) { return w <= (i >> 1); }, R[w]);
-#pragma unroll
-      for (int c = 0; c < CW; ++c)
-#pragma unroll
-        for (int i = 0; i < 2 * NS; ++i) S[c][i] *= last;
+      }
+      Split<T> R[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        Split<T> f[CW];
+        float x[8], y[8];
+        values_of(ld_frag_t(sV + 32 * u * L::PV, L::PV, lane), y);
+        pair_values(acc[2 * u], acc[2 * u + 1], x);
 #pragma unroll
-        for (int c = 0; c < CW; ++c) {
-          float x[8];
-          pair_values(acc[c][2 * u], acc[c][2 * u + 1], x);
-          if (!FIRST && v0 + 16 * c < V)
-            st_frag((T*)p.N + (unit * V + v0 + 16 * c) * C + 32 * u + 8 * g, frag_of<T>(x));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
-          f[c] = split_of<T>(x);
+        for (int e = 0; e < 8; ++e) {
+          const int t = 32 * u + 8 * g + e;
+          x[e] = sf[2 * C + t] * (y[e] - sf[t] * x[e]);
         }
+        R[u] = split_of<T>(x);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
+#pragma unroll
+      for (int w = 0; w < NU; ++w)
+#pragma unroll
+        for (int u = w; u < NU; ++u)
+          mma_split_pair(acc, u, [&](int x) {
+            return ld_split<T>(sT, L::LO,
+                               (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
+          }, R[w]);
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        float x[8];
+        pair_values(acc[2 * u], acc[2 * u + 1], x);
+        if constexpr (!FIRST) {
+          nf[u] = frag_of<T>(x);
+          if (a.train && vin) st_frag((T*)p.N + (unit * V + v) * C + 32 * u + 8 * g, nf[u]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
         mma_rows(S, [&](int i) {
           return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-        }, f);
+        }, split_of<T>(x));
       }
     }
-    if (n + 1 < nc) put(n + 1);
-  }
-  if (idle) return;
+    if constexpr (!FIRST) {
+      __syncthreads();   // the scores are there
+      if (!idle) {
+        const int len = min(C, at.T - n * C);
+        T* to = (T*)a.o + (((long)at.b * a.T + at.t + n * C) * HV + hv) * V + v;
 #pragma unroll
-  for (int c = 0; c < CW; ++c) {
-    const int v = v0 + 16 * c;
-    if (map) {   // [KP][KP]: column v, rows in the lane's order
-      const long tile = (long)KP * KP;
-      T* M = (T*)(p.M + ((long)at.seg * HV + hv) * tile * 4);
-      T* Mt = (T*)(p.Mt + ((long)at.seg * HV + hv) * tile * 4);
+        for (int u = 0; u < NU; ++u) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        float x[8], y[8];
-        pair_values(S[c][2 * s], S[c][2 * s + 1], x);
-        const Split<T> f = split_of<T>(x);
-        if (a.train) st_frag(Mt + v * KP + 32 * s + 8 * g, high_of(f));
-        values_of(high_of(f), y);
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) M[(32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
-        if constexpr (sizeof(T) == 2) {
-          if (a.train) st_frag(Mt + tile + v * KP + 32 * s + 8 * g, f.lo);
-          values_of(f.lo, y);
+            for (int r = 0; r < 4; ++r) {
+              const int t = 32 * u + 8 * g + 4 * x + r;
+              o[2 * u + x][r] *= (float)a.scale * sRq[t] * sf[4 * C + t];
+            }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) M[tile + (32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
+          for (int w = 0; w <= u; ++w)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              mma(o[2 * u + x],
+                  ld_split<T>(sP, L::LO,
+                              (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g), nf[w]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int t = 32 * u + 8 * g + 4 * x + r;
+              if (vin && t < len) to[(long)t * HV * V] = from_f32<T>(o[2 * u + x][r]);
+            }
         }
       }
-    } else if (FIRST) {
-      store_state(S[c], p.E + ((long)at.seg * HV + hv) * K * V + v, v < V, g, K, V);
-    } else if (a.ht && at.j + 1 == at.count) {
-      store_state(S[c], a.ht + ((long)at.seq * HV + hv) * K * V + v, v < V, g, K, V);
     }
+    if (n + 1 < nc) {
+      // the scores' tiles have been read (their barrier is behind, or there is none of them); with
+      // one buffer, so must the chunk's be
+      if (L::BUFS == 1) __syncthreads();
+      put(n + 1);
+    }
+  }
+  if (idle) return;
+  if (map) {   // [KP][KP]: column v, rows in the lane's order
+    const long tile = (long)KP * KP;
+    T* M = (T*)(p.M + ((long)at.seg * HV + hv) * tile * 4);
+    T* Mt = (T*)(p.Mt + ((long)at.seg * HV + hv) * tile * 4);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      float x[8], y[8];
+      pair_values(S[2 * s], S[2 * s + 1], x);
+      const Split<T> f = split_of<T>(x);
+      if (a.train) st_frag(Mt + v * KP + 32 * s + 8 * g, high_of(f));
+      values_of(high_of(f), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) M[(32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
+      if constexpr (sizeof(T) == 2) {
+        if (a.train) st_frag(Mt + tile + v * KP + 32 * s + 8 * g, f.lo);
+        values_of(f.lo, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) M[tile + (32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
+      }
+    }
+  } else if (FIRST) {
+    store_state(S, p.E + ((long)at.seg * HV + hv) * K * V + v, vin, g, K, V);
+  } else if (a.ht && at.j + 1 == at.count) {
+    store_state(S, a.ht + ((long)at.seq * HV + hv) * K * V + v, vin, g, K, V);
   }
 }
 
-template <typename T, int KP, int CW, int NW>
-struct DscanLds : ScanShape<T, KP, CW, NW> {
-  using B = ScanShape<T, KP, CW, NW>;
+template <typename T, int KP, int NW>
+struct DscanLds : ScanShape<T, KP, NW> {
+  using B = ScanShape<T, KP, NW>;
   static constexpr int C = B::C;
-  static constexpr int K0 = 0, Q0 = C * B::PK, T0 = 2 * C * B::PK, P0 = T0 + B::PARTS * C * B::PT;
-  static constexpr int V0 = P0 + B::PARTS * C * B::PT, END = V0 + C * B::PV;
+  static constexpr int K0 = 0, Q0 = C * B::PK, T0 = 2 * C * B::PK, P0 = T0 + B::TRI * B::PT;
+  static constexpr int V0 = P0 + B::TRI * B::PT, END = V0 + C * B::PV;
   static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
   static constexpr int BYTES = F0 + (3 * C + 1) * 4;
+  static_assert(BYTES <= LDS_MOST, "LDS");
 };
 
-template <typename T, int KP, int CW, int NW, bool FIRST>
+template <typename T, int KP, int NW, bool FIRST>
 __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
-  using L = DscanLds<T, KP, CW, NW>;
-  constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, COLS = L::COLS, LO = C * L::PT;
+  using L = DscanLds<T, KP, NW>;
+  constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, COLS = L::COLS;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -295,10 +382,10 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   const T* qp = (const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh;
   const int vc = V - vb * COLS;
   const T* dp = (const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh + vb * COLS;
-  const int w0 = 16 * CW * wave, v0 = vb * COLS + w0 + ci;
-  const bool idle = v0 - ci >= V;
+  const int w0 = 16 * wave, v = vb * COLS + w0 + ci;
+  const bool idle = v - ci >= V, vin = v < V;
 
-  f32x4 S[CW][2 * NS];   // dS, as the forward's states
+  f32x4 S[2 * NS];   // dS, as the forward's states
   const float* from = nullptr;
   if (at.j + 1 < at.count) {
     if (!FIRST) from = p.dE + ((long)(at.seg + 1) * HV + hv) * K * V;
@@ -306,15 +393,11 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     from = a.dht + ((long)at.seq * HV + hv) * K * V;
   }
 #pragma unroll
-  for (int c = 0; c < CW; ++c) {
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) S[c][i] = zero4();
-    if (from) load_state(S[c], from + min(v0 + 16 * c, V - 1), v0 + 16 * c < V, g, K, V);
-  }
+  for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
+  if (from) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  TileStream<T, L::PARTS * C, C, NT> ft(C, C, tid);
-  TileStream<T, C, C, NT> fp[2] = {{C, C, tid}, {C, C, tid}};
+  TileStream<T, L::TRI, 32, NT> ft(32, 32, tid), fp(32, 32, tid);
   TileStream<T, C, COLS, NT> fd(a.do_st, vc, tid);
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
@@ -323,18 +406,15 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     const long unit = (long)(at.chunk + n) * HV + hv;
     fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
     fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * (C * C * 4)), C, L::PARTS * C, C, tid);
-#pragma unroll
-    for (int i = 0; i < L::PARTS; ++i)   // rows past the end have not been written
-      fp[i].next((const T*)(p.P + unit * (C * C * 4)) + i * C * C, C, len, C, tid);
+    ft.next((const T*)(p.Tm + unit * p.tri_bytes), 32, L::TRI, 32, tid);
+    fp.next((const T*)(p.P + unit * p.tri_bytes), 32, L::TRI, 32, tid);
     fd.next(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|
+    for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|; e^{G_C}
       const int x = i * NT + tid, t = x % C;
-      const float e = vec[t + (x < C ? C : 0)], r = vec[t + (x < 2 * C ? 3 * C : 4 * C)];
-      ff[i] = x < 3 * C ? e * r : vec[C - 1];
-      fr[i] = x < C ? 1.f : x < 2 * C ? vec[2 * C + t] : x < 3 * C ? (float)a.scale : 1.f;
+      ff[i] = vec[x < C ? C + t : x < 2 * C ? t : x < 3 * C ? 4 * C + t : 5 * C - 1];
+      fr[i] = vec[x < 2 * C ? 2 * C + t : 6 * C + t];
     }
   };
   T* sm = (T*)smem;
@@ -346,116 +426,89 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     const int len = min(C, at.T - n * C);
     fk.put(sK, L::PK, len, K, tid);
     fq.put(sQ, L::PK, len, K, tid);
-    ft.put(sT, L::PT, L::PARTS * C, C, tid);
-#pragma unroll
-    for (int i = 0; i < L::PARTS; ++i) fp[i].put(sP + i * LO, L::PT, len, C, tid);
+    ft.put(sT, L::PT, L::TRI, 32, tid);
+    fp.put(sP, L::PT, L::TRI, 32, tid);
     fd.put(sV, L::PV, len, vc, tid);
 #pragma unroll
-    for (int i = 0; i < NF; ++i)
-      if (i * NT + tid <= 3 * C) sf[i * NT + tid] = ff[i] * fr[i];
+    for (int i = 0; i < NF; ++i) {
+      const int x = i * NT + tid;
+      if (x <= 3 * C)
+        sf[x] = x < C || x == 3 * C ? ff[i] : ff[i] * fr[i] * (x < 2 * C ? 1.f : (float)a.scale);
+    }
     __syncthreads();
     if (n > 0) fetch(n - 1);
     if (idle) continue;
     const long unit = (long)(at.chunk + n) * HV + hv;
     const float last = sf[3 * C];
 
-    f32x4 acc[CW][2 * NU];
+    f32x4 acc[2 * NU];
 #pragma unroll
-    for (int c = 0; c < CW; ++c)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i) acc[c][i] = zero4();
+    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      Split<T> f[CW];
-#pragma unroll
-      for (int c = 0; c < CW; ++c) {
-        float x[8];
-        pair_values(S[c][2 * s], S[c][2 * s + 1], x);
-        f[c] = split_of<T>(x);
-        if (!FIRST && v0 + 16 * c < V)
-          st_frag((T*)p.dS + (unit * V + v0 + 16 * c) * KP + 32 * s + 8 * g, high_of(f[c]));
-      }
+      float x[8];
+      pair_values(S[2 * s], S[2 * s + 1], x);
+      const Split<T> f = split_of<T>(x);
+      if (!FIRST && vin) st_frag((T*)p.dS + (unit * V + v) * KP + 32 * s + 8 * g, high_of(f));
       mma_rows(acc, [&](int i) {
         return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
       }, f);
     }
-    Frag<T> df[NU][CW];
+    Frag<T> df[NU];
 #pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-      for (int c = 0; c < CW; ++c)
-        df[u][c] = ld_frag_t(sV + w0 + 16 * c + 32 * u * L::PV, L::PV, lane);
+    for (int u = 0; u < NU; ++u) df[u] = ld_frag_t(sV + w0 + 32 * u * L::PV, L::PV, lane);
 #pragma unroll
     for (int i = 0; i < 2 * NU; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float d = sf[32 * (i >> 1) + 8 * g + 4 * (i & 1) + r];
-#pragma unroll
-        for (int c = 0; c < CW; ++c) acc[c][i][r] *= d;
-      }
-#pragma unroll
-    for (int w = 0; w < NU; ++w)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i)
-        if (w >= (i >> 1)) {
-          const Split<T> f =
-              ld_split_t<T>(sP + 32 * w * L::PT + 32 * (i >> 1), LO, L::PT, lane, i & 1);
-#pragma unroll
-          for (int c = 0; c < CW; ++c) mma(acc[c][i], f, df[w][c]);
-        }
-    Split<T> R[NU][CW];
+      for (int r = 0; r < 4; ++r) acc[i][r] *= sf[32 * (i >> 1) + 8 * g + 4 * (i & 1) + r];
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
-      for (int c = 0; c < CW; ++c) {
-        float x[8];
-        pair_values(acc[c][2 * u], acc[c][2 * u + 1], x);
-        R[u][c] = split_of<T>(x);
-      }
+      for (int w = 0; w <= u; ++w)
 #pragma unroll
-    for (int c = 0; c < CW; ++c)
-#pragma unroll
-      for (int i = 0; i < 2 * NU; ++i) acc[c][i] = zero4();
-#pragma unroll
-    for (int w = 0; w < NU; ++w)
-      mma_split_rows(acc, [&](int i) {
-        return ld_split_t<T>(sT + 32 * w * L::PT + 32 * (i >> 1), LO, L::PT, lane, i & 1);
-      }, [&](int i) { return w >= (i >> 1); }, R[w]);
-#pragma unroll
-    for (int c = 0; c < CW; ++c)
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) S[c][i] *= last;
+        for (int x = 0; x < 2; ++x)
+          mma(acc[2 * w + x],
+              ld_split_t<T>(sP + 32 * tri_block(u, w) * L::PT, L::LO, L::PT, lane, x), df[u]);
+    Split<T> R[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      Split<T> fo[CW], fy[CW];
+      float x[8];
+      pair_values(acc[2 * u], acc[2 * u + 1], x);
+      R[u] = split_of<T>(x);
+    }
 #pragma unroll
-      for (int c = 0; c < CW; ++c) {
-        float x[8];
-        values_of(df[u][c], x);
+    for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= sf[2 * C + 32 * u + 8 * g + e];
-        fo[c] = split_of<T>(x);
-        pair_values(acc[c][2 * u], acc[c][2 * u + 1], x);
-        if (!FIRST && v0 + 16 * c < V)
-          st_frag((T*)p.Y + (unit * V + v0 + 16 * c) * C + 32 * u + 8 * g, frag_of<T>(x));
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
-        fy[c] = split_of<T>(x);
-      }
+      for (int w = 0; w <= u; ++w)
+        mma_split_pair(acc, w, [&](int x) {
+          return ld_split_t<T>(sT + 32 * tri_block(u, w) * L::PT, L::LO, L::PT, lane, x);
+        }, R[u]);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      float x[8];
+      values_of(df[u], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= sf[2 * C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {
         return ld_pair_t(sQ + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, fo);
+      }, split_of<T>(x));
+      pair_values(acc[2 * u], acc[2 * u + 1], x);
+      if (!FIRST && vin) st_frag((T*)p.Y + (unit * V + v) * C + 32 * u + 8 * g, frag_of<T>(x));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {
         return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, fy);
+      }, split_of<T>(x));
     }
   }
   if (idle) return;
   float* to = FIRST ? p.dE + ((long)at.seg * HV + hv) * K * V
               : a.dh0 && at.j == 0 ? a.dh0 + ((long)at.seq * HV + hv) * K * V : nullptr;
-#pragma unroll
-  for (int c = 0; c < CW; ++c)
-    if (to) store_state(S[c], to + v0 + 16 * c, v0 + 16 * c < V, g, K, V);
+  if (to) store_state(S, to + v, vin, g, K, V);
 }
 
 // E_j <- M_j E_{j-1} + E_j along the segments of a sequence and head, or dE_j <- M_j^T dE_{j+1} +
@@ -541,45 +594,45 @@ __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaP
   }
 }
 
-template <typename T, int KP, int CW, int NW, bool BACK, bool FIRST>
+template <typename T, int KP, int NW, bool BACK, bool FIRST>
 hipError_t launch(const DeltaParams& p, hipStream_t st) {
-  using S = ScanShape<T, KP, CW, NW>;
-  constexpr int lds = BACK ? (int)DscanLds<T, KP, CW, NW>::BYTES : (int)ScanLds<T, KP, CW, NW>::BYTES;
+  using S = ScanShape<T, KP, NW>;
+  constexpr int lds = BACK ? (int)DscanLds<T, KP, NW>::BYTES : (int)ScanLds<T, KP, NW, FIRST>::BYTES;
   const void* f;
   if constexpr (BACK)
-    f = (const void*)delta_dscan_kernel<T, KP, CW, NW, FIRST>;
+    f = (const void*)delta_dscan_kernel<T, KP, NW, FIRST>;
   else
-    f = (const void*)delta_scan_kernel<T, KP, CW, NW, FIRST>;
+    f = (const void*)delta_scan_kernel<T, KP, NW, FIRST>;
   const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   const long cols = (p.a.V + S::COLS - 1) / S::COLS +
                     (FIRST && !BACK ? (KP + S::COLS - 1) / S::COLS : 0);
   const unsigned grid = (unsigned)(cols * p.a.HV * p.a.nsegs);
   if constexpr (BACK)
-    delta_dscan_kernel<T, KP, CW, NW, FIRST><<<grid, S::NT, lds, st>>>(p);
+    delta_dscan_kernel<T, KP, NW, FIRST><<<grid, S::NT, lds, st>>>(p);
   else
-    delta_scan_kernel<T, KP, CW, NW, FIRST><<<grid, S::NT, lds, st>>>(p);
+    delta_scan_kernel<T, KP, NW, FIRST><<<grid, S::NT, lds, st>>>(p);
   return hipGetLastError();
 }
 
-template <typename T, int KP, int CW, int NW, bool BACK>
+template <typename T, int KP, int NW, bool BACK>
 hipError_t passes(const DeltaParams& p, hipStream_t st) {
   if (p.multi) {
-    if (const hipError_t e = launch<T, KP, CW, NW, BACK, true>(p, st)) return e;
+    if (const hipError_t e = launch<T, KP, NW, BACK, true>(p, st)) return e;
     const unsigned grid = (unsigned)((p.a.V + 15) / 16 * p.a.HV * p.a.nseq);
     delta_fold_kernel<T, KP, BACK><<<grid, KP == 64 ? 128 : 256, 0, st>>>(p);
     if (const hipError_t e = hipGetLastError()) return e;
   }
-  return launch<T, KP, CW, NW, BACK, false>(p, st);
+  return launch<T, KP, NW, BACK, false>(p, st);
 }
 
 template <typename T, int KP, bool BACK>
 hipError_t run(const DeltaParams& p, hipStream_t st) {
-  // two lots of 16 columns a wave read each of the chunk's tiles once for both; with 256 keys their
-  // states do not fit the registers
+  // eight waves a block share the chunk's tiles, two waves a SIMD; with 256 keys a wave's state
+  // leaves no room for a second one
   if constexpr (KP < 256)
-    if (p.a.V > 64) return passes<T, KP, 1, 8, BACK>(p, st);
-  return passes<T, KP, 1, 4, BACK>(p, st);
+    if (p.a.V > 64) return passes<T, KP, 8, BACK>(p, st);
+  return passes<T, KP, 4, BACK>(p, st);
 }
 template <typename T, int KP>
 hipError_t run(const DeltaParams& p, bool back, hipStream_t st) {
