@@ -89,8 +89,8 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
       !grid_fits((a->V / 16 + 1) * a->HV * a->nseq, 64))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   // offsets within a chunk are 32 bits of bytes
-  for (int64_t st : {a->q_st, a->k_st, a->v_st, backward ? a->do_st : 0})
-    if (st >= (1 << 24) || st <= -(1 << 24))
+  for (int64_t st : {a->q_st, a->k_st, a->v_st, backward ? a->do_st : 0, a->HV * a->V})
+    if (st < 0 || st >= (1 << 24))
       return fail(TOPS_GLA_EUNSUPPORTED, "tokens must lie less than 2^24 elements apart (%lld)",
                   (long long)st);
   if (a->chunks > 0 && any_null({a->q, a->k, a->v, a->g, a->beta}))

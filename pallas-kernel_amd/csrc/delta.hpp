@@ -316,59 +316,137 @@ __device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, floa
   for (int r = 0; r < 4; ++r) x[r] = a[r], x[4 + r] = b[r];
 }
 
+// A value that is there whatever becomes of it: a choice made with it needs no branch around what it
+// comes from (the compiler puts LDS reads and exponentials into such branches, one wait for each).
+__device__ __forceinline__ float pinned(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// 8 floats in a row in LDS, 16-byte aligned.
+__device__ __forceinline__ void ld_eight(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = pinned(a.x), x[1] = pinned(a.y), x[2] = pinned(a.z), x[3] = pinned(a.w);
+  x[4] = pinned(b.x), x[5] = pinned(b.y), x[6] = pinned(b.z), x[7] = pinned(b.w);
+}
+// e^{sign (G - Gj)} for 8 tokens j in a row.
+template <typename T>
+__device__ __forceinline__ void decays(double G, const double* Gj, float sign, float (&d)[8]) {
+  double y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = G - Gj[e];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] = pinned(gexp<T>(sign * (float)y[e]));
+}
+
+// 8 elements at any address of theirs, as whole registers (loads of them are not taken apart).
+template <typename T>
+struct Piece;
+template <>
+struct Piece<bf16> {
+  typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+  u32x4_t x;
+  __device__ __forceinline__ void get(const void* base, uint32_t off) {
+    x = *reinterpret_cast<const Any*>((const char*)base + off);
+  }
+  __device__ __forceinline__ Frag<bf16> frag() const {
+    Frag<bf16> f;
+    f.d = make_uint4(x[0], x[1], x[2], x[3]);
+    return f;
+  }
+};
+template <>
+struct Piece<float> {
+  typedef float Any __attribute__((ext_vector_type(4), aligned(4)));
+  f32x4 x, y;
+  __device__ __forceinline__ void get(const void* base, uint32_t off) {
+    x = *reinterpret_cast<const Any*>((const char*)base + off);
+    y = *reinterpret_cast<const Any*>((const char*)base + off + 16);
+  }
+  __device__ __forceinline__ Frag<float> frag() const {
+    Frag<float> f;
+    f.a = make_float4(x[0], x[1], x[2], x[3]);
+    f.b = make_float4(y[0], y[1], y[2], y[3]);
+    return f;
+  }
+};
+template <typename T>
+using Eight = Run<T, 8>;
+template <typename T>
+__device__ __forceinline__ Frag<T> cut_frag(const Frag<T>& f, int c, int cols) {
+  return __builtin_bit_cast(Frag<T>, cut_run(__builtin_bit_cast(Eight<T>, f), c, cols));
+}
+
 // A [C][W] tile on its way to LDS in pieces of 8 elements. The loads have no conditions, so that
 // they are all on their way at once: a piece past the tile's rows or columns loads one inside.
 // `put` zeroes what is past `len` rows and `cols` columns. Fewer than 8 columns may be left of rows
-// that hold 8 at least: the load then begins before them. Offsets are 32 bits of bytes from a base
-// that is the same for all lanes (rows lie less than 2^24 elements apart).
+// that hold 8 at least: the load then begins before them. Offsets are 32 bits of bytes, without a
+// sign, from a base that is the same for all lanes, 8 elements before the tile: the least of them is
+// one element (rows lie at least 0 and less than 2^24 elements apart).
 template <typename T, int C, int W, int NT>
 struct TileFetch {
   static constexpr int PER = C * W / 8, N = (PER + NT - 1) / NT;
-  Run<T, 8> r[N];
-  __device__ __forceinline__ static int offset(int i, int st, int len, int cols, int tid) {
-    const int p = i * NT + tid;
-    return (min(p / (W / 8), len - 1) * st + min(p % (W / 8) * 8, cols - 8)) * (int)sizeof(T);
+  static constexpr uint32_t ES = sizeof(T);
+  Piece<T> r[N];
+  __device__ __forceinline__ static int row_of(int i, int tid) { return (i * NT + tid) / (W / 8); }
+  __device__ __forceinline__ static int col_of(int i, int tid) {
+    return (i * NT + tid) % (W / 8) * 8;
   }
   __device__ __forceinline__ void get(const T* src, long st, int len, int cols, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      r[i] = get_run<T, 8>((const T*)((const char*)src + offset(i, (int)st, len, cols, tid)));
+      r[i].get(src - 8, (uint32_t)min(row_of(i, tid), len - 1) * (uint32_t)st * ES +
+                            (uint32_t)(min(col_of(i, tid), cols - 8) + 8) * ES);
   }
-  __device__ __forceinline__ void mask(int len, int cols, int tid) {
-    if (len >= C && cols >= W && PER % NT == 0) return;
+  // The piece as it belongs into the tile.
+  __device__ __forceinline__ Frag<T> piece(int i, int len, int cols, int tid) const {
+    Frag<T> f = cut_frag<T>(r[i].frag(), col_of(i, tid), cols);
+    return row_of(i, tid) < min(len, C) ? f : Frag<T>{};
+  }
+  __device__ __forceinline__ void put(T* dst, int pitch, int len, int cols, int tid) const {
+    const bool whole = len >= C && cols >= W && PER % NT == 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int p = i * NT + tid, row = p / (W / 8);
-      r[i] = row < min(len, C) ? cut_run(r[i], p % (W / 8) * 8, cols) : Run<T, 8>{};
-    }
-  }
-  __device__ __forceinline__ void put(T* dst, int pitch, int len, int cols, int tid) {
-    mask(len, cols, tid);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int p = i * NT + tid;
-      if (PER % NT == 0 || p < PER)
-        st_frag(dst + p / (W / 8) * pitch + p % (W / 8) * 8, frag_of<T>(r[i]));
+      const Frag<T> f = whole ? r[i].frag() : piece(i, len, cols, tid);
+      if (PER % NT == 0 || i * NT + tid < PER)
+        st_frag(dst + row_of(i, tid) * pitch + col_of(i, tid), f);
     }
   }
 };
-// The same for tile after tile of one source: the offsets of whole tiles stay in registers.
+// The same for tile after tile of one source, whose rows lie `st` >= 0 apart: their offsets stay in
+// registers.
 template <typename T, int C, int W, int NT>
 struct TileStream : TileFetch<T, C, W, NT> {
   using Base = TileFetch<T, C, W, NT>;
-  int off[Base::N];
-  __device__ __forceinline__ TileStream(long st, int cols, int tid) {
-#pragma unroll
-    for (int i = 0; i < Base::N; ++i) off[i] = Base::offset(i, (int)st, C, cols, tid);
-  }
-  __device__ __forceinline__ void next(const T* src, long st, int len, int cols, int tid) {
-    if (len < C) {   // a sequence's last tile
-      Base::get(src, st, len, cols, tid);
-      return;
-    }
+  static_assert(NT % (W / 8) == 0, "the pieces of a thread lie in one column");
+  uint32_t row[Base::N], col;
+  __device__ __forceinline__ TileStream(long st, int cols, int tid)
+      : col((uint32_t)(min(Base::col_of(0, tid), cols - 8) + 8) * Base::ES) {
 #pragma unroll
     for (int i = 0; i < Base::N; ++i)
-      Base::r[i] = get_run<T, 8>((const T*)((const char*)src + off[i]));
+      row[i] = (uint32_t)Base::row_of(i, tid) * (uint32_t)st * Base::ES;
+  }
+  __device__ __forceinline__ void next(const T* src, long st, int len) {
+    const uint32_t last = (uint32_t)(min(len, C) - 1) * (uint32_t)st * Base::ES;
+#pragma unroll
+    for (int i = 0; i < Base::N; ++i) Base::r[i].get(src - 8, min(row[i], last) + col);
+  }
+};
+// [ROWS][32] tiles in a row, whole and aligned.
+template <typename T, int ROWS, int NT>
+struct BlockStream {
+  static constexpr int PER = ROWS * 4, N = (PER + NT - 1) / NT;
+  Frag<T> r[N];
+  __device__ __forceinline__ void next(const T* src, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      r[i] = ld_frag(src + 8 * (PER % NT == 0 ? i * NT + tid : min(i * NT + tid, PER - 1)));
+  }
+  __device__ __forceinline__ void put(T* dst, int pitch, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i * NT + tid;
+      if (PER % NT == 0 || p < PER) st_frag(dst + p / 4 * pitch + p % 4 * 8, r[i]);
+    }
   }
 };
 

@@ -137,9 +137,13 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       fd.put(sD, L::PK, V - v0, KP, tid);
       fo.put(sO, L::PS, at.len, V - v0, tid);
 #pragma unroll
-      for (int x = 0; x < decltype(fs)::N; ++x)
+      for (int x = 0; x < decltype(fs)::N; ++x) {
+        float ss[8], dd[8];
+        values_of(fs.piece(x, V - v0, KP, tid), ss);
+        values_of(fd.piece(x, V - v0, KP, tid), dd);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sd = fmaf(to_f32(fs.r[x].v[e]), to_f32(fd.r[x].v[e]), sd);
+        for (int e = 0; e < 8; ++e) sd = fmaf(ss[e], dd[e], sd);
+      }
       const Run<T, 8> vr = fv;
       __syncthreads();
       if (v0 + VS < V) fetch(v0 + VS);
@@ -200,15 +204,16 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
       for (int u = 0; u < NU; ++u)
         if (u <= uw) {
-          float x[8], y[8];
+          float x[8], y[8], d[8], rj[8];
+          const int j = 32 * u + 8 * g;
+          decays<T>(Gi, sG + j, 1.f, d);
+          ld_eight(sf + 3 * C + j, rj);
           pair_values(B[0][2 * u], B[0][2 * u + 1], x);
           pair_values(B[1][2 * u], B[1][2 * u + 1], y);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int j = 32 * u + 8 * g + e;
-            const float d = j <= i ? gexp<T>((float)(Gi - sG[j])) : 0.f, rj = sf[3 * C + j];
-            x[e] = j <= i ? x[e] * (d * (aq * rj)) : 0.f;
-            y[e] = j < i ? y[e] * (d * (ak * rj)) : 0.f;
+            x[e] = j + e <= i ? x[e] * (d[e] * (aq * rj[e])) : 0.f;
+            y[e] = j + e < i ? y[e] * (d[e] * (ak * rj[e])) : 0.f;
           }
           const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
 #pragma unroll
@@ -235,16 +240,18 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
       for (int u = 0; u < NU; ++u)
         if (u >= uw) {
-          float x[8], y[8];
+          float x[8], y[8], d[8], rq[8], bj[8], rj[8];
+          const int j = 32 * u + 8 * g;
+          decays<T>(Gi, sG + j, -1.f, d);
+          ld_eight(sf + 6 * C + j, rq);
+          ld_eight(sf + 2 * C + j, bj);
+          ld_eight(sf + 3 * C + j, rj);
           pair_values(B[0][2 * u], B[0][2 * u + 1], x);
           pair_values(B[1][2 * u], B[1][2 * u + 1], y);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int j = 32 * u + 8 * g + e;
-            const float d = j >= i ? gexp<T>((float)(sG[j] - Gi)) : 0.f;
-            const float aj = scale * sf[6 * C + j], bj = sf[2 * C + j] * sf[3 * C + j];
-            x[e] = j >= i ? x[e] * (d * (aj * rk)) : 0.f;
-            y[e] = j > i ? -(y[e] * (d * (bj * rk))) : 0.f;
+            x[e] = j + e >= i ? x[e] * (d[e] * (scale * rq[e] * rk)) : 0.f;
+            y[e] = j + e > i ? -(y[e] * (d[e] * (bj[e] * rj[e] * rk))) : 0.f;
           }
           const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
 #pragma unroll

@@ -108,19 +108,26 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
       delta_gsum(p, unit)[tid] = G;
     }
     if (wave < NB) {
+      const int row0 = 16 * wave + 4 * (lane >> 4);
+      float f[4];
+      double gr[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f[r] = sBeta[row0 + r] * sRk[row0 + r];
+        gr[r] = sG[row0 + r];
+      }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         if (j > wave) continue;
         const int col = 16 * j + (lane & 15);
         const double gj = sG[col];
+        const float rj = sRk[col];
+        float d[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * wave + 4 * (lane >> 4) + r;
-          // a product only where it counts: what is masked may be anything
-          sA[row * PA + col] =
-              row > col ? sBeta[row] * sRk[row] * sRk[col] * kk[j][r] * expf((float)(sG[row] - gj))
-                        : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) d[r] = pinned(f[r] * rj * expf((float)(gr[r] - gj)));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)   // a choice, no product: what is masked may be anything
+          sA[(row0 + r) * PA + col] = row0 + r > col ? kk[j][r] * d[r] : 0.f;
       }
     }
     __syncthreads();

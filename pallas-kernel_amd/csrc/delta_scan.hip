@@ -66,6 +66,11 @@ struct ScanShape {
 };
 constexpr int LDS_MOST = 160 * 1024;
 
+template <typename T>
+__device__ __forceinline__ T* at_off(char* base, uint32_t off) {
+  return (T*)(base + off);
+}
+
 // FIRST: the first pass, which has E (and M) and no outputs.
 template <typename T, int KP, int NW, bool FIRST>
 struct ScanLds : ScanShape<T, KP, NW> {
@@ -85,7 +90,7 @@ struct ScanLds : ScanShape<T, KP, NW> {
 template <typename T, int KP, int NW, bool FIRST>
 __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   using L = ScanLds<T, KP, NW, FIRST>;
-  constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, COLS = L::COLS;
+  constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, COLS = L::COLS, ES = L::ES;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -123,23 +128,26 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       S[i][r] = map && v == 32 * (i >> 1) + 8 * g + 4 * (i & 1) + r ? 1.f : 0.f;
   if (from && !map) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
+  // byte offsets of a lane's stores from bases that are the same for all
+  const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
+  const uint32_t o_off = (uint32_t)(8 * g * HV * V + v) * ES;
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  TileStream<T, L::TRI, 32, NT> ft(32, 32, tid);
-  TileStream<T, C, COLS, NT> fv(a.v_st, min(vc, V), tid);
+  BlockStream<T, L::TRI, NT> ft;
+  TileStream<T, C, COLS, NT> fv(a.v_st, vc, tid);
   constexpr int NF = (5 * C + NT - 1) / NT;
   float ff[NF];
   double fg = 0.;
   auto fetch = [&](int n) {
     const int len = min(C, at.T - n * C);
     const long unit = (long)(at.chunk + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * p.tri_bytes), 32, L::TRI, 32, tid);
-    if (!map) fv.next(vp + (long)n * C * a.v_st, a.v_st, len, vc, tid);
+    fk.next(kp + (long)n * C * a.k_st, a.k_st, len);
+    ft.next((const T*)(p.Tm + unit * p.tri_bytes), tid);
+    if (!map) fv.next(vp + (long)n * C * a.v_st, a.v_st, len);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
     for (int i = 0; i < NF; ++i) ff[i] = vec[min(i * NT + tid, 5 * C - 1)];
     if (!FIRST) {
-      fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
+      fq.next(qp + (long)n * C * a.q_st, a.q_st, len);
       fg = delta_gsum(p, unit)[min(tid, C - 1)];
     }
   };
@@ -152,7 +160,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     T* sm = (T*)buf;
     const int len = min(C, at.T - n * C);
     fk.put(sm + L::K0, L::PK, len, K, tid);
-    ft.put(sm + L::T0, L::PT, L::TRI, 32, tid);
+    ft.put(sm + L::T0, L::PT, tid);
     fv.put(sm + L::V0, L::PV, map ? 0 : len, vc, tid);
     float* sf = (float*)(buf + L::F0);
 #pragma unroll
@@ -201,14 +209,13 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           sRq[i] = rq;
           if (a.train && vb == 0) delta_vec(p, unit)[6 * C + i] = rq;
         }
-        const double gi = sG[i];
-        float x[8];
+        float x[8], d[8], rk[8];
+        const int j0 = 32 * u + 8 * g;
+        decays<T>(sG[i], sG + j0, 1.f, d);
+        ld_eight(sf + 3 * C + j0, rk);
         pair_values(acc[0], acc[1], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = 32 * u + 8 * g + e;
-          x[e] = j <= i ? fq * sf[3 * C + j] * x[e] * gexp<T>((float)(gi - sG[j])) : 0.f;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = j0 + e <= i ? x[e] * (fq * rk[e] * d[e]) : 0.f;
         // in two parts: of the three operands of o this one is the cheapest to have exact
         const Split<T> f = split_of<T>(x);
         const int row = 32 * tri_block(tile / 2, u) + i % 32;
@@ -235,8 +242,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
         }, f);
         if constexpr (!FIRST) {
-          if (a.train && vin)
-            st_frag((T*)p.S + (unit * V + v) * KP + 32 * s + 8 * g, high_of(f));
+          if (a.train && vin) st_frag(at_off<T>(p.S + unit * V * KP * ES, s_off) + 32 * s, high_of(f));
 #pragma unroll
           for (int i = 0; i < 2 * NU; ++i)
             mma(o[i],
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         pair_values(acc[2 * u], acc[2 * u + 1], x);
         if constexpr (!FIRST) {
           nf[u] = frag_of<T>(x);
-          if (a.train && vin) st_frag((T*)p.N + (unit * V + v) * C + 32 * u + 8 * g, nf[u]);
+          if (a.train && vin) st_frag(at_off<T>(p.N + unit * V * C * ES, n_off) + 32 * u, nf[u]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
@@ -288,7 +294,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       __syncthreads();   // the scores are there
       if (!idle) {
         const int len = min(C, at.T - n * C);
-        T* to = (T*)a.o + (((long)at.b * a.T + at.t + n * C) * HV + hv) * V + v;
+        char* to = (char*)a.o + (((long)at.b * a.T + at.t + n * C) * HV + hv) * V * ES;
+        const float scale = (float)a.scale;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
 #pragma unroll
@@ -296,7 +303,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int t = 32 * u + 8 * g + 4 * x + r;
-              o[2 * u + x][r] *= (float)a.scale * sRq[t] * sf[4 * C + t];
+              o[2 * u + x][r] *= scale * sRq[t] * sf[4 * C + t];
             }
 #pragma unroll
           for (int w = 0; w <= u; ++w)
@@ -310,7 +317,9 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int t = 32 * u + 8 * g + 4 * x + r;
-              if (vin && t < len) to[(long)t * HV * V] = from_f32<T>(o[2 * u + x][r]);
+              if (vin && t < len)
+                *at_off<T>(to + (long)(32 * u + 4 * x + r) * HV * V * ES, o_off) =
+                    from_f32<T>(o[2 * u + x][r]);
             }
         }
       }
@@ -397,18 +406,20 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   if (from) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  TileStream<T, L::TRI, 32, NT> ft(32, 32, tid), fp(32, 32, tid);
+  BlockStream<T, L::TRI, NT> ft, fp;
   TileStream<T, C, COLS, NT> fd(a.do_st, vc, tid);
+  constexpr int ES = (int)sizeof(T);
+  const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
   auto fetch = [&](int n) {
     const int len = min(C, at.T - n * C);
     const long unit = (long)(at.chunk + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len, K, tid);
-    fq.next(qp + (long)n * C * a.q_st, a.q_st, len, K, tid);
-    ft.next((const T*)(p.Tm + unit * p.tri_bytes), 32, L::TRI, 32, tid);
-    fp.next((const T*)(p.P + unit * p.tri_bytes), 32, L::TRI, 32, tid);
-    fd.next(dp + (long)n * C * a.do_st, a.do_st, len, vc, tid);
+    fk.next(kp + (long)n * C * a.k_st, a.k_st, len);
+    fq.next(qp + (long)n * C * a.q_st, a.q_st, len);
+    ft.next((const T*)(p.Tm + unit * p.tri_bytes), tid);
+    fp.next((const T*)(p.P + unit * p.tri_bytes), tid);
+    fd.next(dp + (long)n * C * a.do_st, a.do_st, len);
     const float* vec = delta_vec(p, unit);
 #pragma unroll
     for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|; e^{G_C}
@@ -426,8 +437,8 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     const int len = min(C, at.T - n * C);
     fk.put(sK, L::PK, len, K, tid);
     fq.put(sQ, L::PK, len, K, tid);
-    ft.put(sT, L::PT, L::TRI, 32, tid);
-    fp.put(sP, L::PT, L::TRI, 32, tid);
+    ft.put(sT, L::PT, tid);
+    fp.put(sP, L::PT, tid);
     fd.put(sV, L::PV, len, vc, tid);
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
@@ -449,7 +460,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Split<T> f = split_of<T>(x);
-      if (!FIRST && vin) st_frag((T*)p.dS + (unit * V + v) * KP + 32 * s + 8 * g, high_of(f));
+      if (!FIRST && vin) st_frag(at_off<T>(p.dS + unit * V * KP * ES, s_off) + 32 * s, high_of(f));
       mma_rows(acc, [&](int i) {
         return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
       }, f);
@@ -497,7 +508,8 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
         return ld_pair_t(sQ + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
       }, split_of<T>(x));
       pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (!FIRST && vin) st_frag((T*)p.Y + (unit * V + v) * C + 32 * u + 8 * g, frag_of<T>(x));
+      if (!FIRST && vin)
+        st_frag(at_off<T>(p.Y + unit * V * C * ES, n_off) + 32 * u, frag_of<T>(x));
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {

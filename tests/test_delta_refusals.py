@@ -157,7 +157,7 @@ PTRS = dict.fromkeys(("q", "k", "v", "g", "beta", "o"), 64)
     (dict(T=65, dtype=0, chunks=2), 1, "chunks"), (dict(seqs=64, batch=2), 1, "batch == 1"),
     (dict(seqs=64, chunks=3), 1, "bad nseq, chunks"), (dict(seqs=64, chunks=0), 1, "bad nseq"),
     (dict(batch=1 << 20, nseq=1 << 20, T=1 << 20), 2, "2^31"),
-    (dict(PTRS, q_st=1 << 24), 2, "2^24"), (dict(PTRS, v_st=-(1 << 24)), 2, "2^24"),
+    (dict(PTRS, q_st=1 << 24), 2, "2^24"), (dict(PTRS, v_st=-1), 2, "2^24"), (dict(PTRS, HV=1 << 10, V=1 << 14), 2, "2^24"),
     (dict(T=(1 << 31) - 64, chunks=(1 << 25) - 1), 2, "2^31"),
     (dict(T=1 << 30, chunks=1 << 24, nsegs=1 << 22, HV=1 << 12), 2, "grid"), (dict(), 1, "NULL"),
     (dict(PTRS, o=0), 1, "o must"), (PTRS, 1, "keep"), (dict(PTRS, keep=256), 1, "keep"),
