@@ -403,13 +403,18 @@ struct TileFetch {
     return row_of(i, tid) < min(len, C) ? f : Frag<T>{};
   }
   __device__ __forceinline__ void put(T* dst, int pitch, int len, int cols, int tid) const {
-    const bool whole = len >= C && cols >= W && PER % NT == 0;
+    dst += row_of(0, tid) * pitch + col_of(0, tid);   // NT / (W / 8) rows from piece to piece
+    constexpr int ROWS = NT / (W / 8);
+    static_assert(NT % (W / 8) == 0, "the pieces of a thread lie in one column");
+    if (PER % NT == 0 && len >= C && cols >= W) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const Frag<T> f = whole ? r[i].frag() : piece(i, len, cols, tid);
-      if (PER % NT == 0 || i * NT + tid < PER)
-        st_frag(dst + row_of(i, tid) * pitch + col_of(i, tid), f);
+      for (int i = 0; i < N; ++i) st_frag(dst + i * ROWS * pitch, r[i].frag());
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (PER % NT == 0 || i * NT + tid < PER)
+        st_frag(dst + i * ROWS * pitch, piece(i, len, cols, tid));
   }
 };
 // The same for tile after tile of one source, whose rows lie `st` >= 0 apart: their offsets stay in
@@ -425,7 +430,7 @@ struct TileStream : TileFetch<T, C, W, NT> {
     for (int i = 0; i < Base::N; ++i)
       row[i] = (uint32_t)Base::row_of(i, tid) * (uint32_t)st * Base::ES;
   }
-  __device__ __forceinline__ void next(const T* src, long st, int len) {
+  __device__ __forceinline__ void next(const T* src, int st, int len) {
     const uint32_t last = (uint32_t)(min(len, C) - 1) * (uint32_t)st * Base::ES;
 #pragma unroll
     for (int i = 0; i < Base::N; ++i) Base::r[i].get(src - 8, min(row[i], last) + col);
@@ -487,6 +492,22 @@ __device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& 
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       mma(acc[2 * u + h], part == 1 ? a[h].lo : a[h].hi, part == 0 ? b.lo : b.hi);
+}
+
+// acc[2 u + h] += a[h] b, the same way.
+template <int N>
+__device__ __forceinline__ void mma_pair(f32x4 (&acc)[N], int u, const Split<float> (&a)[2],
+                                         const Frag<float>& b) {
+  mma(acc[2 * u], a[0], b);
+  mma(acc[2 * u + 1], a[1], b);
+}
+template <int N>
+__device__ __forceinline__ void mma_pair(f32x4 (&acc)[N], int u, const Split<bf16> (&a)[2],
+                                         const Frag<bf16>& b) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], a[h].lo, b);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], a[h].hi, b);
 }
 
 __device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }

@@ -70,6 +70,18 @@ template <typename T>
 __device__ __forceinline__ T* at_off(char* base, uint32_t off) {
   return (T*)(base + off);
 }
+// The first n of 8 elements to any address of theirs.
+template <typename T>
+__device__ __forceinline__ void put_frag(T* p, const Frag<T>& f, int n) {
+  const Run<T, 8> r = __builtin_bit_cast(Eight<T>, f);
+  if (n >= 8) {
+    *reinterpret_cast<Run<T, 8>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = r.v[e];
+  }
+}
 
 // FIRST: the first pass, which has E (and M) and no outputs.
 template <typename T, int KP, int NW, bool FIRST>
@@ -130,35 +142,55 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 
   // byte offsets of a lane's stores from bases that are the same for all
   const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
-  const uint32_t o_off = (uint32_t)(8 * g * HV * V + v) * ES;
+  const uint32_t o_off =
+      (uint32_t)(tid / (COLS / 8) * HV * V + vb * COLS + tid % (COLS / 8) * 8) * ES;
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
   BlockStream<T, L::TRI, NT> ft;
   TileStream<T, C, COLS, NT> fv(a.v_st, vc, tid);
   constexpr int NF = (5 * C + NT - 1) / NT;
   float ff[NF];
   double fg = 0.;
-  auto fetch = [&](int n) {
-    const int len = min(C, at.T - n * C);
-    const long unit = (long)(at.chunk + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len);
-    ft.next((const T*)(p.Tm + unit * p.tri_bytes), tid);
-    if (!map) fv.next(vp + (long)n * C * a.v_st, a.v_st, len);
-    const float* vec = delta_vec(p, unit);
+  // where the next chunk's inputs lie, and this chunk's other parts; all of them go on by their steps
+  const long unit0 = (long)at.chunk * HV + hv;
+  const int k_st = (int)a.k_st, q_st = (int)a.q_st, v_st = (int)a.v_st;
+  const char* Tn = p.Tm + unit0 * p.tri_bytes;
+  const char* vecn = p.vec + unit0 * p.vec_bytes;
+  char *vecc = p.vec + unit0 * p.vec_bytes, *Pc = p.P + unit0 * p.tri_bytes;
+  char *Sc = p.S + unit0 * V * KP * ES, *Nc = p.N + unit0 * V * C * ES;
+  char* oc = (char*)a.o + (((long)at.b * a.T + at.t) * HV + hv) * V * ES;
+  const long t_step = (long)HV * p.tri_bytes, vec_step = (long)HV * p.vec_bytes;
+  const long s_step = (long)HV * V * KP * ES, n_step = (long)HV * V * C * ES;
+  const int o_row = HV * V * ES;   // and a row of o
+  const float scale = (float)a.scale;
+  const bool l2norm = a.l2norm != 0, keep = a.train != 0, keep_p = keep && vb == 0;
+  // in two lots in the second pass, as the loads of all waves at once hold up the waves
+  auto fetch = [&](int len) {
+    fk.next(kp, k_st, len);
+    kp += (long)C * k_st;
+    if (!map) {
+      fv.next(vp, v_st, len);
+      vp += (long)C * v_st;
+    }
+  };
+  auto fetch2 = [&](int len) {
+    ft.next((const T*)Tn, tid);
+    const float* vec = (const float*)vecn;
 #pragma unroll
     for (int i = 0; i < NF; ++i) ff[i] = vec[min(i * NT + tid, 5 * C - 1)];
     if (!FIRST) {
-      fq.next(qp + (long)n * C * a.q_st, a.q_st, len);
-      fg = delta_gsum(p, unit)[min(tid, C - 1)];
+      fq.next(qp, q_st, len);
+      qp += (long)C * q_st;
+      fg = ((const double*)(vecn + 28 * C))[min(tid, C - 1)];
     }
+    Tn += t_step;
+    vecn += vec_step;
   };
   unsigned char* rest = smem + L::BUFS * L::ONE;
   T *sQ = (T*)rest + L::Q0, *sP = (T*)rest + L::P0;
   double* sG = (double*)(rest + L::G0);
   float* sRq = (float*)(rest + L::R0);
-  auto put = [&](int n) {
-    unsigned char* buf = smem + n % L::BUFS * L::ONE;
+  auto put = [&](unsigned char* buf, int len) {
     T* sm = (T*)buf;
-    const int len = min(C, at.T - n * C);
     fk.put(sm + L::K0, L::PK, len, K, tid);
     ft.put(sm + L::T0, L::PT, tid);
     fv.put(sm + L::V0, L::PV, map ? 0 : len, vc, tid);
@@ -171,65 +203,103 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       if (tid < C) sG[tid] = fg;
     }
   };
-  if (nc > 0) {
-    fetch(0);
-    put(0);
-  }
-  for (int n = 0; n < nc; ++n) {
-    __syncthreads();
-    if (n + 1 < nc) fetch(n + 1);
-    const unsigned char* buf = smem + n % L::BUFS * L::ONE;
-    const T *sm = (const T*)buf, *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + w0;
-    const float* sf = (const float*)(buf + L::F0);   // e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|,
-    const long unit = (long)(at.chunk + n) * HV + hv;   // e^G
-    const float last = sf[5 * C - 1];
-    if (!FIRST) {
-      // The scores of 16 tokens (columns) with 32 before or among them (rows), item after item of the
-      // lower ones: a lane has 8 in a row of P.
-      constexpr int ITEMS = NU == 2 ? 6 : 2;
-      for (int it = wave; it < ITEMS; it += NW) {
-        const int u = it == 4 || it == 5, tile = it < 4 ? it : it - 2, i = 16 * tile + ci;
-        f32x4 acc[2] = {zero4(), zero4()};
-        float qq = 0.f;
+  // a chunk's outputs, which its waves left where its values were, in whole rows
+  auto store_o = [&](const unsigned char* buf, int len) {
+    constexpr int ROWS = NT / (COLS / 8);
+    const int row = tid / (COLS / 8), col = tid % (COLS / 8) * 8;
+    const T* so = (const T*)buf + L::V0 + row * L::PV + col;
+    if (col < vc) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          const Frag<T> qf = ld_frag(sQ + i * L::PK + 32 * s + 8 * g);
-          float x[8];
-          values_of(qf, x);
+      for (int i = 0; i < C / ROWS; ++i)
+        if (row + i * ROWS < len)
+          put_frag(at_off<T>(oc + (long)(i * ROWS) * o_row, o_off),
+                   ld_frag(so + i * ROWS * L::PV), vc - col);
+    }
+    oc += (long)C * o_row;
+  };
+  // The scores of 16 tokens (columns) with 32 before or among them (rows), of six such items in a
+  // chunk of 64 and two in one of 32: a lane has 8 in a row of P.
+  auto scores = [&](int it, const T* sK, const float* sf) {
+    const int u = it >= 4, tile = it < 4 ? it : it - 2, i = 16 * tile + ci, j0 = 32 * u + 8 * g;
+    f32x4 acc[2] = {zero4(), zero4()};
+    float qq = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) qq = fmaf(x[e], x[e], qq);
+    for (int s0 = 0; s0 < NS; s0 += 4) {
+      constexpr int B = NS < 4 ? NS : 4;   // a few reads on their way at once
+      Frag<T> qf[B], kf[B][2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            mma(acc[x], ld_frag(sK + (32 * u + pair_row(lane, x)) * L::PK + 32 * s + 8 * g), qf);
-        }
-        qq = swap32_add(qq, qq);
-        qq = swap16_add(qq, qq);
-        const float rq = a.l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f, fq = (float)a.scale * rq;
-        if (u == 0 && g == 0) {
-          sRq[i] = rq;
-          if (a.train && vb == 0) delta_vec(p, unit)[6 * C + i] = rq;
-        }
-        float x[8], d[8], rk[8];
-        const int j0 = 32 * u + 8 * g;
-        decays<T>(sG[i], sG + j0, 1.f, d);
-        ld_eight(sf + 3 * C + j0, rk);
-        pair_values(acc[0], acc[1], x);
+      for (int s = 0; s < B; ++s) {
+        qf[s] = ld_frag(sQ + i * L::PK + 32 * (s0 + s) + 8 * g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = j0 + e <= i ? x[e] * (fq * rk[e] * d[e]) : 0.f;
-        // in two parts: of the three operands of o this one is the cheapest to have exact
-        const Split<T> f = split_of<T>(x);
-        const int row = 32 * tri_block(tile / 2, u) + i % 32;
-        T* out = (T*)(p.P + unit * p.tri_bytes) + row * 32 + 8 * g;
-        st_frag(sP + row * L::PT + 8 * g, high_of(f));
-        if (a.train && vb == 0) st_frag(out, high_of(f));
-        if constexpr (sizeof(T) == 2) {
-          st_frag(sP + L::LO + row * L::PT + 8 * g, f.lo);
-          if (a.train && vb == 0) st_frag(out + delta_blocks<T>() * 1024, f.lo);
-        }
+        for (int x = 0; x < 2; ++x)
+          kf[s][x] = ld_frag(sK + (32 * u + pair_row(lane, x)) * L::PK + 32 * (s0 + s) + 8 * g);
+      }
+#pragma unroll
+      for (int s = 0; s < B; ++s) {
+        mma(acc[0], kf[s][0], qf[s]);
+        mma(acc[1], kf[s][1], qf[s]);
+      }
+#pragma unroll
+      for (int s = 0; s < B; ++s) {
+        float x[8];
+        values_of(qf[s], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qq = fmaf(x[e], x[e], qq);
       }
     }
+    qq = swap32_add(qq, qq);
+    qq = swap16_add(qq, qq);
+    const float rq = l2norm ? rsqrtf(qq + DELTA_L2_EPS) : 1.f, fq = scale * rq;
+    if (u == 0 && g == 0) {
+      sRq[i] = fq * sf[4 * C + i];
+      if (keep_p) ((float*)vecc)[6 * C + i] = rq;
+    }
+    float x[8], d[8], rk[8];
+    decays<T>(sG[i], sG + j0, 1.f, d);
+    ld_eight(sf + 3 * C + j0, rk);
+    pair_values(acc[0], acc[1], x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = j0 + e <= i ? x[e] * (fq * rk[e] * d[e]) : 0.f;
+    // in two parts: of the three operands of o this one is the cheapest to have exact
+    const Split<T> f = split_of<T>(x);
+    const int row = 32 * tri_block(tile / 2, u) + i % 32;
+    st_frag(sP + row * L::PT + 8 * g, high_of(f));
+    if constexpr (sizeof(T) == 2) st_frag(sP + L::LO + row * L::PT + 8 * g, f.lo);
+    if (keep_p) {
+      T* out = at_off<T>(Pc, (uint32_t)(row * 32 + 8 * g) * ES);
+      st_frag(out, high_of(f));
+      if constexpr (sizeof(T) == 2) st_frag(out + delta_blocks<T>() * 1024, f.lo);
+    }
+  };
+  unsigned char *buf = smem, *other = smem + (L::BUFS - 1) * L::ONE;   // this chunk's, the next one's
+  int left = at.T;   // tokens from this chunk on
+  if (nc > 0) {
+    fetch(left);
+    fetch2(left);
+    put(buf, left);
+  }
+  for (int n = 0; n < nc; ++n, left -= C) {
+    const bool more = n + 1 < nc;
+    __syncthreads();
+    // The two halves of the block's waves, one of each on a SIMD, go through a chunk in different
+    // orders, so that loads, products and conversions of one lie beside others of the other.
+    const bool early = wave < NW / 2;
+    auto aside = [&]() {
+      if (more) fetch(left - C);
+      if constexpr (!FIRST) {
+        constexpr int ITEMS = NU == 2 ? 6 : 2;
+        if (L::BUFS == 2 && n > 0) store_o(other, C);
+        if (ITEMS % NW == 0 || wave < ITEMS) scores(wave, (const T*)buf + L::K0, (const float*)(buf + L::F0));
+        if (ITEMS > NW && wave + NW < ITEMS) scores(wave + NW, (const T*)buf + L::K0, (const float*)(buf + L::F0));
+      }
+    };
+    if (early) aside();
+    const T *sm = (const T*)buf, *sK = sm + L::K0, *sT = sm + L::T0, *sV = sm + L::V0 + w0;
+    const float* sf = (const float*)(buf + L::F0);   // e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|,
+    const float last = sf[5 * C - 1];                // e^G
     f32x4 acc[2 * NU], o[FIRST ? 1 : 2 * NU];
     Frag<T> nf[NU];
+    if (idle && !early) aside();
     if (!idle) {
 #pragma unroll
       for (int i = 0; i < 2 * NU; ++i) acc[i] = o[FIRST ? 0 : i] = zero4();
@@ -242,7 +312,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
         }, f);
         if constexpr (!FIRST) {
-          if (a.train && vin) st_frag(at_off<T>(p.S + unit * V * KP * ES, s_off) + 32 * s, high_of(f));
+          if (keep && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, high_of(f));
 #pragma unroll
           for (int i = 0; i < 2 * NU; ++i)
             mma(o[i],
@@ -250,6 +320,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
                 high_of(f));
         }
       }
+      if (!early) aside();
+      if (more) fetch2(left - C);
       Split<T> R[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
@@ -281,7 +353,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         pair_values(acc[2 * u], acc[2 * u + 1], x);
         if constexpr (!FIRST) {
           nf[u] = frag_of<T>(x);
-          if (a.train && vin) st_frag(at_off<T>(p.N + unit * V * C * ES, n_off) + 32 * u, nf[u]);
+          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, nf[u]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
@@ -291,45 +363,58 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       }
     }
     if constexpr (!FIRST) {
-      __syncthreads();   // the scores are there
+      __syncthreads();   // the scores are there, and no values are read any more
       if (!idle) {
-        const int len = min(C, at.T - n * C);
-        char* to = (char*)a.o + (((long)at.b * a.T + at.t + n * C) * HV + hv) * V * ES;
-        const float scale = (float)a.scale;
+        T* so = (T*)buf + L::V0 + w0 + ci;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
+          float f[8];
+          ld_eight(sRq + 32 * u + 8 * g, f);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 8; ++x) o[2 * u + x / 4][x % 4] *= f[x];
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int t = 32 * u + 8 * g + 4 * x + r;
-              o[2 * u + x][r] *= scale * sRq[t] * sf[4 * C + t];
-            }
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int w = 0; w <= u; ++w)
+          for (int w = 0; w <= u; ++w) {
+            Split<T> f[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-              mma(o[2 * u + x],
-                  ld_split<T>(sP, L::LO,
-                              (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g), nf[w]);
+              f[x] = ld_split<T>(sP, L::LO,
+                                 (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
+            mma_pair(o, u, f, nf[w]);
+          }
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int t = 32 * u + 8 * g + 4 * x + r;
-              if (vin && t < len)
-                *at_off<T>(to + (long)(32 * u + 4 * x + r) * HV * V * ES, o_off) =
-                    from_f32<T>(o[2 * u + x][r]);
-            }
-        }
+          for (int x = 0; x < 8; ++x)
+            so[(32 * u + 8 * g + x) * L::PV] = from_f32<T>(o[2 * u + x / 4][x % 4]);
       }
     }
-    if (n + 1 < nc) {
+    if (more) {
+      if (idle) fetch2(left - C);
       // the scores' tiles have been read (their barrier is behind, or there is none of them); with
-      // one buffer, so must the chunk's be
-      if (L::BUFS == 1) __syncthreads();
-      put(n + 1);
+      // one buffer, so must the chunk's be, and its outputs
+      if (L::BUFS == 1) {
+        __syncthreads();
+        if (!FIRST) {
+          store_o(buf, C);
+          __syncthreads();
+        }
+      }
+      put(other, left - C);
+      unsigned char* x = buf;
+      buf = other;
+      other = x;
     }
+    vecc += vec_step;
+    Pc += t_step;
+    Sc += s_step;
+    Nc += n_step;
+  }
+  if (!FIRST && nc > 0) {
+    __syncthreads();
+    store_o(buf, left + C);
   }
   if (idle) return;
   if (map) {   // [KP][KP]: column v, rows in the lane's order
@@ -410,31 +495,52 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   TileStream<T, C, COLS, NT> fd(a.do_st, vc, tid);
   constexpr int ES = (int)sizeof(T);
   const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
+  // where the chunk before has its inputs, and this chunk its outputs; all go back by their steps
+  const long unit0 = (long)(at.chunk + nc - 1) * HV + hv;
+  const int k_st = (int)a.k_st, q_st = (int)a.q_st, d_st = (int)a.do_st;
+  kp += (long)(nc - 1) * C * k_st;
+  qp += (long)(nc - 1) * C * q_st;
+  dp += (long)(nc - 1) * C * d_st;
+  const char *Tn = p.Tm + unit0 * p.tri_bytes, *Pn = p.P + unit0 * p.tri_bytes;
+  const char* vecn = p.vec + unit0 * p.vec_bytes;
+  char *Sc = p.dS + unit0 * V * KP * ES, *Yc = p.Y + unit0 * V * C * ES;
+  const long t_step = (long)HV * p.tri_bytes, vec_step = (long)HV * p.vec_bytes;
+  const long s_step = (long)HV * V * KP * ES, n_step = (long)HV * V * C * ES;
+  const float scale = (float)a.scale;
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
-  auto fetch = [&](int n) {
-    const int len = min(C, at.T - n * C);
-    const long unit = (long)(at.chunk + n) * HV + hv;
-    fk.next(kp + (long)n * C * a.k_st, a.k_st, len);
-    fq.next(qp + (long)n * C * a.q_st, a.q_st, len);
-    ft.next((const T*)(p.Tm + unit * p.tri_bytes), tid);
-    fp.next((const T*)(p.P + unit * p.tri_bytes), tid);
-    fd.next(dp + (long)n * C * a.do_st, a.do_st, len);
-    const float* vec = delta_vec(p, unit);
+  auto fetch = [&](int len) {
+    fk.next(kp, k_st, len);
+    fd.next(dp, d_st, len);
+    kp -= (long)C * k_st;
+    dp -= (long)C * d_st;
+  };
+  auto fetch2 = [&](int len) {
+    fq.next(qp, q_st, len);
+    ft.next((const T*)Tn, tid);
+    fp.next((const T*)Pn, tid);
+    const float* vec = (const float*)vecn;
 #pragma unroll
     for (int i = 0; i < NF; ++i) {   // e^{G_C - G} / |k|, beta e^G / |k|, scale e^G / |q|; e^{G_C}
       const int x = i * NT + tid, t = x % C;
       ff[i] = vec[x < C ? C + t : x < 2 * C ? t : x < 3 * C ? 4 * C + t : 5 * C - 1];
       fr[i] = vec[x < 2 * C ? 2 * C + t : 6 * C + t];
     }
+    qp -= (long)C * q_st;
+    Tn -= t_step;
+    Pn -= t_step;
+    vecn -= vec_step;
   };
   T* sm = (T*)smem;
   T *sK = sm + L::K0, *sQ = sm + L::Q0, *sT = sm + L::T0, *sP = sm + L::P0, *sV = sm + L::V0;
   float* sf = (float*)(smem + L::F0);
-  if (nc > 0) fetch(nc - 1);
-  for (int n = nc - 1; n >= 0; --n) {
+  int len = at.T - (nc - 1) * C;   // of the last chunk alone less than C
+  if (nc > 0) {
+    fetch(len);
+    fetch2(len);
+  }
+  for (int n = nc - 1; n >= 0; --n, len = C) {
     __syncthreads();
-    const int len = min(C, at.T - n * C);
     fk.put(sK, L::PK, len, K, tid);
     fq.put(sQ, L::PK, len, K, tid);
     ft.put(sT, L::PT, tid);
@@ -444,12 +550,14 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     for (int i = 0; i < NF; ++i) {
       const int x = i * NT + tid;
       if (x <= 3 * C)
-        sf[x] = x < C || x == 3 * C ? ff[i] : ff[i] * fr[i] * (x < 2 * C ? 1.f : (float)a.scale);
+        sf[x] = x < C || x == 3 * C ? ff[i] : ff[i] * fr[i] * (x < 2 * C ? 1.f : scale);
     }
     __syncthreads();
-    if (n > 0) fetch(n - 1);
-    if (idle) continue;
-    const long unit = (long)(at.chunk + n) * HV + hv;
+    if (n > 0) fetch(C);
+    if (idle) {
+      if (n > 0) fetch2(C);
+      continue;
+    }
     const float last = sf[3 * C];
 
     f32x4 acc[2 * NU];
@@ -460,7 +568,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Split<T> f = split_of<T>(x);
-      if (!FIRST && vin) st_frag(at_off<T>(p.dS + unit * V * KP * ES, s_off) + 32 * s, high_of(f));
+      if (!FIRST && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, high_of(f));
       mma_rows(acc, [&](int i) {
         return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
       }, f);
@@ -480,6 +588,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
         for (int x = 0; x < 2; ++x)
           mma(acc[2 * w + x],
               ld_split_t<T>(sP + 32 * tri_block(u, w) * L::PT, L::LO, L::PT, lane, x), df[u]);
+    if (n > 0) fetch2(C);
     Split<T> R[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -509,13 +618,15 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       }, split_of<T>(x));
       pair_values(acc[2 * u], acc[2 * u + 1], x);
       if (!FIRST && vin)
-        st_frag(at_off<T>(p.Y + unit * V * C * ES, n_off) + 32 * u, frag_of<T>(x));
+        st_frag(at_off<T>(Yc, n_off) + 32 * u, frag_of<T>(x));
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {
         return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
       }, split_of<T>(x));
     }
+    Sc -= s_step;
+    Yc -= n_step;
   }
   if (idle) return;
   float* to = FIRST ? p.dE + ((long)at.seg * HV + hv) * K * V
