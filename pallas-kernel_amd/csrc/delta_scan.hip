@@ -286,6 +286,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     const bool early = wave < NW / 2;
     auto aside = [&]() {
       if (more) fetch(left - C);
+      if (FIRST && more) fetch2(left - C);
       if constexpr (!FIRST) {
         constexpr int ITEMS = NU == 2 ? 6 : 2;
         if (L::BUFS == 2 && n > 0) store_o(other, C);
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         }
       }
       if (!early) aside();
-      if (more) fetch2(left - C);
+      if (!FIRST && more) fetch2(left - C);
       Split<T> R[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       }
     }
     if (more) {
-      if (idle) fetch2(left - C);
+      if (!FIRST && idle) fetch2(left - C);
       // the scores' tiles have been read (their barrier is behind, or there is none of them); with
       // one buffer, so must the chunk's be, and its outputs
       if (L::BUFS == 1) {

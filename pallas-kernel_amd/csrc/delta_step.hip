@@ -2,9 +2,9 @@
 // (include/tops_gla_delta.h).
 //
 // Bound by memory: the state of a row and head is read and written once, however many tokens come.
-// A wave holds all K rows of 16 columns of the state: a lane four columns of K / 16 consecutive
-// rows, so that the sums over the keys are sums of a lane and of the 16 lanes with its columns
-// (two rotations in a row of lanes, two swaps of rows), without LDS. One round of them serves a
+// A wave holds all K rows of 32 columns of the state, whole lines of 128 bytes: a lane four columns
+// of K / 8 consecutive rows, so that the sums over the keys are sums of a lane and of the 8 lanes
+// with its columns (a rotation in a row of lanes, two swaps of rows), without LDS. One round serves a
 // token: with S' = e^g S, o = scale S_t^T q = scale (S'^T q + (q k) n), so S'^T k, S'^T q, q k and
 // the norms are summed together, before n is known.
 #include "delta.hpp"
@@ -14,7 +14,6 @@ namespace tops {
 namespace {
 
 __device__ __forceinline__ float key_sum(float x) {
-  x += dpp<0x124>(x);
   x += dpp<0x128>(x);
   x = swap16_add(x, x);
   return swap32_add(x, x);
@@ -25,16 +24,16 @@ template <typename T, int KR>
 __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int K = (int)a.K, V = (int)a.V, T_ = (int)a.T;
-  const int vt = (V + 63) / 64;
+  const int vt = (V + 127) / 128;
   long blk = blockIdx.x;
   const int vb = (int)(blk % vt);
   blk /= vt;
   const int hv = (int)(blk % a.HV);
   const long b = blk / a.HV;
   const int h = hv / (int)(a.HV / a.H);
-  const int c0 = vb * 64 + wave * 16 + (lane & 3) * 4;
-  const int r0 = (lane >> 2) * KR;
-  if (vb * 64 + wave * 16 >= V) return;
+  const int c0 = vb * 128 + wave * 32 + (lane & 7) * 4;
+  const int r0 = (lane >> 3) * KR;
+  if (vb * 128 + wave * 32 >= V) return;
   const int nc = V - c0, nr = K - r0;
   T* o = (T*)a.o + ((b * T_) * a.HV + hv) * V + c0;
   const long o_st = a.HV * V;
@@ -44,7 +43,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_arg
     slot = a.idx64 ? ((const int64_t*)a.slots_idx)[b] : (long)((const int32_t*)a.slots_idx)[b];
   if (slot < 0 || slot >= a.slots) {
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    if (lane < 4 && nc > 0)
+    if (lane < 8 && nc > 0)
       for (int t = 0; t < T_; ++t) put_run<T, 4>(o + t * o_st, zero, nc);
     return;
   }
@@ -73,7 +72,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_arg
   const T* k = (const T*)a.k + b * a.k_sb + h * a.k_sh + r0;
   const T* v = (const T*)a.v + b * a.v_sb + hv * a.v_sh + c0;
   const long g0 = b * a.g_sb + hv, b0 = b * a.beta_sb + hv;
-  const bool whole = K == 16 * KR && V % 16 == 0;   // no lane of a wave is past the end
+  const bool whole = K == 8 * KR && V % 32 == 0;   // no lane of a wave is past the end
   for (int t = 0; t < T_; ++t) {
     Run<T, KR> qr, kr;
     Run<T, 4> vr;
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_arg
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[r][e] = fmaf(x, n[e], ge * s[r][e]);
     }
-    if (lane < 4 && nc > 0) put_run<T, 4>(o + t * o_st, y, nc);
+    if (lane < 8 && nc > 0) put_run<T, 4>(o + t * o_st, y, nc);
   }
 #pragma unroll
   for (int r = 0; r < KR; ++r)
@@ -139,18 +138,18 @@ __global__ __launch_bounds__(256) void delta_step_kernel(tops_gla_delta_step_arg
 template <typename T>
 void launch(const tops_gla_delta_step_args& a, unsigned grid, hipStream_t st) {
   if (a.K <= 64)
-    delta_step_kernel<T, 4><<<grid, 256, 0, st>>>(a);
-  else if (a.K <= 128)
     delta_step_kernel<T, 8><<<grid, 256, 0, st>>>(a);
-  else
+  else if (a.K <= 128)
     delta_step_kernel<T, 16><<<grid, 256, 0, st>>>(a);
+  else
+    delta_step_kernel<T, 32><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace
 
 hipError_t run_delta_step(const tops_gla_delta_step_args& a, hipStream_t st) {
   if (a.batch == 0 || a.T == 0) return hipSuccess;
-  const unsigned grid = (unsigned)((a.V + 63) / 64 * a.HV * a.batch);
+  const unsigned grid = (unsigned)((a.V + 127) / 128 * a.HV * a.batch);
   if (a.dtype == DT_BF16)
     launch<bf16>(a, grid, st);
   else

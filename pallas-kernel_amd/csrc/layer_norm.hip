@@ -6,43 +6,57 @@
 //
 // Bound by memory: x (and dy) are read once into registers, the mean comes before the squares of
 // the differences (a variance from sum and sum of squares loses what a large mean covers), and the
-// next row's loads are on their way while a row is worked on. A row belongs to one wave up to 2048
-// features, to a block of 4 or 8 waves above; a thread holds at most 32 features, whose share of
-// w, b, dw and db stays in its registers over all its rows. The weights' sums go through one
-// partial row a block in a workspace and a second kernel, in fixed order.
+// next row's loads are on their way while a row is worked on. A thread holds at most 16 features,
+// whose share of w, b, dw and db stays in its registers over all its rows: up to 1024 features a row
+// belongs to one wave, above to a block of 2 to 16. The weights' sums go through one partial row a
+// block in a workspace and a second kernel, in fixed order.
 #include "delta.hpp"
 
 namespace tops {
 
 namespace {
 
-// Threads of a row by its features: 32 a thread at most.
-int row_threads(long D) { return D <= 2048 ? 64 : D <= 8192 ? 256 : 512; }
-int block_threads(long D) { return D <= 8192 ? 256 : 512; }
+constexpr long FWD_WAVES = 16, BWD_WAVES = 8;
+
+// Threads of a row by its features, 16 a thread at most, and of a block: four rows of one wave, or
+// one row.
+int row_threads(long D) {
+  return D <= 1024 ? 64 : D <= 2048 ? 128 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024;
+}
+constexpr int block_threads(int nt) { return nt == 64 ? 256 : nt; }
 long norm_blocks(long rows, long D, bool backward) {
-  const long per = block_threads(D) / row_threads(D);
-  // two waves a SIMD in the backward, four in the forward; fewer where the rows do not go round
-  const long most = (backward ? 512 : 1024) * 256 / block_threads(D);
+  const int nt = row_threads(D), bt = block_threads(nt);
+  const long per = bt / nt;
+  const long most = (backward ? BWD_WAVES : FWD_WAVES) * 256 * 64 / bt;   // waves a CU
   return std::min((rows + per - 1) / per, most);
 }
 
-template <int NT>
-__device__ __forceinline__ float row_sum(float x, float* sm, int tid) {
+__device__ __forceinline__ float wave_sum(float x) {
   x += dpp<0x121>(x);
   x += dpp<0x122>(x);
   x += dpp<0x124>(x);
   x += dpp<0x128>(x);
   x = swap16_add(x, x);
-  x = swap32_add(x, x);
-  if constexpr (NT > 64) {
-    __syncthreads();   // the values of the sum before have been read
-    if ((tid & 63) == 0) sm[tid >> 6] = x;
-    __syncthreads();
-    x = 0.f;
+  return swap32_add(x, x);
+}
+// Sums of N values over the threads of a row; `sm` is one of two places that take turns, so that a
+// sum needs one barrier.
+template <int NT, int N>
+__device__ __forceinline__ void row_sum(float (&x)[N], float (*sm)[16], int tid) {
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) x += sm[i];
+  for (int n = 0; n < N; ++n) x[n] = wave_sum(x[n]);
+  if constexpr (NT > 64) {
+    if ((tid & 63) == 0)
+#pragma unroll
+      for (int n = 0; n < N; ++n) sm[n][tid >> 6] = x[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      x[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT / 64; ++i) x[n] += sm[n][i];
+    }
   }
-  return x;
 }
 
 // Features c .. c + VEC - 1 of run i of a thread: runs of a row's threads lie side by side.
@@ -80,12 +94,13 @@ __device__ __forceinline__ void load_weights(const float* w, int D, int tid, flo
 }
 
 template <typename T, int NT, int R>
-__global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_fwd_kernel(
+__global__ __launch_bounds__(block_threads(NT)) void layer_norm_fwd_kernel(
     tops_gla_layer_norm_args a) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  constexpr int PER = (NT > 256 ? NT : 256) / NT;
-  __shared__ float sm[8];
+  constexpr int PER = block_threads(NT) / NT;
+  __shared__ float sm[2][1][16];
   const int D = (int)a.D, tid = threadIdx.x % NT;
+  const float eps = (float)a.eps;
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
   float w[R][VEC], b[R][VEC];
@@ -102,29 +117,31 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_fwd_kernel(
   };
   if (row < a.rows) load(row);
   for (; row < a.rows; row += step) {
-    float v[R][VEC], s = 0.f;
+    float v[R][VEC], s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const bool in = run_col<NT, VEC>(tid, i) < D;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         v[i][e] = in ? to_f32(nx[i].v[e]) : 0.f;
-        s += v[i][e];
+        s[0] += v[i][e];
       }
     }
     if (row + step < a.rows) load(row + step);
-    const float mean = row_sum<NT>(s, sm, tid) / (float)D;
-    s = 0.f;
+    row_sum<NT>(s, sm[0], tid);
+    const float mean = s[0] / (float)D;   // a row of one value has exactly its mean
+    s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int c = run_col<NT, VEC>(tid, i);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         v[i][e] = c + e < D ? v[i][e] - mean : 0.f;
-        s = fmaf(v[i][e], v[i][e], s);
+        s[0] = fmaf(v[i][e], v[i][e], s[0]);
       }
     }
-    const float rstd = 1.f / sqrtf(row_sum<NT>(s, sm, tid) / (float)D + (float)a.eps);
+    row_sum<NT>(s, sm[1], tid);
+    const float rstd = 1.f / sqrtf(s[0] / (float)D + eps);
     if (a.stats && tid == 0) {
       a.stats[2 * row] = mean;
       a.stats[2 * row + 1] = rstd;
@@ -141,11 +158,10 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_fwd_kernel(
 }
 
 template <typename T, int NT, int R>
-__global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
+__global__ __launch_bounds__(block_threads(NT)) void layer_norm_bwd_kernel(
     tops_gla_layer_norm_args a) {
-  constexpr int VEC = 16 / (int)sizeof(T), BT = NT > 256 ? NT : 256;
-  constexpr int PER = BT / NT;
-  __shared__ float sm[8];
+  constexpr int VEC = 16 / (int)sizeof(T), PER = block_threads(NT) / NT;
+  __shared__ float sm[2][2][16];
   __shared__ float part[PER > 1 ? 2 * R * VEC * NT : 1];
   const int D = (int)a.D, tid = threadIdx.x % NT;
   const T *x = (const T*)a.x, *dy = (const T*)a.dy;
@@ -160,6 +176,8 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
   long row = (long)blockIdx.x * PER + threadIdx.x / NT;
   Run<T, VEC> nx[R], nd[R];
   float mean = 0.f, rstd = 0.f;
+  const float inv = 1.f / (float)D;
+  int turn = 0;
   auto load = [&](long r) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -172,7 +190,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
   };
   if (row < a.rows) load(row);
   for (; row < a.rows; row += step) {
-    float n[R][VEC], u[R][VEC], s = 0.f, sn = 0.f;
+    float n[R][VEC], u[R][VEC], s[2] = {0.f, 0.f};
     const float m = mean, rs = rstd;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -185,19 +203,20 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
         db[i][e] += d;
         dw[i][e] = fmaf(d, n[i][e], dw[i][e]);
         u[i][e] = d * w[i][e];
-        s += u[i][e];
-        sn = fmaf(u[i][e], n[i][e], sn);
+        s[0] += u[i][e];
+        s[1] = fmaf(u[i][e], n[i][e], s[1]);
       }
     }
     if (row + step < a.rows) load(row + step);
-    s = row_sum<NT>(s, sm, tid) / (float)D;
-    sn = row_sum<NT>(sn, sm, tid) / (float)D;
+    row_sum<NT>(s, sm[turn], tid);
+    turn ^= 1;
+    const float m1 = s[0] * inv, m2 = s[1] * inv;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int c = run_col<NT, VEC>(tid, i);
       float r[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) r[e] = rs * (u[i][e] - s - n[i][e] * sn);
+      for (int e = 0; e < VEC; ++e) r[e] = rs * (u[i][e] - m1 - n[i][e] * m2);
       if (c < D) put_run<T, VEC>(dx + row * D + c, r, D - c);
     }
   }
@@ -239,22 +258,22 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void layer_norm_bwd_kernel(
   }
 }
 
-// Sums `parts` rows of 2 D partial sums: 64 columns a block, its 16 waves a sixteenth of the rows
-// each.
+// Sums `parts` rows of 2 D partial sums: 32 columns a block, a thirty-second of the rows for each
+// half of its waves.
 __global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* ws, int parts, int D,
                                                               float* dw, float* db) {
-  __shared__ float sm[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  __shared__ float sm[32][33];
+  const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + col;
   float s = 0.f;
   if (c < 2 * D)
-    for (int r = wave; r < parts; r += 16) s += ws[(long)r * 2 * D + c];
-  sm[wave][lane] = s;
+    for (int r = part; r < parts; r += 32) s += ws[(long)r * 2 * D + c];
+  sm[part][col] = s;
   __syncthreads();
-  if (wave == 0 && c < 2 * D) {
+  if (part == 0 && c < 2 * D) {
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += sm[i][lane];
+    for (int i = 0; i < 32; ++i) s += sm[i][col];
     if (c < D) {
       if (dw) dw[c] = s;
     } else if (db) {
@@ -265,36 +284,36 @@ __global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* ws, i
 
 template <typename T, int NT, int R>
 void launch(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
-  const int nb = (int)norm_blocks(a.rows, a.D, backward), bt = NT > 256 ? NT : 256;
+  const int nb = (int)norm_blocks(a.rows, a.D, backward);
   if (backward)
-    layer_norm_bwd_kernel<T, NT, R><<<nb, bt, 0, st>>>(a);
+    layer_norm_bwd_kernel<T, NT, R><<<nb, block_threads(NT), 0, st>>>(a);
   else
-    layer_norm_fwd_kernel<T, NT, R><<<nb, bt, 0, st>>>(a);
+    layer_norm_fwd_kernel<T, NT, R><<<nb, block_threads(NT), 0, st>>>(a);
+}
+template <typename T, int NT>
+void launch(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
+  constexpr int VEC = 16 / (int)sizeof(T), MOST = 16 / VEC;
+  if constexpr (NT == 64) {   // rows of more threads are more than half of what these hold
+    if (a.D <= 64 * VEC) return launch<T, NT, 1>(a, backward, st);
+    if (VEC == 4 && a.D <= 128 * VEC) return launch<T, NT, 2>(a, backward, st);
+  }
+  launch<T, NT, MOST>(a, backward, st);
 }
 
 template <typename T>
 hipError_t run(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int nt = row_threads(a.D);
-  const long r = (a.D + (long)nt * VEC - 1) / ((long)nt * VEC);   // runs a thread
   if (a.rows > 0) {
-    if (nt == 64) {
-      if (r <= 1) launch<T, 64, 1>(a, backward, st);
-      else if (r <= 2) launch<T, 64, 2>(a, backward, st);
-      else if (r <= 4) launch<T, 64, 4>(a, backward, st);
-      else if constexpr (VEC == 4) launch<T, 64, 8>(a, backward, st);
-    } else if (nt == 256) {
-      if (r <= 2) launch<T, 256, 2>(a, backward, st);
-      else if (r <= 4) launch<T, 256, 4>(a, backward, st);
-      else if constexpr (VEC == 4) launch<T, 256, 8>(a, backward, st);
-    } else {
-      if (r <= 4) launch<T, 512, 4>(a, backward, st);
-      else if constexpr (VEC == 4) launch<T, 512, 8>(a, backward, st);
+    switch (row_threads(a.D)) {
+      case 64: launch<T, 64>(a, backward, st); break;
+      case 128: launch<T, 128>(a, backward, st); break;
+      case 256: launch<T, 256>(a, backward, st); break;
+      case 512: launch<T, 512>(a, backward, st); break;
+      default: launch<T, 1024>(a, backward, st);
     }
   }
   if (backward && a.ws) {
     const int parts = (int)norm_blocks(a.rows, a.D, true);
-    layer_norm_sum_kernel<<<(unsigned)((2 * a.D + 63) / 64), 1024, 0, st>>>(
+    layer_norm_sum_kernel<<<(unsigned)((2 * a.D + 31) / 32), 1024, 0, st>>>(
         (const float*)a.ws, parts, (int)a.D, a.dw, a.db);
   }
   return hipGetLastError();
