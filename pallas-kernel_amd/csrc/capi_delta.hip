@@ -145,12 +145,21 @@ int64_t tops_gla_delta_chunk(int64_t dtype) {
 }
 
 int64_t tops_gla_delta_segment(int64_t nseq, int64_t chunks, int64_t HV, int64_t V) {
-  if (nseq < 1 || chunks < 1 || HV < 1 || V < 1) return 1 << 20;
-  // a block for each CU of the second pass; a first pass costs twice that, so that two or three
-  // segments of a sequence gain nothing
+  const int64_t whole = 1 << 20;
+  if (nseq < 1 || chunks < 1 || HV < 1 || V < 1) return whole;
+  // a block for each CU in the second pass: two segments of 32 chunks, 8 sequences of 16 heads,
+  // take 217 us forward (uncut 238, three segments 285), three of 22, 5 sequences, 363 (uncut 422,
+  // two 365), four of 2 chunks, one sequence, 46 (uncut 58). Below 6 chunks the first pass costs
+  // what the second saves (two of 2 chunks 40, uncut 36)
   const int64_t blocks = (V + 127) / 128 * HV * nseq, per = (chunks + nseq - 1) / nseq;
-  const int64_t segs = std::min<int64_t>(256 / std::max<int64_t>(1, blocks), per / 4);
-  return segs < 4 ? 1 << 20 : std::min<int64_t>((per + segs - 1) / segs, 1 << 20);
+  const int64_t segs = 256 / std::max<int64_t>(1, blocks);
+  if (segs < 2 || per < 6) return whole;
+  int64_t L = std::max<int64_t>((per + segs - 1) / segs, 2);
+  // the fold goes from segment to segment, each about a quarter of two passes' chunk: least in sum
+  // at L = sqrt(per / 4) (per = 256, one head: L = 4 181 us, 8 156, 16 194; 1024: 8 390, 16 306,
+  // 32 385)
+  while (L * L * 4 < per && L < whole) ++L;
+  return std::min(L, whole);
 }
 
 int64_t tops_gla_delta_bytes(const tops_gla_delta_sizes* z, int64_t backward) {

@@ -56,6 +56,14 @@ __device__ __forceinline__ SegAt seg_at(const tops_gla_delta_args& a, int C, int
   return x;
 }
 
+// Blocks n a segment (or sequence): its neighbouring heads and columns, which read the same keys, go
+// to one XCD, and every XCD has a part of every segment. (Whole segments to an XCD: a sequence of
+// 200 chunks behind 40 of 4 had one XCD at work, 1083 us a call, so 393; equal ones the same.)
+__device__ __forceinline__ int spread(int blk, int n) {
+  const int r = blk % n;
+  return blk - r + xcd_remap(r, n);
+}
+
 // A head's columns go to blocks of NW waves of 16, of V or, in a first pass, then of KP for M.
 template <typename T, int KP, int NW>
 struct ScanShape {
@@ -109,7 +117,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   const int g = lane >> 4, ci = lane & 15;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + COLS - 1) / COLS, mt = FIRST ? (KP + COLS - 1) / COLS : 0;
-  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);   // a head's columns on one XCD
+  int blk = spread((int)blockIdx.x, (vt + mt) * HV);
   const int vb = blk % (vt + mt);
   blk /= vt + mt;
   const int hv = blk % HV, h = hv / (HV / (int)a.H);
@@ -466,7 +474,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   const int g = lane >> 4, ci = lane & 15;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + COLS - 1) / COLS;
-  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  int blk = spread((int)blockIdx.x, vt * HV);
   const int vb = blk % vt;
   blk /= vt;
   const int hv = blk % HV, h = hv / (HV / (int)a.H);
@@ -647,7 +655,7 @@ __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaP
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   const int K = (int)a.K, V = (int)a.V, HV = (int)a.HV;
   const int vt = (V + 15) / 16;
-  int blk = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  int blk = spread((int)blockIdx.x, vt * HV);
   const int v = blk % vt * 16 + (lane & 15);
   blk /= vt;
   const int hv = blk % HV, seq = blk / HV;

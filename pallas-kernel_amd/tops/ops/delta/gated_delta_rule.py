@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import math
 import struct
 
 import torch
@@ -33,6 +34,26 @@ def _tokens(t, dt):
     return t if 0 <= t.stride(1) < 1 << 24 else t.contiguous()
 
 
+_CUS = 256
+
+
+def _segment(counts, blocks):
+    """Chunks in a segment of packed sequences of ``counts`` chunks, with ``blocks`` blocks for the
+    heads and columns of each; tops_gla_delta_segment has the rule for equal lengths.
+
+    All segments should run at once, or the last ones wait for a whole one (lengths of 28, 5, 33,
+    2, 47, 1, 8 and 9 chunks, 16 heads: L = 10 has 272 blocks and takes 192 us, 11 has 256 and 159,
+    12 164, 17 200, uncut 299). Where the sequences alone are more than the CUs hold, their ends
+    differ anyway, and what is long among them is cut by the average (40 of 4 chunks and one of
+    200: 393 us, uncut 1242; 64 of 6 and one of 60: 538, uncut 596)."""
+    longest = max(counts)
+    L = max(-(-sum(counts) * blocks // _CUS), 2, math.isqrt(max(0, longest - 1) // 4) + 1)
+    if len(counts) * blocks <= _CUS:
+        while L < longest and sum(-(-n // L) for n in counts) * blocks > _CUS:
+            L += 1
+    return L if longest >= 6 and longest >= 2 * L else max(1, longest)
+
+
 class _Chunks:
     """The chunks that a call's sequences are cut into, and the segments that these run in."""
 
@@ -49,19 +70,19 @@ class _Chunks:
         self.nseq = len(cu) - 1
         counts = [-((a - b) // C) for a, b in zip(cu, cu[1:])]
         self.n = sum(counts)
-        # the longest sequences are cut however many there are
-        self.L = lib.tops_gla_delta_segment(1, self.n, HV, V)
 
         def make():
+            L = _segment(counts, HV * -(-V // 128))
             chunks, segs, seq = [0], [0], []
             for s, n in enumerate(counts):
-                k = max(1, -(-n // self.L))
+                k = max(1, -(-n // L))
                 chunks.append(chunks[-1] + n)
                 segs.append(segs[-1] + k)
                 seq += [s] * k
-            return [*cu, *chunks, *segs, *seq], len(seq)
+            return [*cu, *chunks, *segs, *seq], (len(seq), L)
 
-        self.table, self.nsegs = device_table(("delta", tuple(cu), C, self.L), make, device)
+        key = "delta", tuple(cu), C, HV * -(-V // 128)
+        self.table, (self.nsegs, self.L) = device_table(key, make, device)
 
     def bytes(self, HV, K, V, dt, train, backward):
         return _lib.load().tops_gla_delta_bytes(

@@ -3,6 +3,7 @@ types, CPU tensors), and the C entry points' own, before any HIP call. And the o
 differences."""
 
 import ctypes
+import importlib
 import os
 import re
 import struct
@@ -245,10 +246,20 @@ def test_segments():
     f = _lib.load().tops_gla_delta_segment
     whole = 1 << 20
     assert f(1, 256, 16, 128) == 16 and f(2, 128, 16, 128) == 8
-    assert f(1, 3, 1, 64) == whole and f(1, 12, 1, 64) == whole and f(1, 16, 1, 64) == 4
-    assert f(8, 1024, 32, 128) == whole and f(2, 128, 64, 128) == whole
+    assert f(1, 3, 1, 64) == whole and f(1, 12, 1, 64) == 2 and f(1, 256, 1, 64) == 8
+    assert f(8, 1024, 32, 128) == whole and f(2, 128, 64, 128) == 32
     assert f(0, 0, 1, 64) == whole and f(1, 0, 1, 64) == whole
     assert f(1, 1 << 25, 1, 64) == 1 << 17
+
+
+def test_segments_of_packed_sequences():
+    """All segments at once where they fit, by the average where they do not, none of few chunks."""
+    f = importlib.import_module("tops.ops.delta.gated_delta_rule")._segment
+    for counts in ([28, 5, 33, 2, 47, 1, 8, 9], [30, 40, 50], [0, 256, 0], [7]):
+        L = f(counts, 16)
+        assert 2 <= L <= max(counts) / 2 and sum(-(-n // L) for n in counts) * 16 <= 256
+    assert f([4] * 40 + [200], 16) == 23 and f([4] * 40, 16) == 4
+    assert f([0, 0], 16) == 1 and f([3, 5, 1], 1) == 5 and f([60] * 16, 16) == 60
 
 
 # ---------------------------------------------------------------------------
