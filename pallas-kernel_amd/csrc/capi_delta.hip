@@ -196,8 +196,8 @@ int tops_gla_delta_step(const tops_gla_delta_step_args* a, void* stream) {
   if (a->slots_idx == nullptr && a->batch > a->slots)
     return fail(TOPS_GLA_EINVAL, "the states hold %lld rows, the batch %lld", (long long)a->slots,
                 (long long)a->batch);
-  if (a->batch > kMax || a->T > kMax || !grid_fits((a->V + 127) / 128 * a->HV, 256) ||
-      !grid_fits((a->V + 127) / 128 * a->HV * a->batch, 256))
+  if (a->batch > kMax || a->T > kMax || !grid_fits((a->V + 31) / 32 * a->HV, 64) ||
+      !grid_fits((a->V + 31) / 32 * a->HV * a->batch, 64))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   if (a->batch > 0 && a->T > 0 && any_null({a->q, a->k, a->v, a->g, a->beta, a->o}))
     return fail(TOPS_GLA_EINVAL, "q, k, v, g, beta and o must not be NULL");
