@@ -79,12 +79,32 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   double* sG = (double*)(smem + L::G0);
   float* sf = (float*)(smem + L::F0);   // the unit's vectors; dG, k . beta z, <S, dS>
   float *sdG = sf + 7 * C, *sKz = sf + 8 * C, *sSum = sf + 9 * C;
+  const int group = HV / H;
+  // a slab of a value head, on its way while the one before is multiplied; all of a block's first
+  // loads start together
+  TileFetch<T, VS, C, NT> fn, fy;
+  TileFetch<T, VS, KP, NT> fs, fd;
+  TileFetch<T, C, VS, NT> fo;
+  Run<T, 8> fv;
+  auto fetch = [&](int hv, int v0) {
+    const long unit = (long)chunk * HV + hv;
+    fn.get((const T*)p.N + (unit * V + v0) * C, C, V - v0, C, tid);
+    fy.get((const T*)p.Y + (unit * V + v0) * C, C, V - v0, C, tid);
+    fs.get((const T*)p.S + (unit * V + v0) * KP, KP, V - v0, KP, tid);
+    fd.get((const T*)p.dS + (unit * V + v0) * KP, KP, V - v0, KP, tid);
+    fo.get((const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh + v0, a.do_st, at.len,
+           V - v0, tid);
+    if (!key)
+      fv = get_run<T, 8>((const T*)a.v + at.b * a.v_sb + (at.t + (long)min(i, at.len - 1)) * a.v_st +
+                         hv * a.v_sh + min(v0 + 8 * g, V - 8));
+  };
   {
-    TileFetch<T, C, KP, NT> f;
-    f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
-    f.put(sK, L::PK, at.len, K, tid);
-    f.get((const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh, a.q_st, at.len, K, tid);
-    f.put(sQ, L::PK, at.len, K, tid);
+    TileFetch<T, C, KP, NT> fk, fq;
+    fk.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
+    fq.get((const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh, a.q_st, at.len, K, tid);
+    fetch(h * group, 0);
+    fk.put(sK, L::PK, at.len, K, tid);
+    fq.put(sQ, L::PK, at.len, K, tid);
   }
   const T *kr = sK + i * L::PK, *qr = sQ + i * L::PK;
   const float scale = (float)a.scale;
@@ -93,28 +113,11 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
   for (int x = 0; x < (GROUP ? 2 * NS : 1); ++x) sum[x] = zero4();
 
-  const int group = HV / H;
   for (int gi = 0; gi < group; ++gi) {
     const int hv = h * group + gi;
     const long unit = (long)chunk * HV + hv;
     const long tok = (long)at.b * a.T + at.t + i;
-    const T* vp = (const T*)a.v + at.b * a.v_sb + (at.t + (long)min(i, at.len - 1)) * a.v_st +
-                  hv * a.v_sh;
-    const T* dop = (const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh;
     T* dvp = (T*)a.dv + (tok * HV + hv) * V;
-    TileFetch<T, VS, C, NT> fn, fy;
-    TileFetch<T, VS, KP, NT> fs, fd;
-    TileFetch<T, C, VS, NT> fo;
-    Run<T, 8> fv;
-    auto fetch = [&](int v0) {
-      fn.get((const T*)p.N + (unit * V + v0) * C, C, V - v0, C, tid);
-      fy.get((const T*)p.Y + (unit * V + v0) * C, C, V - v0, C, tid);
-      fs.get((const T*)p.S + (unit * V + v0) * KP, KP, V - v0, KP, tid);
-      fd.get((const T*)p.dS + (unit * V + v0) * KP, KP, V - v0, KP, tid);
-      fo.get(dop + v0, a.do_st, at.len, V - v0, tid);
-      if (!key) fv = get_run<T, 8>(vp + min(v0 + 8 * g, V - 8));
-    };
-    fetch(0);
     if (GROUP) __syncthreads();   // the vectors of the head before have been read
     {
       const float* vec = delta_vec(p, unit);
@@ -146,7 +149,10 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
       }
       const Run<T, 8> vr = fv;
       __syncthreads();
-      if (v0 + VS < V) fetch(v0 + VS);
+      if (v0 + VS < V)
+        fetch(hv, v0 + VS);
+      else if (GROUP && gi + 1 < group)
+        fetch(hv + 1, 0);
       beta = sf[2 * C + i];
       if (!key) {
         const Frag<T> of = ld_frag(sO + i * L::PS + 8 * g);
