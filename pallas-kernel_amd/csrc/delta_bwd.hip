@@ -5,7 +5,8 @@
 // normed ones:
 //   dN = P^T dO + e^{G_C - G} (K dS),   Y = Tm^T dN,
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) - K^T (beta e^G Y),
-// which goes from chunk to chunk (delta_scan.hip); then, here, for every chunk at once, with dP = dO N^T for j <= i and E = Y N^T for j < i:
+// which goes from chunk to chunk (delta_scan.hip); then, here, for every chunk at once, with
+// dP = dO N^T for j <= i and E = Y N^T for j < i:
 //   dq  = scale (e^G (dO S^T) + (dP D) K),
 //   z   = -(e^G (Y S^T) + (E D) K),                    (what k reads with, over beta)
 //   dkw = e^{G_C - G} (N dS^T) + scale (dP D)^T Q - (beta E D)^T K,     (what k writes with)
@@ -23,7 +24,9 @@ namespace {
 
 template <typename T, int KP>
 struct GradLds {
-  static constexpr int C = delta_c<T>(), VS = 32;   // values of a slab
+  // values of a slab: as many as registers have room for (K = 64, V = 128, two value heads a key
+  // head: 45 us for 52 with 32; K = 128: 64 spill, 310 us of gradients for 286)
+  static constexpr int C = delta_c<T>(), VS = sizeof(T) == 2 && KP == 64 ? 64 : 32;
   static constexpr int PK = pitch_of<T>(KP), PC = pitch_of<T>(C), PS = pitch_of<T>(VS);
   static constexpr int K0 = 0, Q0 = C * PK, N0 = 2 * C * PK, Y0 = N0 + VS * PC, S0 = Y0 + VS * PC;
   static constexpr int D0 = S0 + VS * PK, O0 = D0 + VS * PK, END = O0 + C * PS;
@@ -62,7 +65,8 @@ __device__ __forceinline__ float row_dot(const T* row, const f32x4 (&acc)[2 * NS
 template <typename T, int KP, bool GROUP>
 __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParams p) {
   using L = GradLds<T, KP>;
-  constexpr int C = L::C, NT = 8 * C, NS = KP / 32, NU = C / 32, VS = L::VS, NW = C / 16;
+  constexpr int C = L::C, NT = 8 * C, NS = KP / 32, NU = C / 32, NW = C / 16;
+  constexpr int VS = L::VS, NH = VS / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tw = wave % NW;
@@ -85,7 +89,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   TileFetch<T, VS, C, NT> fn, fy;
   TileFetch<T, VS, KP, NT> fs, fd;
   TileFetch<T, C, VS, NT> fo;
-  Run<T, 8> fv;
+  Run<T, 8> fv[NH];
   auto fetch = [&](int hv, int v0) {
     const long unit = (long)chunk * HV + hv;
     fn.get((const T*)p.N + (unit * V + v0) * C, C, V - v0, C, tid);
@@ -95,8 +99,11 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     fo.get((const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh + v0, a.do_st, at.len,
            V - v0, tid);
     if (!key)
-      fv = get_run<T, 8>((const T*)a.v + at.b * a.v_sb + (at.t + (long)min(i, at.len - 1)) * a.v_st +
-                         hv * a.v_sh + min(v0 + 8 * g, V - 8));
+#pragma unroll
+      for (int u = 0; u < NH; ++u)
+        fv[u] = get_run<T, 8>((const T*)a.v + at.b * a.v_sb + hv * a.v_sh +
+                              (at.t + (long)min(i, at.len - 1)) * a.v_st +
+                              min(v0 + 32 * u + 8 * g, V - 8));
   };
   {
     TileFetch<T, C, KP, NT> fk, fq;
@@ -147,50 +154,59 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
         for (int e = 0; e < 8; ++e) sd = fmaf(ss[e], dd[e], sd);
       }
-      const Run<T, 8> vr = fv;
+      Run<T, 8> vr[NH];
+#pragma unroll
+      for (int u = 0; u < NH; ++u) vr[u] = fv[u];
       __syncthreads();
       if (v0 + VS < V)
         fetch(hv, v0 + VS);
       else if (GROUP && gi + 1 < group)
         fetch(hv + 1, 0);
       beta = sf[2 * C + i];
-      if (!key) {
-        const Frag<T> of = ld_frag(sO + i * L::PS + 8 * g);
-        const Frag<T> yf = ld_frag_t(sY + 16 * tw, L::PC, lane);
-        const int c = v0 + 8 * g;
-        float y[8], x[8];   // dv, and v . Y (Y is 0 past the end)
-        values_of(yf, y);
-        values_of(frag_of<T>(cut_run(vr, c, V)), x);
+#pragma unroll 1
+      for (int u = 0; u < NH; ++u) {   // 32 values
+        const T *uN = sN + 32 * u * L::PC, *uY = sY + 32 * u * L::PC, *uO = sO + 32 * u;
+        if (u > 0 && v0 + 32 * u >= V) break;
+        if (!key) {
+          const Frag<T> of = ld_frag(uO + i * L::PS + 8 * g);
+          const Frag<T> yf = ld_frag_t(uY + 16 * tw, L::PC, lane);
+          const int c = v0 + 32 * u + 8 * g;
+          float y[8], x[8];   // dv, and v . Y (Y is 0 past the end)
+          values_of(yf, y);
+          values_of(frag_of<T>(cut_run(u ? vr[NH - 1] : vr[0], c, V)), x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          vy = in ? fmaf(x[e], y[e], vy) : 0.f;
-          y[e] *= beta;
-        }
-        if (in && c < V) put_run<T, 8>(dvp + c, y, V - c);
-#pragma unroll
-        for (int n = 0; n < 2 * NU; ++n)
-          if ((n >> 1) <= uw) {
-            const Frag<T> f = ld_pair_t(sN + 32 * (n >> 1), L::PC, lane, n & 1);
-            mma(B[0][n], f, of);
-            mma(B[1][n], f, yf);
+          for (int e = 0; e < 8; ++e) {
+            vy = in ? fmaf(x[e], y[e], vy) : 0.f;
+            y[e] *= beta;
           }
+          if (in && c < V) put_run<T, 8>(dvp + c, y, V - c);
 #pragma unroll
-        for (int n = 0; n < 2 * NS; ++n) {
-          const Frag<T> f = ld_pair_t(sS + 32 * (n >> 1), L::PK, lane, n & 1);
-          mma(A[0][n], f, of);
-          mma(A[1][n], f, yf);
-        }
-      } else {
-        const Frag<T> nf = ld_frag_t(sN + 16 * tw, L::PC, lane);
+          for (int n = 0; n < 2 * NU; ++n)
+            if ((n >> 1) <= uw) {
+              const Frag<T> f = ld_pair_t(uN + 32 * (n >> 1), L::PC, lane, n & 1);
+              mma(B[0][n], f, of);
+              mma(B[1][n], f, yf);
+            }
 #pragma unroll
-        for (int n = 0; n < 2 * NU; ++n)
-          if ((n >> 1) >= uw) {
-            mma(B[0][n], ld_frag(sO + (32 * (n >> 1) + pair_row(lane, n & 1)) * L::PS + 8 * g), nf);
-            mma(B[1][n], ld_pair_t(sY + 32 * (n >> 1), L::PC, lane, n & 1), nf);
+          for (int n = 0; n < 2 * NS; ++n) {
+            const Frag<T> f =
+                ld_pair_t(sS + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1);
+            mma(A[0][n], f, of);
+            mma(A[1][n], f, yf);
           }
+        } else {
+          const Frag<T> nf = ld_frag_t(uN + 16 * tw, L::PC, lane);
 #pragma unroll
-        for (int n = 0; n < 2 * NS; ++n)
-          mma(A[0][n], ld_pair_t(sD + 32 * (n >> 1), L::PK, lane, n & 1), nf);
+          for (int n = 0; n < 2 * NU; ++n)
+            if ((n >> 1) >= uw) {
+              const int r = 32 * (n >> 1) + pair_row(lane, n & 1);
+              mma(B[0][n], ld_frag(uO + r * L::PS + 8 * g), nf);
+              mma(B[1][n], ld_pair_t(uY + 32 * (n >> 1), L::PC, lane, n & 1), nf);
+            }
+#pragma unroll
+          for (int n = 0; n < 2 * NS; ++n)
+            mma(A[0][n], ld_pair_t(sD + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1), nf);
+        }
       }
     }
     // Gradients of the raw q and k, but for the norms' own part; z times beta (times 1 where beta is
