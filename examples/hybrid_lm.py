@@ -1,7 +1,9 @@
 """A small language model of a selective state space block and a gated linear attention block with
 normed, rotated queries and keys: trained on a synthetic task, then served token by token.
 
-    python examples/hybrid_lm.py [--steps 1000]
+    python examples/hybrid_lm.py [--steps 1000] [--delta]
+
+With ``--delta`` a block of the gated delta rule behind a layer norm goes between the two.
 
 The task: a sequence of random symbols, a separator, and the same symbols again; the loss counts
 the second half. Serving runs prompts of different lengths packed into one row, keeps their states
@@ -19,6 +21,8 @@ from torch import nn
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..",
                                 "pallas-kernel_amd"))
 
+from tops.modules import LayerNorm   # noqa: E402
+from tops.ops.delta import gated_delta_rule, gated_delta_rule_step   # noqa: E402
 from tops.ops.gla import chunk_gla, fused_recurrent_gla   # noqa: E402
 from tops.ops.rope import qk_norm_rope, rotary_inv_freq   # noqa: E402
 from tops.ops.ssm import (causal_conv1d, causal_conv1d_step, selective_scan,   # noqa: E402
@@ -73,6 +77,49 @@ class SelectiveBlock(nn.Module):
         return h + self.out_proj(y)
 
 
+class DeltaBlock(nn.Module):
+    """Gated delta rule of convolved queries, keys and values, behind a layer norm; each key head
+    serves two value heads."""
+
+    def __init__(self, width, heads, conv_width=4):
+        super().__init__()
+        self.heads, self.dim, self.W = heads, width // heads, conv_width
+        self.sizes = [width // 2, width // 2, width]
+        self.norm = LayerNorm(width)
+        self.qkv = nn.Linear(width, 2 * width, bias=False)
+        self.conv = nn.Parameter(torch.randn(2 * width, conv_width) * conv_width ** -0.5)
+        self.gates = nn.Linear(width, 2 * heads)
+        self.A_log = nn.Parameter(torch.log(torch.linspace(0.01, 0.5, heads)))
+        self.out_proj = nn.Linear(width, width, bias=False)
+
+    def _inputs(self, h):
+        x = self.norm(h)
+        a, b = self.gates(x).float().chunk(2, -1)
+        return self.qkv(x), -torch.exp(self.A_log.float()) * F.softplus(a), torch.sigmoid(b)
+
+    def _heads(self, x):
+        return [t.unflatten(-1, (-1, self.dim)) for t in x.split(self.sizes, -1)]
+
+    def forward(self, h, cu=None, keep=False):
+        x, g, beta = self._inputs(h)
+        x, window = causal_conv1d(x, self.conv, activation="silu", output_final_state=keep,
+                                  cu_seqlens=cu)
+        o, state = gated_delta_rule(*self._heads(x), g, beta, output_final_state=keep,
+                                    cu_seqlens=cu, qk_l2norm=True)
+        return h + self.out_proj(o.flatten(-2)), (window, state)
+
+    def empty_pool(self, slots, like):
+        return (like.new_zeros(slots, self.W, sum(self.sizes)),
+                torch.zeros(slots, self.heads, self.dim, self.dim, device=like.device))
+
+    def step(self, h, pool, slots):
+        x, g, beta = self._inputs(h)
+        x = causal_conv1d_step(x, pool[0], self.conv, activation="silu", state_indices=slots)
+        o = gated_delta_rule_step(pool[1], *self._heads(x), g, beta, qk_l2norm=True,
+                                  state_indices=slots)
+        return h + self.out_proj(o.flatten(-2))
+
+
 class AttentionBlock(nn.Module):
     """Gated linear attention of queries and keys that are normed for each head and rotated."""
 
@@ -112,18 +159,23 @@ class AttentionBlock(nn.Module):
 
 
 class HybridLM(nn.Module):
-    def __init__(self, vocab=64, width=256, heads=4):
+    def __init__(self, vocab=64, width=256, heads=4, delta=False):
         super().__init__()
         self.embed = nn.Embedding(vocab, width)
         self.ssm = SelectiveBlock(width, 2 * width)
         self.attention = AttentionBlock(width, heads)
         self.norm = nn.RMSNorm(width)
         self.head = nn.Linear(width, vocab, bias=False)
+        self.delta = DeltaBlock(width, heads) if delta else None
 
     def forward(self, tokens, positions=None, cu=None, keep=False):
         h, ssm = self.ssm(self.embed(tokens), cu, keep)
+        more = ()
+        if self.delta:
+            h, delta = self.delta(h, cu, keep)
+            more = delta,
         h, att = self.attention(h, positions, cu, keep)
-        return self.head(self.norm(h)), (ssm, att)
+        return self.head(self.norm(h)), (ssm, att, *more)
 
     @torch.no_grad()
     def prefill(self, prompts, pools, slots):
@@ -134,19 +186,24 @@ class HybridLM(nn.Module):
             cu.append(cu[-1] + len(p))
         dev = self.embed.weight.device
         tokens = torch.tensor([t for p in prompts for t in p], device=dev)[None]
-        logits, ((window, state), att) = self(tokens, positions_of(cu, dev), cu, True)
+        logits, states = self(tokens, positions_of(cu, dev), cu, True)
         at = slots.long()
-        pools[0][0][at], pools[0][1][at], pools[1][at] = window, state, att
+        for pool, state in zip(pools, states):
+            for p, s in zip(pool, state) if isinstance(pool, tuple) else [(pool, state)]:
+                p[at] = s
         return logits[0, torch.tensor(cu[1:], device=dev) - 1]
 
     def empty_pools(self, slots):
         like = self.embed.weight
-        return self.ssm.empty_pool(slots, like), self.attention.empty_pool(slots, like)
+        pools = self.ssm.empty_pool(slots, like), self.attention.empty_pool(slots, like)
+        return (*pools, self.delta.empty_pool(slots, like)) if self.delta else pools
 
     @torch.no_grad()
     def step(self, tokens, positions, pools, slots):
         """The next token of each sequence: tokens and positions [B]."""
         h = self.ssm.step(self.embed(tokens), pools[0], slots)
+        if self.delta:
+            h = self.delta.step(h, pools[2], slots)
         h = self.attention.step(h, positions, pools[1], slots)
         return self.head(self.norm(h))
 
@@ -193,10 +250,11 @@ def generate(model, prompts, new, slots=None):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=1000)
+    ap.add_argument("--delta", action="store_true")
     args = ap.parse_args()
     torch.manual_seed(0)
     dev = torch.device("cuda:0")
-    model = HybridLM().to(dev)
+    model = HybridLM(delta=args.delta).to(dev)
     train(model, args.steps, dev)
     gen = torch.Generator().manual_seed(1)
     symbols = [torch.randint(1, 64, (n,), generator=gen).tolist() for n in (5, 24, 12)]
