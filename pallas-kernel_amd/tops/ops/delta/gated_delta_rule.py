@@ -198,10 +198,13 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
 
     Inputs may be views with any strides whose last dimension is contiguous (others are copied).
     bfloat16 q, k and v are read and written as they are, and multiplied in bfloat16 with float32
-    sums; states and what goes into them keep the accuracy of float32 (operands in two parts).
-    Other types of q, k and v are computed in float32. g and beta are read in float32 or bfloat16,
-    whatever the others' type, and their gradients returned in it: with bfloat16 q, k and v these
-    have the accuracy of bfloat16 products.
+    sums. States are float32, and multiplied as two bfloat16 parts of 16 bits: final states and
+    gradients of initial ones are a few 1e-6 of their size off. Other types of q, k and v are
+    computed in float32. g and beta are read in float32 or bfloat16, whatever the others' type, and
+    their gradients returned in it: with bfloat16 q, k and v these have the accuracy of bfloat16
+    products. Inputs that are not finite make the outputs of their chunk of 64 tokens (float32: 32)
+    and of all later ones of the sequence and head not finite, also those before them in the chunk.
+    A second derivative raises.
 
     Returns ``(o, final_state)``: o ``[B, T, HV, V]`` in v's type, final_state ``[sequences, HV, K,
     V]`` float32 with ``output_final_state``, else None.

@@ -112,6 +112,66 @@ def test_segments(lens, K, V, dt):
         check(x, r, norm=True)
 
 
+@pytest.mark.parametrize("lens", [[400], [130] * 10 + [900, 0, 640]])
+@pytest.mark.parametrize("dt", [FL, BF])
+def test_segments_of_few_chunks_and_of_many_sequences(lens, dt):
+    """Two chunks a segment; and more blocks than run at once, long sequences among short ones."""
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    x, r = make(1, cu[-1], 3, 6, 32, 500, dt, S=len(lens), norm=True)
+    x["g"] *= 0.05
+    check(x, r, cu=cu, norm=True)
+
+
+@pytest.mark.parametrize("value", [-50.0, float(torch.finfo(FL).min), -torch.inf])
+@pytest.mark.parametrize("dt", [FL, BF])
+def test_strong_decays_over_segments(value, dt):
+    """A segment that forgets all before it, at its first, last or another token, and one that
+    does not."""
+    x, r = make(1, 1000, 1, 2, 64, 32, dt, norm=True, gdt=FL)
+    x["g"] *= 0.05
+    x["g"][:, [128, 255, 300, 511, 512, 513]] = value
+    if value == -torch.inf:   # the oracle's gradients of these decays are inf * 0
+        d = {n: t.to(DEV).requires_grad_() for n, t in x.items()}
+        o, ht = gated_delta_rule(**d, output_final_state=True, qk_l2norm=True)
+        grads = torch.autograd.grad([o, ht], list(d.values()),
+                                    [torch.ones_like(o), torch.ones_like(ht)])
+        assert all(torch.isfinite(t).all() for t in grads)
+        x["g"].clamp_(min=-1000.0)   # e^-1000 is 0 in the oracle too
+    check(x, r, norm=True)
+
+
+def test_packed_sequences_are_independent():
+    """Inputs of a sequence that are not finite leave the others' outputs, final states and
+    gradients as they are, with segments and without."""
+    lens = [70, 900, 60, 800, 3]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    x, r = make(1, cu[-1], 1, 2, 64, 32, BF, S=len(lens), norm=True)
+    up = r(1, cu[-1], 2, 32).to(BF).to(DEV), r(len(lens), 2, 64, 32).to(DEV)
+
+    def run(**bad):
+        d = {n: t.to(DEV) for n, t in x.items()}
+        for n, (i, b) in bad.items():
+            d[n][0, i] = b
+        d = {n: t.requires_grad_() for n, t in d.items()}
+        o, ht = gated_delta_rule(**d, output_final_state=True, cu_seqlens=cu, qk_l2norm=True)
+        *grads, dh = torch.autograd.grad([o, ht], list(d.values()), up)
+        tokens = [t.split(lens, 1) for t in (o, *grads)]
+        return [[ht[s], dh[s], *(t[s] for t in tokens)] for s in range(len(lens))]
+
+    want = run()
+    for name, bad in (("v", torch.inf), ("k", torch.nan), ("g", torch.inf), ("beta", torch.nan)):
+        for s in (1, 2):   # a sequence of segments, and one without
+            got = run(**{name: (cu[s] + 30, bad)})
+            assert not torch.isfinite(got[s][0]).all()
+            for e in range(len(lens)):
+                if e != s:
+                    assert all(torch.equal(a, b) for a, b in zip(want[e], got[e])), (name, s, e)
+
+
 @pytest.mark.parametrize("B,T", [(0, 5), (2, 0), (0, 0)])
 @pytest.mark.parametrize("dt", [FL, BF])
 def test_no_tokens(B, T, dt):
@@ -330,6 +390,29 @@ def test_captured(cu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out)), i
+
+
+def test_two_graphs_and_eager_calls_in_turn():
+    """Two captured calls, one of segments, replayed in turn with eager calls between."""
+    runs = []
+    for T, K in ((70, 64), (700, 128)):
+        x, _ = make(1, T, 1, 2, K, 64, BF, norm=True)
+        d = {n: t.to(DEV) for n, t in x.items()}
+        call = lambda d=d: gated_delta_rule(   # noqa: E731
+            **d, output_final_state=True, qk_l2norm=True)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        runs.append((d, call, graph, out))
+    for i in range(4):
+        for d, *_ in runs:
+            d["v"].mul_(0.7).add_(0.1 * i)
+        for _, _, graph, _ in runs:
+            graph.replay()
+        for _, call, _, out in runs:
+            assert all(torch.equal(a, b) for a, b in zip(call(), out)), i
 
 
 def test_packed_lengths_new_to_a_capture_raise():
