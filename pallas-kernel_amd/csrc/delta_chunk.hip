@@ -30,12 +30,19 @@ __device__ __forceinline__ void mma16(f32x4& acc, const float* X, int px, const 
 
 // A block has a chunk and a key head, and goes through its value heads. K K^T on the matrix units;
 // the inverse in float32: the 16 x 16 diagonal blocks by substitution, a lane a column, then the
-// blocks below them, one diagonal after another: T_ij = -T_ii sum_k A_ik T_kj.
+// blocks below them, one diagonal after another: T_ij = -T_ii sum_k A_ik T_kj. Bound by the latency
+// of these few steps: four blocks a CU, T where the keys were, gates on their way early: 16384 tokens
+// of 16 heads of 128 keys in 47 us (three blocks, in turn: 57); the keys read and T written alone
+// would take 24.
 template <typename T, int KP>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
+__global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
   constexpr int C = delta_c<T>(), NB = C / 16, PK = pitch_of<T>(KP), PA = C + 4;
-  __shared__ __attribute__((aligned(16))) T sK[C * PK];
-  __shared__ __attribute__((aligned(16))) float sA[C * PA], sT[C * PA];
+  // the keys, and then, for each value head, T
+  constexpr int FIRST = std::max(C * PK * (int)sizeof(T), C * PA * 4);
+  __shared__ __attribute__((aligned(16))) unsigned char first[FIRST];
+  __shared__ __attribute__((aligned(16))) float sA[C * PA];
+  T* sK = (T*)first;
+  float* sT = (float*)first;
   __shared__ double sG[C];
   __shared__ float sBeta[C], sRk[C];
   const tops_gla_delta_args& a = p.a;
@@ -43,6 +50,17 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
   const int H = (int)a.H, HV = (int)a.HV, K = (int)a.K;
   const int chunk = (int)(blockIdx.x / H), h = (int)(blockIdx.x % H);
   const ChunkAt at = delta_chunk_at(a, C, chunk);
+  // the first value head's gates on their way with the keys, the next one's while a head is worked on
+  const long g_at = at.b * a.g_sb + (long)(at.t + min(lane, at.len - 1)) * a.g_st;
+  const long b_at = at.b * a.beta_sb + (long)(at.t + min(lane, at.len - 1)) * a.beta_st;
+  float g_next = 0.f, beta_next = 0.f;
+  auto gates = [&](int hv) {
+    if (wave == 0) {
+      g_next = get_any(a.g, (int)a.g_dtype, g_at + hv);
+      beta_next = get_any(a.beta, (int)a.beta_dtype, b_at + hv);
+    }
+  };
+  gates(h * (HV / H));
   {
     TileFetch<T, C, KP, 256> f;
     f.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
@@ -71,17 +89,14 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
       if (j <= wave) mma_tile<T>(kk[j], sK + wave * 16 * PK, PK, sK + j * 16 * PK, PK, KP, lane);
     }
   }
+  __syncthreads();
   const int group = HV / H;
   for (int gi = 0; gi < group; ++gi) {
     const int hv = h * group + gi;
     const long unit = (long)chunk * HV + hv;
     if (wave == 0) {
-      float g = 0.f, beta = 0.f;
-      if (lane < at.len) {
-        g = log_decay(get_any(a.g, (int)a.g_dtype, at.b * a.g_sb + (at.t + lane) * a.g_st + hv));
-        beta = get_any(a.beta, (int)a.beta_dtype,
-                       at.b * a.beta_sb + (at.t + lane) * a.beta_st + hv);
-      }
+      const float g = lane < at.len ? log_decay(g_next) : 0.f;
+      const float beta = lane < at.len ? beta_next : 0.f;
       double s = g;
 #pragma unroll
       for (int o = 1; o < C; o <<= 1) {
@@ -93,7 +108,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p) {
         sBeta[lane] = beta;
       }
     }
-    for (int i = tid; i < C * C; i += 256) sT[i / C * PA + i % C] = 0.f;
+    if (gi + 1 < group) gates(hv + 1);
+#pragma unroll
+    for (int b = 0; b < C / 32; ++b)   // what is stored of T above the diagonal blocks
+      sT[(32 * b + tid / 16) * PA + 32 * b + 16 + tid % 16] = 0.f;
     __syncthreads();
     if (tid < C) {
       float* vec = delta_vec(p, unit);
