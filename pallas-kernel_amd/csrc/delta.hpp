@@ -127,7 +127,7 @@ struct DeltaParams {
                                 // right side
   // where a sequence has several segments, for each of all segments and value heads: the state
   // after it [K][V] (E) or the gradient of the state before it (dE), float32, and what it makes of
-  // a state before it, [KP][KP] in two layouts (M row-major, Mt column-major), tiles as Tm's
+  // a state before it, [KP][KP] (M, and Mt its transpose), in the order of the fold's operands, parts as Tm's
   float *E, *dE;
   char *M, *Mt;
   int multi;

@@ -1,7 +1,7 @@
 // The states of the gated delta rule, from chunk to chunk, and their gradients the other way
 // (include/tops_gla_delta.h; formulas and names in delta_chunk.hip and delta_bwd.hip).
 //
-// The columns of S and N are independent of one another: a wave owns 16 or 32 of them over all
+// The columns of S and N are independent of one another: a wave owns 16 of them over all
 // chunks of a sequence and head, with the state in its accumulators; K S, Tm R and K^T N hand their
 // results on as operands without leaving a lane. A block's waves share the chunk's tiles in LDS,
 // with the next chunk's on their way.
@@ -12,6 +12,16 @@
 // from the identity and without values. A first pass has E and M of all segments at once, the fold
 // E_j <- M_j E_{j-1} + E_j the state after each, and a second pass runs all segments from there.
 // The gradients run with the same maps transposed.
+//
+// A chunk's step of the second pass has, for 128 keys and a wave's 16 values, 116 matrix
+// instructions of 16 cycles (the state's products in two parts, the system, scores and outputs) and
+// 740 others, most of them making operands: for the two waves of a SIMD 9600 cycles, of the 14400 that
+// a step takes; the rest are waits for LDS and barriers (44 % of a wave's time). Eight waves a block
+// share the tiles (against four with twice the columns 7 to 15 % faster), and its halves go through
+// the step in different orders, so that one's matrix instructions meet the other's others (second
+// pass 127 -> 118 us). 16384 tokens of 16 heads of 128 x 128: first pass 141 us (29 blocks a head for
+// 16 segments), second, with the outputs, 117, 2.9 TB/s; training of 2 x 4096 tokens: 80 and 79,
+// and the gradients' 54 and 65.
 #include "delta.hpp"
 
 namespace tops {
@@ -62,6 +72,14 @@ __device__ __forceinline__ SegAt seg_at(const tops_gla_delta_args& a, int C, int
 __device__ __forceinline__ int spread(int blk, int n) {
   const int r = blk % n;
   return blk - r + xcd_remap(r, n);
+}
+
+// Where a map's element (row, col) lies: in the order of the fold's operands (rows of pair_row, 8
+// columns a lane), so that a wave's load is 1024 bytes side by side.
+template <int KP>
+__device__ __forceinline__ int map_at(int row, int col) {
+  const int lane = 16 * (col >> 3 & 3) + 4 * (row >> 3 & 3) + (row & 3);
+  return (((row >> 5) * 2 + (row >> 2 & 1)) * (KP / 32) + (col >> 5)) * 512 + 8 * lane + (col & 7);
 }
 
 // A head's columns go to blocks of NW waves of 16, of V or, in a first pass, then of KP for M.
@@ -426,7 +444,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     store_o(buf, left + C);
   }
   if (idle) return;
-  if (map) {   // [KP][KP]: column v, rows in the lane's order
+  if (map) {   // column v, rows in the lane's order
     const long tile = (long)KP * KP;
     T* M = (T*)(p.M + ((long)at.seg * HV + hv) * tile * 4);
     T* Mt = (T*)(p.Mt + ((long)at.seg * HV + hv) * tile * 4);
@@ -435,15 +453,16 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       float x[8], y[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Split<T> f = split_of<T>(x);
-      if (a.train) st_frag(Mt + v * KP + 32 * s + 8 * g, high_of(f));
+      const int row = 32 * s + 8 * g;
+      if (a.train) st_frag(Mt + map_at<KP>(v, row), high_of(f));
       values_of(high_of(f), y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) M[(32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
+      for (int e = 0; e < 8; ++e) M[map_at<KP>(row + e, v)] = from_f32<T>(y[e]);
       if constexpr (sizeof(T) == 2) {
-        if (a.train) st_frag(Mt + tile + v * KP + 32 * s + 8 * g, f.lo);
+        if (a.train) st_frag(Mt + tile + map_at<KP>(v, row), f.lo);
         values_of(f.lo, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) M[tile + (32 * s + 8 * g + e) * KP + v] = from_f32<T>(y[e]);
+        for (int e = 0; e < 8; ++e) M[tile + map_at<KP>(row + e, v)] = from_f32<T>(y[e]);
       }
     }
   } else if (FIRST) {
@@ -646,7 +665,9 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 // E_j <- M_j E_{j-1} + E_j along the segments of a sequence and head, or dE_j <- M_j^T dE_{j+1} +
 // dE_j the other way. A block has 16 columns, each of its waves KP / 4 or KP / 2 of the rows; the
 // states go from wave to wave through LDS as operands, the maps and parts of the next segment are
-// on their way meanwhile.
+// on their way meanwhile. Bound by the maps' way through the caches, each read by every block of the
+// head: 16 segments of 16 heads of 128 x 128 in 22 us (maps in rows, 64 bytes a row and load: 33; two
+// segments ahead so: 40).
 template <typename T, int KP, bool BACK>
 __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaParams p) {
   constexpr int NS = KP / 32, NW = KP == 64 ? 2 : 4, NR = NS / NW, PARTS = sizeof(T) == 2 ? 2 : 1;
@@ -684,8 +705,7 @@ __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaP
     for (int i = 0; i < 2 * NR; ++i)
 #pragma unroll
       for (int s = 0; s < NS; ++s)
-        M[i][s] = ld_split<T>(m, (int)tile, (k0 + 32 * (i >> 1) + pair_row(lane, i & 1)) * KP +
-                                                32 * s + 8 * g);
+        M[i][s] = ld_split<T>(m, (int)tile, ((wave * 2 * NR + i) * NS + s) * 512 + 8 * lane);
     load_rows(E, state(n) + min(v, V - 1), k0 + 8 * g, K, V);
   };
   auto share = [&](int n) {   // the wave's rows of the state after step n, and to memory
