@@ -50,7 +50,7 @@ def _segment(counts, blocks):
     L = max(-(-sum(counts) * blocks // _CUS), 2, math.isqrt(max(0, longest - 1) // 4) + 1)
     if len(counts) * blocks <= _CUS:
         while L < longest and sum(-(-n // L) for n in counts) * blocks > _CUS:
-            L += 1
+            L += max(1, L // 32)
     return L if longest >= 6 and longest >= 2 * L else max(1, longest)
 
 
