@@ -10,24 +10,34 @@
 // whose share of w, b, dw and db stays in its registers over all its rows: up to 1024 features a row
 // belongs to one wave, above to a block of 2 to 16. The weights' sums go through one partial row a
 // block in a workspace and a second kernel, in fixed order.
+//
+// What bounds it is how many loads are on their way: the gradients of 32768 x 2048 bfloat16, 403 MB,
+// take 84 us, 4.8 TB/s, with 8 features a thread and 20 waves a CU, with 16 features, twice the
+// registers, and 12 waves 105, 8 waves 139. In float32 16 features are as many bytes again: 16384 x
+// 2048 in 91 us, sums included, with 8 waves of 16 features, 95 with 20 of 8; 65536 x 768 in 123 with
+// 8 waves, 128 with 12. The forward's 268 MB take 64 us, 4.2 TB/s, with 16 features (with 8: 71). The
+// sums over 1280 blocks' partial rows take 12.
 #include "delta.hpp"
 
 namespace tops {
 
 namespace {
 
-constexpr long FWD_WAVES = 16, BWD_WAVES = 8;
-
-// Threads of a row by its features, 16 a thread at most, and of a block: four rows of one wave, or
-// one row.
-int row_threads(long D) {
-  return D <= 1024 ? 64 : D <= 2048 ? 128 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024;
+// Threads of a row by its features: 16 a thread, or 8 (`few`: the gradients of bfloat16), but 16 where
+// 64 threads have them (a block of 128 would write a partial row for each row) or 1024 threads must.
+// And of a block: four rows of one wave, or one row.
+int row_threads(long D, bool few) {
+  if (D <= 1024) return 64;
+  const long n = few ? D : D / 2 + D % 2;
+  return n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024;
 }
 constexpr int block_threads(int nt) { return nt == 64 ? 256 : nt; }
-long norm_blocks(long rows, long D, bool backward) {
-  const int nt = row_threads(D), bt = block_threads(nt);
-  const long per = bt / nt;
-  const long most = (backward ? BWD_WAVES : FWD_WAVES) * 256 * 64 / bt;   // waves a CU
+// The blocks that run at once, in whole ones a CU (few features leave registers for 20 waves, 16 of
+// them in bfloat16 for 12).
+long norm_blocks(long rows, long D, bool backward, bool bf16) {
+  const int nt = row_threads(D, backward && bf16), bt = block_threads(nt);
+  const long per = bt / nt, waves = !backward ? 16 : !bf16 ? 8 : D <= 8 * nt ? 20 : 12;
+  const long most = std::max(1L, waves * 64 / bt) * 256;
   return std::min((rows + per - 1) / per, most);
 }
 
@@ -282,37 +292,47 @@ __global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* ws, i
   }
 }
 
-template <typename T, int NT, int R>
-void launch(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
-  const int nb = (int)norm_blocks(a.rows, a.D, backward);
-  if (backward)
+template <typename T, int NT, int R, bool BACK>
+void launch(const tops_gla_layer_norm_args& a, hipStream_t st) {
+  const int nb = (int)norm_blocks(a.rows, a.D, BACK, sizeof(T) == 2);
+  if constexpr (BACK)
     layer_norm_bwd_kernel<T, NT, R><<<nb, block_threads(NT), 0, st>>>(a);
   else
     layer_norm_fwd_kernel<T, NT, R><<<nb, block_threads(NT), 0, st>>>(a);
 }
-template <typename T, int NT>
-void launch(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
+// The runs of a thread: rows of more than a wave are more than half of what their threads hold.
+template <typename T, int NT, bool BACK>
+void launch(const tops_gla_layer_norm_args& a, hipStream_t st) {
   constexpr int VEC = 16 / (int)sizeof(T), MOST = 16 / VEC;
-  if constexpr (NT == 64) {   // rows of more threads are more than half of what these hold
-    if (a.D <= 64 * VEC) return launch<T, NT, 1>(a, backward, st);
-    if (VEC == 4 && a.D <= 128 * VEC) return launch<T, NT, 2>(a, backward, st);
+  constexpr bool FEW = BACK && sizeof(T) == 2;
+  if constexpr (NT == 64) {
+    if (a.D <= 64 * VEC) return launch<T, NT, 1, BACK>(a, st);
+    if (VEC == 4 && a.D <= 128 * VEC) return launch<T, NT, 2, BACK>(a, st);
+    launch<T, NT, MOST, BACK>(a, st);
+  } else if constexpr (!FEW) {
+    launch<T, NT, MOST, BACK>(a, st);
+  } else {
+    if (NT < 1024 || a.D <= 8 * NT) return launch<T, NT, MOST / 2, BACK>(a, st);
+    if constexpr (NT == 1024) launch<T, NT, MOST, BACK>(a, st);
   }
-  launch<T, NT, MOST>(a, backward, st);
 }
 
-template <typename T>
-hipError_t run(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st) {
+template <typename T, bool BACK>
+hipError_t run(const tops_gla_layer_norm_args& a, hipStream_t st) {
   if (a.rows > 0) {
-    switch (row_threads(a.D)) {
-      case 64: launch<T, 64>(a, backward, st); break;
-      case 128: launch<T, 128>(a, backward, st); break;
-      case 256: launch<T, 256>(a, backward, st); break;
-      case 512: launch<T, 512>(a, backward, st); break;
-      default: launch<T, 1024>(a, backward, st);
+    constexpr bool FEW = BACK && sizeof(T) == 2;
+    switch (row_threads(a.D, FEW)) {
+      case 64: launch<T, 64, BACK>(a, st); break;
+      case 128:
+        if constexpr (!FEW) launch<T, 128, BACK>(a, st);
+        break;
+      case 256: launch<T, 256, BACK>(a, st); break;
+      case 512: launch<T, 512, BACK>(a, st); break;
+      default: launch<T, 1024, BACK>(a, st);
     }
   }
-  if (backward && a.ws) {
-    const int parts = (int)norm_blocks(a.rows, a.D, true);
+  if (BACK && a.ws) {
+    const int parts = (int)norm_blocks(a.rows, a.D, true, sizeof(T) == 2);
     layer_norm_sum_kernel<<<(unsigned)((2 * a.D + 31) / 32), 1024, 0, st>>>(
         (const float*)a.ws, parts, (int)a.D, a.dw, a.db);
   }
@@ -321,13 +341,15 @@ hipError_t run(const tops_gla_layer_norm_args& a, bool backward, hipStream_t st)
 
 }  // namespace
 
-long layer_norm_part_rows(long rows, long D, int) { return norm_blocks(rows, D, true); }
+long layer_norm_part_rows(long rows, long D, int dtype) {
+  return norm_blocks(rows, D, true, dtype == DT_BF16);
+}
 
 hipError_t run_layer_norm_fwd(const tops_gla_layer_norm_args& a, hipStream_t st) {
-  return a.dtype == DT_BF16 ? run<bf16>(a, false, st) : run<float>(a, false, st);
+  return a.dtype == DT_BF16 ? run<bf16, false>(a, st) : run<float, false>(a, st);
 }
 hipError_t run_layer_norm_bwd(const tops_gla_layer_norm_args& a, hipStream_t st) {
-  return a.dtype == DT_BF16 ? run<bf16>(a, true, st) : run<float>(a, true, st);
+  return a.dtype == DT_BF16 ? run<bf16, true>(a, st) : run<float, true>(a, st);
 }
 
 }  // namespace tops
