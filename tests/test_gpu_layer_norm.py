@@ -60,6 +60,12 @@ def test_rows(rows, dt):
     check(*make((rows, 48), dt))
 
 
+@pytest.mark.parametrize("rows,D", [(3000, 1100), (700, 5000), (600, 9000)])
+@pytest.mark.parametrize("dt", [FL, BF])
+def test_more_rows_than_blocks(rows, D, dt):
+    check(*make((rows, D), dt))
+
+
 @pytest.mark.parametrize("shape", [(0, 16), (2, 0, 16), (16,), (2, 3, 4, 16)])
 def test_shapes(shape):
     check(*make(shape, FL))
