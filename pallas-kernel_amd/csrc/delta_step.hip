@@ -8,7 +8,7 @@
 // token: with S' = e^g S, o = scale S_t^T q = scale (S'^T q + (q k) n), so S'^T k, S'^T q, q k and
 // the norms are summed together, before n is known.
 //
-// Measured: 128 rows of 16 heads of 128 x 128, 268 MB, in 54.7 us, 4.9 TB/s, as a large copy has. A
+// Measured: 128 rows of 16 heads of 128 x 128, 268 MB, in 54.2 us, 4.95 TB/s, as a large copy has. A
 // wave is a block of its own (four a block: 58.8 us), neighbouring columns on one XCD (each on the
 // next: 56.3 us, and 64 so 50 us with 100 columns, where lines are shared). A token's inputs asked for
 // with the state or the token before were no faster (60.5 us: 252 registers for 131). One row of 16

@@ -42,10 +42,10 @@ def _segment(counts, blocks):
     heads and columns of each; tops_gla_delta_segment has the rule for equal lengths.
 
     All segments should run at once, or the last ones wait for a whole one (lengths of 28, 5, 33,
-    2, 47, 1, 8 and 9 chunks, 16 heads: L = 10 has 272 blocks and takes 192 us, 11 has 256 and 159,
-    12 164, 17 200, uncut 299). Where the sequences alone are more than the CUs hold, their ends
+    2, 47, 1, 8 and 9 chunks, 16 heads: L = 10 has 272 blocks and takes 186 us, 11 has 256 and 151,
+    12 157, 17 195, uncut 296). Where the sequences alone are more than the CUs hold, their ends
     differ anyway, and what is long among them is cut by the average (40 of 4 chunks and one of
-    200: 393 us, uncut 1242; 64 of 6 and one of 60: 538, uncut 596)."""
+    200: 373 us, uncut 1233; 64 of 6 and one of 60: 523, uncut 583)."""
     longest = max(counts)
     L = max(-(-sum(counts) * blocks // _CUS), 2, math.isqrt(max(0, longest - 1) // 4) + 1)
     if len(counts) * blocks <= _CUS:
