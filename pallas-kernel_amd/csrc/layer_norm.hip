@@ -16,7 +16,7 @@
 // registers, and 12 waves 105, 8 waves 139. In float32 16 features are as many bytes again: 16384 x
 // 2048 in 91 us, sums included, with 8 waves of 16 features, 95 with 20 of 8; 65536 x 768 in 123 with
 // 8 waves, 128 with 12. The forward's 268 MB take 64 us, 4.2 TB/s, with 16 features (with 8: 71). The
-// sums over 1280 blocks' partial rows take 12.
+// sums over 1280 blocks' partial rows take 5 with 8 of a thread's loads on their way, 12 with one.
 #include "delta.hpp"
 
 namespace tops {
@@ -276,8 +276,10 @@ __global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* ws, i
   const int col = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + col;
   float s = 0.f;
-  if (c < 2 * D)
+  if (c < 2 * D) {
+#pragma unroll 8
     for (int r = part; r < parts; r += 32) s += ws[(long)r * 2 * D + c];
+  }
   sm[part][col] = s;
   __syncthreads();
   if (part == 0 && c < 2 * D) {
