@@ -494,22 +494,6 @@ __device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& 
       mma(acc[2 * u + h], part == 1 ? a[h].lo : a[h].hi, part == 0 ? b.lo : b.hi);
 }
 
-// acc[2 u + h] += a[h] b, the same way.
-template <int N>
-__device__ __forceinline__ void mma_pair(f32x4 (&acc)[N], int u, const Split<float> (&a)[2],
-                                         const Frag<float>& b) {
-  mma(acc[2 * u], a[0], b);
-  mma(acc[2 * u + 1], a[1], b);
-}
-template <int N>
-__device__ __forceinline__ void mma_pair(f32x4 (&acc)[N], int u, const Split<bf16> (&a)[2],
-                                         const Frag<bf16>& b) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], a[h].lo, b);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], a[h].hi, b);
-}
-
 __device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }
 __device__ __forceinline__ Frag<bf16> high_of(const Split<bf16>& s) { return s.hi; }
 

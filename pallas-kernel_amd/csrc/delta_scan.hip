@@ -286,7 +286,6 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     pair_values(acc[0], acc[1], x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = j0 + e <= i ? x[e] * (fq * rk[e] * d[e]) : 0.f;
-    // in two parts: of the three operands of o this one is the cheapest to have exact
     const Split<T> f = split_of<T>(x);
     const int row = 32 * tri_block(tile / 2, u) + i % 32;
     st_frag(sP + row * L::PT + 8 * g, high_of(f));
@@ -325,7 +324,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     const float* sf = (const float*)(buf + L::F0);   // e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|,
     const float last = sf[5 * C - 1];                // e^G
     f32x4 acc[2 * NU], o[FIRST ? 1 : 2 * NU];
-    Frag<T> nf[NU];
+    Split<T> nf[NU];
     if (idle && !early) aside();
     if (!idle) {
 #pragma unroll
@@ -343,8 +342,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
           for (int i = 0; i < 2 * NU; ++i)
             mma(o[i],
-                ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g),
-                high_of(f));
+                ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g), f);
         }
       }
       if (!early) aside();
@@ -379,8 +377,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         float x[8];
         pair_values(acc[2 * u], acc[2 * u + 1], x);
         if constexpr (!FIRST) {
-          nf[u] = frag_of<T>(x);
-          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, nf[u]);
+          nf[u] = split_of<T>(x);
+          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, high_of(nf[u]));
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
@@ -403,14 +401,11 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int w = 0; w <= u; ++w) {
-            Split<T> f[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              f[x] = ld_split<T>(sP, L::LO,
+          for (int w = 0; w <= u; ++w)
+            mma_split_pair(o, u, [&](int x) {
+              return ld_split<T>(sP, L::LO,
                                  (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
-            mma_pair(o, u, f, nf[w]);
-          }
+            }, nf[w]);
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
