@@ -115,13 +115,13 @@ inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 // Per chunk and value head ("unit"): vectors over the chunk's tokens, [7][C] float and [C] double,
 //   e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|, e^G, e^{G_C - G}, 1 / |q|
 // (norms 1 without l2norm) and G, the sums of the log decays (in 64 bits: differences of it go into
-// exponentials); then, in the operands' type, two of them (high and low part) where it is bfloat16,
+// exponentials); then, in the operands' type, three parts of it where that is bfloat16,
 //   Tm the inverse of 1 + tril(beta k k^T decay), P the masked and scaled scores, both as the lower
 // of their 32 x 32 blocks (0, 0), (1, 0), (1, 1);
 // and, for the backward, N [V][C] the written values, S [V][KP] the state before the chunk.
 struct DeltaParams {
   tops_gla_delta_args a;   // 8 <= K, 8 <= V
-  int C, KP, parts;   // tokens of a chunk, padded keys, parts of a split tile (2 or 1)
+  int C, KP;   // tokens of a chunk, padded keys
   char *vec, *Tm, *P, *N, *S;   // in keep, the last three with `train`
   char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
                                 // right side
@@ -131,7 +131,7 @@ struct DeltaParams {
   float *E, *dE;
   char *M, *Mt;
   int multi;
-  long vec_bytes, tri_bytes, keep_bytes, ws_bytes;
+  long vec_bytes, tri_bytes, map_bytes, keep_bytes, ws_bytes;
 };
 // The layout for given sizes; pointers from base addresses that may be NULL.
 DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws);
@@ -204,59 +204,70 @@ __device__ __forceinline__ void st_frag(T* p, const Frag<T>& f) {   // 16-byte a
   __builtin_memcpy(__builtin_assume_aligned(p, 16), &f, sizeof(f));
 }
 
-// A float operand with the accuracy of its accumulator: in bfloat16 a high and a low part, whose
-// sum is 2^-18 of the value off at most. States and what they are made of go through products of
-// such operands, so that a state is as exact in bfloat16 calls as float32 allows.
-template <typename T>
-struct Split;
-template <>
-struct Split<float> {
-  Frag<float> f;
-};
-template <>
-struct Split<bf16> {
-  Frag<bf16> hi, lo;
+// A float operand in N parts of its products' type, the largest first. In bfloat16 three parts hold
+// all 24 bits of a float: states and what they are made of go through such products, so that a state
+// is as exact in bfloat16 calls as float32 sums allow. Two parts are 2^-17 of the value off at most
+// (half a step of a remainder that is half a step itself): what goes into a result of bfloat16.
+template <typename T, int N>
+struct Split {
+  Frag<T> p[N];
 };
 template <typename T>
-__device__ __forceinline__ Split<T> split_of(const float (&x)[8]);
-template <>
-__device__ __forceinline__ Split<float> split_of<float>(const float (&x)[8]) {
-  return {frag_of<float>(x)};
-}
-template <>
-__device__ __forceinline__ Split<bf16> split_of<bf16>(const float (&x)[8]) {
-  Split<bf16> s;
-  s.hi = frag_of<bf16>(x);
-  // hides the packed words, whose halves the compiler would otherwise convert once more
-  asm("" : "+v"(s.hi.d.x), "+v"(s.hi.d.y), "+v"(s.hi.d.z), "+v"(s.hi.d.w));
-  float h[8];
-  values_of(s.hi, h);
+constexpr int WHOLE = sizeof(T) == 2 ? 3 : 1;
+template <typename T>
+constexpr int TWO = sizeof(T) == 2 ? 2 : 1;
+template <typename T>
+using Whole = Split<T, WHOLE<T>>;
+template <typename T>
+using Two = Split<T, TWO<T>>;
+
+template <typename T, int N>
+__device__ __forceinline__ Split<T, N> split_of(const float (&x)[8]) {
+  Split<T, N> s;
+  s.p[0] = frag_of<T>(x);
+  if constexpr (N > 1) {
+    float r[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = x[e] - h[e];
-  s.lo = frag_of<bf16>(h);
+    for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      uint4& d = s.p[i - 1].d;
+      // hides the packed words, whose halves the compiler would otherwise convert once more
+      asm("" : "+v"(d.x), "+v"(d.y), "+v"(d.z), "+v"(d.w));
+      float h[8];
+      values_of(s.p[i - 1], h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] -= h[e];
+      s.p[i] = frag_of<T>(r);
+    }
+  }
   return s;
 }
-__device__ __forceinline__ void mma(f32x4& acc, const Frag<float>& a, const Split<float>& b) {
-  mma(acc, a, b.f);
+template <typename T>
+__device__ __forceinline__ Two<T> two_of(const Whole<T>& w) {
+  Two<T> s;
+#pragma unroll
+  for (int i = 0; i < TWO<T>; ++i) s.p[i] = w.p[i];
+  return s;
 }
-__device__ __forceinline__ void mma(f32x4& acc, const Frag<bf16>& a, const Split<bf16>& b) {
-  mma(acc, a, b.lo);
-  mma(acc, a, b.hi);
+// The products of the parts, the smallest first; those of two small parts that are below what the
+// others leave off are left out.
+template <typename T, int N>
+__device__ __forceinline__ void mma(f32x4& acc, const Frag<T>& a, const Split<T, N>& b) {
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i) mma(acc, a, b.p[i]);
 }
-__device__ __forceinline__ void mma(f32x4& acc, const Split<float>& a, const Frag<float>& b) {
-  mma(acc, a.f, b);
+template <typename T, int N>
+__device__ __forceinline__ void mma(f32x4& acc, const Split<T, N>& a, const Frag<T>& b) {
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i) mma(acc, a.p[i], b);
 }
-__device__ __forceinline__ void mma(f32x4& acc, const Split<bf16>& a, const Frag<bf16>& b) {
-  mma(acc, a.lo, b);
-  mma(acc, a.hi, b);
-}
-__device__ __forceinline__ void mma(f32x4& acc, const Split<float>& a, const Split<float>& b) {
-  mma(acc, a.f, b.f);
-}
-__device__ __forceinline__ void mma(f32x4& acc, const Split<bf16>& a, const Split<bf16>& b) {
-  mma(acc, a.hi, b.lo);   // the product of the low parts is below what the sum keeps
-  mma(acc, a.lo, b.hi);
-  mma(acc, a.hi, b.hi);
+template <typename T, int N>
+__device__ __forceinline__ void mma(f32x4& acc, const Split<T, N>& a, const Split<T, N>& b) {
+#pragma unroll
+  for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i <= s; ++i) mma(acc, a.p[i], b.p[s - i]);
 }
 
 // Output tiles come in pairs (h = 0, 1) of 32 rows: row 4 g + r of tile h stands for row
@@ -286,29 +297,20 @@ __device__ __forceinline__ Frag<float> ld_pair_t(const float* M, int P, int lane
   f.b = make_float4(p[4 * P], p[5 * P], p[6 * P], p[7 * P]);
   return f;
 }
-// Split fragments of a tile in LDS whose low part lies `lo` elements behind its high part.
-template <typename T>
-__device__ __forceinline__ Split<T> ld_split(const T* tile, int lo, int off);
-template <>
-__device__ __forceinline__ Split<float> ld_split<float>(const float* tile, int, int off) {
-  return {ld_frag(tile + off)};
+// Split fragments of a tile whose parts lie `step` elements apart.
+template <typename T, int N>
+__device__ __forceinline__ Split<T, N> ld_split(const T* tile, int step, int off) {
+  Split<T, N> s;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s.p[i] = ld_frag(tile + i * step + off);
+  return s;
 }
-template <>
-__device__ __forceinline__ Split<bf16> ld_split<bf16>(const bf16* tile, int lo, int off) {
-  return {ld_frag(tile + off), ld_frag(tile + lo + off)};
-}
-
-template <typename T>
-__device__ __forceinline__ Split<T> ld_split_t(const T* tile, int lo, int P, int lane, int h);
-template <>
-__device__ __forceinline__ Split<float> ld_split_t<float>(const float* tile, int, int P, int lane,
-                                                          int h) {
-  return {ld_pair_t(tile, P, lane, h)};
-}
-template <>
-__device__ __forceinline__ Split<bf16> ld_split_t<bf16>(const bf16* tile, int lo, int P, int lane,
-                                                        int h) {
-  return {ld_pair_t(tile, P, lane, h), ld_pair_t(tile + lo, P, lane, h)};
+template <typename T, int N>
+__device__ __forceinline__ Split<T, N> ld_split_t(const T* tile, int step, int P, int lane, int h) {
+  Split<T, N> s;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s.p[i] = ld_pair_t(tile + i * step, P, lane, h);
+  return s;
 }
 // The 8 values of a lane in a pair of accumulators.
 __device__ __forceinline__ void pair_values(const f32x4& a, const f32x4& b, float (&x)[8]) {
@@ -457,45 +459,32 @@ struct BlockStream {
 
 // acc[i] += A(i) B for N tiles of rows, part after part of a split operand, so that a product does
 // not wait for the one before it.
-template <int N, typename F>
-__device__ __forceinline__ void mma_rows(f32x4 (&acc)[N], const F& rows, const Split<float>& b) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) mma(acc[i], rows(i), b.f);
-}
-template <int N, typename F>
-__device__ __forceinline__ void mma_rows(f32x4 (&acc)[N], const F& rows, const Split<bf16>& b) {
+template <typename T, int N, int P, typename F>
+__device__ __forceinline__ void mma_rows(f32x4 (&acc)[N], const F& rows, const Split<T, P>& b) {
   constexpr int W = N < 4 ? N : 4;
 #pragma unroll
   for (int i = 0; i < N; i += W) {
-    Frag<bf16> a[W];
+    Frag<T> a[W];
 #pragma unroll
     for (int x = 0; x < W; ++x) a[x] = rows(i + x);
 #pragma unroll
-    for (int x = 0; x < W; ++x) mma(acc[i + x], a[x], b.lo);
+    for (int part = P - 1; part >= 0; --part)
 #pragma unroll
-    for (int x = 0; x < W; ++x) mma(acc[i + x], a[x], b.hi);
+      for (int x = 0; x < W; ++x) mma(acc[i + x], a[x], b.p[part]);
   }
 }
-// The same with the rows in two parts too, for the pair of tiles u.
-template <int N, typename F>
+// The same with the rows in as many parts, for the pair of tiles u.
+template <typename T, int N, int P, typename F>
 __device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& rows,
-                                               const Split<float>& b) {
+                                               const Split<T, P>& b) {
+  const Split<T, P> a[2] = {rows(0), rows(1)};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], rows(h), b);
+  for (int s = P - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i <= s; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) mma(acc[2 * u + h], a[h].p[i], b.p[s - i]);
 }
-template <int N, typename F>
-__device__ __forceinline__ void mma_split_pair(f32x4 (&acc)[N], int u, const F& rows,
-                                               const Split<bf16>& b) {
-  const Split<bf16> a[2] = {rows(0), rows(1)};
-#pragma unroll
-  for (int part = 0; part < 3; ++part)   // the product of the low parts is below the sum's step
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      mma(acc[2 * u + h], part == 1 ? a[h].lo : a[h].hi, part == 0 ? b.lo : b.hi);
-}
-
-__device__ __forceinline__ Frag<float> high_of(const Split<float>& s) { return s.f; }
-__device__ __forceinline__ Frag<bf16> high_of(const Split<bf16>& s) { return s.hi; }
 
 // A lane's rows of its column of a state: row k + 32 s + 4 h + r in S[2 s + h][r], k its first. `at`
 // is the column in row 0. Rows past K are the last one's when they are loaded.

@@ -188,9 +188,9 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = t[e];
-      const Split<T> s = split_of<T>(y);
-      st_frag(out + 8 * i, high_of(s));
-      if constexpr (sizeof(T) == 2) st_frag(out + TRI + 8 * i, s.lo);
+      const Whole<T> s = split_of<T, WHOLE<T>>(y);
+#pragma unroll
+      for (int part = 0; part < WHOLE<T>; ++part) st_frag(out + part * TRI + 8 * i, s.p[part]);
     }
     __syncthreads();
   }
@@ -206,7 +206,9 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   p.C = delta_chunk_of((int)z.dtype);
   p.KP = delta_key_pad(z.K);
   p.vec_bytes = 36 * p.C;
-  p.tri_bytes = z.dtype == DT_BF16 ? 3 * 1024 * 4 : 1024 * 4;
+  const long whole = z.dtype == DT_BF16 ? 2 * WHOLE<bf16> : 4;   // bytes of an element in all parts
+  p.tri_bytes = (z.dtype == DT_BF16 ? 3 : 1) * 1024 * whole;
+  p.map_bytes = (long)p.KP * p.KP * whole;
   p.multi = z.nsegs > z.nseq;
   long at = 0;
   auto take = [&](void* base, long bytes) {
@@ -214,7 +216,7 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
     at += up(bytes);
     return x;
   };
-  const long ends = p.multi ? segs * z.K * z.V * 4 : 0, maps = p.multi ? segs * p.KP * p.KP * 4 : 0;
+  const long ends = p.multi ? segs * z.K * z.V * 4 : 0, maps = p.multi ? segs * p.map_bytes : 0;
   p.vec = take(keep, units * p.vec_bytes);
   p.Tm = take(keep, units * p.tri_bytes);
   p.P = take(keep, z.train ? units * p.tri_bytes : 0);

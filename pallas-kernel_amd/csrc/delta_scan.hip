@@ -85,10 +85,10 @@ __device__ __forceinline__ int map_at(int row, int col) {
 // A head's columns go to blocks of NW waves of 16, of V or, in a first pass, then of KP for M.
 template <typename T, int KP, int NW>
 struct ScanShape {
-  static constexpr int C = delta_c<T>(), PARTS = sizeof(T) == 2 ? 2 : 1, COLS = 16 * NW;
+  static constexpr int C = delta_c<T>(), COLS = 16 * NW;
   static constexpr int PK = pitch_of<T>(KP), PT = pitch_of<T>(32), PV = pitch_of<T>(COLS);
-  static constexpr int NT = 64 * NW, TRI = PARTS * delta_blocks<T>() * 32;   // rows of Tm or P
-  static constexpr int LO = delta_blocks<T>() * 32 * PT;   // from a high part to its low part
+  static constexpr int NT = 64 * NW, TRI = delta_blocks<T>() * 32;   // rows of a part of Tm or P
+  static constexpr int PART = TRI * PT;   // from a part to the next one
 };
 constexpr int LDS_MOST = 160 * 1024;
 
@@ -114,11 +114,11 @@ template <typename T, int KP, int NW, bool FIRST>
 struct ScanLds : ScanShape<T, KP, NW> {
   using B = ScanShape<T, KP, NW>;
   static constexpr int C = B::C, ES = (int)sizeof(T);
-  static constexpr int K0 = 0, T0 = C * B::PK, V0 = T0 + B::TRI * B::PT, END = V0 + C * B::PV;
+  static constexpr int K0 = 0, T0 = C * B::PK, V0 = T0 + WHOLE<T> * B::PART, END = V0 + C * B::PV;
   static constexpr int F0 = END * ES;   // five vectors of floats
   static constexpr int ONE = F0 + 5 * C * 4;
-  // the scores' part: q, P, the sums of log decays, 1 / |q|
-  static constexpr int Q0 = 0, P0 = C * B::PK, G0 = (P0 + B::TRI * B::PT) * ES, R0 = G0 + 8 * C;
+  // the scores' part: q, two parts of P, the sums of log decays, 1 / |q|
+  static constexpr int Q0 = 0, P0 = C * B::PK, G0 = (P0 + TWO<T> * B::PART) * ES, R0 = G0 + 8 * C;
   static constexpr int REST = FIRST ? 0 : R0 + 4 * C;
   static constexpr int BUFS = 2 * ONE + REST <= LDS_MOST ? 2 : 1;   // of the chunk's tiles
   static constexpr int BYTES = BUFS * ONE + REST;
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   const uint32_t o_off =
       (uint32_t)(tid / (COLS / 8) * HV * V + vb * COLS + tid % (COLS / 8) * 8) * ES;
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  BlockStream<T, L::TRI, NT> ft;
+  BlockStream<T, WHOLE<T> * L::TRI, NT> ft;
   TileStream<T, C, COLS, NT> fv(a.v_st, vc, tid);
   constexpr int NF = (5 * C + NT - 1) / NT;
   float ff[NF];
@@ -286,14 +286,15 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     pair_values(acc[0], acc[1], x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = j0 + e <= i ? x[e] * (fq * rk[e] * d[e]) : 0.f;
-    const Split<T> f = split_of<T>(x);
+    const Whole<T> f = split_of<T, WHOLE<T>>(x);
     const int row = 32 * tri_block(tile / 2, u) + i % 32;
-    st_frag(sP + row * L::PT + 8 * g, high_of(f));
-    if constexpr (sizeof(T) == 2) st_frag(sP + L::LO + row * L::PT + 8 * g, f.lo);
+#pragma unroll
+    for (int part = 0; part < TWO<T>; ++part)
+      st_frag(sP + part * L::PART + row * L::PT + 8 * g, f.p[part]);
     if (keep_p) {
       T* out = at_off<T>(Pc, (uint32_t)(row * 32 + 8 * g) * ES);
-      st_frag(out, high_of(f));
-      if constexpr (sizeof(T) == 2) st_frag(out + delta_blocks<T>() * 1024, f.lo);
+#pragma unroll
+      for (int part = 0; part < WHOLE<T>; ++part) st_frag(out + part * L::TRI * 32, f.p[part]);
     }
   };
   unsigned char *buf = smem, *other = smem + (L::BUFS - 1) * L::ONE;   // this chunk's, the next one's
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     const float* sf = (const float*)(buf + L::F0);   // e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|,
     const float last = sf[5 * C - 1];                // e^G
     f32x4 acc[2 * NU], o[FIRST ? 1 : 2 * NU];
-    Split<T> nf[NU];
+    Two<T> nf[NU];
     if (idle && !early) aside();
     if (!idle) {
 #pragma unroll
@@ -333,21 +334,20 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
       for (int s = 0; s < NS; ++s) {
         float x[8];
         pair_values(S[2 * s], S[2 * s + 1], x);
-        const Split<T> f = split_of<T>(x);
+        const Whole<T> f = split_of<T, WHOLE<T>>(x);
         mma_rows(acc, [&](int i) {
           return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
         }, f);
         if constexpr (!FIRST) {
-          if (keep && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, high_of(f));
-#pragma unroll
-          for (int i = 0; i < 2 * NU; ++i)
-            mma(o[i],
-                ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g), f);
+          if (keep && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, f.p[0]);
+          mma_rows(o, [&](int i) {
+            return ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
+          }, two_of<T>(f));
         }
       }
       if (!early) aside();
       if (!FIRST && more) fetch2(left - C);
-      Split<T> R[NU];
+      Whole<T> R[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         float x[8], y[8];
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           const int t = 32 * u + 8 * g + e;
           x[e] = sf[2 * C + t] * (y[e] - sf[t] * x[e]);
         }
-        R[u] = split_of<T>(x);
+        R[u] = split_of<T, WHOLE<T>>(x);
       }
 #pragma unroll
       for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
@@ -367,8 +367,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
         for (int u = w; u < NU; ++u)
           mma_split_pair(acc, u, [&](int x) {
-            return ld_split<T>(sT, L::LO,
-                               (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
+            return ld_split<T, WHOLE<T>>(sT, L::PART,
+                                         (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
           }, R[w]);
 #pragma unroll
       for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
@@ -377,14 +377,14 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         float x[8];
         pair_values(acc[2 * u], acc[2 * u + 1], x);
         if constexpr (!FIRST) {
-          nf[u] = split_of<T>(x);
-          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, high_of(nf[u]));
+          nf[u] = split_of<T, TWO<T>>(x);
+          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, nf[u].p[0]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
         mma_rows(S, [&](int i) {
           return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-        }, split_of<T>(x));
+        }, split_of<T, WHOLE<T>>(x));
       }
     }
     if constexpr (!FIRST) {
@@ -403,8 +403,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
           for (int w = 0; w <= u; ++w)
             mma_split_pair(o, u, [&](int x) {
-              return ld_split<T>(sP, L::LO,
-                                 (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
+              return ld_split<T, TWO<T>>(sP, L::PART,
+                                         (32 * tri_block(u, w) + pair_row(lane, x)) * L::PT + 8 * g);
             }, nf[w]);
 #pragma unroll
         for (int u = 0; u < NU; ++u)
@@ -440,24 +440,22 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   }
   if (idle) return;
   if (map) {   // column v, rows in the lane's order
-    const long tile = (long)KP * KP;
-    T* M = (T*)(p.M + ((long)at.seg * HV + hv) * tile * 4);
-    T* Mt = (T*)(p.Mt + ((long)at.seg * HV + hv) * tile * 4);
+    constexpr int TILE = KP * KP;
+    T* M = (T*)(p.M + ((long)at.seg * HV + hv) * p.map_bytes);
+    T* Mt = (T*)(p.Mt + ((long)at.seg * HV + hv) * p.map_bytes);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       float x[8], y[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
-      const Split<T> f = split_of<T>(x);
+      const Whole<T> f = split_of<T, WHOLE<T>>(x);
       const int row = 32 * s + 8 * g;
-      if (a.train) st_frag(Mt + map_at<KP>(v, row), high_of(f));
-      values_of(high_of(f), y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) M[map_at<KP>(row + e, v)] = from_f32<T>(y[e]);
-      if constexpr (sizeof(T) == 2) {
-        if (a.train) st_frag(Mt + tile + map_at<KP>(v, row), f.lo);
-        values_of(f.lo, y);
+      for (int part = 0; part < WHOLE<T>; ++part) {
+        if (a.train) st_frag(Mt + part * TILE + map_at<KP>(v, row), f.p[part]);
+        values_of(f.p[part], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) M[tile + map_at<KP>(row + e, v)] = from_f32<T>(y[e]);
+        for (int e = 0; e < 8; ++e)
+          M[part * TILE + map_at<KP>(row + e, v)] = from_f32<T>(y[e]);
       }
     }
   } else if (FIRST) {
@@ -471,8 +469,8 @@ template <typename T, int KP, int NW>
 struct DscanLds : ScanShape<T, KP, NW> {
   using B = ScanShape<T, KP, NW>;
   static constexpr int C = B::C;
-  static constexpr int K0 = 0, Q0 = C * B::PK, T0 = 2 * C * B::PK, P0 = T0 + B::TRI * B::PT;
-  static constexpr int V0 = P0 + B::TRI * B::PT, END = V0 + C * B::PV;
+  static constexpr int K0 = 0, Q0 = C * B::PK, T0 = 2 * C * B::PK, P0 = T0 + WHOLE<T> * B::PART;
+  static constexpr int V0 = P0 + WHOLE<T> * B::PART, END = V0 + C * B::PV;
   static constexpr int F0 = END * (int)sizeof(T);   // three vectors of floats, e^{G_C}
   static constexpr int BYTES = F0 + (3 * C + 1) * 4;
   static_assert(BYTES <= LDS_MOST, "LDS");
@@ -514,7 +512,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   if (from) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
-  BlockStream<T, L::TRI, NT> ft, fp;
+  BlockStream<T, WHOLE<T> * L::TRI, NT> ft, fp;
   TileStream<T, C, COLS, NT> fd(a.do_st, vc, tid);
   constexpr int ES = (int)sizeof(T);
   const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
@@ -590,8 +588,8 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
     for (int s = 0; s < NS; ++s) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
-      const Split<T> f = split_of<T>(x);
-      if (!FIRST && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, high_of(f));
+      const Whole<T> f = split_of<T, WHOLE<T>>(x);
+      if (!FIRST && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, f.p[0]);
       mma_rows(acc, [&](int i) {
         return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
       }, f);
@@ -610,14 +608,15 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
           mma(acc[2 * w + x],
-              ld_split_t<T>(sP + 32 * tri_block(u, w) * L::PT, L::LO, L::PT, lane, x), df[u]);
+              ld_split_t<T, WHOLE<T>>(sP + 32 * tri_block(u, w) * L::PT, L::PART, L::PT, lane, x),
+              df[u]);
     if (n > 0) fetch2(C);
-    Split<T> R[NU];
+    Whole<T> R[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       float x[8];
       pair_values(acc[2 * u], acc[2 * u + 1], x);
-      R[u] = split_of<T>(x);
+      R[u] = split_of<T, WHOLE<T>>(x);
     }
 #pragma unroll
     for (int i = 0; i < 2 * NU; ++i) acc[i] = zero4();
@@ -626,7 +625,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 #pragma unroll
       for (int w = 0; w <= u; ++w)
         mma_split_pair(acc, w, [&](int x) {
-          return ld_split_t<T>(sT + 32 * tri_block(u, w) * L::PT, L::LO, L::PT, lane, x);
+          return ld_split_t<T, WHOLE<T>>(sT + 32 * tri_block(u, w) * L::PT, L::PART, L::PT, lane, x);
         }, R[u]);
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) S[i] *= last;
@@ -638,7 +637,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       for (int e = 0; e < 8; ++e) x[e] *= sf[2 * C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {
         return ld_pair_t(sQ + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, split_of<T>(x));
+      }, split_of<T, WHOLE<T>>(x));
       pair_values(acc[2 * u], acc[2 * u + 1], x);
       if (!FIRST && vin)
         st_frag(at_off<T>(Yc, n_off) + 32 * u, frag_of<T>(x));
@@ -646,7 +645,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {
         return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
-      }, split_of<T>(x));
+      }, split_of<T, WHOLE<T>>(x));
     }
     Sc -= s_step;
     Yc -= n_step;
@@ -658,14 +657,14 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 }
 
 // E_j <- M_j E_{j-1} + E_j along the segments of a sequence and head, or dE_j <- M_j^T dE_{j+1} +
-// dE_j the other way. A block has 16 columns, each of its waves KP / 4 or KP / 2 of the rows; the
+// dE_j the other way. A block has 16 columns, each of its waves 32 of the rows; the
 // states go from wave to wave through LDS as operands, the maps and parts of the next segment are
 // on their way meanwhile. Bound by the maps' way through the caches, each read by every block of the
-// head: 16 segments of 16 heads of 128 x 128 in 22 us (maps in rows, 64 bytes a row and load: 33; two
-// segments ahead so: 40).
+// head: 16 segments of 16 heads of 128 x 128 in 31 us (with maps in two parts 22, in rows, 64 bytes a
+// row and load, 33; two segments ahead so 40).
 template <typename T, int KP, bool BACK>
-__global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaParams p) {
-  constexpr int NS = KP / 32, NW = KP == 64 ? 2 : 4, NR = NS / NW, PARTS = sizeof(T) == 2 ? 2 : 1;
+__global__ __launch_bounds__(2 * KP) void delta_fold_kernel(DeltaParams p) {
+  constexpr int NS = KP / 32, PARTS = WHOLE<T>;
   __shared__ __attribute__((aligned(16))) Frag<T> sh[2][PARTS][NS][64];
   const tops_gla_delta_args& a = p.a;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
@@ -685,35 +684,31 @@ __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaP
     first = seq * count;
   }
   if (count < 3) return;   // the first segment to run is where it should be
-  const long tile = (long)KP * KP;
-  const int k0 = wave * NR * 32;   // the wave's rows: k0 + 32 s + 8 g + 4 h + r as ever
+  const int k0 = wave * 32;   // the wave's rows: k0 + 8 g + 4 h + r as ever
   auto state = [&](int n) {
     const int j = BACK ? count - 1 - n : n;
     return (BACK ? p.dE : p.E) + ((long)(first + j) * HV + hv) * K * V;
   };
-  Split<T> M[2 * NR][NS];
-  f32x4 E[2 * NR];
+  Whole<T> M[2][NS];
+  f32x4 E[2];
   auto fetch = [&](int n) {
     const int j = BACK ? count - 1 - n : n;
-    const T* m = (const T*)((BACK ? p.Mt : p.M) + ((long)(first + j) * HV + hv) * tile * 4);
+    const T* m = (const T*)((BACK ? p.Mt : p.M) + ((long)(first + j) * HV + hv) * p.map_bytes);
 #pragma unroll
-    for (int i = 0; i < 2 * NR; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int s = 0; s < NS; ++s)
-        M[i][s] = ld_split<T>(m, (int)tile, ((wave * 2 * NR + i) * NS + s) * 512 + 8 * lane);
+        M[i][s] = ld_split<T, PARTS>(m, KP * KP, ((wave * 2 + i) * NS + s) * 512 + 8 * lane);
     load_rows(E, state(n) + min(v, V - 1), k0 + 8 * g, K, V);
   };
   auto share = [&](int n) {   // the wave's rows of the state after step n, and to memory
+    float x[8];
 #pragma unroll
-    for (int s = 0; s < NR; ++s) {
-      float x[8];
+    for (int e = 0; e < 8; ++e)
+      x[e] = v < V && k0 + 8 * g + e < K ? E[e / 4][e % 4] : 0.f;
+    const Whole<T> f = split_of<T, PARTS>(x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = v < V && k0 + 32 * s + 8 * g + e < K ? E[2 * s + e / 4][e % 4] : 0.f;
-      const Split<T> f = split_of<T>(x);
-      sh[n & 1][0][wave * NR + s][lane] = high_of(f);
-      if constexpr (PARTS == 2) sh[n & 1][1][wave * NR + s][lane] = f.lo;
-    }
+    for (int part = 0; part < PARTS; ++part) sh[n & 1][part][wave][lane] = f.p[part];
     if (n > 0 && v < V) store_rows(E, state(n) + v, k0 + 8 * g, K, V);
   };
   load_rows(E, state(0) + min(v, V - 1), k0 + 8 * g, K, V);
@@ -721,21 +716,19 @@ __global__ __launch_bounds__(KP == 64 ? 128 : 256) void delta_fold_kernel(DeltaP
   fetch(1);
   for (int n = 1; n + 1 < count; ++n) {
     __syncthreads();
-    f32x4 acc[2 * NR];
+    f32x4 acc[2];
 #pragma unroll
-    for (int i = 0; i < 2 * NR; ++i) acc[i] = E[i];
+    for (int i = 0; i < 2; ++i) acc[i] = E[i];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      Split<T> f;
-      if constexpr (PARTS == 2)
-        f = {sh[(n - 1) & 1][0][s][lane], sh[(n - 1) & 1][1][s][lane]};
-      else
-        f = {sh[(n - 1) & 1][0][s][lane]};
+      Whole<T> f;
 #pragma unroll
-      for (int i = 0; i < 2 * NR; ++i) mma(acc[i], M[i][s], f);
+      for (int part = 0; part < PARTS; ++part) f.p[part] = sh[(n - 1) & 1][part][s][lane];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma(acc[i], M[i][s], f);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * NR; ++i) E[i] = acc[i];
+    for (int i = 0; i < 2; ++i) E[i] = acc[i];
     share(n);
     if (n + 2 < count) fetch(n + 1);
   }
@@ -767,7 +760,7 @@ hipError_t passes(const DeltaParams& p, hipStream_t st) {
   if (p.multi) {
     if (const hipError_t e = launch<T, KP, NW, BACK, true>(p, st)) return e;
     const unsigned grid = (unsigned)((p.a.V + 15) / 16 * p.a.HV * p.a.nseq);
-    delta_fold_kernel<T, KP, BACK><<<grid, KP == 64 ? 128 : 256, 0, st>>>(p);
+    delta_fold_kernel<T, KP, BACK><<<grid, 2 * KP, 0, st>>>(p);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   return launch<T, KP, NW, BACK, false>(p, st);

@@ -77,3 +77,18 @@ def test_outputs_are_rounded_once(B, T, H, HV, K, V, cu):
     _, (o, _) = run(x, cu)
     _, (want, _) = oracle(x, cu)
     rounded_once("o", o, want, K, T)
+
+
+@pytest.mark.parametrize("B,T,H,HV,K,V,cu", CASES)
+def test_states_are_float32(B, T, H, HV, K, V, cu):
+    """Final states: two sums, the values and the state, of such sums; gradients of initial ones: of
+    both passes."""
+    x, do, dh = make(B, T, H, HV, K, V, cu, FL)
+    d, (o, ht) = run(x, cu)
+    c, (ro, rht) = oracle(x, cu)
+    e = off(ht, rht)
+    assert e <= 2 ** 0.5 * sums(K, T), f"ht: {e:.3g} off, {2 ** 0.5 * sums(K, T):.3g} allowed"
+    got, = torch.autograd.grad([o, ht], [d["initial_state"]], [do.to(DEV), dh.to(DEV)])
+    want, = torch.autograd.grad([ro, rht], [c["initial_state"]], [do.to(F64), dh.to(F64)])
+    e = off(got, want)
+    assert e <= 2 * sums(K, T), f"dh0: {e:.3g} off, {2 * sums(K, T):.3g} allowed"
