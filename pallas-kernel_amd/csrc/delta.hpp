@@ -118,13 +118,14 @@ inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 // exponentials); then, in the operands' type, three parts of it where that is bfloat16,
 //   Tm the inverse of 1 + tril(beta k k^T decay), P the masked and scaled scores, both as the lower
 // of their 32 x 32 blocks (0, 0), (1, 0), (1, 1);
-// and, for the backward, N [V][C] the written values, S [V][KP] the state before the chunk.
+// and, for the backward, in two such parts side by side in a row, N [V][2][C] the written values and
+// S [V][2][KP] the state before the chunk.
 struct DeltaParams {
   tops_gla_delta_args a;   // 8 <= K, 8 <= V
   int C, KP;   // tokens of a chunk, padded keys
   char *vec, *Tm, *P, *N, *S;   // in keep, the last three with `train`
-  char *dS, *Y;                 // in ws: the gradient of the state after the chunk, of the system's
-                                // right side
+  char *dS, *Y;                 // in ws, as S and N: the gradient of the state after the chunk, of the
+                                // system's right side
   // where a sequence has several segments, for each of all segments and value heads: the state
   // after it [K][V] (E) or the gradient of the state before it (dE), float32, and what it makes of
   // a state before it, [KP][KP] (M, and Mt its transpose), in the order of the fold's operands, parts as Tm's
@@ -242,6 +243,17 @@ __device__ __forceinline__ Split<T, N> split_of(const float (&x)[8]) {
     }
   }
   return s;
+}
+template <typename T, int N>
+__device__ __forceinline__ void sum_of(const Split<T, N>& s, float (&x)[8]) {
+  values_of(s.p[N - 1], x);
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) {
+    float h[8];
+    values_of(s.p[i], h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += h[e];
+  }
 }
 template <typename T>
 __device__ __forceinline__ Two<T> two_of(const Whole<T>& w) {

@@ -14,8 +14,12 @@
 //   dG_i = q . dq + beta k . z - k . dkw,  dG_C += sum k . e^{G_C - G} (N dS^T) + e^{G_C} <S, dS>,
 // and dg the sums of dG from a token to its chunk's end. The terms of pairs on one side of a token
 // cancel in that sum, which is why both sides of a pair multiply the same rounded operand: one that
-// has all its factors, for the raw q and k. (Rounded before the factors of one side, the operands
-// of the other differ by a bfloat16 step, and dg was 9e-3 off at 40 tokens of one head.)
+// has all its factors, for the raw q and k.
+//
+// What the products take from the passes (N, Y, S, dS) and the scores' gradients are two bfloat16 parts
+// where the operands' type is that: a gradient of bfloat16 is then rounded once, its own rounding, and
+// one of float32 (dg, dbeta) about 1e-5 off. (In one part gradients were 3e-3 off, where their own
+// rounding is 1.7e-3, and a training step took 513 us instead of 592.)
 #include "delta.hpp"
 
 namespace tops {
@@ -24,17 +28,23 @@ namespace {
 
 template <typename T, int KP>
 struct GradLds {
-  // values of a slab: as many as registers have room for (K = 64, V = 128, two value heads a key
-  // head: 45 us for 52 with 32; K = 128: 64 spill, 310 us of gradients for 286)
+  // values of a slab: K = 64, V = 128, two value heads a key head, 5000 tokens: forward and backward in
+  // 225 us, 232 with 32; K = 128 has no room in LDS for 64
   static constexpr int C = delta_c<T>(), VS = sizeof(T) == 2 && KP == 64 ? 64 : 32;
-  static constexpr int PK = pitch_of<T>(KP), PC = pitch_of<T>(C), PS = pitch_of<T>(VS);
+  static constexpr int PK = pitch_of<T>(KP), PS = pitch_of<T>(VS);
+  static constexpr int PC = pitch_of<T>(TWO<T> * C), PD = pitch_of<T>(TWO<T> * KP);   // parts in a row
   static constexpr int K0 = 0, Q0 = C * PK, N0 = 2 * C * PK, Y0 = N0 + VS * PC, S0 = Y0 + VS * PC;
-  static constexpr int D0 = S0 + VS * PK, O0 = D0 + VS * PK, END = O0 + C * PS;
+  static constexpr int D0 = S0 + VS * PD, O0 = D0 + VS * PD, END = O0 + C * PS;
   // beta z on its way to the waves of the keys, where the slabs were
   static constexpr int PX = KP + 4, X0 = N0 * (int)sizeof(T);
   static constexpr int G0 = (std::max(END * (int)sizeof(T), X0 + C * PX * 4) + 15) / 16 * 16;
   static constexpr int F0 = G0 + 8 * C;                // after G [C] in 64 bits: [9][C] floats
   static constexpr int BYTES = F0 + (9 * C + 8) * 4;
+  // behind them the sums over value heads of dq and dk, each lane's own, where they fit: of 128 keys
+  // and two value heads a key head forward and backward take 1040 us, 1126 with the sums in registers,
+  // which then spill; 64 keys 218 for 224. With 256 keys there is no room
+  static constexpr int SUMS = 2 * C * PX * 4;
+  static constexpr bool PARK = BYTES + SUMS <= 160 * 1024;
 };
 
 __device__ __forceinline__ float group_sum(float x) {   // over the four lanes of a column
@@ -63,11 +73,10 @@ __device__ __forceinline__ float row_dot(const T* row, const f32x4 (&acc)[2 * NS
 // goes through the value heads of its key head (GROUP: more than one), so that their sums need no
 // second launch.
 //
-// Bound by latency: one block a CU (232 registers), whose loads and products take turns (54 % of a
-// wave's time is waiting): 2 x 4096 tokens, 16 heads of 128 x 128, 436 MB in 155 us, 2.8 TB/s, where
-// the bytes alone take 88. Waves with both roles, four a block: 230 us; two blocks a CU spill, and
-// so do blocks that go on to a next chunk with its loads on their way (205 us; with 64 keys 131 for
-// 136 of the whole backward pass).
+// Bound by latency: one block a CU (249 registers), whose loads and products take turns: 2 x 4096
+// tokens, 16 heads of 128 x 128, 637 MB in 200 us, 3.2 TB/s, where the bytes alone take 129. Two blocks a
+// CU spill. 20 registers spill with 128 keys and several value heads, 65 with 256 keys, 114 with both;
+// float32: 97 with both.
 template <typename T, int KP, bool GROUP>
 __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParams p) {
   using L = GradLds<T, KP>;
@@ -90,18 +99,26 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
   float* sf = (float*)(smem + L::F0);   // the unit's vectors; dG, k . beta z, <S, dS>
   float *sdG = sf + 7 * C, *sKz = sf + 8 * C, *sSum = sf + 9 * C;
   const int group = HV / H;
-  // a slab of a value head, on its way while the one before is multiplied; all of a block's first
-  // loads start together
-  TileFetch<T, VS, C, NT> fn, fy;
-  TileFetch<T, VS, KP, NT> fs, fd;
+  // a slab of a value head, on its way while the one before is multiplied (AHEAD); all of a block's
+  // first loads start together
+  constexpr int NP = TWO<T>;
+  // 256 keys leave no registers for a slab on its way: 1394 us of a training step with 291 spilled ones,
+  // 1129 with 65
+  constexpr bool AHEAD = KP < 256 || sizeof(T) == 4;
+  TileFetch<T, VS, NP * C, NT> fn, fy;
+  TileFetch<T, VS, KP, NT> fs[NP], fd[NP];   // a part each, so that a thread has all of an element
   TileFetch<T, C, VS, NT> fo;
   Run<T, 8> fv[NH];
   auto fetch = [&](int hv, int v0) {
     const long unit = (long)chunk * HV + hv;
-    fn.get((const T*)p.N + (unit * V + v0) * C, C, V - v0, C, tid);
-    fy.get((const T*)p.Y + (unit * V + v0) * C, C, V - v0, C, tid);
-    fs.get((const T*)p.S + (unit * V + v0) * KP, KP, V - v0, KP, tid);
-    fd.get((const T*)p.dS + (unit * V + v0) * KP, KP, V - v0, KP, tid);
+    const long row = (unit * V + v0) * NP;
+    fn.get((const T*)p.N + row * C, NP * C, V - v0, NP * C, tid);
+    fy.get((const T*)p.Y + row * C, NP * C, V - v0, NP * C, tid);
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+      fs[x].get((const T*)p.S + row * KP + x * KP, NP * KP, V - v0, KP, tid);
+      fd[x].get((const T*)p.dS + row * KP + x * KP, NP * KP, V - v0, KP, tid);
+    }
     fo.get((const T*)a.dout + at.b * a.do_sb + at.t * a.do_st + hv * a.do_sh + v0, a.do_st, at.len,
            V - v0, tid);
     if (!key)
@@ -115,16 +132,19 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     TileFetch<T, C, KP, NT> fk, fq;
     fk.get((const T*)a.k + at.b * a.k_sb + at.t * a.k_st + h * a.k_sh, a.k_st, at.len, K, tid);
     fq.get((const T*)a.q + at.b * a.q_sb + at.t * a.q_st + h * a.q_sh, a.q_st, at.len, K, tid);
-    fetch(h * group, 0);
+    if (AHEAD) fetch(h * group, 0);
     fk.put(sK, L::PK, at.len, K, tid);
     fq.put(sQ, L::PK, at.len, K, tid);
   }
   const T *kr = sK + i * L::PK, *qr = sQ + i * L::PK;
   const float scale = (float)a.scale;
-  f32x4 sum[GROUP ? 2 * NS : 1];   // over the value heads: dq, or dk
-  float dots = 0.f;                // and its product with q, or k
+  // over the value heads: dq, or dk, in registers where LDS has no room for them
+  constexpr bool HELD = GROUP && !L::PARK;
+  f32x4 sum[HELD ? 2 * NS : 1];
+  float* parked = (float*)(smem + L::BYTES) + ((key ? C : 0) + i) * L::PX + 8 * g;
+  float dots = 0.f;   // and its product with q, or k
 #pragma unroll
-  for (int x = 0; x < (GROUP ? 2 * NS : 1); ++x) sum[x] = zero4();
+  for (int x = 0; x < (HELD ? 2 * NS : 1); ++x) sum[x] = zero4();
 
   for (int gi = 0; gi < group; ++gi) {
     const int hv = h * group + gi;
@@ -146,17 +166,27 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     for (int x = 0; x < 2 * NU; ++x) B[0][x] = B[1][x] = zero4();
     float vy = 0.f, sd = 0.f, beta = 0.f;
     for (int v0 = 0; v0 < V; v0 += VS) {
+      if (!AHEAD) fetch(hv, v0);
       __syncthreads();
-      fn.put(sN, L::PC, V - v0, C, tid);
-      fy.put(sY, L::PC, V - v0, C, tid);
-      fs.put(sS, L::PK, V - v0, KP, tid);
-      fd.put(sD, L::PK, V - v0, KP, tid);
+      fn.put(sN, L::PC, V - v0, NP * C, tid);
+      fy.put(sY, L::PC, V - v0, NP * C, tid);
+#pragma unroll
+      for (int x = 0; x < NP; ++x) {
+        fs[x].put(sS + x * KP, L::PD, V - v0, KP, tid);
+        fd[x].put(sD + x * KP, L::PD, V - v0, KP, tid);
+      }
       fo.put(sO, L::PS, at.len, V - v0, tid);
 #pragma unroll
-      for (int x = 0; x < decltype(fs)::N; ++x) {
+      for (int x = 0; x < TileFetch<T, VS, KP, NT>::N; ++x) {
+        Split<T, NP> s, d;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          s.p[i] = fs[i].piece(x, V - v0, KP, tid);
+          d.p[i] = fd[i].piece(x, V - v0, KP, tid);
+        }
         float ss[8], dd[8];
-        values_of(fs.piece(x, V - v0, KP, tid), ss);
-        values_of(fd.piece(x, V - v0, KP, tid), dd);
+        sum_of(s, ss);
+        sum_of(d, dd);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sd = fmaf(ss[e], dd[e], sd);
       }
@@ -164,9 +194,9 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
       for (int u = 0; u < NH; ++u) vr[u] = fv[u];
       __syncthreads();
-      if (v0 + VS < V)
+      if (AHEAD && v0 + VS < V)
         fetch(hv, v0 + VS);
-      else if (GROUP && gi + 1 < group)
+      else if (AHEAD && GROUP && gi + 1 < group)
         fetch(hv + 1, 0);
       beta = sf[2 * C + i];
 #pragma unroll 1
@@ -175,10 +205,12 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
         if (u > 0 && v0 + 32 * u >= V) break;
         if (!key) {
           const Frag<T> of = ld_frag(uO + i * L::PS + 8 * g);
-          const Frag<T> yf = ld_frag_t(uY + 16 * tw, L::PC, lane);
+          Two<T> yf;
+#pragma unroll
+          for (int x = 0; x < NP; ++x) yf.p[x] = ld_frag_t(uY + 16 * tw + x * C, L::PC, lane);
           const int c = v0 + 32 * u + 8 * g;
           float y[8], x[8];   // dv, and v . Y (Y is 0 past the end)
-          values_of(yf, y);
+          sum_of(yf, y);
           values_of(frag_of<T>(cut_run(u ? vr[NH - 1] : vr[0], c, V)), x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -189,29 +221,32 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 #pragma unroll
           for (int n = 0; n < 2 * NU; ++n)
             if ((n >> 1) <= uw) {
-              const Frag<T> f = ld_pair_t(uN + 32 * (n >> 1), L::PC, lane, n & 1);
+              const Two<T> f = ld_split_t<T, NP>(uN + 32 * (n >> 1), C, L::PC, lane, n & 1);
               mma(B[0][n], f, of);
               mma(B[1][n], f, yf);
             }
 #pragma unroll
           for (int n = 0; n < 2 * NS; ++n) {
-            const Frag<T> f =
-                ld_pair_t(sS + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1);
+            const Two<T> f =
+                ld_split_t<T, NP>(sS + 32 * u * L::PD + 32 * (n >> 1), KP, L::PD, lane, n & 1);
             mma(A[0][n], f, of);
             mma(A[1][n], f, yf);
           }
         } else {
-          const Frag<T> nf = ld_frag_t(uN + 16 * tw, L::PC, lane);
+          Two<T> nf;
+#pragma unroll
+          for (int x = 0; x < NP; ++x) nf.p[x] = ld_frag_t(uN + 16 * tw + x * C, L::PC, lane);
 #pragma unroll
           for (int n = 0; n < 2 * NU; ++n)
             if ((n >> 1) >= uw) {
               const int r = 32 * (n >> 1) + pair_row(lane, n & 1);
               mma(B[0][n], ld_frag(uO + r * L::PS + 8 * g), nf);
-              mma(B[1][n], ld_pair_t(uY + 32 * (n >> 1), L::PC, lane, n & 1), nf);
+              mma(B[1][n], ld_split_t<T, NP>(uY + 32 * (n >> 1), C, L::PC, lane, n & 1), nf);
             }
 #pragma unroll
           for (int n = 0; n < 2 * NS; ++n)
-            mma(A[0][n], ld_pair_t(sD + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1), nf);
+            mma(A[0][n],
+                ld_split_t<T, NP>(sD + 32 * u * L::PD + 32 * (n >> 1), KP, L::PD, lane, n & 1), nf);
         }
       }
     }
@@ -243,7 +278,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
             x[e] = j + e <= i ? x[e] * (d[e] * (aq * rj[e])) : 0.f;
             y[e] = j + e < i ? y[e] * (d[e] * (ak * rj[e])) : 0.f;
           }
-          const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
+          const Two<T> fx = split_of<T, NP>(x), fyy = split_of<T, NP>(y);
 #pragma unroll
           for (int n = 0; n < 2 * NS; ++n) {
             const Frag<T> f = ld_pair_t(sK + 32 * u * L::PK + 32 * (n >> 1), L::PK, lane, n & 1);
@@ -281,7 +316,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
             x[e] = j + e >= i ? x[e] * (d[e] * (scale * rq[e] * rk)) : 0.f;
             y[e] = j + e > i ? -(y[e] * (d[e] * (bj[e] * rj[e] * rk))) : 0.f;
           }
-          const Frag<T> fx = frag_of<T>(x), fyy = frag_of<T>(y);
+          const Two<T> fx = split_of<T, NP>(x), fyy = split_of<T, NP>(y);
 #pragma unroll
           for (int n = 0; n < 2 * NS; ++n) {
             const int off = 32 * u * L::PK + 32 * (n >> 1);
@@ -337,7 +372,12 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
     }
     if (GROUP) {
 #pragma unroll
-      for (int x = 0; x < 2 * NS; ++x) sum[GROUP ? x : 0] += A[0][x];
+      for (int x = 0; x < 2 * NS; ++x) {
+        f32x4& to = HELD ? sum[HELD ? x : 0]
+                         : *reinterpret_cast<f32x4*>(parked + 32 * (x >> 1) + 4 * (x & 1));
+        if (HELD || gi > 0) A[0][x] += to;
+        to = A[0][x];
+      }
       if (gi + 1 < group) continue;
     }
     if (in) {
@@ -352,9 +392,7 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
         values_of(ld_frag(row + c), x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float d =
-              GROUP ? sum[GROUP ? 2 * s + e / 4 : 0][e % 4] : A[0][2 * s + e / 4][e % 4];
-          y[e] = d - norm * x[e];
+          y[e] = A[0][2 * s + e / 4][e % 4] - norm * x[e];
         }
         put_run<T, 8>(to + c, y, K - c);
       }
@@ -364,7 +402,9 @@ __global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParam
 
 template <typename T, int KP, bool GROUP>
 hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
-  constexpr int lds = GradLds<T, KP>::BYTES;
+  using L = GradLds<T, KP>;
+  constexpr int lds = L::BYTES + (GROUP && L::PARK ? L::SUMS : 0);
+  static_assert(lds <= 160 * 1024, "LDS");
   const hipError_t e = hipFuncSetAttribute((const void*)delta_grad_kernel<T, KP, GROUP>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;

@@ -202,11 +202,12 @@ long up(long n) { return (n + 255) / 256 * 256; }
 
 DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   DeltaParams p{};
-  const long es = z.dtype == DT_BF16 ? 2 : 4, units = z.chunks * z.HV, segs = z.nsegs * z.HV;
+  const long units = z.chunks * z.HV, segs = z.nsegs * z.HV;
   p.C = delta_chunk_of((int)z.dtype);
   p.KP = delta_key_pad(z.K);
   p.vec_bytes = 36 * p.C;
-  const long whole = z.dtype == DT_BF16 ? 2 * WHOLE<bf16> : 4;   // bytes of an element in all parts
+  // bytes of an element in three parts and in two
+  const long whole = z.dtype == DT_BF16 ? 2 * WHOLE<bf16> : 4, two = 4;
   p.tri_bytes = (z.dtype == DT_BF16 ? 3 : 1) * 1024 * whole;
   p.map_bytes = (long)p.KP * p.KP * whole;
   p.multi = z.nsegs > z.nseq;
@@ -220,15 +221,15 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   p.vec = take(keep, units * p.vec_bytes);
   p.Tm = take(keep, units * p.tri_bytes);
   p.P = take(keep, z.train ? units * p.tri_bytes : 0);
-  p.N = take(keep, z.train ? units * z.V * p.C * es : 0);
-  p.S = take(keep, z.train ? units * z.V * p.KP * es : 0);
+  p.N = take(keep, z.train ? units * z.V * p.C * two : 0);
+  p.S = take(keep, z.train ? units * z.V * p.KP * two : 0);
   p.E = (float*)take(keep, ends);
   p.M = take(keep, maps);
   p.Mt = take(keep, z.train ? maps : 0);
   p.keep_bytes = at;
   at = 0;
-  p.dS = take(ws, units * z.V * p.KP * es);
-  p.Y = take(ws, units * z.V * p.C * es);
+  p.dS = take(ws, units * z.V * p.KP * two);
+  p.Y = take(ws, units * z.V * p.C * two);
   p.dE = (float*)take(ws, ends);
   p.ws_bytes = at;
   return p;

@@ -167,7 +167,8 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   if (from && !map) load_state(S, from + min(v, V - 1), vin, g, K, V);
 
   // byte offsets of a lane's stores from bases that are the same for all
-  const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
+  const uint32_t s_off = (uint32_t)(v * TWO<T> * KP + 8 * g) * ES;
+  const uint32_t n_off = (uint32_t)(v * TWO<T> * C + 8 * g) * ES;
   const uint32_t o_off =
       (uint32_t)(tid / (COLS / 8) * HV * V + vb * COLS + tid % (COLS / 8) * 8) * ES;
   TileStream<T, C, KP, NT> fk(a.k_st, K, tid), fq(a.q_st, K, tid);
@@ -182,10 +183,10 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   const char* Tn = p.Tm + unit0 * p.tri_bytes;
   const char* vecn = p.vec + unit0 * p.vec_bytes;
   char *vecc = p.vec + unit0 * p.vec_bytes, *Pc = p.P + unit0 * p.tri_bytes;
-  char *Sc = p.S + unit0 * V * KP * ES, *Nc = p.N + unit0 * V * C * ES;
+  char *Sc = p.S + unit0 * V * KP * TWO<T> * ES, *Nc = p.N + unit0 * V * C * TWO<T> * ES;
   char* oc = (char*)a.o + (((long)at.b * a.T + at.t) * HV + hv) * V * ES;
   const long t_step = (long)HV * p.tri_bytes, vec_step = (long)HV * p.vec_bytes;
-  const long s_step = (long)HV * V * KP * ES, n_step = (long)HV * V * C * ES;
+  const long s_step = (long)HV * V * KP * TWO<T> * ES, n_step = (long)HV * V * C * TWO<T> * ES;
   const int o_row = HV * V * ES;   // and a row of o
   const float scale = (float)a.scale;
   const bool l2norm = a.l2norm != 0, keep = a.train != 0, keep_p = keep && vb == 0;
@@ -339,7 +340,10 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
         }, f);
         if constexpr (!FIRST) {
-          if (keep && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, f.p[0]);
+          if (keep && vin)
+#pragma unroll
+            for (int part = 0; part < TWO<T>; ++part)
+              st_frag(at_off<T>(Sc, s_off) + part * KP + 32 * s, f.p[part]);
           mma_rows(o, [&](int i) {
             return ld_frag(sQ + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
           }, two_of<T>(f));
@@ -378,7 +382,10 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
         pair_values(acc[2 * u], acc[2 * u + 1], x);
         if constexpr (!FIRST) {
           nf[u] = split_of<T, TWO<T>>(x);
-          if (keep && vin) st_frag(at_off<T>(Nc, n_off) + 32 * u, nf[u].p[0]);
+          if (keep && vin)
+#pragma unroll
+            for (int part = 0; part < TWO<T>; ++part)
+              st_frag(at_off<T>(Nc, n_off) + part * C + 32 * u, nf[u].p[part]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= sf[C + 32 * u + 8 * g + e];
@@ -515,7 +522,8 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   BlockStream<T, WHOLE<T> * L::TRI, NT> ft, fp;
   TileStream<T, C, COLS, NT> fd(a.do_st, vc, tid);
   constexpr int ES = (int)sizeof(T);
-  const uint32_t s_off = (uint32_t)(v * KP + 8 * g) * ES, n_off = (uint32_t)(v * C + 8 * g) * ES;
+  const uint32_t s_off = (uint32_t)(v * TWO<T> * KP + 8 * g) * ES;
+  const uint32_t n_off = (uint32_t)(v * TWO<T> * C + 8 * g) * ES;
   // where the chunk before has its inputs, and this chunk its outputs; all go back by their steps
   const long unit0 = (long)(at.chunk + nc - 1) * HV + hv;
   const int k_st = (int)a.k_st, q_st = (int)a.q_st, d_st = (int)a.do_st;
@@ -524,9 +532,9 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
   dp += (long)(nc - 1) * C * d_st;
   const char *Tn = p.Tm + unit0 * p.tri_bytes, *Pn = p.P + unit0 * p.tri_bytes;
   const char* vecn = p.vec + unit0 * p.vec_bytes;
-  char *Sc = p.dS + unit0 * V * KP * ES, *Yc = p.Y + unit0 * V * C * ES;
+  char *Sc = p.dS + unit0 * V * KP * TWO<T> * ES, *Yc = p.Y + unit0 * V * C * TWO<T> * ES;
   const long t_step = (long)HV * p.tri_bytes, vec_step = (long)HV * p.vec_bytes;
-  const long s_step = (long)HV * V * KP * ES, n_step = (long)HV * V * C * ES;
+  const long s_step = (long)HV * V * KP * TWO<T> * ES, n_step = (long)HV * V * C * TWO<T> * ES;
   const float scale = (float)a.scale;
   constexpr int NF = (3 * C + NT) / NT;
   float ff[NF], fr[NF];
@@ -589,7 +597,10 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
       float x[8];
       pair_values(S[2 * s], S[2 * s + 1], x);
       const Whole<T> f = split_of<T, WHOLE<T>>(x);
-      if (!FIRST && vin) st_frag(at_off<T>(Sc, s_off) + 32 * s, f.p[0]);
+      if (!FIRST && vin)
+#pragma unroll
+        for (int part = 0; part < TWO<T>; ++part)
+          st_frag(at_off<T>(Sc, s_off) + part * KP + 32 * s, f.p[part]);
       mma_rows(acc, [&](int i) {
         return ld_frag(sK + (32 * (i >> 1) + pair_row(lane, i & 1)) * L::PK + 32 * s + 8 * g);
       }, f);
@@ -639,8 +650,12 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
         return ld_pair_t(sQ + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
       }, split_of<T, WHOLE<T>>(x));
       pair_values(acc[2 * u], acc[2 * u + 1], x);
-      if (!FIRST && vin)
-        st_frag(at_off<T>(Yc, n_off) + 32 * u, frag_of<T>(x));
+      if (!FIRST && vin) {
+        const Two<T> y = split_of<T, TWO<T>>(x);
+#pragma unroll
+        for (int part = 0; part < TWO<T>; ++part)
+          st_frag(at_off<T>(Yc, n_off) + part * C + 32 * u, y.p[part]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= -sf[C + 32 * u + 8 * g + e];
       mma_rows(S, [&](int i) {

@@ -199,10 +199,11 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
     Inputs may be views with any strides whose last dimension is contiguous (others are copied).
     bfloat16 q, k and v are read and written as they are, and multiplied in bfloat16 with float32
     sums. States are float32, and multiplied as three bfloat16 parts of 24 bits: final states and
-    gradients of initial ones are as exact as float32 sums. Other types of q, k and v are
-    computed in float32. g and beta are read in float32 or bfloat16, whatever the others' type, and
-    their gradients returned in it: with bfloat16 q, k and v these have the accuracy of bfloat16
-    products. Inputs that are not finite make the outputs of their chunk of 64 tokens (float32: 32)
+    gradients of initial ones are as exact as float32 sums. What o and the other gradients are made
+    of is multiplied in two parts of 16 bits: they are rounded once, to their type. Other types of
+    q, k and v are computed in float32. g and beta are read in float32 or bfloat16, whatever the
+    others' type, and their gradients returned in it: float32 ones beside bfloat16 q, k and v are
+    about 1e-5 off. Inputs that are not finite make the outputs of their chunk of 64 tokens (float32: 32)
     and of all later ones of the sequence and head not finite, also those before them in the chunk.
     A second derivative raises.
 

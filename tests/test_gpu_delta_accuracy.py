@@ -92,3 +92,19 @@ def test_states_are_float32(B, T, H, HV, K, V, cu):
     want, = torch.autograd.grad([ro, rht], [c["initial_state"]], [do.to(F64), dh.to(F64)])
     e = off(got, want)
     assert e <= 2 * sums(K, T), f"dh0: {e:.3g} off, {2 * sums(K, T):.3g} allowed"
+
+
+@pytest.mark.parametrize("gdt", [FL, BF])
+@pytest.mark.parametrize("B,T,H,HV,K,V,cu", CASES)
+def test_gradients_are_rounded_once(B, T, H, HV, K, V, cu, gdt):
+    x, do, dh = make(B, T, H, HV, K, V, cu, gdt)
+    d, outs = run(x, cu)
+    c, refs = oracle(x, cu)
+    got = torch.autograd.grad(outs, [d[n] for n in NAMES[:5]], [do.to(DEV), dh.to(DEV)])
+    want = torch.autograd.grad(refs, [c[n] for n in NAMES[:5]], [do.to(F64), dh.to(F64)])
+    for n, t, w in zip(NAMES, got, want):
+        if t.dtype is BF:
+            rounded_once(n, t, w, K, T)
+        else:   # not rounded at all
+            e = off(t, w)
+            assert e <= inside(n, K, T), f"d{n}: {e:.3g} off, {inside(n, K, T):.3g} allowed"
