@@ -33,7 +33,7 @@ extern "C" {
  * `keep` (tops_gla_delta_bytes, 256-byte aligned) is the forward's workspace; with `train` it also
  * holds what the backward reads.
  * 8 <= K <= 256, 8 <= V <= 65536, batch * T < 2^31 - 64, tokens of q, k, v, dout and o at least 0
- * and less than 2^24 elements apart.
+ * and less than 2^24 elements apart (with T <= 1 the inputs' are not looked at).
  */
 typedef struct tops_gla_delta_args {
   const void *q, *k;              /* [B, T, H, K] */

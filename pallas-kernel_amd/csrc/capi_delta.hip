@@ -88,8 +88,10 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
       !grid_fits((a->V / 64 + 5) * a->HV * a->nsegs, 256) ||
       !grid_fits((a->V / 16 + 1) * a->HV * a->nseq, 64))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
-  // offsets within a chunk are 32 bits of bytes
-  for (int64_t st : {a->q_st, a->k_st, a->v_st, backward ? a->do_st : 0, a->HV * a->V})
+  // offsets within a chunk are 32 bits of bytes; a single token has no next one
+  const bool one = a->T <= 1;
+  for (int64_t st : {one ? 0 : a->q_st, one ? 0 : a->k_st, one ? 0 : a->v_st,
+                     one || !backward ? 0 : a->do_st, a->HV * a->V})
     if (st < 0 || st >= (1 << 24))
       return fail(TOPS_GLA_EUNSUPPORTED, "tokens must lie less than 2^24 elements apart (%lld)",
                   (long long)st);
@@ -105,6 +107,7 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
                 (long long)p->keep_bytes);
   p->a = *a;
   p->a.train = a->train || backward;
+  if (one) p->a.q_st = p->a.k_st = p->a.v_st = p->a.do_st = 0;
   if (!backward) return TOPS_GLA_OK;
   if (a->chunks > 0 && any_null({a->dout, a->dq, a->dk, a->dv, a->dg, a->dbeta}))
     return fail(TOPS_GLA_EINVAL, "dout, dq, dk, dv, dg and dbeta must not be NULL");

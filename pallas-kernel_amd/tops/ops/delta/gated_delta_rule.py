@@ -31,7 +31,7 @@ def _gate(t):
 def _tokens(t, dt):
     """``rows`` of [B, T, heads, columns]; the kernels step from token to token in 32 bits."""
     t = rows(t, dt)
-    return t if 0 <= t.stride(1) < 1 << 24 else t.contiguous()
+    return t if t.shape[1] <= 1 or 0 <= t.stride(1) < 1 << 24 else t.contiguous()
 
 
 _CUS = 256
