@@ -82,11 +82,15 @@ int delta_setup(const tops_gla_delta_args* a, bool backward, tops::DeltaParams* 
         a->nsegs < a->nseq || a->nsegs > a->chunks + a->nseq)
       return fail(TOPS_GLA_EINVAL, "bad nseq, chunks or nsegs");
   }
-  // the blocks of the largest launches, of 256 threads or fewer
-  if (!grid_fits(a->chunks, 1) || !grid_fits(a->chunks * a->HV, 256) ||
+  // the largest launches: the inverses, the gradients (refused before the forward that leads to them),
+  // the passes (in 512 threads, half as many blocks), the fold
+  const bool grads = a->train || backward;
+  if (!grid_fits(a->chunks, 1) ||
+      !grid_fits(a->chunks * a->HV, grads ? tops::delta_grad_threads((int)a->dtype) : 256) ||
       !grid_fits((a->V / 64 + 5) * a->HV, 256) ||
       !grid_fits((a->V / 64 + 5) * a->HV * a->nsegs, 256) ||
-      !grid_fits((a->V / 16 + 1) * a->HV * a->nseq, 64))
+      (a->nsegs > a->nseq && !grid_fits((a->V + 15) / 16 * a->HV * a->nseq,
+                                        tops::delta_fold_threads(tops::delta_key_pad(a->K)))))
     return fail(TOPS_GLA_EUNSUPPORTED, "grid too large");
   // offsets within a chunk are 32 bits of bytes; a single token has no next one
   const bool one = a->T <= 1;

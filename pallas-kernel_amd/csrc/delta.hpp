@@ -110,7 +110,10 @@ constexpr int delta_blocks() {   // lower 32 x 32 blocks of a tile of C x C
   return delta_c<T>() == 64 ? 3 : 1;
 }
 __device__ __forceinline__ constexpr int tri_block(int u, int w) { return u * (u + 1) / 2 + w; }
-inline int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
+constexpr int delta_key_pad(long K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
+// Threads of a block: two waves for 16 tokens of a chunk, a wave for 32 padded keys.
+constexpr int delta_grad_threads(int dtype) { return dtype == DT_BF16 ? 512 : 256; }
+constexpr int delta_fold_threads(int KP) { return 2 * KP; }
 
 // Per chunk and value head ("unit"): vectors over the chunk's tokens, [7][C] float and [C] double,
 //   e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|, e^G, e^{G_C - G}, 1 / |q|

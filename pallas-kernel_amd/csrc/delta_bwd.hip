@@ -30,6 +30,7 @@ template <typename T, int KP>
 struct GradLds {
   // values of a slab: K = 64, V = 128, two value heads a key head, 5000 tokens: forward and backward in
   // 225 us, 232 with 32; K = 128 has no room in LDS for 64
+  static constexpr int NT = delta_grad_threads(sizeof(T) == 2 ? DT_BF16 : DT_F32);
   static constexpr int C = delta_c<T>(), VS = sizeof(T) == 2 && KP == 64 ? 64 : 32;
   static constexpr int PK = pitch_of<T>(KP), PS = pitch_of<T>(VS);
   static constexpr int PC = pitch_of<T>(TWO<T> * C), PD = pitch_of<T>(TWO<T> * KP);   // parts in a row
@@ -78,9 +79,9 @@ __device__ __forceinline__ float row_dot(const T* row, const f32x4 (&acc)[2 * NS
 // CU spill. 20 registers spill with 128 keys and several value heads, 65 with 256 keys, 114 with both;
 // float32: 97 with both.
 template <typename T, int KP, bool GROUP>
-__global__ __launch_bounds__(8 * delta_c<T>()) void delta_grad_kernel(DeltaParams p) {
+__global__ __launch_bounds__((GradLds<T, KP>::NT)) void delta_grad_kernel(DeltaParams p) {
   using L = GradLds<T, KP>;
-  constexpr int C = L::C, NT = 8 * C, NS = KP / 32, NU = C / 32, NW = C / 16;
+  constexpr int C = L::C, NT = L::NT, NS = KP / 32, NU = C / 32, NW = C / 16;
   constexpr int VS = L::VS, NH = VS / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const tops_gla_delta_args& a = p.a;
@@ -409,7 +410,7 @@ hipError_t launch_grad(const DeltaParams& p, hipStream_t st) {
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   delta_grad_kernel<T, KP, GROUP>
-      <<<(unsigned)(p.a.chunks * p.a.H), 8 * delta_c<T>(), lds, st>>>(p);
+      <<<(unsigned)(p.a.chunks * p.a.H), L::NT, lds, st>>>(p);
   return hipGetLastError();
 }
 

@@ -678,7 +678,7 @@ __global__ __launch_bounds__(64 * NW) void delta_dscan_kernel(DeltaParams p) {
 // head: 16 segments of 16 heads of 128 x 128 in 31 us (with maps in two parts 22, in rows, 64 bytes a
 // row and load, 33; two segments ahead so 40).
 template <typename T, int KP, bool BACK>
-__global__ __launch_bounds__(2 * KP) void delta_fold_kernel(DeltaParams p) {
+__global__ __launch_bounds__(delta_fold_threads(KP)) void delta_fold_kernel(DeltaParams p) {
   constexpr int NS = KP / 32, PARTS = WHOLE<T>;
   __shared__ __attribute__((aligned(16))) Frag<T> sh[2][PARTS][NS][64];
   const tops_gla_delta_args& a = p.a;
@@ -775,7 +775,7 @@ hipError_t passes(const DeltaParams& p, hipStream_t st) {
   if (p.multi) {
     if (const hipError_t e = launch<T, KP, NW, BACK, true>(p, st)) return e;
     const unsigned grid = (unsigned)((p.a.V + 15) / 16 * p.a.HV * p.a.nseq);
-    delta_fold_kernel<T, KP, BACK><<<grid, 2 * KP, 0, st>>>(p);
+    delta_fold_kernel<T, KP, BACK><<<grid, delta_fold_threads(KP), 0, st>>>(p);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   return launch<T, KP, NW, BACK, false>(p, st);
