@@ -118,7 +118,9 @@ constexpr int delta_fold_threads(int KP) { return 2 * KP; }
 // Per chunk and value head ("unit"): vectors over the chunk's tokens, [7][C] float and [C] double,
 //   e^G / |k|, e^{G_C - G} / |k|, beta, 1 / |k|, e^G, e^{G_C - G}, 1 / |q|
 // (norms 1 without l2norm) and G, the sums of the log decays (in 64 bits: differences of it go into
-// exponentials); then, in the operands' type, three parts of it where that is bfloat16,
+// exponentials), and the first token whose k, g or beta is not finite (C: none), from which on the
+// chunk counts as empty but for a NaN in e^G and e^{G_C - G}, which makes its outputs, the state after
+// the chunk, and gradients NaN; then, in the operands' type, three parts of it where that is bfloat16,
 //   Tm the inverse of 1 + tril(beta k k^T decay), P the masked and scaled scores, both as the lower
 // of their 32 x 32 blocks (0, 0), (1, 0), (1, 1);
 // and, for the backward, in two such parts side by side in a row, N [V][2][C] the written values and
@@ -169,6 +171,9 @@ __device__ __forceinline__ ChunkAt delta_chunk_at(const tops_gla_delta_args& a, 
 
 __device__ __forceinline__ float* delta_vec(const DeltaParams& p, long unit) {
   return (float*)(p.vec + unit * p.vec_bytes);
+}
+__device__ __forceinline__ int* delta_first(const DeltaParams& p, long unit) {
+  return (int*)(p.vec + unit * p.vec_bytes + 36 * p.C);
 }
 __device__ __forceinline__ double* delta_gsum(const DeltaParams& p, long unit) {
   return (double*)(p.vec + unit * p.vec_bytes + 28 * p.C);
@@ -365,6 +370,14 @@ struct Piece<bf16> {
   __device__ __forceinline__ void get(const void* base, uint32_t off) {
     x = *reinterpret_cast<const Any*>((const char*)base + off);
   }
+  // A sum that goes into the sign where an exponent has all its bits.
+  static constexpr uint32_t SIGNS = 0x80008000u;
+  __device__ __forceinline__ uint32_t full() const {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (x[i] & ~SIGNS) + 0x00800080u;
+    return r;
+  }
   __device__ __forceinline__ Frag<bf16> frag() const {
     Frag<bf16> f;
     f.d = make_uint4(x[0], x[1], x[2], x[3]);
@@ -378,6 +391,15 @@ struct Piece<float> {
   __device__ __forceinline__ void get(const void* base, uint32_t off) {
     x = *reinterpret_cast<const Any*>((const char*)base + off);
     y = *reinterpret_cast<const Any*>((const char*)base + off + 16);
+  }
+  static constexpr uint32_t SIGNS = 0x80000000u;
+  __device__ __forceinline__ uint32_t full() const {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r |= ((__float_as_uint(x[i]) & ~SIGNS) + 0x00800000u) |
+           ((__float_as_uint(y[i]) & ~SIGNS) + 0x00800000u);
+    return r;
   }
   __device__ __forceinline__ Frag<float> frag() const {
     Frag<float> f;
@@ -413,6 +435,14 @@ struct TileFetch {
     for (int i = 0; i < N; ++i)
       r[i].get(src - 8, (uint32_t)min(row_of(i, tid), len - 1) * (uint32_t)st * ES +
                             (uint32_t)(min(col_of(i, tid), cols - 8) + 8) * ES);
+  }
+  // Whether a piece of the thread has a value that is not finite (one past the tile's rows or columns
+  // says what the one that was loaded in its place says).
+  __device__ __forceinline__ bool not_finite() const {
+    uint32_t s = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s |= r[i].full();
+    return s & Piece<T>::SIGNS;
   }
   // The piece as it belongs into the tile.
   __device__ __forceinline__ Frag<T> piece(int i, int len, int cols, int tid) const {

@@ -44,7 +44,8 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
   T* sK = (T*)first;
   float* sT = (float*)first;
   __shared__ double sG[C];
-  __shared__ float sBeta[C], sRk[C];
+  __shared__ float sBeta[C], sRk[C], sKK[C];
+  __shared__ int sFirst;
   const tops_gla_delta_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int H = (int)a.H, HV = (int)a.HV, K = (int)a.K;
@@ -87,6 +88,9 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
     for (int j = 0; j < NB; ++j) {
       kk[j] = zero4();
       if (j <= wave) mma_tile<T>(kk[j], sK + wave * 16 * PK, PK, sK + j * 16 * PK, PK, KP, lane);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)   // the diagonal
+        if (j == wave && (lane & 15) == 4 * (lane >> 4) + r) sKK[16 * j + (lane & 15)] = kk[j][r];
     }
   }
   __syncthreads();
@@ -95,8 +99,15 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
     const int hv = h * group + gi;
     const long unit = (long)chunk * HV + hv;
     if (wave == 0) {
-      const float g = lane < at.len ? log_decay(g_next) : 0.f;
-      const float beta = lane < at.len ? beta_next : 0.f;
+      // From the first token on whose k, g or beta is not finite, the chunk has no tokens here: what
+      // comes before it stays as it is, and what is made of the rest is set to NaN below.
+      const bool bad = lane < at.len && !(fabsf(sKK[lane]) < INFINITY && g_next < INFINITY &&
+                                          fabsf(beta_next) < INFINITY);
+      const uint64_t any = __ballot(bad);
+      const int first = any ? __ffsll((unsigned long long)any) - 1 : C;
+      if (lane == 0) sFirst = first;
+      const float g = lane < min(at.len, first) ? log_decay(g_next) : 0.f;
+      const float beta = lane < min(at.len, first) ? beta_next : 0.f;
       double s = g;
 #pragma unroll
       for (int o = 1; o < C; o <<= 1) {
@@ -113,11 +124,15 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
     for (int b = 0; b < C / 32; ++b)   // what is stored of T above the diagonal blocks
       sT[(32 * b + tid / 16) * PA + 32 * b + 16 + tid % 16] = 0.f;
     __syncthreads();
+    const int first = sFirst;
     if (tid < C) {
       float* vec = delta_vec(p, unit);
       const double G = sG[tid];
-      const float rk = sRk[tid], e = expf((float)G), l = expf((float)(sG[C - 1] - G));
-      vec[tid] = e * rk;
+      const bool in = tid < first;
+      const float rk = in ? sRk[tid] : 0.f, e = in ? expf((float)G) : NAN;
+      const float l = first < C ? NAN : expf((float)(sG[C - 1] - G));   // the state after the chunk
+      if (tid == 0) delta_first(p, unit)[0] = first;
+      vec[tid] = in ? e * rk : 0.f;
       vec[C + tid] = l * rk;
       vec[2 * C + tid] = sBeta[tid];
       vec[3 * C + tid] = rk;
@@ -145,7 +160,7 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaParams p) {
         for (int r = 0; r < 4; ++r) d[r] = pinned(f[r] * rj * expf((float)(gr[r] - gj)));
 #pragma unroll
         for (int r = 0; r < 4; ++r)   // a choice, no product: what is masked may be anything
-          sA[(row0 + r) * PA + col] = row0 + r > col ? kk[j][r] * d[r] : 0.f;
+          sA[(row0 + r) * PA + col] = row0 + r > col && row0 + r < first ? kk[j][r] * d[r] : 0.f;
       }
     }
     __syncthreads();
@@ -205,7 +220,7 @@ DeltaParams delta_layout(const tops_gla_delta_sizes& z, void* keep, void* ws) {
   const long units = z.chunks * z.HV, segs = z.nsegs * z.HV;
   p.C = delta_chunk_of((int)z.dtype);
   p.KP = delta_key_pad(z.K);
-  p.vec_bytes = 36 * p.C;
+  p.vec_bytes = 36 * p.C + 16;
   // bytes of an element in three parts and in two
   const long whole = z.dtype == DT_BF16 ? 2 * WHOLE<bf16> : 4, two = 4;
   p.tri_bytes = (z.dtype == DT_BF16 ? 3 : 1) * 1024 * whole;

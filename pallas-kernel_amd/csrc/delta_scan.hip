@@ -120,8 +120,8 @@ struct ScanLds : ScanShape<T, KP, NW> {
   // the scores' part: q, two parts of P, the sums of log decays, 1 / |q|
   static constexpr int Q0 = 0, P0 = C * B::PK, G0 = (P0 + TWO<T> * B::PART) * ES, R0 = G0 + 8 * C;
   static constexpr int REST = FIRST ? 0 : R0 + 4 * C;
-  static constexpr int BUFS = 2 * ONE + REST <= LDS_MOST ? 2 : 1;   // of the chunk's tiles
-  static constexpr int BYTES = BUFS * ONE + REST;
+  static constexpr int BUFS = 2 * ONE + REST + (2 + B::COLS) * 4 <= LDS_MOST ? 2 : 1;   // of the chunk's tiles
+  static constexpr int BYTES = BUFS * ONE + REST + (2 + B::COLS) * 4;
   static_assert(BYTES <= LDS_MOST && ONE % 16 == 0 && G0 % 8 == 0, "LDS");
 };
 
@@ -177,6 +177,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   constexpr int NF = (5 * C + NT - 1) / NT;
   float ff[NF];
   double fg = 0.;
+  int fin = 0;   // tokens before the first one that is not finite
   // where the next chunk's inputs lie, and this chunk's other parts; all of them go on by their steps
   const long unit0 = (long)at.chunk * HV + hv;
   const int k_st = (int)a.k_st, q_st = (int)a.q_st, v_st = (int)a.v_st;
@@ -204,6 +205,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
     const float* vec = (const float*)vecn;
 #pragma unroll
     for (int i = 0; i < NF; ++i) ff[i] = vec[min(i * NT + tid, 5 * C - 1)];
+    fin = *(const int*)(vecn + 36 * C);
     if (!FIRST) {
       fq.next(qp, q_st, len);
       qp += (long)C * q_st;
@@ -216,11 +218,15 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   T *sQ = (T*)rest + L::Q0, *sP = (T*)rest + L::P0;
   double* sG = (double*)(rest + L::G0);
   float* sRq = (float*)(rest + L::R0);
-  auto put = [&](unsigned char* buf, int len) {
+  // chunks with values that are not finite, by turns, and from which token on each column has them
+  int *sFlag = (int*)(smem + L::BYTES - (2 + COLS) * 4), *sFirst = sFlag + 2;
+  auto put = [&](unsigned char* buf, int len, int n) {
     T* sm = (T*)buf;
-    fk.put(sm + L::K0, L::PK, len, K, tid);
+    const int rows = min(len, __builtin_amdgcn_readfirstlane(fin));
+    fk.put(sm + L::K0, L::PK, rows, K, tid);
     ft.put(sm + L::T0, L::PT, tid);
-    fv.put(sm + L::V0, L::PV, map ? 0 : len, vc, tid);
+    fv.put(sm + L::V0, L::PV, map ? 0 : rows, vc, tid);
+    if (!map && fv.not_finite()) sFlag[n & 1] = n;
     float* sf = (float*)(buf + L::F0);
 #pragma unroll
     for (int i = 0; i < NF; ++i)
@@ -303,11 +309,28 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
   if (nc > 0) {
     fetch(left);
     fetch2(left);
-    put(buf, left);
+    if (tid < 2) sFlag[tid] = -1;
+    __syncthreads();
+    put(buf, left, 0);
   }
   for (int n = 0; n < nc; ++n, left -= C) {
     const bool more = n + 1 < nc;
     __syncthreads();
+    // Products would take a value that is not finite to all tokens of its column, so it and what
+    // follows it there are left out, and what is made of them is set to NaN.
+    const bool spoilt = __builtin_amdgcn_readfirstlane(sFlag[n & 1]) == n;
+    if (__builtin_expect(spoilt && !idle, 0)) {
+      T* at0 = (T*)buf + L::V0 + w0 + ci;
+      int first = C;
+#pragma unroll 1
+      for (int t = C - 4 + g; t >= 0; t -= 4)
+        if (!(fabsf(to_f32(at0[t * L::PV])) < INFINITY)) first = t;
+      first = min(first, __shfl_xor(first, 16));
+      first = min(first, __shfl_xor(first, 32));
+#pragma unroll 1
+      for (int t = first; t < C; ++t) at0[t * L::PV] = zero_elem<T>();
+      sFirst[w0 + ci] = first;
+    }
     // The two halves of the block's waves, one of each on a SIMD, go through a chunk in different
     // orders, so that loads, products and conversions of one lie beside others of the other.
     const bool early = wave < NW / 2;
@@ -393,6 +416,18 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           return ld_pair_t(sK + 32 * u * L::PK + 32 * (i >> 1), L::PK, lane, i & 1);
         }, split_of<T, WHOLE<T>>(x));
       }
+      if (__builtin_expect(spoilt, 0)) {
+        const int first = sFirst[w0 + ci];
+        if (!FIRST && keep && vin)
+#pragma unroll 1
+          for (int i = 0; i < 8 * NU; ++i) {   // the tokens that the lane has stored
+            const int t = 32 * (i >> 3) + 8 * g + (i & 7);
+            if (t >= first) at_off<T>(Nc, n_off)[t - 8 * g] = from_f32<T>(NAN);
+          }
+        const float x = first < C ? NAN : 1.f;
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) S[i] *= x;
+      }
     }
     if constexpr (!FIRST) {
       __syncthreads();   // the scores are there, and no values are read any more
@@ -418,6 +453,12 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             so[(32 * u + 8 * g + x) * L::PV] = from_f32<T>(o[2 * u + x / 4][x % 4]);
+        if (__builtin_expect(spoilt, 0))
+#pragma unroll 1
+          for (int i = 0; i < 8 * NU; ++i) {
+            const int t = 32 * (i >> 3) + 8 * g + (i & 7);
+            if (t >= sFirst[w0 + ci]) so[t * L::PV] = from_f32<T>(NAN);
+          }
       }
     }
     if (more) {
@@ -431,7 +472,7 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p) {
           __syncthreads();
         }
       }
-      put(other, left - C);
+      put(other, left - C, n + 1);
       unsigned char* x = buf;
       buf = other;
       other = x;

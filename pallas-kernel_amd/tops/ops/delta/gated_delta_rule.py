@@ -203,8 +203,12 @@ def gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_fi
     of is multiplied in two parts of 16 bits: they are rounded once, to their type. Other types of
     q, k and v are computed in float32. g and beta are read in float32 or bfloat16, whatever the
     others' type, and their gradients returned in it: float32 ones beside bfloat16 q, k and v are
-    about 1e-5 off. Inputs that are not finite make the outputs of their chunk of 64 tokens (float32: 32)
-    and of all later ones of the sequence and head not finite, also those before them in the chunk.
+    about 1e-5 off.
+
+    An input that is not finite makes the outputs of its token and of all later ones of the sequence
+    not finite, for the value heads that it belongs to; one of v does so in its column, and one of q
+    at its own token alone. Gradients may then be not finite for all tokens of the sequence, in the
+    heads that share the key head. Nothing else changes, to the bit.
     A second derivative raises.
 
     Returns ``(o, final_state)``: o ``[B, T, HV, V]`` in v's type, final_state ``[sequences, HV, K,
