@@ -50,6 +50,12 @@ def refuse_grad(name, *tensors):
     if torch.is_grad_enabled() and differentiable(*tensors):
         raise RuntimeError(f"{name} updates its state in place and has no gradient: call it under "
                            "torch.no_grad()")
+    # no_grad leaves forward-mode differentiation on
+    fwd = torch.autograd.forward_ad
+    if fwd._current_level >= 0:
+        for t in tensors:
+            if t is not None and fwd.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} updates its state in place and takes no tangents")
 
 
 def offsets(cu_seqlens, B, T):
