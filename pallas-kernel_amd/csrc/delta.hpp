@@ -27,15 +27,6 @@ template <typename T, int N>
 __device__ __forceinline__ Run<T, N> get_run(const T* p) {
   return *reinterpret_cast<const Run<T, N>*>(p);
 }
-// The first n of them, zeros behind.
-template <typename T, int N>
-__device__ __forceinline__ Run<T, N> get_run(const T* p, int n) {
-  if (n >= N) return get_run<T, N>(p);
-  Run<T, N> r;
-#pragma unroll
-  for (int e = 0; e < N; ++e) r.v[e] = e < n ? p[e] : zero_elem<T>();
-  return r;
-}
 template <typename T, int N>
 __device__ __forceinline__ void put_run(T* p, const float (&x)[N], int n = N) {
   if (n >= N) {
