@@ -65,7 +65,8 @@ int tops_gla_delta_fwd(const tops_gla_delta_args *a, void *stream);
 int tops_gla_delta_bwd(const tops_gla_delta_args *a, void *stream);
 /* Tokens of a chunk (0 for a type that is refused). */
 int64_t tops_gla_delta_chunk(int64_t dtype);
-/* Chunks of a segment for nseq sequences of like lengths, `chunks` chunks in all. */
+/* Chunks of a segment for nseq sequences of like lengths, `chunks` chunks in all; with K > 128, whose
+ * blocks have half the columns, V stands for twice the values. */
 int64_t tops_gla_delta_segment(int64_t nseq, int64_t chunks, int64_t HV, int64_t V);
 /* Bytes of `keep`, or with `backward` of `ws` (0 for sizes that are refused). */
 typedef struct tops_gla_delta_sizes {

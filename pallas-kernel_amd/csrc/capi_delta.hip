@@ -155,16 +155,16 @@ int64_t tops_gla_delta_segment(int64_t nseq, int64_t chunks, int64_t HV, int64_t
   const int64_t whole = 1 << 20;
   if (nseq < 1 || chunks < 1 || HV < 1 || V < 1) return whole;
   // a block for each CU in the second pass: 8 sequences of 16 heads and 32 chunks in two segments
-  // take 208 us forward (uncut 229, three segments 272), 5 of 64 chunks in three 348 (uncut 412, two
-  // 354, four 376), one of 8 chunks in four 43 (uncut 57), one of 256 in 16 288 (uncut 1461). Below 6
-  // chunks the first pass costs what the second saves (4 chunks in two 39, uncut 35)
+  // take 258 us forward (uncut 273, three segments 334), 5 of 64 chunks in three 432 (uncut 495, two
+  // 433, four 460), one of 8 chunks in four 52 (uncut 70), one of 256 in 16 358 (uncut 1801). Below 6
+  // chunks the first pass costs what the second saves (4 chunks in two 46, uncut 42)
   const int64_t blocks = (V + 127) / 128 * HV * nseq, per = (chunks + nseq - 1) / nseq;
   const int64_t segs = 256 / std::max<int64_t>(1, blocks);
   if (segs < 2 || per < 6) return whole;
   int64_t L = std::max<int64_t>((per + segs - 1) / segs, 2);
   // the fold goes from segment to segment, each about a quarter of two passes' chunk: least in sum
-  // at L = sqrt(per / 4) (per = 256, one head: L = 4 139 us, 8 135, 16 184; 1024, two heads: 8 304,
-  // 16 261, 32 362)
+  // at L = sqrt(per / 4) (per = 256, one head: L = 4 187 us, 8 171, 16 232; 1024, two heads: 8 400,
+  // 16 334, 32 451)
   while (L * L * 4 < per && L < whole) ++L;
   return std::min(L, whole);
 }

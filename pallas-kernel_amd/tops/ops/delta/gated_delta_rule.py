@@ -42,37 +42,46 @@ def _segment(counts, blocks):
     heads and columns of each; tops_gla_delta_segment has the rule for equal lengths.
 
     All segments should run at once, or the last ones wait for a whole one (lengths of 28, 5, 33,
-    2, 47, 1, 8 and 9 chunks, 16 heads: L = 10 has 272 blocks and takes 186 us, 11 has 256 and 151,
-    12 157, 17 195, uncut 296). Where the sequences alone are more than the CUs hold, their ends
-    differ anyway, and what is long among them is cut by the average (40 of 4 chunks and one of
-    200: 373 us, uncut 1233; 64 of 6 and one of 60: 523, uncut 583)."""
+    2, 47, 1, 8 and 9 chunks, 16 heads of 128 x 128: L = 10 has 272 blocks and takes 219 us, 11 has
+    256 and 182, 12 190, 17 239, uncut 357). Where the sequences alone are more than half of what
+    the CUs hold, their ends differ anyway, and what is long among them is cut by the average (32
+    such heads: L = 17 293 us, uncut 381; 40 of 4 chunks and one of 200: 441, uncut 1505; 64 of 6
+    and one of 60: 463, uncut 523)."""
     longest = max(counts)
     L = max(-(-sum(counts) * blocks // _CUS), 2, math.isqrt(max(0, longest - 1) // 4) + 1)
-    if len(counts) * blocks <= _CUS:
+    if 2 * len(counts) * blocks <= _CUS:
         while L < longest and sum(-(-n // L) for n in counts) * blocks > _CUS:
             L += max(1, L // 32)
     return L if longest >= 6 and longest >= 2 * L else max(1, longest)
 
 
+def _columns(K):
+    """Columns of a block of the passes: with more than 128 keys 64. (8 heads of
+    256 x 256, 128 chunks: 391 us in segments of 16, 469 in those of 8 that 128 columns would give;
+    the packed sequences above 310 for 386.)"""
+    return 128 if K <= 128 else 64
+
+
 class _Chunks:
     """The chunks that a call's sequences are cut into, and the segments that these run in."""
 
-    def __init__(self, B, T, cu, dt, HV, V, device):
+    def __init__(self, B, T, cu, dt, HV, K, V, device):
         lib = _lib.load()
         C = lib.tops_gla_delta_chunk(dtype_code(dt))
         self.table = None
         if cu is None:
             per = -(-T // C)
             self.nseq, self.n = B, B * per
-            self.L = lib.tops_gla_delta_segment(B, self.n, HV, V)
+            self.L = lib.tops_gla_delta_segment(B, self.n, HV, V * 128 // _columns(K))
             self.nsegs = B * max(1, -(-per // self.L))
             return
         self.nseq = len(cu) - 1
         counts = [-((a - b) // C) for a, b in zip(cu, cu[1:])]
         self.n = sum(counts)
+        blocks = HV * -(-V // _columns(K))
 
         def make():
-            L = _segment(counts, HV * -(-V // 128))
+            L = _segment(counts, blocks)
             chunks, segs, seq = [0], [0], []
             for s, n in enumerate(counts):
                 k = max(1, -(-n // L))
@@ -81,7 +90,7 @@ class _Chunks:
                 seq += [s] * k
             return [*cu, *chunks, *segs, *seq], (len(seq), L)
 
-        key = "delta", tuple(cu), C, HV * -(-V // 128)
+        key = "delta", tuple(cu), C, blocks
         self.table, (self.nsegs, self.L) = device_table(key, make, device)
 
     def bytes(self, HV, K, V, dt, train, backward):
@@ -108,7 +117,7 @@ def _forward(q, k, v, g, beta, h0, scale, norm, want, cu, train):
     HV, V = v.shape[2:]
     x = _tokens(q, dt), _tokens(k, dt), _tokens(v, dt), _gate(g), _gate(beta)
     h0 = f32(h0)
-    ch = _Chunks(B, T, cu, dt, HV, V, dev)
+    ch = _Chunks(B, T, cu, dt, HV, K, V, dev)
     o = torch.empty(B, T, HV, V, dtype=dt, device=dev)
     ht = torch.empty(ch.nseq, HV, K, V, dtype=torch.float32, device=dev) if want else None
     nkeep = ch.bytes(HV, K, V, dt, train, False)

@@ -29,7 +29,8 @@ PARTS = {"o": 3, "q": 3, "k": 6, "v": 1, "beta": 4, "g": 13}
 NAMES = ("q", "k", "v", "g", "beta", "initial_state")
 
 CASES = [(1, 40, 1, 1, 64, 64, None), (2, 200, 1, 2, 128, 128, None), (1, 130, 2, 2, 200, 40, None),
-         (1, 1100, 1, 2, 64, 96, None), (1, 900, 1, 2, 128, 64, [0, 30, 700, 700, 900])]
+         (1, 1100, 1, 2, 64, 96, None), (1, 900, 1, 2, 128, 64, [0, 30, 700, 700, 900]),
+         (1, 1100, 1, 1, 256, 40, None), (1, 1000, 1, 2, 200, 130, [0, 620, 1000])]
 
 
 def make(B, T, H, HV, K, V, cu, gdt):
