@@ -13,15 +13,15 @@
 // E_j <- M_j E_{j-1} + E_j the state after each, and a second pass runs all segments from there.
 // The gradients run with the same maps transposed.
 //
-// A chunk's step of the second pass has, for 128 keys and a wave's 16 values, 116 matrix
-// instructions of 16 cycles (the state's products in two parts, the system, scores and outputs) and
-// 740 others, most of them making operands: for the two waves of a SIMD 9600 cycles, of the 14400 that
-// a step takes; the rest are waits for LDS and barriers (44 % of a wave's time). Eight waves a block
-// share the tiles (against four with twice the columns 7 to 15 % faster), and its halves go through
-// the step in different orders, so that one's matrix instructions meet the other's others (second
-// pass 127 -> 118 us). 16384 tokens of 16 heads of 128 x 128: first pass 141 us (29 blocks a head for
-// 16 segments), second, with the outputs, 117, 2.9 TB/s; training of 2 x 4096 tokens: 80 and 79,
-// and the gradients' 54 and 65.
+// A chunk's step of the second pass has, for 128 keys and a wave's 16 values, 188 matrix instructions
+// of 16 cycles (states, the system and written values in three parts, what goes into outputs in two), 850
+// others, most of them making operands, and 177 LDS accesses. For the two waves of a SIMD these are 6000
+// and 6800 cycles, for a CU's LDS 9700, half of them bank conflicts, of the 17500 that a step takes: none of
+// the three is full, a wave waits 37 % of its time. Eight waves a block share the tiles, and its halves go
+// through the step in different orders, so that one's matrix instructions meet the other's others. 16384
+// tokens of 16 heads of 128 x 128: first pass 191 us (29 blocks a head for 16 segments, 464 in two rounds of
+// the CUs), second, with the outputs, 151; training of 2 x 4096 tokens: 106 and 110, and the gradients' 70
+// and 94. (With every operand in one part less, states 3.5e-6 off and outputs 2.3e-3: 141 and 117.)
 #include "delta.hpp"
 
 namespace tops {

@@ -11,8 +11,10 @@
 // Measured: 128 rows of 16 heads of 128 x 128, 268 MB, in 54.2 us, 4.95 TB/s, as a large copy has. A
 // wave is a block of its own (four a block: 58.8 us), neighbouring columns on one XCD (each on the
 // next: 56.3 us, and 64 so 50 us with 100 columns, where lines are shared). A token's inputs asked for
-// with the state or the token before were no faster (60.5 us: 252 registers for 131). One row of 16
-// heads takes 9 us, the time of its few memory accesses one after another.
+// with the state or the token before were no faster there, with one token a row (60.5 us: 252 registers
+// for 131); of several tokens of few rows, where registers are free, that has not been measured (16 rows
+// of 4 tokens: 16 us, 7 of bytes). One row of 16 heads takes 8 us, the time of its few memory accesses one
+// after another.
 #include "delta.hpp"
 
 namespace tops {
